@@ -89,7 +89,7 @@ def _quantize(x, group):
     """bf16 values ``[..., n]`` -> codes ``[..., n]`` (fp32 whole numbers) and scale, offset ``[..., n / group]`` bf16."""
     x = x.float().unflatten(-1, (-1, group))
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
-    s = ((hi - lo) / 15 * 16).bfloat16().float()
+    s = ((hi - lo) / torch.full_like(lo, 15) * 16).bfloat16().float()         # (by a number, it is a product with 1 / 15 on a GPU)
     s = torch.where(s < LEAST, torch.zeros_like(s), s)
     o = (lo - s).bfloat16().float()
     c = torch.where(s > 0, ((x - o) / s * 16).round() - 16, torch.zeros_like(x)).clamp(0, 15)
