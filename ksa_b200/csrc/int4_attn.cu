@@ -1,0 +1,494 @@
+// Decode attention over a KV cache of four bits: out = softmax(q K^T * scale) V over a slice [start, start + length) of the cache for every
+// (sequence, query token), the G = Hq / Hkv heads of a KV head together.
+//
+// What bounds it is reading the slice once, 160 bytes a slot and KV head at head dim 128 (bf16: 512).  Hence:
+//   * all (slice, KV head) items in a row are one sequence of tiles of 32 slots, and every CTA takes an equal run of it, whatever the
+//     slices' lengths are (they are known on the device only).  A run that covers part of an item leaves (max, sum, output) behind, and a
+//     second kernel merges the parts of an item in a fixed order; an item within one run is finished there;
+//   * each warp keeps tiles in flight through a ring of its own, filled by bulk copies (a tile is contiguous: 2 KB of codes and 512 bytes of
+//     scales for K and for V), so no warp waits for another before the end of an item's run;
+//   * both products are mma.sync m16n8k16 with the values straight from their codes (int4.cuh) as an operand.  A lane's four words of a key
+//     are values 32 t .. 32 t + 31 of it, one group with one scale; the order of the head dimension in the product is q's as well, so nothing is
+//     moved.  The probabilities leave the first product in the layout of the second one's right operand (out^T = V^T P^T);
+//     V^T wants the same value of two neighbouring keys in a register, which is a byte permutation of two words before the shift.
+// Nothing outside a slice enters a result: slots of the slice's first and last tile that lie outside get probability 0 and scale and offset 0, so
+// that a NaN there stays there.
+#include "host.h"
+#include "int4.cuh"
+
+namespace ksa {
+
+constexpr int kI4Warps = 4;
+constexpr int kI4Tile = 32;        // slots of a tile
+constexpr int kI4Stages = 3;       // tiles in flight of a warp
+constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
+
+struct Int4Attn {
+  const bf16* q;                   // [B, Tq, Hq, D], strides below, heads' rows contiguous
+  long long q_sb, q_st, q_sh;
+  const uint8_t *k, *v;            // [B, Hkv, cap, D / 2]
+  const uint32_t *k_meta, *v_meta; // [B, Hkv, cap, D / 32]
+  const int *start, *len;          // [B, Tq]
+  float* part_o;                   // [CTAs + items, heads, D]
+  float2* part_ml;                 // [CTAs + items, heads]: max (log2 units), sum
+  bf16* out;                       // [B, Tq, Hq, D]
+  int rows, Tq, Hq, Hkv, cap;      // rows = B * Tq
+  int heads, blocks;               // query heads of an item; items of a KV head
+  int ctas;
+  float scale;                     // * log2(e)
+};
+
+__device__ __forceinline__ void i4_slice(const Int4Attn& a, int row, int& lo, int& hi) {
+  const long long s = a.start[row], e = s + max(a.len[row], 0);
+  lo = (int)max(s, 0LL);
+  hi = (int)min(e, (long long)a.cap);          // whatever the device holds as slices: never past the cache
+}
+__device__ __forceinline__ int i4_tiles(int lo, int hi) {
+  return hi > lo ? (hi - (lo & ~(kI4Align - 1)) + kI4Tile - 1) / kI4Tile : 0;
+}
+// Tiles of one item of each row in [from, to), summed by a warp.
+__device__ __forceinline__ long long i4_sum_tiles(const Int4Attn& a, int from, int to, int lane) {
+  long long n = 0;
+  for (int r = from + lane; r < to; r += 32) {
+    int lo, hi;
+    i4_slice(a, r, lo, hi);
+    n += i4_tiles(lo, hi);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+  return n;
+}
+// CTAs that take part: a tile for each of their warps, at least.
+__device__ __forceinline__ int i4_active(const Int4Attn& a, long long total) {
+  return (int)max(1LL, min((long long)a.ctas, (total + kI4Warps - 1) / kI4Warps));
+}
+
+// A place in the sequence of tiles.
+struct Int4Cursor {
+  long long at;                    // index in the sequence
+  int row, head, tile;             // row, item of the row (KV head and block of its query heads), tile of the item
+  int lo, hi, n;                   // the row's slice and tiles
+  __device__ __forceinline__ void load(const Int4Attn& a) {
+    i4_slice(a, row, lo, hi);
+    n = i4_tiles(lo, hi);
+  }
+  // to the first row that holds tile `to`, counted from the first tile of row 0
+  __device__ __forceinline__ void seek(const Int4Attn& a, long long to, int lane) {
+    const int per_row = a.Hkv * a.blocks;
+    long long left = to;
+    row = 0;
+    while (row + 32 < a.rows) {                                  // whole steps of 32 rows
+      const long long step = i4_sum_tiles(a, row, row + 32, lane) * per_row;
+      if (left < step) break;
+      left -= step;
+      row += 32;
+    }
+    for (; row < a.rows; ++row) {
+      load(a);
+      const long long here = (long long)n * per_row;
+      if (left < here) break;
+      left -= here;
+    }
+    at = to;
+    if (row >= a.rows) return;
+    head = (int)(left / n);
+    tile = (int)(left % n);
+  }
+  __device__ __forceinline__ void advance(const Int4Attn& a, int by) {
+    at += by;
+    if (row >= a.rows) return;
+    tile += by;
+    while (tile >= n) {
+      tile -= n;
+      if (++head == a.Hkv * a.blocks) {
+        head = 0;
+        do {
+          if (++row >= a.rows) return;
+          load(a);
+        } while (n == 0);
+      }
+    }
+  }
+};
+
+template <int D>
+struct Int4Stage {
+  uint32_t k[kI4Tile * D / 8];
+  uint32_t v[kI4Tile * D / 8];
+  uint32_t k_meta[kI4Tile * D / 32];
+  uint32_t v_meta[kI4Tile * D / 32];
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
+// Slots [first, first + 32) of the cursor's KV head, cut to the cache.  One lane.
+template <int D>
+__device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, Int4Stage<D>& s, uint64_t* bar) {
+  const int first = (c.lo & ~(kI4Align - 1)) + c.tile * kI4Tile, n = min(kI4Tile, a.cap - first);
+  const long long at = ((long long)(c.row / a.Tq) * a.Hkv + c.head / a.blocks) * a.cap + first;
+  mbar_expect_tx(bar, n * (D + D / 4));
+  bulk_load(s.k, a.k + at * (D / 2), n * (D / 2), bar);
+  bulk_load(s.k_meta, a.k_meta + at * (D / 32), n * (D / 8), bar);
+  bulk_load(s.v, a.v + at * (D / 2), n * (D / 2), bar);
+  bulk_load(s.v_meta, a.v_meta + at * (D / 32), n * (D / 8), bar);
+}
+
+// NT: query heads of an item in eights (1 or 2).
+template <int D, int NT>
+__global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kernel(const Int4Attn a, int* status) {
+  constexpr int WK = D / 32;       // words of a key that a lane multiplies with the queries
+  constexpr int WV = D / 64;       // words of a value row of which a lane holds the dimensions
+  extern __shared__ __align__(128) uint8_t raw[];
+  Int4Stage<D>* ring = reinterpret_cast<Int4Stage<D>*>(raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kI4Warps * kI4Stages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + kI4Warps * kI4Stages);
+  float* s_m = reinterpret_cast<float*>(full + kI4Warps * kI4Stages + 2);      // [warps][heads]
+  float* s_l = s_m + kI4Warps * a.heads;
+  float* s_o = s_l + kI4Warps * a.heads;                                       // [warps][heads][D]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const WaitGuard guard{abort_flag, status};
+  grid_dependency_launch();
+  if (lane == 0) {
+    for (int i = 0; i < kI4Stages; ++i) mbar_init(&full[warp * kI4Stages + i], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  grid_dependency_wait();
+
+  const int per_row = a.Hkv * a.blocks;
+  const long long total = i4_sum_tiles(a, 0, a.rows, lane) * per_row;
+  const int active = i4_active(a, total), cta = blockIdx.x;
+  if (cta >= active) return;
+  const long long t0 = total * cta / active, t1 = total * (cta + 1) / active;
+  if (t0 >= t1) return;
+
+  Int4Cursor piece;                // the item that the CTA is at, by its first tile of this run
+  piece.seek(a, t0, lane);
+  Int4Cursor next = piece;         // what this warp asks for next
+  next.advance(a, warp);
+  uint64_t* bars = full + warp * kI4Stages;
+  Int4Stage<D>* stages = ring + warp * kI4Stages;
+  int filling = 0, stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  auto fetch = [&]() {
+    if (next.at < t1) {
+      if (lane == 0) i4_fetch<D>(a, next, stages[filling], &bars[filling]);
+      next.advance(a, kI4Warps);
+      if (++filling == kI4Stages) filling = 0;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kI4Stages; ++i) fetch();
+
+  long long mine = t0 + warp;      // index of the next tile of this warp
+  while (piece.at < t1) {
+    const long long item0 = piece.at - piece.tile;               // the item's first tile
+    const long long end = min(t1, item0 + piece.n);
+    const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
+    const int heads = min(a.heads, (kvh + 1) * (a.Hq / a.Hkv) - h0);
+    const int b = piece.row / a.Tq, tq = piece.row % a.Tq;
+    // queries: rows g and g + 8, in the order in which a lane holds a key's values
+    uint4 qa[WK], qb[WK];
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      qa[w] = qb[w] = make_uint4(0, 0, 0, 0);
+      const bf16* src = a.q + b * a.q_sb + tq * a.q_st + (h0 + g) * a.q_sh + t * (D / 4) + w * 8;
+      if (g < heads) qa[w] = *reinterpret_cast<const uint4*>(src);
+      if (NT == 2 && g + 8 < heads) qb[w] = *reinterpret_cast<const uint4*>(src + 8 * a.q_sh);
+    }
+    float o[WV * 4][NT][4], m[NT], l[NT];
+#pragma unroll
+    for (int i = 0; i < WV * 4; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) { m[n] = -INFINITY; l[n] = 0.f; }
+
+    for (; mine < end; mine += kI4Warps) {
+      const int first = (piece.lo & ~(kI4Align - 1)) + (int)(mine - item0) * kI4Tile;
+      ok = ok && mbar_wait(&bars[stage], phase, guard, kTimeoutTmaFull);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const Int4Stage<D>& s = stages[stage];
+      const bool whole = first >= piece.lo && first + kI4Tile <= piece.hi;
+      // ---- scores: this lane's slots are 16 u + 8 j + 4 e + t of the tile
+      float p[NT][2][2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = u * 16 + j * 8 + (g & 1) * 4 + (g >> 1);
+          const uint32_t meta = s.k_meta[key * (D / 32) + t * WK / 4];
+          const uint32_t s2 = i4_scale2(meta), o2 = i4_offset2(meta);
+          uint32_t words[WK];
+          if (D == 128) *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(&s.k[key * (D / 8) + t * WK]);
+          else *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(&s.k[key * (D / 8) + t * WK]);
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < WK; ++w) {
+            uint32_t x[4];
+            i4_values(x, words[w], s2, o2);
+            mma_bf16(c, qa[w].x, qb[w].x, qa[w].y, qb[w].y, x[0], x[1]);
+            mma_bf16(c, qa[w].z, qb[w].z, qa[w].w, qb[w].w, x[2], x[3]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) p[n][u][j][e] = c[n * 2 + e] * a.scale;
+        }
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = first + u * 16 + j * 8 + e * 4 + t;
+              const bool in = key >= piece.lo && key < piece.hi;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) p[n][u][j][e] = in ? p[n][u][j][e] : -INFINITY;
+            }
+      }
+      // ---- running maximum and sum of each query (rows g and g + 8, shared by the four lanes of a row)
+      float corr[NT];
+      bool moved = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float mx = m[n];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[n][i >> 2][(i >> 1) & 1][i & 1]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        corr[n] = mx == m[n] ? 1.f : fast_exp2(m[n] - mx);
+        moved |= mx != m[n];
+        m[n] = mx;
+        l[n] *= corr[n];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float& x = p[n][i >> 2][(i >> 1) & 1][i & 1];
+          x = fast_exp2(x - mx);
+          l[n] += x;
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float c0 = __shfl_sync(0xffffffffu, corr[n], t * 8), c1 = __shfl_sync(0xffffffffu, corr[n], t * 8 + 4);
+#pragma unroll
+          for (int i = 0; i < WV * 4; ++i) {
+            o[i][n][0] *= c0; o[i][n][1] *= c1; o[i][n][2] *= c0; o[i][n][3] *= c1;
+          }
+        }
+      }
+      // ---- out^T += V^T P^T: this lane's dimensions are D / 8 * g and on
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) pb[n][j] = pack_bf16x2(p[n][u][j][0], p[n][u][j][1]);
+        uint32_t words[4][WV], meta[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = u * 16 + i * 4 + t;
+          if (D == 128) *reinterpret_cast<uint2*>(words[i]) = *reinterpret_cast<const uint2*>(&s.v[key * (D / 8) + g * WV]);
+          else words[i][0] = s.v[key * (D / 8) + g];
+          meta[i] = s.v_meta[key * (D / 32) + g * WV / 4];
+          if (!whole && (first + key < piece.lo || first + key >= piece.hi)) meta[i] = 0;
+        }
+        uint32_t s2[2], o2[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x5410);
+          o2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x7632);
+        }
+#pragma unroll
+        for (int w = 0; w < WV; ++w) {
+          uint32_t even[2][4], odd[2][4];      // [pair of keys][value of the word / 2]
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            i4_values(even[j], __byte_perm(words[2 * j][w], words[2 * j + 1][w], 0x5410), s2[j], o2[j]);
+            i4_values(odd[j], __byte_perm(words[2 * j][w], words[2 * j + 1][w], 0x7632), s2[j], o2[j]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], pb[n][0], pb[n][1]);
+        }
+      }
+      __syncwarp();
+      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
+      fetch();
+    }
+
+    // ---- the warps' parts of the item -> one
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+      const int q = n * 8 + g;
+      if (t == 0 && q < heads) { s_m[warp * a.heads + q] = m[n]; s_l[warp * a.heads + q] = l[n]; }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int qe = n * 8 + t * 2 + e;
+        if (qe < heads) {
+          float* dst = s_o + (warp * a.heads + qe) * D + g * (D / 8);
+#pragma unroll
+          for (int i = 0; i < WV * 4; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][n][e], o[i][n][2 + e]);
+        }
+      }
+    }
+    __syncthreads();
+    const bool alone = piece.tile == 0 && end == item0 + piece.n;          // the whole item is here
+    const long long part = cta + (long long)piece.row * per_row + piece.head;
+    for (int i = threadIdx.x; i < heads * D; i += kI4Warps * 32) {
+      const int q = i / D, d = i % D;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kI4Warps; ++w) mx = fmaxf(mx, s_m[w * a.heads + q]);
+      float sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < kI4Warps; ++w) {
+        const float mw = s_m[w * a.heads + q], f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
+        sum = fmaf(s_l[w * a.heads + q], f, sum);
+        acc = fmaf(s_o[(w * a.heads + q) * D + d], f, acc);
+      }
+      if (alone) {
+        a.out[((long long)piece.row * a.Hq + h0 + q) * D + d] = __float2bfloat16(__fdividef(acc, sum));
+      } else {
+        a.part_o[(part * a.heads + q) * D + d] = acc;
+        if (d == 0) a.part_ml[part * a.heads + q] = make_float2(mx, sum);
+      }
+    }
+    __syncthreads();
+    piece.advance(a, (int)(end - piece.at));
+  }
+  // after a wait that gave up: this warp's copies that are still in flight land before the block leaves
+  if (!ok && lane == 0) {
+    const long long began = clock64();
+    for (int i = 0; i < kI4Stages && mine < next.at; ++i, mine += kI4Warps) {
+      while (!mbar_try_wait(&bars[stage], phase) && clock64() - began < kWaitLimitCycles) {}
+      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
+    }
+  }
+}
+
+// Items that several CTAs shared, and empty ones.
+template <int D>
+__global__ void __launch_bounds__(128) int4_attn_merge_kernel(const Int4Attn a) {
+  grid_dependency_launch();
+  grid_dependency_wait();
+  const int per_row = a.Hkv * a.blocks, lane = threadIdx.x & 31;
+  const long long item = blockIdx.x;
+  const int row = (int)(item / per_row), head = (int)(item % per_row);
+  int lo, hi;
+  i4_slice(a, row, lo, hi);
+  const int n = i4_tiles(lo, hi), group = a.Hq / a.Hkv;
+  const int kvh = head / a.blocks, h0 = kvh * group + head % a.blocks * a.heads, heads = min(a.heads, (kvh + 1) * group - h0);
+  bf16* out = a.out + ((long long)row * a.Hq + h0) * D;
+  if (n == 0) {
+    for (int i = threadIdx.x; i < heads * D; i += 128) out[i] = __float2bfloat16(0.f);
+    return;
+  }
+  const long long before = i4_sum_tiles(a, 0, row, lane), total = (before + i4_sum_tiles(a, row, a.rows, lane)) * per_row;
+  const long long first = before * per_row + (long long)head * n, last = first + n - 1;
+  const int active = i4_active(a, total);
+  const long long c0 = ((first + 1) * active - 1) / total, c1 = ((last + 1) * active - 1) / total;
+  if (c0 == c1) return;
+  const long long part0 = c0 + item;
+  const int parts = (int)(c1 - c0 + 1);
+  for (int i = threadIdx.x; i < heads * D; i += 128) {
+    const int q = i / D, d = i % D;
+    float mx = -INFINITY;
+    for (int s = 0; s < parts; ++s) mx = fmaxf(mx, a.part_ml[(part0 + s) * a.heads + q].x);
+    float sum = 0.f, acc = 0.f;
+    for (int s = 0; s < parts; ++s) {
+      const float2 ml = a.part_ml[(part0 + s) * a.heads + q];
+      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
+      sum = fmaf(ml.y, f, sum);
+      acc = fmaf(a.part_o[((part0 + s) * a.heads + q) * D + d], f, acc);
+    }
+    out[i] = __float2bfloat16(__fdividef(acc, sum));
+  }
+}
+
+template <int D>
+static size_t i4_smem(int heads) {
+  return sizeof(Int4Stage<D>) * kI4Warps * kI4Stages + (kI4Warps * kI4Stages + 2) * 8 + sizeof(float) * kI4Warps * heads * (D + 2);
+}
+
+struct Int4Shape {
+  int heads, blocks;
+  long long items;
+  int ctas;
+};
+constexpr int kI4SmShared = 227 * 1024;
+static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
+  Int4Shape s;
+  const int group = Hq / Hkv;
+  s.heads = group < 16 ? group : 16;
+  s.blocks = (group + 15) / 16;
+  s.items = (long long)rows * Hkv * s.blocks;
+  const long long most = (s.items * ((cap + kI4Align + kI4Tile - 1) / kI4Tile) + kI4Warps - 1) / kI4Warps;
+  const int fit = kI4SmShared / ((int)(D == 128 ? i4_smem<128>(s.heads) : i4_smem<64>(s.heads)) + 1024), regs = s.heads <= 8 ? 3 : 2;
+  const long long room = (long long)sm_count() * (fit < regs ? fit : regs);          // all of them at once
+  s.ctas = (int)(most < 1 ? 1 : most < room ? most : room);
+  return s;
+}
+
+template <int D, int NT>
+static int launch_int4_attn(const Int4Attn& a, long long items, cudaStream_t st) {
+  static PerDevice raised;
+  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT>, i4_smem<D>(NT * 8)));
+  int* status = status_word();
+  KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Warps * 32), i4_smem<D>(a.heads), st, a, status));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3((unsigned)items), dim3(128), 0, st, a));
+  return 0;
+}
+
+}  // namespace ksa
+
+using namespace ksa;
+
+// Floats of the workspace of ksa_int4_decode_attn on the current device.
+KSA_API long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap) {
+  if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv != 0 || cap <= 0) return 0;
+  const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
+  return (s.ctas + s.items) * s.heads * (D + 2LL);
+}
+
+// q [B, Tq, Hq, D] with strides in elements (rows of a head contiguous); cache as written by ksa_int4_cache_write; start, len [B, Tq] int32;
+// out [B, Tq, Hq, D].  A slice without slots gives zeros.
+KSA_API int ksa_int4_decode_attn(const void* q, const void* k, const void* k_meta, const void* v, const void* v_meta, const void* start,
+                                 const void* len, void* workspace, void* out, int B, int Tq, int Hq, int Hkv, int D, int cap, long long q_sb,
+                                 long long q_st, long long q_sh, float scale, void* stream) {
+  KSA_ENTER(q);
+  KSA_REQUIRE(D == 128 || D == 64, "int4_decode_attn: head_dim %d unsupported (64 or 128)", D);
+  KSA_REQUIRE(Hkv > 0 && Hq >= Hkv && Hq % Hkv == 0, "int4_decode_attn: %d query heads over %d key heads", Hq, Hkv);
+  KSA_REQUIRE(cap > 0 && cap % kI4Align == 0, "int4_decode_attn: capacity %d is no multiple of %d", cap, kI4Align);
+  KSA_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_meta) |
+                reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(v_meta)) & 15) == 0 && q_sb % 8 == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
+              "int4_decode_attn: queries and cache must be 16-byte aligned");
+  KSA_REQUIRE(B >= 0 && Tq >= 0 && (long long)B * Tq < (1 << 28), "int4_decode_attn: bad shape");
+  if (B == 0 || Tq == 0) return 0;
+  const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
+  KSA_REQUIRE(s.items < (1LL << 31) - s.ctas, "int4_decode_attn: too many queries");
+  const long long parts = s.ctas + s.items;
+  float* ws = (float*)workspace;
+  Int4Attn a{(const bf16*)q, q_sb, q_st, q_sh, (const uint8_t*)k, (const uint8_t*)v, (const uint32_t*)k_meta, (const uint32_t*)v_meta,
+             (const int*)start, (const int*)len, ws, (float2*)(ws + parts * s.heads * D), (bf16*)out, B * Tq, Tq, Hq, Hkv, cap, s.heads, s.blocks,
+             s.ctas, scale * 1.4426950408889634f};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (D == 128) return s.heads <= 8 ? launch_int4_attn<128, 1>(a, s.items, st) : launch_int4_attn<128, 2>(a, s.items, st);
+  return s.heads <= 8 ? launch_int4_attn<64, 1>(a, s.items, st) : launch_int4_attn<64, 2>(a, s.items, st);
+}

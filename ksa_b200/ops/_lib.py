@@ -64,6 +64,12 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_kv_cache_append": [P] * 5 + [I] * 5 + [L, L, P],
     "ksa_kv_cache_fill": [P, P, P, P, I, I, I, I, I, I, L, I, I, I, I, I, P],
     "ksa_kv_cache_move": [P] * 5 + [I] * 5 + [P],
+    "ksa_int4_cache_write": [P] * 8 + [I] * 5 + [L, L, L, I, P],
+    "ksa_int4_cache_read": [P] * 7 + [I] * 5 + [P],
+    "ksa_int4_decode_attn": [P] * 9 + [I] * 6 + [L, L, L, F, P],
+    "ksa_int4_weight": [P, P, P, I, I, I, L, I, P],
+    "ksa_int4_weight_values": [P, P, P, I, I, I, I, P],
+    "ksa_int4_linear": [P, P, P, P, I, I, I, I, I, L, L, P],
     "ksa_peer_gather": [P, I, I, L, I, P, P, ctypes.c_uint, I, P],
     "ksa_peer_reduce_adamw": [P, I, I, L, L, P, P, P, P, P, F, F, F, F, F, P, P, P, ctypes.c_uint, I, P],
     "ksa_signal_set": [P, I, P, ctypes.c_uint, P],
@@ -111,6 +117,8 @@ def load() -> ctypes.CDLL:
     lib.ksa_gemm_tall_plan.restype = I
     lib.ksa_gemm_narrow_plan.argtypes = [I] * 6
     lib.ksa_gemm_narrow_plan.restype = I
+    lib.ksa_int4_attn_workspace.argtypes = [I] * 6
+    lib.ksa_int4_attn_workspace.restype = L
     lib.ksa_set_dependent_launch.argtypes = [I]
     lib.ksa_set_dependent_launch.restype = I
     for name, sig in _SIGNATURES.items():
@@ -184,7 +192,8 @@ def _address(x: torch.Tensor) -> int:
 
 
 # kernels launched by one call of an entry point (default 1)
-_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2}
+_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2,
+                     "ksa_int4_decode_attn": 2}
 _launch_count = 0
 
 

@@ -235,6 +235,55 @@ def decode_attention(q, k_cache, v_cache, lengths: torch.Tensor, start: Optional
     return torch.einsum("bhqk,bhkd->bqhd", p, vf).to(q.dtype)
 
 
+# ---------------------------------------------------------------- four bits
+_INT4_LEAST, _INT4_MOST = 2.0 ** -100, 2.0 ** 126
+
+
+def int4_quantize(x: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x`` ``[..., n]`` -> codes ``[..., n / 2]`` uint8 and ``[..., n / group, 2]`` bf16 (scale, offset) in the format of
+    :mod:`ksa_b200.ops.int4`; every step in fp32."""
+    x = x.float().unflatten(-1, (-1, group))
+    bad = ~torch.isfinite(x).all(-1, keepdim=True)
+    x = torch.nan_to_num(x, nan=0.0).clamp(-_INT4_MOST, _INT4_MOST)
+    lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    s = ((hi - lo) / torch.full_like(lo, 15) * 16).bfloat16().float()    # a division: by a number, a GPU multiplies with 1 / 15
+    s = torch.where(s < _INT4_LEAST, torch.zeros_like(s), s)
+    o = (lo - s).bfloat16().float()
+    c = torch.where(s > 0, ((x - o) / s * 16).round() - 16, torch.zeros_like(x)).clamp(0, 15)
+    c = torch.where(bad, torch.zeros_like(c), c).to(torch.uint8).flatten(-2).unflatten(-1, (-1, 8))
+    codes = (c[..., [0, 4, 1, 5]] | (c[..., [2, 6, 3, 7]] << 4)).flatten(-2)
+    scale = torch.cat([s, o], -1).masked_fill(bad, float("nan")).bfloat16()
+    return codes, scale
+
+
+def int4_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """What codes ``[..., n / 2]`` with scales ``[..., groups, 2]`` stand for: ``[..., n]`` bf16."""
+    b = codes.unflatten(-1, (-1, 4))
+    c = torch.cat([b & 15, b >> 4], -1)[..., [0, 2, 4, 6, 1, 3, 5, 7]].flatten(-2)
+    u = (1 + c.float() / 16).unflatten(-1, (scale.shape[-2], -1))
+    # the product is exact in fp32 (13 bits); the sum is rounded to bf16 as if once, because where fp32 loses bits of it the product is less
+    # than a quarter of a step of the offset
+    return (u * scale[..., :1].float() + scale[..., 1:].float()).bfloat16().flatten(-2)
+
+
+def int4_decode_attention(q, k, k_scale, v, v_scale, start: torch.Tensor, length: torch.Tensor, scale: float):
+    """:func:`decode_attention` over a cache in four bits; ``start`` / ``length`` ``[B, Tq]``, cut to the cache, one query and slice at a
+    time, so that nothing outside a slice is read.  Zeros for a slice without slots."""
+    B, Tq, Hq, D = q.shape
+    Hkv, cap = k.shape[1], k.shape[2]
+    out = torch.zeros(B, Tq, Hq, D, dtype=q.dtype, device=q.device)
+    for b in range(B):
+        for t in range(Tq):
+            first = int(start[b, t])
+            lo, hi = max(first, 0), min(first + max(int(length[b, t]), 0), cap)
+            if hi <= lo:
+                continue
+            kf, vf = (int4_values(c[b, :, lo:hi], s[b, :, lo:hi]).float() for c, s in ((k, k_scale), (v, v_scale)))
+            p = torch.softmax(q[b, t].float().view(Hkv, Hq // Hkv, D) @ kf.transpose(1, 2) * scale, -1)
+            out[b, t] = (p @ vf).reshape(Hq, D).to(q.dtype)
+    return out
+
+
 # ---------------------------------------------------------------- losses
 def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100):
     """fp32 token cross entropy: returns ``(sum_loss, n_valid)`` (``muse/losses/ce.py:32-140``)."""
