@@ -118,8 +118,8 @@ static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr
 using namespace ksa;
 
 // k, v: [B, T, H, D] rows with strides (sb, st, sh) in elements.  Rows whose slot is negative or past the cache are not written; of several
-// rows with one slot the last stays: `last` is a workspace [B, cap] int32 of -1 for that, or null where T is at most 64 (rows
-// look at the slots behind theirs) or `distinct` says that no slot occurs twice.
+// rows with one slot the last stays: `last` is a workspace [B, cap] int32 for that, or null where T is at most 64 (rows look at
+// the slots behind theirs) or `distinct` says that no slot occurs twice.
 KSA_API int ksa_int4_cache_write(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* slots,
                                  void* last, int B, int T, int H, int D, int cap, long long sb, long long st, long long sh, int distinct,
                                  void* stream) {
@@ -136,9 +136,11 @@ KSA_API int ksa_int4_cache_write(const void* k, const void* v, void* k_codes, vo
   KSA_REQUIRE((n + kI4Threads - 1) / kI4Threads < (1LL << 31), "int4_cache_write: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool table = !distinct && T > kI4Scan;
-  if (table)
+  if (table) {
+    KSA_CHECK_CUDA(cudaMemsetAsync(last, 0xFF, (size_t)B * cap * sizeof(int), s));
     KSA_CHECK_CUDA(launch_kernel(int4_last_row_kernel, dim3((unsigned)(((long long)B * T + kI4Threads - 1) / kI4Threads)), dim3(kI4Threads), 0, s,
                                  (const int*)slots, (int*)last, B, T, cap));
+  }
   Int4Write a{(const bf16*)k, (const bf16*)v, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_meta, (uint32_t*)v_meta, (const int*)slots,
               table ? (const int*)last : nullptr, sb, st, sh, B, T, H, D, cap, !distinct && !table && T > 1};
   KSA_CHECK_CUDA(launch_stream_kernel(n * 21, int4_cache_write_kernel, dim3((unsigned)((n + kI4Threads - 1) / kI4Threads)), dim3(kI4Threads), 0, s, a));

@@ -76,6 +76,16 @@ int ksa_attn_bwd_fused(const void* q, const void* k, const void* v, const void* 
                        long long dv_rs, long long dv_bs, long long dks_rs, long long dks_bs, long long dvs_rs, long long dvs_bs,
                        int q_off, int k_off, int s_off, int chunk, int n_sum, int window, int tok_window, float scale,
                        void* part_k, void* part_v, const void* q_doc_start, const void* k_doc_end, void* stream);
+int ksa_int4_cache_write(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* slots, void* last,
+                         int B, int T, int H, int D, int cap, long long sb, long long st, long long sh, int distinct, void* stream);
+int ksa_int4_cache_read(const void* k_codes, const void* k_meta, const void* v_codes, const void* v_meta, const void* start, void* k, void* v,
+                        int B, int H, int D, int cap, int rows, void* stream);
+int ksa_int4_decode_attn(const void* q, const void* k, const void* k_meta, const void* v, const void* v_meta, const void* start,
+                         const void* len, void* workspace, void* out, int B, int Tq, int Hq, int Hkv, int D, int cap, long long q_sb,
+                         long long q_st, long long q_sh, float scale, void* stream);
+long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap);
+int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
+                    long long ldc, void* stream);
 int ksa_summary_attn_bwd(const void* q, const void* k, const void* v, const void* ks, const void* vs, const void* o,
                          const void* dout, const void* lse, void* dq, void* dk, void* dv, void* dks, void* dvs, int B, int Hq,
                          int Hkv, int D, int Nq, int seq_len, long long q_rs, long long q_bs, long long k_rs, long long k_bs,
@@ -661,12 +671,141 @@ PyObject* py_attention_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool aligned(const Tensor* t) { return (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15) == 0; }
+
+// The four tensors of a cache in four bits: codes [B, H, cap, D / 2], scales [B, H, cap, D / 32, 2].
+struct Int4Cache {
+  const Tensor *k, *ks, *v, *vs;
+  int B = 0, H = 0, cap = 0, D = 0;
+  explicit Int4Cache(Args& a) : k(a.tensor(at::kByte)), ks(a.tensor()), v(a.tensor(at::kByte)), vs(a.tensor()) {}
+  bool ok() {
+    if (k->dim() != 4 || ks->dim() != 5 || k->sizes() != v->sizes() || ks->sizes() != vs->sizes()) return false;
+    for (int i = 0; i < 4; ++i)
+      if (!fits(k->size(i)) || k->size(i) > INT_MAX / 2) return false;
+    B = (int)k->size(0); H = (int)k->size(1); cap = (int)k->size(2); D = (int)(2 * k->size(3));
+    if (D % 32 != 0 || cap % 16 != 0 || ks->size(0) != B || ks->size(1) != H || ks->size(2) != cap || ks->size(3) != D / 32 || ks->size(4) != 2)
+      return false;
+    for (const Tensor* t : {k, ks, v, vs})
+      if (!t->is_contiguous() || !aligned(t)) return false;
+    return true;
+  }
+};
+bool ints(const Tensor* t, at::IntArrayRef sizes) { return t->sizes() == sizes && t->is_contiguous(); }
+bool eights(const Tensor* t) {       // rows of the last dimension, on 16-byte boundaries
+  if (t->stride(-1) != 1 || !aligned(t)) return false;
+  for (int64_t i = 0; i + 1 < t->dim(); ++i)
+    if (t->stride(i) % 8 != 0) return false;
+  return true;
+}
+bool differentiated(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+
+// int4_cache_write(k cache, k scales, v cache, v scales, k_new, v_new, slots, distinct) -> True
+PyObject* py_int4_cache_write(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  Int4Cache c(a);
+  const Tensor *k = a.tensor(), *x = a.tensor(), *slots = a.tensor(at::kInt);
+  const int distinct = a.integer() != 0;
+  if (!a.ok() || !c.ok() || k->dim() != 4 || k->sizes() != x->sizes() || k->strides() != x->strides() || !eights(k) || !eights(x) ||
+      k->size(0) != c.B || k->size(2) != c.H || k->size(3) != c.D || !fits(k->size(1)) || !ints(slots, {k->size(0), k->size(1)}) ||
+      differentiated({k, x}))
+    return none();
+  const int T = (int)k->size(1);
+  {
+    pybind11::gil_scoped_release no_gil;
+    Tensor last;
+    if (!distinct && T > 64) last = a.empty({c.B, c.cap}, at::kInt);
+    LAUNCH(ksa_int4_cache_write, k->const_data_ptr(), x->const_data_ptr(), c.k->mutable_data_ptr(), c.ks->mutable_data_ptr(),
+           c.v->mutable_data_ptr(), c.vs->mutable_data_ptr(), slots->const_data_ptr(), last.defined() ? last.mutable_data_ptr() : nullptr, c.B, T,
+           c.H, c.D, c.cap, k->stride(0), k->stride(1), k->stride(2), distinct, a.stream());
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// int4_cache_read(k cache, k scales, v cache, v scales, start, rows) -> (k, v)
+PyObject* py_int4_cache_read(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  Int4Cache c(a);
+  const Tensor* start = a.tensor(at::kInt);
+  const long long rows = a.integer();
+  if (!a.ok() || !c.ok() || !vector(start, c.B) || rows <= 0) return none();
+  Tensor k, x;
+  {
+    pybind11::gil_scoped_release no_gil;
+    k = a.empty({c.B, c.H, rows, c.D});
+    x = a.empty({c.B, c.H, rows, c.D});
+    LAUNCH(ksa_int4_cache_read, c.k->const_data_ptr(), c.ks->const_data_ptr(), c.v->const_data_ptr(), c.vs->const_data_ptr(),
+           start->const_data_ptr(), k.mutable_data_ptr(), x.mutable_data_ptr(), c.B, c.H, c.D, c.cap, (int)rows, a.stream());
+  }
+  return wrap(k, x);
+  END_HANDLE_TH_ERRORS
+}
+
+// int4_decode_attention(q, k cache, k scales, v cache, v scales, start, length, scale) -> out
+PyObject* py_int4_decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  const Tensor* q = a.tensor();
+  Int4Cache c(a);
+  const Tensor *start = a.tensor(at::kInt), *length = a.tensor(at::kInt);
+  const float scale = a.real();
+  if (!a.ok() || !c.ok() || q->dim() != 4 || !eights(q) || q->size(0) != c.B || q->size(3) != c.D || (c.D != 64 && c.D != 128) || !fits(q->size(1)) ||
+      !fits(q->size(2)) || q->size(2) % c.H != 0 || !ints(start, {q->size(0), q->size(1)}) || !ints(length, {q->size(0), q->size(1)}) ||
+      differentiated({q}))
+    return none();
+  const int Tq = (int)q->size(1), Hq = (int)q->size(2);
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = a.empty({c.B, Tq, Hq, c.D});
+    const Tensor workspace = a.empty({(int64_t)ksa_int4_attn_workspace(c.B, Tq, Hq, c.H, c.D, c.cap)}, at::kFloat);
+    check("ksa_int4_decode_attn",
+          ksa_int4_decode_attn(q->const_data_ptr(), c.k->const_data_ptr(), c.ks->const_data_ptr(), c.v->const_data_ptr(), c.vs->const_data_ptr(),
+                               start->const_data_ptr(), length->const_data_ptr(), workspace.mutable_data_ptr(), out.mutable_data_ptr(), c.B, Tq,
+                               Hq, c.H, c.D, c.cap, q->stride(0), q->stride(1), q->stride(2), scale, a.stream()), 2);
+  }
+  return wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// int4_linear(x, codes, scales) -> y [..., N], at most 16 rows
+PyObject* py_int4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  const Tensor *x = a.tensor(), *w = a.tensor(at::kByte), *s = a.tensor();
+  if (!a.ok() || !packed2d(w) || s->dim() != 3 || !s->is_contiguous() || !aligned(w) || !aligned(s) || x->dim() < 1) return none();
+  const long long N = w->size(0), K = 2 * w->size(1), groups = s->size(0), pitch = s->size(1), M = x->numel() / K;
+  if (K != x->size(-1) || M > 16 || !fits(N) || !fits(K) || pitch != (N + 3) / 4 * 4 || s->size(2) != 2 || K % groups != 0 ||
+      (K / groups != 32 && K / groups != 64 && K / groups != 128) || !(x->is_contiguous() || (x->dim() == 2 && eights(x))) || !aligned(x) ||
+      differentiated({x}))
+    return none();
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    auto sizes = x->sizes().vec();
+    sizes.back() = N;
+    y = a.empty(sizes);
+    LAUNCH(ksa_int4_linear, x->const_data_ptr(), w->const_data_ptr(), s->const_data_ptr(), y.mutable_data_ptr(), (int)M, (int)N, (int)K,
+           (int)(K / groups), (int)pitch, x->dim() == 2 ? x->stride(0) : K, N, a.stream());
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(g_launches.load()); }
 
 #define FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FN(gemm), FN(linear), FN(linear_dw), FN(dual_linear), FN(rms_norm), FN(rms_norm_bwd), FN(qk_norm_rope),
                            FN(qk_norm_rope_bwd), FN(swiglu), FN(swiglu_bwd), FN(linear_swiglu), FN(gemm_swiglu), FN(norm_linear), FN(attention),
-                           FN(attention_bwd), FN(launches), {nullptr, nullptr, 0, nullptr}};
+                           FN(attention_bwd), FN(int4_cache_write), FN(int4_cache_read),
+                           FN(int4_decode_attention), FN(int4_linear), FN(launches), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "ksa_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -18,6 +18,7 @@ import torch
 
 from . import _lib
 from . import reference as ref
+from ._lib import native as _native
 
 CACHE_GROUP = 32          # values of a cache row that share a scale
 CACHE_SLOTS = 16          # the capacity of a cache is a multiple of this
@@ -117,6 +118,8 @@ def int4_cache_write(cache: Int4Cache, k_new: torch.Tensor, v_new: torch.Tensor,
     """``k_new`` / ``v_new`` ``[B, T, Hkv, D]`` (views of packed rows allowed) go, quantised, into slots ``slots[b, t]``.  Rows whose
     slot is negative or past the capacity are not written; of several rows of a sequence with one slot the last stays.
     ``distinct=True`` vouches that no slot occurs twice in a sequence (saves looking for it in calls of more than 64 rows)."""
+    if _native.int4_cache_write(*cache, k_new, v_new, slots, distinct):
+        return
     B, H, cap, D = _check_cache(cache)
     _require(k_new.dim() == 4 and k_new.shape == v_new.shape and k_new.shape[0] == B and tuple(k_new.shape[2:]) == (H, D),
              f"keys {tuple(k_new.shape)} and values {tuple(v_new.shape)} do not fit a cache of {B} x {H} heads of {D}")
@@ -138,7 +141,7 @@ def int4_cache_write(cache: Int4Cache, k_new: torch.Tensor, v_new: torch.Tensor,
             and k_new.data_ptr() % 16 == 0 and v_new.data_ptr() % 16 == 0):
         k_new, v_new = k_new.clone(memory_format=torch.contiguous_format), v_new.clone(memory_format=torch.contiguous_format)
     with _on(k_new):
-        last = torch.full((B, cap), -1, dtype=torch.int32, device=k_new.device) if T > _TABLE_ROWS and not distinct else None
+        last = torch.empty((B, cap), dtype=torch.int32, device=k_new.device) if T > _TABLE_ROWS and not distinct else None
         _lib.call("ksa_int4_cache_write", k_new, v_new, cache.k, cache.k_scale, cache.v, cache.v_scale, slots, last, B, T, H, D, cap,
                   k_new.stride(0), k_new.stride(1), k_new.stride(2), int(distinct))
 
@@ -146,6 +149,9 @@ def int4_cache_write(cache: Int4Cache, k_new: torch.Tensor, v_new: torch.Tensor,
 def int4_cache_read(cache: Int4Cache, start: torch.Tensor, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values of slots ``start[b] .. start[b] + rows`` of every sequence: ``(k, v)``, each ``[B, Hkv, rows, D]`` bf16; zeros for
     slots outside the cache."""
+    made = _native.int4_cache_read(*cache, start, rows)
+    if made is not None:
+        return made
     B, H, cap, D = _check_cache(cache)
     _require(rows >= 0, f"{rows} rows")
     start = _int32(start, (B,), cache.k.device, "start")
@@ -166,6 +172,10 @@ def int4_decode_attention(q: torch.Tensor, cache: Int4Cache, start: torch.Tensor
     """``q`` ``[B, Tq, Hq, D]``: query ``(b, t)`` attends slots ``start[b, t] .. start[b, t] + length[b, t]`` of sequence ``b``, cut to the
     cache, with no mask inside; zeros where no slot is left.  ``Hq`` is a multiple of the cache's heads; ``D`` is 64 or 128
     on a GPU; ``scale`` defaults to ``D ** -0.5``.  Slots outside a query's slice do not touch its result, whatever they hold."""
+    if q.dim() == 4 and q.shape[3] > 0:
+        made = _native.int4_decode_attention(q, *cache, start, length, q.shape[3] ** -0.5 if scale is None else scale)
+        if made is not None:
+            return made
     B, Hkv, cap, D = _check_cache(cache)
     _require(q.dim() == 4 and q.shape[0] == B and q.shape[3] == D and q.shape[2] > 0 and q.shape[2] % Hkv == 0,
              f"queries {tuple(q.shape)} do not fit a cache of {B} x {Hkv} heads of {D}")
@@ -247,6 +257,9 @@ def _weight_values(weight: Int4Weight, out: torch.Tensor) -> None:
 def int4_linear(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """``x @ W.T`` for ``x`` ``[..., K]`` and ``W = int4_dequantize_weight(weight)``.  At most 16 rows (a decode step) read the codes
     once; more rows multiply with the bf16 values, written out for the call."""
+    made = _native.int4_linear(x, *weight)
+    if made is not None:
+        return made
     N, K, group, pitch = _check_weight(weight)
     _require(x.dim() >= 1 and x.shape[-1] == K, f"rows {tuple(x.shape)} do not fit a weight [{N}, {K}]")
     _require(x.device == weight.codes.device, "rows and weight are on different devices")
