@@ -18,7 +18,9 @@ constexpr int kI4CacheGroup = 32;
 template <int I>
 __device__ __forceinline__ uint32_t i4_unit(uint32_t w) {
   const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (x & 0x00780078u) | 0x3F803F80u;
+  uint32_t u;                       // (x & 0x00780078) | 0x3F803F80: the compiler makes two operations of the plain form
+  asm("lop3.b32 %0, %1, 0x00780078, 0x3F803F80, 0xEA;" : "=r"(u) : "r"(x));
+  return u;
 }
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -76,8 +78,14 @@ __device__ __forceinline__ void i4_quantize(const uint4& raw, uint32_t& word, ui
   }
 }
 
+// Each row of an 8 x 8 matrix of 16-bit values lies in four lanes; afterwards each column does.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }

@@ -9,8 +9,9 @@
 //     scales for K and for V), so no warp waits for another before the end of an item's run;
 //   * both products are mma.sync m16n8k16 with the values straight from their codes (int4.cuh) as an operand.  A lane's four words of a key
 //     are values 32 t .. 32 t + 31 of it, one group with one scale; the order of the head dimension in the product is q's as well, so nothing is
-//     moved.  The probabilities leave the first product in the layout of the second one's right operand (out^T = V^T P^T);
-//     V^T wants the same value of two neighbouring keys in a register, which is a byte permutation of two words before the shift.
+//     moved.  Keys are the 16 rows of the first product and value dimensions those of the second, queries the 8 columns of both, so up to
+//     eight heads waste no row; the probabilities become the second one's right operand by movmatrix.  V^T wants the same value of two
+//     neighbouring keys in a register, which is a byte permutation of two words before the shift.
 // Nothing outside a slice enters a result: slots of the slice's first and last tile that lie outside get probability 0 and scale and offset 0, so
 // that a NaN there stays there.
 #include "host.h"
@@ -46,59 +47,93 @@ __device__ __forceinline__ void i4_slice(const Int4Attn& a, int row, int& lo, in
 __device__ __forceinline__ int i4_tiles(int lo, int hi) {
   return hi > lo ? (hi - (lo & ~(kI4Align - 1)) + kI4Tile - 1) / kI4Tile : 0;
 }
-// Tiles of one item of each row in [from, to), summed by a warp.
-__device__ __forceinline__ long long i4_sum_tiles(const Int4Attn& a, int from, int to, int lane) {
-  long long n = 0;
-  for (int r = from + lane; r < to; r += 32) {
-    int lo, hi;
-    i4_slice(a, r, lo, hi);
-    n += i4_tiles(lo, hi);
+__device__ __forceinline__ int i4_row_tiles(const Int4Attn& a, int row) {
+  if (row >= a.rows) return 0;
+  int lo, hi;
+  i4_slice(a, row, lo, hi);
+  return i4_tiles(lo, hi);
+}
+// Quotients of sizes that fit 32 bits on all but gigantic calls.
+__device__ __forceinline__ long long i4_div(long long n, long long d) {
+  return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+}
+// Tiles of one item of each row in [0, rows), and of those before `row`, summed by a warp.
+__device__ __forceinline__ long long i4_sum_tiles(const Int4Attn& a, int row, long long& before, int lane) {
+  long long n = 0, m = 0;
+  for (int r = lane; r < a.rows; r += 32) {
+    const int here = i4_row_tiles(a, r);
+    n += here;
+    if (r < row) m += here;
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+  for (int d = 16; d > 0; d >>= 1) {
+    n += __shfl_xor_sync(0xffffffffu, n, d);
+    m += __shfl_xor_sync(0xffffffffu, m, d);
+  }
+  before = m;
   return n;
 }
-// CTAs that take part: a tile for each of their warps, at least.
-__device__ __forceinline__ int i4_active(const Int4Attn& a, long long total) {
-  return (int)max(1LL, min((long long)a.ctas, (total + kI4Warps - 1) / kI4Warps));
-}
+// How the sequence of `total` tiles is shared: CTAs that take part (a tile for each of their warps, at least), and their runs, the first
+// `more` of which have one tile more than the others.
+struct Int4Share {
+  int ctas;
+  long long per, more;
+  __device__ __forceinline__ Int4Share(const Int4Attn& a, long long total) {
+    ctas = (int)max(1LL, min((long long)a.ctas, (total + kI4Warps - 1) / kI4Warps));
+    per = i4_div(total, ctas);
+    more = total - per * ctas;
+  }
+  __device__ __forceinline__ long long first(int cta) const { return per * cta + min((long long)cta, more); }
+  __device__ __forceinline__ int owner(long long tile) const {
+    const long long wide = more * (per + 1);
+    return (int)(tile < wide ? i4_div(tile, per + 1) : more + i4_div(tile - wide, per));
+  }
+};
 
 // A place in the sequence of tiles.
 struct Int4Cursor {
   long long at;                    // index in the sequence
   int row, head, tile;             // row, item of the row (KV head and block of its query heads), tile of the item
   int lo, hi, n;                   // the row's slice and tiles
+  long long base;                  // where the item's first tile starts in the cache, in slots
   __device__ __forceinline__ void load(const Int4Attn& a) {
     i4_slice(a, row, lo, hi);
     n = i4_tiles(lo, hi);
   }
-  // to the first row that holds tile `to`, counted from the first tile of row 0
+  __device__ __forceinline__ void enter(const Int4Attn& a) {
+    base = ((long long)(row / a.Tq) * a.Hkv + head / a.blocks) * a.cap + (lo & ~(kI4Align - 1));
+  }
+  // tile `to`, which has to be there, by a warp: 32 rows at a time
   __device__ __forceinline__ void seek(const Int4Attn& a, long long to, int lane) {
     const int per_row = a.Hkv * a.blocks;
     long long left = to;
-    row = 0;
-    while (row + 32 < a.rows) {                                  // whole steps of 32 rows
-      const long long step = i4_sum_tiles(a, row, row + 32, lane) * per_row;
-      if (left < step) break;
-      left -= step;
-      row += 32;
-    }
-    for (; row < a.rows; ++row) {
-      load(a);
-      const long long here = (long long)n * per_row;
-      if (left < here) break;
-      left -= here;
-    }
     at = to;
-    if (row >= a.rows) return;
-    head = (int)(left / n);
-    tile = (int)(left % n);
+    for (int base = 0; base < a.rows; base += 32) {
+      const int mine = i4_row_tiles(a, base + lane);
+      long long sum = mine;                                      // of the rows up to this lane's
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += x;
+      }
+      const long long all = __shfl_sync(0xffffffffu, sum, 31) * per_row;
+      if (left >= all) { left -= all; continue; }
+      const int who = __ffs(__ballot_sync(0xffffffffu, left < sum * per_row)) - 1;
+      left -= __shfl_sync(0xffffffffu, sum - mine, who) * per_row;
+      row = base + who;
+      break;
+    }
+    load(a);
+    head = (int)i4_div(left, n);
+    tile = (int)(left - (long long)head * n);
+    enter(a);
   }
   __device__ __forceinline__ void advance(const Int4Attn& a, int by) {
     at += by;
     if (row >= a.rows) return;
     tile += by;
-    while (tile >= n) {
+    if (tile < n) return;
+    do {
       tile -= n;
       if (++head == a.Hkv * a.blocks) {
         head = 0;
@@ -107,7 +142,8 @@ struct Int4Cursor {
           load(a);
         } while (n == 0);
       }
-    }
+    } while (tile >= n);
+    enter(a);
   }
 };
 
@@ -127,8 +163,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // Slots [first, first + 32) of the cursor's KV head, cut to the cache.  One lane.
 template <int D>
 __device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, Int4Stage<D>& s, uint64_t* bar) {
-  const int first = (c.lo & ~(kI4Align - 1)) + c.tile * kI4Tile, n = min(kI4Tile, a.cap - first);
-  const long long at = ((long long)(c.row / a.Tq) * a.Hkv + c.head / a.blocks) * a.cap + first;
+  const int first = c.tile * kI4Tile, n = min(kI4Tile, a.cap - (c.lo & ~(kI4Align - 1)) - first);
+  const long long at = c.base + first;
   mbar_expect_tx(bar, n * (D + D / 4));
   bulk_load(s.k, a.k + at * (D / 2), n * (D / 2), bar);
   bulk_load(s.k_meta, a.k_meta + at * (D / 32), n * (D / 8), bar);
@@ -161,11 +197,12 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
   grid_dependency_wait();
 
   const int per_row = a.Hkv * a.blocks;
-  const long long total = i4_sum_tiles(a, 0, a.rows, lane) * per_row;
-  const int active = i4_active(a, total), cta = blockIdx.x;
-  if (cta >= active) return;
-  const long long t0 = total * cta / active, t1 = total * (cta + 1) / active;
-  if (t0 >= t1) return;
+  long long none;
+  const long long total = i4_sum_tiles(a, 0, none, lane) * per_row;
+  const Int4Share share(a, total);
+  const int cta = blockIdx.x;
+  if (cta >= share.ctas || total == 0) return;
+  const long long t0 = share.first(cta), t1 = share.first(cta + 1);
 
   Int4Cursor piece;                // the item that the CTA is at, by its first tile of this run
   piece.seek(a, t0, lane);
@@ -193,16 +230,17 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
     const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
     const int heads = min(a.heads, (kvh + 1) * (a.Hq / a.Hkv) - h0);
     const int b = piece.row / a.Tq, tq = piece.row % a.Tq;
-    // queries: rows g and g + 8, in the order in which a lane holds a key's values
-    uint4 qa[WK], qb[WK];
+    // queries: column g of each block of eight, in the order in which a lane holds a key's values
+    uint4 qv[NT][WK];
 #pragma unroll
-    for (int w = 0; w < WK; ++w) {
-      qa[w] = qb[w] = make_uint4(0, 0, 0, 0);
-      const bf16* src = a.q + b * a.q_sb + tq * a.q_st + (h0 + g) * a.q_sh + t * (D / 4) + w * 8;
-      if (g < heads) qa[w] = *reinterpret_cast<const uint4*>(src);
-      if (NT == 2 && g + 8 < heads) qb[w] = *reinterpret_cast<const uint4*>(src + 8 * a.q_sh);
-    }
-    float o[WV * 4][NT][4], m[NT], l[NT];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        qv[n][w] = make_uint4(0, 0, 0, 0);
+        if (n * 8 + g < heads)
+          qv[n][w] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + tq * a.q_st + (h0 + n * 8 + g) * a.q_sh + t * (D / 4) + w * 8);
+      }
+    float o[WV * 4][NT][4], m[NT][2], l[NT][2];      // of queries 2 t and 2 t + 1 of each block
 #pragma unroll
     for (int i = 0; i < WV * 4; ++i)
 #pragma unroll
@@ -210,7 +248,9 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) { m[n] = -INFINITY; l[n] = 0.f; }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
 
     for (; mine < end; mine += kI4Warps) {
       const int first = (piece.lo & ~(kI4Align - 1)) + (int)(mine - item0) * kI4Tile;
@@ -219,74 +259,91 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
       if (!ok) break;
       const Int4Stage<D>& s = stages[stage];
       const bool whole = first >= piece.lo && first + kI4Tile <= piece.hi;
-      // ---- scores: this lane's slots are 16 u + 8 j + 4 e + t of the tile
-      float p[NT][2][2][2];
+      // ---- scores^T = K q^T: row g + 8 j of a block of sixteen is slot 8 j + 4 (g & 1) + g / 2, which V's loads want
+      float p[NT][2][2][2];                        // [u: block of sixteen][j][query 2 t + e]
+      const int slot0 = (g & 1) * 4 + (g >> 1);
+      uint32_t words[2][2][WK], s2[2][2], o2[2][2];
+      float c[2][NT][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = u * 16 + j * 8 + slot0;
+          const uint32_t meta = s.k_meta[key * (D / 32) + t * WK / 4];
+          s2[u][j] = i4_scale2(meta);
+          o2[u][j] = i4_offset2(meta);
+          if (D == 128) *reinterpret_cast<uint4*>(words[u][j]) = *reinterpret_cast<const uint4*>(&s.k[key * (D / 8) + t * WK]);
+          else *reinterpret_cast<uint2*>(words[u][j]) = *reinterpret_cast<const uint2*>(&s.k[key * (D / 8) + t * WK]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[u][n][e] = 0.f;
+      }
+#pragma unroll
+      for (int w = 0; w < WK; ++w)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {               // two chains of products side by side
+          uint32_t x[4], y[4];
+          i4_values(x, words[u][0][w], s2[u][0], o2[u][0]);
+          i4_values(y, words[u][1][w], s2[u][1], o2[u][1]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16(c[u][n], x[0], y[0], x[1], y[1], qv[n][w].x, qv[n][w].y);
+            mma_bf16(c[u][n], x[2], y[2], x[3], y[3], qv[n][w].z, qv[n][w].w);
+          }
+        }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = u * 16 + j * 8 + (g & 1) * 4 + (g >> 1);
-          const uint32_t meta = s.k_meta[key * (D / 32) + t * WK / 4];
-          const uint32_t s2 = i4_scale2(meta), o2 = i4_offset2(meta);
-          uint32_t words[WK];
-          if (D == 128) *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(&s.k[key * (D / 8) + t * WK]);
-          else *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(&s.k[key * (D / 8) + t * WK]);
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int w = 0; w < WK; ++w) {
-            uint32_t x[4];
-            i4_values(x, words[w], s2, o2);
-            mma_bf16(c, qa[w].x, qb[w].x, qa[w].y, qb[w].y, x[0], x[1]);
-            mma_bf16(c, qa[w].z, qb[w].z, qa[w].w, qb[w].w, x[2], x[3]);
-          }
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) p[n][u][j][e] = c[n * 2 + e] * a.scale;
-        }
+            for (int e = 0; e < 2; ++e) p[n][u][j][e] = c[u][n][j * 2 + e] * a.scale;
       if (!whole) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) {
+            const int key = first + u * 16 + j * 8 + slot0;
+            if (key < piece.lo || key >= piece.hi) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = first + u * 16 + j * 8 + e * 4 + t;
-              const bool in = key >= piece.lo && key < piece.hi;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) p[n][u][j][e] = in ? p[n][u][j][e] : -INFINITY;
+              for (int n = 0; n < NT; ++n) p[n][u][j][0] = p[n][u][j][1] = -INFINITY;
             }
+          }
       }
-      // ---- running maximum and sum of each query (rows g and g + 8, shared by the four lanes of a row)
-      float corr[NT];
+      // ---- running maximum and sum of queries 2 t and 2 t + 1, the columns of this lane's outputs as well
+      float corr[NT][2];
       bool moved = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float mx = m[n];
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, p[n][i >> 2][(i >> 1) & 1][i & 1]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        corr[n] = mx == m[n] ? 1.f : fast_exp2(m[n] - mx);
-        moved |= mx != m[n];
-        m[n] = mx;
-        l[n] *= corr[n];
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(p[n][0][0][e], p[n][0][1][e]), fmaxf(p[n][1][0][e], p[n][1][1][e]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx, m[n][e]);
+          corr[n][e] = mx == m[n][e] ? 1.f : fast_exp2(m[n][e] - mx);
+          moved |= mx != m[n][e];
+          m[n][e] = mx;
+          float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float& x = p[n][i >> 2][(i >> 1) & 1][i & 1];
-          x = fast_exp2(x - mx);
-          l[n] += x;
+          for (int i = 0; i < 4; ++i) {
+            float& x = p[n][i >> 1][i & 1][e];
+            x = fast_exp2(x - mx);
+            sum += x;
+          }
+          l[n][e] = fmaf(l[n][e], corr[n][e], sum);
         }
-      }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float c0 = __shfl_sync(0xffffffffu, corr[n], t * 8), c1 = __shfl_sync(0xffffffffu, corr[n], t * 8 + 4);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < WV * 4; ++i) {
-            o[i][n][0] *= c0; o[i][n][1] *= c1; o[i][n][2] *= c0; o[i][n][3] *= c1;
+            o[i][n][0] *= corr[n][0]; o[i][n][1] *= corr[n][1]; o[i][n][2] *= corr[n][0]; o[i][n][3] *= corr[n][1];
           }
-        }
       }
       // ---- out^T += V^T P^T: this lane's dimensions are D / 8 * g and on
 #pragma unroll
@@ -295,29 +352,29 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) pb[n][j] = pack_bf16x2(p[n][u][j][0], p[n][u][j][1]);
-        uint32_t words[4][WV], meta[4];
+          for (int j = 0; j < 2; ++j) pb[n][j] = transpose8(pack_bf16x2(p[n][u][j][0], p[n][u][j][1]));
+        uint32_t rows[4][WV], meta[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = u * 16 + i * 4 + t;
-          if (D == 128) *reinterpret_cast<uint2*>(words[i]) = *reinterpret_cast<const uint2*>(&s.v[key * (D / 8) + g * WV]);
-          else words[i][0] = s.v[key * (D / 8) + g];
+          if (D == 128) *reinterpret_cast<uint2*>(rows[i]) = *reinterpret_cast<const uint2*>(&s.v[key * (D / 8) + g * WV]);
+          else rows[i][0] = s.v[key * (D / 8) + g];
           meta[i] = s.v_meta[key * (D / 32) + g * WV / 4];
           if (!whole && (first + key < piece.lo || first + key >= piece.hi)) meta[i] = 0;
         }
-        uint32_t s2[2], o2[2];
+        uint32_t vs2[2], vo2[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          s2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x5410);
-          o2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x7632);
+          vs2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x5410);
+          vo2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x7632);
         }
 #pragma unroll
         for (int w = 0; w < WV; ++w) {
           uint32_t even[2][4], odd[2][4];      // [pair of keys][value of the word / 2]
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            i4_values(even[j], __byte_perm(words[2 * j][w], words[2 * j + 1][w], 0x5410), s2[j], o2[j]);
-            i4_values(odd[j], __byte_perm(words[2 * j][w], words[2 * j + 1][w], 0x7632), s2[j], o2[j]);
+            i4_values(even[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x5410), vs2[j], vo2[j]);
+            i4_values(odd[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x7632), vs2[j], vo2[j]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -333,14 +390,15 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
     // ---- the warps' parts of the item -> one
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
-      l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
-      const int q = n * 8 + g;
-      if (t == 0 && q < heads) { s_m[warp * a.heads + q] = m[n]; s_l[warp * a.heads + q] = l[n]; }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int qe = n * 8 + t * 2 + e;
+        float sum = l[n][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         if (qe < heads) {
+          if (g == 0) { s_m[warp * a.heads + qe] = m[n][e]; s_l[warp * a.heads + qe] = sum; }
           float* dst = s_o + (warp * a.heads + qe) * D + g * (D / 8);
 #pragma unroll
           for (int i = 0; i < WV * 4; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[i][n][e], o[i][n][2 + e]);
@@ -382,42 +440,75 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
   }
 }
 
-// Items that several CTAs shared, and empty ones.
+// One query head of an item that several CTAs shared, or of an empty one.  The warps take the parts in turn, a lane D / 32 dimensions.
+constexpr int kI4MergeWarps = 4;
 template <int D>
-__global__ void __launch_bounds__(128) int4_attn_merge_kernel(const Int4Attn a) {
+__global__ void __launch_bounds__(kI4MergeWarps * 32) int4_attn_merge_kernel(const Int4Attn a) {
+  constexpr int V = D / 32;
+  __shared__ float s_o[kI4MergeWarps][D], s_m[kI4MergeWarps], s_l[kI4MergeWarps];
   grid_dependency_launch();
   grid_dependency_wait();
-  const int per_row = a.Hkv * a.blocks, lane = threadIdx.x & 31;
-  const long long item = blockIdx.x;
-  const int row = (int)(item / per_row), head = (int)(item % per_row);
-  int lo, hi;
-  i4_slice(a, row, lo, hi);
-  const int n = i4_tiles(lo, hi), group = a.Hq / a.Hkv;
-  const int kvh = head / a.blocks, h0 = kvh * group + head % a.blocks * a.heads, heads = min(a.heads, (kvh + 1) * group - h0);
-  bf16* out = a.out + ((long long)row * a.Hq + h0) * D;
+  const int per_row = a.Hkv * a.blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int item = blockIdx.x, q = blockIdx.y;
+  const int row = item / per_row, head = item % per_row;
+  const int group = a.Hq / a.Hkv, kvh = head / a.blocks, h0 = kvh * group + head % a.blocks * a.heads;
+  if (h0 + q >= (kvh + 1) * group) return;
+  bf16* out = a.out + ((long long)row * a.Hq + h0 + q) * D;
+  const int n = i4_row_tiles(a, row);
   if (n == 0) {
-    for (int i = threadIdx.x; i < heads * D; i += 128) out[i] = __float2bfloat16(0.f);
+    if (threadIdx.x < D) out[threadIdx.x] = __float2bfloat16(0.f);
     return;
   }
-  const long long before = i4_sum_tiles(a, 0, row, lane), total = (before + i4_sum_tiles(a, row, a.rows, lane)) * per_row;
-  const long long first = before * per_row + (long long)head * n, last = first + n - 1;
-  const int active = i4_active(a, total);
-  const long long c0 = ((first + 1) * active - 1) / total, c1 = ((last + 1) * active - 1) / total;
-  if (c0 == c1) return;
-  const long long part0 = c0 + item;
-  const int parts = (int)(c1 - c0 + 1);
-  for (int i = threadIdx.x; i < heads * D; i += 128) {
-    const int q = i / D, d = i % D;
-    float mx = -INFINITY;
-    for (int s = 0; s < parts; ++s) mx = fmaxf(mx, a.part_ml[(part0 + s) * a.heads + q].x);
-    float sum = 0.f, acc = 0.f;
-    for (int s = 0; s < parts; ++s) {
-      const float2 ml = a.part_ml[(part0 + s) * a.heads + q];
-      const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mx);
-      sum = fmaf(ml.y, f, sum);
-      acc = fmaf(a.part_o[((part0 + s) * a.heads + q) * D + d], f, acc);
+  long long before;
+  const long long total = i4_sum_tiles(a, row, before, lane) * per_row;
+  const Int4Share share(a, total);
+  const long long first = before * per_row + (long long)head * n;
+  const int c0 = share.owner(first), parts = share.owner(first + n - 1) - c0 + 1;
+  if (parts == 1) return;
+  const long long part0 = ((long long)c0 + item) * a.heads + q;          // in rows of part_o
+  float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+  constexpr int kAtOnce = 4;
+  for (int s = warp; s < parts; s += kI4MergeWarps * kAtOnce) {
+    float2 ml[kAtOnce];
+    float v[kAtOnce][V];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int at = s + i * kI4MergeWarps;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (at < parts) {
+        const long long r = part0 + (long long)at * a.heads;
+        ml[i] = a.part_ml[r];
+        if (V == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(a.part_o + r * D + lane * V);
+        else *reinterpret_cast<float2*>(v[i]) = *reinterpret_cast<const float2*>(a.part_o + r * D + lane * V);
+      }
     }
-    out[i] = __float2bfloat16(__fdividef(acc, sum));
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (s + i * kI4MergeWarps >= parts) break;
+      const float mx = fmaxf(m, ml[i].x), f0 = m == mx ? 1.f : fast_exp2(m - mx), f1 = ml[i].x == mx ? 1.f : fast_exp2(ml[i].x - mx);
+      m = mx;
+      l = l * f0 + ml[i].y * f1;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[k] = o[k] * f0 + v[i][k] * f1;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) s_o[warp][lane * V + k] = o[k];
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float mx = s_m[0], sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 1; w < kI4MergeWarps; ++w) mx = fmaxf(mx, s_m[w]);
+#pragma unroll
+    for (int w = 0; w < kI4MergeWarps; ++w) {
+      const float f = s_m[w] == mx ? 1.f : fast_exp2(s_m[w] - mx);
+      sum = fmaf(s_l[w], f, sum);
+      acc = fmaf(s_o[w][threadIdx.x], f, acc);
+    }
+    out[threadIdx.x] = __float2bfloat16(__fdividef(acc, sum));
   }
 }
 
@@ -452,7 +543,7 @@ static int launch_int4_attn(const Int4Attn& a, long long items, cudaStream_t st)
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
   KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Warps * 32), i4_smem<D>(a.heads), st, a, status));
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3((unsigned)items), dim3(128), 0, st, a));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3((unsigned)items, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
   return 0;
 }
 
