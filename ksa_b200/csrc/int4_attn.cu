@@ -19,9 +19,11 @@
 
 namespace ksa {
 
-constexpr int kI4Warps = 4;
+constexpr int kI4Warps = 4;        // that compute; one more fetches
+constexpr int kI4Threads = kI4Warps * 32 + 32;
 constexpr int kI4Tile = 32;        // slots of a tile
-constexpr int kI4Stages = 3;       // tiles in flight of a warp
+constexpr int kI4Chunk = kI4Warps * kI4Tile;       // slots fetched at once, a tile for each warp
+constexpr int kI4Stages = 3;       // chunks in flight of a CTA
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
 
 struct Int4Attn {
@@ -128,31 +130,29 @@ struct Int4Cursor {
     tile = (int)(left - (long long)head * n);
     enter(a);
   }
+  // by `by` tiles, at most to the first of the next item
   __device__ __forceinline__ void advance(const Int4Attn& a, int by) {
     at += by;
-    if (row >= a.rows) return;
     tile += by;
     if (tile < n) return;
-    do {
-      tile -= n;
-      if (++head == a.Hkv * a.blocks) {
-        head = 0;
-        do {
-          if (++row >= a.rows) return;
-          load(a);
-        } while (n == 0);
-      }
-    } while (tile >= n);
+    tile = 0;
+    if (++head == a.Hkv * a.blocks) {
+      head = 0;
+      do {
+        if (++row >= a.rows) return;
+        load(a);
+      } while (n == 0);
+    }
     enter(a);
   }
 };
 
 template <int D>
 struct Int4Stage {
-  uint32_t k[kI4Tile * D / 8];
-  uint32_t v[kI4Tile * D / 8];
-  uint32_t k_meta[kI4Tile * D / 32];
-  uint32_t v_meta[kI4Tile * D / 32];
+  uint32_t k[kI4Chunk * D / 8];
+  uint32_t v[kI4Chunk * D / 8];
+  uint32_t k_meta[kI4Chunk * D / 32];
+  uint32_t v_meta[kI4Chunk * D / 32];
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -160,10 +160,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// Slots [first, first + 32) of the cursor's KV head, cut to the cache.  One lane.
+// The tiles of the cursor's item from its own on, `tiles` of them, cut to the cache.  One thread.
 template <int D>
-__device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, Int4Stage<D>& s, uint64_t* bar) {
-  const int first = c.tile * kI4Tile, n = min(kI4Tile, a.cap - (c.lo & ~(kI4Align - 1)) - first);
+__device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, int tiles, Int4Stage<D>& s, uint64_t* bar) {
+  const int first = c.tile * kI4Tile, n = min(tiles * kI4Tile, a.cap - (c.lo & ~(kI4Align - 1)) - first);
   const long long at = c.base + first;
   mbar_expect_tx(bar, n * (D + D / 4));
   bulk_load(s.k, a.k + at * (D / 2), n * (D / 2), bar);
@@ -171,26 +171,28 @@ __device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c,
   bulk_load(s.v, a.v + at * (D / 2), n * (D / 2), bar);
   bulk_load(s.v_meta, a.v_meta + at * (D / 32), n * (D / 8), bar);
 }
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kI4Warps * 32) : "memory"); }
 
 // NT: query heads of an item in eights (1 or 2).
 template <int D, int NT>
-__global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kernel(const Int4Attn a, int* status) {
+__global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(const Int4Attn a, int* status) {
   constexpr int WK = D / 32;       // words of a key that a lane multiplies with the queries
   constexpr int WV = D / 64;       // words of a value row of which a lane holds the dimensions
   extern __shared__ __align__(128) uint8_t raw[];
   Int4Stage<D>* ring = reinterpret_cast<Int4Stage<D>*>(raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kI4Warps * kI4Stages);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + kI4Warps * kI4Stages);
-  float* s_m = reinterpret_cast<float*>(full + kI4Warps * kI4Stages + 2);      // [warps][heads]
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kI4Stages);
+  uint64_t* empty = full + kI4Stages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kI4Stages);
+  float* s_m = reinterpret_cast<float*>(empty + kI4Stages + 2);      // [warps][heads]
   float* s_l = s_m + kI4Warps * a.heads;
-  float* s_o = s_l + kI4Warps * a.heads;                                       // [warps][heads][D]
+  float* s_o = s_l + kI4Warps * a.heads;                             // [warps][heads][D]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const WaitGuard guard{abort_flag, status};
   grid_dependency_launch();
-  if (lane == 0) {
-    for (int i = 0; i < kI4Stages; ++i) mbar_init(&full[warp * kI4Stages + i], 1);
-    if (warp == 0) *abort_flag = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kI4Stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kI4Warps); }
+    *abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -203,30 +205,33 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
   const int cta = blockIdx.x;
   if (cta >= share.ctas || total == 0) return;
   const long long t0 = share.first(cta), t1 = share.first(cta + 1);
-
-  Int4Cursor piece;                // the item that the CTA is at, by its first tile of this run
+  Int4Cursor piece;                // the item that the warp is at, by its first tile of this run
   piece.seek(a, t0, lane);
-  Int4Cursor next = piece;         // what this warp asks for next
-  next.advance(a, warp);
-  uint64_t* bars = full + warp * kI4Stages;
-  Int4Stage<D>* stages = ring + warp * kI4Stages;
-  int filling = 0, stage = 0;
+  int stage = 0;
   uint32_t phase = 0;
-  bool ok = true;
-  auto fetch = [&]() {
-    if (next.at < t1) {
-      if (lane == 0) i4_fetch<D>(a, next, stages[filling], &bars[filling]);
-      next.advance(a, kI4Warps);
-      if (++filling == kI4Stages) filling = 0;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kI4Stages; ++i) fetch();
 
-  long long mine = t0 + warp;      // index of the next tile of this warp
+  if (warp == kI4Warps) {
+    // ---------------------------------------------------------------- the warp that fetches
+    int chunks = 0;
+    while (piece.at < t1) {
+      const int tiles = (int)min((long long)min(kI4Warps, piece.n - piece.tile), t1 - piece.at);
+      if (chunks >= kI4Stages && !__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty))) break;
+      if (elect_one()) i4_fetch<D>(a, piece, tiles, ring[stage], &full[stage]);
+      ++chunks;
+      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
+      piece.advance(a, tiles);
+    }
+    // whatever the others have given up on: the last copies land before the block leaves
+    const long long began = clock64();
+    for (int i = max(0, chunks - kI4Stages); i < chunks; ++i)
+      while (!mbar_try_wait(&full[i % kI4Stages], (i / kI4Stages) & 1) && clock64() - began < kWaitLimitCycles) {}
+    return;
+  }
+
+  // ------------------------------------------------------------------ the warps that compute
+  bool ok = true;
   while (piece.at < t1) {
-    const long long item0 = piece.at - piece.tile;               // the item's first tile
-    const long long end = min(t1, item0 + piece.n);
+    const int end = (int)min((long long)piece.n, piece.tile + (t1 - piece.at));        // tiles [piece.tile, end) of the item
     const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
     const int heads = min(a.heads, (kvh + 1) * (a.Hq / a.Hkv) - h0);
     const int b = piece.row / a.Tq, tq = piece.row % a.Tq;
@@ -252,12 +257,13 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
 #pragma unroll
       for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
 
-    for (; mine < end; mine += kI4Warps) {
-      const int first = (piece.lo & ~(kI4Align - 1)) + (int)(mine - item0) * kI4Tile;
-      ok = ok && mbar_wait(&bars[stage], phase, guard, kTimeoutTmaFull);
-      ok = __all_sync(0xffffffffu, ok);
+    for (int chunk = piece.tile; chunk < end; chunk += kI4Warps) {
+      const int first = (piece.lo & ~(kI4Align - 1)) + (chunk + warp) * kI4Tile;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
-      const Int4Stage<D>& s = stages[stage];
+      if (chunk + warp < end) {
+      const uint32_t *sk = ring[stage].k + warp * (kI4Tile * D / 8), *sv = ring[stage].v + warp * (kI4Tile * D / 8);
+      const uint32_t *skm = ring[stage].k_meta + warp * (kI4Tile * D / 32), *svm = ring[stage].v_meta + warp * (kI4Tile * D / 32);
       const bool whole = first >= piece.lo && first + kI4Tile <= piece.hi;
       // ---- scores^T = K q^T: row g + 8 j of a block of sixteen is slot 8 j + 4 (g & 1) + g / 2, which V's loads want
       float p[NT][2][2][2];                        // [u: block of sixteen][j][query 2 t + e]
@@ -269,11 +275,11 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int key = u * 16 + j * 8 + slot0;
-          const uint32_t meta = s.k_meta[key * (D / 32) + t * WK / 4];
+          const uint32_t meta = skm[key * (D / 32) + t * WK / 4];
           s2[u][j] = i4_scale2(meta);
           o2[u][j] = i4_offset2(meta);
-          if (D == 128) *reinterpret_cast<uint4*>(words[u][j]) = *reinterpret_cast<const uint4*>(&s.k[key * (D / 8) + t * WK]);
-          else *reinterpret_cast<uint2*>(words[u][j]) = *reinterpret_cast<const uint2*>(&s.k[key * (D / 8) + t * WK]);
+          if (D == 128) *reinterpret_cast<uint4*>(words[u][j]) = *reinterpret_cast<const uint4*>(&sk[key * (D / 8) + t * WK]);
+          else *reinterpret_cast<uint2*>(words[u][j]) = *reinterpret_cast<const uint2*>(&sk[key * (D / 8) + t * WK]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -357,9 +363,9 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = u * 16 + i * 4 + t;
-          if (D == 128) *reinterpret_cast<uint2*>(rows[i]) = *reinterpret_cast<const uint2*>(&s.v[key * (D / 8) + g * WV]);
-          else rows[i][0] = s.v[key * (D / 8) + g];
-          meta[i] = s.v_meta[key * (D / 32) + g * WV / 4];
+          if (D == 128) *reinterpret_cast<uint2*>(rows[i]) = *reinterpret_cast<const uint2*>(&sv[key * (D / 8) + g * WV]);
+          else rows[i][0] = sv[key * (D / 8) + g];
+          meta[i] = svm[key * (D / 32) + g * WV / 4];
           if (!whole && (first + key < piece.lo || first + key >= piece.hi)) meta[i] = 0;
         }
         uint32_t vs2[2], vo2[2];
@@ -382,9 +388,10 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
             for (int n = 0; n < NT; ++n) mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], pb[n][0], pb[n][1]);
         }
       }
+      }
       __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
       if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
-      fetch();
     }
 
     // ---- the warps' parts of the item -> one
@@ -405,8 +412,8 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
         }
       }
     }
-    __syncthreads();
-    const bool alone = piece.tile == 0 && end == item0 + piece.n;          // the whole item is here
+    compute_sync();
+    const bool alone = piece.tile == 0 && end == piece.n;          // the whole item is here
     const long long part = cta + (long long)piece.row * per_row + piece.head;
     for (int i = threadIdx.x; i < heads * D; i += kI4Warps * 32) {
       const int q = i / D, d = i % D;
@@ -427,16 +434,8 @@ __global__ void __launch_bounds__(kI4Warps * 32, NT == 1 ? 3 : 2) int4_attn_kern
         if (d == 0) a.part_ml[part * a.heads + q] = make_float2(mx, sum);
       }
     }
-    __syncthreads();
-    piece.advance(a, (int)(end - piece.at));
-  }
-  // after a wait that gave up: this warp's copies that are still in flight land before the block leaves
-  if (!ok && lane == 0) {
-    const long long began = clock64();
-    for (int i = 0; i < kI4Stages && mine < next.at; ++i, mine += kI4Warps) {
-      while (!mbar_try_wait(&bars[stage], phase) && clock64() - began < kWaitLimitCycles) {}
-      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
-    }
+    compute_sync();
+    piece.advance(a, end - piece.tile);
   }
 }
 
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(kI4MergeWarps * 32) int4_attn_merge_kernel(con
 
 template <int D>
 static size_t i4_smem(int heads) {
-  return sizeof(Int4Stage<D>) * kI4Warps * kI4Stages + (kI4Warps * kI4Stages + 2) * 8 + sizeof(float) * kI4Warps * heads * (D + 2);
+  return sizeof(Int4Stage<D>) * kI4Stages + (2 * kI4Stages + 2) * 8 + sizeof(float) * kI4Warps * heads * (D + 2);
 }
 
 struct Int4Shape {
@@ -542,7 +541,7 @@ static int launch_int4_attn(const Int4Attn& a, long long items, cudaStream_t st)
   KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT>, i4_smem<D>(NT * 8)));
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Warps * 32), i4_smem<D>(a.heads), st, a, status));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Threads), i4_smem<D>(a.heads), st, a, status));
   KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3((unsigned)items, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
   return 0;
 }
