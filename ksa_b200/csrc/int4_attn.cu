@@ -14,16 +14,20 @@
 //     neighbouring keys in a register, which is a byte permutation of two words before the shift.
 // Nothing outside a slice enters a result: slots of the slice's first and last tile that lie outside get probability 0 and scale and offset 0, so
 // that a NaN there stays there.
+#include <math.h>
+
 #include "host.h"
 #include "int4.cuh"
 
 namespace ksa {
 
-constexpr int kI4Warps = 4;        // that compute; one more fetches
+constexpr int kI4Tile = 32;        // slots of a tile, which one warp takes
+constexpr int kI4Warps = 4;        // that compute, each the same tile of every group of kI4Warps tiles; one more fetches
 constexpr int kI4Threads = kI4Warps * 32 + 32;
-constexpr int kI4Tile = 32;        // slots of a tile
-constexpr int kI4Chunk = kI4Warps * kI4Tile;       // slots fetched at once, a tile for each warp
-constexpr int kI4Stages = 3;       // chunks in flight of a CTA
+constexpr int kI4Spread = 4;       // tiles that a CTA gets at least
+// CTAs of an SM (fifteen warps get 128 registers each, ten 168)
+template <int NT>
+constexpr int i4_ctas() { return NT == 1 ? 3 : 2; }
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
 
 struct Int4Attn {
@@ -34,11 +38,13 @@ struct Int4Attn {
   const int *start, *len;          // [B, Tq]
   float* part_o;                   // [CTAs + items, heads, D]
   float2* part_ml;                 // [CTAs + items, heads]: max (log2 units), sum
+  int2* shared;                    // [CTAs]: the item that begins in a CTA's run and goes on behind it, and over how many CTAs (0: none does)
   bf16* out;                       // [B, Tq, Hq, D]
   int rows, Tq, Hq, Hkv, cap;      // rows = B * Tq
   int heads, blocks;               // query heads of an item; items of a KV head
-  int ctas;
-  float scale;                     // * log2(e)
+  int ctas, groups;                // of the grid; of the ring, kI4Warps tiles each
+  float scale;                     // its magnitude * log2(e)
+  uint32_t negate;                 // the sign bits of a pair of queries where the scale is negative
 };
 
 __device__ __forceinline__ void i4_slice(const Int4Attn& a, int row, int& lo, int& hi) {
@@ -59,29 +65,24 @@ __device__ __forceinline__ int i4_row_tiles(const Int4Attn& a, int row) {
 __device__ __forceinline__ long long i4_div(long long n, long long d) {
   return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
 }
-// Tiles of one item of each row in [0, rows), and of those before `row`, summed by a warp.
-__device__ __forceinline__ long long i4_sum_tiles(const Int4Attn& a, int row, long long& before, int lane) {
-  long long n = 0, m = 0;
-  for (int r = lane; r < a.rows; r += 32) {
-    const int here = i4_row_tiles(a, r);
-    n += here;
-    if (r < row) m += here;
-  }
+// Rows' tiles, 32 rows at a time: this lane's row's, and the sum up to it.
+__device__ __forceinline__ long long i4_scan(int mine, int lane) {
+  long long sum = mine;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    n += __shfl_xor_sync(0xffffffffu, n, d);
-    m += __shfl_xor_sync(0xffffffffu, m, d);
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += x;
   }
-  before = m;
-  return n;
+  return sum;
 }
-// How the sequence of `total` tiles is shared: CTAs that take part (a tile for each of their warps, at least), and their runs, the first
+
+// How the sequence of `total` tiles is shared: CTAs that take part, and their runs, the first
 // `more` of which have one tile more than the others.
 struct Int4Share {
   int ctas;
   long long per, more;
   __device__ __forceinline__ Int4Share(const Int4Attn& a, long long total) {
-    ctas = (int)max(1LL, min((long long)a.ctas, (total + kI4Warps - 1) / kI4Warps));
+    ctas = (int)max(1LL, min((long long)a.ctas, (total + kI4Spread - 1) / kI4Spread));
     per = i4_div(total, ctas);
     more = total - per * ctas;
   }
@@ -102,21 +103,28 @@ struct Int4Cursor {
     i4_slice(a, row, lo, hi);
     n = i4_tiles(lo, hi);
   }
+  // The number of tiles, by a warp; `mine` and `sum` keep the last 32 rows' scan, which is all of it for up to 32 rows.
+  static __device__ __forceinline__ long long count(const Int4Attn& a, int& mine, long long& sum, int lane) {
+    long long rows = 0;
+    for (int base = 0; base < a.rows; base += 32) {
+      mine = i4_row_tiles(a, base + lane);
+      sum = i4_scan(mine, lane);
+      rows += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return rows * (a.Hkv * a.blocks);
+  }
   __device__ __forceinline__ void enter(const Int4Attn& a) {
     base = ((long long)(row / a.Tq) * a.Hkv + head / a.blocks) * a.cap + (lo & ~(kI4Align - 1));
   }
-  // tile `to`, which has to be there, by a warp: 32 rows at a time
-  __device__ __forceinline__ void seek(const Int4Attn& a, long long to, int lane) {
+  // tile `to`, which has to be there, by a warp
+  __device__ __forceinline__ void seek(const Int4Attn& a, long long to, int mine, long long sum, int lane) {
     const int per_row = a.Hkv * a.blocks;
     long long left = to;
     at = to;
     for (int base = 0; base < a.rows; base += 32) {
-      const int mine = i4_row_tiles(a, base + lane);
-      long long sum = mine;                                      // of the rows up to this lane's
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += x;
+      if (a.rows > 32) {
+        mine = i4_row_tiles(a, base + lane);
+        sum = i4_scan(mine, lane);
       }
       const long long all = __shfl_sync(0xffffffffu, sum, 31) * per_row;
       if (left >= all) { left -= all; continue; }
@@ -147,51 +155,56 @@ struct Int4Cursor {
   }
 };
 
-template <int D>
-struct Int4Stage {
-  uint32_t k[kI4Chunk * D / 8];
-  uint32_t v[kI4Chunk * D / 8];
-  uint32_t k_meta[kI4Chunk * D / 32];
-  uint32_t v_meta[kI4Chunk * D / 32];
-};
-
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// The tiles of the cursor's item from its own on, `tiles` of them, cut to the cache.  One thread.
+// The ring: tile i of a CTA's run lies in slot i % (groups * kI4Warps) of each of the four parts.
 template <int D>
-__device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, int tiles, Int4Stage<D>& s, uint64_t* bar) {
+struct Int4Ring {
+  uint32_t *k, *v, *k_meta, *v_meta;
+  __device__ __forceinline__ Int4Ring(uint8_t* raw, int tiles) {
+    k = reinterpret_cast<uint32_t*>(raw);
+    v = k + tiles * (kI4Tile * D / 8);
+    k_meta = v + tiles * (kI4Tile * D / 8);
+    v_meta = k_meta + tiles * (kI4Tile * D / 32);
+  }
+};
+// `tiles` tiles of the cursor's item from its own on, cut to the cache, into the ring from `slot` on.  One thread; `last`: the group is complete.
+template <int D>
+__device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c, int tiles, const Int4Ring<D>& ring, int slot, uint64_t* bar, bool last) {
   const int first = c.tile * kI4Tile, n = min(tiles * kI4Tile, a.cap - (c.lo & ~(kI4Align - 1)) - first);
   const long long at = c.base + first;
-  mbar_expect_tx(bar, n * (D + D / 4));
-  bulk_load(s.k, a.k + at * (D / 2), n * (D / 2), bar);
-  bulk_load(s.k_meta, a.k_meta + at * (D / 32), n * (D / 8), bar);
-  bulk_load(s.v, a.v + at * (D / 2), n * (D / 2), bar);
-  bulk_load(s.v_meta, a.v_meta + at * (D / 32), n * (D / 8), bar);
+  if (last) mbar_expect_tx(bar, n * (D + D / 4));
+  else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(n * (D + D / 4)) : "memory");
+  bulk_load(ring.k + slot * (kI4Tile * D / 8), a.k + at * (D / 2), n * (D / 2), bar);
+  bulk_load(ring.k_meta + slot * (kI4Tile * D / 32), a.k_meta + at * (D / 32), n * (D / 8), bar);
+  bulk_load(ring.v + slot * (kI4Tile * D / 8), a.v + at * (D / 2), n * (D / 2), bar);
+  bulk_load(ring.v_meta + slot * (kI4Tile * D / 32), a.v_meta + at * (D / 32), n * (D / 8), bar);
 }
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kI4Warps * 32) : "memory"); }
 
 // NT: query heads of an item in eights (1 or 2).
 template <int D, int NT>
-__global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(const Int4Attn a, int* status) {
+__global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(const Int4Attn a, int* status) {
   constexpr int WK = D / 32;       // words of a key that a lane multiplies with the queries
   constexpr int WV = D / 64;       // words of a value row of which a lane holds the dimensions
   extern __shared__ __align__(128) uint8_t raw[];
-  Int4Stage<D>* ring = reinterpret_cast<Int4Stage<D>*>(raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kI4Stages);
-  uint64_t* empty = full + kI4Stages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + kI4Stages);
-  float* s_m = reinterpret_cast<float*>(empty + kI4Stages + 2);      // [warps][heads]
+  const int slots = a.groups * kI4Warps;
+  const Int4Ring<D> ring(raw, slots);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring.v_meta + slots * (kI4Tile * D / 32));
+  uint64_t* empty = full + a.groups;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + a.groups);
+  float* s_m = reinterpret_cast<float*>(empty + a.groups + 2);                // [warps][heads]
   float* s_l = s_m + kI4Warps * a.heads;
-  float* s_o = s_l + kI4Warps * a.heads;                             // [warps][heads][D]
+  float* s_o = s_l + kI4Warps * a.heads;                                    // [warps][heads][D]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const WaitGuard guard{abort_flag, status};
   grid_dependency_launch();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kI4Stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kI4Warps); }
+    for (int i = 0; i < a.groups; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kI4Warps); }
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -199,39 +212,57 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(
   grid_dependency_wait();
 
   const int per_row = a.Hkv * a.blocks;
-  long long none;
-  const long long total = i4_sum_tiles(a, 0, none, lane) * per_row;
+  int row_tiles;
+  long long row_sum;
+  const long long total = Int4Cursor::count(a, row_tiles, row_sum, lane);
   const Int4Share share(a, total);
   const int cta = blockIdx.x;
-  if (cta >= share.ctas || total == 0) return;
-  const long long t0 = share.first(cta), t1 = share.first(cta + 1);
+  if (warp == 0) {                 // rows without tiles
+    for (int row = cta; row < a.rows; row += gridDim.x)
+      if (i4_row_tiles(a, row) == 0)
+        for (int i = lane; i < a.Hq * (D / 8); i += 32) reinterpret_cast<uint4*>(a.out)[(long long)row * a.Hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
+  }
+  if (cta >= share.ctas || total == 0) {
+    if (threadIdx.x == 0) a.shared[cta] = make_int2(0, 0);
+    return;
+  }
+  const long long t0 = share.first(cta);
+  const int run = (int)(share.first(cta + 1) - t0);                  // tiles of this CTA
   Int4Cursor piece;                // the item that the warp is at, by its first tile of this run
-  piece.seek(a, t0, lane);
-  int stage = 0;
-  uint32_t phase = 0;
+  piece.seek(a, t0, row_tiles, row_sum, lane);
 
   if (warp == kI4Warps) {
     // ---------------------------------------------------------------- the warp that fetches
-    int chunks = 0;
-    while (piece.at < t1) {
-      const int tiles = (int)min((long long)min(kI4Warps, piece.n - piece.tile), t1 - piece.at);
-      if (chunks >= kI4Stages && !__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty))) break;
-      if (elect_one()) i4_fetch<D>(a, piece, tiles, ring[stage], &full[stage]);
-      ++chunks;
-      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
-      piece.advance(a, tiles);
+    int done = 0, slot = 0, group = 0;
+    uint32_t phase = 1;            // a fresh barrier counts as one whose tiles have been given back
+    while (done < run) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[group], phase, guard, kTimeoutStageEmpty))) break;
+      const int end = min(run, done + kI4Warps);
+      while (done < end) {
+        const int tiles = min(end - done, piece.n - piece.tile);
+        if (elect_one()) i4_fetch<D>(a, piece, tiles, ring, slot, &full[group], done + tiles == end);
+        done += tiles;
+        slot += tiles;
+        piece.advance(a, tiles);
+      }
+      if (++group == a.groups) { group = slot = 0; phase ^= 1; }
     }
     // whatever the others have given up on: the last copies land before the block leaves
     const long long began = clock64();
-    for (int i = max(0, chunks - kI4Stages); i < chunks; ++i)
-      while (!mbar_try_wait(&full[i % kI4Stages], (i / kI4Stages) & 1) && clock64() - began < kWaitLimitCycles) {}
+    const int groups = (done + kI4Warps - 1) / kI4Warps;
+    for (int i = max(0, groups - a.groups); i < groups; ++i)
+      while (!mbar_try_wait(&full[i % a.groups], (i / a.groups) & 1) && clock64() - began < kWaitLimitCycles) {}
     return;
   }
 
   // ------------------------------------------------------------------ the warps that compute
   bool ok = true;
-  while (piece.at < t1) {
-    const int end = (int)min((long long)piece.n, piece.tile + (t1 - piece.at));        // tiles [piece.tile, end) of the item
+  // A warp has a tile in every group and so waits for each: barriers know two phases, and copies of later groups may land first.
+  int mine = warp, group = 0;      // this warp's tile, its group in the ring
+  uint32_t phase = 0;
+  int before = 0;                  // tiles of the run ahead of the item
+  while (before < run) {
+    const int here = min(run - before, piece.n - piece.tile);      // tiles of the item in the run
     const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
     const int heads = min(a.heads, (kvh + 1) * (a.Hq / a.Hkv) - h0);
     const int b = piece.row / a.Tq, tq = piece.row % a.Tq;
@@ -244,6 +275,7 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(
         qv[n][w] = make_uint4(0, 0, 0, 0);
         if (n * 8 + g < heads)
           qv[n][w] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + tq * a.q_st + (h0 + n * 8 + g) * a.q_sh + t * (D / 4) + w * 8);
+        qv[n][w].x ^= a.negate; qv[n][w].y ^= a.negate; qv[n][w].z ^= a.negate; qv[n][w].w ^= a.negate;
       }
     float o[WV * 4][NT][4], m[NT][2], l[NT][2];      // of queries 2 t and 2 t + 1 of each block
 #pragma unroll
@@ -257,130 +289,125 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(
 #pragma unroll
       for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
 
-    for (int chunk = piece.tile; chunk < end; chunk += kI4Warps) {
-      const int first = (piece.lo & ~(kI4Align - 1)) + (chunk + warp) * kI4Tile;
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
+    while (mine < before + here) {
+      const int slot = group * kI4Warps + warp;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[group], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
-      if (chunk + warp < end) {
-      const uint32_t *sk = ring[stage].k + warp * (kI4Tile * D / 8), *sv = ring[stage].v + warp * (kI4Tile * D / 8);
-      const uint32_t *skm = ring[stage].k_meta + warp * (kI4Tile * D / 32), *svm = ring[stage].v_meta + warp * (kI4Tile * D / 32);
-      const bool whole = first >= piece.lo && first + kI4Tile <= piece.hi;
-      // ---- scores^T = K q^T: row g + 8 j of a block of sixteen is slot 8 j + 4 (g & 1) + g / 2, which V's loads want
-      float p[NT][2][2][2];                        // [u: block of sixteen][j][query 2 t + e]
-      const int slot0 = (g & 1) * 4 + (g >> 1);
-      uint32_t words[2][2][WK], s2[2][2], o2[2][2];
-      float c[2][NT][4];
+      const int first = (piece.lo & ~(kI4Align - 1)) + (piece.tile + mine - before) * kI4Tile;
+      const uint32_t *sk = ring.k + slot * (kI4Tile * D / 8), *sv = ring.v + slot * (kI4Tile * D / 8);
+      const uint32_t *skm = ring.k_meta + slot * (kI4Tile * D / 32), *svm = ring.v_meta + slot * (kI4Tile * D / 32);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = u * 16 + j * 8 + slot0;
-          const uint32_t meta = skm[key * (D / 32) + t * WK / 4];
-          s2[u][j] = i4_scale2(meta);
-          o2[u][j] = i4_offset2(meta);
-          if (D == 128) *reinterpret_cast<uint4*>(words[u][j]) = *reinterpret_cast<const uint4*>(&sk[key * (D / 8) + t * WK]);
-          else *reinterpret_cast<uint2*>(words[u][j]) = *reinterpret_cast<const uint2*>(&sk[key * (D / 8) + t * WK]);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[u][n][e] = 0.f;
-      }
-#pragma unroll
-      for (int w = 0; w < WK; ++w)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {               // two chains of products side by side
-          uint32_t x[4], y[4];
-          i4_values(x, words[u][0][w], s2[u][0], o2[u][0]);
-          i4_values(y, words[u][1][w], s2[u][1], o2[u][1]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_bf16(c[u][n], x[0], y[0], x[1], y[1], qv[n][w].x, qv[n][w].y);
-            mma_bf16(c[u][n], x[2], y[2], x[3], y[3], qv[n][w].z, qv[n][w].w);
-          }
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) p[n][u][j][e] = c[u][n][j * 2 + e] * a.scale;
-      if (!whole) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < kI4Tile / 16; ++u) {
+        const int key0 = first + u * 16;                         // the block's first slot
+        if (key0 >= piece.hi || key0 + 16 <= piece.lo) continue;
+        const bool whole = key0 >= piece.lo && key0 + 16 <= piece.hi;
+        // ---- scores^T = K q^T: row g + 8 j is slot 8 j + 4 (g & 1) + (g / 2 ^ g & 1) of the block, for fewer conflicts of V's loads
+        const int slot0 = u * 16 + (g & 1) * 4 + ((g >> 1) ^ (g & 1));
+        float c[NT][4];                                          // [n][2 j + e]: key j of this lane, query 2 t + e
+        {
+          uint32_t words[2][WK], s2[2], o2[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int key = first + u * 16 + j * 8 + slot0;
-            if (key < piece.lo || key >= piece.hi) {
+            const int key = slot0 + j * 8;
+            const uint32_t meta = skm[key * (D / 32) + t * WK / 4];
+            s2[j] = i4_scale2(meta);
+            o2[j] = i4_offset2(meta);
+            if (D == 128) *reinterpret_cast<uint4*>(words[j]) = *reinterpret_cast<const uint4*>(&sk[key * (D / 8) + t * WK]);
+            else *reinterpret_cast<uint2*>(words[j]) = *reinterpret_cast<const uint2*>(&sk[key * (D / 8) + t * WK]);
+          }
 #pragma unroll
-              for (int n = 0; n < NT; ++n) p[n][u][j][0] = p[n][u][j][1] = -INFINITY;
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[n][e] = 0.f;
+#pragma unroll
+          for (int w = 0; w < WK; ++w) {
+            uint32_t x[4], y[4];
+            i4_values(x, words[0][w], s2[0], o2[0]);
+            i4_values(y, words[1][w], s2[1], o2[1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_bf16(c[n], x[0], y[0], x[1], y[1], qv[n][w].x, qv[n][w].y);
+              mma_bf16(c[n], x[2], y[2], x[3], y[3], qv[n][w].z, qv[n][w].w);
             }
           }
-      }
-      // ---- running maximum and sum of queries 2 t and 2 t + 1, the columns of this lane's outputs as well
-      float corr[NT][2];
-      bool moved = false;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(p[n][0][0][e], p[n][0][1][e]), fmaxf(p[n][1][0][e], p[n][1][1][e]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx, m[n][e]);
-          corr[n][e] = mx == m[n][e] ? 1.f : fast_exp2(m[n][e] - mx);
-          moved |= mx != m[n][e];
-          m[n][e] = mx;
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float& x = p[n][i >> 1][i & 1][e];
-            x = fast_exp2(x - mx);
-            sum += x;
-          }
-          l[n][e] = fmaf(l[n][e], corr[n][e], sum);
         }
-      if (__any_sync(0xffffffffu, moved)) {
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int key = first + slot0 + j * 8;
+            if (key < piece.lo || key >= piece.hi) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) c[n][2 * j] = c[n][2 * j + 1] = -INFINITY;
+            }
+          }
+        }
+        // ---- probabilities relative to m, which is the greatest score of some time ago: it moves when one is 16 powers of two above it (always
+        // in a warp's first block), so that most blocks need no maximum over their rows and no correction of the outputs
+        float x[NT][4], top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < WV * 4; ++i) {
-            o[i][n][0] *= corr[n][0]; o[i][n][1] *= corr[n][1]; o[i][n][2] *= corr[n][0]; o[i][n][3] *= corr[n][1];
-          }
-      }
-      // ---- out^T += V^T P^T: this lane's dimensions are D / 8 * g and on
+          for (int e = 0; e < 4; ++e) x[n][e] = fmaf(c[n][e], a.scale, -m[n][e & 1]);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int n = 0; n < NT; ++n) top = max3(max3(top, x[n][0], x[n][1]), x[n][2], x[n][3]);
+        if (__builtin_expect(__any_sync(0xffffffffu, top > 16.f), 0)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(c[n][e], c[n][2 + e]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              mx = fmaxf(mx * a.scale, m[n][e]);
+              const float corr = fast_exp2(m[n][e] - mx);
+              m[n][e] = mx;
+              l[n][e] *= corr;
+#pragma unroll
+              for (int i = 0; i < WV * 4; ++i) { o[i][n][e] *= corr; o[i][n][2 + e] *= corr; }
+              x[n][e] = fmaf(c[n][e], a.scale, -mx);
+              x[n][2 + e] = fmaf(c[n][2 + e], a.scale, -mx);
+            }
+        }
         uint32_t pb[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) pb[n][j] = transpose8(pack_bf16x2(p[n][u][j][0], p[n][u][j][1]));
+          for (int e = 0; e < 4; ++e) x[n][e] = fast_exp2(x[n][e]);
+          l[n][0] += x[n][0] + x[n][2];
+          l[n][1] += x[n][1] + x[n][3];
+          pb[n][0] = transpose8(pack_bf16x2(x[n][0], x[n][1]));
+          pb[n][1] = transpose8(pack_bf16x2(x[n][2], x[n][3]));
+        }
+        // ---- out^T += V^T P^T: this lane's dimensions are D / 8 * g and on
         uint32_t rows[4][WV], meta[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = u * 16 + i * 4 + t;
+          const int key = u * 16 + i * 4 + (t ^ (i & 1));
           if (D == 128) *reinterpret_cast<uint2*>(rows[i]) = *reinterpret_cast<const uint2*>(&sv[key * (D / 8) + g * WV]);
           else rows[i][0] = sv[key * (D / 8) + g];
           meta[i] = svm[key * (D / 32) + g * WV / 4];
-          if (!whole && (first + key < piece.lo || first + key >= piece.hi)) meta[i] = 0;
         }
-        uint32_t vs2[2], vo2[2];
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + i * 4 + (t ^ (i & 1));
+            if (key < piece.lo || key >= piece.hi) meta[i] = 0;
+          }
+        }
+        uint32_t s2[2], o2[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          vs2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x5410);
-          vo2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x7632);
+          s2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x5410);
+          o2[j] = __byte_perm(meta[2 * j], meta[2 * j + 1], 0x7632);
         }
 #pragma unroll
         for (int w = 0; w < WV; ++w) {
           uint32_t even[2][4], odd[2][4];      // [pair of keys][value of the word / 2]
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            i4_values(even[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x5410), vs2[j], vo2[j]);
-            i4_values(odd[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x7632), vs2[j], vo2[j]);
+            i4_values(even[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x5410), s2[j], o2[j]);
+            i4_values(odd[j], __byte_perm(rows[2 * j][w], rows[2 * j + 1][w], 0x7632), s2[j], o2[j]);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -388,10 +415,10 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(
             for (int n = 0; n < NT; ++n) mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], pb[n][0], pb[n][1]);
         }
       }
-      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
-      if (++stage == kI4Stages) { stage = 0; phase ^= 1; }
+      if (lane == 0) mbar_arrive(&empty[group]);
+      mine += kI4Warps;
+      if (++group == a.groups) { group = 0; phase ^= 1; }
     }
 
     // ---- the warps' parts of the item -> one
@@ -413,58 +440,59 @@ __global__ void __launch_bounds__(kI4Threads, NT == 1 ? 3 : 2) int4_attn_kernel(
       }
     }
     compute_sync();
-    const bool alone = piece.tile == 0 && end == piece.n;          // the whole item is here
+    const bool alone = here == piece.n;                              // the whole item is here
     const long long part = cta + (long long)piece.row * per_row + piece.head;
-    for (int i = threadIdx.x; i < heads * D; i += kI4Warps * 32) {
-      const int q = i / D, d = i % D;
+    for (int i = threadIdx.x; i < heads * (D / 4); i += kI4Warps * 32) {
+      const int q = i / (D / 4), d = i % (D / 4) * 4;
       float mx = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kI4Warps; ++w) mx = fmaxf(mx, s_m[w * a.heads + q]);
-      float sum = 0.f, acc = 0.f;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kI4Warps; ++w) {
-        const float mw = s_m[w * a.heads + q], f = mw == -INFINITY ? 0.f : fast_exp2(mw - mx);
+        const float mw = s_m[w * a.heads + q], f = mw == mx ? 1.f : fast_exp2(mw - mx);
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * a.heads + q) * D + d);
         sum = fmaf(s_l[w * a.heads + q], f, sum);
-        acc = fmaf(s_o[(w * a.heads + q) * D + d], f, acc);
+        acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
       }
       if (alone) {
-        a.out[((long long)piece.row * a.Hq + h0 + q) * D + d] = __float2bfloat16(__fdividef(acc, sum));
+        uint2 y;
+        y.x = pack_bf16x2(__fdividef(acc.x, sum), __fdividef(acc.y, sum));
+        y.y = pack_bf16x2(__fdividef(acc.z, sum), __fdividef(acc.w, sum));
+        *reinterpret_cast<uint2*>(a.out + ((long long)piece.row * a.Hq + h0 + q) * D + d) = y;
       } else {
-        a.part_o[(part * a.heads + q) * D + d] = acc;
+        *reinterpret_cast<float4*>(a.part_o + (part * a.heads + q) * D + d) = acc;
         if (d == 0) a.part_ml[part * a.heads + q] = make_float2(mx, sum);
       }
     }
     compute_sync();
-    piece.advance(a, end - piece.tile);
+    before += here;
+    if (before == run && threadIdx.x == 0) {
+      const bool goes_on = piece.tile == 0 && here < piece.n;
+      a.shared[cta] = make_int2((int)(part - cta), goes_on ? share.owner(t0 + run - here + piece.n - 1) - cta + 1 : 0);
+    }
+    piece.advance(a, here);
   }
 }
 
-// One query head of an item that several CTAs shared, or of an empty one.  The warps take the parts in turn, a lane D / 32 dimensions.
-constexpr int kI4MergeWarps = 4;
+// One query head of an item that begins in a CTA's run and goes on behind it.  The warps take its parts in turn, a lane D / 32 dimensions.
+constexpr int kI4MergeWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kI4MergeWarps * 32) int4_attn_merge_kernel(const Int4Attn a) {
   constexpr int V = D / 32;
   __shared__ float s_o[kI4MergeWarps][D], s_m[kI4MergeWarps], s_l[kI4MergeWarps];
   grid_dependency_launch();
   grid_dependency_wait();
-  const int per_row = a.Hkv * a.blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int item = blockIdx.x, q = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = blockIdx.y;
+  const int2 what = a.shared[blockIdx.x];
+  const int item = what.x, parts = what.y, per_row = a.Hkv * a.blocks;
+  if (parts == 0) return;
   const int row = item / per_row, head = item % per_row;
   const int group = a.Hq / a.Hkv, kvh = head / a.blocks, h0 = kvh * group + head % a.blocks * a.heads;
   if (h0 + q >= (kvh + 1) * group) return;
   bf16* out = a.out + ((long long)row * a.Hq + h0 + q) * D;
-  const int n = i4_row_tiles(a, row);
-  if (n == 0) {
-    if (threadIdx.x < D) out[threadIdx.x] = __float2bfloat16(0.f);
-    return;
-  }
-  long long before;
-  const long long total = i4_sum_tiles(a, row, before, lane) * per_row;
-  const Int4Share share(a, total);
-  const long long first = before * per_row + (long long)head * n;
-  const int c0 = share.owner(first), parts = share.owner(first + n - 1) - c0 + 1;
-  if (parts == 1) return;
-  const long long part0 = ((long long)c0 + item) * a.heads + q;          // in rows of part_o
+  const long long part0 = ((long long)blockIdx.x + item) * a.heads + q;          // in rows of part_o
   float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) o[i] = 0.f;
@@ -511,38 +539,39 @@ __global__ void __launch_bounds__(kI4MergeWarps * 32) int4_attn_merge_kernel(con
   }
 }
 
-template <int D>
-static size_t i4_smem(int heads) {
-  return sizeof(Int4Stage<D>) * kI4Stages + (2 * kI4Stages + 2) * 8 + sizeof(float) * kI4Warps * heads * (D + 2);
-}
-
+constexpr int kI4SmShared = 228 * 1024;      // of which every block costs 1024 besides its own
+constexpr int kI4MostGroups = 6;
 struct Int4Shape {
-  int heads, blocks;
+  int heads, blocks, groups;
   long long items;
   int ctas;
+  size_t smem;
 };
-constexpr int kI4SmShared = 227 * 1024;
 static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
   Int4Shape s;
   const int group = Hq / Hkv;
   s.heads = group < 16 ? group : 16;
   s.blocks = (group + 15) / 16;
   s.items = (long long)rows * Hkv * s.blocks;
-  const long long most = (s.items * ((cap + kI4Align + kI4Tile - 1) / kI4Tile) + kI4Warps - 1) / kI4Warps;
-  const int fit = kI4SmShared / ((int)(D == 128 ? i4_smem<128>(s.heads) : i4_smem<64>(s.heads)) + 1024), regs = s.heads <= 8 ? 3 : 2;
-  const long long room = (long long)sm_count() * (fit < regs ? fit : regs);          // all of them at once
+  const int per_group = kI4Warps * kI4Tile * (D + D / 4) + 16;
+  const int rest = 16 + kI4Warps * s.heads * (D + 2) * (int)sizeof(float);
+  const int per_sm = s.heads <= 8 ? i4_ctas<1>() : i4_ctas<2>();
+  s.groups = (kI4SmShared / per_sm - 1024 - rest) / per_group;
+  if (s.groups > kI4MostGroups) s.groups = kI4MostGroups;
+  s.smem = (size_t)s.groups * per_group + rest;
+  const long long most = (s.items * ((cap + kI4Align + kI4Tile - 1) / kI4Tile) + kI4Spread - 1) / kI4Spread, room = (long long)sm_count() * per_sm;
   s.ctas = (int)(most < 1 ? 1 : most < room ? most : room);
   return s;
 }
 
 template <int D, int NT>
-static int launch_int4_attn(const Int4Attn& a, long long items, cudaStream_t st) {
+static int launch_int4_attn(const Int4Attn& a, const Int4Shape& s, cudaStream_t st) {
   static PerDevice raised;
-  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT>, i4_smem<D>(NT * 8)));
+  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT>, kI4SmShared / i4_ctas<NT>() - 1024));
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Threads), i4_smem<D>(a.heads), st, a, status));
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3((unsigned)items, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Threads), s.smem, st, a, status));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3(a.ctas, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
   return 0;
 }
 
@@ -554,7 +583,7 @@ using namespace ksa;
 KSA_API long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap) {
   if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv != 0 || cap <= 0) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
-  return (s.ctas + s.items) * s.heads * (D + 2LL);
+  return (s.ctas + s.items) * s.heads * (D + 2LL) + 2LL * s.ctas;
 }
 
 // q [B, Tq, Hq, D] with strides in elements (rows of a head contiguous); cache as written by ksa_int4_cache_write; start, len [B, Tq] int32;
@@ -570,15 +599,17 @@ KSA_API int ksa_int4_decode_attn(const void* q, const void* k, const void* k_met
                 reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(v_meta)) & 15) == 0 && q_sb % 8 == 0 && q_st % 8 == 0 && q_sh % 8 == 0,
               "int4_decode_attn: queries and cache must be 16-byte aligned");
   KSA_REQUIRE(B >= 0 && Tq >= 0 && (long long)B * Tq < (1 << 28), "int4_decode_attn: bad shape");
+  KSA_REQUIRE(fabsf(scale) < INFINITY, "int4_decode_attn: the scale is not finite");
   if (B == 0 || Tq == 0) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
   KSA_REQUIRE(s.items < (1LL << 31) - s.ctas, "int4_decode_attn: too many queries");
   const long long parts = s.ctas + s.items;
   float* ws = (float*)workspace;
   Int4Attn a{(const bf16*)q, q_sb, q_st, q_sh, (const uint8_t*)k, (const uint8_t*)v, (const uint32_t*)k_meta, (const uint32_t*)v_meta,
-             (const int*)start, (const int*)len, ws, (float2*)(ws + parts * s.heads * D), (bf16*)out, B * Tq, Tq, Hq, Hkv, cap, s.heads, s.blocks,
-             s.ctas, scale * 1.4426950408889634f};
+             (const int*)start, (const int*)len, ws, (float2*)(ws + parts * s.heads * D),
+             (int2*)(ws + parts * s.heads * (D + 2LL)), (bf16*)out, B * Tq, Tq, Hq, Hkv, cap, s.heads, s.blocks,
+             s.ctas, s.groups, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (D == 128) return s.heads <= 8 ? launch_int4_attn<128, 1>(a, s.items, st) : launch_int4_attn<128, 2>(a, s.items, st);
-  return s.heads <= 8 ? launch_int4_attn<64, 1>(a, s.items, st) : launch_int4_attn<64, 2>(a, s.items, st);
+  if (D == 128) return s.heads <= 8 ? launch_int4_attn<128, 1>(a, s, st) : launch_int4_attn<128, 2>(a, s, st);
+  return s.heads <= 8 ? launch_int4_attn<64, 1>(a, s, st) : launch_int4_attn<64, 2>(a, s, st);
 }
