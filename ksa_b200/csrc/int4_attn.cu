@@ -28,6 +28,12 @@ constexpr int kI4Spread = 4;       // tiles that a CTA gets at least
 // CTAs of an SM (fifteen warps get 128 registers each, ten 168)
 template <int NT>
 constexpr int i4_ctas() { return NT == 1 ? 3 : 2; }
+// Short slices: the CTAs of an item are a cluster and merge through its shared memory, in one launch and with nothing to look up but the own row's
+// slice.  As long as all clusters are on the device at once, full caches took, in us, by the sequence and here (32 query heads, 8 key heads of
+// 128): one sequence of 256 slots 5.8 -> 4.0, 1168 8.6 -> 5.0, 4096 7.2 -> 7.1, 8192 11.1 -> 11.4, 16384 14.8 -> 19.7; six of 1168 10.9 -> 6.5, of
+// 4096 16.3 -> 12.3, of 16384 29.5 -> 31.7; eight of 4096, which do not fit, 17.9 -> 19.9, twelve of 1168 13.9 -> 13.0, 24 of 1168 17.7 -> 25.0.
+// Sixteen query heads a key head (32 over 2): one sequence of 4096 8.1 -> 8.8, two of 8192 15.5 -> 13.4, eight 20.4 -> 16.8, of 16384 24.8 -> 28.3.
+constexpr int kI4Cluster = 8, kI4ClusterSlots = 4096;
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
 
 struct Int4Attn {
@@ -61,41 +67,34 @@ __device__ __forceinline__ int i4_row_tiles(const Int4Attn& a, int row) {
   i4_slice(a, row, lo, hi);
   return i4_tiles(lo, hi);
 }
-// Quotients of sizes that fit 32 bits on all but gigantic calls.
-__device__ __forceinline__ long long i4_div(long long n, long long d) {
-  return ((n | d) >> 32) == 0 ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
-}
-// Rows' tiles, 32 rows at a time: this lane's row's, and the sum up to it.
-__device__ __forceinline__ long long i4_scan(int mine, int lane) {
-  long long sum = mine;
+// Rows' tiles, 32 rows at a time: the sum up to this lane's row.
+__device__ __forceinline__ int i4_scan(int mine, int lane) {
+  int sum = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, sum, d);
+    const int x = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += x;
   }
   return sum;
 }
 
-// How the sequence of `total` tiles is shared: CTAs that take part, and their runs, the first
-// `more` of which have one tile more than the others.
+// How the sequence of `total` tiles is shared: CTAs that take part, and their runs, the first `more` of which have one tile more than the others.
 struct Int4Share {
-  int ctas;
-  long long per, more;
-  __device__ __forceinline__ Int4Share(const Int4Attn& a, long long total) {
-    ctas = (int)max(1LL, min((long long)a.ctas, (total + kI4Spread - 1) / kI4Spread));
-    per = i4_div(total, ctas);
+  int ctas, per, more;
+  __device__ __forceinline__ Int4Share(const Int4Attn& a, int total) {
+    ctas = max(1, min(a.ctas, (total + kI4Spread - 1) / kI4Spread));
+    per = total / ctas;
     more = total - per * ctas;
   }
-  __device__ __forceinline__ long long first(int cta) const { return per * cta + min((long long)cta, more); }
-  __device__ __forceinline__ int owner(long long tile) const {
-    const long long wide = more * (per + 1);
-    return (int)(tile < wide ? i4_div(tile, per + 1) : more + i4_div(tile - wide, per));
+  __device__ __forceinline__ int first(int cta) const { return per * cta + min(cta, more); }
+  __device__ __forceinline__ int owner(int tile) const {
+    const int wide = more * (per + 1);
+    return tile < wide ? tile / (per + 1) : more + (tile - wide) / per;
   }
 };
 
 // A place in the sequence of tiles.
 struct Int4Cursor {
-  long long at;                    // index in the sequence
   int row, head, tile;             // row, item of the row (KV head and block of its query heads), tile of the item
   int lo, hi, n;                   // the row's slice and tiles
   long long base;                  // where the item's first tile starts in the cache, in slots
@@ -103,30 +102,31 @@ struct Int4Cursor {
     i4_slice(a, row, lo, hi);
     n = i4_tiles(lo, hi);
   }
+  __device__ __forceinline__ void enter(const Int4Attn& a) {
+    base = ((long long)(a.Tq == 1 ? row : row / a.Tq) * a.Hkv + (a.blocks == 1 ? head : head / a.blocks)) * a.cap + (lo & ~(kI4Align - 1));
+  }
   // The number of tiles, by a warp; `mine` and `sum` keep the last 32 rows' scan, which is all of it for up to 32 rows.
-  static __device__ __forceinline__ long long count(const Int4Attn& a, int& mine, long long& sum, int lane) {
-    long long rows = 0;
+  static __device__ __forceinline__ int count(const Int4Attn& a, int& mine, int& sum, int lane) {
+    const int per_row = a.Hkv * a.blocks;
+    if (a.rows == 1) return (sum = mine = i4_row_tiles(a, 0)) * per_row;
+    int rows = 0;
     for (int base = 0; base < a.rows; base += 32) {
       mine = i4_row_tiles(a, base + lane);
       sum = i4_scan(mine, lane);
       rows += __shfl_sync(0xffffffffu, sum, 31);
     }
-    return rows * (a.Hkv * a.blocks);
+    return rows * per_row;
   }
-  __device__ __forceinline__ void enter(const Int4Attn& a) {
-    base = ((long long)(row / a.Tq) * a.Hkv + head / a.blocks) * a.cap + (lo & ~(kI4Align - 1));
-  }
-  // tile `to`, which has to be there, by a warp
-  __device__ __forceinline__ void seek(const Int4Attn& a, long long to, int mine, long long sum, int lane) {
+  // tile `left` of the sequence, which has to be there, by a warp
+  __device__ __forceinline__ void seek(const Int4Attn& a, int left, int mine, int sum, int lane) {
     const int per_row = a.Hkv * a.blocks;
-    long long left = to;
-    at = to;
-    for (int base = 0; base < a.rows; base += 32) {
+    row = 0;
+    for (int base = 0; a.rows > 1 && base < a.rows; base += 32) {
       if (a.rows > 32) {
         mine = i4_row_tiles(a, base + lane);
         sum = i4_scan(mine, lane);
       }
-      const long long all = __shfl_sync(0xffffffffu, sum, 31) * per_row;
+      const int all = __shfl_sync(0xffffffffu, sum, 31) * per_row;
       if (left >= all) { left -= all; continue; }
       const int who = __ffs(__ballot_sync(0xffffffffu, left < sum * per_row)) - 1;
       left -= __shfl_sync(0xffffffffu, sum - mine, who) * per_row;
@@ -134,13 +134,12 @@ struct Int4Cursor {
       break;
     }
     load(a);
-    head = (int)i4_div(left, n);
-    tile = (int)(left - (long long)head * n);
+    head = left / n;
+    tile = left - head * n;
     enter(a);
   }
   // by `by` tiles, at most to the first of the next item
   __device__ __forceinline__ void advance(const Int4Attn& a, int by) {
-    at += by;
     tile += by;
     if (tile < n) return;
     tile = 0;
@@ -185,8 +184,31 @@ __device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c,
 }
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kI4Warps * 32) : "memory"); }
 
-// NT: query heads of an item in eights (1 or 2).
-template <int D, int NT>
+__device__ __forceinline__ float4 ld_cluster(const float4* local, uint32_t rank) {
+  float4 v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(local)), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster(const float2* local, uint32_t rank) {
+  float2 v;
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+               : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(local)), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void i4_store(bf16* out, const float4& o, float sum) {
+  const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);       // 0: a slice without slots
+  uint2 y;
+  y.x = pack_bf16x2(o.x * inv, o.y * inv);
+  y.y = pack_bf16x2(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(out) = y;
+}
+
+// NT: query heads of an item in eights (1 or 2).  kCluster: an item is shared by the kI4Cluster CTAs of a cluster, which merge through its shared memory.
+template <int D, int NT, bool kCluster>
 __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(const Int4Attn a, int* status) {
   constexpr int WK = D / 32;       // words of a key that a lane multiplies with the queries
   constexpr int WV = D / 64;       // words of a value row of which a lane holds the dimensions
@@ -199,6 +221,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
   float* s_m = reinterpret_cast<float*>(empty + a.groups + 2);                // [warps][heads]
   float* s_l = s_m + kI4Warps * a.heads;
   float* s_o = s_l + kI4Warps * a.heads;                                    // [warps][heads][D]
+  float2* s_ml = reinterpret_cast<float2*>(s_o + kI4Warps * a.heads * D);   // [heads], kCluster: the CTA's
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const WaitGuard guard{abort_flag, status};
@@ -211,25 +234,36 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
   __syncthreads();
   grid_dependency_wait();
 
-  const int per_row = a.Hkv * a.blocks;
-  int row_tiles;
-  long long row_sum;
-  const long long total = Int4Cursor::count(a, row_tiles, row_sum, lane);
-  const Int4Share share(a, total);
-  const int cta = blockIdx.x;
-  if (warp == 0) {                 // rows without tiles
-    for (int row = cta; row < a.rows; row += gridDim.x)
-      if (i4_row_tiles(a, row) == 0)
-        for (int i = lane; i < a.Hq * (D / 8); i += 32) reinterpret_cast<uint4*>(a.out)[(long long)row * a.Hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
+  const int per_row = a.Hkv * a.blocks, cta = blockIdx.x;
+  Int4Cursor piece;                // the item that the warp is at, by its first tile of this CTA's run
+  int t0, run;                     // the run: its first tile, its tiles
+  Int4Share share(a, 0);
+  if (kCluster) {
+    const int item = cta / kI4Cluster, rank = cta % kI4Cluster;
+    piece.row = item / per_row;
+    piece.head = item - piece.row * per_row;
+    piece.load(a);
+    piece.enter(a);
+    t0 = piece.tile = (int)((long long)piece.n * rank / kI4Cluster);
+    run = (int)((long long)piece.n * (rank + 1) / kI4Cluster) - t0;
+  } else {
+    int row_tiles, row_sum;
+    const int total = Int4Cursor::count(a, row_tiles, row_sum, lane);
+    share = Int4Share(a, total);
+    if (warp == 0) {               // rows without tiles
+      for (int row = cta; row < a.rows; row += gridDim.x)
+        if (i4_row_tiles(a, row) == 0)
+          for (int i = lane; i < a.Hq * (D / 8); i += 32)
+            reinterpret_cast<uint4*>(a.out)[(long long)row * a.Hq * (D / 8) + i] = make_uint4(0, 0, 0, 0);
+    }
+    if (cta >= share.ctas || total == 0) {
+      if (threadIdx.x == 0) a.shared[cta] = make_int2(0, 0);
+      return;
+    }
+    t0 = share.first(cta);
+    run = share.first(cta + 1) - t0;
+    piece.seek(a, t0, row_tiles, row_sum, lane);
   }
-  if (cta >= share.ctas || total == 0) {
-    if (threadIdx.x == 0) a.shared[cta] = make_int2(0, 0);
-    return;
-  }
-  const long long t0 = share.first(cta);
-  const int run = (int)(share.first(cta + 1) - t0);                  // tiles of this CTA
-  Int4Cursor piece;                // the item that the warp is at, by its first tile of this run
-  piece.seek(a, t0, row_tiles, row_sum, lane);
 
   if (warp == kI4Warps) {
     // ---------------------------------------------------------------- the warp that fetches
@@ -252,6 +286,11 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
     const int groups = (done + kI4Warps - 1) / kI4Warps;
     for (int i = max(0, groups - a.groups); i < groups; ++i)
       while (!mbar_try_wait(&full[i % a.groups], (i / a.groups) & 1) && clock64() - began < kWaitLimitCycles) {}
+    if (kCluster) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
     return;
   }
 
@@ -261,7 +300,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
   int mine = warp, group = 0;      // this warp's tile, its group in the ring
   uint32_t phase = 0;
   int before = 0;                  // tiles of the run ahead of the item
-  while (before < run) {
+  do {
     const int here = min(run - before, piece.n - piece.tile);      // tiles of the item in the run
     const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
     const int heads = min(a.heads, (kvh + 1) * (a.Hq / a.Hkv) - h0);
@@ -440,8 +479,9 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
       }
     }
     compute_sync();
-    const bool alone = here == piece.n;                              // the whole item is here
+    const bool alone = !kCluster && here == piece.n;                 // the whole item is here
     const long long part = cta + (long long)piece.row * per_row + piece.head;
+    bf16* out = a.out + ((long long)piece.row * a.Hq + h0) * D;
     for (int i = threadIdx.x; i < heads * (D / 4); i += kI4Warps * 32) {
       const int q = i / (D / 4), d = i % (D / 4) * 4;
       float mx = -INFINITY;
@@ -456,15 +496,43 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
         sum = fmaf(s_l[w * a.heads + q], f, sum);
         acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
       }
-      if (alone) {
-        uint2 y;
-        y.x = pack_bf16x2(__fdividef(acc.x, sum), __fdividef(acc.y, sum));
-        y.y = pack_bf16x2(__fdividef(acc.z, sum), __fdividef(acc.w, sum));
-        *reinterpret_cast<uint2*>(a.out + ((long long)piece.row * a.Hq + h0 + q) * D + d) = y;
+      if (kCluster) {              // in the place of the first warp's
+        *reinterpret_cast<float4*>(s_o + q * D + d) = acc;
+        if (d == 0) s_ml[q] = make_float2(mx, sum);
+      } else if (alone) {
+        i4_store(out + q * D + d, acc, sum);
       } else {
         *reinterpret_cast<float4*>(a.part_o + (part * a.heads + q) * D + d) = acc;
         if (d == 0) a.part_ml[part * a.heads + q] = make_float2(mx, sum);
       }
+    }
+    if (kCluster) {
+      cluster_sync();
+      // every CTA finishes its share of the outputs
+      const int n = heads * (D / 4), share_n = (n + kI4Cluster - 1) / kI4Cluster, rank = cta % kI4Cluster;
+      for (int i = rank * share_n + (int)threadIdx.x; i < min((rank + 1) * share_n, n); i += kI4Warps * 32) {
+        const int q = i / (D / 4), d = i % (D / 4) * 4;
+        float2 ml[kI4Cluster];
+        float4 x[kI4Cluster];
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < kI4Cluster; ++r) {
+          ml[r] = ld_cluster(s_ml + q, r);
+          x[r] = ld_cluster(reinterpret_cast<const float4*>(s_o + q * D + d), r);
+        }
+#pragma unroll
+        for (int r = 0; r < kI4Cluster; ++r) mx = fmaxf(mx, ml[r].x);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < kI4Cluster; ++r) {
+          const float f = ml[r].x == mx ? 1.f : fast_exp2(ml[r].x - mx);
+          sum = fmaf(ml[r].y, f, sum);
+          acc.x = fmaf(x[r].x, f, acc.x); acc.y = fmaf(x[r].y, f, acc.y); acc.z = fmaf(x[r].z, f, acc.z); acc.w = fmaf(x[r].w, f, acc.w);
+        }
+        i4_store(out + q * D + d, acc, sum);
+      }
+      cluster_sync();              // nobody leaves while its part may still be read
+      return;
     }
     compute_sync();
     before += here;
@@ -473,7 +541,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
       a.shared[cta] = make_int2((int)(part - cta), goes_on ? share.owner(t0 + run - here + piece.n - 1) - cta + 1 : 0);
     }
     piece.advance(a, here);
-  }
+  } while (before < run);
 }
 
 // One query head of an item that begins in a CTA's run and goes on behind it.  The warps take its parts in turn, a lane D / 32 dimensions.
@@ -542,8 +610,8 @@ __global__ void __launch_bounds__(kI4MergeWarps * 32) int4_attn_merge_kernel(con
 constexpr int kI4SmShared = 228 * 1024;      // of which every block costs 1024 besides its own
 constexpr int kI4MostGroups = 6;
 struct Int4Shape {
-  int heads, blocks, groups;
-  long long items;
+  int heads, blocks, groups, cluster;
+  long long items, tiles;          // tiles: at most
   int ctas;
   size_t smem;
 };
@@ -554,23 +622,46 @@ static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
   s.blocks = (group + 15) / 16;
   s.items = (long long)rows * Hkv * s.blocks;
   const int per_group = kI4Warps * kI4Tile * (D + D / 4) + 16;
-  const int rest = 16 + kI4Warps * s.heads * (D + 2) * (int)sizeof(float);
+  const int rest = 16 + (kI4Warps * (D + 2) + 2) * s.heads * (int)sizeof(float);
   const int per_sm = s.heads <= 8 ? i4_ctas<1>() : i4_ctas<2>();
   s.groups = (kI4SmShared / per_sm - 1024 - rest) / per_group;
   if (s.groups > kI4MostGroups) s.groups = kI4MostGroups;
   s.smem = (size_t)s.groups * per_group + rest;
-  const long long most = (s.items * ((cap + kI4Align + kI4Tile - 1) / kI4Tile) + kI4Spread - 1) / kI4Spread, room = (long long)sm_count() * per_sm;
+  s.tiles = s.items * (((long long)cap + kI4Align + kI4Tile - 1) / kI4Tile);
+  const long long most = (s.tiles + kI4Spread - 1) / kI4Spread, room = (long long)sm_count() * per_sm;
   s.ctas = (int)(most < 1 ? 1 : most < room ? most : room);
+  s.cluster = s.items * kI4Cluster <= room && cap <= (s.heads <= 8 ? kI4ClusterSlots : 2 * kI4ClusterSlots);
   return s;
 }
 
 template <int D, int NT>
 static int launch_int4_attn(const Int4Attn& a, const Int4Shape& s, cudaStream_t st) {
-  static PerDevice raised;
-  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT>, kI4SmShared / i4_ctas<NT>() - 1024));
+  constexpr int most = kI4SmShared / i4_ctas<NT>() - 1024;
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT>, dim3(a.ctas), dim3(kI4Threads), s.smem, st, a, status));
+  if (s.cluster) {
+    static PerDevice raised;
+    KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, true>, most));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(s.items * kI4Cluster));
+    cfg.blockDim = dim3(kI4Threads);
+    cfg.dynamicSmemBytes = s.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = kI4Cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = dependent_launches() ? 2 : 1;
+    KSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, int4_attn_kernel<D, NT, true>, a, status));
+    return 0;
+  }
+  static PerDevice raised;
+  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, false>, most));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT, false>, dim3(a.ctas), dim3(kI4Threads), s.smem, st, a, status));
   KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3(a.ctas, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
   return 0;
 }
@@ -581,7 +672,7 @@ using namespace ksa;
 
 // Floats of the workspace of ksa_int4_decode_attn on the current device.
 KSA_API long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap) {
-  if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv != 0 || cap <= 0) return 0;
+  if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv != 0 || cap <= 0 || (long long)B * Tq >= (1 << 28)) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
   return (s.ctas + s.items) * s.heads * (D + 2LL) + 2LL * s.ctas;
 }
@@ -602,7 +693,7 @@ KSA_API int ksa_int4_decode_attn(const void* q, const void* k, const void* k_met
   KSA_REQUIRE(fabsf(scale) < INFINITY, "int4_decode_attn: the scale is not finite");
   if (B == 0 || Tq == 0) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
-  KSA_REQUIRE(s.items < (1LL << 31) - s.ctas, "int4_decode_attn: too many queries");
+  KSA_REQUIRE(s.tiles < (1LL << 31) - s.ctas, "int4_decode_attn: too many queries and slots");
   const long long parts = s.ctas + s.items;
   float* ws = (float*)workspace;
   Int4Attn a{(const bf16*)q, q_sb, q_st, q_sh, (const uint8_t*)k, (const uint8_t*)v, (const uint32_t*)k_meta, (const uint32_t*)v_meta,
