@@ -29,9 +29,10 @@ constexpr int kI4Spread = 4;       // tiles that a CTA gets at least
 template <int NT>
 constexpr int i4_ctas() { return NT == 1 ? 3 : 2; }
 // Short slices: the CTAs of an item are a cluster and merge through its shared memory, in one launch and with nothing to look up but the own row's
-// slice.  As long as all clusters are on the device at once, full caches took, in us, by the sequence and here (32 query heads, 8 key heads of
+// slice.  Full caches took, in us, by the sequence and here (32 query heads, 8 key heads of
 // 128): one sequence of 256 slots 5.8 -> 4.0, 1168 8.6 -> 5.0, 4096 7.2 -> 7.1, 8192 11.1 -> 11.4, 16384 14.8 -> 19.7; six of 1168 10.9 -> 6.5, of
-// 4096 16.3 -> 12.3, of 16384 29.5 -> 31.7; eight of 4096, which do not fit, 17.9 -> 19.9, twelve of 1168 13.9 -> 13.0, 24 of 1168 17.7 -> 25.0.
+// 4096 16.3 -> 12.3, of 16384 29.5 -> 31.7; in two rounds of clusters twelve of 1168 13.9 -> 13.0, of 2048 16.6 -> 16.3, of 4096 21.0 -> 22.7; in
+// four 24 of 1168 17.7 -> 25.0.
 // Sixteen query heads a key head (32 over 2): one sequence of 4096 8.1 -> 8.8, two of 8192 15.5 -> 13.4, eight 20.4 -> 16.8, of 16384 24.8 -> 28.3.
 constexpr int kI4Cluster = 8, kI4ClusterSlots = 4096;
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
@@ -630,7 +631,8 @@ static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
   s.tiles = s.items * (((long long)cap + kI4Align + kI4Tile - 1) / kI4Tile);
   const long long most = (s.tiles + kI4Spread - 1) / kI4Spread, room = (long long)sm_count() * per_sm;
   s.ctas = (int)(most < 1 ? 1 : most < room ? most : room);
-  s.cluster = s.items * kI4Cluster <= room && cap <= (s.heads <= 8 ? kI4ClusterSlots : 2 * kI4ClusterSlots);
+  const long long rounds = (s.items * kI4Cluster + room - 1) / room;
+  s.cluster = rounds <= 2 && cap <= (s.heads <= 8 ? kI4ClusterSlots : 2 * kI4ClusterSlots) / rounds;
   return s;
 }
 

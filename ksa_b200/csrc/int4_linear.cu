@@ -1,134 +1,315 @@
-// Products of a few rows with weights of four bits: C[M, N] = A[M, K] * W[N, K]^T, M <= 16, W as int4.cuh says.
+// Products of a few rows with weights of four bits: C[M, N] = A[M, K] * W[N, K]^T, M <= 16, W as int4.cuh says; with kGlu W holds gate rows and then up
+// rows, and C[M, N / 2] = silu(gate) * up.
 //
-// What bounds it is reading the codes and scales once (N * K * (1/2 + 4 / group) bytes).  One CTA per SM owns the same number of weight rows
-// (+-1); its warps share K in segments of 128 and keep their sums to themselves until the end of up to 64 rows, where they meet in shared memory.
-// mma.sync m16n8k16 takes the activations as its 16 rows (weights in eights, so that a CTA's share of rows need not be a multiple of 16); a
-// lane's 16 bytes of a weight row are values 32 t .. 32 t + 31 of the segment, in that order for the activations as well.
+// What bounds it is reading the codes and scales once, N * K * (1/2 + 4 / group) bytes; next to that the issue slots: a lane's eight codes cost
+// twelve operations and two mma.sync.  Hence:
+//   * one CTA per SM, and each owns the same number of weight rows (+-1) whatever N is; it takes them in passes of up to 128, and a pass in
+//     rounds of some segments of 128 columns.  A warp fetches rounds into a ring, one box of codes and one of scales each (a box of a single segment, 4 KB,
+//     cost its 0.5 us whatever its size), as far ahead as the ring reaches, in the engine's decode step ahead of the previous kernel's end;
+//   * sixteen warps multiply: a round has 16 / kParts segments, and kParts warps share the rows of a segment.  They keep their sums of a pass and
+//     leave them in shared memory; two more warps add the sums up and write the results while the others are at the next pass;
+//   * mma.sync m16n8k16 takes the activations as its 16 rows and weights in eights, so that a CTA's share of rows need not be a multiple of 16; a
+//     lane's 16 bytes of a weight row are columns 32 t .. 32 t + 31 of the segment, in that order for the activations as well.  Activations that several passes
+//     want stay in shared memory, others are read as they are needed.
 #include "host.h"
 #include "int4.cuh"
 
 namespace ksa {
 
-constexpr int kI4LWarps = 16;
-constexpr int kI4LThreads = kI4LWarps * 32;
-constexpr int kI4LOctets = 6;      // eights of weight rows of a pass
+constexpr int kI4LWarps = 16;                       // that multiply
+constexpr int kI4LAdders = 2;                       // that add up and write
+constexpr int kI4LThreads = (kI4LWarps + kI4LAdders + 1) * 32;
+constexpr int kI4LOctets = 4;                       // eights of weight rows of a warp
+constexpr int kI4LMostStages = 12;
+constexpr int kI4LSmemMost = 227 * 1024;
 
 struct Int4Linear {
   const bf16* A;
-  const uint8_t* W;                // [N, K / 2]
   const uint32_t* meta;            // [K / group, pitch]
   bf16* C;
   long long lda, ldc;
-  int M, N, K, group, pitch, rows; // rows of a CTA
-  int early;                       // the weights are read ahead of the wait
+  int M, N, K, group, pitch;       // N: rows of the weight
+  int n_out, per_cta, per_pass;    // output columns: of all, of a CTA, of a pass
+  int segments, stages, stage_bytes;
+  int meta_words, meta_at;         // words of a group's scales in a stage, and where they begin
+  int x_pitch;                     // bytes of an activation row in shared memory, 0: none are kept
+  int ragged;                      // the last segment is not whole: a box for each
+  int early;                       // weights are read ahead of the wait
 };
 
-// NB: activation rows in eights (1 or 2)
-template <int NB>
-__global__ void __launch_bounds__(kI4LThreads) int4_linear_kernel(const Int4Linear a) {
-  extern __shared__ float part[];                    // [warps][NB * 8][octets * 8 + 4]
-  constexpr int kPitch = kI4LOctets * 8 + 4;
+// NB: activation rows in eights.  kParts: warps that share a segment's rows, up to 32 each (kGlu: the first half of them gate rows, the other their up rows).
+template <int NB, int kParts, bool kGlu>
+__global__ void __launch_bounds__(kI4LThreads, 1)
+int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_meta, const Int4Linear a, int* status) {
+  static_assert(!kGlu || kParts >= 2, "parts for gate and up rows");
+  constexpr int kTurns = kI4LWarps / kParts;                                // segments of a round
+  constexpr int kRows = kI4LOctets * 8 * kParts, kPitch = kRows + 8;        // rows of a pass; floats of a row of sums
+  constexpr int kSets = kGlu ? 2 : 1, kPerSet = kParts / kSets;             // boxes of a round, warps for the rows of one
+  extern __shared__ __align__(128) uint8_t raw[];
+  uint8_t* ring = raw;
+  float* part = reinterpret_cast<float*>(ring + a.stages * a.stage_bytes);  // [turns][NB * 8][kPitch]
+  uint8_t* xs = reinterpret_cast<uint8_t*>(part + kTurns * NB * 8 * kPitch);
+  uint64_t* full = reinterpret_cast<uint64_t*>(xs + a.M * a.x_pitch);
+  uint64_t* empty = full + a.stages;
+  uint64_t* left = empty + a.stages;                                         // the sums of a pass are there
+  uint64_t* added = left + 1;                                                // and have been read
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(added + 1);
+
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int r0 = blockIdx.x * a.rows, r1 = min(a.N, r0 + a.rows);
-  const int segments = (a.K + 127) / 128;
+  const WaitGuard guard{abort_flag, status};
+  const int r0 = (int)blockIdx.x * a.per_cta, mine = min(a.per_cta, a.n_out - r0);
+  const int passes = (mine + a.per_pass - 1) / a.per_pass, rounds = (a.segments + kTurns - 1) / kTurns;
+  const int groups = 128 / a.group;                                          // of a segment
+  const int set_bytes = (kTurns * a.per_pass * 64 + 127) / 128 * 128, meta_bytes = (kTurns * groups * a.meta_words * 4 + 127) / 128 * 128;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], kI4LWarps); }
+    mbar_init(left, kI4LWarps);
+    mbar_init(added, kI4LAdders);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tm);
+    tma_prefetch_desc(&tm_meta);
+  }
+  __syncthreads();
   grid_dependency_launch();
-  if (!a.early) grid_dependency_wait();
-  bool waited = !a.early;
-  for (int base = r0; base < r1; base += kI4LOctets * 8) {
-    const int octets = min(kI4LOctets, (r1 - base + 7) / 8);
+
+  if (warp == kI4LWarps + kI4LAdders) {
+    // ---------------------------------------------------------------- the warp that fetches
+    if (!a.early) grid_dependency_wait();
+    const int total = passes * rounds;
+    const uint32_t bytes = kSets * kTurns * (a.per_pass * 64 + groups * a.meta_words * 4);       // also past the matrix's edges
+    int stage = 0, round = 0, row = r0, done = 0;
+    uint32_t phase = 1;
+    for (; done < total; ++done) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase, guard, kTimeoutStageEmpty))) break;
+      uint8_t* dst = ring + stage * a.stage_bytes;
+      if (elect_one()) {
+        mbar_expect_tx(&full[stage], bytes);
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          const int from = s * a.n_out + row;
+          if (!a.ragged) tma_load_3d(dst + s * set_bytes, &tm, 0, from, round * kTurns, &full[stage]);
+          tma_load_2d(dst + a.meta_at + s * meta_bytes, &tm_meta, from & ~3, round * kTurns * groups, &full[stage]);
+        }
+      }
+      __syncwarp();
+      if (a.ragged && lane < kTurns) {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+          tma_load_2d(dst + s * set_bytes + lane * a.per_pass * 64, &tm, (round * kTurns + lane) * 32, s * a.n_out + row, &full[stage]);
+      }
+      __syncwarp();
+      if (++stage == a.stages) { stage = 0; phase ^= 1; }
+      if (++round == rounds) { round = 0; row += a.per_pass; }
+    }
+    if (a.early) grid_dependency_wait();
+    // whatever the others have given up on: the last copies land before the block leaves
+    const long long began = clock64();
+    for (int i = max(0, done - a.stages); i < done; ++i)
+      while (!mbar_try_wait(&full[i % a.stages], (i / a.stages) & 1) && clock64() - began < kWaitLimitCycles) {}
+    return;
+  }
+  grid_dependency_wait();
+
+  if (warp >= kI4LWarps) {
+    // ---------------------------------------------------------------- the warps that add up: four columns of a row at a time
+    const int me = (warp - kI4LWarps) * 32 + lane;
+    for (int p = 0; p < passes; ++p) {
+      const int row = r0 + p * a.per_pass, rows = min(a.per_pass, r0 + mine - row), quads = (rows + 3) / 4;
+      if (!__all_sync(0xffffffffu, mbar_wait(left, p & 1, guard, kTimeoutAccFull))) break;
+      for (int i = me; i < a.M * quads; i += kI4LAdders * 32) {
+        const int m = i / quads, c = (i - m * quads) * 4;
+        float v[kSets][4];
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[s][e] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kTurns; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(part + (w * NB * 8 + m) * kPitch + s * (kRows / 2) + c);
+            v[s][0] += x.x; v[s][1] += x.y; v[s][2] += x.z; v[s][3] += x.w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = v[0][e];
+          if (kGlu) {
+            // gate and up are rounded to bf16 first, as the separate projection and activation do
+            const float gt = __bfloat162float(__float2bfloat16(y)), up = __bfloat162float(__float2bfloat16(v[kSets - 1][e]));
+            y = gt / (1.f + __expf(-gt)) * up;
+          }
+          if (c + e < rows) a.C[m * a.ldc + row + c + e] = __float2bfloat16(y);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(added);
+    }
+    return;
+  }
+
+  // ------------------------------------------------------------------ the warps that multiply
+  if (a.x_pitch > 0) {
+    // an activation's 16 bytes w of the 64 that lane t wants of a segment lie at 4 w + t: four lanes read 64 bytes in a row
+    const int per = a.segments * 16;
+    for (int i = threadIdx.x; i < a.M * per; i += kI4LWarps * 32) {
+      const int m = i / per, c = i - m * per;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (c * 8 < a.K) v = *reinterpret_cast<const uint4*>(a.A + m * a.lda + c * 8);
+      *reinterpret_cast<uint4*>(xs + m * a.x_pitch + (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16) = v;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kI4LWarps * 32) : "memory");
+  }
+  const int turn = warp / kParts, set = kGlu ? warp % kParts / kPerSet : 0, which = warp % kParts % kPerSet;
+  bool ok = true;
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int p = 0; p < passes; ++p) {
+    const int row = r0 + p * a.per_pass, octets = (min(a.per_pass, r0 + mine - row) + 7) / 8;
+    // this warp's eights of the rows, and the first of them
+    const int each = (octets + kPerSet - 1) / kPerSet, at = which * each * 8, count = max(0, min(each, octets - which * each));
+    const int skip = (set * a.n_out + row) & 3;
     float acc[kI4LOctets][4];
 #pragma unroll
     for (int i = 0; i < kI4LOctets; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-    for (int seg = warp; seg < segments; seg += kI4LWarps) {
-      const int col = seg * 128 + t * 32;
-      const bool in = col < a.K;
-      uint4 w[kI4LOctets];
-      uint32_t m[kI4LOctets];
-#pragma unroll
-      for (int i = 0; i < kI4LOctets; ++i) {
-        w[i] = make_uint4(0, 0, 0, 0);
-        m[i] = 0;
-        const int row = base + i * 8 + g;
-        if (i < octets && row < r1 && in) {
-          w[i] = *reinterpret_cast<const uint4*>(a.W + (long long)row * (a.K / 2) + col / 2);
-          m[i] = a.meta[(long long)(col / a.group) * a.pitch + row];
-        }
-      }
-      if (!waited) { grid_dependency_wait(); waited = true; }
+    for (int round = 0; round < rounds; ++round) {
+      const int seg = round * kTurns + turn, col = seg * 128 + t * 32;
       uint4 x[NB][4];
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           x[n][q] = make_uint4(0, 0, 0, 0);
-          if (n * 8 + g < a.M && in) x[n][q] = *reinterpret_cast<const uint4*>(a.A + (n * 8 + g) * a.lda + col + q * 8);
+          if (n * 8 + g < a.M && col < a.K) {
+            if (a.x_pitch > 0) x[n][q] = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * a.x_pitch + seg * 256 + (q * 4 + t) * 16);
+            else x[n][q] = *reinterpret_cast<const uint4*>(a.A + (n * 8 + g) * a.lda + col + q * 8);
+          }
         }
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
+      if (!ok) break;
+      if (seg < a.segments) {                                                // what lies past K in the last one is zeros, scales and all
+        const uint8_t* src = ring + stage * a.stage_bytes;
+        const uint8_t* codes = src + set * set_bytes + (turn * a.per_pass + at + g) * 64 + t * 16;
+        const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + a.meta_at + set * meta_bytes) +
+                               (turn * groups + t * 32 / a.group) * a.meta_words + skip + at + g;
 #pragma unroll
-      for (int i = 0; i < kI4LOctets; ++i) {
-        if (i >= octets) break;
-        const uint32_t s2 = i4_scale2(m[i]), o2 = i4_offset2(m[i]);
-        const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        for (int i = 0; i < kI4LOctets; ++i) {
+          if (i >= count) break;
+          const uint4 w = *reinterpret_cast<const uint4*>(codes + i * 512);
+          const uint32_t m = meta[i * 8], s2 = i4_scale2(m), o2 = i4_offset2(m), words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t v[4];
-          i4_values(v, words[q], s2, o2);
-          const uint4 xa = x[0][q], xb = NB == 2 ? x[NB - 1][q] : make_uint4(0, 0, 0, 0);
-          mma_bf16(acc[i], xa.x, xb.x, xa.y, xb.y, v[0], v[1]);
-          mma_bf16(acc[i], xa.z, xb.z, xa.w, xb.w, v[2], v[3]);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[4];
+            i4_values(v, words[q], s2, o2);
+            const uint4 xa = x[0][q], xb = NB == 2 ? x[NB - 1][q] : make_uint4(0, 0, 0, 0);
+            mma_bf16(acc[i], xa.x, xb.x, xa.y, xb.y, v[0], v[1]);
+            mma_bf16(acc[i], xa.z, xb.z, xa.w, xb.w, v[2], v[3]);
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[stage]);
+      if (++stage == a.stages) { stage = 0; phase ^= 1; }
     }
-    if (!waited) { grid_dependency_wait(); waited = true; }
-    // ---- the warps' sums: acc[i] = (row g, weights 2 t, 2 t + 1), (row g + 8, the same)
+    // ---- this warp's sums: acc[i] = (row g, weights 2 t and 2 t + 1), (row g + 8, the same)
+    if (p > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(added, (p - 1) & 1, guard, kTimeoutAccEmpty));
+    if (!ok) break;
 #pragma unroll
     for (int i = 0; i < kI4LOctets; ++i) {
-      if (i >= octets) break;
-      float* dst = part + (warp * NB * 8 + g) * kPitch + i * 8 + t * 2;
-      *reinterpret_cast<float2*>(dst) = make_float2(acc[i][0], acc[i][1]);
-      if (NB == 2) *reinterpret_cast<float2*>(dst + 8 * kPitch) = make_float2(acc[i][2], acc[i][3]);
+      if (i >= count) break;
+      float* dst = part + (turn * NB * 8 + g) * kPitch + set * (kRows / 2) + at + i * 8 + t * 2;
+      if (g < a.M) *reinterpret_cast<float2*>(dst) = make_float2(acc[i][0], acc[i][1]);
+      if (NB == 2 && g + 8 < a.M) *reinterpret_cast<float2*>(dst + 8 * kPitch) = make_float2(acc[i][2], acc[i][3]);
     }
-    __syncthreads();
-    const int n = min(kI4LOctets * 8, r1 - base);
-    for (int i = threadIdx.x; i < a.M * n; i += kI4LThreads) {
-      const int row = i / n, c = i - row * n;
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kI4LWarps; ++w) s += part[(w * NB * 8 + row) * kPitch + c];
-      a.C[row * a.ldc + base + c] = __float2bfloat16(s);
-    }
-    __syncthreads();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(left);
   }
+}
+
+// How a CTA of `per_cta` output columns takes them with `parts` warps to a segment: rows of a pass, and the eights of rows that a warp multiplies in all,
+// with what a round costs besides (two of them) and a pass (four).
+static int i4l_cost(int per_cta, int segments, int parts, int sets, int* per_pass) {
+  const int most = kI4LOctets * 8 * parts / sets, passes = (per_cta + most - 1) / most, turns = kI4LWarps / parts;
+  *per_pass = (per_cta + passes - 1) / passes;
+  const int octets = (*per_pass + 7) / 8, each = (octets * sets + parts - 1) / parts;
+  return passes * ((segments + turns - 1) / turns * (each + 2) + 4);
+}
+
+template <int NB, int kParts, bool kGlu>
+static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) {
+  constexpr int kTurns = kI4LWarps / kParts, kRows = kI4LOctets * 8 * kParts, kPitch = kRows + 8, kSets = kGlu ? 2 : 1;
+  int* status = status_word();
+  KSA_REQUIRE(status != nullptr, "int4_linear: no status word");
+  const int groups = 128 / a.group;
+  a.meta_words = (a.per_pass + 3 + 3) / 4 * 4;
+  a.meta_at = kSets * ((kTurns * a.per_pass * 64 + 127) / 128 * 128) + 512;       // the last eight may reach past the rows
+  a.stage_bytes = a.meta_at + kSets * ((kTurns * groups * a.meta_words * 4 + 127) / 128 * 128) + 128;
+  const int part = kTurns * NB * 8 * kPitch * 4, per_stage = a.stage_bytes + 16, rest = part + 32;
+  // activations that several passes want stay, where a ring of 64 KB and three rounds finds room beside them
+  const int passes = (a.per_cta + a.per_pass - 1) / a.per_pass, x_pitch = a.segments * 256 + 64;
+  const int least = 3 * per_stage > 64 * 1024 ? 3 * per_stage : 64 * 1024;
+  a.x_pitch = passes > 1 && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
+  a.stages = (kI4LSmemMost - rest - a.M * a.x_pitch) / per_stage;
+  const int wanted = passes * ((a.segments + kTurns - 1) / kTurns);
+  if (a.stages > wanted) a.stages = wanted;
+  if (a.stages > kI4LMostStages) a.stages = kI4LMostStages;
+  KSA_REQUIRE(a.stages >= 1, "int4_linear: no room for a round");
+  const size_t smem = (size_t)a.stages * per_stage + rest + a.M * a.x_pitch;
+  CUtensorMap tm, tm_meta;
+  {
+    uint64_t dims[3] = {(uint64_t)(a.ragged ? a.K / 4 : 32), (uint64_t)a.N, (uint64_t)a.segments}, str[3] = {2, (uint64_t)a.K / 2, 64};
+    uint32_t box[3] = {32, (uint32_t)a.per_pass, (uint32_t)kTurns};
+    if (const int rc = make_tmap(&tm, codes, 2, a.ragged ? 2 : 3, dims, str, box, false)) return rc;
+  }
+  {
+    uint64_t dims[2] = {(uint64_t)a.pitch, (uint64_t)(a.K / a.group)}, str[2] = {4, (uint64_t)a.pitch * 4};
+    uint32_t box[2] = {(uint32_t)a.meta_words, (uint32_t)(kTurns * groups)};
+    if (const int rc = make_tmap(&tm_meta, a.meta, 4, 2, dims, str, box, false)) return rc;
+  }
+  auto kern = int4_linear_kernel<NB, kParts, kGlu>;
+  static PerDevice raised;
+  KSA_CHECK_CUDA(raise_smem_limit(raised, kern, kI4LSmemMost));
+  KSA_CHECK_CUDA(launch_kernel(kern, dim3((a.n_out + a.per_cta - 1) / a.per_cta), dim3(kI4LThreads), smem, st, tm, tm_meta, a, status));
+  return 0;
 }
 
 }  // namespace ksa
 
 using namespace ksa;
 
-// A [M <= 16, K] (row pitch lda), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc).
+// A [M <= 16, K] (row pitch lda), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc); glu: gate rows and then up rows, C [M, N / 2].
 KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
-                            long long ldc, void* stream) {
+                            long long ldc, int glu, void* stream) {
   KSA_ENTER(A);
   KSA_REQUIRE(M >= 0 && M <= 16, "int4_linear: %d rows (at most 16)", M);
   KSA_REQUIRE(group == 32 || group == 64 || group == 128, "int4_linear: groups of %d values (32, 64 or 128)", group);
-  KSA_REQUIRE(K > 0 && K % group == 0 && N >= 0 && pitch >= N, "int4_linear: K %d is no multiple of the group of %d", K, group);
-  KSA_REQUIRE(lda % 8 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(codes)) & 15) == 0 &&
-                  (reinterpret_cast<uintptr_t>(meta) & 3) == 0, "int4_linear: rows and codes must be 16-byte aligned");
+  KSA_REQUIRE(K > 0 && K % group == 0 && N >= 0 && pitch >= N && pitch % 4 == 0, "int4_linear: K %d is no multiple of the group of %d", K, group);
+  KSA_REQUIRE(!glu || N % 2 == 0, "int4_linear: gate and up rows must be as many, got %d together", N);
+  KSA_REQUIRE(lda % 8 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(meta)) & 15) == 0,
+              "int4_linear: rows, codes and scales must be 16-byte aligned");
   if (M == 0 || N == 0) return 0;
-  const int sms = sm_count(), rows = (N + sms - 1) / sms;
-  Int4Linear a{(const bf16*)A, (const uint8_t*)codes, (const uint32_t*)meta, (bf16*)C, lda, ldc, M, N, K, group, pitch, rows, weights_early()};
-  const dim3 grid((N + rows - 1) / rows);
-  const size_t smem = (size_t)kI4LWarps * (M > 8 ? 16 : 8) * (kI4LOctets * 8 + 4) * sizeof(float);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (M > 8) {
-    static PerDevice raised;
-    KSA_CHECK_CUDA(raise_smem_limit(raised, int4_linear_kernel<2>, smem));
-    KSA_CHECK_CUDA(launch_kernel(int4_linear_kernel<2>, grid, dim3(kI4LThreads), smem, st, a));
-  } else {
-    static PerDevice raised;
-    KSA_CHECK_CUDA(raise_smem_limit(raised, int4_linear_kernel<1>, smem));
-    KSA_CHECK_CUDA(launch_kernel(int4_linear_kernel<1>, grid, dim3(kI4LThreads), smem, st, a));
+  const int sms = sm_count();
+  KSA_REQUIRE(sms > 0, "int4_linear: no device");
+  Int4Linear a{};
+  a.A = (const bf16*)A; a.meta = (const uint32_t*)meta; a.C = (bf16*)C;
+  a.lda = lda; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.group = group; a.pitch = pitch;
+  a.n_out = glu ? N / 2 : N;
+  a.per_cta = (a.n_out + sms - 1) / sms;
+  a.segments = (K + 127) / 128;
+  a.ragged = K % 128 != 0;
+  a.early = weights_early();
+  int parts = 0, best = 0;
+  for (int p = glu ? 2 : 1; p <= 4; p *= 2) {
+    int per_pass;
+    const int cost = i4l_cost(a.per_cta, a.segments, p, glu ? 2 : 1, &per_pass);
+    if (parts == 0 || cost < best) { parts = p; best = cost; a.per_pass = per_pass; }
   }
-  return 0;
+  if (a.ragged) a.per_pass += a.per_pass & 1;        // a box begins on 128 bytes
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (glu && parts == 2) return M <= 8 ? launch_int4_linear<1, 2, true>(a, codes, st) : launch_int4_linear<2, 2, true>(a, codes, st);
+  if (glu) return M <= 8 ? launch_int4_linear<1, 4, true>(a, codes, st) : launch_int4_linear<2, 4, true>(a, codes, st);
+  if (parts == 1) return M <= 8 ? launch_int4_linear<1, 1, false>(a, codes, st) : launch_int4_linear<2, 1, false>(a, codes, st);
+  if (parts == 2) return M <= 8 ? launch_int4_linear<1, 2, false>(a, codes, st) : launch_int4_linear<2, 2, false>(a, codes, st);
+  return M <= 8 ? launch_int4_linear<1, 4, false>(a, codes, st) : launch_int4_linear<2, 4, false>(a, codes, st);
 }

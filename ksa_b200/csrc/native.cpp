@@ -85,7 +85,7 @@ int ksa_int4_decode_attn(const void* q, const void* k, const void* k_meta, const
                          long long q_st, long long q_sh, float scale, void* stream);
 long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap);
 int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
-                    long long ldc, void* stream);
+                    long long ldc, int glu, void* stream);
 int ksa_summary_attn_bwd(const void* q, const void* k, const void* v, const void* ks, const void* vs, const void* o,
                          const void* dout, const void* lse, void* dq, void* dk, void* dv, void* dks, void* dvs, int B, int Hq,
                          int Hkv, int D, int Nq, int seq_len, long long q_rs, long long q_bs, long long k_rs, long long k_bs,
@@ -775,25 +775,27 @@ PyObject* py_int4_decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) 
   END_HANDLE_TH_ERRORS
 }
 
-// int4_linear(x, codes, scales) -> y [..., N], at most 16 rows
+// int4_linear(x, codes, scales, glu) -> y [..., N] (glu: [..., N / 2]), at most 16 rows
 PyObject* py_int4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(v, n);
   const Tensor *x = a.tensor(), *w = a.tensor(at::kByte), *s = a.tensor();
+  const int glu = a.integer() != 0;
   if (!a.ok() || !packed2d(w) || s->dim() != 3 || !s->is_contiguous() || !aligned(w) || !aligned(s) || x->dim() < 1) return none();
   const long long N = w->size(0), K = 2 * w->size(1), groups = s->size(0), pitch = s->size(1), M = x->numel() / K;
   if (K != x->size(-1) || M > 16 || !fits(N) || !fits(K) || pitch != (N + 3) / 4 * 4 || s->size(2) != 2 || K % groups != 0 ||
       (K / groups != 32 && K / groups != 64 && K / groups != 128) || !(x->is_contiguous() || (x->dim() == 2 && eights(x))) || !aligned(x) ||
-      differentiated({x}))
+      (glu && N % 2 != 0) || differentiated({x}))
     return none();
+  const long long out = glu ? N / 2 : N;
   Tensor y;
   {
     pybind11::gil_scoped_release no_gil;
     auto sizes = x->sizes().vec();
-    sizes.back() = N;
+    sizes.back() = out;
     y = a.empty(sizes);
     LAUNCH(ksa_int4_linear, x->const_data_ptr(), w->const_data_ptr(), s->const_data_ptr(), y.mutable_data_ptr(), (int)M, (int)N, (int)K,
-           (int)(K / groups), (int)pitch, x->dim() == 2 ? x->stride(0) : K, N, a.stream());
+           (int)(K / groups), (int)pitch, x->dim() == 2 ? x->stride(0) : K, out, glu, a.stream());
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS

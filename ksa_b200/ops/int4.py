@@ -257,34 +257,48 @@ def _weight_values(weight: Int4Weight, out: torch.Tensor) -> None:
 def int4_linear(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """``x @ W.T`` for ``x`` ``[..., K]`` and ``W = int4_dequantize_weight(weight)``.  At most 16 rows (a decode step) read the codes
     once; more rows multiply with the bf16 values, written out for the call."""
-    made = _native.int4_linear(x, *weight)
+    return _linear(x, weight, False)
+
+
+def int4_linear_swiglu(x: torch.Tensor, w13: Int4Weight) -> torch.Tensor:
+    """``swiglu(int4_linear(x, w13))`` with ``w13 = [gate rows | up rows]``; for at most 16 rows in one launch."""
+    return _linear(x, w13, True)
+
+
+def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
+    made = _native.int4_linear(x, *weight, glu)
     if made is not None:
         return made
     N, K, group, pitch = _check_weight(weight)
     _require(x.dim() >= 1 and x.shape[-1] == K, f"rows {tuple(x.shape)} do not fit a weight [{N}, {K}]")
+    _require(not glu or N % 2 == 0, f"{N} rows are not as many gate as up rows")
     _require(x.device == weight.codes.device, "rows and weight are on different devices")
     _require_inference(x)
     if not x.is_cuda:
-        return ref.linear(x, int4_dequantize_weight(weight).to(x.dtype))
+        y = ref.linear(x, int4_dequantize_weight(weight).to(x.dtype))
+        return ref.swiglu(y) if glu else y
     if x.dtype != torch.bfloat16:
         raise TypeError(f"the sm_100a kernels take bf16 activations, got {x.dtype}")
-    M = x.numel() // K
+    M, out_shape = x.numel() // K, (*x.shape[:-1], N // 2 if glu else N)
     if M > FEW_ROWS:
-        from . import linear
+        from . import linear, swiglu
         values = torch.empty((-(-N // 8) * 8, K), dtype=torch.bfloat16, device=x.device)       # the products take columns in eights
         values[N:].zero_()
         _weight_values(weight, values)
         with _on(x):
             y = linear(x.reshape(M, K), values)
-        return (y if N % 8 == 0 else y[:, :N].contiguous()).view(*x.shape[:-1], N)
+            if glu:
+                gate, up = y[:, :N // 2], y[:, N // 2:N]
+                y = swiglu(y) if N % 16 == 0 else ref.swiglu(torch.cat([gate, up], -1))
+        return (y if glu or N % 8 == 0 else y[:, :N].contiguous()).view(out_shape)
     rows = x.reshape(M, K)
     if M > 0 and (rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.data_ptr() % 16 != 0):
         rows = rows.clone(memory_format=torch.contiguous_format)
-    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    out = torch.empty((M, out_shape[-1]), dtype=x.dtype, device=x.device)
     with _on(x):
-        _lib.call("ksa_int4_linear", rows, weight.codes, weight.scale, out, M, N, K, group, pitch, rows.stride(0), N)
-    return out.view(*x.shape[:-1], N)
+        _lib.call("ksa_int4_linear", rows, weight.codes, weight.scale, out, M, N, K, group, pitch, rows.stride(0), out.shape[1], int(glu))
+    return out.view(out_shape)
 
 
 __all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_cache_read", "int4_decode_attention",
-           "int4_quantize_weight", "int4_dequantize_weight", "int4_linear"]
+           "int4_quantize_weight", "int4_dequantize_weight", "int4_linear", "int4_linear_swiglu"]

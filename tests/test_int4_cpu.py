@@ -91,6 +91,7 @@ def test_linear_is_that_with_the_values():
         assert torch.equal(ops.int4_linear(x, wq), x @ ops.int4_dequantize_weight(wq).float().t())
         assert torch.equal(ops.int4_dequantize_weight(wq), ref.int4_values(*ref.int4_quantize(w, group)))
     assert ops.int4_linear(torch.randn(0, 192), wq).shape == (0, 10)
+    assert torch.equal(ops.int4_linear_swiglu(x, wq), ops.swiglu(ops.int4_linear(x, wq)))
 
 
 def _refused(error, fn, *args, **kw):
@@ -130,5 +131,6 @@ def test_refusals():
     _refused(ValueError, ops.int4_linear, torch.randn(2, 128), w._replace(scale=w.scale[:3]))
     _refused(TypeError, ops.int4_linear, torch.randn(2, 128), w._replace(codes=w.codes.int()))
     _refused(RuntimeError, ops.int4_linear, torch.randn(2, 128, requires_grad=True), w)
+    _refused(ValueError, ops.int4_linear_swiglu, torch.randn(2, 128), ops.int4_quantize_weight(_bf16(7, 128), 32))
     with torch.no_grad():
         ops.int4_linear(torch.randn(2, 128, requires_grad=True), w)

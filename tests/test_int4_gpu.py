@@ -306,6 +306,24 @@ def test_linear_with_a_last_segment_that_is_not_whole(N, K):
         _check_linear(ops.int4_linear(x, w), x, w)
 
 
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("F,K", [(1, 128), (5, 256), (150, 384), (4864, 256), (9728, 128), (333, 1152)])
+def test_linear_swiglu(F, K, group):
+    """Against 64 bits: gate and up are as `_check_linear` has them, rounded to bf16; silu has a slope of at most 1.1, and the result is
+    rounded once more, with 2^-20 for the fp32 exponential, division and products."""
+    w = ops.int4_quantize_weight((_randn(2 * F, K, seed=F) * 0.1).bfloat16(), group)
+    wd = ops.int4_dequantize_weight(w).double()
+    for M in (1, 8, 11, 16, 19):
+        x = _randn(M, K, seed=M)
+        y, mag = x.double() @ wd.t(), x.double().abs() @ wd.abs().t()
+        err = HALF * y.abs() * 1.01 + (K / 16 + 64) * FP32 * mag
+        gate, up, dg, du = y[:, :F], y[:, F:], err[:, :F], err[:, F:]
+        expect = torch.nn.functional.silu(gate) * up
+        bound = 1.1 * dg * (up.abs() + du) + torch.nn.functional.silu(gate).abs() * du + (HALF + 2.0 ** -20) * (expect.abs() + dg * up.abs()) * 1.01 + 1e-30
+        assert ((ops.int4_linear_swiglu(x, w).double() - expect).abs() <= bound).all()
+    _lib.check_status()
+
+
 def test_linear_rows_of_any_layout():
     N, K = 200, 256
     w = ops.int4_quantize_weight(_randn(N, K, seed=1))
