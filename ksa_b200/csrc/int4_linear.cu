@@ -8,9 +8,8 @@
 //     cost its 0.5 us whatever its size), as far ahead as the ring reaches, in the engine's decode step ahead of the previous kernel's end;
 //   * sixteen warps multiply: a round has 16 / kParts segments, and kParts warps share the rows of a segment.  They keep their sums of a pass and
 //     leave them in shared memory; two more warps add the sums up and write the results while the others are at the next pass;
-//   * mma.sync m16n8k16 takes the activations as its 16 rows and weights in eights, so that a CTA's share of rows need not be a multiple of 16; a
-//     lane's 16 bytes of a weight row are columns 32 t .. 32 t + 31 of the segment, in that order for the activations as well.  Activations that several passes
-//     want stay in shared memory, others are read as they are needed.
+//   * mma.sync m16n8k16 multiplies 16 weight rows by 8 activation rows; a lane's 16 bytes of a weight row are columns 32 t .. 32 t + 31 of the segment, in
+//     that order for the activations as well.  Activations that several passes want stay in shared memory, others are read as they are needed.
 #include "host.h"
 #include "int4.cuh"
 
@@ -19,7 +18,7 @@ namespace ksa {
 constexpr int kI4LWarps = 16;                       // that multiply
 constexpr int kI4LAdders = 2;                       // that add up and write
 constexpr int kI4LThreads = (kI4LWarps + kI4LAdders + 1) * 32;
-constexpr int kI4LOctets = 4;                       // eights of weight rows of a warp
+constexpr int kI4LBlocks = 2;                       // blocks of 16 weight rows of a warp
 constexpr int kI4LMostStages = 12;
 constexpr int kI4LSmemMost = 227 * 1024;
 
@@ -37,13 +36,47 @@ struct Int4Linear {
   int early;                       // weights are read ahead of the wait
 };
 
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+// acc[i] += rows 16 i + (g, g + 8) of the segment at `codes` times the activations' columns of it
+template <int NB, int kCount>
+__device__ __forceinline__ void i4l_multiply(float (&acc)[kI4LBlocks][NB][4], const uint4 (&x)[NB][4], const uint8_t* codes, const uint32_t* meta) {
+  uint32_t words[kCount][2][4], s2[kCount][2], o2[kCount][2];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<uint4*>(words[i][h]) = *reinterpret_cast<const uint4*>(codes + (i * 16 + h * 8) * 64);
+      const uint32_t m = meta[i * 16 + h * 8];
+      s2[i][h] = i4_scale2(m);
+      o2[i][h] = i4_offset2(m);
+    }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      uint32_t v[4], w[4];
+      i4_values(v, words[i][0][q], s2[i][0], o2[i][0]);
+      i4_values(w, words[i][1][q], s2[i][1], o2[i][1]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        mma_bf16(acc[i][n], v[0], w[0], v[1], w[1], x[n][q].x, x[n][q].y);
+        mma_bf16(acc[i][n], v[2], w[2], v[3], w[3], x[n][q].z, x[n][q].w);
+      }
+    }
+}
+
 // NB: activation rows in eights.  kParts: warps that share a segment's rows, up to 32 each (kGlu: the first half of them gate rows, the other their up rows).
 template <int NB, int kParts, bool kGlu>
 __global__ void __launch_bounds__(kI4LThreads, 1)
 int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_meta, const Int4Linear a, int* status) {
   static_assert(!kGlu || kParts >= 2, "parts for gate and up rows");
   constexpr int kTurns = kI4LWarps / kParts;                                // segments of a round
-  constexpr int kRows = kI4LOctets * 8 * kParts, kPitch = kRows + 8;        // rows of a pass; floats of a row of sums
+  constexpr int kRows = kI4LBlocks * 16 * kParts, kPitch = kRows + 8;        // rows of a pass; floats of a row of sums
   constexpr int kSets = kGlu ? 2 : 1, kPerSet = kParts / kSets;             // boxes of a round, warps for the rows of one
   extern __shared__ __align__(128) uint8_t raw[];
   uint8_t* ring = raw;
@@ -150,104 +183,110 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   // ------------------------------------------------------------------ the warps that multiply
   if (a.x_pitch > 0) {
     // an activation's 16 bytes w of the 64 that lane t wants of a segment lie at 4 w + t: four lanes read 64 bytes in a row
-    const int per = a.segments * 16;
+    const int per = rounds * kTurns * 16;
     for (int i = threadIdx.x; i < a.M * per; i += kI4LWarps * 32) {
       const int m = i / per, c = i - m * per;
       uint4 v = make_uint4(0, 0, 0, 0);
-      if (c * 8 < a.K) v = *reinterpret_cast<const uint4*>(a.A + m * a.lda + c * 8);
+      if (c * 8 < a.K) v = *reinterpret_cast<const uint4*>(a.A + m * a.lda + c * 8);         // zeros behind
       *reinterpret_cast<uint4*>(xs + m * a.x_pitch + (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16) = v;
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kI4LWarps * 32) : "memory");
   }
   const int turn = warp / kParts, set = kGlu ? warp % kParts / kPerSet : 0, which = warp % kParts % kPerSet;
+  const int t_group = t * 32 / a.group;
+  // this lane's activations of the warp's first segment, and those eight rows on; a row past the last is the last one again, in sums that nobody reads
+  const int x_row = min(g, a.M - 1), x_next = NB == 2 ? min(g + 8, a.M - 1) - x_row : 0;
+  const bf16* x_first = a.A + x_row * a.lda + turn * 128 + t * 32;
+  const long long x_eight = x_next * a.lda;
+  const uint32_t x_kept = smem_u32(xs) + x_row * a.x_pitch + turn * 256 + t * 16, kept_eight = x_next * a.x_pitch;
   bool ok = true;
   int stage = 0;
   uint32_t phase = 0;
   for (int p = 0; p < passes; ++p) {
-    const int row = r0 + p * a.per_pass, octets = (min(a.per_pass, r0 + mine - row) + 7) / 8;
-    // this warp's eights of the rows, and the first of them
-    const int each = (octets + kPerSet - 1) / kPerSet, at = which * each * 8, count = max(0, min(each, octets - which * each));
+    const int row = r0 + p * a.per_pass, blocks = (min(a.per_pass, r0 + mine - row) + 15) / 16;
+    // this warp's blocks of the rows, and the first row of them
+    const int each = (blocks + kPerSet - 1) / kPerSet, at = which * each * 16, count = max(0, min(each, blocks - which * each));
     const int skip = (set * a.n_out + row) & 3;
-    float acc[kI4LOctets][4];
+    float acc[kI4LBlocks][NB][4];
 #pragma unroll
-    for (int i = 0; i < kI4LOctets; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-    for (int round = 0; round < rounds; ++round) {
-      const int seg = round * kTurns + turn, col = seg * 128 + t * 32;
-      uint4 x[NB][4];
+    for (int i = 0; i < kI4LBlocks; ++i)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          x[n][q] = make_uint4(0, 0, 0, 0);
-          if (n * 8 + g < a.M && col < a.K) {
-            if (a.x_pitch > 0) x[n][q] = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * a.x_pitch + seg * 256 + (q * 4 + t) * 16);
-            else x[n][q] = *reinterpret_cast<const uint4*>(a.A + (n * 8 + g) * a.lda + col + q * 8);
-          }
-        }
+        for (int e = 0; e < 4; ++e) acc[i][n][e] = 0.f;
+    // where this lane reads: in a stage, and the activations of the pass's first segment
+    const uint32_t codes_at = set * set_bytes + (turn * a.per_pass + at + g) * 64 + t * 16;
+    const uint32_t meta_at = a.meta_at + set * meta_bytes + ((turn * groups + t_group) * a.meta_words + skip + at + g) * 4;
+    const bf16* xp = x_first;
+    uint32_t xk = x_kept;
+    for (int round = 0, seg = turn; round < rounds; ++round, seg += kTurns, xp += kTurns * 128, xk += kTurns * 256) {
+      // past K everything of the weights is zero, and any of the row's columns will do
+      uint4 x[NB][4];
+      if (a.x_pitch > 0) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[n][q] = ld_shared(xk + n * kept_eight + q * 64);
+      } else {
+        const bf16* from = seg * 128 + t * 32 < a.K ? xp : x_first - (turn * 128 + t * 32);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) x[n][q] = *reinterpret_cast<const uint4*>(from + n * x_eight + q * 8);
+      }
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
       if (seg < a.segments) {                                                // what lies past K in the last one is zeros, scales and all
         const uint8_t* src = ring + stage * a.stage_bytes;
-        const uint8_t* codes = src + set * set_bytes + (turn * a.per_pass + at + g) * 64 + t * 16;
-        const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + a.meta_at + set * meta_bytes) +
-                               (turn * groups + t * 32 / a.group) * a.meta_words + skip + at + g;
-#pragma unroll
-        for (int i = 0; i < kI4LOctets; ++i) {
-          if (i >= count) break;
-          const uint4 w = *reinterpret_cast<const uint4*>(codes + i * 512);
-          const uint32_t m = meta[i * 8], s2 = i4_scale2(m), o2 = i4_offset2(m), words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[4];
-            i4_values(v, words[q], s2, o2);
-            const uint4 xa = x[0][q], xb = NB == 2 ? x[NB - 1][q] : make_uint4(0, 0, 0, 0);
-            mma_bf16(acc[i], xa.x, xb.x, xa.y, xb.y, v[0], v[1]);
-            mma_bf16(acc[i], xa.z, xb.z, xa.w, xb.w, v[2], v[3]);
-          }
-        }
+        const uint8_t* codes = src + codes_at;
+        const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + meta_at);
+        if (count == 2) i4l_multiply<NB, 2>(acc, x, codes, meta);            // two chains of products side by side
+        else if (count == 1) i4l_multiply<NB, 1>(acc, x, codes, meta);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[stage]);
       if (++stage == a.stages) { stage = 0; phase ^= 1; }
     }
-    // ---- this warp's sums: acc[i] = (row g, weights 2 t and 2 t + 1), (row g + 8, the same)
+    // ---- this warp's sums: acc[i][n] = (weight row g, activations 2 t and 2 t + 1), (weight row g + 8, the same)
     if (p > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(added, (p - 1) & 1, guard, kTimeoutAccEmpty));
     if (!ok) break;
 #pragma unroll
-    for (int i = 0; i < kI4LOctets; ++i) {
+    for (int i = 0; i < kI4LBlocks; ++i) {
       if (i >= count) break;
-      float* dst = part + (turn * NB * 8 + g) * kPitch + set * (kRows / 2) + at + i * 8 + t * 2;
-      if (g < a.M) *reinterpret_cast<float2*>(dst) = make_float2(acc[i][0], acc[i][1]);
-      if (NB == 2 && g + 8 < a.M) *reinterpret_cast<float2*>(dst + 8 * kPitch) = make_float2(acc[i][2], acc[i][3]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = n * 8 + t * 2 + (e & 1);
+          if (m < a.M) part[(turn * NB * 8 + m) * kPitch + set * (kRows / 2) + at + i * 16 + (e >> 1) * 8 + g] = acc[i][n][e];
+        }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(left);
   }
 }
 
-// How a CTA of `per_cta` output columns takes them with `parts` warps to a segment: rows of a pass, and the eights of rows that a warp multiplies in all,
-// with what a round costs besides (two of them) and a pass (four).
+// How a CTA of `per_cta` output columns takes them with `parts` warps to a segment: rows of a pass, and the blocks of rows that a warp multiplies in all,
+// with what a round costs besides (one of them) and a pass (two).
 static int i4l_cost(int per_cta, int segments, int parts, int sets, int* per_pass) {
-  const int most = kI4LOctets * 8 * parts / sets, passes = (per_cta + most - 1) / most, turns = kI4LWarps / parts;
+  const int most = kI4LBlocks * 16 * parts / sets, passes = (per_cta + most - 1) / most, turns = kI4LWarps / parts;
   *per_pass = (per_cta + passes - 1) / passes;
-  const int octets = (*per_pass + 7) / 8, each = (octets * sets + parts - 1) / parts;
-  return passes * ((segments + turns - 1) / turns * (each + 2) + 4);
+  const int each = ((*per_pass + 15) / 16 * sets + parts - 1) / parts;
+  return passes * ((segments + turns - 1) / turns * (each + 1) + 2);
 }
 
 template <int NB, int kParts, bool kGlu>
 static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) {
-  constexpr int kTurns = kI4LWarps / kParts, kRows = kI4LOctets * 8 * kParts, kPitch = kRows + 8, kSets = kGlu ? 2 : 1;
+  constexpr int kTurns = kI4LWarps / kParts, kRows = kI4LBlocks * 16 * kParts, kPitch = kRows + 8, kSets = kGlu ? 2 : 1;
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_linear: no status word");
   const int groups = 128 / a.group;
   a.meta_words = (a.per_pass + 3 + 3) / 4 * 4;
-  a.meta_at = kSets * ((kTurns * a.per_pass * 64 + 127) / 128 * 128) + 512;       // the last eight may reach past the rows
-  a.stage_bytes = a.meta_at + kSets * ((kTurns * groups * a.meta_words * 4 + 127) / 128 * 128) + 128;
+  a.meta_at = kSets * ((kTurns * a.per_pass * 64 + 127) / 128 * 128) + 1024;      // the last block may reach past the rows
+  a.stage_bytes = a.meta_at + kSets * ((kTurns * groups * a.meta_words * 4 + 127) / 128 * 128) + 128;          // (its scales as well)
   const int part = kTurns * NB * 8 * kPitch * 4, per_stage = a.stage_bytes + 16, rest = part + 32;
   // activations that several passes want stay, where a ring of 64 KB and three rounds finds room beside them
-  const int passes = (a.per_cta + a.per_pass - 1) / a.per_pass, x_pitch = a.segments * 256 + 64;
+  const int passes = (a.per_cta + a.per_pass - 1) / a.per_pass, x_pitch = (a.segments + kTurns - 1) / kTurns * kTurns * 256 + 64;
   const int least = 3 * per_stage > 64 * 1024 ? 3 * per_stage : 64 * 1024;
   a.x_pitch = passes > 1 && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
   a.stages = (kI4LSmemMost - rest - a.M * a.x_pitch) / per_stage;
