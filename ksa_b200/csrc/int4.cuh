@@ -38,44 +38,67 @@ __device__ __forceinline__ void i4_values(uint32_t (&v)[4], uint32_t w, uint32_t
   v[3] = fma_bf16x2(i4_unit<3>(w), s2, o2);
 }
 
-// Eight values of each of the `kLanes` neighbouring lanes that hold a group -> this lane's word of codes and the group's scale and offset.
-// Every step is one IEEE operation (the library is built with approximate division otherwise), so that a host computes the same codes.
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Sixteen values of each of the `kLanes` neighbouring lanes that hold a group -> this lane's words of codes and the group's scale and offset.
+// The codes are those of one IEEE operation after another, c = rint(((x - O) / S) * 16) - 16 (the library is built with approximate division
+// otherwise), so that a host computes the same; many values of a coarse grid lie exactly between two codes.  A division costs ten operations a
+// value.  Instead t = x - O is multiplied by 16 / S in two terms: an approximation r to 2^-22, and what it leaves, e = (16 - r S) / S to 2^-22 of it.
+// RN(t r + RN(t e)) is t * 16 / S to within 2^-43 before the last rounding, and the quotient of 24 bits by 8 bits lies at least 2^-33 from the
+// middle between two floats (t - m S is a multiple of 2^-33 t for a middle m of 25 bits, and not zero: m S has more than 24 bits), so that
+// the last rounding is the division's.  The range is divided by 15, of four bits, in the same way.
 // Magnitudes over 2^126 count as 2^126, which keeps scale and offset finite; a group with an infinity or a NaN becomes NaN as a whole.
 template <int kLanes>
-__device__ __forceinline__ void i4_quantize(const uint4& raw, uint32_t& word, uint32_t& meta) {
+__device__ __forceinline__ void i4_quantize(const uint4 (&raw)[2], uint2& words, uint32_t& meta) {
   constexpr float kMost = 8.507059173023462e37f, kLeast = 7.888609052210118e-31f;      // 2^126, 2^-100
-  const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-  float f[8], lo = INFINITY, hi = -INFINITY;
-  bool bad = false;
+  constexpr float kRound = 12582912.f;                           // 1.5 * 2^23: a sum with it has whole numbers in its lowest bits
+  const uint32_t u[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t lo2 = u[0], hi2 = u[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16;
-    bad |= (bits & 0x7F800000u) == 0x7F800000u;
-    f[i] = fminf(fmaxf(__uint_as_float(bits), -kMost), kMost);
-    lo = fminf(lo, f[i]);
-    hi = fmaxf(hi, f[i]);
-  }
-  if (bad) hi = INFINITY;
+  for (int i = 1; i < 8; ++i) { lo2 = min_bf16x2(lo2, u[i]); hi2 = max_nan_bf16x2(hi2, u[i]); }
 #pragma unroll
   for (int d = 1; d < kLanes; d *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    lo2 = min_bf16x2(lo2, __shfl_xor_sync(0xffffffffu, lo2, d));
+    hi2 = max_nan_bf16x2(hi2, __shfl_xor_sync(0xffffffffu, hi2, d));
   }
-  float s = __bfloat162float(__float2bfloat16_rn(__fmul_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f), 16.f)));
+  lo2 = min_bf16x2(lo2, __byte_perm(lo2, lo2, 0x1032));
+  hi2 = max_nan_bf16x2(hi2, __byte_perm(hi2, hi2, 0x1032));
+  const bool bad = (hi2 & 0x7F80u) == 0x7F80u || (lo2 & 0x7F80u) == 0x7F80u;
+  const float lo = fminf(fmaxf(__uint_as_float(lo2 << 16), -kMost), kMost), hi = fminf(fmaxf(__uint_as_float(hi2 << 16), -kMost), kMost);
+  const float range = __fsub_rn(hi, lo);                         // * 16 / 15
+  float s = __bfloat162float(__float2bfloat16_rn(fmaf(range, 1.0666667222976685f, __fmul_rn(range, -5.563100202721216e-08f))));
   if (s < kLeast) s = 0.f;
   const float o = __bfloat162float(__float2bfloat16_rn(__fsub_rn(lo, s)));
-  meta = pack_bf16x2(s, o);
-  word = 0;
-  if (hi == INFINITY) {
-    meta = 0x7FFF7FFFu;
-  } else if (s > 0.f) {
+  meta = bad ? 0x7FFF7FFFu : pack_bf16x2(s, o);
+  words = make_uint2(0, 0);
+  if (bad || s == 0.f) return;
+  const float down = s > 1.1529215e18f ? 8.6736174e-19f : 1.f;   // 2^60, 2^-60: keeps e normal
+  const float to = -o * down, sd = s * down, r = __fdividef(16.f, sd), e = fmaf(-r, sd, 16.f) * (r * 0.0625f);
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float even = 0.f, odd = 0.f;                                 // four codes each, as one number
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float c = rintf(__fmul_rn(__fdiv_rn(__fsub_rn(f[i], o), s), 16.f));
-      const uint32_t code = (uint32_t)(int)fminf(fmaxf(c - 16.f, 0.f), 15.f);
-      word |= code << ((i & 1) * 16 + (i / 2) * 4);
+      const uint32_t pair = u[h * 4 + i / 2];
+      const float x = __uint_as_float(i & 1 ? pair & 0xFFFF0000u : pair << 16), t = fmaf(x, down, to);
+      const float y = fminf(fmaxf(fmaf(t, r, __fmul_rn(t, e)), 16.f), 31.f), c = __fsub_rn(__fadd_rn(y, kRound), kRound);
+      if (i & 1) odd = fmaf(c, (float)(1 << (i / 2 * 4)), odd);
+      else even = fmaf(c, (float)(1 << (i / 2 * 4)), even);
     }
+    // 16 * (1 + 16 + 256 + 4096) = 69904 too much each
+    w[h] = __byte_perm(__float_as_uint(even + (kRound - 69904.f)), __float_as_uint(odd + (kRound - 69904.f)), 0x5410);
   }
+  words = make_uint2(w[0], w[1]);
 }
 
 // Each row of an 8 x 8 matrix of 16-bit values lies in four lanes; afterwards each column does.

@@ -21,6 +21,7 @@ from . import reference as ref
 from ._lib import native as _native
 
 CACHE_GROUP = 32          # values of a cache row that share a scale
+CACHE_DIM = 2048          # largest head dimension
 CACHE_SLOTS = 16          # the capacity of a cache is a multiple of this
 FEW_ROWS = 16             # rows that the kernel of ``int4_linear`` takes
 _TABLE_ROWS = 64          # rows of a sequence from which a write finds the last row of each slot in a table
@@ -79,8 +80,8 @@ def _check_cache(c: Int4Cache) -> Tuple[int, int, int, int]:
     _require(c.k.dim() == 4 and c.k_scale.dim() == 5, "an int4 cache has codes of 4 dimensions and scales of 5")
     B, H, cap, half = c.k.shape
     D = 2 * half
-    _require(D % CACHE_GROUP == 0 and D > 0 and cap % CACHE_SLOTS == 0 and cap > 0 and H > 0,
-             f"an int4 cache takes head dims in multiples of {CACHE_GROUP} and capacities in multiples of {CACHE_SLOTS}, got {D} and {cap}")
+    _require(D % CACHE_GROUP == 0 and 0 < D <= CACHE_DIM and cap % CACHE_SLOTS == 0 and cap > 0 and H > 0,
+             f"an int4 cache takes head dims in multiples of {CACHE_GROUP} up to {CACHE_DIM} and capacities in multiples of {CACHE_SLOTS}, got {D} and {cap}")
     for codes, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
         _require(codes.shape == c.k.shape and tuple(scale.shape) == (B, H, cap, D // CACHE_GROUP, 2),
                  "the parts of an int4 cache do not fit together")
@@ -105,7 +106,7 @@ def _int32(x: torch.Tensor, shape, device, what: str) -> torch.Tensor:
 # =============================================================================== cache
 def int4_cache(batch: int, kv_heads: int, capacity: int, head_dim: int, device=None) -> Int4Cache:
     """An empty cache (every slot stands for zeros) of at least ``capacity`` slots."""
-    _require(head_dim > 0 and head_dim % CACHE_GROUP == 0, f"head_dim {head_dim} is no multiple of {CACHE_GROUP}")
+    _require(0 < head_dim <= CACHE_DIM and head_dim % CACHE_GROUP == 0, f"head_dim {head_dim} is no multiple of {CACHE_GROUP} up to {CACHE_DIM}")
     _require(batch >= 0 and kv_heads > 0 and capacity > 0, "an int4 cache needs heads and slots")
     cap = -(-capacity // CACHE_SLOTS) * CACHE_SLOTS
     codes = lambda: torch.zeros(batch, kv_heads, cap, head_dim // 2, dtype=torch.uint8, device=device)

@@ -62,6 +62,26 @@ def test_write_and_read_are_the_plain_form_to_the_bit(B, T, H, D, cap):
             assert (x[b][:, ~inside] == 0).all()
 
 
+def test_codes_next_to_the_middle_between_two():
+    """Rows on a coarse grid: many values lie exactly between two codes, or a rounding away from it."""
+    g = _gen(7)
+    B, T, H, D = 2, 600, 2, 128
+    k = (torch.randint(-64, 65, (B, T, H, D), device=DEV, generator=g) / 16).bfloat16()
+    scale = torch.exp2(torch.randint(-110, 110, (B, T, H, 1), device=DEV, generator=g).float())
+    v = (torch.randint(-30, 31, (B, T, H, D), device=DEV, generator=g).float() * scale).bfloat16()
+    cache = ops.int4_cache(B, H, T, D, DEV)
+    ops.int4_cache_write(cache, k, v, torch.arange(T, device=DEV).repeat(B, 1), distinct=True)
+    ties = 0
+    for rows, codes, scales in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        c, s = ref.int4_quantize(rows.cpu(), 32)
+        s_, o_ = s[..., 0].double().repeat_interleave(32, -1), s[..., 1].double().repeat_interleave(32, -1)
+        y = (rows.cpu().double() - o_) / s_ * 16
+        ties += int(((y - y.floor() - 0.5).abs() < 1e-9).sum())
+        assert torch.equal(codes[:, :, :T].transpose(1, 2).cpu(), c)
+        _same(scales[:, :, :T].transpose(1, 2).cpu().float(), s.float())
+    assert ties > 1000                  # the inputs are what they are meant to be
+
+
 @pytest.mark.parametrize("T", [2, 64, 65, 3000])
 def test_the_last_row_of_a_slot_stays(T):
     B, H, D, cap = 2, 2, 64, 32
