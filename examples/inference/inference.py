@@ -21,7 +21,11 @@ def main():
     ap.add_argument("--top-p", type=float, default=0.9)
     ap.add_argument("--greedy", action="store_true")
     ap.add_argument("--engine", action="store_true", help="generate with ksa_b200's inference engine instead of HF generate")
+    ap.add_argument("--kv-cache", default="bf16", choices=["bf16", "int4"], help="with --engine: int4 holds keys and values in four bits")
+    ap.add_argument("--weights", default="bf16", choices=["bf16", "int4"], help="with --engine: int4 decodes with weights in four bits")
     a = ap.parse_args()
+    if not a.engine and "int4" in (a.kv_cache, a.weights):
+        ap.error("--kv-cache int4 and --weights int4 need --engine")
     dtype = torch.bfloat16 if a.device.startswith("cuda") else torch.float32
     if a.engine:
         import os
@@ -44,7 +48,8 @@ def main():
     t0 = time.perf_counter()
     if a.engine:
         from ksa_b200.inference import KsaInferenceEngine
-        eng = KsaInferenceEngine(model, max_len=ids.shape[1] + a.max_new_tokens + model.config.summary_chunk_size, batch=1)
+        eng = KsaInferenceEngine(model, max_len=ids.shape[1] + a.max_new_tokens + model.config.summary_chunk_size, batch=1,
+                                 kv_cache=a.kv_cache, weights=a.weights)
         with torch.no_grad():
             out = eng.generate(ids, a.max_new_tokens, eos_id=model.config.eos_token_id,
                                temperature=0.0 if a.greedy else a.temperature, top_p=a.top_p)

@@ -104,6 +104,29 @@ __global__ void __launch_bounds__(kI4Threads) int4_cache_read_kernel(Int4Read a)
   *reinterpret_cast<uint4*>(a.v + to) = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// Slots [src[b], src[b] + rows) -> [dst[b], dst[b] + rows) of the sequences with enable[b] != 0, eight bytes a thread; slots outside the cache are left out.
+struct Int4Move {
+  uint8_t *k_codes, *k_meta, *v_codes, *v_meta;
+  const int *src, *dst, *enable;
+  int B, H, D, cap, rows;
+};
+__global__ void __launch_bounds__(kI4Threads) int4_cache_move_kernel(Int4Move a) {
+  grid_dependency_enter();
+  const int codes = a.D / 16, per = codes + a.D / 64;            // of a row: units of codes, and of codes and scales
+  const long long i = (long long)blockIdx.x * kI4Threads + threadIdx.x;
+  if (i >= (long long)a.B * a.H * a.rows * per * 2) return;
+  const int c = (int)(i % per), kv = (int)(i / per % 2), r = (int)(i / per / 2 % a.rows);
+  const long long bh = i / per / 2 / a.rows;
+  const int b = (int)(bh / a.H);
+  if (!a.enable[b]) return;
+  const long long from = (long long)a.src[b] + r, to = (long long)a.dst[b] + r;
+  if (from < 0 || to < 0 || from >= a.cap || to >= a.cap) return;
+  uint8_t* base = c < codes ? (kv ? a.v_codes : a.k_codes) : (kv ? a.v_meta : a.k_meta);
+  const int width = c < codes ? codes : a.D / 64, at = c < codes ? c : c - codes;
+  uint2* rows = reinterpret_cast<uint2*>(base) + bh * a.cap * width + at;
+  rows[to * width] = rows[from * width];
+}
+
 // Weights: rows [N, K] (row pitch `ld`) -> codes [N, K / 2], scales [K / group, pitch] words; a row's groups of kLanes * 16 values.
 template <int kLanes>
 __global__ void __launch_bounds__(kI4Threads) int4_weight_kernel(const bf16* w, uint2* codes, uint32_t* meta, int N, int K, long long ld, int pitch) {
@@ -189,6 +212,21 @@ KSA_API int ksa_int4_cache_read(const void* k_codes, const void* k_meta, const v
              (bf16*)v, H, D, cap, rows, in_block, Int4Divide(of_head), Int4Divide(H), Int4Divide(D / 8)};
   KSA_CHECK_CUDA(launch_stream_kernel((long long)B * H * rows * D * 5, int4_cache_read_kernel, dim3((unsigned)blocks), dim3(kI4Threads), 0,
                                       reinterpret_cast<cudaStream_t>(stream), a));
+  return 0;
+}
+
+// src, dst, enable: [B].  A sequence's two ranges must not overlap.
+KSA_API int ksa_int4_cache_move(void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* src, const void* dst, const void* enable, int B,
+                                int H, int D, int cap, int rows, void* stream) {
+  KSA_ENTER(k_codes);
+  KSA_REQUIRE(D > 0 && D % 64 == 0, "int4_cache_move: head_dim %d is no multiple of 64", D);
+  KSA_REQUIRE(B >= 0 && rows >= 0 && H > 0 && cap > 0, "int4_cache_move: bad shape");
+  const long long n = (long long)B * H * rows * (D / 16 + D / 64) * 2, blocks = (n + kI4Threads - 1) / kI4Threads;
+  if (n == 0) return 0;
+  KSA_REQUIRE(blocks < (1LL << 31), "int4_cache_move: too many rows");
+  Int4Move a{(uint8_t*)k_codes, (uint8_t*)k_meta, (uint8_t*)v_codes, (uint8_t*)v_meta, (const int*)src, (const int*)dst, (const int*)enable, B, H, D, cap,
+             rows};
+  KSA_CHECK_CUDA(launch_kernel(int4_cache_move_kernel, dim3((unsigned)blocks), dim3(kI4Threads), 0, reinterpret_cast<cudaStream_t>(stream), a));
   return 0;
 }
 

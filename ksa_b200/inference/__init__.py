@@ -1,4 +1,4 @@
-from .cache import CacheSpec, CacheState, FullLayerCache, KsaLayerCache
+from .cache import CacheSpec, CacheState, FullLayerCache, Int4LayerCache, KsaLayerCache
 from .engine import KsaInferenceEngine
 
-__all__ = ["CacheSpec", "CacheState", "FullLayerCache", "KsaLayerCache", "KsaInferenceEngine"]
+__all__ = ["CacheSpec", "CacheState", "FullLayerCache", "Int4LayerCache", "KsaLayerCache", "KsaInferenceEngine"]

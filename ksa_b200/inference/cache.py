@@ -28,6 +28,8 @@ from typing import List, Optional, Tuple
 
 import torch
 
+from .. import ops
+
 
 @dataclass
 class CacheSpec:
@@ -69,6 +71,28 @@ class FullLayerCache:
         self.k = torch.zeros(batch, n_kv_heads, max_len, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         self.max_len = max_len
+
+
+class Int4LayerCache:
+    """Cache of one layer in four bits (``ops.Int4Cache``) with the slots of ``KsaLayerCache`` (``spec``) or ``FullLayerCache``."""
+
+    def __init__(self, spec: Optional[CacheSpec], slots: int, batch: int, n_kv_heads: int, head_dim: int, device):
+        self.spec = spec
+        self.data = ops.int4_cache(batch, n_kv_heads, slots, head_dim, device)
+
+
+def layer_cache(kind: str, spec: Optional[CacheSpec], max_len: int, batch: int, n_kv_heads: int, head_dim: int, dtype, device):
+    """The cache of a summary layer (``spec``) or of a full layer, in the model's type (``"bf16"``) or in four bits (``"int4"``)."""
+    if kind == "int4":
+        return Int4LayerCache(spec, spec.capacity if spec is not None else max_len, batch, n_kv_heads, head_dim, device)
+    if spec is not None:
+        return KsaLayerCache(spec, batch, n_kv_heads, head_dim, dtype, device)
+    return FullLayerCache(max_len, batch, n_kv_heads, head_dim, dtype, device)
+
+
+def cache_tensors(cache) -> Tuple[torch.Tensor, ...]:
+    """All tensors of a layer's cache; slots are their third dimension."""
+    return tuple(cache.data) if isinstance(cache, Int4LayerCache) else (cache.k, cache.v)
 
 
 class CacheState:
@@ -119,3 +143,16 @@ def flush_plan(spec: CacheSpec, st: CacheState) -> Tuple[torch.Tensor, torch.Ten
     src_sum = torch.zeros(B, dtype=torch.int32, device=dev)
     dst_sum = spec.sum0 + st.chunks * S
     return src_text, dst_text, src_sum, dst_sum
+
+
+def prompt_slots(spec: Optional[CacheSpec], length: int, device) -> Tuple[int, torch.Tensor]:
+    """Where a prompt's text rows go: (first row that is kept, slots of the rows from there on).  A summary layer keeps the last
+    ``window`` complete chunks, chunk ``c`` in ring place ``c % window``, and the rest from right to left in the current chunk."""
+    if spec is None:
+        return 0, torch.arange(length, dtype=torch.int32, device=device)
+    C, W = spec.chunk, spec.window
+    full = length // C
+    first = max(0, full - W) * C
+    t = torch.arange(first, length, dtype=torch.int32, device=device)
+    ring = spec.text0 + (t // C) % max(W, 1) * C + t % C
+    return first, torch.where(t < full * C, ring, spec.n_sum + C - 1 - (t - full * C))

@@ -21,7 +21,7 @@ import torch
 from .. import ops
 from ..models.qwen3_ksa import _add_norm, _row_linear
 from ..ops import _lib, reference as ref
-from .cache import (CacheSpec, CacheState, FullLayerCache, KsaLayerCache, flush_plan, summary_step_slices,
+from .cache import (CacheSpec, CacheState, Int4LayerCache, cache_tensors, flush_plan, layer_cache, prompt_slots, summary_step_slices,
                     text_step_slices)
 
 
@@ -112,9 +112,69 @@ def _step_slices(spec: CacheSpec, st: CacheState):
     return out[0], out[0], out[1]
 
 
+# a layer's cache of either kind
+def _append(cache, k_new, v_new, slots):
+    if isinstance(cache, Int4LayerCache):
+        ops.int4_cache_write(cache.data, k_new, v_new, slots)
+    else:
+        _cache_append(k_new, v_new, cache.k, cache.v, slots)
+
+
+def _attend(cache, q, start, length, scale, counters=None):
+    if isinstance(cache, Int4LayerCache):
+        return ops.int4_decode_attention(q, cache.data, start, length, scale)
+    return _decode_attention(q, cache.k, cache.v, start, length, scale, counters)
+
+
+def _move(cache, src, dst, enable, rows):
+    if not isinstance(cache, Int4LayerCache):
+        _cache_move(cache.k, cache.v, src, dst, enable, rows)
+    elif rows > 0:
+        ops.int4_cache_move(cache.data, src, dst, enable, rows)
+
+
+def _rotate_and_append(cache, qkv, a, pos, cfg, slots):
+    """Norm and rotation of a step's rows ``[q | k | v]``; the keys and values of its text rows, the first ``len(slots)``, go into the cache."""
+    Hq, Hkv, Dh = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+    q_w, k_w = a._norm_w(a.q_norm), a._norm_w(a.k_norm)
+    if not isinstance(cache, Int4LayerCache):
+        return ops.qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, Hkv, Dh, cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama", cache.k,
+                                       cache.v, slots)
+    qkv = ops.qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, Hkv, Dh, cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama")
+    n = slots.numel()
+    heads = qkv[:n, Hq * Dh:].view(n, 1, 2 * Hkv, Dh)
+    _append(cache, heads[:, :, :Hkv], heads[:, :, Hkv:], slots.view(n, 1))
+    return qkv
+
+
+class _Int4Layer:
+    """The projections of one layer in four bits."""
+
+    def __init__(self, layer, group: int):
+        a = layer.attn
+        quantize = lambda w: ops.int4_quantize_weight(w.detach(), group)
+        self.qkv, self.out = quantize(a.wqkv.weight), quantize(a.output_proj.weight)
+        own = getattr(a, "wqkv_summary", None)
+        self.qkv_summary = self.qkv if own is None else quantize(own.weight)
+        self.w13, self.w2 = quantize(layer.mlp.w13.weight), quantize(layer.mlp.w2.weight)
+
+
 class KsaInferenceEngine:
-    def __init__(self, model, max_len: int, batch: int, device=None, dtype=None, cuda_graph: bool = True):
+    """``kv_cache="int4"`` holds keys and values in four bits (5 bits a value with their scales, ``ops.int4``): they are quantised as
+    they are written, and decode steps attend over the quantised values; the prompt's own attention is unchanged.
+    ``weights="int4"`` lets decode steps read projections and output head in four bits (groups of ``weight_group`` values along a
+    row); prefill keeps the model's weights, which stay in memory.  Tensor parallelism takes the cache, not the weights."""
+
+    def __init__(self, model, max_len: int, batch: int, device=None, dtype=None, cuda_graph: bool = True, kv_cache: str = "bf16",
+                 weights: str = "bf16", weight_group: int = 64):
+        if kv_cache not in ("bf16", "int4") or weights not in ("bf16", "int4"):
+            raise ValueError(f"kv_cache and weights are 'bf16' (the model's type) or 'int4', got {kv_cache!r} and {weights!r}")
+        if weights == "int4" and getattr(model, "tp", None) is not None:
+            raise ValueError("weights in four bits are not available with tensor parallelism")
         self.model = model.eval()
+        self.kv_cache = kv_cache
+        self._int4 = [_Int4Layer(layer, weight_group) for layer in model.layers] if weights == "int4" else None
+        self._int4_head = ops.int4_quantize_weight(model.lm_head_weight.detach(), weight_group) if weights == "int4" else None
         # steps that do not cross a chunk boundary replay one captured CUDA graph (all indices come from device
         # counters, so the launch sequence is the same every step); boundary steps (1 in ``chunk``) run eagerly
         self.cuda_graph = cuda_graph
@@ -136,13 +196,9 @@ class KsaInferenceEngine:
         self.layer_caches: List[object] = []
         self.specs: List[Optional[CacheSpec]] = []
         for layer in model.layers:
-            if layer.is_summary_layer:
-                spec = CacheSpec(self.C, self.S, layer.window_chunks, max_len // self.C + 1)
-                self.specs.append(spec)
-                self.layer_caches.append(KsaLayerCache(spec, batch, Hkv, Dh, self.dtype, self.device))
-            else:
-                self.specs.append(None)
-                self.layer_caches.append(FullLayerCache(max_len, batch, Hkv, Dh, self.dtype, self.device))
+            spec = CacheSpec(self.C, self.S, layer.window_chunks, max_len // self.C + 1) if layer.is_summary_layer else None
+            self.specs.append(spec)
+            self.layer_caches.append(layer_cache(kv_cache, spec, max_len, batch, Hkv, Dh, self.dtype, self.device))
         self.state = CacheState(batch, self.device)
         self.host_len = [0] * batch
         self._boundary_dev = torch.zeros(batch, dtype=torch.int32, device=self.device)
@@ -158,22 +214,18 @@ class KsaInferenceEngine:
         cfg = self.cfg
         Hkv, Dh = cfg.num_kv_heads, cfg.head_dim
         for li, old in enumerate(self.layer_caches):
-            if self.specs[li] is not None:
-                sp = self.specs[li]
-                spec = CacheSpec(sp.chunk, sp.n_sum, sp.window, max_len // self.C + 1)
-                new = KsaLayerCache(spec, self.batch, Hkv, Dh, self.dtype, self.device)
-                self.specs[li] = spec
-            else:
-                new = FullLayerCache(max_len, self.batch, Hkv, Dh, self.dtype, self.device)
-            cap = old.k.shape[2]
-            new.k[:, :, :cap] = old.k
-            new.v[:, :, :cap] = old.v
+            sp = self.specs[li]
+            if sp is not None:
+                self.specs[li] = CacheSpec(sp.chunk, sp.n_sum, sp.window, max_len // self.C + 1)
+            new = layer_cache(self.kv_cache, self.specs[li], max_len, self.batch, Hkv, Dh, self.dtype, self.device)
+            for to, was in zip(cache_tensors(new), cache_tensors(old)):
+                to[:, :, :was.shape[2]] = was
             self.layer_caches[li] = new
         self.max_len = max_len
         self._graphs = {}
 
     def cache_bytes(self) -> int:
-        return sum(c.k.numel() * c.k.element_size() * 2 for c in self.layer_caches)
+        return sum(t.numel() * t.element_size() for c in self.layer_caches for t in cache_tensors(c))
 
     # ------------------------------------------------------------------ prefill
     @torch.no_grad()
@@ -228,8 +280,34 @@ class KsaInferenceEngine:
                 for i, r in enumerate(rows):
                     dst[r, :, slots] = src[i].transpose(0, 1)
 
+        def put_int4(cache, k, v, slots):
+            """``k`` / ``v`` ``[B, n, H, D]`` -> slots ``[n]`` of every sequence."""
+            slots = slots.expand(B, -1).contiguous()
+            if contiguous:
+                ops.int4_cache_write(cache.data.rows(sel), k, v, slots, distinct=True)
+            else:
+                for i, r in enumerate(rows):
+                    ops.int4_cache_write(cache.data.rows(slice(r, r + 1)), k[i:i + 1], v[i:i + 1], slots[i:i + 1], distinct=True)
+
+        places = {}      # layers with the same cache geometry share the rows' slots
+
+        def sink_int4(cache, spec, qkv):
+            key = None if spec is None else (spec.chunk, spec.n_sum, spec.window)
+            if key not in places:
+                places[key] = prompt_slots(spec, L, qkv.device)
+            first, slots = places[key]
+            text = qkv[:B * L, Hq * Dh:].view(B, L, 2 * Hkv, Dh)[:, first:]
+            if first < L:
+                put_int4(cache, text[:, :, :Hkv], text[:, :, Hkv:], slots)
+            if spec is not None and Ns > 0:
+                sums = qkv[B * L:, Hq * Dh:].view(B, Ns, 2 * Hkv, Dh)
+                put_int4(cache, sums[:, :, :Hkv], sums[:, :, Hkv:], spec.sum0 + torch.arange(Ns, dtype=torch.int32, device=qkv.device))
+
         def sink(layer_idx, qkv, is_summary_layer):
             cache = self.layer_caches[layer_idx]
+            if isinstance(cache, Int4LayerCache):
+                sink_int4(cache, self.specs[layer_idx] if is_summary_layer else None, qkv)
+                return
             if contiguous and _cache_fill(qkv, cache.k[sel], cache.v[sel], B, L, Ns if is_summary_layer else 0, Hq, Hkv, Dh,
                                           self.specs[layer_idx] if is_summary_layer else None):
                 return
@@ -307,10 +385,18 @@ class KsaInferenceEngine:
 
     def _logits(self, hidden: torch.Tensor) -> torch.Tensor:
         model, tp = self.model, getattr(self.model, "tp", None)
+        if self._int4_head is not None:
+            return ops.int4_linear(hidden, self._int4_head)
         logits = ops.linear(hidden, model.lm_head_weight)
         if tp is not None and logits.shape[-1] != self.cfg.vocab_size:
             logits = tp.gather_logits(logits)
         return logits
+
+    @staticmethod
+    def _mlp(layer, w4, h, tp):
+        if w4 is None:
+            return layer.mlp(h, tp)
+        return ops.int4_linear(ops.int4_linear_swiglu(h, w4.w13), w4.w2)
 
     def _decode_impl(self, tokens: torch.Tensor, any_boundary: bool, with_head: bool = True) -> torch.Tensor:
         """Device work of one decode step (launches only; the host mirror of the lengths is advanced by the caller).
@@ -357,10 +443,13 @@ class KsaInferenceEngine:
         full_len = None     # slice lengths of the full-attention layers
         slices_of = {}      # layers with the same cache geometry share the step's slot / slice tensors
         # ordinary steps without tensor parallelism: residual add + norm live inside the projection that follows them
-        fuse_norm = tp is None and not any_boundary and B <= 4
+        fuse_norm = tp is None and not any_boundary and B <= 4 and self._int4 is None
+        if self._int4 is not None and tp is not None:
+            raise ValueError("weights in four bits are not available with tensor parallelism")
         for li, layer in enumerate(model.layers):
             a = layer.attn
             cache = self.layer_caches[li]
+            w4 = self._int4[li] if self._int4 is not None else None
             if fuse_norm:
                 x, qkv = ops.norm_linear(x, delta, layer.sa_norm.scale, cfg.norm_eps, a.wqkv.weight)
                 h = None
@@ -373,10 +462,13 @@ class KsaInferenceEngine:
                 elif any_boundary:
                     if layer.sa_norm_summary is not None:
                         h = torch.cat([h[:B], ops.rms_norm(x[B:], layer.sa_norm_summary.scale, cfg.norm_eps)])
-                    w_s = a.wqkv_summary.weight if a.wqkv_summary is not None else a.wqkv.weight
-                    qkv = ops.dual_linear(h, a.wqkv.weight, w_s, B)
+                    if w4 is not None:
+                        qkv = torch.cat([ops.int4_linear(h[:B], w4.qkv), ops.int4_linear(h[B:], w4.qkv_summary)])
+                    else:
+                        w_s = a.wqkv_summary.weight if a.wqkv_summary is not None else a.wqkv.weight
+                        qkv = ops.dual_linear(h, a.wqkv.weight, w_s, B)
                 else:
-                    qkv = ops.linear(h, a.wqkv.weight)
+                    qkv = ops.int4_linear(h, w4.qkv) if w4 is not None else ops.linear(h, a.wqkv.weight)
                 skey = (spec.chunk, spec.n_sum, spec.window, spec.max_chunks)
                 if skey not in slices_of:
                     slot_t, start_t, len_t = _step_slices(spec, st)
@@ -385,9 +477,7 @@ class KsaInferenceEngine:
                                        len_t.view(B, 1).to(torch.int32).contiguous(), start_t, len_t)
                 slot_t1, start_t1, len_t1, start_t, len_t = slices_of[skey]
                 # norm + rotation of q / k, and the text tokens' K / V go into the cache in the same kernel
-                qkv = ops.qk_norm_rope_decode(qkv, a._norm_w(a.q_norm), a._norm_w(a.k_norm), pos_all, Hq, Hkv, Dh,
-                                              cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama", cache.k, cache.v,
-                                              slot_t1)
+                qkv = _rotate_and_append(cache, qkv, a, pos_all, cfg, slot_t1)
                 q_t = qkv[:B, :Hq * Dh].view(B, 1, Hq, Dh)
                 if any_boundary:
                     slot_s, start_s, len_s = summary_step_slices(spec, B, dev)
@@ -395,44 +485,39 @@ class KsaInferenceEngine:
                     q_s = qkv[B:, :Hq * Dh].view(B, S, Hq, Dh)
                     k_s = qkv[B:, Hq * Dh:(Hq + Hkv) * Dh].view(B, S, Hkv, Dh)
                     v_s = qkv[B:, (Hq + Hkv) * Dh:].view(B, S, Hkv, Dh)
-                    _cache_append(k_s, v_s, cache.k, cache.v, off)
+                    _append(cache, k_s, v_s, off)
                     q_all = torch.cat([q_t, q_s], dim=1)
                     starts = torch.cat([start_t.view(B, 1), start_s], dim=1).to(torch.int32)
                     lens = torch.cat([len_t.view(B, 1), len_s * boundary[:, None]], dim=1).to(torch.int32)
-                    att = _decode_attention(q_all, cache.k, cache.v, starts, lens, scale,
-                                            self._merge_counters)                             # [B, 1+S, Hq, Dh]
+                    att = _attend(cache, q_all, starts, lens, scale, self._merge_counters)    # [B, 1+S, Hq, Dh]
                     att = torch.cat([att[:, 0].reshape(B, Hq * Dh), att[:, 1:].reshape(B * S, Hq * Dh)], dim=0)
                     # flush: chunk text -> ring, scratch summaries -> summary region (boundary sequences only)
                     src_t, dst_t, src_s, dst_s = flush_plan(spec, st)
                     if spec.window > 0:
-                        _cache_move(cache.k, cache.v, src_t, dst_t, boundary, C)
-                    _cache_move(cache.k, cache.v, src_s, dst_s, boundary, S)
+                        _move(cache, src_t, dst_t, boundary, C)
+                    _move(cache, src_s, dst_s, boundary, S)
                 else:
-                    att = _decode_attention(q_t, cache.k, cache.v, start_t1, len_t1, scale,
-                                            self._merge_counters).reshape(B, Hq * Dh)
-                attn_out = _row_linear(tp, att, a.output_proj.weight)
+                    att = _attend(cache, q_t, start_t1, len_t1, scale, self._merge_counters).reshape(B, Hq * Dh)
+                attn_out = ops.int4_linear(att, w4.out) if w4 is not None else _row_linear(tp, att, a.output_proj.weight)
                 if fuse_norm:
                     x, delta = layer.mlp.forward_after_norm(x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
                 else:
                     x, h2 = _add_norm(tp, x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
-                    delta = layer.mlp(h2, tp)
+                    delta = self._mlp(layer, w4, h2, tp)
             else:
                 if not fuse_norm:
-                    qkv = ops.linear(h[:B], a.wqkv.weight)
-                qkv = ops.qk_norm_rope_decode(qkv, a._norm_w(a.q_norm), a._norm_w(a.k_norm), pos_all[:B], Hq, Hkv, Dh,
-                                              cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama", cache.k, cache.v,
-                                              st.text_len)
+                    qkv = ops.int4_linear(h[:B], w4.qkv) if w4 is not None else ops.linear(h[:B], a.wqkv.weight)
+                qkv = _rotate_and_append(cache, qkv, a, pos_all[:B], cfg, st.text_len)
                 q_t = qkv[:, :Hq * Dh].view(B, 1, Hq, Dh)
                 if full_len is None:
                     full_len = (st.text_len + 1).view(B, 1).to(torch.int32)
-                att = _decode_attention(q_t, cache.k, cache.v, self._zero_starts, full_len, scale,
-                                        self._merge_counters).reshape(B, Hq * Dh)
-                attn_out = _row_linear(tp, att, a.output_proj.weight)
+                att = _attend(cache, q_t, self._zero_starts, full_len, scale, self._merge_counters).reshape(B, Hq * Dh)
+                attn_out = ops.int4_linear(att, w4.out) if w4 is not None else _row_linear(tp, att, a.output_proj.weight)
                 if fuse_norm:
                     x, delta = layer.mlp.forward_after_norm(x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
                 else:
                     x, h2 = _add_norm(tp, x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
-                    delta = layer.mlp(h2[:B], tp)
+                    delta = self._mlp(layer, w4, h2[:B], tp)
         if fuse_norm and with_head:
             out = ops.norm_linear(x, delta, model.norm.scale, cfg.norm_eps, model.lm_head_weight)[1]
         else:

@@ -591,10 +591,18 @@ def norm_linear(x: torch.Tensor, delta: Optional[torch.Tensor], norm_w: torch.Te
 
 def qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor],
                         pos: torch.Tensor, Hq: int, Hkv: int, D: int, theta: float, eps: float, interleaved: bool,
-                        k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+                        k_cache: Optional[torch.Tensor] = None, v_cache: Optional[torch.Tensor] = None,
+                        slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``qk_norm_rope_packed`` for the few rows of a decode step, with the cache append in the same kernel: the new K
     and V of row ``i < len(slots)`` (sequence ``i``) also go to ``k_cache`` / ``v_cache`` ``[B, Hkv, cap, D]`` at slot
-    ``slots[i]`` (negative: not cached).  Inference only (no autograd)."""
+    ``slots[i]`` (negative: not cached); without a cache nothing else is written.  Inference only (no autograd)."""
+    if k_cache is None:
+        if not (_cuda(qkv) and D == 128 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1):
+            return qk_norm_rope_packed(qkv, q_w, k_w, pos, Hq, Hkv, D, theta, eps, interleaved)
+        out = torch.empty((qkv.shape[0], (Hq + 2 * Hkv) * D), dtype=qkv.dtype, device=qkv.device)
+        _lib.call("ksa_qknorm_rope_decode", qkv, out, q_w, k_w, pos.to(torch.int32), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, Hkv, D,
+                  float(theta), float(eps), int(interleaved), None, None, None, 0, 0)
+        return out
     n = slots.numel()
     if _cuda(qkv) and D == 128 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1:
         T = qkv.shape[0]
@@ -1188,13 +1196,13 @@ def adamw_step(master, grad, m, v, out_bf16, hyper, beta1, beta2, eps, weight_de
               float(weight_decay), float(clip_value), sumsq)
 
 
-from .int4 import (Int4Cache, Int4Weight, int4_cache, int4_cache_read, int4_cache_write, int4_decode_attention,  # noqa: E402
+from .int4 import (Int4Cache, Int4Weight, int4_cache, int4_cache_move, int4_cache_read, int4_cache_write, int4_decode_attention,  # noqa: E402
                    int4_dequantize_weight, int4_linear, int4_linear_swiglu, int4_quantize_weight)
 
 __all__ = [
     "gemm", "linear", "dual_linear", "attention_packed", "rms_norm", "add_rms_norm", "qk_norm_rope_packed", "qk_norm_rope_decode", "swiglu", "linear_swiglu", "norm_linear", "embedding",
     "ksa_attention", "causal_attention", "linear_cross_entropy", "adamw_step", "UNBOUNDED_WINDOW",
     "SummaryLayout", "get_layout",
-    "Int4Cache", "Int4Weight", "int4_cache", "int4_cache_read", "int4_cache_write", "int4_decode_attention", "int4_dequantize_weight",
+    "Int4Cache", "Int4Weight", "int4_cache", "int4_cache_move", "int4_cache_read", "int4_cache_write", "int4_decode_attention", "int4_dequantize_weight",
     "int4_linear", "int4_linear_swiglu", "int4_quantize_weight",
 ]

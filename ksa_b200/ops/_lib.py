@@ -66,6 +66,7 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_kv_cache_move": [P] * 5 + [I] * 5 + [P],
     "ksa_int4_cache_write": [P] * 8 + [I] * 5 + [L, L, L, I, P],
     "ksa_int4_cache_read": [P] * 7 + [I] * 5 + [P],
+    "ksa_int4_cache_move": [P] * 7 + [I] * 5 + [P],
     "ksa_int4_decode_attn": [P] * 9 + [I] * 6 + [L, L, L, F, P],
     "ksa_int4_weight": [P, P, P, I, I, I, L, I, P],
     "ksa_int4_weight_values": [P, P, P, I, I, I, I, P],
@@ -192,8 +193,7 @@ def _address(x: torch.Tensor) -> int:
 
 
 # kernels launched by one call of an entry point (default 1)
-_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2,
-                     "ksa_int4_decode_attn": 2}
+_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2}
 _launch_count = 0
 
 

@@ -168,6 +168,23 @@ def int4_cache_read(cache: Int4Cache, start: torch.Tensor, rows: int) -> Tuple[t
     return out[0], out[1]
 
 
+def int4_cache_move(cache: Int4Cache, src: torch.Tensor, dst: torch.Tensor, enable: torch.Tensor, rows: int) -> None:
+    """Slots ``src[b] .. src[b] + rows`` go to ``dst[b] .. dst[b] + rows`` in the sequences with ``enable[b] != 0`` (all ``[B]``), as they
+    are; slots outside the cache are left out.  The two ranges of a sequence must not overlap.  Head dims in multiples of 64."""
+    B, H, cap, D = _check_cache(cache)
+    _require(rows >= 0 and D % 64 == 0, f"{rows} rows of heads of {D} (a multiple of 64 is moved)")
+    src, dst, enable = (_int32(x, (B,), cache.k.device, n) for x, n in ((src, "src"), (dst, "dst"), (enable, "enable")))
+    if not cache.k.is_cuda:
+        for b, (s, d, on) in enumerate(zip(src.tolist(), dst.tolist(), enable.tolist())):
+            lo, hi = max(0, -s, -d), min(rows, cap - s, cap - d)
+            if on and hi > lo:
+                for t in cache:
+                    t[b, :, d + lo:d + hi] = t[b, :, s + lo:s + hi].clone()
+        return
+    with _on(cache.k):
+        _lib.call("ksa_int4_cache_move", cache.k, cache.k_scale, cache.v, cache.v_scale, src, dst, enable, B, H, D, cap, rows)
+
+
 def int4_decode_attention(q: torch.Tensor, cache: Int4Cache, start: torch.Tensor, length: torch.Tensor,
                           scale: Optional[float] = None) -> torch.Tensor:
     """``q`` ``[B, Tq, Hq, D]``: query ``(b, t)`` attends slots ``start[b, t] .. start[b, t] + length[b, t]`` of sequence ``b``, cut to the
@@ -301,5 +318,5 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
     return out.view(out_shape)
 
 
-__all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_cache_read", "int4_decode_attention",
+__all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_cache_read", "int4_cache_move", "int4_decode_attention",
            "int4_quantize_weight", "int4_dequantize_weight", "int4_linear", "int4_linear_swiglu"]

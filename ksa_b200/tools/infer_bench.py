@@ -48,6 +48,9 @@ def main(argv=None) -> None:
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--warmup-decode", type=int, default=8)
     ap.add_argument("--no-warmup-prefill", action="store_true")
+    ap.add_argument("--kv-cache", default="bf16", choices=["bf16", "int4"], help="int4: keys and values in four bits, quantised as they are written")
+    ap.add_argument("--weights", default="bf16", choices=["bf16", "int4"],
+                    help="int4: decode steps read projections and output head in four bits (one GPU)")
     ap.add_argument("--tp-two-phase-min", type=int, default=None,
                     help="smallest group that uses the reduce-scatter + gather form for prefill (default 3)")
     ap.add_argument("--tp-separate-gather", action="store_true",
@@ -88,7 +91,7 @@ def main(argv=None) -> None:
         if model.output is not None and cfg.vocab_size % world == 0:     # vocabulary-parallel head
             n = cfg.vocab_size // world
             model.output.weight = torch.nn.Parameter(model.output.weight[rank * n:(rank + 1) * n].clone())
-    eng = KsaInferenceEngine(model, max_len=L + a.decode + a.warmup_decode + C, batch=B)
+    eng = KsaInferenceEngine(model, max_len=L + a.decode + a.warmup_decode + C, batch=B, kv_cache=a.kv_cache, weights=a.weights)
     g = torch.Generator().manual_seed(1)
     prompt = torch.randint(0, min(cfg.vocab_size, 150000), (B, L), generator=g).to(dev)
 
@@ -128,6 +131,7 @@ def main(argv=None) -> None:
         steps = max(a.decode, 1)
         print(json.dumps({
             "model": a.preset, "tp": world, "batch": B, "prompt_len": L, "decode_steps": a.decode, "dtype": "bf16",
+            "kv_cache": a.kv_cache, "weights": a.weights,
             "tp_prefill": (None if tp is None else
                            {"two_phase": bool(tp.two_phase_rows), "fused_gather": tp.fused_gather,
                             "push_partials": tp.push_partials}),
