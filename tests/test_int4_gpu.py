@@ -344,6 +344,19 @@ def test_linear_swiglu(F, K, group):
     _lib.check_status()
 
 
+@pytest.mark.parametrize("N,K", [(5, 160), (777, 1280), (33000, 2048)])
+def test_linear_in_blocks_and_with_values(N, K):
+    """Rows on both sides of the rules: up to 32 or 80 in blocks, the last of them of one row, of a few, or whole."""
+    w = ops.int4_quantize_weight((_randn(N, K, seed=N) * 0.05).bfloat16(), 32)
+    for M in (17, 32, 33, 65, 80, 81):
+        x = _randn(M, K + 8, seed=M)[:, :K]
+        y = ops.int4_linear(x, w)
+        _check_linear(y, x, w)
+        if M <= 32:
+            assert torch.equal(y, torch.cat([ops.int4_linear(part, w) for part in x.split(16)]))
+    _lib.check_status()
+
+
 def test_linear_rows_of_any_layout():
     N, K = 200, 256
     w = ops.int4_quantize_weight(_randn(N, K, seed=1))
