@@ -10,6 +10,8 @@
 //     leave them in shared memory; two more warps add the sums up and write the results while the others are at the next pass;
 //   * mma.sync m16n8k16 multiplies 16 weight rows by 8 activation rows; a lane's 16 bytes of a weight row are columns 32 t .. 32 t + 31 of the segment, in
 //     that order for the activations as well.  Activations that several passes want stay in shared memory, others are read as they are needed.
+#include "int4_linear.h"
+
 #include "host.h"
 #include "int4.cuh"
 
@@ -20,6 +22,11 @@ constexpr int kI4LAdders = 2;                       // that add up and write
 constexpr int kI4LThreads = (kI4LWarps + kI4LAdders + 1) * 32;
 constexpr int kI4LBlocks = 2;                       // blocks of 16 weight rows of a warp
 constexpr int kI4LMostStages = 12;
+constexpr int kI4LMostRows = 16;
+// Nine rows and more of a large weight go to int4_linear_wide.cu: from 192 weight rows a CTA and 2048 columns.  Measured on 16 rows, this kernel against
+// that one: [19456, 2560] 17.8 us against 18.6, [28416, 2560] 22.2 against 19.1, [37888, 4096] 35.6 against 25.7, [151936, 2560] 71 against 60, but
+// [40000, 1024] 14.8 against 16.6, [100000, 512] 20.1 against 23.8; on one row [151936, 2560] 52 against 59.
+constexpr int kI4LWideRows = 192, kI4LWideColumns = 2048;
 constexpr int kI4LSmemMost = 227 * 1024;
 
 struct Int4Linear {
@@ -317,19 +324,23 @@ static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) 
 
 using namespace ksa;
 
-// A [M <= 16, K] (row pitch lda), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc); glu: gate rows and then up rows, C [M, N / 2].
+// A [M <= 64, K] (row pitch lda; M <= 16 with glu), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc); glu: gate rows and then up rows, C [M, N / 2].
 KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
                             long long ldc, int glu, void* stream) {
   KSA_ENTER(A);
-  KSA_REQUIRE(M >= 0 && M <= 16, "int4_linear: %d rows (at most 16)", M);
+  KSA_REQUIRE(M >= 0 && M <= (glu ? kI4LMostRows : kI4WMostRows), "int4_linear: %d rows (at most %d)", M, glu ? kI4LMostRows : kI4WMostRows);
   KSA_REQUIRE(group == 32 || group == 64 || group == 128, "int4_linear: groups of %d values (32, 64 or 128)", group);
   KSA_REQUIRE(K > 0 && K % group == 0 && N >= 0 && pitch >= N && pitch % 4 == 0, "int4_linear: K %d is no multiple of the group of %d", K, group);
   KSA_REQUIRE(!glu || N % 2 == 0, "int4_linear: gate and up rows must be as many, got %d together", N);
   KSA_REQUIRE(lda % 8 == 0 && ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(meta)) & 15) == 0,
               "int4_linear: rows, codes and scales must be 16-byte aligned");
   if (M == 0 || N == 0) return 0;
+  const bool spread = M > 1 && lda < K;                                      // rows that lie in one another
+  KSA_REQUIRE(M <= kI4LMostRows || !spread, "int4_linear: %d rows at a pitch of %lld for %d values", M, lda, K);
   const int sms = sm_count();
   KSA_REQUIRE(sms > 0, "int4_linear: no device");
+  if (!glu && !spread && (M > kI4LMostRows || (M > 8 && K >= kI4LWideColumns && N >= kI4LWideRows * sms)))
+    return int4_linear_wide(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, 0, reinterpret_cast<cudaStream_t>(stream));
   Int4Linear a{};
   a.A = (const bf16*)A; a.meta = (const uint32_t*)meta; a.C = (bf16*)C;
   a.lda = lda; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.group = group; a.pitch = pitch;

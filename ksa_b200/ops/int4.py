@@ -23,7 +23,8 @@ from ._lib import native as _native
 CACHE_GROUP = 32          # values of a cache row that share a scale
 CACHE_DIM = 2048          # largest head dimension
 CACHE_SLOTS = 16          # the capacity of a cache is a multiple of this
-FEW_ROWS = 16             # rows that the kernel of ``int4_linear`` takes
+FEW_ROWS = 32             # rows that the kernels of ``int4_linear`` take
+FUSED_ROWS = 16           # and that of ``int4_linear_swiglu``
 _TABLE_ROWS = 64          # rows of a sequence from which a write finds the last row of each slot in a table
 
 
@@ -273,8 +274,8 @@ def _weight_values(weight: Int4Weight, out: torch.Tensor) -> None:
 
 
 def int4_linear(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
-    """``x @ W.T`` for ``x`` ``[..., K]`` and ``W = int4_dequantize_weight(weight)``.  At most 16 rows (a decode step) read the codes
-    once, some more in blocks of 16; many rows multiply with the bf16 values, written out for the call."""
+    """``x @ W.T`` for ``x`` ``[..., K]`` and ``W = int4_dequantize_weight(weight)``.  At most 32 rows (a decode step) read the codes
+    once, some more in blocks of 32; many rows multiply with the bf16 values, written out for the call."""
     return _linear(x, weight, False)
 
 
@@ -284,11 +285,12 @@ def int4_linear_swiglu(x: torch.Tensor, w13: Int4Weight) -> torch.Tensor:
 
 
 def _block_rows(N: int, K: int) -> int:
-    """Rows up to which blocks of 16 read the codes, once each.  More rows multiply with the bf16 values, written out for the call, at a
-    cost that hardly depends on them.  Measured, values against blocks: ``[2560, 9728]`` 25.3 us against 23.9 for 32 rows, 25.5 against
-    34.8 for 48; ``[4096, 4096]`` 17.8 against 15.2 and 19.8 against 22.5; ``[19456, 2560]`` 51.4 against 34.6 and 52.1 against 51.2.
-    Values that outgrow the L2 cache come from memory again: ``[151936, 2560]`` 372 us against 361 for 80 rows, 374 against 430 for 96."""
-    return 80 if 2 * N * K > 126 << 20 else 32
+    """Rows up to which blocks of ``FEW_ROWS`` read the codes, once each.  More rows multiply with the bf16 values, written out for the call, at
+    a cost that hardly depends on them.  Measured, values against blocks: a weight of ``[1280, 1280]`` 6.5 us against 10.0 for 32 rows,
+    ``[2560, 4096]`` 13.7 against 10.5, ``[2560, 9728]`` 25.3 against 14.2, for 33 rows 13.8 against 15.5 and 25.5 against 22.3; what nearly fills
+    the L2 cache, ``[19456, 2560]``, 51.7 against 35.8 for 33 rows, 55 against 45 for 64, 55 against 62 for 80; values that outgrow it,
+    ``[151936, 2560]``, 378 against 332 for 128 rows."""
+    return FUSED_ROWS if N * K <= 4 << 20 else 32 if 2 * N * K <= 64 << 20 else 64 if 2 * N * K <= 126 << 20 else 128
 
 
 def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
@@ -306,6 +308,11 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
     if x.dtype != torch.bfloat16:
         raise TypeError(f"the sm_100a kernels take bf16 activations, got {x.dtype}")
     M, out_shape = x.numel() // K, (*x.shape[:-1], N // 2 if glu else N)
+    if glu and FUSED_ROWS < M <= _block_rows(N, K):
+        from . import swiglu
+        y = _linear(x.reshape(M, K), weight, False)
+        with _on(x):
+            return (swiglu(y) if N % 16 == 0 else ref.swiglu(y)).view(out_shape)
     if M > _block_rows(N, K):
         from . import linear, swiglu
         values = torch.empty((-(-N // 8) * 8, K), dtype=torch.bfloat16, device=x.device)       # the products take columns in eights
@@ -318,7 +325,7 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
                 y = swiglu(y) if N % 16 == 0 else ref.swiglu(torch.cat([gate, up], -1))
         return (y if glu or N % 8 == 0 else y[:, :N].contiguous()).view(out_shape)
     rows = x.reshape(M, K)
-    if M > 0 and (rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.data_ptr() % 16 != 0):
+    if M > 0 and (rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0):
         rows = rows.clone(memory_format=torch.contiguous_format)
     out = torch.empty((M, out_shape[-1]), dtype=x.dtype, device=x.device)
     with _on(x):

@@ -344,16 +344,15 @@ def test_linear_swiglu(F, K, group):
     _lib.check_status()
 
 
-@pytest.mark.parametrize("N,K", [(5, 160), (777, 1280), (33000, 2048)])
+@pytest.mark.parametrize("N,K", [(5, 160), (777, 1280), (2500, 2304), (33001, 2080)])
 def test_linear_in_blocks_and_with_values(N, K):
-    """Rows on both sides of the rules: up to 32 or 80 in blocks, the last of them of one row, of a few, or whole."""
+    """Rows on both sides of the rules: up to 32 in one launch, more in blocks of 32 or with the values written out, and the same bits each time."""
     w = ops.int4_quantize_weight((_randn(N, K, seed=N) * 0.05).bfloat16(), 32)
-    for M in (17, 32, 33, 65, 80, 81):
+    for M in (9, 16, 17, 32, 33, 65, 80, 129):
         x = _randn(M, K + 8, seed=M)[:, :K]
         y = ops.int4_linear(x, w)
         _check_linear(y, x, w)
-        if M <= 32:
-            assert torch.equal(y, torch.cat([ops.int4_linear(part, w) for part in x.split(16)]))
+        assert torch.equal(y, ops.int4_linear(x, w))
     _lib.check_status()
 
 
