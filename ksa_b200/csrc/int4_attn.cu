@@ -5,8 +5,8 @@
 //   * all (slice, KV head) items in a row are one sequence of tiles of 32 slots, and every CTA takes an equal run of it, whatever the
 //     slices' lengths are (they are known on the device only).  A run that covers part of an item leaves (max, sum, output) behind, and a
 //     second kernel merges the parts of an item in a fixed order; an item within one run is finished there;
-//   * each warp keeps tiles in flight through a ring of its own, filled by bulk copies (a tile is contiguous: 2 KB of codes and 512 bytes of
-//     scales for K and for V), so no warp waits for another before the end of an item's run;
+//   * a warp of its own keeps tiles in flight through a ring, four at a time (a tile is contiguous: 2 KB of codes and 512 bytes of scales for K and for
+//     V, and up to four of one item are one bulk copy each), and four warps take one tile of every group of four;
 //   * both products are mma.sync m16n8k16 with the values straight from their codes (int4.cuh) as an operand.  A lane's four words of a key
 //     are values 32 t .. 32 t + 31 of it, one group with one scale; the order of the head dimension in the product is q's as well, so nothing is
 //     moved.  Keys are the 16 rows of the first product and value dimensions those of the second, queries the 8 columns of both, so up to

@@ -783,7 +783,7 @@ PyObject* py_int4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (!a.ok() || !packed2d(w) || s->dim() != 3 || !s->is_contiguous() || !aligned(w) || !aligned(s) || x->dim() < 1) return none();
   const long long N = w->size(0), K = 2 * w->size(1), groups = s->size(0), pitch = s->size(1), M = x->numel() / K;
   if (K != x->size(-1) || M > (glu || N * K <= 4 << 20 ? 16 : 32) || !fits(N) || !fits(K) || pitch != (N + 3) / 4 * 4 || s->size(2) != 2 || K % groups != 0 ||
-      (K / groups != 32 && K / groups != 64 && K / groups != 128) || !(x->is_contiguous() || (x->dim() == 2 && eights(x))) || !aligned(x) ||
+      (K / groups != 32 && K / groups != 64 && K / groups != 128) || !(x->is_contiguous() || (x->dim() == 2 && eights(x) && (M <= 16 || x->stride(0) >= K))) || !aligned(x) ||
       (glu && N % 2 != 0) || differentiated({x}))
     return none();
   const long long out = glu ? N / 2 : N;

@@ -360,11 +360,17 @@ def test_linear_rows_of_any_layout():
     N, K = 200, 256
     w = ops.int4_quantize_weight(_randn(N, K, seed=1))
     for x in (_randn(4, 3 * K, seed=2)[:, K:2 * K], _randn(K, 5, seed=3).t(), _randn(2, 3, K, seed=4), _randn(6 * K + 1, seed=5)[1:].view(6, K),
-              _randn(1, K, seed=6).expand(7, K), _randn(K, seed=7)):
+              _randn(1, K, seed=6).expand(7, K), _randn(1, K, seed=6).expand(30, K), _randn(K, seed=7)):
         y = ops.int4_linear(x, w)
         assert y.shape == (*x.shape[:-1], N)
         _check_linear(y, x, w)
     assert ops.int4_linear(_randn(0, K), w).shape == (0, N)
+    w = ops.int4_quantize_weight(_randn(3000, 1536, seed=8))               # more than 16 rows of it go in one launch
+    for x in (_randn(20, 2000, seed=2)[:, 64:1600], _randn(1536, 17, seed=3).t(), _randn(2, 3, 4, 1536, seed=4), _randn(1, 1536, seed=6).expand(30, 1536),
+              _randn(24 * 768 + 1536, seed=9).as_strided((24, 1536), (768, 1))):
+        y = ops.int4_linear(x, w)
+        assert y.shape == (*x.shape[:-1], 3000)
+        _check_linear(y, x, w)
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
