@@ -177,38 +177,38 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
   } else if (warp >= kI4WIssuers) {
     // ---------------------------------------------------------------- the warps that multiply: 128 weight rows x activation rows, 16 columns at a time
     const int group = warp - kI4WIssuers;
-    const uint32_t idesc = umma_idesc_bf16(128, a.cols, 0, 0), slots = tmem + group * kI4WSlots * 64;
-    const uint64_t x_desc = smem_desc_kmajor_sw128(smem_u32(a.keep ? kept : ring + a.b_at)), panel16 = panel >> 4;
-    int half = group & 1, stage = group >> 1, k = stage, slot = 0, set = 0, taken = 0;      // half `half` of step `k` of a pass
-    uint32_t phase = 0, slot_phase = 0, accumulate = 0;
+    const uint32_t idesc = umma_idesc_bf16(128, a.cols, 0, 0), panel16 = panel >> 4, stage16 = a.stage_bytes >> 4;
+    const uint64_t x_desc = smem_desc_kmajor_sw128(smem_u32(a.keep ? kept : ring + a.b_at));
+    uint64_t *my_full = slot_full + group * kI4WSlots, *my_empty = slot_empty + group * kI4WSlots;
+    int half = group & 1, stage = group >> 1, k = stage, slot = 0, set = 0;             // half `half` of step `k` of a pass
+    uint32_t phase = 0, slot_phase = 0, accumulate = 0, sums_phase = 1;
     bool ok = !a.keep || __all_sync(0xffffffffu, mbar_wait(x_full, 0, guard, kTimeoutTmaFull));
     int left = total - stage;
-    while (k >= count) k -= count;
+    for (; k >= count; k -= count) {}
     while (ok && left > 0) {
-      if (accumulate == 0 && taken >= sets)
-        ok = __all_sync(0xffffffffu, mbar_wait(&sums_empty[group * 2 + set], (taken / sets - 1) & 1, guard, kTimeoutAccEmpty));
-      if (ok && !a.keep) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&slot_full[group * kI4WSlots + slot], slot_phase, guard, kTimeoutSoftmax));
+      const bool last = k + 1 + half >= count;                       // of this group in the pass
+      const uint64_t desc = x_desc + (a.keep ? k * 4 * panel16 : stage * stage16) + half * 2 * panel16;
+      const uint32_t sums = tmem + kI4WSums + (group * sets + set) * a.cols, from = tmem + (group * kI4WSlots + slot) * 64;
+      if (accumulate == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sums_empty[group * 2 + set], sums_phase, guard, kTimeoutAccEmpty));
+      if (!a.keep) ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&my_full[slot], slot_phase, guard, kTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
-      const bool last = k + 1 + half >= count;                       // of this group in the pass
-      const uint64_t desc = x_desc + (uint32_t)(a.keep ? k * 4 * panel : stage * a.stage_bytes) / 16 + half * 2 * panel16;
-      const uint32_t sums = tmem + kI4WSums + (group * sets + set) * a.cols, from = slots + slot * 64;
       if (elect_one()) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) umma_ts(sums, from + e * 8, desc + (e >> 2) * panel16 + (e & 3) * 2, idesc, e == 0 ? accumulate : 1);
-        umma_commit(&slot_empty[group * kI4WSlots + slot]);
+        umma_commit(&my_empty[slot]);
         if (!a.keep) umma_commit(&empty[stage]);
         if (last) umma_commit(&sums_full[group * 2 + set]);
       }
       __syncwarp();
       accumulate = !last;
-      if (last) { ++taken; set = taken % sets; }
+      if (last && ++set == sets) { set = 0; sums_phase ^= 1; }
       if (++slot == kI4WSlots) { slot = 0; slot_phase ^= 1; }
       const int ahead = 1 + half;
       half ^= 1;
       left -= ahead;
-      for (k += ahead; k >= count;) k -= count;
+      for (k += ahead; k >= count; k -= count) {}
       if ((stage += ahead) >= a.stages) { stage -= a.stages; phase ^= 1; }
     }
     if (elect_one()) umma_commit(ended);
