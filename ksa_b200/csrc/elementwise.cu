@@ -6,6 +6,7 @@
 // All of them move 16 bytes per thread per access and keep their statistics in fp32.
 #include "common.cuh"
 #include "host.h"
+#include "int4.cuh"
 
 #include "vec.cuh"
 
@@ -530,13 +531,35 @@ __global__ void __launch_bounds__(256) qknorm_rope_fwd128_kernel(QkRopeArgs a) {
 // and the new K / V rows of the first `cache_rows` rows written straight into the KV cache [B, Hkv, cap, 128] at
 // slots[row] (row = sequence; negative slot: not cached).
 struct QkRopeCacheArgs {
-  bf16* k_cache;
+  bf16* k_cache;               // kInt4: codes [B, Hkv, cap, 64 bytes]
   bf16* v_cache;
   const int* slots;
   int cache_rows, cap;
+  uint32_t *k_meta, *v_meta;   // kInt4: scales [B, Hkv, cap, 4]
 };
 
+// A head's 64 words, a pair of them in each lane, quantised into a row of a cache of four bits by lanes 0 .. 7.  One launch instead of two: a step's
+// rotation and write of one row of 32 + 8 heads 3.2 -> 2.0 us, of sixteen 3.4 -> 2.4.
 template <bool IL>
+__device__ __forceinline__ void rope_store_int4(uint32_t oa, uint32_t ob, int lane, uint2* codes, uint32_t* meta) {
+  const int j = lane & 7;
+  uint32_t x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int from = IL ? (j * 8 + i) / 2 : (j * 8 + i) & 31;
+    const uint32_t xa = __shfl_sync(0xffffffffu, oa, from), xb = __shfl_sync(0xffffffffu, ob, from);
+    x[i] = (IL ? i & 1 : j >= 4) ? xb : xa;
+  }
+  const uint4 raw[2] = {make_uint4(x[0], x[1], x[2], x[3]), make_uint4(x[4], x[5], x[6], x[7])};
+  uint2 words;
+  uint32_t m;
+  i4_quantize<kI4CacheGroup / 16>(raw, words, m);
+  if (lane >= 8) return;
+  codes[j] = words;
+  if (j % 2 == 0) meta[j / 2] = m;
+}
+
+template <bool IL, bool kInt4>
 __global__ void __launch_bounds__(256) qknorm_rope_decode128_kernel(QkRopeArgs a, QkRopeCacheArgs c) {
   grid_dependency_launch();
   grid_dependency_wait();
@@ -579,9 +602,14 @@ __global__ void __launch_bounds__(256) qknorm_rope_decode128_kernel(QkRopeArgs a
   dst[offB] = ob;
   if (head >= a.Hq && c.k_cache != nullptr && row < c.cache_rows) {
     const int slot = c.slots[row];
-    if (slot >= 0) {
+    if (slot >= 0 && (!kInt4 || slot < c.cap)) {
       const bool is_v = head >= H;
       const int kh = is_v ? head - H : head - a.Hq;
+      if (kInt4) {
+        const long long at = ((long long)row * a.Hkv + kh) * c.cap + slot;
+        rope_store_int4<IL>(oa, ob, lane, reinterpret_cast<uint2*>(is_v ? c.v_cache : c.k_cache) + at * 8, (is_v ? c.v_meta : c.k_meta) + at * 4);
+        return;
+      }
       uint32_t* cd = reinterpret_cast<uint32_t*>(is_v ? c.v_cache : c.k_cache) +
                      (((long long)row * a.Hkv + kh) * c.cap + slot) * 64;
       cd[offA] = oa;
@@ -919,14 +947,34 @@ KSA_API int ksa_qknorm_rope_decode(const void* qkv, void* out, const void* q_w, 
   if (rows == 0) return 0;
   QkRopeArgs a{(const bf16*)qkv, (bf16*)out, (const bf16*)q_w, (const bf16*)k_w, (const int*)pos, nullptr,
                in_stride, out_stride, rows, Hq, Hkv, D, log2f(theta), eps, interleaved, 1};
-  QkRopeCacheArgs c{(bf16*)k_cache, (bf16*)v_cache, (const int*)slots, cache_rows, cap};
+  QkRopeCacheArgs c{(bf16*)k_cache, (bf16*)v_cache, (const int*)slots, cache_rows, cap, nullptr, nullptr};
   const int warps = rows * (Hq + 2 * Hkv);
   if (interleaved)
-    KSA_CHECK_CUDA(launch_kernel(qknorm_rope_decode128_kernel<true>, dim3((warps + 7) / 8), dim3(256), 0, ST(stream), a,
+    KSA_CHECK_CUDA(launch_kernel(qknorm_rope_decode128_kernel<true, false>, dim3((warps + 7) / 8), dim3(256), 0, ST(stream), a,
                                  c));
   else
-    KSA_CHECK_CUDA(launch_kernel(qknorm_rope_decode128_kernel<false>, dim3((warps + 7) / 8), dim3(256), 0, ST(stream), a,
+    KSA_CHECK_CUDA(launch_kernel(qknorm_rope_decode128_kernel<false, false>, dim3((warps + 7) / 8), dim3(256), 0, ST(stream), a,
                                  c));
+  return 0;
+}
+
+// The same with K / V of rows [0, cache_rows) quantised into a cache of four bits (codes [B, Hkv, cap, 64], scales [B, Hkv, cap, 4] words) at slots[row]:
+// not those with a slot that is negative or past the cache.
+KSA_API int ksa_qknorm_rope_decode_int4(const void* qkv, void* out, const void* q_w, const void* k_w, const void* pos, long long in_stride,
+                                        long long out_stride, int rows, int Hq, int Hkv, int D, float theta, float eps, int interleaved,
+                                        void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* slots, int cache_rows, int cap,
+                                        void* stream) {
+  KSA_ENTER(qkv);
+  KSA_REQUIRE(D == 128, "qknorm_rope_decode_int4: head_dim %d unsupported (128)", D);
+  KSA_REQUIRE(cache_rows >= 0 && cache_rows <= rows && cap > 0, "qknorm_rope_decode_int4: %d rows for the cache of %d", cache_rows, rows);
+  KSA_REQUIRE(((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes)) & 7) == 0 &&
+              ((reinterpret_cast<uintptr_t>(k_meta) | reinterpret_cast<uintptr_t>(v_meta)) & 3) == 0, "qknorm_rope_decode_int4: misaligned cache");
+  if (rows == 0) return 0;
+  QkRopeArgs a{(const bf16*)qkv, (bf16*)out, (const bf16*)q_w, (const bf16*)k_w, (const int*)pos, nullptr,
+               in_stride, out_stride, rows, Hq, Hkv, D, log2f(theta), eps, interleaved, 1};
+  QkRopeCacheArgs c{(bf16*)k_codes, (bf16*)v_codes, (const int*)slots, cache_rows, cap, (uint32_t*)k_meta, (uint32_t*)v_meta};
+  auto kern = interleaved ? qknorm_rope_decode128_kernel<true, true> : qknorm_rope_decode128_kernel<false, true>;
+  KSA_CHECK_CUDA(launch_kernel(kern, dim3((rows * (Hq + 2 * Hkv) + 7) / 8), dim3(256), 0, ST(stream), a, c));
   return 0;
 }
 

@@ -442,7 +442,8 @@ int int4_linear_wide(const void* A, const void* codes, const void* meta, void* C
   a.stages = a.stages / 3 * 3;
   KSA_REQUIRE(a.stages >= 3, "int4_linear: no room for three stages");
   size_t smem = (size_t)a.stages * a.stage_bytes + rest;
-  if (smem < (size_t)kTmemClusterAlone) smem = kTmemClusterAlone;            // all of the tensor memory: alone on its SM
+  if (smem < (size_t)kTmemClusterAlone) smem = kTmemClusterAlone;            // all of the tensor memory: alone on its SM (host.h)
+  static_assert(kI4WSmemMost >= kTmemClusterAlone, "the limit raised above covers it");
   CUtensorMap tm, tm_meta, tm_x;
   {
     uint64_t dims[2] = {(uint64_t)K / 4, (uint64_t)N}, str[2] = {2, (uint64_t)K / 2};

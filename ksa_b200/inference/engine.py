@@ -140,11 +140,7 @@ def _rotate_and_append(cache, qkv, a, pos, cfg, slots):
     if not isinstance(cache, Int4LayerCache):
         return ops.qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, Hkv, Dh, cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama", cache.k,
                                        cache.v, slots)
-    qkv = ops.qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, Hkv, Dh, cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama")
-    n = slots.numel()
-    heads = qkv[:n, Hq * Dh:].view(n, 1, 2 * Hkv, Dh)
-    _append(cache, heads[:, :, :Hkv], heads[:, :, Hkv:], slots.view(n, 1))
-    return qkv
+    return ops.int4_qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, cfg.rope_base, cfg.norm_eps, cfg.rope_impl == "llama", cache.data, slots)
 
 
 class _Int4Layer:
@@ -462,7 +458,9 @@ class KsaInferenceEngine:
                 elif any_boundary:
                     if layer.sa_norm_summary is not None:
                         h = torch.cat([h[:B], ops.rms_norm(x[B:], layer.sa_norm_summary.scale, cfg.norm_eps)])
-                    if w4 is not None:
+                    if w4 is not None and w4.qkv_summary is w4.qkv:
+                        qkv = ops.int4_linear(h, w4.qkv)
+                    elif w4 is not None:
                         qkv = torch.cat([ops.int4_linear(h[:B], w4.qkv), ops.int4_linear(h[B:], w4.qkv_summary)])
                     else:
                         w_s = a.wqkv_summary.weight if a.wqkv_summary is not None else a.wqkv.weight

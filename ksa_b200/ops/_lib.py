@@ -40,6 +40,7 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_rmsnorm_bwd": [P, P, P, P, P, P, P, P, I, I, I, P],
     "ksa_qknorm_rope_fwd": [P, P, P, P, P, P, L, L, I, I, I, I, F, F, I, I, P],
     "ksa_qknorm_rope_decode": [P, P, P, P, P, L, L, I, I, I, I, F, F, I, P, P, P, I, I, P],
+    "ksa_qknorm_rope_decode_int4": [P, P, P, P, P, L, L, I, I, I, I, F, F, I, P, P, P, P, P, I, I, P],
     "ksa_qknorm_rope_bwd": [P, P, P, P, P, P, P, P, P, L, L, I, I, I, I, F, F, I, I, P],
     "ksa_swiglu_fwd": [P, P, L, I, P],
     "ksa_swiglu_bwd": [P, P, P, L, I, P],

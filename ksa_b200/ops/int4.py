@@ -148,6 +148,31 @@ def int4_cache_write(cache: Int4Cache, k_new: torch.Tensor, v_new: torch.Tensor,
                   k_new.stride(0), k_new.stride(1), k_new.stride(2), int(distinct))
 
 
+def int4_qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor], pos: torch.Tensor, Hq: int, theta: float,
+                             eps: float, interleaved: bool, cache: Int4Cache, slots: torch.Tensor) -> torch.Tensor:
+    """``ops.qk_norm_rope_decode`` of rows ``[q | k | v]`` whose keys and values go, quantised, into ``cache``: those of row ``i < len(slots)``
+    (sequence ``i``) into slot ``slots[i]``, as :func:`int4_cache_write` would write them; at head dim 128 in the same launch."""
+    from . import qk_norm_rope_decode
+    B, H, cap, D = _check_cache(cache)
+    _require(qkv.dim() == 2 and qkv.shape[1] == (Hq + 2 * H) * D, f"rows {tuple(qkv.shape)} are not {Hq} query and twice {H} key heads of {D}")
+    _require(qkv.device == cache.k.device, "rows and cache are on different devices")
+    _require_inference(qkv)
+    n = slots.numel()
+    _require(n <= min(B, qkv.shape[0]), f"{n} slots for {qkv.shape[0]} rows and a cache of {B}")
+    slots = _int32(slots.reshape(-1), (n,), cache.k.device, "slots")
+    if not (qkv.is_cuda and D == 128 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0):
+        out = qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, H, D, theta, eps, interleaved)
+        heads = out[:n, Hq * D:].view(n, 1, 2 * H, D)
+        int4_cache_write(cache.rows(slice(0, n)), heads[:, :, :H], heads[:, :, H:], slots.view(n, 1))
+        return out
+    _require(pos.shape == qkv.shape[:1] and pos.device == qkv.device, f"positions {tuple(pos.shape)} for {qkv.shape[0]} rows")
+    out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+    with _on(qkv):
+        _lib.call("ksa_qknorm_rope_decode_int4", qkv, out, q_w, k_w, pos.to(torch.int32).contiguous(), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, H,
+                  D, float(theta), float(eps), int(interleaved), cache.k, cache.k_scale, cache.v, cache.v_scale, slots, n, cap)
+    return out
+
+
 def int4_cache_read(cache: Int4Cache, start: torch.Tensor, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values of slots ``start[b] .. start[b] + rows`` of every sequence: ``(k, v)``, each ``[B, Hkv, rows, D]`` bf16; zeros for
     slots outside the cache."""
@@ -336,5 +361,5 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
     return out.view(out_shape)
 
 
-__all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_cache_read", "int4_cache_move", "int4_decode_attention",
+__all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_qk_norm_rope_decode", "int4_cache_read", "int4_cache_move", "int4_decode_attention",
            "int4_quantize_weight", "int4_dequantize_weight", "int4_linear", "int4_linear_swiglu"]

@@ -67,6 +67,21 @@ def test_cache_write_read_and_slots():
     assert [t.data_ptr() for t in cache.rows(slice(1, 2))] == [t[1:].data_ptr() for t in cache]
 
 
+def test_rotation_with_the_write():
+    H, D, Hq = 2, 64, 4
+    qkv, pos = torch.randn(3, (Hq + 2 * H) * D), torch.tensor([5, 0, 9])
+    got, expect, slots = ops.int4_cache(2, H, 16, D), ops.int4_cache(2, H, 16, D), torch.tensor([3, 16])
+    out = ops.int4_qk_norm_rope_decode(qkv, None, None, pos, Hq, 1e4, 1e-6, False, got, slots)
+    assert torch.equal(out, ops.qk_norm_rope_packed(qkv, None, None, pos, Hq, H, D, 1e4, 1e-6, False))
+    heads = out[:2, Hq * D:].view(2, 1, 2 * H, D)
+    ops.int4_cache_write(expect, heads[:, :, :H], heads[:, :, H:], slots.view(2, 1))
+    assert all(torch.equal(a, b) for a, b in zip(got, expect)) and got.k[0, :, 3].any() and not got.k[1].any()
+    with pytest.raises(ValueError):
+        ops.int4_qk_norm_rope_decode(qkv, None, None, pos, Hq, 1e4, 1e-6, False, got, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.int4_qk_norm_rope_decode(qkv[:, :-1], None, None, pos, Hq, 1e4, 1e-6, False, got, slots)
+
+
 def test_attention_is_that_over_the_values_of_the_slice():
     cache = ops.int4_cache(2, 2, 48, 64)
     k, v = _bf16(2, 48, 2, 64), _bf16(2, 48, 2, 64)

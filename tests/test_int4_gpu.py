@@ -96,6 +96,27 @@ def test_the_last_row_of_a_slot_stays(T):
         _same(a.cpu().float(), b.float())
 
 
+@pytest.mark.parametrize("rows,n,Hq,H,D", [(1, 1, 32, 8, 128), (5, 3, 4, 2, 128), (16, 16, 2, 1, 128), (4, 4, 4, 2, 64), (3, 0, 2, 1, 128)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norms", [False, True])
+def test_rotation_with_the_write_is_both_to_the_bit(rows, n, Hq, H, D, interleaved, norms):
+    qkv = _randn(rows, (Hq + 2 * H) * D + 16, seed=rows)[:, :(Hq + 2 * H) * D]
+    q_w, k_w = (1 + _randn(D, seed=1) * 0.1, 1 + _randn(D, seed=2) * 0.1) if norms else (None, None)
+    pos = torch.arange(rows, device=DEV) * 1000 + 3
+    slots = torch.tensor([7, -1, 48, 47, -5, 31, 0, 1, 2, 3, 4, 5, 6, 8, 9, 10], device=DEV, dtype=torch.int32)[:n]
+    got, expect = _cache(n + 1, H, 48, D, seed=3), _cache(n + 1, H, 48, D, seed=3)
+    out = ops.int4_qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, 1e4, 1e-6, interleaved, got, slots)
+    assert torch.equal(out, ops.qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, H, D, 1e4, 1e-6, interleaved))
+    heads = out[:n, Hq * D:].view(n, 1, 2 * H, D)
+    ops.int4_cache_write(expect.rows(slice(0, n)), heads[:, :, :H], heads[:, :, H:], slots.view(n, 1))
+    for a, b in zip(got, expect):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError):
+        ops.int4_qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, 1e4, 1e-6, interleaved, got, torch.zeros(rows + 1, device=DEV, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.int4_qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq + 1, 1e4, 1e-6, interleaved, got, slots)
+
+
 def test_write_takes_rows_of_any_layout():
     B, T, H, D = 2, 6, 2, 64
     base = _randn(B, H, D, T + 1, seed=4)
