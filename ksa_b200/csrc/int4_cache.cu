@@ -12,6 +12,10 @@ namespace ksa {
 
 constexpr int kI4Threads = 256;
 constexpr int kI4Scan = 64;      // rows of a sequence up to which a row looks through the slots behind its own
+// Up to so many rows of a sequence, slots, and rows that all blocks look at together, each block finds the last rows of its slots in shared memory; beyond
+// that a kernel of its own makes a table of them in memory.  Table against this, random slots, 8 heads of 128 (and on the host 5 us less): one sequence of
+// 100 rows 4.3 -> 2.7 us, 512 4.5 -> 3.1, 1024 5.3 -> 4.0, 2048 6.6 -> 6.9, 4096 8.8 -> 11.0; eight of 512 8.8 -> 8.1, of 2048 23.1 -> 30.1.
+constexpr int kI4BlockRows = 2048, kI4BlockCap = 8192, kI4BlockWork = 768 << 10;
 
 // Quotients by a size that is known at the launch, of numbers below 2^31: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
 // n / d = (mulhi(n, m) + n) >> l.
@@ -32,6 +36,7 @@ struct Int4Write {
   const int* last;               // [B, cap]: the last row of each slot, or null
   long long sb, st, sh;          // strides of k and v in elements
   int B, T, H, D, cap, scan;     // scan: look for later rows of the same slot
+  int in_shared;                 // the last row of each slot is found in shared memory
   int in_block;                  // rows of a block
   Int4Divide heads_of, rows_of, chunks_of;           // by H, by T, by D / 16
 };
@@ -57,6 +62,23 @@ __global__ void __launch_bounds__(kI4Threads) int4_cache_write_kernel(Int4Write 
   const long long src = b * a.sb + t * a.st + h * a.sh + c * 16;
   const uint4 k[2] = {*reinterpret_cast<const uint4*>(a.k + src), *reinterpret_cast<const uint4*>(a.k + src + 8)};
   const uint4 v[2] = {*reinterpret_cast<const uint4*>(a.v + src), *reinterpret_cast<const uint4*>(a.v + src + 8)};
+  if (a.in_shared) {
+    // the last of the sequence's rows from the block's first on in each of their slots; a block may hold the end of one sequence and the next ones
+    extern __shared__ int last_row[];
+    const int first = block * in_block, b0 = a.rows_of(first), b1 = a.rows_of(min(first + in_block, rows) - 1);
+    for (int s = b0; s <= b1; ++s) {
+      const int* slots = a.slots + (long long)s * a.T;
+      const int from = (s == b0 ? first - b0 * a.T : 0) + threadIdx.x;
+      for (int i = from; i < a.T; i += kI4Threads)
+        if ((unsigned)slots[i] < (unsigned)a.cap) last_row[slots[i]] = -1;
+      __syncthreads();
+      for (int i = from; i < a.T; i += kI4Threads)
+        if ((unsigned)slots[i] < (unsigned)a.cap) atomicMax(&last_row[slots[i]], i);
+      __syncthreads();
+      if (b == s && keep) keep = last_row[slot] == t;
+      if (s < b1) __syncthreads();
+    }
+  }
   if (keep && a.last != nullptr) keep = a.last[(long long)b * a.cap + slot] == t;
   if (keep && a.scan)
     for (int later = t + 1; later < a.T; ++later) keep &= a.slots[row - t + later] != slot;
@@ -158,15 +180,31 @@ __global__ void __launch_bounds__(kI4Threads) int4_weight_values_kernel(const ui
   *reinterpret_cast<uint4*>(w + i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// How a write finds the last row of a slot: a look at the slots behind its own, shared memory, or a table made ahead.
+enum Int4Last : int { kI4Look, kI4Shared, kI4Table };
+static long long i4_blocks(int B, int T, int H, int D) {
+  const int in_block = kI4Threads / (D / 16);
+  return ((long long)B * T + in_block - 1) / in_block * H;
+}
+static Int4Last i4_last(int B, int T, int H, int D, int cap) {
+  if (T <= kI4Scan) return kI4Look;
+  return T <= kI4BlockRows && cap <= kI4BlockCap && i4_blocks(B, T, H, D) * T <= kI4BlockWork ? kI4Shared : kI4Table;
+}
+
 static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
 }  // namespace ksa
 
 using namespace ksa;
 
+// Whether ksa_int4_cache_write of rows whose slots may repeat wants its workspace [B, cap] int32.
+KSA_API long long ksa_int4_cache_write_table(int B, int T, int H, int D, int cap) {
+  return B > 0 && H > 0 && D >= 16 && D <= 16 * kI4Threads && i4_last(B, T, H, D, cap) == kI4Table;
+}
+
 // k, v: [B, T, H, D] rows with strides (sb, st, sh) in elements.  Rows whose slot is negative or past the cache are not written; of several
-// rows with one slot the last stays: `last` is a workspace [B, cap] int32 for that, or null where T is at most 64 (rows look at
-// the slots behind theirs) or `distinct` says that no slot occurs twice.
+// rows with one slot the last stays: `last` is the workspace that ksa_int4_cache_write_table asks for, null where it does not or
+// `distinct` says that no slot occurs twice.
 KSA_API int ksa_int4_cache_write(const void* k, const void* v, void* k_codes, void* k_meta, void* v_codes, void* v_meta, const void* slots,
                                  void* last, int B, int T, int H, int D, int cap, long long sb, long long st, long long sh, int distinct,
                                  void* stream) {
@@ -178,22 +216,24 @@ KSA_API int ksa_int4_cache_write(const void* k, const void* v, void* k_codes, vo
               "int4_cache_write: rows must be 16-byte aligned");
   KSA_REQUIRE(!misaligned(k_codes, 8) && !misaligned(v_codes, 8) && !misaligned(k_meta, 4) && !misaligned(v_meta, 4),
               "int4_cache_write: cache tensors must be 8-byte aligned");
-  KSA_REQUIRE(distinct || T <= kI4Scan || last != nullptr, "int4_cache_write: %d rows need the workspace of last rows", T);
   if (B == 0 || T == 0) return 0;
   const int in_block = kI4Threads / (D / 16);
-  const long long rows = (long long)B * T, blocks = (rows + in_block - 1) / in_block * H;
+  const long long rows = (long long)B * T, blocks = i4_blocks(B, T, H, D);
   KSA_REQUIRE(rows < (1LL << 31) - kI4Threads && blocks < (1LL << 31), "int4_cache_write: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const bool table = !distinct && T > kI4Scan;
+  const Int4Last how = i4_last(B, T, H, D, cap);
+  const bool in_shared = !distinct && how == kI4Shared, table = !distinct && how == kI4Table;
+  KSA_REQUIRE(!table || last != nullptr, "int4_cache_write: %d rows need the workspace of last rows", T);
   if (table) {
     KSA_CHECK_CUDA(cudaMemsetAsync(last, 0xFF, (size_t)B * cap * sizeof(int), s));
     KSA_CHECK_CUDA(launch_kernel(int4_last_row_kernel, dim3((unsigned)(((long long)B * T + kI4Threads - 1) / kI4Threads)), dim3(kI4Threads), 0, s,
                                  (const int*)slots, (int*)last, B, T, cap));
   }
   Int4Write a{(const bf16*)k, (const bf16*)v, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint32_t*)k_meta, (uint32_t*)v_meta, (const int*)slots,
-              table ? (const int*)last : nullptr, sb, st, sh, B, T, H, D, cap, !distinct && !table && T > 1, in_block,
+              table ? (const int*)last : nullptr, sb, st, sh, B, T, H, D, cap, !distinct && T > 1 && how == kI4Look, in_shared, in_block,
               Int4Divide(H), Int4Divide(T), Int4Divide(D / 16)};
-  KSA_CHECK_CUDA(launch_stream_kernel(rows * H * D * 5, int4_cache_write_kernel, dim3((unsigned)blocks), dim3(kI4Threads), 0, s, a));
+  KSA_CHECK_CUDA(launch_stream_kernel(rows * H * D * 5, int4_cache_write_kernel, dim3((unsigned)blocks), dim3(kI4Threads), in_shared ? cap * sizeof(int) : 0,
+                                      s, a));
   return 0;
 }
 

@@ -84,6 +84,7 @@ int ksa_int4_decode_attn(const void* q, const void* k, const void* k_meta, const
                          const void* len, void* workspace, void* out, int B, int Tq, int Hq, int Hkv, int D, int cap, long long q_sb,
                          long long q_st, long long q_sh, float scale, void* stream);
 long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap);
+long long ksa_int4_cache_write_table(int B, int T, int H, int D, int cap);
 int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
                     long long ldc, int glu, void* stream);
 int ksa_summary_attn_bwd(const void* q, const void* k, const void* v, const void* ks, const void* vs, const void* o,
@@ -719,7 +720,7 @@ PyObject* py_int4_cache_write(PyObject*, PyObject* const* v, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     Tensor last;
-    if (!distinct && T > 64) last = a.empty({c.B, c.cap}, at::kInt);
+    if (!distinct && ksa_int4_cache_write_table(c.B, T, c.H, c.D, c.cap)) last = a.empty({c.B, c.cap}, at::kInt);
     LAUNCH(ksa_int4_cache_write, k->const_data_ptr(), x->const_data_ptr(), c.k->mutable_data_ptr(), c.ks->mutable_data_ptr(),
            c.v->mutable_data_ptr(), c.vs->mutable_data_ptr(), slots->const_data_ptr(), last.defined() ? last.mutable_data_ptr() : nullptr, c.B, T,
            c.H, c.D, c.cap, k->stride(0), k->stride(1), k->stride(2), distinct, a.stream());

@@ -121,6 +121,8 @@ def load() -> ctypes.CDLL:
     lib.ksa_gemm_narrow_plan.restype = I
     lib.ksa_int4_attn_workspace.argtypes = [I] * 6
     lib.ksa_int4_attn_workspace.restype = L
+    lib.ksa_int4_cache_write_table.argtypes = [I] * 5
+    lib.ksa_int4_cache_write_table.restype = L
     lib.ksa_set_dependent_launch.argtypes = [I]
     lib.ksa_set_dependent_launch.restype = I
     for name, sig in _SIGNATURES.items():

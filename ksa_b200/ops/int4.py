@@ -25,7 +25,6 @@ CACHE_DIM = 2048          # largest head dimension
 CACHE_SLOTS = 16          # the capacity of a cache is a multiple of this
 FEW_ROWS = 32             # rows that the kernels of ``int4_linear`` take
 FUSED_ROWS = 16           # and that of ``int4_linear_swiglu``
-_TABLE_ROWS = 64          # rows of a sequence from which a write finds the last row of each slot in a table
 
 
 class Int4Cache(NamedTuple):
@@ -143,7 +142,8 @@ def int4_cache_write(cache: Int4Cache, k_new: torch.Tensor, v_new: torch.Tensor,
             and k_new.data_ptr() % 16 == 0 and v_new.data_ptr() % 16 == 0):
         k_new, v_new = k_new.clone(memory_format=torch.contiguous_format), v_new.clone(memory_format=torch.contiguous_format)
     with _on(k_new):
-        last = torch.empty((B, cap), dtype=torch.int32, device=k_new.device) if T > _TABLE_ROWS and not distinct else None
+        table = not distinct and _lib.load().ksa_int4_cache_write_table(B, T, H, D, cap)
+        last = torch.empty((B, cap), dtype=torch.int32, device=k_new.device) if table else None
         _lib.call("ksa_int4_cache_write", k_new, v_new, cache.k, cache.k_scale, cache.v, cache.v_scale, slots, last, B, T, H, D, cap,
                   k_new.stride(0), k_new.stride(1), k_new.stride(2), int(distinct))
 

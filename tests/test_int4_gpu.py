@@ -96,6 +96,19 @@ def test_the_last_row_of_a_slot_stays(T):
         _same(a.cpu().float(), b.float())
 
 
+@pytest.mark.parametrize("B,T,H,D,cap", [(3, 65, 1, 32, 48), (5, 100, 2, 32, 16), (2, 1501, 2, 64, 8192), (1, 2048, 1, 128, 80), (1, 2049, 1, 128, 80),
+                                         (2, 300, 2, 64, 8208), (9, 1000, 8, 64, 1008), (3, 70, 1, 2048, 32)])
+def test_the_last_row_of_a_slot_stays_however_it_is_found(B, T, H, D, cap):
+    k, v = _randn(B, T, H, D, seed=1), _randn(B, T, H, D, seed=2)
+    slots = torch.randint(-2, min(cap, T // 2) + 2, (B, T), device=DEV, generator=_gen(3), dtype=torch.int32)
+    cache, once = ops.int4_cache(B, H, cap, D, DEV), ops.int4_cache(B, H, cap, D, DEV)
+    ops.int4_cache_write(cache, k, v, slots)
+    later = (slots[:, None, :] == slots[:, :, None]) & (torch.arange(T, device=DEV)[None, None, :] > torch.arange(T, device=DEV)[None, :, None])
+    ops.int4_cache_write(once, k, v, torch.where(later.any(2), -1, slots).to(torch.int32), distinct=True)
+    for a, b in zip(cache, once):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("rows,n,Hq,H,D", [(1, 1, 32, 8, 128), (5, 3, 4, 2, 128), (16, 16, 2, 1, 128), (4, 4, 4, 2, 64), (3, 0, 2, 1, 128)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("norms", [False, True])
