@@ -183,6 +183,11 @@ __device__ __forceinline__ void i4_fetch(const Int4Attn& a, const Int4Cursor& c,
   bulk_load(ring.v + slot * (kI4Tile * D / 8), a.v + at * (D / 2), n * (D / 2), bar);
   bulk_load(ring.v_meta + slot * (kI4Tile * D / 32), a.v_meta + at * (D / 32), n * (D / 8), bar);
 }
+__device__ __forceinline__ uint32_t ld_shared1(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kI4Warps * 32) : "memory"); }
 
 __device__ __forceinline__ float4 ld_cluster(const float4* local, uint32_t rank) {
@@ -296,6 +301,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
   }
 
   // ------------------------------------------------------------------ the warps that compute
+  const uint32_t k_at = smem_u32(ring.k), v_at = smem_u32(ring.v), k_meta_at = smem_u32(ring.k_meta), v_meta_at = smem_u32(ring.v_meta);
   bool ok = true;
   // A warp has a tile in every group and so waits for each: barriers know two phases, and copies of later groups may land first.
   int mine = warp, group = 0;      // this warp's tile, its group in the ring
@@ -334,8 +340,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[group], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
       const int first = (piece.lo & ~(kI4Align - 1)) + (piece.tile + mine - before) * kI4Tile;
-      const uint32_t *sk = ring.k + slot * (kI4Tile * D / 8), *sv = ring.v + slot * (kI4Tile * D / 8);
-      const uint32_t *skm = ring.k_meta + slot * (kI4Tile * D / 32), *svm = ring.v_meta + slot * (kI4Tile * D / 32);
+      const uint32_t sk = k_at + slot * (kI4Tile * D / 2), sv = v_at + slot * (kI4Tile * D / 2);
+      const uint32_t skm = k_meta_at + slot * (kI4Tile * D / 8), svm = v_meta_at + slot * (kI4Tile * D / 8);
 #pragma unroll
       for (int u = 0; u < kI4Tile / 16; ++u) {
         const int key0 = first + u * 16;                         // the block's first slot
@@ -349,11 +355,12 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int key = slot0 + j * 8;
-            const uint32_t meta = skm[key * (D / 32) + t * WK / 4];
+            const uint32_t meta = ld_shared1(skm + (key * (D / 32) + t * WK / 4) * 4);
             s2[j] = i4_scale2(meta);
             o2[j] = i4_offset2(meta);
-            if (D == 128) *reinterpret_cast<uint4*>(words[j]) = *reinterpret_cast<const uint4*>(&sk[key * (D / 8) + t * WK]);
-            else *reinterpret_cast<uint2*>(words[j]) = *reinterpret_cast<const uint2*>(&sk[key * (D / 8) + t * WK]);
+            const uint32_t at = sk + (key * (D / 8) + t * WK) * 4;
+            if constexpr (D == 128) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(words[j][0]), "=r"(words[j][1]), "=r"(words[j][2 % WK]), "=r"(words[j][3 % WK]) : "r"(at) : "memory");
+            else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(words[j][0]), "=r"(words[j][1]) : "r"(at) : "memory");
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
@@ -424,9 +431,10 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = u * 16 + i * 4 + (t ^ (i & 1));
-          if (D == 128) *reinterpret_cast<uint2*>(rows[i]) = *reinterpret_cast<const uint2*>(&sv[key * (D / 8) + g * WV]);
-          else rows[i][0] = sv[key * (D / 8) + g];
-          meta[i] = svm[key * (D / 32) + g * WV / 4];
+          const uint32_t at = sv + (key * (D / 8) + g * WV) * 4;
+          if constexpr (D == 128) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(rows[i][0]), "=r"(rows[i][WV - 1]) : "r"(at) : "memory");
+          else rows[i][0] = ld_shared1(at);
+          meta[i] = ld_shared1(svm + (key * (D / 32) + g * WV / 4) * 4);
         }
         if (__builtin_expect(!whole, 0)) {
 #pragma unroll

@@ -53,15 +53,17 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
 // others are taken as zeros (18 rows to a CTA: [2560, 9728] 9.0 -> 8.4 us, [2560, 4096] 4.8 -> 4.4; where several warps
 // share the rows nothing is gained).
 template <int NB, int kCount, bool kShort>
-__device__ __forceinline__ void i4l_multiply(float (&acc)[kI4LBlocks][NB][4], const uint4 (&x)[NB][4], const uint8_t* codes, const uint32_t* meta) {
+__device__ __forceinline__ void i4l_multiply(float (&acc)[kI4LBlocks][NB][4], const uint4 (&x)[NB][4], uint32_t codes, uint32_t meta) {
   uint32_t words[kCount][2][4], s2[kCount][2], o2[kCount][2];
 #pragma unroll
   for (int i = 0; i < kCount; ++i)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (kShort && i == kCount - 1 && h == 1) break;
-      *reinterpret_cast<uint4*>(words[i][h]) = *reinterpret_cast<const uint4*>(codes + (i * 16 + h * 8) * 64);
-      const uint32_t m = meta[i * 16 + h * 8];
+      const uint4 four = ld_shared(codes + (i * 16 + h * 8) * 64);
+      words[i][h][0] = four.x; words[i][h][1] = four.y; words[i][h][2] = four.z; words[i][h][3] = four.w;
+      uint32_t m;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m) : "r"(meta + (i * 16 + h * 8) * 4) : "memory");
       s2[i][h] = i4_scale2(m);
       o2[i][h] = i4_offset2(m);
     }
@@ -209,6 +211,7 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   const bf16* x_first = a.A + x_row * a.lda + turn * 128 + t * 32;
   const long long x_eight = x_next * a.lda;
   const uint32_t x_kept = smem_u32(xs) + x_row * a.x_pitch + turn * 256 + t * 16, kept_eight = x_next * a.x_pitch;
+  const uint32_t ring_at = smem_u32(ring);
   bool ok = true;
   int stage = 0;
   uint32_t phase = 0;
@@ -248,9 +251,7 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
       if (seg < a.segments) {                                                // what lies past K in the last one is zeros, scales and all
-        const uint8_t* src = ring + stage * a.stage_bytes;
-        const uint8_t* codes = src + codes_at;
-        const uint32_t* meta = reinterpret_cast<const uint32_t*>(src + meta_at);
+        const uint32_t src = ring_at + stage * a.stage_bytes, codes = src + codes_at, meta = src + meta_at;
         if (kParts == 1 && count == 2 && few) i4l_multiply<NB, 2, true>(acc, x, codes, meta);
         else if (count == 2) i4l_multiply<NB, 2, false>(acc, x, codes, meta);            // two chains of products side by side
         else if (count == 1) i4l_multiply<NB, 1, false>(acc, x, codes, meta);
