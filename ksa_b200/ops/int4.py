@@ -166,6 +166,9 @@ def int4_qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w
         int4_cache_write(cache.rows(slice(0, n)), heads[:, :, :H], heads[:, :, H:], slots.view(n, 1))
         return out
     _require(pos.shape == qkv.shape[:1] and pos.device == qkv.device, f"positions {tuple(pos.shape)} for {qkv.shape[0]} rows")
+    for w in (q_w, k_w):
+        _require(w is None or (w.shape == (D,) and w.dtype == qkv.dtype and w.device == qkv.device and w.is_contiguous() and w.data_ptr() % 4 == 0),
+                 f"norm weights are {D} contiguous bf16 values beside the rows")
     out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
     with _on(qkv):
         _lib.call("ksa_qknorm_rope_decode_int4", qkv, out, q_w, k_w, pos.to(torch.int32).contiguous(), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, H,
@@ -333,6 +336,8 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
     if x.dtype != torch.bfloat16:
         raise TypeError(f"the sm_100a kernels take bf16 activations, got {x.dtype}")
     M, out_shape = x.numel() // K, (*x.shape[:-1], N // 2 if glu else N)
+    if M == 0 or N == 0:
+        return torch.empty(out_shape, dtype=x.dtype, device=x.device)
     if glu and FUSED_ROWS < M <= _block_rows(N, K):
         from . import swiglu
         y = _linear(x.reshape(M, K), weight, False)
@@ -350,7 +355,7 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
                 y = swiglu(y) if N % 16 == 0 else ref.swiglu(torch.cat([gate, up], -1))
         return (y if glu or N % 8 == 0 else y[:, :N].contiguous()).view(out_shape)
     rows = x.reshape(M, K)
-    if M > 0 and (rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0):
+    if rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0:
         rows = rows.clone(memory_format=torch.contiguous_format)
     out = torch.empty((M, out_shape[-1]), dtype=x.dtype, device=x.device)
     with _on(x):

@@ -420,7 +420,20 @@ def test_weights_are_the_plain_form_to_the_bit(group):
         _same(ops.int4_dequantize_weight(got).float(), ref.int4_values(codes, scale).float())
 
 
+def test_a_weight_without_rows():
+    w = ops.int4_quantize_weight(_randn(0, 256))
+    for M in (0, 1, 20, 40, 200):
+        assert ops.int4_linear(_randn(M, 256), w).shape == (M, 0) and ops.int4_linear_swiglu(_randn(M, 256), w).shape == (M, 0)
+    assert ops.int4_dequantize_weight(w).shape == (0, 256)
+
+
 def test_refusals_on_the_device():
+    cache, rows, none = _cache(2, 2, 32, 128, seed=1), _randn(2, 8 * 128), torch.zeros(2, device=DEV, dtype=torch.int32)
+    for w in (torch.ones(128, device=DEV), torch.ones(64, device=DEV).bfloat16(), torch.ones(128).bfloat16(), _randn(256)[::2]):
+        with pytest.raises(ValueError):
+            ops.int4_qk_norm_rope_decode(rows, w, None, none, 4, 1e4, 1e-6, False, cache, none)
+    with pytest.raises(ValueError):
+        ops.int4_qk_norm_rope_decode(rows, None, None, none[:1], 4, 1e4, 1e-6, False, cache, none)
     cache = _cache(1, 2, 32, 96, seed=1)
     q, one = _randn(1, 1, 4, 96), torch.ones(1, 1, device=DEV, dtype=torch.int32)
     with pytest.raises(ValueError):
