@@ -407,6 +407,50 @@ def test_linear_rows_of_any_layout():
         _check_linear(y, x, w)
 
 
+def test_chains_of_clusters_on_two_streams_and_in_graphs():
+    """Products whose CTAs share K and hold all tensor memory, one after the other (each reads what the one before wrote), between bf16
+    products, beside the same on another stream, and replayed."""
+    n = 2304                            # more than 2 ** 22 values: 24 rows go in one launch
+    ws = [ops.int4_quantize_weight((_randn(n, n, seed=i) * 0.03).bfloat16()) for i in range(3)]
+    plain = (_randn(n, n, seed=9) * 0.03).bfloat16()
+    xs = [_randn(24, n, seed=20 + i) for i in range(2)]
+
+    def chain(x):
+        with torch.no_grad():
+            for w in ws:
+                x = ops.linear(ops.int4_linear(ops.int4_linear(x, w), w), plain)
+            return x
+    alone = [chain(x) for x in xs]
+    torch.cuda.synchronize()
+    one = ops.int4_linear(xs[0], ws[0])
+    _check_linear(one, xs[0], ws[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        got = []
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(chain(x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(chain(x))
+        graphs.append(g)
+    for _ in range(5):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, alone))
+    xs[0].copy_(_randn(24, n, seed=30))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], chain(xs[0]))
+    _lib.check_status()
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_weights_are_the_plain_form_to_the_bit(group):
     w = _randn(101, 384, seed=group)
