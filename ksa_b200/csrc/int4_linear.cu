@@ -29,6 +29,17 @@ constexpr int kI4LMostRows = 16;
 constexpr int kI4LWideRows = 192, kI4LWideColumns = 2048;
 constexpr int kI4LSmemMost = 227 * 1024;
 
+// Optional residual add and RMSNorm ahead of the product (as in gemv.cu): the activations are bf16(rms_norm(bf16(A + delta)) * w), made by every CTA for
+// itself and kept in its shared memory, while the ring fills.  Block 0 leaves A + delta in `res`.
+struct Int4Norm {
+  const bf16 *delta, *w;           // rows [0, delta_rows) have a delta
+  bf16* res;                       // null: nobody wants it
+  long long ld_delta, ld_res;
+  float eps;
+  int delta_rows;
+};
+constexpr int kI4LNormRows = 4;
+
 struct Int4Linear {
   const bf16* A;
   const uint32_t* meta;            // [K / group, pitch]
@@ -41,6 +52,7 @@ struct Int4Linear {
   int x_pitch;                     // bytes of an activation row in shared memory, 0: none are kept
   int ragged;                      // the last segment is not whole: a box for each
   int early;                       // weights are read ahead of the wait
+  Int4Norm norm;
 };
 
 __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
@@ -83,7 +95,7 @@ __device__ __forceinline__ void i4l_multiply(float (&acc)[kI4LBlocks][NB][4], co
 }
 
 // NB: activation rows in eights.  kParts: warps that share a segment's rows, up to 32 each (kGlu: the first half of them gate rows, the other their up rows).
-template <int NB, int kParts, bool kGlu>
+template <int NB, int kParts, bool kGlu, bool kNorm>
 __global__ void __launch_bounds__(kI4LThreads, 1)
 int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_meta, const Int4Linear a, int* status) {
   static_assert(!kGlu || kParts >= 2, "parts for gate and up rows");
@@ -193,7 +205,73 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   }
 
   // ------------------------------------------------------------------ the warps that multiply
-  if (a.x_pitch > 0) {
+  if (kNorm) {
+    float* s_sum = part;                                             // [warps][rows], before the first sums
+    const int per = rounds * kTurns * 16;                            // pieces of 16 bytes, with zeros behind the row
+    float sum[kI4LNormRows] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = threadIdx.x; c < per; c += kI4LWarps * 32) {
+      uint4 xv[kI4LNormRows], dv[kI4LNormRows];
+#pragma unroll
+      for (int m = 0; m < kI4LNormRows; ++m) {
+        xv[m] = dv[m] = make_uint4(0, 0, 0, 0);
+        if (m < a.M && c * 8 < a.K) {
+          xv[m] = *reinterpret_cast<const uint4*>(a.A + m * a.lda + c * 8);
+          if (m < a.norm.delta_rows) dv[m] = *reinterpret_cast<const uint4*>(a.norm.delta + m * a.norm.ld_delta + c * 8);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < kI4LNormRows; ++m) {
+        if (m >= a.M) break;
+        const uint32_t x4[4] = {xv[m].x, xv[m].y, xv[m].z, xv[m].w}, d4[4] = {dv[m].x, dv[m].y, dv[m].z, dv[m].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          o[q] = x4[q];
+          if (m < a.norm.delta_rows) {
+            const float2 x = unpack_bf16x2(x4[q]), d = unpack_bf16x2(d4[q]);
+            o[q] = pack_bf16x2(x.x + d.x, x.y + d.y);
+          }
+          const float2 f = unpack_bf16x2(o[q]);
+          sum[m] += f.x * f.x + f.y * f.y;
+        }
+        const uint4 r = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(xs + m * a.x_pitch + (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16) = r;
+        if (blockIdx.x == 0 && a.norm.res != nullptr && c * 8 < a.K) *reinterpret_cast<uint4*>(a.norm.res + m * a.norm.ld_res + c * 8) = r;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < kI4LNormRows; ++m) {
+      sum[m] = warp_sum(sum[m]);
+      if (lane == 0) s_sum[warp * kI4LNormRows + m] = sum[m];
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kI4LWarps * 32) : "memory");
+    float rstd[kI4LNormRows] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kI4LWarps; ++w)
+#pragma unroll
+      for (int m = 0; m < kI4LNormRows; ++m) rstd[m] += s_sum[w * kI4LNormRows + m];
+#pragma unroll
+    for (int m = 0; m < kI4LNormRows; ++m) rstd[m] = rsqrtf(rstd[m] / (float)a.K + a.norm.eps);
+    for (int c = threadIdx.x; c * 8 < a.K; c += kI4LWarps * 32) {    // a thread's own pieces again
+      const uint4 wv = *reinterpret_cast<const uint4*>(a.norm.w + c * 8);
+      const uint32_t w4[4] = {wv.x, wv.y, wv.z, wv.w};
+#pragma unroll
+      for (int m = 0; m < kI4LNormRows; ++m) {
+        if (m >= a.M) break;
+        uint4* at = reinterpret_cast<uint4*>(xs + m * a.x_pitch + (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16);
+        const uint4 xv = *at;
+        const uint32_t x4[4] = {xv.x, xv.y, xv.z, xv.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 x = unpack_bf16x2(x4[q]), f = unpack_bf16x2(w4[q]);
+          o[q] = pack_bf16x2(x.x * rstd[m] * f.x, x.y * rstd[m] * f.y);
+        }
+        *at = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kI4LWarps * 32) : "memory");
+  } else if (a.x_pitch > 0) {
     // an activation's 16 bytes w of the 64 that lane t wants of a segment lie at 4 w + t: four lanes read 64 bytes in a row
     const int per = rounds * kTurns * 16;
     for (int i = threadIdx.x; i < a.M * per; i += kI4LWarps * 32) {
@@ -236,7 +314,7 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     for (int round = 0, seg = turn; round < rounds; ++round, seg += kTurns, xp += kTurns * 128, xk += kTurns * 256) {
       // past K everything of the weights is zero, and any of the row's columns will do
       uint4 x[NB][4];
-      if (a.x_pitch > 0) {
+      if (kNorm || a.x_pitch > 0) {
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -288,7 +366,7 @@ static int i4l_cost(int per_cta, int segments, int parts, int sets, int* per_pas
   return passes * ((segments + turns - 1) / turns * (each + 1) + 2);
 }
 
-template <int NB, int kParts, bool kGlu>
+template <int NB, int kParts, bool kGlu, bool kNorm = false>
 static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) {
   constexpr int kTurns = kI4LWarps / kParts, kRows = kI4LBlocks * 16 * kParts, kPitch = kRows + 8, kSets = kGlu ? 2 : 1;
   int* status = status_word();
@@ -301,7 +379,8 @@ static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) 
   // activations that several passes want stay, where a ring of 64 KB and three rounds finds room beside them
   const int passes = (a.per_cta + a.per_pass - 1) / a.per_pass, x_pitch = (a.segments + kTurns - 1) / kTurns * kTurns * 256 + 64;
   const int least = 3 * per_stage > 64 * 1024 ? 3 * per_stage : 64 * 1024;
-  a.x_pitch = passes > 1 && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
+  a.x_pitch = (passes > 1 || kNorm) && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
+  KSA_REQUIRE(!kNorm || a.x_pitch > 0, "int4_norm_linear: no room for %d rows of %d values", a.M, a.K);
   a.stages = (kI4LSmemMost - rest - a.M * a.x_pitch) / per_stage;
   const int wanted = passes * ((a.segments + kTurns - 1) / kTurns);
   if (a.stages > wanted) a.stages = wanted;
@@ -319,21 +398,15 @@ static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) 
     uint32_t box[2] = {(uint32_t)a.meta_words, (uint32_t)(kTurns * groups)};
     if (const int rc = make_tmap(&tm_meta, a.meta, 4, 2, dims, str, box, false)) return rc;
   }
-  auto kern = int4_linear_kernel<NB, kParts, kGlu>;
+  auto kern = int4_linear_kernel<NB, kParts, kGlu, kNorm>;
   static PerDevice raised;
   KSA_CHECK_CUDA(raise_smem_limit(raised, kern, kI4LSmemMost));
   KSA_CHECK_CUDA(launch_kernel(kern, dim3((a.n_out + a.per_cta - 1) / a.per_cta), dim3(kI4LThreads), smem, st, tm, tm_meta, a, status));
   return 0;
 }
 
-}  // namespace ksa
-
-using namespace ksa;
-
-// A [M <= 64, K] (row pitch lda; M <= 16 with glu), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc); glu: gate rows and then up rows, C [M, N / 2].
-KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
-                            long long ldc, int glu, void* stream) {
-  KSA_ENTER(A);
+static int int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda, long long ldc,
+                       int glu, const Int4Norm* norm, cudaStream_t st) {
   KSA_REQUIRE(M >= 0 && M <= (glu ? kI4LMostRows : kI4WMostRows), "int4_linear: %d rows (at most %d)", M, glu ? kI4LMostRows : kI4WMostRows);
   KSA_REQUIRE(group == 32 || group == 64 || group == 128, "int4_linear: groups of %d values (32, 64 or 128)", group);
   KSA_REQUIRE(K > 0 && K % group == 0 && N >= 0 && pitch >= N && pitch % 4 == 0, "int4_linear: K %d is no multiple of the group of %d", K, group);
@@ -345,8 +418,8 @@ KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, 
   KSA_REQUIRE(M <= kI4LMostRows || !spread, "int4_linear: %d rows at a pitch of %lld for %d values", M, lda, K);
   const int sms = sm_count();
   KSA_REQUIRE(sms > 0, "int4_linear: no device");
-  if (!glu && !spread && (M > kI4LMostRows || (M > 8 && K >= kI4LWideColumns && N >= kI4LWideRows * sms)))
-    return int4_linear_wide(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, 0, reinterpret_cast<cudaStream_t>(stream));
+  if (norm == nullptr && !glu && !spread && (M > kI4LMostRows || (M > 8 && K >= kI4LWideColumns && N >= kI4LWideRows * sms)))
+    return int4_linear_wide(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, 0, st);
   Int4Linear a{};
   a.A = (const bf16*)A; a.meta = (const uint32_t*)meta; a.C = (bf16*)C;
   a.lda = lda; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.group = group; a.pitch = pitch;
@@ -362,10 +435,40 @@ KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, 
     if (parts == 0 || cost < best) { parts = p; best = cost; a.per_pass = per_pass; }
   }
   if (a.ragged) a.per_pass += a.per_pass & 1;        // a box begins on 128 bytes
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (norm != nullptr) {
+    a.norm = *norm;
+    if (glu) return parts == 2 ? launch_int4_linear<1, 2, true, true>(a, codes, st) : launch_int4_linear<1, 4, true, true>(a, codes, st);
+    return parts == 1 ? launch_int4_linear<1, 1, false, true>(a, codes, st) :
+           parts == 2 ? launch_int4_linear<1, 2, false, true>(a, codes, st) : launch_int4_linear<1, 4, false, true>(a, codes, st);
+  }
   if (glu && parts == 2) return M <= 8 ? launch_int4_linear<1, 2, true>(a, codes, st) : launch_int4_linear<2, 2, true>(a, codes, st);
   if (glu) return M <= 8 ? launch_int4_linear<1, 4, true>(a, codes, st) : launch_int4_linear<2, 4, true>(a, codes, st);
   if (parts == 1) return M <= 8 ? launch_int4_linear<1, 1, false>(a, codes, st) : launch_int4_linear<2, 1, false>(a, codes, st);
   if (parts == 2) return M <= 8 ? launch_int4_linear<1, 2, false>(a, codes, st) : launch_int4_linear<2, 2, false>(a, codes, st);
   return M <= 8 ? launch_int4_linear<1, 4, false>(a, codes, st) : launch_int4_linear<2, 4, false>(a, codes, st);
+}
+
+}  // namespace ksa
+
+using namespace ksa;
+
+// A [M <= 32, K] (row pitch lda; M <= 16 with glu), codes [N, K / 2], scales [K / group, pitch] words -> C [M, N] (row pitch ldc); glu: gate rows and
+// then up rows, C [M, N / 2].
+KSA_API int ksa_int4_linear(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda,
+                            long long ldc, int glu, void* stream) {
+  KSA_ENTER(A);
+  return int4_linear(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, glu, nullptr, reinterpret_cast<cudaStream_t>(stream));
+}
+
+// res = x + delta (rows [0, delta_rows), the others are x's; null: not wanted) and C = rms_norm(res, norm_w, eps) * W^T, M <= 4.
+KSA_API int ksa_int4_norm_linear(const void* x, const void* delta, const void* norm_w, void* res, const void* codes, const void* meta, void* C, int M,
+                                 int N, int K, int group, int pitch, long long ldx, long long ld_delta, long long ld_res, long long ldc, float eps,
+                                 int delta_rows, int glu, void* stream) {
+  KSA_ENTER(x);
+  KSA_REQUIRE(M <= kI4LNormRows, "int4_norm_linear: %d rows (at most %d)", M, kI4LNormRows);
+  KSA_REQUIRE(norm_w != nullptr && delta_rows >= 0 && delta_rows <= M && (delta_rows == 0 || delta != nullptr), "int4_norm_linear: incomplete arguments");
+  KSA_REQUIRE(((reinterpret_cast<uintptr_t>(delta) | reinterpret_cast<uintptr_t>(norm_w) | reinterpret_cast<uintptr_t>(res)) & 15) == 0 &&
+              ld_delta % 8 == 0 && ld_res % 8 == 0, "int4_norm_linear: rows must be 16-byte aligned");
+  const Int4Norm norm{(const bf16*)delta, (const bf16*)norm_w, (bf16*)res, ld_delta, ld_res, eps, delta_rows};
+  return int4_linear(x, codes, meta, C, M, N, K, group, pitch, ldx, ldc, glu, &norm, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -394,6 +394,13 @@ class KsaInferenceEngine:
             return layer.mlp(h, tp)
         return ops.int4_linear(ops.int4_linear_swiglu(h, w4.w13), w4.w2)
 
+    def _mlp_after_norm(self, layer, w4, x, attn_out):
+        """``res = x + attn_out`` and the feed-forward block on its norm."""
+        if w4 is None:
+            return layer.mlp.forward_after_norm(x, attn_out, layer.mlp_norm.scale, self.cfg.norm_eps)
+        x, h = ops.int4_norm_linear(x, attn_out, layer.mlp_norm.scale, self.cfg.norm_eps, w4.w13, glu=True)
+        return x, ops.int4_linear(h, w4.w2)
+
     def _decode_impl(self, tokens: torch.Tensor, any_boundary: bool, with_head: bool = True) -> torch.Tensor:
         """Device work of one decode step (launches only; the host mirror of the lengths is advanced by the caller).
         ``any_boundary``: some sequence closes a chunk in this step; which ones is read from ``_boundary_dev``."""
@@ -439,7 +446,7 @@ class KsaInferenceEngine:
         full_len = None     # slice lengths of the full-attention layers
         slices_of = {}      # layers with the same cache geometry share the step's slot / slice tensors
         # ordinary steps without tensor parallelism: residual add + norm live inside the projection that follows them
-        fuse_norm = tp is None and not any_boundary and B <= 4 and self._int4 is None
+        fuse_norm = tp is None and not any_boundary and B <= 4
         if self._int4 is not None and tp is not None:
             raise ValueError("weights in four bits are not available with tensor parallelism")
         for li, layer in enumerate(model.layers):
@@ -447,7 +454,8 @@ class KsaInferenceEngine:
             cache = self.layer_caches[li]
             w4 = self._int4[li] if self._int4 is not None else None
             if fuse_norm:
-                x, qkv = ops.norm_linear(x, delta, layer.sa_norm.scale, cfg.norm_eps, a.wqkv.weight)
+                x, qkv = (ops.norm_linear(x, delta, layer.sa_norm.scale, cfg.norm_eps, a.wqkv.weight) if w4 is None else
+                          ops.int4_norm_linear(x, delta, layer.sa_norm.scale, cfg.norm_eps, w4.qkv))
                 h = None
             else:
                 x, h = _add_norm(tp, x, delta, layer.sa_norm.scale, cfg.norm_eps)
@@ -498,7 +506,7 @@ class KsaInferenceEngine:
                     att = _attend(cache, q_t, start_t1, len_t1, scale, self._merge_counters).reshape(B, Hq * Dh)
                 attn_out = ops.int4_linear(att, w4.out) if w4 is not None else _row_linear(tp, att, a.output_proj.weight)
                 if fuse_norm:
-                    x, delta = layer.mlp.forward_after_norm(x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
+                    x, delta = self._mlp_after_norm(layer, w4, x, attn_out)
                 else:
                     x, h2 = _add_norm(tp, x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
                     delta = self._mlp(layer, w4, h2, tp)
@@ -512,7 +520,7 @@ class KsaInferenceEngine:
                 att = _attend(cache, q_t, self._zero_starts, full_len, scale, self._merge_counters).reshape(B, Hq * Dh)
                 attn_out = ops.int4_linear(att, w4.out) if w4 is not None else _row_linear(tp, att, a.output_proj.weight)
                 if fuse_norm:
-                    x, delta = layer.mlp.forward_after_norm(x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
+                    x, delta = self._mlp_after_norm(layer, w4, x, attn_out)
                 else:
                     x, h2 = _add_norm(tp, x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
                     delta = self._mlp(layer, w4, h2[:B], tp)

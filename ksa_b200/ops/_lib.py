@@ -71,6 +71,7 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_int4_decode_attn": [P] * 9 + [I] * 6 + [L, L, L, F, P],
     "ksa_int4_weight": [P, P, P, I, I, I, L, I, P],
     "ksa_int4_weight_values": [P, P, P, I, I, I, I, P],
+    "ksa_int4_norm_linear": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P],
     "ksa_int4_linear": [P, P, P, P, I, I, I, I, I, L, L, I, P],
     "ksa_peer_gather": [P, I, I, L, I, P, P, ctypes.c_uint, I, P],
     "ksa_peer_reduce_adamw": [P, I, I, L, L, P, P, P, P, P, F, F, F, F, F, P, P, P, ctypes.c_uint, I, P],

@@ -25,6 +25,8 @@ CACHE_DIM = 2048          # largest head dimension
 CACHE_SLOTS = 16          # the capacity of a cache is a multiple of this
 FEW_ROWS = 32             # rows that the kernels of ``int4_linear`` take
 FUSED_ROWS = 16           # and that of ``int4_linear_swiglu``
+NORM_ROWS = 4             # rows that ``int4_norm_linear`` takes in one launch,
+NORM_VALUES = 32768       # and values, which every CTA keeps in shared memory
 
 
 class Int4Cache(NamedTuple):
@@ -312,6 +314,38 @@ def int4_linear_swiglu(x: torch.Tensor, w13: Int4Weight) -> torch.Tensor:
     return _linear(x, w13, True)
 
 
+def int4_norm_linear(x: torch.Tensor, delta: Optional[torch.Tensor], norm_w: torch.Tensor, eps: float, weight: Int4Weight,
+                     glu: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``ops.norm_linear`` with a weight in four bits: ``res = x + delta`` (the first rows of ``x`` where ``delta`` has fewer), and the product
+    of ``rms_norm(res, norm_w)`` (``glu``: of gate and up rows, with its activation).  Returns ``(res, y)``; for up to 4 rows in one launch."""
+    from . import add_rms_norm, rms_norm
+    N, K, group, pitch = _check_weight(weight)
+    _require(x.dim() == 2 and x.shape[1] == K and norm_w.shape == (K,), f"rows {tuple(x.shape)} and norm {tuple(norm_w.shape)} do not fit a weight [{N}, {K}]")
+    _require(delta is None or (delta.dim() == 2 and delta.shape[1] == K and delta.shape[0] <= x.shape[0]), "the added rows do not fit the rows")
+    _require(not glu or N % 2 == 0, f"{N} rows are not as many gate as up rows")
+    _require(all(t is None or t.device == weight.codes.device for t in (x, delta, norm_w)), "rows, norm and weight are on different devices")
+    _require_inference(x, norm_w.detach(), *(() if delta is None else (delta,)))
+    M = x.shape[0]
+    rows = [t for t in (x, delta) if t is not None]
+    if (x.is_cuda and 0 < M <= NORM_ROWS and M * K <= NORM_VALUES and N > 0 and norm_w.is_contiguous() and norm_w.data_ptr() % 16 == 0
+            and all(t.dtype == torch.bfloat16 for t in (*rows, norm_w))
+            and all(t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 for t in rows)):
+        res = x if delta is None else torch.empty((M, K), dtype=x.dtype, device=x.device)
+        y = torch.empty((M, N // 2 if glu else N), dtype=x.dtype, device=x.device)
+        with _on(x):
+            _lib.call("ksa_int4_norm_linear", x, delta, norm_w.detach(), None if delta is None else res, weight.codes, weight.scale, y, M, N, K, group, pitch,
+                      x.stride(0), K if delta is None else delta.stride(0), K, y.shape[1], float(eps), 0 if delta is None else delta.shape[0], int(glu))
+        return res, y
+    step = min(NORM_ROWS, NORM_VALUES // K)
+    if x.is_cuda and step < M and step > 0 and (M <= NORM_ROWS or K > 8192):       # rows wider than the norm's own kernel takes, too
+        parts = [int4_norm_linear(x[r:r + step], None if delta is None or r >= delta.shape[0] else delta[r:r + step], norm_w, eps, weight, glu)
+                 for r in range(0, M, step)]
+        return x if delta is None else torch.cat([res for res, _ in parts]), torch.cat([y for _, y in parts])
+    with (_on(x) if x.is_cuda else contextlib.nullcontext()):
+        res, h = (x, rms_norm(x, norm_w.detach(), eps)) if delta is None else add_rms_norm(x, delta, norm_w.detach(), eps)
+        return res, _linear(h, weight, glu)
+
+
 def _block_rows(N: int, K: int) -> int:
     """Rows up to which blocks of ``FEW_ROWS`` read the codes, once each.  More rows multiply with the bf16 values, written out for the call, at
     a cost that hardly depends on them.  Measured, values against blocks: a weight of ``[1280, 1280]`` 6.5 us against 10.0 for 32 rows,
@@ -367,4 +401,4 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
 
 
 __all__ = ["Int4Cache", "Int4Weight", "int4_cache", "int4_cache_write", "int4_qk_norm_rope_decode", "int4_cache_read", "int4_cache_move", "int4_decode_attention",
-           "int4_quantize_weight", "int4_dequantize_weight", "int4_linear", "int4_linear_swiglu"]
+           "int4_quantize_weight", "int4_dequantize_weight", "int4_linear", "int4_linear_swiglu", "int4_norm_linear"]

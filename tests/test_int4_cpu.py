@@ -67,6 +67,19 @@ def test_cache_write_read_and_slots():
     assert [t.data_ptr() for t in cache.rows(slice(1, 2))] == [t[1:].data_ptr() for t in cache]
 
 
+def test_norm_ahead_of_the_product():
+    x, delta, norm = torch.randn(3, 64), torch.randn(2, 64), torch.rand(64) + 0.5
+    w = ops.int4_quantize_weight(torch.randn(10, 64))
+    for d in (None, delta):
+        for glu in (False, True):
+            res, y = ops.int4_norm_linear(x, d, norm, 1e-6, w, glu)
+            expect = x if d is None else torch.cat([x[:2] + d, x[2:]])
+            h = expect * (expect.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * norm
+            assert torch.allclose(res, expect) and torch.allclose(y, (ops.int4_linear_swiglu if glu else ops.int4_linear)(h, w), atol=1e-4)
+    with pytest.raises(ValueError):
+        ops.int4_norm_linear(x, torch.randn(4, 64), norm, 1e-6, w)
+
+
 def test_rotation_with_the_write():
     H, D, Hq = 2, 64, 4
     qkv, pos = torch.randn(3, (Hq + 2 * H) * D), torch.tensor([5, 0, 9])

@@ -464,6 +464,38 @@ def test_weights_are_the_plain_form_to_the_bit(group):
         _same(ops.int4_dequantize_weight(got).float(), ref.int4_values(codes, scale).float())
 
 
+@pytest.mark.parametrize("M", [1, 3, 4, 5])
+@pytest.mark.parametrize("N,K,group", [(6, 32, 32), (777 * 2, 160, 32), (6144, 2560, 64), (2560, 4096, 128), (39000, 256, 64), (40, 32768, 128)])
+@pytest.mark.parametrize("glu", [False, True])
+def test_norm_ahead_of_the_product(M, N, K, group, glu):
+    """Against the product of the norm's own rounding in 64 bits: a value of the norm is off by one rounding to bf16 and 2^-20 of fp32 (a sum of K
+    squares in parts, a root, two products), which the product sees as that share of its terms' magnitudes."""
+    w = ops.int4_quantize_weight((_randn(N, K, seed=N) * 0.1).bfloat16(), group)
+    wd = ops.int4_dequantize_weight(w).double()
+    wide = _randn(M, K + 8, seed=1)
+    norm_w = (1 + _randn(K, seed=2) * 0.2).bfloat16()
+    for n in (None, M, M // 2):
+        x, delta = wide[:, :K], None if n is None else _randn(n, K, seed=3)
+        res, y = ops.int4_norm_linear(x, delta, norm_w, 1e-6, w, glu)
+        expect = x.clone()
+        if n is not None:
+            expect[:n] = (x[:n].float() + delta.float()).bfloat16()
+        assert torch.equal(res, expect)
+        r = expect.double()
+        h = r * (r.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * norm_w.double()
+        p, mag = h @ wd.t(), h.abs() @ wd.abs().t()
+        err = (HALF + 2.0 ** -20) * 1.01 * mag + HALF * p.abs() * 1.01 + (K / 16 + 64) * FP32 * mag * 1.01
+        if not glu:
+            assert ((y.double() - p).abs() <= err + 1e-30).all()
+            continue
+        F = N // 2
+        gate, up, dg, du = p[:, :F], p[:, F:], err[:, :F], err[:, F:]
+        z = torch.nn.functional.silu(gate) * up
+        bound = 1.1 * dg * (up.abs() + du) + torch.nn.functional.silu(gate).abs() * du + (HALF + 2.0 ** -20) * (z.abs() + 1.1 * dg * up.abs()) * 1.01 + 1e-30
+        assert ((y.double() - z).abs() <= bound).all()
+    _lib.check_status()
+
+
 def test_a_weight_without_rows():
     w = ops.int4_quantize_weight(_randn(0, 256))
     for M in (0, 1, 20, 40, 200):
@@ -478,6 +510,10 @@ def test_refusals_on_the_device():
             ops.int4_qk_norm_rope_decode(rows, w, None, none, 4, 1e4, 1e-6, False, cache, none)
     with pytest.raises(ValueError):
         ops.int4_qk_norm_rope_decode(rows, None, None, none[:1], 4, 1e4, 1e-6, False, cache, none)
+    w, x, one = ops.int4_quantize_weight(_randn(8, 64)), _randn(2, 64), torch.ones(64, device=DEV).bfloat16()
+    for bad in ((x[:, :32], None, one), (x, _randn(3, 64), one), (x, _randn(2, 32), one), (x, None, one[:32]), (x, None, one.cpu())):
+        with pytest.raises(ValueError):
+            ops.int4_norm_linear(*bad, 1e-6, w)
     cache = _cache(1, 2, 32, 96, seed=1)
     q, one = _randn(1, 1, 4, 96), torch.ones(1, 1, device=DEV, dtype=torch.int32)
     with pytest.raises(ValueError):
