@@ -30,7 +30,8 @@ constexpr int kI4LWideRows = 192, kI4LWideColumns = 2048;
 constexpr int kI4LSmemMost = 227 * 1024;
 
 // Optional residual add and RMSNorm ahead of the product (as in gemv.cu): the activations are bf16(rms_norm(bf16(A + delta)) * w), made by every CTA for
-// itself and kept in its shared memory, while the ring fills.  Block 0 leaves A + delta in `res`.
+// itself and kept in its shared memory, while the ring fills.  Block 0 leaves A + delta in `res`.  Against two launches, one and four rows:
+// [6144, 2560] 8.3 -> 6.4 us and 8.7 -> 8.2, gate and up rows of [19456, 2560] 14.8 -> 13.7 and 16.6 -> 15.5.
 struct Int4Norm {
   const bf16 *delta, *w;           // rows [0, delta_rows) have a delta
   bf16* res;                       // null: nobody wants it
