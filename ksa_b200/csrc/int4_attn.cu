@@ -680,11 +680,11 @@ static int launch_int4_attn(const Int4Attn& a, const Int4Shape& s, cudaStream_t 
 
 using namespace ksa;
 
-// Floats of the workspace of ksa_int4_decode_attn on the current device.
+// Floats of the workspace of ksa_int4_decode_attn on the current device: none where clusters merge.
 KSA_API long long ksa_int4_attn_workspace(int B, int Tq, int Hq, int Hkv, int D, int cap) {
   if (B <= 0 || Tq <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv != 0 || cap <= 0 || (long long)B * Tq >= (1 << 28)) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
-  return (s.ctas + s.items) * s.heads * (D + 2LL) + 2LL * s.ctas;
+  return s.cluster ? 0 : (s.ctas + s.items) * s.heads * (D + 2LL) + 2LL * s.ctas;
 }
 
 // q [B, Tq, Hq, D] with strides in elements (rows of a head contiguous); cache as written by ksa_int4_cache_write; start, len [B, Tq] int32;
@@ -704,6 +704,7 @@ KSA_API int ksa_int4_decode_attn(const void* q, const void* k, const void* k_met
   if (B == 0 || Tq == 0) return 0;
   const Int4Shape s = i4_shape(B * Tq, Hq, Hkv, D, cap);
   KSA_REQUIRE(s.tiles < (1LL << 31) - s.ctas, "int4_decode_attn: too many queries and slots");
+  KSA_REQUIRE(s.cluster || workspace != nullptr, "int4_decode_attn: no workspace");
   const long long parts = s.ctas + s.items;
   float* ws = (float*)workspace;
   Int4Attn a{(const bf16*)q, q_sb, q_st, q_sh, (const uint8_t*)k, (const uint8_t*)v, (const uint32_t*)k_meta, (const uint32_t*)v_meta,

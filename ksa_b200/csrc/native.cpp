@@ -766,9 +766,11 @@ PyObject* py_int4_decode_attention(PyObject*, PyObject* const* v, Py_ssize_t n) 
   {
     pybind11::gil_scoped_release no_gil;
     out = a.empty({c.B, Tq, Hq, c.D});
-    const Tensor workspace = a.empty({(int64_t)ksa_int4_attn_workspace(c.B, Tq, Hq, c.H, c.D, c.cap)}, at::kFloat);
+    const long long floats = ksa_int4_attn_workspace(c.B, Tq, Hq, c.H, c.D, c.cap);
+    Tensor workspace;
+    if (floats > 0) workspace = a.empty({(int64_t)floats}, at::kFloat);
     LAUNCH(ksa_int4_decode_attn, q->const_data_ptr(), c.k->const_data_ptr(), c.ks->const_data_ptr(), c.v->const_data_ptr(),
-           c.vs->const_data_ptr(), start->const_data_ptr(), length->const_data_ptr(), workspace.mutable_data_ptr(), out.mutable_data_ptr(), c.B,
+           c.vs->const_data_ptr(), start->const_data_ptr(), length->const_data_ptr(), floats > 0 ? workspace.mutable_data_ptr() : nullptr, out.mutable_data_ptr(), c.B,
            Tq, Hq, c.H, c.D, c.cap, q->stride(0), q->stride(1), q->stride(2), scale, a.stream());
   }
   return wrap(out);

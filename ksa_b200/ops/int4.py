@@ -243,7 +243,7 @@ def int4_decode_attention(q: torch.Tensor, cache: Int4Cache, start: torch.Tensor
     out = torch.empty((B, Tq, Hq, D), dtype=q.dtype, device=q.device)
     with _on(q):
         n = _lib.load().ksa_int4_attn_workspace(B, Tq, Hq, Hkv, D, cap)
-        workspace = torch.empty(n, dtype=torch.float32, device=q.device)
+        workspace = torch.empty(n, dtype=torch.float32, device=q.device) if n > 0 else None
         _lib.call("ksa_int4_decode_attn", q, cache.k, cache.k_scale, cache.v, cache.v_scale, start, length, workspace, out, B, Tq, Hq, Hkv, D,
                   cap, q.stride(0), q.stride(1), q.stride(2), scale)
     return out
