@@ -9,7 +9,7 @@
 //   * sixteen warps multiply: a round has 16 / kParts segments, and kParts warps share the rows of a segment.  They keep their sums of a pass and
 //     leave them in shared memory; two more warps add the sums up and write the results while the others are at the next pass;
 //   * mma.sync m16n8k16 multiplies 16 weight rows by 8 activation rows; a lane's 16 bytes of a weight row are columns 32 t .. 32 t + 31 of the segment, in
-//     that order for the activations as well.  Activations that several passes want stay in shared memory, others are read as they are needed.
+//     that order for the activations as well.  Activations that several passes want, and few of one pass, stay in shared memory, others are read as they are needed.
 #include "int4_linear.h"
 
 #include "host.h"
@@ -275,11 +275,20 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
   } else if (a.x_pitch > 0) {
     // an activation's 16 bytes w of the 64 that lane t wants of a segment lie at 4 w + t: four lanes read 64 bytes in a row
     const int per = rounds * kTurns * 16;
-    for (int i = threadIdx.x; i < a.M * per; i += kI4LWarps * 32) {
-      const int m = i / per, c = i - m * per;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (c * 8 < a.K) v = *reinterpret_cast<const uint4*>(a.A + m * a.lda + c * 8);         // zeros behind
-      *reinterpret_cast<uint4*>(xs + m * a.x_pitch + (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16) = v;
+    constexpr int kAtOnce = NB * 4;
+    for (int c = threadIdx.x; c < per; c += kI4LWarps * 32) {
+      const int at = (c & ~15) * 16 + ((c & 3) * 4 + ((c >> 2) & 3)) * 16;
+      for (int m0 = 0; m0 < a.M; m0 += kAtOnce) {
+        uint4 v[kAtOnce];
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m) {
+          v[m] = make_uint4(0, 0, 0, 0);
+          if (m0 + m < a.M && c * 8 < a.K) v[m] = *reinterpret_cast<const uint4*>(a.A + (m0 + m) * a.lda + c * 8);         // zeros behind
+        }
+#pragma unroll
+        for (int m = 0; m < kAtOnce; ++m)
+          if (m0 + m < a.M) *reinterpret_cast<uint4*>(xs + (m0 + m) * a.x_pitch + at) = v[m];
+      }
     }
     asm volatile("bar.sync 1, %0;" ::"n"(kI4LWarps * 32) : "memory");
   }
@@ -377,10 +386,12 @@ static int launch_int4_linear(Int4Linear a, const void* codes, cudaStream_t st) 
   a.meta_at = kSets * ((kTurns * a.per_pass * 64 + 127) / 128 * 128) + 1024;      // the last block may reach past the rows
   a.stage_bytes = a.meta_at + kSets * ((kTurns * groups * a.meta_words * 4 + 127) / 128 * 128) + 128;          // (its scales as well)
   const int part = kTurns * NB * 8 * kPitch * 4, per_stage = a.stage_bytes + 16, rest = part + 32;
-  // activations that several passes want stay, where a ring of 64 KB and three rounds finds room beside them
+  // Activations stay where a ring of 64 KB and three rounds finds room beside them: those that several passes want, and few of one pass, a piece or
+  // none a thread and row, which come in while the ring fills ([6144, 2560] x 4 rows 6.2 -> 5.8 us, x 1 row 5.9 -> 5.7; more of them keep the first
+  // round waiting: [2560, 9728] x 5 rows 8.5 -> 10.0, [6144, 2560] x 16 rows 7.9 -> 9.0)
   const int passes = (a.per_cta + a.per_pass - 1) / a.per_pass, x_pitch = (a.segments + kTurns - 1) / kTurns * kTurns * 256 + 64;
   const int least = 3 * per_stage > 64 * 1024 ? 3 * per_stage : 64 * 1024;
-  a.x_pitch = (passes > 1 || kNorm) && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
+  a.x_pitch = (passes > 1 || kNorm || (a.M <= 4 && a.K <= kI4LWarps * 32 * 8)) && (long long)a.M * x_pitch + rest + least <= kI4LSmemMost ? x_pitch : 0;
   KSA_REQUIRE(!kNorm || a.x_pitch > 0, "int4_norm_linear: no room for %d rows of %d values", a.M, a.K);
   a.stages = (kI4LSmemMost - rest - a.M * a.x_pitch) / per_stage;
   const int wanted = passes * ((a.segments + kTurns - 1) / kTurns);
