@@ -23,10 +23,11 @@ constexpr int kI4LThreads = (kI4LWarps + kI4LAdders + 1) * 32;
 constexpr int kI4LBlocks = 2;                       // blocks of 16 weight rows of a warp
 constexpr int kI4LMostStages = 12;
 constexpr int kI4LMostRows = 16;
-// Nine rows and more of a large weight go to int4_linear_wide.cu: from 192 weight rows a CTA and 2048 columns.  Measured on 16 rows, this kernel against
-// that one: [19456, 2560] 17.8 us against 18.6, [28416, 2560] 22.2 against 19.1, [37888, 4096] 35.6 against 25.7, [151936, 2560] 71 against 60, but
-// [40000, 1024] 14.8 against 16.6, [100000, 512] 20.1 against 23.8; on one row [151936, 2560] 52 against 59.
-constexpr int kI4LWideRows = 192, kI4LWideColumns = 2048;
+// Nine rows and more of a large weight go to int4_linear_wide.cu: from 80 weight rows a CTA and 1536 columns.  Measured on 16 rows, this kernel against
+// that one: [6144, 2560] 7.7 us against 10.0, [2560, 9728] 11.5 against 12.6, [12000, 4096] 18.8 against 14.4, [19456, 2560] 16.8 against 16.4, [19456, 4096]
+// 27.2 against 22.5, [151936, 2560] 71 against 54, but [40000, 1024] 15.2 against 15.7, [100000, 512] 20.3 against 20.4; on nine rows [12000, 4096] 15.8
+// against 14.6, [19456, 4096] 21.8 against 22.2; on one row [151936, 2560] 52 against 53, [86978, 2368] 31 against 33.
+constexpr int kI4LWideRows = 80, kI4LWideColumns = 1536;
 constexpr int kI4LSmemMost = 227 * 1024;
 
 // Optional residual add and RMSNorm ahead of the product (as in gemv.cu): the activations are bf16(rms_norm(bf16(A + delta)) * w), made by every CTA for

@@ -4,13 +4,13 @@
 // issue slots as the unpacking and twice as many from nine rows on, and every eight activation rows want registers.  Here:
 //   * a lane unpacks a row of the weight, 128 columns at a time, into tensor memory, where tcgen05.mma takes it as the operand of 128 rows; the
 //     activations, a TMA copy with its swizzle, are the other one, 16 or 32 of them at much the same price;
-//   * three groups of four warps unpack halves of the ring's stages in turn, each with two slots of its own, sums of its own and a warp that
-//     issues its products.  With all warps at one stage, or with one thread issuing for all, each stage waited for a chain of barriers:
-//     [151936, 2560] x 16 rows 79 us, with groups but one issuer 72, one of the unpacking warps issuing 80, this 60;
+//   * three groups of four warps unpack the ring's stages in turn, each with its own slot, its own sums and a warp that issues its products.  What
+//     decides is how few instructions and barriers there are to a stage: [151936, 2560] x 16 rows with all warps at one stage 79 us, with groups but
+//     one issuer 72, with half a stage and two slots to a group 60, four groups with one 60, this 54 (the fetch alone 33, without the stores 40);
 //   * four more warps add up the groups' sums of a pass, in their order, and write them while the next pass is being unpacked;
 //   * activations that several passes want and that fit stay in shared memory, others come with each stage;
 //   * few rows of the weight: the CTAs of a cluster share K, and each adds up some of the activation rows from the others' shared memory.
-// Measured on 32 rows: [151936, 2560] 87 us (2.5 TB/s), [19456, 2560] 19, [6144, 2560] 12.6, [2560, 9728] 14.2 on clusters of four, 27 without.
+// Measured on 32 rows: [151936, 2560] 81 us (2.7 TB/s), [19456, 2560] 18, [6144, 2560] 12.0, [2560, 9728] 13.5 on clusters of four.
 #include "int4_linear.h"
 
 #include "host.h"
@@ -18,15 +18,14 @@
 
 namespace ksa {
 
-constexpr int kI4WGroups = 3;                       // four warps each that unpack: a group takes every third half of a stage
+constexpr int kI4WGroups = 3;                       // four warps each that unpack: a group takes every third stage
 constexpr int kI4WUnpackers = 4 * kI4WGroups;
 constexpr int kI4WWriters = kI4WUnpackers;          // first of the four that write results
 constexpr int kI4WFetch = kI4WWriters + 4;
 constexpr int kI4WIssuers = kI4WFetch + 1;          // first of those that multiply, one to a group
 constexpr int kI4WThreads = (kI4WIssuers + kI4WGroups) * 32;
 constexpr int kI4WStep = 256;                       // columns of a stage
-constexpr int kI4WSlots = 2;                        // of each group: 128 unpacked columns, 64 of tensor memory
-constexpr int kI4WSums = kI4WGroups * kI4WSlots * 64;           // behind them each group's sums: two sets of 16 columns, or one of 32
+constexpr int kI4WSums = kI4WGroups * 128;          // each group unpacks a stage into 128 columns; behind them its sums: two sets of 16 columns, or one of 32
 constexpr int kI4WMostStages = 15;                  // a multiple of three: a stage of the ring belongs to the same groups all the time
 constexpr int kI4WSmemMost = 227 * 1024;
 constexpr int kI4WKeepMost = 96 * 1024;             // activations that stay
@@ -90,8 +89,8 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
   uint64_t* full = reinterpret_cast<uint64_t*>(part + (a.parts > 1 ? a.cols * 128 : 0));
   uint64_t* empty = full + kI4WMostStages;
   uint64_t* slot_full = empty + kI4WMostStages;
-  uint64_t* slot_empty = slot_full + kI4WGroups * kI4WSlots;
-  uint64_t* sums_full = slot_empty + kI4WGroups * kI4WSlots;                            // [group][set]
+  uint64_t* slot_empty = slot_full + kI4WGroups;
+  uint64_t* sums_full = slot_empty + kI4WGroups;                            // [group][set]
   uint64_t* sums_empty = sums_full + kI4WGroups * 2;
   uint64_t* x_full = sums_empty + kI4WGroups * 2;
   uint64_t* ended = x_full + 1;
@@ -107,8 +106,8 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
   const int step0 = rank * a.steps / a.parts, count = (rank + 1) * a.steps / a.parts - step0, total = passes * count;
   const int groups = kI4WStep / a.group, panel = a.cols * 128, sets = a.cols == 16 ? 2 : 1;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < a.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], a.keep ? 8 : 2); }
-    for (int i = 0; i < kI4WGroups * kI4WSlots; ++i) { mbar_init(&slot_full[i], 4); mbar_init(&slot_empty[i], 1); }
+    for (int i = 0; i < a.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], a.keep ? 4 : 1); }
+    for (int i = 0; i < kI4WGroups; ++i) { mbar_init(&slot_full[i], 4); mbar_init(&slot_empty[i], 1); }
     for (int i = 0; i < kI4WGroups * 2; ++i) { mbar_init(&sums_full[i], 1); mbar_init(&sums_empty[i], 4); }
     mbar_init(x_full, 1);
     mbar_init(ended, kI4WGroups);
@@ -179,37 +178,35 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
     const int group = warp - kI4WIssuers;
     const uint32_t idesc = umma_idesc_bf16(128, a.cols, 0, 0), panel16 = panel >> 4, stage16 = a.stage_bytes >> 4;
     const uint64_t x_desc = smem_desc_kmajor_sw128(smem_u32(a.keep ? kept : ring + a.b_at));
-    uint64_t *my_full = slot_full + group * kI4WSlots, *my_empty = slot_empty + group * kI4WSlots;
-    int half = group & 1, stage = group >> 1, k = stage, slot = 0, set = 0;             // half `half` of step `k` of a pass
+    uint64_t *my_full = slot_full + group, *my_empty = slot_empty + group;
+    int stage = group, k = stage, set = 0;             // step `k` of a pass
     uint32_t phase = 0, slot_phase = 0, accumulate = 0, sums_phase = 1;
     bool ok = !a.keep || __all_sync(0xffffffffu, mbar_wait(x_full, 0, guard, kTimeoutTmaFull));
     int left = total - stage;
     for (; k >= count; k -= count) {}
     while (ok && left > 0) {
-      const bool last = k + 1 + half >= count;                       // of this group in the pass
-      const uint64_t desc = x_desc + (a.keep ? k * 4 * panel16 : stage * stage16) + half * 2 * panel16;
-      const uint32_t sums = tmem + kI4WSums + (group * sets + set) * a.cols, from = tmem + (group * kI4WSlots + slot) * 64;
+      const bool last = k + kI4WGroups >= count;                     // of this group in the pass
+      const uint64_t desc = x_desc + (a.keep ? k * 4 * panel16 : stage * stage16);
+      const uint32_t sums = tmem + kI4WSums + (group * sets + set) * a.cols, from = tmem + group * 128;
       if (accumulate == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sums_empty[group * 2 + set], sums_phase, guard, kTimeoutAccEmpty));
       if (!a.keep) ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&my_full[slot], slot_phase, guard, kTimeoutSoftmax));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(my_full, slot_phase, guard, kTimeoutSoftmax));
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) umma_ts(sums, from + e * 8, desc + (e >> 2) * panel16 + (e & 3) * 2, idesc, e == 0 ? accumulate : 1);
-        umma_commit(&my_empty[slot]);
+        for (int e = 0; e < 16; ++e) umma_ts(sums, from + e * 8, desc + (e >> 2) * panel16 + (e & 3) * 2, idesc, e == 0 ? accumulate : 1);
+        umma_commit(my_empty);
         if (!a.keep) umma_commit(&empty[stage]);
         if (last) umma_commit(&sums_full[group * 2 + set]);
       }
       __syncwarp();
       accumulate = !last;
       if (last && ++set == sets) { set = 0; sums_phase ^= 1; }
-      if (++slot == kI4WSlots) { slot = 0; slot_phase ^= 1; }
-      const int ahead = 1 + half;
-      half ^= 1;
-      left -= ahead;
-      for (k += ahead; k >= count; k -= count) {}
-      if ((stage += ahead) >= a.stages) { stage -= a.stages; phase ^= 1; }
+      slot_phase ^= 1;
+      left -= kI4WGroups;
+      for (k += kI4WGroups; k >= count; k -= count) {}
+      if ((stage += kI4WGroups) >= a.stages) { stage -= a.stages; phase ^= 1; }
     }
     if (elect_one()) umma_commit(ended);
     __syncwarp();
@@ -217,7 +214,7 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
     // ---------------------------------------------------------------- the warps that unpack, a weight row to a lane
     const int quarter = warp & 3, group = warp >> 2;
     const int row = min(quarter * 32 + lane, a.per_pass - 1);        // lanes past the pass's rows make sums that nobody reads
-    const uint32_t out = tmem + group * kI4WSlots * 64 + ((uint32_t)(quarter * 32) << 16), ring_at = smem_u32(ring);
+    const uint32_t out = tmem + group * 128 + ((uint32_t)(quarter * 32) << 16), ring_at = smem_u32(ring);
     uint32_t chunk_at[2], meta_at[2];                                // of 64 columns; the next ones lie 32 bytes and some groups on
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -225,58 +222,58 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
       meta_at[c] = a.meta_at + (c * 32 / a.group * a.meta_words + row) * 4;
     }
     const uint32_t meta_half = 128 / a.group * a.meta_words * 4, meta_quarter = 64 / a.group * a.meta_words * 4;
-    uint32_t half = group & 1, at = ring_at + (group >> 1) * a.stage_bytes, skip = r0 & 3;
-    uint64_t* slots_full = slot_full + group * kI4WSlots;
-    int stage = group >> 1, k = stage, left = total - k, slot = 0;
+    uint32_t at = ring_at + group * a.stage_bytes, skip = r0 & 3;
+    int stage = group, k = stage, left = total - k;
     uint32_t phase = 0, slot_phase = 1;
     bool ok = true;
     while (left > 0) {
       for (; k >= count; k -= count) skip = (skip + a.per_pass) & 3;
       ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
       if (!ok) break;
-      uint4 words[4];
-      uint32_t m[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        words[c] = ld_shared(at + (chunk_at[c & 1] ^ (half * 64 + (c >> 1) * 32)));
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[c]) : "r"(at + meta_at[c & 1] + half * meta_half + (c >> 1) * meta_quarter + skip * 4) : "memory");
-      }
-      __syncwarp();
-      if (a.keep) {                                                    // nothing else of the stage is wanted
-        if (lane == 0) mbar_arrive(&empty[stage]);
-        __syncwarp();
-      }
-      ok = __all_sync(0xffffffffu, mbar_wait(slots_full + (slot_empty - slot_full) + slot, slot_phase, guard, kTimeoutAccEmpty));
-      if (!ok) break;
-      tc_fence_after();
+      for (uint32_t half = 0; half < 2; ++half) {
+        uint4 words[4];
+        uint32_t m[4];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint32_t v[32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t s2 = i4_scale2(m[s * 2 + h]), o2 = i4_offset2(m[s * 2 + h]);
-          const uint32_t four[4] = {words[s * 2 + h].x, words[s * 2 + h].y, words[s * 2 + h].z, words[s * 2 + h].w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
-            i4_values(w, four[q], s2, o2);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[h * 16 + q * 4 + e] = w[e];
-          }
+        for (int c = 0; c < 4; ++c) {
+          words[c] = ld_shared(at + (chunk_at[c & 1] ^ (half * 64 + (c >> 1) * 32)));
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[c]) : "r"(at + meta_at[c & 1] + half * meta_half + (c >> 1) * meta_quarter + skip * 4) : "memory");
         }
-        tmem_st32(out + slot * 64 + s * 32, v);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          uint32_t v[32];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t s2 = i4_scale2(m[s * 2 + h]), o2 = i4_offset2(m[s * 2 + h]);
+            const uint32_t four[4] = {words[s * 2 + h].x, words[s * 2 + h].y, words[s * 2 + h].z, words[s * 2 + h].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t w[4];
+              i4_values(w, four[q], s2, o2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[h * 16 + q * 4 + e] = w[e];
+            }
+          }
+          if (half == 0 && s == 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(slot_empty + group, slot_phase, guard, kTimeoutAccEmpty));
+            tc_fence_after();
+          }
+          if (ok) tmem_st32(out + half * 64 + s * 32, v);
+        }
       }
+      if (!ok) break;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&slots_full[slot]);
-      if (++slot == kI4WSlots) { slot = 0; slot_phase ^= 1; }
-      const uint32_t ahead = 1 + half;
-      half ^= 1;
-      left -= ahead;
-      k += ahead;
-      at += ahead * a.stage_bytes;
-      if ((stage += ahead) >= a.stages) { stage -= a.stages; at -= a.stages * a.stage_bytes; phase ^= 1; }
+      if (lane == 0) {
+        mbar_arrive(slot_full + group);
+        if (a.keep) mbar_arrive(&empty[stage]);                      // nothing else of the stage is wanted
+      }
+      slot_phase ^= 1;
+      left -= kI4WGroups;
+      k += kI4WGroups;
+      at += kI4WGroups * a.stage_bytes;
+      if ((stage += kI4WGroups) >= a.stages) { stage -= a.stages; at -= a.stages * a.stage_bytes; phase ^= 1; }
     }
   } else {
     // ---------------------------------------------------------------- the warps that write: a weight row to a thread
@@ -290,7 +287,7 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
       bool with[kI4WGroups];                                         // a pass of one step has work for two groups
 #pragma unroll
       for (int g = 0; g < kI4WGroups; ++g) {
-        with[g] = (g + 3 - 2 * p * count % 3) % 3 < 2 * count;
+        with[g] = (g + 3 - p * count % 3) % 3 < count;
         if (with[g] && ok) ok = __all_sync(0xffffffffu, mbar_wait(&sums_full[g * 2 + taken[g] % sets], taken[g] / sets & 1, guard, kTimeoutAccFull));
       }
       if (a.parts > 1 && p > 0 && ok) ok = __all_sync(0xffffffffu, cluster_bar_wait(freed, (p - 1) & 1, guard, kTimeoutPeerFlag));
@@ -400,8 +397,8 @@ static int wide_room(int parts) {
 }
 
 // How `rooms` clusters of `parts` CTAs take N rows: quarters of a stage's time (0.6 us) of a CTA, with what a pass costs besides.  Measured with 1, 2, 4 and 8
-// CTAs to a cluster, 16 rows: [6144, 2560] 11.8 us, 9.8, 11.6, 16.4; [2560, 4096] 14.7, 11.4, 8.7, 10.7; [2560, 9728] 26.7, 19.1, 13.5, 14.6;
-// [19456, 2560] 18.6, 22.8, 25.8, 42.9.
+// CTAs to a cluster, 16 rows and half a stage at a time: [6144, 2560] 11.8 us, 9.8, 11.6, 16.4; [2560, 4096] 14.7, 11.4, 8.7, 10.7; [2560, 9728] 26.7, 19.1,
+// 13.5, 14.6; [19456, 2560] 18.6, 22.8, 25.8, 42.9.
 static int wide_cost(int N, int steps, int parts, int rooms, int* per_cluster, int* per_pass) {
   const int passes = (N + rooms * 128 - 1) / (rooms * 128);
   *per_pass = (N + rooms * passes - 1) / (rooms * passes);
@@ -439,8 +436,8 @@ int int4_linear_wide(const void* A, const void* codes, const void* meta, void* C
   a.stages = (kI4WSmemMost - rest) / a.stage_bytes;
   if (a.stages > passes * count + 2) a.stages = passes * count + 2;
   if (a.stages > kI4WMostStages) a.stages = kI4WMostStages;
-  a.stages = a.stages / 3 * 3;
-  KSA_REQUIRE(a.stages >= 3, "int4_linear: no room for three stages");
+  a.stages = a.stages / kI4WGroups * kI4WGroups;
+  KSA_REQUIRE(a.stages >= kI4WGroups, "int4_linear: no room for three stages");
   size_t smem = (size_t)a.stages * a.stage_bytes + rest;
   if (smem < (size_t)kTmemClusterAlone) smem = kTmemClusterAlone;            // all of the tensor memory: alone on its SM (host.h)
   static_assert(kI4WSmemMost >= kTmemClusterAlone, "the limit raised above covers it");

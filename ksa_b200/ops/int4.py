@@ -348,10 +348,10 @@ def int4_norm_linear(x: torch.Tensor, delta: Optional[torch.Tensor], norm_w: tor
 
 def _block_rows(N: int, K: int) -> int:
     """Rows up to which blocks of ``FEW_ROWS`` read the codes, once each.  More rows multiply with the bf16 values, written out for the call, at
-    a cost that hardly depends on them.  Measured, values against blocks: a weight of ``[1280, 1280]`` 6.5 us against 10.0 for 32 rows,
-    ``[2560, 4096]`` 13.7 against 10.5, ``[2560, 9728]`` 25.3 against 14.2, for 33 rows 13.8 against 15.5 and 25.5 against 22.3; what nearly fills
-    the L2 cache, ``[19456, 2560]``, 51.7 against 35.8 for 33 rows, 55 against 45 for 64, 55 against 62 for 80; values that outgrow it,
-    ``[151936, 2560]``, 378 against 332 for 128 rows."""
+    a cost that hardly depends on them.  Measured, values against blocks: a weight of ``[1280, 1280]`` 6.5 us against 9.3 for 32 rows,
+    ``[2560, 4096]`` 13.7 against 10.3, ``[2560, 9728]`` 25.3 against 13.5, for 33 rows 13.7 against 15.0 and 25.5 against 21.0; what nearly fills
+    the L2 cache, gate and up rows of ``[19456, 2560]``, 52 against 34 for 33 rows, 56 against 42 for 64, 58 against 61 for 96; values that outgrow it,
+    ``[151936, 2560]``, 379 against 311 for 128 rows."""
     return FUSED_ROWS if N * K <= 4 << 20 else 32 if 2 * N * K <= 64 << 20 else 64 if 2 * N * K <= 126 << 20 else 128
 
 
