@@ -284,7 +284,7 @@ int4_linear_wide_kernel(const __grid_constant__ CUtensorMap tm, const __grid_con
     int taken[kI4WGroups] = {};
     for (int p = 0; p < passes; ++p) {
       const int row = r0 + p * a.per_pass, rows = min(a.per_pass, r0 + mine - row);
-      bool with[kI4WGroups];                                         // a pass of one step has work for two groups
+      bool with[kI4WGroups];                                         // a pass of one or two steps has no work for some
 #pragma unroll
       for (int g = 0; g < kI4WGroups; ++g) {
         with[g] = (g + 3 - p * count % 3) % 3 < count;
