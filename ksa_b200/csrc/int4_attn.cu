@@ -11,7 +11,11 @@
 //     are values 32 t .. 32 t + 31 of it, one group with one scale; the order of the head dimension in the product is q's as well, so nothing is
 //     moved.  Keys are the 16 rows of the first product and value dimensions those of the second, queries the 8 columns of both, so up to
 //     eight heads waste no row; the probabilities become the second one's right operand by movmatrix.  V^T wants the same value of two
-//     neighbouring keys in a register, which is a byte permutation of two words before the shift.
+//     neighbouring keys in a register, which is a byte permutation of two words before the shift;
+//   * a probability enters the second product as two bf16 terms, its rounding and what that leaves, which keeps 16 bits of it.  Up to four heads leave
+//     half of the eight columns free, and these hold the same queries once more: there the second terms go along in the same instructions.  More
+//     heads cost the second product twice.  Against probabilities of eight bits: one sequence of 131071 slots, 32 heads over 8, 44.6 -> 45.9 us, 64 over 8
+//     49 -> 52.5; 16 of 32768, 32 over 8, 137 -> 142, 32 over 2 62 -> 69.5.
 // Nothing outside a slice enters a result: slots of the slice's first and last tile that lie outside get probability 0 and scale and offset 0, so
 // that a NaN there stays there.
 #include <math.h>
@@ -213,9 +217,16 @@ __device__ __forceinline__ void i4_store(bf16* out, const float4& o, float sum) 
   *reinterpret_cast<uint2*>(out) = y;
 }
 
-// NT: query heads of an item in eights (1 or 2).  kCluster: an item is shared by the kI4Cluster CTAs of a cluster, which merge through its shared memory.
-template <int D, int NT, bool kCluster>
+// A pair of probabilities without those bits of their bf16 roundings that `low` and `high` select (byte_perm): 0x1044 and 0x3244 all, 0x4444 none.
+__device__ __forceinline__ uint32_t i4_rest(float x, float y, uint32_t low, uint32_t high) {
+  const uint32_t r = pack_bf16x2(x, y);
+  return pack_bf16x2(x - __uint_as_float(__byte_perm(r, 0, low)), y - __uint_as_float(__byte_perm(r, 0, high)));
+}
+
+// NT: query heads of an item in eights (1 or 2).  kTwin: four heads at most, columns 4 to 7 are 0 to 3 again.  kCluster: an item is shared by the kI4Cluster CTAs of a cluster, which merge through its shared memory.
+template <int D, int NT, bool kTwin, bool kCluster>
 __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(const Int4Attn a, int* status) {
+  static_assert(!kTwin || NT == 1, "half of eight columns");
   constexpr int WK = D / 32;       // words of a key that a lane multiplies with the queries
   constexpr int WV = D / 64;       // words of a value row of which a lane holds the dimensions
   extern __shared__ __align__(128) uint8_t raw[];
@@ -307,6 +318,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
   int mine = warp, group = 0;      // this warp's tile, its group in the ring
   uint32_t phase = 0;
   int before = 0;                  // tiles of the run ahead of the item
+  const uint32_t low = t < 2 ? 0x4444 : 0x1044, high = t < 2 ? 0x4444 : 0x3244;            // kTwin: columns 0 to 3 take the rounding, the others the rest
   do {
     const int here = min(run - before, piece.n - piece.tile);      // tiles of the item in the run
     const int kvh = piece.head / a.blocks, h0 = kvh * (a.Hq / a.Hkv) + piece.head % a.blocks * a.heads;
@@ -319,8 +331,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
 #pragma unroll
       for (int w = 0; w < WK; ++w) {
         qv[n][w] = make_uint4(0, 0, 0, 0);
-        if (n * 8 + g < heads)
-          qv[n][w] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + tq * a.q_st + (h0 + n * 8 + g) * a.q_sh + t * (D / 4) + w * 8);
+        const int qe = kTwin ? g & 3 : n * 8 + g;
+        if (qe < heads) qv[n][w] = *reinterpret_cast<const uint4*>(a.q + b * a.q_sb + tq * a.q_st + (h0 + qe) * a.q_sh + t * (D / 4) + w * 8);
         qv[n][w].x ^= a.negate; qv[n][w].y ^= a.negate; qv[n][w].z ^= a.negate; qv[n][w].w ^= a.negate;
       }
     float o[WV * 4][NT][4], m[NT][2], l[NT][2];      // of queries 2 t and 2 t + 1 of each block
@@ -416,15 +428,18 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
               x[n][2 + e] = fmaf(c[n][2 + e], a.scale, -mx);
             }
         }
-        uint32_t pb[NT][2];
+        uint32_t pb[NT][2], rest[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[n][e] = fast_exp2(x[n][e]);
           l[n][0] += x[n][0] + x[n][2];
           l[n][1] += x[n][1] + x[n][3];
-          pb[n][0] = transpose8(pack_bf16x2(x[n][0], x[n][1]));
-          pb[n][1] = transpose8(pack_bf16x2(x[n][2], x[n][3]));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            pb[n][j] = transpose8(kTwin ? i4_rest(x[n][2 * j], x[n][2 * j + 1], low, high) : pack_bf16x2(x[n][2 * j], x[n][2 * j + 1]));
+            if (!kTwin) rest[n][j] = transpose8(i4_rest(x[n][2 * j], x[n][2 * j + 1], 0x1044, 0x3244));
+          }
         }
         // ---- out^T += V^T P^T: this lane's dimensions are D / 8 * g and on
         uint32_t rows[4][WV], meta[4];
@@ -460,13 +475,23 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], pb[n][0], pb[n][1]);
+            for (int n = 0; n < NT; ++n) {
+              mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], pb[n][0], pb[n][1]);
+              if (!kTwin) mma_bf16(o[w * 4 + i][n], even[0][i], odd[0][i], even[1][i], odd[1][i], rest[n][0], rest[n][1]);
+            }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[group]);
       mine += kI4Warps;
       if (++group == a.groups) { group = 0; phase ^= 1; }
+    }
+
+    if (kTwin) {
+#pragma unroll
+      for (int i = 0; i < WV * 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][0][e] += __shfl_xor_sync(0xffffffffu, o[i][0][e], 2);
     }
 
     // ---- the warps' parts of the item -> one
@@ -644,14 +669,14 @@ static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
   return s;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool kTwin>
 static int launch_int4_attn(const Int4Attn& a, const Int4Shape& s, cudaStream_t st) {
   constexpr int most = kI4SmShared / i4_ctas<NT>() - 1024;
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_decode_attn: no status word");
   if (s.cluster) {
     static PerDevice raised;
-    KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, true>, most));
+    KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, kTwin, true>, most));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(s.items * kI4Cluster));
     cfg.blockDim = dim3(kI4Threads);
@@ -666,12 +691,12 @@ static int launch_int4_attn(const Int4Attn& a, const Int4Shape& s, cudaStream_t 
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = dependent_launches() ? 2 : 1;
-    KSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, int4_attn_kernel<D, NT, true>, a, status));
+    KSA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, int4_attn_kernel<D, NT, kTwin, true>, a, status));
     return 0;
   }
   static PerDevice raised;
-  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, false>, most));
-  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT, false>, dim3(a.ctas), dim3(kI4Threads), s.smem, st, a, status));
+  KSA_CHECK_CUDA(raise_smem_limit(raised, int4_attn_kernel<D, NT, kTwin, false>, most));
+  KSA_CHECK_CUDA(launch_kernel(int4_attn_kernel<D, NT, kTwin, false>, dim3(a.ctas), dim3(kI4Threads), s.smem, st, a, status));
   KSA_CHECK_CUDA(launch_kernel(int4_attn_merge_kernel<D>, dim3(a.ctas, a.heads), dim3(kI4MergeWarps * 32), 0, st, a));
   return 0;
 }
@@ -712,6 +737,7 @@ KSA_API int ksa_int4_decode_attn(const void* q, const void* k, const void* k_met
              (int2*)(ws + parts * s.heads * (D + 2LL)), (bf16*)out, B * Tq, Tq, Hq, Hkv, cap, s.heads, s.blocks,
              s.ctas, s.groups, fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f), scale < 0.f ? 0x80008000u : 0u};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (D == 128) return s.heads <= 8 ? launch_int4_attn<128, 1>(a, s, st) : launch_int4_attn<128, 2>(a, s, st);
-  return s.heads <= 8 ? launch_int4_attn<64, 1>(a, s, st) : launch_int4_attn<64, 2>(a, s, st);
+  if (D == 128)
+    return s.heads <= 4 ? launch_int4_attn<128, 1, true>(a, s, st) : s.heads <= 8 ? launch_int4_attn<128, 1, false>(a, s, st) : launch_int4_attn<128, 2, false>(a, s, st);
+  return s.heads <= 4 ? launch_int4_attn<64, 1, true>(a, s, st) : s.heads <= 8 ? launch_int4_attn<64, 1, false>(a, s, st) : launch_int4_attn<64, 2, false>(a, s, st);
 }

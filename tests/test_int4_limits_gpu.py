@@ -1,0 +1,56 @@
+"""Operators in four bits at the ends of what they take: probabilities that need all their bits, scores and values at the ends of fp32,
+infinite activations, rows of any pitch and alignment."""
+import pytest
+import torch
+
+from ksa_b200 import ops
+from ksa_b200.ops import _lib, reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF = 2.0 ** -8                # a rounding to bf16, relative
+FP32 = 2.0 ** -23               # an addition in a matrix instruction, which may truncate
+
+
+def _randn(*shape, seed=0):
+    return torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).bfloat16()
+
+
+def _filled(k, v, cap):
+    """A cache of ``cap`` slots that holds rows ``k`` and ``v`` ``[B, n, H, D]`` from slot 0 on."""
+    B, n, H, D = k.shape
+    cache = ops.int4_cache(B, H, cap, D, DEV)
+    ops.int4_cache_write(cache, k, v, torch.arange(n, device=DEV, dtype=torch.int32).repeat(B, 1), distinct=True)
+    return cache
+
+
+def _exact(q, cache, lo, hi, scale):
+    """Attention of ``q`` ``[B, 1, Hq, D]`` over slots lo .. hi in 64 bits: the result, sum p |v|, the scores and sum |q k|."""
+    B, _, Hq, D = q.shape
+    H = cache.k.shape[1]
+    k, v = (ref.int4_values(c[:, :, lo:hi], s[:, :, lo:hi]).double() for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    qq = q.double().view(B, H, Hq // H, D)
+    z = qq @ k.transpose(2, 3) * scale
+    p = torch.softmax(z, -1)
+    return tuple(x.reshape(B, Hq, -1) for x in (p @ v, p @ v.abs(), z, qq.abs() @ k.abs().transpose(2, 3) * abs(scale)))
+
+
+# ------------------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (4, 2, 64), (32, 8, 128), (12, 2, 128), (16, 2, 64), (9, 1, 128), (32, 2, 64), (34, 2, 128)])
+@pytest.mark.parametrize("cap", [96, 16400])             # on clusters, and by runs of tiles with a merge
+@pytest.mark.parametrize("n", [1, 6, 40])
+def test_probabilities_are_not_rounded_to_bf16(Hq, Hkv, D, cap, n):
+    """Values that nearly cancel, so that a result's own rounding is small beside one of the probabilities.  Per output, A = sum p |v|: a score is off
+    by its fp32 additions (D at most, of sum |q k|), two fp32 products and the exponential (2^-21), in the numerator and the denominator; a probability
+    goes into the product as two bf16 terms, which leaves HALF * HALF of it; fp32 sums add 2^-23 for each of at most n + 64 additions in a row, above and below."""
+    B = 2
+    k, v = 0.5 * _randn(B, n, Hkv, D, seed=n), _randn(B, n, Hkv, D, seed=n + 1)
+    k[:, 1::2] = k[:, 0:n - n % 2:2] + 0.02 * _randn(B, n // 2, Hkv, D, seed=n + 2)
+    v[:, 1::2] = -v[:, 0:n - n % 2:2]
+    cache, q = _filled(k, v, cap), 0.5 * _randn(B, 1, Hq, D, seed=n + 3)
+    out = ops.int4_decode_attention(q, cache, torch.zeros(B, 1, device=DEV, dtype=torch.int32), torch.full((B, 1), n, device=DEV, dtype=torch.int32))
+    _lib.check_status()
+    expect, A, z, mag = _exact(q, cache, 0, n, D ** -0.5)
+    score = D * FP32 * mag.amax(-1, keepdim=True) + 2 * FP32 * z.abs().amax(-1, keepdim=True) + 2.0 ** -21
+    bound = HALF * expect.abs() + A * (HALF * HALF + 2.02 * score + 2 * (n + 64) * FP32)
+    assert float(((out[:, 0].double() - expect).abs() / bound.clamp(min=1e-30)).max()) <= 1
