@@ -525,7 +525,8 @@ class KsaInferenceEngine:
                     x, h2 = _add_norm(tp, x, attn_out, layer.mlp_norm.scale, cfg.norm_eps)
                     delta = self._mlp(layer, w4, h2[:B], tp)
         if fuse_norm and with_head:
-            out = ops.norm_linear(x, delta, model.norm.scale, cfg.norm_eps, model.lm_head_weight)[1]
+            out = (ops.norm_linear(x, delta, model.norm.scale, cfg.norm_eps, model.lm_head_weight) if self._int4_head is None else
+                   ops.int4_norm_linear(x, delta, model.norm.scale, cfg.norm_eps, self._int4_head))[1]
         else:
             _, out = _add_norm(tp, x[:B], delta[:B], model.norm.scale, cfg.norm_eps)
             out = self._logits(out) if with_head else out
