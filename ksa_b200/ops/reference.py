@@ -260,10 +260,10 @@ def int4_values(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """What codes ``[..., n / 2]`` with scales ``[..., groups, 2]`` stand for: ``[..., n]`` bf16."""
     b = codes.unflatten(-1, (-1, 4))
     c = torch.cat([b & 15, b >> 4], -1)[..., [0, 2, 4, 6, 1, 3, 5, 7]].flatten(-2)
-    u = (1 + c.float() / 16).unflatten(-1, (scale.shape[-2], -1))
-    # the product is exact in fp32 (13 bits); the sum is rounded to bf16 as if once, because where fp32 loses bits of it the product is less
-    # than a quarter of a step of the offset
-    return (u * scale[..., :1].float() + scale[..., 1:].float()).bfloat16().flatten(-2)
+    u = (1 + c.double() / 16).unflatten(-1, (scale.shape[-2], -1))
+    # the product has 13 bits, and passes fp32 in a group from -2^126 to 2^126; the sum is rounded to bf16 as if once, because where fp32 loses
+    # bits of it the product is less than a quarter of a step of the offset
+    return (u * scale[..., :1].double() + scale[..., 1:].double()).float().bfloat16().flatten(-2)
 
 
 def int4_decode_attention(q, k, k_scale, v, v_scale, start: torch.Tensor, length: torch.Tensor, scale: float):
