@@ -18,6 +18,7 @@
 //     49 -> 52.5; 16 of 32768, 32 over 8, 137 -> 142, 32 over 2 62 -> 69.5.
 // Nothing outside a slice enters a result: slots of the slice's first and last tile that lie outside get probability 0 and scale and offset 0, so
 // that a NaN there stays there.
+#include <float.h>
 #include <math.h>
 
 #include "host.h"
@@ -40,6 +41,11 @@ constexpr int i4_ctas() { return NT == 1 ? 3 : 2; }
 // Sixteen query heads a key head (32 over 2): one sequence of 4096 8.1 -> 8.8, two of 8192 15.5 -> 13.4, eight 20.4 -> 16.8, of 16384 24.8 -> 28.3.
 constexpr int kI4Cluster = 8, kI4ClusterSlots = 4096;
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
+// Probabilities are 2^(score - m), and m is the greatest score of some time ago plus kI4Above: it moves when a score is kI4Late powers of two above that
+// one.  Sums of up to 2^24 probabilities so stay below 1, and those of values, which reach 2^126, within fp32; what is lost are outputs below 2^-94.
+// Before the first score m is the least number, so that scores of minus infinity (products past fp32) weigh nothing.
+constexpr float kI4Late = 8.f, kI4Above = 32.f;
+constexpr float kI4Least = -FLT_MAX;
 
 struct Int4Attn {
   const bf16* q;                   // [B, Tq, Hq, D], strides below, heads' rows contiguous
@@ -209,8 +215,9 @@ __device__ __forceinline__ float2 ld_cluster(const float2* local, uint32_t rank)
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void i4_store(bf16* out, const float4& o, float sum) {
-  const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);       // 0: a slice without slots
+// Zeros for a slice without slots; one whose slots all weigh nothing is 0 / 0.
+__device__ __forceinline__ void i4_store(bf16* out, const float4& o, float sum, bool empty) {
+  const float inv = empty ? 0.f : __fdividef(1.f, sum);
   uint2 y;
   y.x = pack_bf16x2(o.x * inv, o.y * inv);
   y.y = pack_bf16x2(o.z * inv, o.w * inv);
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) { m[n][e] = -INFINITY; l[n][e] = 0.f; }
+      for (int e = 0; e < 2; ++e) { m[n][e] = kI4Least; l[n][e] = 0.f; }
 
     while (mine < before + here) {
       const int slot = group * kI4Warps + warp;
@@ -400,8 +407,8 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
             }
           }
         }
-        // ---- probabilities relative to m, which is the greatest score of some time ago: it moves when one is 16 powers of two above it (always
-        // in a warp's first block), so that most blocks need no maximum over their rows and no correction of the outputs
+        // ---- probabilities relative to m, which moves seldom (always in a warp's first block), so that most blocks need no maximum over their rows
+        // and no correction of the outputs
         float x[NT][4], top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
           for (int e = 0; e < 4; ++e) x[n][e] = fmaf(c[n][e], a.scale, -m[n][e & 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) top = max3(max3(top, x[n][0], x[n][1]), x[n][2], x[n][3]);
-        if (__builtin_expect(__any_sync(0xffffffffu, top > 16.f), 0)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, top > kI4Late - kI4Above), 0)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              mx = fmaxf(mx * a.scale, m[n][e]);
+              mx = fmaxf(fmaf(mx, a.scale, kI4Above), m[n][e]);
               const float corr = fast_exp2(m[n][e] - mx);
               m[n][e] = mx;
               l[n][e] *= corr;
@@ -534,7 +541,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
         *reinterpret_cast<float4*>(s_o + q * D + d) = acc;
         if (d == 0) s_ml[q] = make_float2(mx, sum);
       } else if (alone) {
-        i4_store(out + q * D + d, acc, sum);
+        i4_store(out + q * D + d, acc, sum, false);
       } else {
         *reinterpret_cast<float4*>(a.part_o + (part * a.heads + q) * D + d) = acc;
         if (d == 0) a.part_ml[part * a.heads + q] = make_float2(mx, sum);
@@ -563,7 +570,7 @@ __global__ void __launch_bounds__(kI4Threads, i4_ctas<NT>()) int4_attn_kernel(co
           sum = fmaf(ml[r].y, f, sum);
           acc.x = fmaf(x[r].x, f, acc.x); acc.y = fmaf(x[r].y, f, acc.y); acc.z = fmaf(x[r].z, f, acc.z); acc.w = fmaf(x[r].w, f, acc.w);
         }
-        i4_store(out + q * D + d, acc, sum);
+        i4_store(out + q * D + d, acc, sum, piece.n == 0);
       }
       cluster_sync();              // nobody leaves while its part may still be read
       return;

@@ -220,7 +220,8 @@ def int4_decode_attention(q: torch.Tensor, cache: Int4Cache, start: torch.Tensor
                           scale: Optional[float] = None) -> torch.Tensor:
     """``q`` ``[B, Tq, Hq, D]``: query ``(b, t)`` attends slots ``start[b, t] .. start[b, t] + length[b, t]`` of sequence ``b``, cut to the
     cache, with no mask inside; zeros where no slot is left.  ``Hq`` is a multiple of the cache's heads; ``D`` is 64 or 128
-    on a GPU; ``scale`` defaults to ``D ** -0.5``.  Slots outside a query's slice do not touch its result, whatever they hold."""
+    on a GPU; ``scale`` defaults to ``D ** -0.5``.  Slots outside a query's slice do not touch its result, whatever they hold.  A score below
+    what fp32 holds is minus infinity, and NaN comes out where all of a slice are."""
     if q.dim() == 4 and q.shape[3] > 0:
         made = _native.int4_decode_attention(q, *cache, start, length, q.shape[3] ** -0.5 if scale is None else scale)
         if made is not None:

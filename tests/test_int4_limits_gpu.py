@@ -54,3 +54,38 @@ def test_probabilities_are_not_rounded_to_bf16(Hq, Hkv, D, cap, n):
     score = D * FP32 * mag.amax(-1, keepdim=True) + 2 * FP32 * z.abs().amax(-1, keepdim=True) + 2.0 ** -21
     bound = HALF * expect.abs() + A * (HALF * HALF + 2.02 * score + 2 * (n + 64) * FP32)
     assert float(((out[:, 0].double() - expect).abs() / bound.clamp(min=1e-30)).max()) <= 1
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 128), (16, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("cap,n,low", [(96, 40, 16), (96, 90, 64), (16400, 300, 128), (16400, 300, 290)])
+def test_scores_below_fp32_get_no_weight(Hq, Hkv, D, cap, n, low):
+    """The scores of the first slots are products past -3.4e38; the plain form gives them no weight.  Bounds as in the test above, over the other slots."""
+    k, v, q = 0.1 * _randn(1, n, Hkv, D, seed=1), _randn(1, n, Hkv, D, seed=2), _randn(1, 1, Hq, D, seed=3).abs() + 1
+    k[:, :low] = -2.0 ** 126
+    cache = _filled(k, v, cap)
+    zero, whole = torch.zeros(1, 1, device=DEV, dtype=torch.int32), torch.full((1, 1), n, device=DEV, dtype=torch.int32)
+    out = ops.int4_decode_attention(q, cache, zero, whole)
+    expect, A, z, mag = _exact(q, cache, low, n, D ** -0.5)
+    score = D * FP32 * mag.amax(-1, keepdim=True) + 2 * FP32 * z.abs().amax(-1, keepdim=True) + 2.0 ** -21
+    bound = HALF * expect.abs() + A * (HALF + 2.02 * score + 2 * (n + 64) * FP32)
+    assert ((out[:, 0].double() - expect).abs() <= bound).all()
+    only = ops.int4_decode_attention(q, cache, zero, zero + low)                 # nothing has a weight: no number, as in the plain form
+    assert only.isnan().all() and ref.int4_decode_attention(q.cpu(), *(t.cpu() for t in cache), zero.cpu(), zero.cpu() + low, D ** -0.5).isnan().all()
+    assert (ops.int4_decode_attention(q, cache, zero, zero) == 0).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 2, 128), (16, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("cap,n", [(96, 90), (16400, 3000)])
+def test_values_as_large_as_the_format_holds(Hq, Hkv, D, cap, n):
+    """Values up to 2^126, and scores that rise by less than what moves the reference maximum: no sum of theirs may pass fp32."""
+    v = (_randn(1, n, Hkv, D, seed=1).sign() * 2.0 ** 126).bfloat16()
+    v[:, :, :, 0] = 2.0 ** 126
+    k = torch.zeros(1, n, Hkv, D, device=DEV, dtype=torch.bfloat16)
+    k[:, 16:, :, 0] = 10 / 8                                                       # e^10 = 2^14.4 times the weight of the first slots
+    cache, q = _filled(k, v, cap), torch.zeros(1, 1, Hq, D, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 8
+    out = ops.int4_decode_attention(q, cache, torch.zeros(1, 1, device=DEV, dtype=torch.int32), torch.full((1, 1), n, device=DEV, dtype=torch.int32), 1.0)
+    expect, A, z, mag = _exact(q, cache, 0, n, 1.0)
+    score = D * FP32 * mag.amax(-1, keepdim=True) + 2 * FP32 * z.abs().amax(-1, keepdim=True) + 2.0 ** -21
+    assert out.isfinite().all()
+    assert ((out[:, 0].double() - expect).abs() <= HALF * expect.abs() + A * (HALF + 2.02 * score + 2 * (n + 64) * FP32)).all()
