@@ -325,7 +325,7 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
     const bf16* xp = x_first;
     uint32_t xk = x_kept;
     for (int round = 0, seg = turn; round < rounds; ++round, seg += kTurns, xp += kTurns * 128, xk += kTurns * 256) {
-      // past K everything of the weights is zero, and any of the row's columns will do
+      // past K the weights are zeros, and so are the activations: an infinity there would make them NaN
       uint4 x[NB][4];
       if (kKept) {
 #pragma unroll
@@ -333,11 +333,11 @@ int4_linear_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant
 #pragma unroll
           for (int q = 0; q < 4; ++q) x[n][q] = ld_shared(xk + n * kept_eight + q * 64);
       } else {
-        const bf16* from = seg * 128 + t * 32 < a.K ? xp : x_first - (turn * 128 + t * 32);
+        const bool inside = seg * 128 + t * 32 < a.K;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) x[n][q] = *reinterpret_cast<const uint4*>(from + n * x_eight + q * 8);
+          for (int q = 0; q < 4; ++q) x[n][q] = inside ? *reinterpret_cast<const uint4*>(xp + n * x_eight + q * 8) : make_uint4(0, 0, 0, 0);
       }
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull));
       if (!ok) break;

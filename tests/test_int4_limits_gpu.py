@@ -89,3 +89,26 @@ def test_values_as_large_as_the_format_holds(Hq, Hkv, D, cap, n):
     score = D * FP32 * mag.amax(-1, keepdim=True) + 2 * FP32 * z.abs().amax(-1, keepdim=True) + 2.0 ** -21
     assert out.isfinite().all()
     assert ((out[:, 0].double() - expect).abs() <= HALF * expect.abs() + A * (HALF + 2.02 * score + 2 * (n + 64) * FP32)).all()
+
+
+# ------------------------------------------------------------------------------------------------- products
+@pytest.mark.parametrize("N,K,group", [(300, 160, 32), (5, 32, 32), (64, 2080, 32), (1000, 320, 64), (777, 384, 128), (12000, 1568, 32)])
+def test_infinite_activations(N, K, group):
+    """An infinity times a weight is one, and a NaN only where the weight is zero, wherever in the row it stands and however many rows there are."""
+    w = ops.int4_quantize_weight((_randn(N, K, seed=N) * 0.05).bfloat16(), group)
+    wd = ops.int4_dequantize_weight(w).double().cpu()
+    for M in (1, 5, 8, 11, 16, 20, 40):
+        x = _randn(M, K, seed=M)
+        for m, c in enumerate((3, K - 1, 31, K // 2, 0)):
+            if m < M:
+                x[m, c] = float("inf") if m % 2 == 0 else float("-inf")
+        expect = x.double().cpu() @ wd.t()
+        got = ops.int4_linear(x, w).double().cpu()
+        assert torch.equal(got.isnan(), expect.isnan()) and torch.equal(got[expect.isinf()], expect[expect.isinf()]), M
+        assert torch.equal(got.isfinite(), expect.isfinite())
+        if N % 2 == 0:
+            F = N // 2
+            glu, finite = ops.int4_linear_swiglu(x, w), expect.isfinite()
+            both = finite[:, :F] & finite[:, F:]
+            assert glu.cpu()[both].isfinite().all()
+    _lib.check_status()
