@@ -797,7 +797,7 @@ PyObject* py_int4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
     sizes.back() = out;
     y = a.empty(sizes);
     LAUNCH(ksa_int4_linear, x->const_data_ptr(), w->const_data_ptr(), s->const_data_ptr(), y.mutable_data_ptr(), (int)M, (int)N, (int)K,
-           (int)(K / groups), (int)pitch, x->dim() == 2 ? x->stride(0) : K, out, glu, a.stream());
+           (int)(K / groups), (int)pitch, x->is_contiguous() ? K : x->stride(0), out, glu, a.stream());      // (one row is contiguous at any pitch)
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS

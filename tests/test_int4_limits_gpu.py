@@ -112,3 +112,18 @@ def test_infinite_activations(N, K, group):
             both = finite[:, :F] & finite[:, F:]
             assert glu.cpu()[both].isfinite().all()
     _lib.check_status()
+
+
+def test_one_row_at_any_pitch():
+    """A single row counts as contiguous at any pitch."""
+    for N, K in ((200, 256), (12000, 1536)):
+        w = ops.int4_quantize_weight(_randn(N, K, seed=1))
+        wd = ops.int4_dequantize_weight(w).double()
+        for x in (_randn(K, 1, seed=2).t(), _randn(1, K + 3, seed=3)[:, :K], _randn(4, K + 1, seed=4)[:1, :K], _randn(1, K, seed=5).as_strided((1, K), (0, 1))):
+            assert x.is_contiguous()
+            for xx in (x, x[0], x[None]):
+                y = ops.int4_linear(xx, w)
+                expect, mag = xx.double() @ wd.t(), xx.double().abs() @ wd.abs().t()
+                assert y.shape == expect.shape
+                assert ((y.double() - expect).abs() <= HALF * expect.abs() + (K / 16 + 64) * FP32 * mag).all()
+            assert torch.equal(ops.int4_linear_swiglu(x, w), ops.int4_linear_swiglu(x.clone(), w))
