@@ -944,6 +944,7 @@ KSA_API int ksa_qknorm_rope_decode(const void* qkv, void* out, const void* q_w, 
   KSA_REQUIRE(D == 128, "qknorm_rope_decode: head_dim %d unsupported (128)", D);
   KSA_REQUIRE(k_cache == nullptr || (v_cache != nullptr && slots != nullptr && cache_rows <= rows && cap > 0),
               "qknorm_rope_decode: cache arguments are incomplete");
+  KSA_REQUIRE(in_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(qkv) & 3) == 0, "qknorm_rope_decode: rows must be 4-byte aligned");
   if (rows == 0) return 0;
   QkRopeArgs a{(const bf16*)qkv, (bf16*)out, (const bf16*)q_w, (const bf16*)k_w, (const int*)pos, nullptr,
                in_stride, out_stride, rows, Hq, Hkv, D, log2f(theta), eps, interleaved, 1};
@@ -967,6 +968,7 @@ KSA_API int ksa_qknorm_rope_decode_int4(const void* qkv, void* out, const void* 
   KSA_ENTER(qkv);
   KSA_REQUIRE(D == 128, "qknorm_rope_decode_int4: head_dim %d unsupported (128)", D);
   KSA_REQUIRE(cache_rows >= 0 && cache_rows <= rows && cap > 0, "qknorm_rope_decode_int4: %d rows for the cache of %d", cache_rows, rows);
+  KSA_REQUIRE(in_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(qkv) & 3) == 0, "qknorm_rope_decode_int4: rows must be 4-byte aligned");
   KSA_REQUIRE(((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes)) & 7) == 0 &&
               ((reinterpret_cast<uintptr_t>(k_meta) | reinterpret_cast<uintptr_t>(v_meta)) & 3) == 0, "qknorm_rope_decode_int4: misaligned cache");
   if (rows == 0) return 0;

@@ -530,6 +530,14 @@ def _qk_norm_weight_grads(qkv, d_out, q_w, k_w, pos, Hq, Hkv, D, theta, eps, int
     return out
 
 
+def _in_words(qkv: torch.Tensor) -> bool:
+    """Whether the pairs of values that the kernels read as words begin on four bytes."""
+    try:
+        return qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0
+    except RuntimeError:      # a wrapper of a transform: its calls meet the autograd function
+        return True
+
+
 def qk_norm_rope_packed(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Optional[torch.Tensor],
                         pos: torch.Tensor, Hq: int, Hkv: int, D: int, theta: float, eps: float = 1e-6,
                         interleaved: bool = False) -> torch.Tensor:
@@ -546,7 +554,9 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Opt
         return torch.cat([q.reshape(T, Hq * D), k.reshape(T, Hkv * D), qkv[:, (Hq + Hkv) * D:]], dim=1)
     _require_bf16(qkv, q_w, k_w)
     assert qkv.stride(1) == 1
-    return _run(_QkNormRopeFn, qkv, q_w, k_w, pos.to(torch.int32), Hq, Hkv, D, theta, eps, interleaved)
+    if not _in_words(qkv):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    return _run(_QkNormRopeFn, qkv, q_w, k_w, pos.to(torch.int32).contiguous(), Hq, Hkv, D, theta, eps, interleaved)
 
 
 def norm_linear(x: torch.Tensor, delta: Optional[torch.Tensor], norm_w: torch.Tensor, eps: float,
@@ -596,11 +606,13 @@ def qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Opt
     """``qk_norm_rope_packed`` for the few rows of a decode step, with the cache append in the same kernel: the new K
     and V of row ``i < len(slots)`` (sequence ``i``) also go to ``k_cache`` / ``v_cache`` ``[B, Hkv, cap, D]`` at slot
     ``slots[i]`` (negative: not cached); without a cache nothing else is written.  Inference only (no autograd)."""
+    if _cuda(qkv) and (qkv.stride(1) != 1 or not _in_words(qkv)):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
     if k_cache is None:
         if not (_cuda(qkv) and D == 128 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1):
             return qk_norm_rope_packed(qkv, q_w, k_w, pos, Hq, Hkv, D, theta, eps, interleaved)
         out = torch.empty((qkv.shape[0], (Hq + 2 * Hkv) * D), dtype=qkv.dtype, device=qkv.device)
-        _lib.call("ksa_qknorm_rope_decode", qkv, out, q_w, k_w, pos.to(torch.int32), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, Hkv, D,
+        _lib.call("ksa_qknorm_rope_decode", qkv, out, q_w, k_w, pos.to(torch.int32).contiguous(), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, Hkv, D,
                   float(theta), float(eps), int(interleaved), None, None, None, 0, 0)
         return out
     n = slots.numel()
@@ -609,7 +621,7 @@ def qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Opt
         out = torch.empty((T, (Hq + 2 * Hkv) * D), dtype=qkv.dtype, device=qkv.device)
         sl = slots.reshape(-1)
         sl = sl if sl.dtype == torch.int32 and sl.is_contiguous() else sl.to(torch.int32).contiguous()
-        _lib.call("ksa_qknorm_rope_decode", qkv, out, q_w, k_w, pos.to(torch.int32), qkv.stride(0), out.stride(0), T, Hq,
+        _lib.call("ksa_qknorm_rope_decode", qkv, out, q_w, k_w, pos.to(torch.int32).contiguous(), qkv.stride(0), out.stride(0), T, Hq,
                   Hkv, D, float(theta), float(eps), int(interleaved), k_cache, v_cache, sl, n, k_cache.shape[2])
         return out
     out = qk_norm_rope_packed(qkv, q_w, k_w, pos, Hq, Hkv, D, theta, eps, interleaved)

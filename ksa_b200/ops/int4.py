@@ -154,7 +154,6 @@ def int4_qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w
                              eps: float, interleaved: bool, cache: Int4Cache, slots: torch.Tensor) -> torch.Tensor:
     """``ops.qk_norm_rope_decode`` of rows ``[q | k | v]`` whose keys and values go, quantised, into ``cache``: those of row ``i < len(slots)``
     (sequence ``i``) into slot ``slots[i]``, as :func:`int4_cache_write` would write them; at head dim 128 in the same launch."""
-    from . import qk_norm_rope_decode
     B, H, cap, D = _check_cache(cache)
     _require(qkv.dim() == 2 and qkv.shape[1] == (Hq + 2 * H) * D, f"rows {tuple(qkv.shape)} are not {Hq} query and twice {H} key heads of {D}")
     _require(qkv.device == cache.k.device, "rows and cache are on different devices")
@@ -162,19 +161,31 @@ def int4_qk_norm_rope_decode(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w
     n = slots.numel()
     _require(n <= min(B, qkv.shape[0]), f"{n} slots for {qkv.shape[0]} rows and a cache of {B}")
     slots = _int32(slots.reshape(-1), (n,), cache.k.device, "slots")
-    if not (qkv.is_cuda and D == 128 and qkv.dtype == torch.bfloat16 and qkv.stride(1) == 1 and qkv.stride(0) % 2 == 0 and qkv.data_ptr() % 4 == 0):
-        out = qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, H, D, theta, eps, interleaved)
-        heads = out[:n, Hq * D:].view(n, 1, 2 * H, D)
-        int4_cache_write(cache.rows(slice(0, n)), heads[:, :, :H], heads[:, :, H:], slots.view(n, 1))
-        return out
     _require(pos.shape == qkv.shape[:1] and pos.device == qkv.device, f"positions {tuple(pos.shape)} for {qkv.shape[0]} rows")
     for w in (q_w, k_w):
-        _require(w is None or (w.shape == (D,) and w.dtype == qkv.dtype and w.device == qkv.device and w.is_contiguous() and w.data_ptr() % 4 == 0),
-                 f"norm weights are {D} contiguous bf16 values beside the rows")
-    out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _require(w is None or (w.shape == (D,) and w.device == qkv.device), f"norm weights are {D} values beside the rows")
+    if not qkv.is_cuda:
+        return _rotate_then_write(qkv, q_w, k_w, pos, Hq, theta, eps, interleaved, cache, slots)
+    for w in (q_w, k_w):
+        _require(w is None or (w.dtype == qkv.dtype and w.is_contiguous() and w.data_ptr() % 4 == 0), f"norm weights are {D} contiguous bf16 values")
+    pos = pos.to(torch.int32).contiguous()
+    if qkv.stride(1) != 1 or qkv.stride(0) % 2 != 0 or qkv.data_ptr() % 4 != 0:            # pairs of values are read as words
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
     with _on(qkv):
-        _lib.call("ksa_qknorm_rope_decode_int4", qkv, out, q_w, k_w, pos.to(torch.int32).contiguous(), qkv.stride(0), out.stride(0), qkv.shape[0], Hq, H,
-                  D, float(theta), float(eps), int(interleaved), cache.k, cache.k_scale, cache.v, cache.v_scale, slots, n, cap)
+        if D != 128 or qkv.dtype != torch.bfloat16:
+            return _rotate_then_write(qkv, q_w, k_w, pos, Hq, theta, eps, interleaved, cache, slots)
+        out = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _lib.call("ksa_qknorm_rope_decode_int4", qkv, out, q_w, k_w, pos, qkv.stride(0), out.stride(0), qkv.shape[0], Hq, H, D, float(theta), float(eps),
+                  int(interleaved), cache.k, cache.k_scale, cache.v, cache.v_scale, slots, n, cap)
+    return out
+
+
+def _rotate_then_write(qkv, q_w, k_w, pos, Hq, theta, eps, interleaved, cache, slots):
+    from . import qk_norm_rope_decode
+    H, D, n = cache.k.shape[1], 2 * cache.k.shape[3], slots.numel()
+    out = qk_norm_rope_decode(qkv, q_w, k_w, pos, Hq, H, D, theta, eps, interleaved)
+    heads = out[:n, Hq * D:].view(n, 1, 2 * H, D)
+    int4_cache_write(cache.rows(slice(0, n)), heads[:, :, :H], heads[:, :, H:], slots.view(n, 1))
     return out
 
 

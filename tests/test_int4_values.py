@@ -26,3 +26,28 @@ def test_groups_as_wide_as_the_format_holds(device):
         assert exact.isfinite().all() and got.isfinite().all()
         assert ((got.double() - exact).abs() <= 2.0 ** -8 * exact.abs()).all()
         assert torch.equal(got, ref.int4_values(codes, scale)[:, :, :4])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_rotation_of_rows_of_any_layout(device, D):
+    """Rows that begin between two words, at an odd pitch, or with strided values, and strided positions: as contiguous ones, to the bit."""
+    Hq, H, rows = 4, 2, 3
+    W, g = (Hq + 2 * H) * D, torch.Generator().manual_seed(1)
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    draw = lambda *shape: torch.randn(*shape, generator=g).to(device, dtype)
+    pos, slots = torch.tensor([5, 1, 900, 1, 77, 1], dtype=torch.int32, device=device)[::2], torch.tensor([3, 40, 9, 1], device=device)[::2]
+    for qkv in (draw(rows, W + 3)[:, 1:W + 1], draw(rows, W + 1)[:, :W], draw(rows * W + 1)[1:].view(rows, W), draw(W, rows).t(), draw(1, W).expand(rows, W)):
+        outs = []
+        for x, p, s in ((qkv, pos, slots), (qkv.clone(memory_format=torch.contiguous_format), pos.clone(), slots.clone())):
+            cache = ops.int4_cache(2, H, 16, D, device)
+            outs.append((ops.int4_qk_norm_rope_decode(x, None, None, p, Hq, 1e4, 1e-6, False, cache, s), *cache))
+            outs[-1] += (ops.qk_norm_rope_decode(x, None, None, p, Hq, H, D, 1e4, 1e-6, False),)
+            k, v = (torch.zeros(2, H, 16, D, dtype=dtype, device=device) for _ in range(2))
+            outs[-1] += (ops.qk_norm_rope_decode(x, None, None, p, Hq, H, D, 1e4, 1e-6, False, k, v, s), k, v)
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+        assert outs[0][1][0, :, 3].any()
+    cache, qkv, ones = ops.int4_cache(2, H, 16, D, device), draw(rows, W), torch.ones(D, device=device, dtype=dtype)
+    for bad in ((ones[:D // 2], None, pos), (None, torch.ones(2 * D, device=device, dtype=dtype), pos), (None, None, pos[:2]), (None, None, pos[:, None])):
+        with pytest.raises(ValueError):
+            ops.int4_qk_norm_rope_decode(qkv, *bad, Hq, 1e4, 1e-6, False, cache, slots)
