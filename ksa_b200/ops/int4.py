@@ -337,25 +337,36 @@ def int4_norm_linear(x: torch.Tensor, delta: Optional[torch.Tensor], norm_w: tor
     _require(not glu or N % 2 == 0, f"{N} rows are not as many gate as up rows")
     _require(all(t is None or t.device == weight.codes.device for t in (x, delta, norm_w)), "rows, norm and weight are on different devices")
     _require_inference(x, norm_w.detach(), *(() if delta is None else (delta,)))
-    M = x.shape[0]
-    rows = [t for t in (x, delta) if t is not None]
-    if (x.is_cuda and 0 < M <= NORM_ROWS and M * K <= NORM_VALUES and N > 0 and norm_w.is_contiguous() and norm_w.data_ptr() % 16 == 0
-            and all(t.dtype == torch.bfloat16 for t in (*rows, norm_w))
-            and all(t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 for t in rows)):
+    if not x.is_cuda:
+        res, h = (x, rms_norm(x, norm_w.detach(), eps)) if delta is None else add_rms_norm(x, delta, norm_w.detach(), eps)
+        return res, _linear(h, weight, glu)
+    M, norm_w = x.shape[0], norm_w.detach()
+    if not norm_w.is_contiguous() or norm_w.data_ptr() % 16 != 0:
+        norm_w = norm_w.clone(memory_format=torch.contiguous_format)
+    rows, delta = _aligned_rows(x), None if delta is None else _aligned_rows(delta)
+    n = 0 if delta is None else delta.shape[0]
+    if 0 < M <= NORM_ROWS and M * K <= NORM_VALUES and N > 0 and all(t is None or t.dtype == torch.bfloat16 for t in (x, delta, norm_w)):
         res = x if delta is None else torch.empty((M, K), dtype=x.dtype, device=x.device)
         y = torch.empty((M, N // 2 if glu else N), dtype=x.dtype, device=x.device)
         with _on(x):
-            _lib.call("ksa_int4_norm_linear", x, delta, norm_w.detach(), None if delta is None else res, weight.codes, weight.scale, y, M, N, K, group, pitch,
-                      x.stride(0), K if delta is None else delta.stride(0), K, y.shape[1], float(eps), 0 if delta is None else delta.shape[0], int(glu))
+            _lib.call("ksa_int4_norm_linear", rows, delta, norm_w, None if delta is None else res, weight.codes, weight.scale, y, M, N, K, group, pitch,
+                      rows.stride(0), K if delta is None else delta.stride(0), K, y.shape[1], float(eps), n, int(glu))
         return res, y
     step = min(NORM_ROWS, NORM_VALUES // K)
-    if x.is_cuda and step < M and step > 0 and (M <= NORM_ROWS or K > 8192):       # rows wider than the norm's own kernel takes, too
-        parts = [int4_norm_linear(x[r:r + step], None if delta is None or r >= delta.shape[0] else delta[r:r + step], norm_w, eps, weight, glu)
-                 for r in range(0, M, step)]
+    if step < M <= NORM_ROWS and step > 0:
+        parts = [int4_norm_linear(rows[r:r + step], None if r >= n else delta[r:r + step], norm_w, eps, weight, glu) for r in range(0, M, step)]
         return x if delta is None else torch.cat([res for res, _ in parts]), torch.cat([y for _, y in parts])
-    with (_on(x) if x.is_cuda else contextlib.nullcontext()):
-        res, h = (x, rms_norm(x, norm_w.detach(), eps)) if delta is None else add_rms_norm(x, delta, norm_w.detach(), eps)
+    with _on(x):
+        if K > 8192:               # wider than the norm's own kernel takes
+            res = x if delta is None else torch.cat([(rows[:n].float() + delta.float()).to(x.dtype), rows[n:]])
+            return res, _linear(ref.rms_norm(res, norm_w, eps), weight, glu)
+        res, h = (x, rms_norm(rows, norm_w, eps)) if delta is None else add_rms_norm(rows, delta, norm_w, eps)
         return res, _linear(h, weight, glu)
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` ``[M, K]`` with rows that kernels can read: on 16 bytes, beside or behind one another."""
+    return x if x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _block_rows(N: int, K: int) -> int:

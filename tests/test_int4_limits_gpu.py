@@ -127,3 +127,32 @@ def test_one_row_at_any_pitch():
                 assert y.shape == expect.shape
                 assert ((y.double() - expect).abs() <= HALF * expect.abs() + (K / 16 + 64) * FP32 * mag).all()
             assert torch.equal(ops.int4_linear_swiglu(x, w), ops.int4_linear_swiglu(x.clone(), w))
+
+
+def _layouts(M, K):
+    """Rows between two vectors of 16 bytes, at an odd pitch, with strided values, one row for all, rows within one another."""
+    return (_randn(M * K + 1, seed=2)[1:].view(M, K), _randn(M, K + 3, seed=3)[:, 1:K + 1], _randn(K, M, seed=4).t(), _randn(1, K, seed=5).expand(M, K),
+            _randn(M * K, seed=6).as_strided((M, K), (8, 1)))
+
+
+@pytest.mark.parametrize("M", [1, 3, 4, 9])
+@pytest.mark.parametrize("K", [256, 8192, 9728, 40960])
+def test_norm_ahead_of_the_product_takes_rows_of_any_layout_and_width(M, K):
+    """Bounds as in the test of this operator: a rounding of the norm, 2^-20 of its fp32, and those of the product."""
+    w = ops.int4_quantize_weight((_randn(64, K, seed=1) * 0.1).bfloat16())
+    wd, norm_w = ops.int4_dequantize_weight(w).double(), (1 + _randn(2 * K + 1, seed=2) * 0.2).bfloat16()
+    for x in _layouts(M, K):
+        for delta in (None, _randn(M, K + 1, seed=7)[:, 1:], _randn(K, M // 2, seed=8).t()):
+            for nw in (norm_w[1:K + 1], norm_w[:2 * K:2]):
+                res, y = ops.int4_norm_linear(x, delta, nw, 1e-6, w)
+                expect = x.clone(memory_format=torch.contiguous_format)
+                if delta is not None:
+                    n = delta.shape[0]
+                    expect[:n] = (expect[:n].float() + delta.float()).bfloat16()
+                assert torch.equal(res, expect)
+                r = expect.double()
+                h = r * (r.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * nw.double()
+                p, mag = h @ wd.t(), h.abs() @ wd.abs().t()
+                assert ((y.double() - p).abs() <= (HALF + 2.0 ** -20) * 1.01 * mag + HALF * p.abs() * 1.01 + (K / 16 + 64) * FP32 * mag * 1.01).all()
+                assert torch.equal(ops.int4_norm_linear(x, delta, nw, 1e-6, w, True)[1].isfinite(), torch.ones(M, 32, device=DEV, dtype=torch.bool))
+    _lib.check_status()
