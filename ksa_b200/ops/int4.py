@@ -400,20 +400,20 @@ def _linear(x: torch.Tensor, weight: Int4Weight, glu: bool) -> torch.Tensor:
         y = _linear(x.reshape(M, K), weight, False)
         with _on(x):
             return (swiglu(y) if N % 16 == 0 else ref.swiglu(y)).view(out_shape)
+    rows = _aligned_rows(x.reshape(M, K))
+    if rows.stride(0) < K:
+        rows = rows.clone(memory_format=torch.contiguous_format)
     if M > _block_rows(N, K):
         from . import linear, swiglu
         values = torch.empty((-(-N // 8) * 8, K), dtype=torch.bfloat16, device=x.device)       # the products take columns in eights
         values[N:].zero_()
         _weight_values(weight, values)
         with _on(x):
-            y = linear(x.reshape(M, K), values)
+            y = linear(rows, values)
             if glu:
                 gate, up = y[:, :N // 2], y[:, N // 2:N]
                 y = swiglu(y) if N % 16 == 0 else ref.swiglu(torch.cat([gate, up], -1))
         return (y if glu or N % 8 == 0 else y[:, :N].contiguous()).view(out_shape)
-    rows = x.reshape(M, K)
-    if rows.stride(1) != 1 or rows.stride(0) % 8 != 0 or rows.stride(0) < K or rows.data_ptr() % 16 != 0:
-        rows = rows.clone(memory_format=torch.contiguous_format)
     out = torch.empty((M, out_shape[-1]), dtype=x.dtype, device=x.device)
     with _on(x):
         for r in range(0, M, FEW_ROWS):

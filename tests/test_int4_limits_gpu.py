@@ -135,6 +135,18 @@ def _layouts(M, K):
             _randn(M * K, seed=6).as_strided((M, K), (8, 1)))
 
 
+@pytest.mark.parametrize("N,K", [(96, 256), (2500, 2048)])
+def test_many_rows_of_any_layout(N, K):
+    w = ops.int4_quantize_weight((_randn(N, K, seed=1) * 0.1).bfloat16())
+    for M in (12, 30, 200):
+        for x in _layouts(M, K):
+            plain = x.clone(memory_format=torch.contiguous_format)
+            wd = ops.int4_dequantize_weight(w).double()
+            expect, mag = plain.double() @ wd.t(), plain.double().abs() @ wd.abs().t()
+            assert ((ops.int4_linear(x, w).double() - expect).abs() <= HALF * expect.abs() + (K / 16 + 64) * FP32 * mag).all()
+            assert torch.equal(ops.int4_linear_swiglu(x, w), ops.int4_linear_swiglu(plain, w))
+
+
 @pytest.mark.parametrize("M", [1, 3, 4, 9])
 @pytest.mark.parametrize("K", [256, 8192, 9728, 40960])
 def test_norm_ahead_of_the_product_takes_rows_of_any_layout_and_width(M, K):
