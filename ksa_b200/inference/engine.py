@@ -157,7 +157,7 @@ class _Int4Layer:
 
 class KsaInferenceEngine:
     """``kv_cache="int4"`` holds keys and values in four bits (5 bits a value with their scales, ``ops.int4``): they are quantised as
-    they are written, and decode steps attend over the quantised values; the prompt's own attention is unchanged.
+    they are written, and decode steps attend over the quantised values; the prompt's own attention is unchanged; head dims of 64 and 128.
     ``weights="int4"`` lets decode steps read projections and output head in four bits (groups of ``weight_group`` values along a
     row), quantised when the engine is made; prefill keeps the model's weights, which stay in memory.  Tensor parallelism takes the cache, not the weights."""
 
@@ -165,6 +165,10 @@ class KsaInferenceEngine:
                  weights: str = "bf16", weight_group: int = 64):
         if kv_cache not in ("bf16", "int4") or weights not in ("bf16", "int4"):
             raise ValueError(f"kv_cache and weights are 'bf16' (the model's type) or 'int4', got {kv_cache!r} and {weights!r}")
+        head_dim, cuda = model.config.head_dim, next(model.parameters()).is_cuda
+        if kv_cache == "int4" and (head_dim not in (64, 128) if cuda else head_dim % 64 != 0 and any(layer.is_summary_layer for layer in model.layers)):
+            # what attention on a GPU takes, and what a closed chunk's move takes
+            raise ValueError(f"a cache in four bits takes head dims of {'64 and 128' if cuda else '64 and its multiples'}, the model has {head_dim}")
         if weights == "int4" and getattr(model, "tp", None) is not None:
             raise ValueError("weights in four bits are not available with tensor parallelism")
         self.model = model.eval()

@@ -67,3 +67,14 @@ def test_steps_read_the_codes_alone(device, B, own_summary):
         logits, got = plain.decode_step(token), eng.decode_step(token)
         off = float((got.float() - logits.float()).norm() / logits.float().norm())
         assert off < bound, (step, off)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("head", [32, 96])
+def test_head_dims_are_refused_when_the_engine_is_made(device, head):
+    """A cache of such heads can be written; its attention (on a GPU) and its moves cannot, and the first step or closed chunk would say so."""
+    cfg = get_preset("qwen3-ksa-tiny").merge({"num_layers": 2, "summary_layer_freq": [1, 0], "embed_dim": 64, "intermediate_dim": 128, "vocab_size": 512,
+                                              "head_dim": head, "num_heads": 2, "num_kv_heads": 1, "summary_chunk_size": 8, "summary_token_begin": 505})
+    model = get_model_class(cfg.model_class)(cfg).eval().to(device)
+    with pytest.raises(ValueError):
+        KsaInferenceEngine(model, 64, 1, kv_cache="int4")
