@@ -435,7 +435,7 @@ static int int4_linear(const void* A, const void* codes, const void* meta, void*
   const int sms = sm_count();
   KSA_REQUIRE(sms > 0, "int4_linear: no device");
   if (norm == nullptr && !glu && !spread && (M > kI4LMostRows || (M > 8 && K >= kI4LWideColumns && N >= kI4LWideRows * sms)))
-    return int4_linear_wide(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, 0, st);
+    return int4_linear_wide(A, codes, meta, C, M, N, K, group, pitch, lda, ldc, st);
   Int4Linear a{};
   a.A = (const bf16*)A; a.meta = (const uint32_t*)meta; a.C = (bf16*)C;
   a.lda = lda; a.ldc = ldc; a.M = M; a.N = N; a.K = K; a.group = group; a.pitch = pitch;

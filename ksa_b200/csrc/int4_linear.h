@@ -7,8 +7,8 @@ namespace ksa {
 
 constexpr int kI4WMostRows = 32, kI4WMostParts = 8;
 
-// Up to 32 rows with a pitch lda >= K; `parts` CTAs share K (0: as the sizes suggest).
+// Up to 32 rows with a pitch lda >= K.
 int int4_linear_wide(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda, long long ldc,
-                     int parts, cudaStream_t st);
+                     cudaStream_t st);
 
 }  // namespace ksa

@@ -409,7 +409,7 @@ static int wide_cost(int N, int steps, int parts, int rooms, int* per_cluster, i
 }
 
 int int4_linear_wide(const void* A, const void* codes, const void* meta, void* C, int M, int N, int K, int group, int pitch, long long lda, long long ldc,
-                     int parts, cudaStream_t st) {
+                     cudaStream_t st) {
   int* status = status_word();
   KSA_REQUIRE(status != nullptr, "int4_linear: no status word");
   static PerDevice raised;
@@ -419,14 +419,14 @@ int int4_linear_wide(const void* A, const void* codes, const void* meta, void* C
   a.cols = (M + 15) / 16 * 16;
   a.steps = (K + kI4WStep - 1) / kI4WStep;
   int best = 0;
-  for (int p = parts > 0 ? parts : 1; p <= (parts > 0 ? parts : kI4WMostParts) && p <= a.steps; p *= 2) {
+  for (int p = 1; p <= kI4WMostParts && p <= a.steps; p *= 2) {
     const int room = p == 1 ? sm_count() : wide_room(p);
     if (room <= 0) continue;
     int per_cluster, per_pass;
     const int cost = wide_cost(N, a.steps, p, room, &per_cluster, &per_pass);
     if (a.parts == 0 || cost < best) { best = cost; a.parts = p; a.per_cluster = per_cluster; a.per_pass = per_pass; }
   }
-  KSA_REQUIRE(a.parts > 0, "int4_linear: no room for a cluster of %d", parts);
+  KSA_REQUIRE(a.parts > 0, "int4_linear: no device");
   const int passes = a.per_cluster / a.per_pass, count = (a.steps + a.parts - 1) / a.parts, step_x = 4 * a.cols * 128;
   a.keep = passes > 1 && (long long)count * step_x <= kI4WKeepMost ? count * step_x : 0;
   a.meta_words = (a.per_pass + 3 + 3) / 4 * 4;
