@@ -7,7 +7,8 @@ or 128 along ``K`` of a weight row) with least value ``lo`` and greatest ``hi`` 
 ``c = rint((x - O) / S * 16) - 16``, cut to 0 .. 15, stands for ``bf16(S * (1 + c / 16) + O)``: those bf16 values are what reading
 returns and what attention and products compute with, to the bit.  The error is at most half a step, ``(hi - lo) / 30``, and the
 roundings of ``S``, ``O`` and the result to bf16.  Eight codes make a little-endian 32-bit word, its nibbles from the lowest being
-values 0, 2, 4, 6, 1, 3, 5, 7.  A group that holds an infinity or a NaN stands for NaN; finite magnitudes over 2^126 count as 2^126.
+values 0, 2, 4, 6, 1, 3, 5, 7.  A group that holds an infinity or a NaN stands for NaN; finite magnitudes over 2^126 count as 2^126, and those
+below 2^-126 as zero.
 """
 from __future__ import annotations
 

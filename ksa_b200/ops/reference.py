@@ -236,7 +236,7 @@ def decode_attention(q, k_cache, v_cache, lengths: torch.Tensor, start: Optional
 
 
 # ---------------------------------------------------------------- four bits
-_INT4_LEAST, _INT4_MOST = 2.0 ** -100, 2.0 ** 126
+_INT4_LEAST, _INT4_MOST, _INT4_NORMAL = 2.0 ** -100, 2.0 ** 126, 2.0 ** -126
 
 
 def int4_quantize(x: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -245,6 +245,7 @@ def int4_quantize(x: torch.Tensor, group: int) -> Tuple[torch.Tensor, torch.Tens
     x = x.float().unflatten(-1, (-1, group))
     bad = ~torch.isfinite(x).all(-1, keepdim=True)
     x = torch.nan_to_num(x, nan=0.0).clamp(-_INT4_MOST, _INT4_MOST)
+    x = torch.where(x.abs() < _INT4_NORMAL, torch.zeros_like(x), x)
     lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
     s = ((hi - lo) / torch.full_like(lo, 15) * 16).bfloat16().float()    # a division: by a number, a GPU multiplies with 1 / 15
     s = torch.where(s < _INT4_LEAST, torch.zeros_like(s), s)

@@ -51,3 +51,19 @@ def test_rotation_of_rows_of_any_layout(device, D):
     for bad in ((ones[:D // 2], None, pos), (None, torch.ones(2 * D, device=device, dtype=dtype), pos), (None, None, pos[:2]), (None, None, pos[:, None])):
         with pytest.raises(ValueError):
             ops.int4_qk_norm_rope_decode(qkv, *bad, Hq, 1e4, 1e-6, False, cache, slots)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_magnitudes_below_the_normal_ones_count_as_zero(device):
+    x = torch.randn(2, 4, 1, 64, generator=torch.Generator().manual_seed(0)).bfloat16() * 1e-30
+    x[0], x[0, 1], x[0, 2], x[0, 3, :, 5] = 0, -2e-39, 1e-39, 2e-39
+    x[1, :, :, ::3] = 1e-39
+    zeroed = torch.where(x.abs() < 2.0 ** -126, torch.zeros_like(x), x)
+    assert not torch.equal(x, zeroed)
+    slots, made = torch.arange(4).repeat(2, 1), []
+    for rows, dev in ((x, device), (zeroed, "cpu")):
+        cache = ops.int4_cache(2, 1, 16, 64, dev)
+        ops.int4_cache_write(cache, rows.to(dev), rows.to(dev), slots.to(dev))
+        made.append([t.cpu().float() for t in (*cache, *ops.int4_cache_read(cache, torch.zeros(2, dtype=torch.int32, device=dev), 4))])
+    assert all(torch.equal(a, b) for a, b in zip(*made))
+    assert made[0][4][0].count_nonzero() == 0
