@@ -35,10 +35,11 @@ template <int NT>
 constexpr int i4_ctas() { return NT == 1 ? 3 : 2; }
 // Short slices: the CTAs of an item are a cluster and merge through its shared memory, in one launch and with nothing to look up but the own row's
 // slice.  Full caches took, in us, by the sequence and here (32 query heads, 8 key heads of
-// 128): one sequence of 256 slots 5.8 -> 4.0, 1168 8.6 -> 5.0, 4096 7.2 -> 7.1, 8192 11.1 -> 11.4, 16384 14.8 -> 19.7; six of 1168 10.9 -> 6.5, of
-// 4096 16.3 -> 12.3, of 16384 29.5 -> 31.7; in two rounds of clusters twelve of 1168 13.9 -> 13.0, of 2048 16.6 -> 16.3, of 4096 21.0 -> 22.7; in
-// four 24 of 1168 17.7 -> 25.0.
-// Sixteen query heads a key head (32 over 2): one sequence of 4096 8.1 -> 8.8, two of 8192 15.5 -> 13.4, eight 20.4 -> 16.8, of 16384 24.8 -> 28.3.
+// 128): one sequence of 256 slots 6.0 -> 4.0, 1168 8.9 -> 5.0, 4096 7.9 -> 7.7, 8192 12.2 -> 11.9, 16384 14.8 -> 19.7; six of 1168 12.1 -> 7.6, of
+// 4096 17.1 -> 12.6, of 16384 37 -> 35; in two rounds of clusters twelve of 1168 14.8 -> 14.6, of 2048 17.4 -> 17.0, of 4096 24.0 -> 25.1; in
+// four 24 of 1168 19.2 -> 28.4.
+// Sixteen query heads a key head: two items of 2048 slots 9.1 -> 6.8, of 4096 8.3 -> 9.3, of 8192 10.8 -> 14.9; four of 4096 10.4 -> 9.7, of 8192 13.7 -> 15.1;
+// eight of 8192 19.2 -> 16.5, sixteen 21.6 -> 20.4.  So more than four items go up to twice as many slots.
 constexpr int kI4Cluster = 8, kI4ClusterSlots = 4096;
 constexpr int kI4Align = 16;       // tiles start at multiples of this, and so does the capacity
 // Probabilities are 2^(score - m), and m is the greatest score of some time ago plus kI4Above: it moves when a score is kI4Late powers of two above that
@@ -672,7 +673,7 @@ static Int4Shape i4_shape(int rows, int Hq, int Hkv, int D, int cap) {
   const long long most = (s.tiles + kI4Spread - 1) / kI4Spread, room = (long long)sm_count() * per_sm;
   s.ctas = (int)(most < 1 ? 1 : most < room ? most : room);
   const long long rounds = (s.items * kI4Cluster + room - 1) / room;
-  s.cluster = rounds <= 2 && cap <= (s.heads <= 8 ? kI4ClusterSlots : 2 * kI4ClusterSlots) / rounds;
+  s.cluster = rounds <= 2 && cap <= (s.heads > 8 && s.items > 4 ? 2 * kI4ClusterSlots : kI4ClusterSlots) / rounds;
   return s;
 }
 
