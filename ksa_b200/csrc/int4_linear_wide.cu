@@ -10,7 +10,7 @@
 //   * four more warps add up the groups' sums of a pass, in their order, and write them while the next pass is being unpacked;
 //   * activations that several passes want and that fit stay in shared memory, others come with each stage;
 //   * few rows of the weight: the CTAs of a cluster share K, and each adds up some of the activation rows from the others' shared memory.
-// Measured on 32 rows: [151936, 2560] 81 us (2.7 TB/s), [19456, 2560] 18, [6144, 2560] 12.0, [2560, 9728] 13.5 on clusters of four.
+// Measured on 32 rows: [151936, 2560] 78 us (2.8 TB/s), [19456, 2560] 20, [6144, 2560] 11.8, [2560, 9728] 13.3 on clusters of four.
 #include "int4_linear.h"
 
 #include "host.h"
@@ -29,7 +29,7 @@ constexpr int kI4WSums = kI4WGroups * 128;          // each group unpacks a stag
 constexpr int kI4WMostStages = 15;                  // a multiple of three: a stage of the ring belongs to the same groups all the time
 constexpr int kI4WSmemMost = 227 * 1024;
 // Activations that stay, up to so many bytes, where several passes want them: 32 rows of [40000, 2048] (128 KB) 25.0 -> 24.2 us, but of [151936, 2560]
-// (160 KB, three stages left) 75.7 -> 81.8.
+// (160 KB, three stages left) 80 -> 85.
 constexpr int kI4WKeepMost = 128 * 1024;
 
 struct Int4Wide {

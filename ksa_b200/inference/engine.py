@@ -159,7 +159,8 @@ class KsaInferenceEngine:
     """``kv_cache="int4"`` holds keys and values in four bits (5 bits a value with their scales, ``ops.int4``): they are quantised as
     they are written, and decode steps attend over the quantised values; the prompt's own attention is unchanged; head dims of 64 and 128.
     ``weights="int4"`` lets decode steps read projections and output head in four bits (groups of ``weight_group`` values along a
-    row), quantised when the engine is made; prefill keeps the model's weights, which stay in memory.  Tensor parallelism takes the cache, not the weights."""
+    row), quantised when the engine is made; prefill keeps the model's weights, which stay in memory.  It pays up to 16 sequences: a step of KSA-4B after 8192
+    tokens 2.28 -> 1.84 ms for one and 4.37 -> 4.11 for 16, but 5.54 -> 5.74 for 32 after 4096.  Tensor parallelism takes the cache, not the weights."""
 
     def __init__(self, model, max_len: int, batch: int, device=None, dtype=None, cuda_graph: bool = True, kv_cache: str = "bf16",
                  weights: str = "bf16", weight_group: int = 64):
