@@ -554,7 +554,7 @@ def qk_norm_rope_packed(qkv: torch.Tensor, q_w: Optional[torch.Tensor], k_w: Opt
         return torch.cat([q.reshape(T, Hq * D), k.reshape(T, Hkv * D), qkv[:, (Hq + Hkv) * D:]], dim=1)
     _require_bf16(qkv, q_w, k_w)
     assert qkv.stride(1) == 1
-    if not _in_words(qkv):
+    if not _observed() and not _in_words(qkv):
         qkv = qkv.clone(memory_format=torch.contiguous_format)
     return _run(_QkNormRopeFn, qkv, q_w, k_w, pos.to(torch.int32).contiguous(), Hq, Hkv, D, theta, eps, interleaved)
 
