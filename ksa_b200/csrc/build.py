@@ -28,9 +28,15 @@ NVCC_FLAGS = [
 ]
 
 
-def _flags() -> list:
+# Sources whose fp32 results are held to rounding errors: exponentials, logarithms, quotients and subnormal numbers as the standard has
+# them.  Memory bounds all of them.
+EXACT_SOURCES = ("grad_norm.cu", "token_losses.cu")
+
+
+def _flags(src: Path = None) -> list:
     """Release flags, plus the device-side bounds checks when ``KSA_DEBUG=1`` is set."""
-    return NVCC_FLAGS + (["-DKSA_DEBUG_CHECKS"] if os.environ.get("KSA_DEBUG") == "1" else [])
+    flags = NVCC_FLAGS + (["-DKSA_DEBUG_CHECKS"] if os.environ.get("KSA_DEBUG") == "1" else [])
+    return [f for f in flags if f != "--use_fast_math"] if src is not None and src.name in EXACT_SOURCES else flags
 
 
 def _nvcc() -> str:
@@ -54,7 +60,7 @@ def _compile(src: Path, force: bool, verbose: bool) -> Path:
     newest = max(src.stat().st_mtime, _headers_mtime())
     if not force and obj.exists() and obj.stat().st_mtime >= newest:
         return obj
-    cmd = [_nvcc(), *_flags(), "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
+    cmd = [_nvcc(), *_flags(src), "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -99,7 +105,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     LIB_DIR.mkdir(exist_ok=True)
     # objects built with other flags (release vs debug checks) are stale whatever their time stamps say
     stamp = OBJ_DIR / "flags.txt"
-    flags_text = " ".join(_flags())
+    flags_text = " ".join([*_flags(), "exact:", *EXACT_SOURCES])
     if not stamp.exists() or stamp.read_text() != flags_text:
         force = True
     stamp.write_text(flags_text)

@@ -1,0 +1,560 @@
+// Log probabilities of given tokens under the output head, and their gradients, without the logits in memory:
+//   x_tv = h_t . w_v / tau,   y_t = x_t,label - log sum_v exp(x_tv);
+//   dx_tv = dy_t ([v = label] - exp(x_tv - lse_t)) / tau,   dh = dx w,   dw = dx^T h.
+//
+// Bound: the products, 2 n V D operations forward and three times that backward (the logits are computed again, from which dx
+// comes in the accumulators' precision; kept in bf16 they would save one product of four and cost their rounding, 2^-9 of a logit).  At 16 rows
+// and fewer the weights' bytes.
+//
+// Rows without a label are left out first: the others are gathered into a dense array, and the kernels take their number from device
+// memory, so that prompts and masked turns cost nothing but their labels, and what their rows hold reaches no sum.
+//
+// One kernel on CTA pairs (gemm2.cu describes its roles and barriers) serves four products, which differ in their epilogue:
+//   kStats  h w^T: every thread has one row of the tile; it takes the maximum and the sum of exponentials of 128 columns, and writes their
+//           log-sum (base 2) as one number.  A second kernel adds those of a row.
+//   kGrad   the same product again: dx in bf16.
+//   kDh     dx w, fp32, over the columns of one slab;  kDw  dx^T h.
+// dx exists for a slab of the vocabulary at a time (the caller says how wide): the slabs' dw are disjoint, and dh is added up in fp32.
+#include "common.cuh"
+#include "host.h"
+#include "pair.cuh"
+#include "vec.cuh"
+
+#include <math.h>
+
+namespace ksa {
+
+constexpr int kLpBM = 128;          // rows of the tile in a CTA; a pair has 256
+constexpr int kLpBN = 256;          // columns of the tile
+constexpr int kLpBNh = 128;         // rows of B staged per CTA
+constexpr int kLpBK = 64;
+constexpr int kLpThreads = 192;     // warp 0 loads, warp 1 issues products, warps 2..5 epilogue
+constexpr int kLpStages = 6;
+constexpr int kLpGroupM = 8;
+constexpr int kLpABytes = kLpBM * kLpBK * 2;
+constexpr int kLpBBytes = kLpBNh * kLpBK * 2;
+constexpr int kLpStageBytes = kLpABytes + kLpBBytes;
+constexpr int kLpStoreBytes = 4 * 2 * 4096;                              // two staging boxes of 128 bytes x 32 rows for each epilogue warp
+constexpr int kLpSmem = kLpStages * kLpStageBytes + kLpStoreBytes + 256 + 1024;
+static_assert(kLpSmem <= 232448, "227 KB");
+static_assert(kLpSmem >= kTmemClusterAlone, "a pair holds all tensor memory: no block of another cluster beside it (host.h)");
+constexpr int kLpStatCols = 128;                                        // columns that share a log-sum
+constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
+
+enum LpMode : int { kStats = 0, kGrad = 1, kDh = 2, kDw = 3 };
+
+struct LpArgs {
+  int M, N, K;                 // at most; *count stands for M, or for K in kDw
+  const int* count;            // rows with a label
+  const int* rows;             // their places among all rows
+  const int* row_label;        // their labels
+  float scale2;                // log2(e) / tau
+  float inv_tau;
+  float* stats;                // kStats: [ceil(N / 128)][ld_stats] log-sums, base 2
+  float* picked;               // kStats: [rows] x of the label times log2(e)
+  long long ld_stats;
+  const float* lse2;           // kGrad: [rows]
+  const float* dy;             // kGrad: gradient of y, by the rows' places
+  int col0;                    // kGrad: first column of the slab
+  int add;                     // kDh, kDw: into fp32, added to what is there
+  int bf16_out;                // kDw
+  int* status;
+};
+
+template <int kMode>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
+log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                      const __grid_constant__ LpArgs a) {
+  constexpr bool kAMn = kMode == kDw, kBMn = kMode == kDh || kMode == kDw;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + kLpStages * kLpStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + kLpStoreBytes);   // used in the leader
+  uint64_t* empty = full + kLpStages;                                   // both CTAs
+  uint64_t* acc_full = empty + kLpStages;                               // both CTAs, 2 buffers
+  uint64_t* acc_empty = acc_full + 2;                                   // used in the leader, 2 buffers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();     // 0 = leader
+  const WaitGuard guard{abort_flag, a.status};
+  const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kLpStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 2) { tmem_alloc2(tmem_slot, 512); tmem_relinquish2(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();          // both CTAs' barriers are initialised before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_enter();
+
+  const int count = *a.count;
+  const int M = kMode == kDw ? a.M : min(count, a.M), N = a.N, K = kMode == kDw ? min(count, a.K) : a.K;
+  const int tiles_m = (M + 2 * kLpBM - 1) / (2 * kLpBM), tiles_n = (N + kLpBN - 1) / kLpBN;
+  const int num_tiles = tiles_m * tiles_n;
+  const int num_kb = (K + kLpBK - 1) / kLpBK;
+  // A last wave of at most half as many tiles as pairs is worked on as halves of 128 columns (gemm2.cu)
+  const int last = num_tiles % n_pairs;
+  const int halves_from = 2 * last <= n_pairs ? num_tiles - last : num_tiles;
+  const int units = 2 * num_tiles - halves_from;
+
+  auto tile_coords = [&](int tile, int& mb, int& nb) {
+    const int per_group = kLpGroupM * tiles_n;
+    const int group = tile / per_group;
+    const int first_m = group * kLpGroupM;
+    const int group_rows = min(tiles_m - first_m, kLpGroupM);
+    const int in_group = tile - group * per_group;
+    mb = first_m + in_group % group_rows;
+    nb = in_group / group_rows;
+  };
+  // A unit is a tile, or one half of its columns: `side` is that half, -1 for the whole
+  auto unit_tile = [&](int unit, int& side) {
+    side = -1;
+    if (unit < halves_from) return unit;
+    side = (unit - halves_from) & 1;
+    return halves_from + ((unit - halves_from) >> 1);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int unit = pair; unit < units && ok; unit += n_pairs) {
+        int mb, nb, side;
+        tile_coords(unit_tile(unit, side), mb, nb);
+        const int row0 = mb * 2 * kLpBM + (int)rank * kLpBM;
+        const int col0 = side < 0 ? nb * kLpBN + (int)rank * kLpBNh : nb * kLpBN + side * kLpBNh + (int)rank * 64;
+        const int boxes = side >= 0 ? 1 : 2;                             // of 64 rows
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty)) { ok = false; break; }
+          uint8_t* sa = smem + stage * kLpStageBytes;
+          uint8_t* sb = sa + kLpABytes;
+          const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kLpABytes + boxes * 8192));
+          if (!kAMn) {
+            tma_load_2d_pair(sa, &tmA, kb * kLpBK, row0, bar);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kLpBM / 64; ++i) tma_load_2d_pair(sa + i * 8192, &tmA, row0 + i * 64, kb * kLpBK, bar);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i >= boxes) break;
+            if (!kBMn) tma_load_2d_pair(sb + i * 8192, &tmB, kb * kLpBK, col0 + i * 64, bar);
+            else tma_load_2d_pair(sb + i * 8192, &tmB, col0 + i * 64, kb * kLpBK, bar);
+          }
+          if (++stage == kLpStages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc_full = umma_idesc_bf16(2 * kLpBM, kLpBN, kAMn ? 1 : 0, kBMn ? 1 : 0);
+      constexpr uint32_t idesc_half = umma_idesc_bf16(2 * kLpBM, kLpBNh, kAMn ? 1 : 0, kBMn ? 1 : 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int unit = pair; unit < units && ok; unit += n_pairs, ++local) {
+        const uint32_t idesc = unit < halves_from ? idesc_full : idesc_half;
+        const int buf = local & 1;
+        const uint32_t acc_phase = (local >> 1) & 1;
+        if (!mbar_wait(&acc_empty[buf], acc_phase ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * kLpBN;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kLpStageBytes);
+          const uint32_t sb = sa + kLpABytes;
+#pragma unroll
+          for (int k = 0; k < kLpBK / 16; ++k) {
+            const uint64_t da = kAMn ? smem_desc_mnmajor_sw128(sa + k * 2048, 8192) : smem_desc_kmajor_sw128(sa + k * 32);
+            const uint64_t db = kBMn ? smem_desc_mnmajor_sw128(sb + k * 2048, 8192) : smem_desc_kmajor_sw128(sb + k * 32);
+            umma2_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+          }
+          umma2_commit_both(&empty[stage]);
+          if (++stage == kLpStages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma2_commit_both(&acc_full[buf]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
+    const int quad = warp & 3;
+    int local = 0;
+    bool ok = true;
+    int out_buf = 0;           // staging box of this warp's next store
+    // one box of 128 bytes x 32 rows: `v` is this lane's row of it
+    auto store_box = [&](const uint32_t (&v)[32], int col, int row, bool add) {
+      uint8_t* box = ring + ((warp - 2) * 2 + out_buf) * 4096;
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the store before the last one has read its box
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        if (add) tma_reduce_add_2d(&tmC, box, col, row);
+        else tma_store_2d(&tmC, box, col, row);
+        tma_store_commit();
+      }
+      out_buf ^= 1;
+    };
+    for (int unit = pair; unit < units && ok; unit += n_pairs, ++local) {
+      int mb, nb, side;
+      tile_coords(unit_tile(unit, side), mb, nb);
+      const int col_base = nb * kLpBN + (side > 0 ? kLpBNh : 0), parts = side < 0 ? 2 : 1;      // of 128 columns
+      const int buf = local & 1;
+      const uint32_t acc_phase = (local >> 1) & 1;
+      const int row_w = mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
+      const int row = row_w + lane;
+      const bool live = kMode == kDw || row < M;
+      int label = -1;
+      float lse2 = 0.f, g = 0.f;
+      if ((kMode == kStats || kMode == kGrad) && live) label = a.row_label[row];
+      if (kMode == kGrad && live) {
+        lse2 = a.lse2[row];
+        g = a.dy[a.rows[row]] * a.inv_tau;
+        label -= a.col0;
+      }
+      if (!mbar_wait(&acc_full[buf], acc_phase, guard, kTimeoutAccFull)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * kLpBN;
+#pragma unroll 1
+      for (int part = 0; part < parts; ++part) {
+        const int col = col_base + part * kLpStatCols;
+        if (col >= N) break;
+        if (kMode == kStats) {
+          uint32_t r[kLpStatCols];
+#pragma unroll
+          for (int i = 0; i < kLpStatCols / 32; ++i) tmem_ld32(t_row + part * kLpStatCols + i * 32, *reinterpret_cast<uint32_t(*)[32]>(r + i * 32));
+          tmem_wait_ld();
+          if (col + kLpStatCols > N)
+#pragma unroll
+            for (int j = 0; j < kLpStatCols; ++j)
+              if (col + j >= N) r[j] = 0xff800000u;                      // minus infinity
+          const int at = label - col;
+          if (__any_sync(0xffffffffu, at >= 0 && at < kLpStatCols)) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < kLpStatCols; ++j) x = j == at ? __uint_as_float(r[j]) : x;
+            if (at >= 0 && at < kLpStatCols) a.picked[row] = x * a.scale2;
+          }
+          float m[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) m[j] = fmaxf(__uint_as_float(r[j]), __uint_as_float(r[4 + j]));
+#pragma unroll
+          for (int j = 8; j < kLpStatCols; j += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = max3(m[i], __uint_as_float(r[j + 2 * i]), __uint_as_float(r[j + 2 * i + 1]));
+          const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+          const float top = mx == -INFINITY ? 0.f : mx * a.scale2;       // (scale2 > 0)
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < kLpStatCols; ++j) s[j & 3] += fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -top));
+          if (live) a.stats[(long long)(col / kLpStatCols) * a.ld_stats + row] = top + __log2f((s[0] + s[1]) + (s[2] + s[3]));
+        } else if (kMode == kGrad) {
+#pragma unroll 1
+          for (int piece = 0; piece < 2; ++piece) {
+            const int c = col + piece * 64;
+            if (c >= N) break;
+            uint32_t out[32];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t r[32];
+              tmem_ld32(t_row + part * kLpStatCols + piece * 64 + half * 32, r);
+              tmem_wait_ld();
+              const int at = label - c - half * 32;
+              float d[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) d[j] = -g * fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -lse2));
+              if (__any_sync(0xffffffffu, at >= 0 && at < 32))
+#pragma unroll
+                for (int j = 0; j < 32; ++j) d[j] = j == at ? d[j] + g : d[j];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
+            }
+            store_box(out, c, row_w, false);
+          }
+        } else {
+          const bool bf = kMode == kDw && a.bf16_out;
+#pragma unroll 1
+          for (int piece = 0; piece < (bf ? 2 : 4); ++piece) {
+            const int c = col + piece * (bf ? 64 : 32);
+            if (c >= N) break;
+            uint32_t out[32];
+            if (bf) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                uint32_t r[32];
+                tmem_ld32(t_row + part * kLpStatCols + piece * 64 + half * 32, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) out[half * 16 + j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+              }
+            } else {
+              tmem_ld32(t_row + part * kLpStatCols + piece * 32, out);
+              tmem_wait_ld();
+            }
+            if (num_kb == 0)                                             // no rows at all: nothing was multiplied
+#pragma unroll
+              for (int j = 0; j < 32; ++j) out[j] = 0u;
+            if (row_w < a.M) store_box(out, c, row_w, a.add != 0);
+          }
+        }
+      }
+      // one arrival per epilogue warp of either CTA on the leader's barrier: this accumulator buffer may be rewritten
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+    }
+    if (kMode != kStats && lane == 0) tma_store_wait0();                 // its stores have written their destination
+  }
+  // The peer's tensor memory and barriers are written by the leader's products and commits: nobody leaves, and nothing is deallocated,
+  // before both CTAs are done.
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, 512);
+  }
+}
+
+// Which rows have a label, in order: rows[i], row_label[i] and count; place[t] of every row (-1: none), and y[t] = 0 for those.
+constexpr int kLpSelect = 1024;
+__global__ void __launch_bounds__(kLpSelect)
+log_probs_select_kernel(const long long* labels, int T, int V, long long ignore, int* rows, int* row_label, int* place, int* count, float* y) {
+  __shared__ int sums[kLpSelect / 32];
+  grid_dependency_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int before = 0;
+  for (int t0 = 0; t0 < T; t0 += kLpSelect) {
+    const int t = t0 + threadIdx.x;
+    const long long label = t < T ? labels[t] : -1;
+    const bool has = t < T && label != ignore && label >= 0 && label < V;
+    const unsigned votes = __ballot_sync(0xffffffffu, has);
+    if (lane == 0) sums[warp] = __popc(votes);
+    __syncthreads();
+    int mine = sums[lane], up = mine;                                    // 32 warps: an inclusive sum over them in every warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += v;
+    }
+    const int at = before + __shfl_sync(0xffffffffu, up - mine, warp) + __popc(votes & ((1u << lane) - 1));
+    if (t < T) {
+      place[t] = has ? at : -1;
+      if (has) { rows[at] = t; row_label[at] = (int)label; }
+      else y[t] = 0.f;
+    }
+    before += __shfl_sync(0xffffffffu, up, 31);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = before;
+}
+
+// dense[i] = h[rows[i]], and zeros up to the next multiple of kLpRowPad.  A warp has a row.
+__global__ void __launch_bounds__(256)
+log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int* count, bf16* dense, int D, int padded, int vec) {
+  grid_dependency_enter();
+  const int n = *count, lane = threadIdx.x & 31, end = min((n + kLpRowPad - 1) / kLpRowPad * kLpRowPad, padded);
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += gridDim.x * 8) {
+    bf16* to = dense + (long long)i * D;
+    const bf16* from = i < n ? h + (long long)rows[i] * ldh : nullptr;
+    if (from == nullptr) {
+      for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
+    } else if (vec) {
+      for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
+    } else {
+      for (int c = lane; c < D; c += 32) to[c] = from[c];
+    }
+  }
+}
+
+// y and lse2 of a row from the log-sums of its columns: 8 rows to a block, 128 threads for each.
+constexpr int kLpSumRows = 8;
+__global__ void __launch_bounds__(1024)
+log_probs_sum_kernel(const float* stats, long long ld, int slots, const float* picked, const int* rows, const int* count, float* y, float* lse2) {
+  __shared__ float2 part[32][kLpSumRows];
+  grid_dependency_enter();
+  const int n = *count, r = threadIdx.x % kLpSumRows, s0 = threadIdx.x / kLpSumRows, row = blockIdx.x * kLpSumRows + r;
+  if ((int)blockIdx.x * kLpSumRows >= n) return;
+  float m = -INFINITY, s = 0.f;                                          // of 2^x
+  if (row < n) {
+#pragma unroll 4
+    for (int i = s0; i < slots; i += 1024 / kLpSumRows) {
+      const float x = stats[(long long)i * ld + row];
+      const float top = fmaxf(m, x);
+      if (top > -INFINITY || x != x) {
+        s = s * exp2f(m == -INFINITY ? -INFINITY : m - top) + exp2f(x - top);
+        m = top;
+      }
+    }
+  }
+  auto add = [](float& m, float& s, float m2, float s2) {
+    const float top = fmaxf(m, m2);
+    const float a = m == -INFINITY ? s : s * exp2f(m - top), b = m2 == -INFINITY ? s2 : s2 * exp2f(m2 - top);      // (0, or what is no number)
+    s = a + b;
+    m = top;
+  };
+#pragma unroll
+  for (int o = 16; o >= kLpSumRows; o >>= 1) add(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  if ((threadIdx.x & 31) < kLpSumRows) part[threadIdx.x >> 5][r] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < kLpSumRows && row < n) {
+    m = part[0][r].x;
+    s = part[0][r].y;
+    for (int w = 1; w < 32; ++w) add(m, s, part[w][r].x, part[w][r].y);
+    const float l = m + log2f(s);
+    lse2[row] = l;
+    y[rows[row]] = (picked[row] - l) * 0.69314718056f;
+  }
+}
+
+// dh[t] = the gathered gradient of row t in bf16, 0 without a label.  A warp has a row.
+__global__ void __launch_bounds__(256) log_probs_scatter_kernel(const float* dense, const int* place, bf16* dh, int T, int D) {
+  grid_dependency_enter();
+  const int lane = threadIdx.x & 31;
+  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += gridDim.x * 8) {
+    const int i = place[t];
+    for (int c = lane * 8; c < D; c += 256) {
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (i >= 0) {
+        const float4 u = *reinterpret_cast<const float4*>(dense + (long long)i * D + c), v = *reinterpret_cast<const float4*>(dense + (long long)i * D + c + 4);
+        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+      }
+      store8(dh + (long long)t * D + c, f);
+    }
+  }
+}
+
+static int lp_map(CUtensorMap* m, const void* base, int elem, long long cols, long long rows, long long pitch, int box_rows) {
+  const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, str[2] = {(uint64_t)elem, (uint64_t)pitch * elem};
+  const uint32_t box[2] = {(uint32_t)(128 / elem), (uint32_t)box_rows};
+  return make_tmap(m, base, elem, 2, dims, str, box, true);
+}
+
+template <int kMode>
+static int launch_log_probs(const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, LpArgs a, cudaStream_t st) {
+  const int sms = sm_count();
+  KSA_REQUIRE(sms > 1, "no device");
+  a.status = status_word();
+  KSA_REQUIRE(a.status != nullptr, "could not allocate the status word");
+  auto kern = log_probs_pair_kernel<kMode>;
+  static PerDevice raised;
+  KSA_CHECK_CUDA(raise_smem_limit(raised, kern, kLpSmem));
+  const long long tiles = (long long)((a.M + 2 * kLpBM - 1) / (2 * kLpBM)) * ((a.N + kLpBN - 1) / kLpBN);
+  KSA_REQUIRE(tiles < (1 << 30), "log_probs: %lld tiles", tiles);
+  const int pairs = (int)(2 * tiles < sms / 2 ? 2 * tiles : sms / 2);     // (fewer rows than all may leave the last ones idle)
+  KSA_CHECK_CUDA(launch_kernel(kern, dim3(2 * pairs), dim3(kLpThreads), (size_t)kLpSmem, st, A, B, C, a));
+  return 0;
+}
+
+}  // namespace ksa
+
+using namespace ksa;
+#define ST(s) reinterpret_cast<cudaStream_t>(s)
+
+// Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
+// Leaves what the backward pass needs: dense [T rounded up to 256, D] bf16, rows, row_label, place [T], count [1] int32, lse2 [T].
+// work: fp32 [T rounded up to 4 times (ceil(V / 128) + 1)].  y [T] fp32.
+KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
+                          void* lse2, void* work, void* y, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
+                          void* stream) {
+  KSA_ENTER(w);
+  KSA_REQUIRE(T > 0 && V > 0 && D > 0, "log_probs: empty problem %d x %d x %d", T, V, D);
+  KSA_REQUIRE(D % 8 == 0 && ldw % 8 == 0 && ldw >= D, "log_probs: D=%d and the weights' pitch %lld must be multiples of 8", D, ldw);
+  KSA_REQUIRE(tau > 0.f && isfinite(tau), "log_probs: the temperature must be a positive number");
+  KSA_REQUIRE(T <= 0x7fffffff - kLpRowPad, "log_probs: %d rows", T);
+  cudaStream_t st = ST(stream);
+  const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad, slots = (V + kLpStatCols - 1) / kLpStatCols;
+  const long long ld = (T + 3LL) / 4 * 4;
+  float* stats = static_cast<float*>(work);
+  float* picked = stats + ld * slots;
+  KSA_CHECK_CUDA(launch_kernel(log_probs_select_kernel, dim3(1), dim3(kLpSelect), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
+                               (int*)row_label, (int*)place, (int*)count, (float*)y));
+  const int vec = ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
+  const int gather_blocks = padded / 8 < 148 * 8 ? padded / 8 : 148 * 8;
+  KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh, (const int*)rows,
+                                      (const int*)count, (bf16*)dense, D, padded, vec));
+  CUtensorMap A, B;
+  int rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
+  if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
+  if (rc) return rc;
+  LpArgs a{};
+  a.M = T; a.N = V; a.K = D;
+  a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
+  a.scale2 = (float)(1.4426950408889634 / (double)tau);
+  a.stats = stats; a.picked = picked; a.ld_stats = ld;
+  rc = launch_log_probs<kStats>(A, B, A, a, st);
+  if (rc) return rc;
+  KSA_CHECK_CUDA(launch_kernel(log_probs_sum_kernel, dim3((T + kLpSumRows - 1) / kLpSumRows), dim3(1024), 0, st, (const float*)stats, ld, slots,
+                               (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2));
+  return 0;
+}
+
+// Backward.  dy [T] fp32; dh [T, D] bf16 or null; dw [V, D] (row pitch lddw) or null, bf16 or (dw_fp32) fp32, there with add_dw added to.
+// dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8); dh32: fp32 [T rounded up to 256, D] where dh is wanted.
+KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
+                              const void* lse2, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
+                              long long lddw, int dw_fp32, int add_dw, int slab, float tau, void* stream) {
+  KSA_ENTER(w);
+  KSA_REQUIRE(T > 0 && V > 0 && D > 0 && D % 8 == 0 && ldw % 8 == 0, "log_probs: backward of %d x %d x %d", T, V, D);
+  KSA_REQUIRE(!dw || lddw % (dw_fp32 ? 4 : 8) == 0, "log_probs: the pitch %lld of the weights' gradient keeps no alignment of 16 bytes", lddw);
+  KSA_REQUIRE(slab > 0 && slab % 8 == 0, "log_probs: %d columns at a time (a multiple of 8)", slab);
+  KSA_REQUIRE(!(add_dw && !dw_fp32), "log_probs: only an fp32 gradient is added to");
+  KSA_REQUIRE(!dh || (reinterpret_cast<uintptr_t>(dh) & 15) == 0, "log_probs: the gradient of the rows must be 16-byte aligned");
+  cudaStream_t st = ST(stream);
+  const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad;
+  CUtensorMap denseK, denseM;
+  int rc = lp_map(&denseK, dense, 2, D, padded, D, kLpBM);
+  if (rc == 0) rc = lp_map(&denseM, dense, 2, D, padded, D, 64);
+  for (long long v0 = 0; v0 < V && rc == 0; v0 += slab) {
+    const int n = V - v0 < slab ? (int)(V - v0) : slab;
+    const bf16* wv = static_cast<const bf16*>(w) + v0 * ldw;
+    CUtensorMap wK, wM, dxOut, dxK, dxM, out;
+    LpArgs a{};
+    a.count = static_cast<const int*>(count); a.rows = static_cast<const int*>(rows); a.row_label = static_cast<const int*>(row_label);
+    a.scale2 = (float)(1.4426950408889634 / (double)tau); a.inv_tau = 1.f / tau;
+    a.lse2 = static_cast<const float*>(lse2); a.dy = static_cast<const float*>(dy); a.col0 = (int)v0;
+    a.M = T; a.N = n; a.K = D;
+    rc = lp_map(&wK, wv, 2, D, n, ldw, 64);
+    if (rc == 0) rc = lp_map(&dxOut, dx, 2, n, padded, slab, 32);
+    if (rc == 0) rc = launch_log_probs<kGrad>(denseK, wK, dxOut, a, st);
+    if (rc == 0 && dh) {
+      a.M = T; a.N = D; a.K = n; a.add = v0 > 0;
+      rc = lp_map(&dxK, dx, 2, n, padded, slab, kLpBM);
+      if (rc == 0) rc = lp_map(&wM, wv, 2, D, n, ldw, 64);
+      if (rc == 0) rc = lp_map(&out, dh32, 4, D, padded, D, 32);
+      if (rc == 0) rc = launch_log_probs<kDh>(dxK, wM, out, a, st);
+    }
+    if (rc == 0 && dw) {
+      a.M = n; a.N = D; a.K = T; a.add = add_dw; a.bf16_out = !dw_fp32;
+      rc = lp_map(&dxM, dx, 2, n, padded, slab, 64);
+      if (rc == 0) rc = dw_fp32 ? lp_map(&out, static_cast<float*>(dw) + v0 * lddw, 4, D, n, lddw, 32) : lp_map(&out, static_cast<bf16*>(dw) + v0 * lddw, 2, D, n, lddw, 32);
+      if (rc == 0) rc = launch_log_probs<kDw>(dxM, denseM, out, a, st);
+    }
+  }
+  if (rc) return rc;
+  if (dh) {
+    const int blocks = (T + 7) / 8 < 148 * 8 ? (T + 7) / 8 : 148 * 8;
+    KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, log_probs_scatter_kernel, dim3(blocks), dim3(256), 0, st, (const float*)dh32, (const int*)place,
+                                        (bf16*)dh, T, D));
+  }
+  return 0;
+}

@@ -1210,10 +1210,14 @@ def adamw_step(master, grad, m, v, out_bf16, hyper, beta1, beta2, eps, weight_de
 
 from .int4 import (Int4Cache, Int4Weight, int4_cache, int4_cache_move, int4_cache_read, int4_cache_write, int4_decode_attention,  # noqa: E402
                    int4_dequantize_weight, int4_linear, int4_linear_swiglu, int4_norm_linear, int4_qk_norm_rope_decode, int4_quantize_weight)
+from .clipping import clip_grad_norm_, grad_norm  # noqa: E402
+from .log_probs import linear_log_probs  # noqa: E402
+from .token_losses import policy_loss, preference_loss  # noqa: E402
 
 __all__ = [
     "gemm", "linear", "dual_linear", "attention_packed", "rms_norm", "add_rms_norm", "qk_norm_rope_packed", "qk_norm_rope_decode", "swiglu", "linear_swiglu", "norm_linear", "embedding",
     "ksa_attention", "causal_attention", "linear_cross_entropy", "adamw_step", "UNBOUNDED_WINDOW",
+    "linear_log_probs", "policy_loss", "preference_loss", "grad_norm", "clip_grad_norm_",
     "SummaryLayout", "get_layout",
     "Int4Cache", "Int4Weight", "int4_cache", "int4_cache_move", "int4_cache_read", "int4_cache_write", "int4_decode_attention", "int4_dequantize_weight",
     "int4_linear", "int4_linear_swiglu", "int4_norm_linear", "int4_qk_norm_rope_decode", "int4_quantize_weight",

@@ -73,6 +73,13 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_int4_weight_values": [P, P, P, I, I, I, I, P],
     "ksa_int4_norm_linear": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P],
     "ksa_int4_linear": [P, P, P, P, I, I, I, I, I, L, L, I, P],
+    "ksa_log_probs": [P] * 11 + [I] * 3 + [L] * 3 + [F, P],
+    "ksa_log_probs_bwd": [P] * 12 + [I] * 3 + [L] * 2 + [I] * 3 + [F, P],
+    "ksa_policy_loss": [P, P, P, P, P, P, I, P, P, P, P, P, I, L, I, L, I, I, P, F, P],
+    "ksa_policy_loss_bwd": [P, P, P, P, I, P, I, L, I, L, I, P],
+    "ksa_preference_loss": [P, P, P, P, I, P, P, P, P, I, L, I, L, F, F, P],
+    "ksa_preference_loss_bwd": [P, P, P, P, I, P, I, L, I, L, P],
+    "ksa_grad_norm": [P, P, P, I, F, F, P, P, P],
     "ksa_peer_gather": [P, I, I, L, I, P, P, ctypes.c_uint, I, P],
     "ksa_peer_reduce_adamw": [P, I, I, L, L, P, P, P, P, P, F, F, F, F, F, P, P, P, ctypes.c_uint, I, P],
     "ksa_signal_set": [P, I, P, ctypes.c_uint, P],
@@ -124,6 +131,10 @@ def load() -> ctypes.CDLL:
     lib.ksa_int4_attn_workspace.restype = L
     lib.ksa_int4_cache_write_table.argtypes = [I] * 5
     lib.ksa_int4_cache_write_table.restype = L
+    lib.ksa_grad_norm_parts.argtypes = [I]
+    lib.ksa_grad_norm_parts.restype = I
+    lib.ksa_token_loss_units.argtypes = [L, I]
+    lib.ksa_token_loss_units.restype = L
     lib.ksa_set_dependent_launch.argtypes = [I]
     lib.ksa_set_dependent_launch.restype = I
     for name, sig in _SIGNATURES.items():
@@ -197,7 +208,9 @@ def _address(x: torch.Tensor) -> int:
 
 
 # kernels launched by one call of an entry point (default 1)
-_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2}
+_KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2,
+                     "ksa_grad_norm": 2, "ksa_policy_loss": 2, "ksa_preference_loss": 2, "ksa_log_probs": 4,
+                     "ksa_log_probs_bwd": 4}
 _launch_count = 0
 
 
@@ -337,3 +350,12 @@ def attn_bwd_num_segments(lq: int) -> int:
 
 def rmsnorm_bwd_parts(rows: int) -> int:
     return load().ksa_rmsnorm_bwd_parts(rows)
+
+
+def grad_norm_parts(tensors: int) -> int:
+    return load().ksa_grad_norm_parts(tensors)
+
+
+def token_loss_units(tokens: int, sequences: int) -> int:
+    return load().ksa_token_loss_units(tokens, sequences)
+

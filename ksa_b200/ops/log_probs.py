@@ -1,0 +1,119 @@
+"""Log probabilities of given tokens under the output head, forward and backward, without logits in memory (``csrc/log_probs.cu``)."""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import reference as ref
+from .token_losses import _Forward, _observed
+
+_ROW_PAD = 256              # rows of the gathered arrays: a multiple of this (kLpRowPad in csrc/log_probs.cu)
+_STAT_COLS = 128            # columns that share a log-sum (kLpStatCols)
+SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16) of so many bytes at a time, or of 256 columns
+
+
+def _slab(padded: int, V: int) -> int:
+    """Columns of the vocabulary that the backward pass takes at a time."""
+    return min(-(-V // 8) * 8, max(256, SLAB_BYTES // (2 * padded) // 256 * 256))
+
+
+class _LinearLogProbsFn(torch.autograd.Function):
+    """``h`` ``[T, D]`` with contiguous rows, ``w`` ``[V, D]``, ``labels`` ``[T]``."""
+
+    @staticmethod
+    def forward(ctx, h, w, labels, ignore_index, temperature):
+        (T, D), V, dev = h.shape, w.shape[0], h.device
+        with torch.cuda.device(dev):
+            y = torch.empty(T, dtype=torch.float32, device=dev)
+            padded = -(-T // _ROW_PAD) * _ROW_PAD
+            dense = torch.empty((padded, D), dtype=h.dtype, device=dev)
+            rows, row_label, place = torch.empty((3, T), dtype=torch.int32, device=dev).unbind()
+            count = torch.empty(1, dtype=torch.int32, device=dev)
+            lse2 = torch.empty(T, dtype=torch.float32, device=dev)
+            work = torch.empty(-(-T // 4) * 4 * (-(-V // _STAT_COLS) + 1), dtype=torch.float32, device=dev)
+            weight = _pitched(w)
+            _lib.call("ksa_log_probs", h, weight, labels, dense, rows, row_label, place, count, lse2, work, y, T, V, D, h.stride(0),
+                      weight.stride(0), ignore_index, float(temperature))
+        ctx.save_for_backward(dense, w, rows, row_label, place, count, lse2)
+        ctx.temperature = temperature
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        dense, w, rows, row_label, place, count, lse2 = ctx.saved_tensors
+        T, (V, D), dev = rows.shape[0], w.shape, w.device
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dh = dw = dh32 = None
+        with torch.cuda.device(dev):
+            dy = dy.to(torch.float32).contiguous()
+            weight = _pitched(w)
+            dx = torch.empty((dense.shape[0], _slab(dense.shape[0], V)), dtype=w.dtype, device=dev)
+            if need_h:
+                dh = torch.empty((T, D), dtype=w.dtype, device=dev)
+                dh32 = torch.empty(dense.shape, dtype=torch.float32, device=dev)
+
+            def run(out, add):
+                _lib.call("ksa_log_probs_bwd", dense, weight, rows, row_label, place, count, lse2, dy, dx, dh32, dh, out, T, V, D,
+                          weight.stride(0), out.stride(0) if out is not None else D, int(out is not None and out.dtype == torch.float32),
+                          int(add), dx.shape[1], float(ctx.temperature))
+
+            if not need_w:
+                run(None, False)
+            else:
+                from . import _weight_grad
+
+                def compute(out, add):
+                    if out is None:
+                        out = torch.empty((V, D), dtype=w.dtype, device=dev)
+                    run(out, add)
+                    return out
+                dw = _weight_grad(w, compute)
+        return dh, dw, None, None, None
+
+
+def _pitched(w: torch.Tensor) -> torch.Tensor:
+    """``w`` with contiguous rows that begin on 16 bytes."""
+    fits = w.stride(1) == 1 and w.stride(0) % 8 == 0 and w.stride(0) >= w.shape[1] and w.data_ptr() % 16 == 0
+    return w if fits else w.clone(memory_format=torch.contiguous_format)
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                     temperature: float = 1.0) -> torch.Tensor:
+    """``log_softmax(hidden @ weight.T / temperature)`` at ``labels``: fp32 of the labels' shape, 0 where the label is ``ignore_index`` or no
+    row of ``weight``.
+
+    ``hidden`` is ``[..., D]``, ``weight`` the output head ``[V, D]`` (both bf16 on a GPU, ``D`` a multiple of 8), ``labels`` ``[...]``.  Rows
+    without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  The logits are never in
+    memory: the forward pass keeps what its tiles' sums need, the backward pass computes them again, at most 4 GB of their gradient at a time.
+    With ``main_grad`` on the weight its gradient goes there."""
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"rows {tuple(hidden.shape)} and an output head {tuple(weight.shape)}")
+    if labels.shape != hidden.shape[:-1] or labels.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"labels are whole numbers of shape {tuple(hidden.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
+    if not (math.isfinite(temperature) and temperature > 0):
+        raise ValueError(f"the temperature must be a positive number, got {temperature}")
+    if weight.shape[0] < 1:
+        raise ValueError("an output head without rows")
+    if not hidden.device == weight.device == labels.device:
+        raise ValueError(f"tensors on {hidden.device}, {weight.device} and {labels.device}")
+    if not hidden.is_cuda:
+        return ref.linear_log_probs(hidden, weight, labels, ignore_index, temperature)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"the sm_100a kernels take bf16 activations/weights, got {hidden.dtype}, {weight.dtype}")
+    if weight.shape[1] % 8 != 0 or weight.shape[1] == 0:
+        raise ValueError(f"the width {weight.shape[1]} must be a multiple of 8")
+    if labels.numel() == 0:
+        return (hidden.sum(-1) * 0).float().reshape(labels.shape) + 0 * weight[:0].sum().float()
+    h2 = hidden.reshape(-1, hidden.shape[-1])
+    if h2.stride(1) != 1:
+        h2 = h2.contiguous()
+    flat = labels.reshape(-1).to(torch.int64).contiguous()
+    if _observed() or (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)):
+        y = _LinearLogProbsFn.apply(h2, weight, flat, ignore_index, temperature)
+    else:
+        y = _LinearLogProbsFn.forward(_Forward(), h2, weight, flat, ignore_index, temperature)
+    return y.view(labels.shape)

@@ -329,3 +329,76 @@ def adamw_step_(master: torch.Tensor, grad: torch.Tensor, m: torch.Tensor, v: to
     if out_bf16 is not None:
         out_bf16.copy_(master)
     return sq
+
+
+# ---------------------------------------------------------------- post-training
+def grad_norm(grads, scale: float = 1.0, max_norm: float = math.inf):
+    """``scale`` times the global 2-norm of the tensors, and the factor that clips it to ``max_norm``, both fp32 scalars."""
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(()), torch.full((), float(scale) * min(1.0, max_norm / 1e-6))
+    total = torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt() * scale
+    norm = total.float()
+    return norm, scale * (max_norm / (norm + 1e-6)).clamp(max=1.0)
+
+
+def sequence_of(n: int, sequences: int, cu_seqlens: Optional[torch.Tensor], device) -> torch.Tensor:
+    """The sequence of every token ``[n]``; ``sequences`` for those behind the last one."""
+    at = torch.arange(n, device=device)
+    if cu_seqlens is None:
+        return at // max(n // max(sequences, 1), 1)
+    return torch.bucketize(at, cu_seqlens.to(torch.int64)[1:], right=True)
+
+
+def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, of, sequences: int, clip_low: float, clip_high: float, kl_coef: float,
+                by_sequence: bool):
+    """Flat arguments: a value for every token (``advantages``: or sequence), ``of`` its sequence.  Returns the loss and the means of
+    its clipped part, of the KL term and of being cut off."""
+    valid = of < sequences
+    if mask is not None:
+        valid = valid & (mask != 0)
+    y = torch.where(valid, log_probs, log_probs.new_zeros(())).double()
+    pick = lambda t: torch.where(valid, t, t.new_zeros(())).double()  # noqa: E731
+    a = pick(advantages if advantages.shape == of.shape else torch.cat([advantages, advantages.new_zeros(1)])[of])
+    d = y - pick(old_log_probs)
+    cut = ((a > 0) & (d > math.log1p(clip_high))) | ((a < 0) & (d < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)))
+    bound = torch.where(a > 0, torch.full_like(a, 1 + clip_high), torch.full_like(a, 1 - clip_low))
+    # (a token that is cut off takes part with a ratio of one and no advantage, so that nothing flows through it)
+    part = torch.where(cut, -bound * a, -torch.exp(torch.where(cut, torch.zeros_like(d), d)) * torch.where(cut, torch.zeros_like(a), a))
+    part = torch.where(valid, part, torch.zeros_like(part))
+    x = pick(ref_log_probs) - y if ref_log_probs is not None else torch.zeros_like(y)
+    kl = torch.expm1(x) - x
+    weight = valid.double()
+    if by_sequence:
+        count = torch.zeros(sequences + 1, dtype=torch.float64, device=y.device).index_add_(0, of, weight)[:sequences]
+        per = torch.where(count > 0, 1 / count.clamp(min=1), torch.zeros_like(count)) / (count > 0).sum().clamp(min=1)
+        weight = weight * torch.cat([per, per.new_zeros(1)])[of]
+    else:
+        weight = weight / weight.sum().clamp(min=1)
+    part, kl = (part * weight).sum(), (kl * weight).sum()
+    loss = part + kl_coef * kl if kl_coef != 0 else part
+    return loss.float(), torch.stack([part, kl, (cut * weight).sum()]).detach().float()
+
+
+def preference_loss(log_probs, ref_log_probs, mask, of, sequences: int, beta: float, label_smoothing: float):
+    """Flat arguments as in :func:`policy_loss`.  Returns the loss and the rewards ``[pairs, 2]``."""
+    valid = of < sequences
+    if mask is not None:
+        valid = valid & (mask != 0)
+    v = torch.where(valid, log_probs, log_probs.new_zeros(())).double()
+    if ref_log_probs is not None:
+        v = v - torch.where(valid, ref_log_probs, ref_log_probs.new_zeros(())).double()
+    rewards = beta * torch.zeros(sequences + 1, dtype=torch.float64, device=v.device).index_add(0, of, v)[:sequences].view(-1, 2)
+    z = rewards[:, 0] - rewards[:, 1]
+    per = F.softplus(-z) + label_smoothing * z if label_smoothing else F.softplus(-z)
+    return (per.sum() / max(z.numel(), 1)).float(), rewards.detach().float()
+
+
+def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                     temperature: float = 1.0) -> torch.Tensor:
+    """``log_softmax(hidden @ weight.T / temperature)`` at ``labels``, fp32; 0 where the label is ignored or no column of the head."""
+    keep = (labels != ignore_index) & (labels >= 0) & (labels < weight.shape[0])
+    rows = hidden[keep].float()                # (rows without a label take part in nothing, whatever they hold)
+    logp = F.log_softmax(F.linear(rows, weight.float()) / temperature, dim=-1)
+    out = torch.zeros(labels.shape, dtype=torch.float32, device=hidden.device)
+    return out.masked_scatter(keep, logp.gather(-1, labels[keep][:, None])[:, 0])
