@@ -14,11 +14,16 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <pybind11/pybind11.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <tuple>
+#include <vector>
 
 extern "C" {
 const char* ksa_last_error();
@@ -95,6 +100,25 @@ int ksa_summary_attn_bwd(const void* q, const void* k, const void* v, const void
                          long long dv_rs, long long dv_bs, long long dks_rs, long long dks_bs, long long dvs_rs, long long dvs_bs,
                          int chunk, int n_sum, int chunk0, int k_off, int s_off, float scale, const void* part_k,
                          const void* part_v, int n_keys, void* stream);
+int ksa_grad_norm_parts(int tensors);
+int ksa_grad_norm(const void* src, const void* dst, const void* meta, int tensors, float scale, float most, void* partial, void* result,
+                  void* stream);
+long long ksa_token_loss_units(long long n, int sequences);
+int ksa_policy_loss(const void* y, const void* old, const void* ref, const void* adv, const void* mask, const void* cu, int wide, void* grad,
+                    void* partial, void* inv, void* loss, void* stats, int types, long long n, int sequences, long long length,
+                    int adv_by_sequence, int by_sequence, const void* bounds, float beta, void* stream);
+int ksa_policy_loss_bwd(const void* grad, const void* inv, const void* dloss, void* dy, int type, const void* cu, int wide, long long n,
+                        int sequences, long long length, int by_sequence, void* stream);
+int ksa_preference_loss(const void* y, const void* ref, const void* mask, const void* cu, int wide, void* partial, void* coef, void* rewards,
+                        void* loss, int types, long long n, int sequences, long long length, float beta, float smoothing, void* stream);
+int ksa_preference_loss_bwd(const void* mask, const void* coef, const void* dloss, void* dy, int type, const void* cu, int wide, long long n,
+                            int sequences, long long length, void* stream);
+int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
+                  void* lse2, void* work, void* y, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
+                  void* stream);
+int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
+                      const void* lse2, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
+                      long long lddw, int dw_fp32, int add_dw, int slab, float tau, void* stream);
 }
 
 namespace {
@@ -107,6 +131,7 @@ void check(const char* name, int rc, int kernels = 1) {
   g_launches.fetch_add(kernels, std::memory_order_relaxed);
 }
 #define LAUNCH(entry, ...) check(#entry, entry(__VA_ARGS__))
+#define LAUNCH_SEVERAL(kernels, entry, ...) check(#entry, entry(__VA_ARGS__), kernels)
 
 // The arguments of one call.  `plain` turns false at the first one that is not of the ordinary kind.
 struct Args {
@@ -803,13 +828,392 @@ PyObject* py_int4_linear(PyObject*, PyObject* const* v, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------------------ post-training
+// The differentiated calls of these operators are autograd nodes of this file: through Python a loss and its gradient took 150 us, whatever their size.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int token_type(const Tensor& t) {
+  return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : t.scalar_type() == at::kHalf ? 2 : -1;
+}
+bool wants_gradient(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+at::TensorOptions on(const Tensor& t, at::ScalarType type) { return at::TensorOptions().dtype(type).device(t.device()); }
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// What a backward pass of kernels returns: no graph of it exists, so whoever differentiates it again gets an error.
+Tensor differentiated_once(const Tensor& t) {
+  if (!c10::GradMode::is_enabled() || !t.defined()) return t;
+  Tensor leaf = t.detach();
+  leaf.set_requires_grad(true);
+  const auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that can be differentiated once", 1);
+  return (*error)({leaf})[0];
+}
+
+// grad_norm(gradients, targets | None, clip, scale, largest norm) -> (norm, factor)
+PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  PyObject *grads = a.next(), *out = a.next();
+  const bool clip = a.integer() != 0;
+  const float scale = a.real(), most = a.real();
+  if (!a.ok() || !(PyList_CheckExact(grads) || PyTuple_CheckExact(grads)) || (out != Py_None && !(PyList_CheckExact(out) || PyTuple_CheckExact(out))))
+    return none();
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(grads);
+  if (count == 0 || count > INT_MAX || (out != Py_None && PySequence_Fast_GET_SIZE(out) != count) || !(scale > 0.f && std::isfinite(scale)) || !(most >= 0.f))
+    return none();
+  std::vector<const void*> src(count);
+  std::vector<void*> dst(clip ? count : 0);
+  std::vector<long long> meta(count);
+  std::vector<const Tensor*> to(dst.size());
+  const auto plain = [&](PyObject* o) -> const Tensor* {
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    if (t.numel() > 0 ? !a.dense(t) : !t.is_cuda() || t.layout() != at::kStrided) return nullptr;
+    return token_type(t) >= 0 && t.is_non_overlapping_and_dense() ? &t : nullptr;
+  };
+  const Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const Tensor* t = plain(PySequence_Fast_GET_ITEM(grads, i));
+    if (!t || (first && t->device() != first->device())) return none();
+    if (!first) first = t;
+    src[i] = t->const_data_ptr();
+    meta[i] = 4 * (long long)t->numel() + token_type(*t);
+    if (!clip) continue;
+    const Tensor* o = out == Py_None ? t : plain(PySequence_Fast_GET_ITEM(out, i));
+    if (!o || o->device() != t->device() || o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() || o->strides() != t->strides() ||
+        o->is_inference())
+      return none();
+    to[i] = o;
+    dst[i] = o->mutable_data_ptr();
+  }
+  if (first->device().index() != c10::cuda::current_device()) return none();
+  if (clip) {                              // memory that is written must not be another tensor's too (in the order of most lists there is nothing to sort)
+    struct Span { uintptr_t lo, hi; bool written; };
+    std::vector<Span> spans;
+    spans.reserve(2 * count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const uintptr_t bytes = (uintptr_t)(meta[i] >> 2) * to[i]->element_size(), s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
+      if (bytes == 0) continue;
+      spans.push_back({d, d + bytes, true});
+      if (s != d) spans.push_back({s, s + bytes, false});
+    }
+    const auto before = [](const Span& x, const Span& y) { return x.lo < y.lo; };
+    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+    uintptr_t any = 0, written = 0;
+    for (const Span& s : spans) {
+      if (s.lo < (s.written ? any : written)) return none();
+      any = std::max(any, s.hi);
+      if (s.written) written = std::max(written, s.hi);
+    }
+  }
+  Tensor result;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const Tensor partial = at::empty({ksa_grad_norm_parts((int)count)}, on(*first, at::kDouble));
+    result = at::empty({2}, on(*first, at::kFloat));
+    LAUNCH_SEVERAL(2, ksa_grad_norm, src.data(), clip ? dst.data() : nullptr, meta.data(), (int)count, scale, most, partial.mutable_data_ptr(),
+                   result.mutable_data_ptr(), stream_of(*first));
+    for (const Tensor* o : to) o->unsafeGetTensorImpl()->bump_version();
+  }
+  return wrap(result.select(0, 0), result.select(0, 1));
+  END_HANDLE_TH_ERRORS
+}
+
+// Tokens as rows or packed: the rules of _sequences in ops/token_losses.py.
+struct TokenArgs {
+  const Tensor* y = nullptr;
+  const Tensor* mask = nullptr;
+  const Tensor* cu = nullptr;
+  long long n = 0, length = 0;
+  int sequences = 0;
+
+  const void* offsets() const { return cu ? cu->const_data_ptr() : nullptr; }
+  int wide() const { return cu && cu->scalar_type() == at::kLong; }
+};
+const Tensor* token_values(Args& a, bool optional = false) {
+  PyObject* o = a.next();
+  if (optional && o == Py_None) return nullptr;
+  if (!THPVariable_CheckExact(o)) { a.plain = false; return nullptr; }
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!a.dense(t) || token_type(t) < 0 || !t.is_contiguous()) a.plain = false;
+  return &t;
+}
+const Tensor* token_integers(Args& a, std::initializer_list<at::ScalarType> types) {
+  PyObject* o = a.next();
+  if (o == Py_None) return nullptr;
+  if (!THPVariable_CheckExact(o)) { a.plain = false; return nullptr; }
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!a.dense(t) || std::find(types.begin(), types.end(), t.scalar_type()) == types.end() || !t.is_contiguous()) a.plain = false;
+  return &t;
+}
+bool token_rows(TokenArgs& t) {
+  if (t.mask && t.mask->sizes() != t.y->sizes()) return false;
+  t.n = t.y->numel();
+  if (t.cu) {
+    t.sequences = (int)t.cu->numel() - 1;
+    return t.cu->dim() == 1 && t.cu->numel() <= INT_MAX && (t.y->dim() == 1 || (t.y->dim() == 2 && t.y->size(0) == 1));
+  }
+  if (t.y->dim() != 1 && t.y->dim() != 2) return false;
+  t.length = t.y->size(-1);
+  t.sequences = t.y->dim() == 1 ? 1 : (int)t.y->size(0);
+  return t.n / t.length <= INT_MAX;
+}
+bool same_shape(const Tensor* t, const Tensor* y) { return !t || t->sizes() == y->sizes(); }
+double real64(PyObject* o, bool& plain) {
+  const double x = PyFloat_Check(o) || PyLong_Check(o) ? PyFloat_AsDouble(o) : (plain = false, 0.0);
+  if (PyErr_Occurred()) { PyErr_Clear(); plain = false; }
+  return x;
+}
+
+struct PolicyCall {
+  TokenArgs t;
+  const Tensor *old = nullptr, *ref = nullptr, *adv = nullptr;
+  int adv_by_sequence = 0, by_sequence = 0;
+  double bounds[4] = {0, 0, 0, 0};
+  float beta = 0;
+
+  // {loss, statistics, gradients up to the normaliser (only where wanted), normalisers}
+  std::tuple<Tensor, Tensor, Tensor, Tensor> run(bool keep) const {
+    const Tensor& y = *t.y;
+    const Tensor loss = at::empty({}, on(y, at::kFloat)), stats = at::empty({3}, on(y, at::kFloat)), inv = at::empty({std::max(t.sequences, 1)}, on(y, at::kFloat));
+    const Tensor partial = at::empty({(int64_t)(4 * ksa_token_loss_units(t.n, t.sequences))}, on(y, at::kDouble));
+    Tensor grad;
+    if (keep) grad = at::empty({(int64_t)t.n}, on(y, at::kFloat));
+    const int types = token_type(y) | token_type(*old) << 4 | (ref ? token_type(*ref) : 0) << 8 | token_type(*adv) << 12;
+    LAUNCH_SEVERAL(2, ksa_policy_loss, y.const_data_ptr(), old->const_data_ptr(), ref ? ref->const_data_ptr() : nullptr, adv->const_data_ptr(),
+                   t.mask ? t.mask->const_data_ptr() : nullptr, t.offsets(), t.wide(), keep ? grad.mutable_data_ptr() : nullptr,
+                   partial.mutable_data_ptr(), inv.mutable_data_ptr(), loss.mutable_data_ptr(), stats.mutable_data_ptr(), types, t.n, t.sequences, t.length,
+                   adv_by_sequence, by_sequence, bounds, beta, stream_of(y));
+    return {loss, stats, grad, inv};
+  }
+};
+struct PolicyNode : public torch::autograd::Function<PolicyNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& y, const PolicyCall* call) {
+    auto [loss, stats, grad, inv] = call->run(true);
+    ctx->save_for_backward({grad, inv, call->t.cu ? *call->t.cu : Tensor()});
+    ctx->saved_data["sequences"] = (int64_t)call->t.sequences;
+    ctx->saved_data["length"] = (int64_t)call->t.length;
+    ctx->saved_data["by_sequence"] = (int64_t)call->by_sequence;
+    ctx->saved_data["shape"] = y.sizes().vec();
+    ctx->saved_data["type"] = (int64_t)y.scalar_type();
+    ctx->mark_non_differentiable({stats});
+    ctx->set_materialize_grads(false);          // (the statistics' would be zeros in memory of their own)
+    return {loss, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &grad = saved[0], &inv = saved[1], &cu = saved[2], &dloss = grads[0];
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    Tensor dy = at::empty(ctx->saved_data["shape"].toIntVector(), on(grad, type));
+    LAUNCH(ksa_policy_loss_bwd, grad.const_data_ptr(), inv.const_data_ptr(), dloss.const_data_ptr(), dy.mutable_data_ptr(), token_type(dy),
+           cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, grad.numel(), (int)ctx->saved_data["sequences"].toInt(),
+           ctx->saved_data["length"].toInt(), (int)ctx->saved_data["by_sequence"].toInt(), stream_of(grad));
+    return {differentiated_once(dy), Tensor()};
+  }
+};
+
+// policy_loss(y, old, advantages, ref | None, mask | None, cu | None, clip_low, clip_high, kl_coef, by_sequence) -> (loss, statistics)
+PyObject* py_policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  PolicyCall c;
+  c.t.y = token_values(a);
+  c.old = token_values(a);
+  c.adv = token_values(a);
+  c.ref = token_values(a, true);
+  c.t.mask = token_integers(a, {at::kBool, at::kByte});
+  c.t.cu = token_integers(a, {at::kInt, at::kLong});
+  const double low = real64(a.next(), a.plain), high = real64(a.next(), a.plain);
+  c.beta = a.real();
+  c.by_sequence = a.integer() != 0;
+  if (!a.ok() || !token_rows(c.t) || !same_shape(c.old, c.t.y) || !same_shape(c.ref, c.t.y) || !(low >= 0 && low <= 1 && high >= 0) || !std::isfinite(c.beta))
+    return none();
+  c.adv_by_sequence = !same_shape(c.adv, c.t.y);
+  if (c.adv_by_sequence && !(c.adv->numel() == c.t.sequences && (c.adv->dim() == 1 || (c.adv->dim() == 2 && c.adv->size(1) == 1)))) return none();
+  if (wants_gradient(*c.old) || wants_gradient(*c.adv) || (c.ref && wants_gradient(*c.ref))) return none();
+  c.bounds[0] = std::log1p(high);
+  c.bounds[1] = low < 1 ? std::log1p(-low) : -INFINITY;
+  c.bounds[2] = 1 + high;
+  c.bounds[3] = 1 - low;
+  Tensor loss, stats;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (wants_gradient(*c.t.y)) {
+      auto made = PolicyNode::apply(*c.t.y, &c);
+      loss = made[0];
+      stats = made[1];
+    } else {
+      std::tie(loss, stats, std::ignore, std::ignore) = c.run(false);
+    }
+  }
+  return wrap(loss, stats);
+  END_HANDLE_TH_ERRORS
+}
+
+struct PreferenceCall {
+  TokenArgs t;
+  const Tensor* ref = nullptr;
+  float beta = 0, smoothing = 0;
+
+  std::tuple<Tensor, Tensor, Tensor> run() const {          // {loss, rewards, coefficients}
+    const Tensor& y = *t.y;
+    const Tensor loss = at::empty({}, on(y, at::kFloat)), rewards = at::empty({t.sequences / 2, 2}, on(y, at::kFloat)), coef = at::empty({t.sequences}, on(y, at::kFloat));
+    const Tensor partial = at::empty({(int64_t)ksa_token_loss_units(t.n, t.sequences)}, on(y, at::kDouble));
+    LAUNCH_SEVERAL(2, ksa_preference_loss, y.const_data_ptr(), ref ? ref->const_data_ptr() : nullptr, t.mask ? t.mask->const_data_ptr() : nullptr, t.offsets(), t.wide(),
+                   partial.mutable_data_ptr(), coef.mutable_data_ptr(), rewards.mutable_data_ptr(), loss.mutable_data_ptr(),
+                   token_type(y) | (ref ? token_type(*ref) : 0) << 4, t.n, t.sequences, t.length, beta, smoothing, stream_of(y));
+    return {loss, rewards, coef};
+  }
+};
+struct PreferenceNode : public torch::autograd::Function<PreferenceNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& y, const PreferenceCall* call) {
+    auto [loss, rewards, coef] = call->run();
+    ctx->save_for_backward({coef, call->t.mask ? *call->t.mask : Tensor(), call->t.cu ? *call->t.cu : Tensor()});
+    ctx->saved_data["length"] = (int64_t)call->t.length;
+    ctx->saved_data["shape"] = y.sizes().vec();
+    ctx->saved_data["type"] = (int64_t)y.scalar_type();
+    ctx->mark_non_differentiable({rewards});
+    ctx->set_materialize_grads(false);
+    return {loss, rewards};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &coef = saved[0], &mask = saved[1], &cu = saved[2], &dloss = grads[0];
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    Tensor dy = at::empty(ctx->saved_data["shape"].toIntVector(), on(coef, type));
+    LAUNCH(ksa_preference_loss_bwd, mask.defined() ? mask.const_data_ptr() : nullptr, coef.const_data_ptr(), dloss.const_data_ptr(), dy.mutable_data_ptr(),
+           token_type(dy), cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, dy.numel(), (int)coef.numel(),
+           ctx->saved_data["length"].toInt(), stream_of(coef));
+    return {differentiated_once(dy), Tensor()};
+  }
+};
+
+// preference_loss(y, ref | None, mask | None, cu | None, beta, label_smoothing) -> (loss, rewards)
+PyObject* py_preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  PreferenceCall c;
+  c.t.y = token_values(a);
+  c.ref = token_values(a, true);
+  c.t.mask = token_integers(a, {at::kBool, at::kByte});
+  c.t.cu = token_integers(a, {at::kInt, at::kLong});
+  c.beta = a.real();
+  c.smoothing = a.real();
+  if (!a.ok() || !token_rows(c.t) || c.t.sequences % 2 != 0 || c.t.sequences == 0 || !same_shape(c.ref, c.t.y) || !std::isfinite(c.beta) ||
+      !(c.smoothing >= 0 && c.smoothing <= 1) || (c.ref && wants_gradient(*c.ref)))
+    return none();
+  Tensor loss, rewards;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (wants_gradient(*c.t.y)) {
+      auto made = PreferenceNode::apply(*c.t.y, &c);
+      loss = made[0];
+      rewards = made[1];
+    } else {
+      std::tie(loss, rewards, std::ignore) = c.run();
+    }
+  }
+  return wrap(loss, rewards);
+  END_HANDLE_TH_ERRORS
+}
+
+struct LogProbsCall {
+  const Tensor* labels = nullptr;
+  long long ignore = 0, pad = 0, columns = 0, slab_bytes = 0;
+  float tau = 1;
+};
+struct LogProbsKept {
+  Tensor y, dense, ints, lse2;             // ints: rows, row_label, place, count
+};
+LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c) {
+  const long long T = c.labels->numel(), V = w.size(0), D = w.size(1), padded = (T + c.pad - 1) / c.pad * c.pad;
+  LogProbsKept k;
+  k.y = at::empty(c.labels->sizes(), on(h, at::kFloat));
+  k.dense = at::empty({(int64_t)padded, (int64_t)D}, on(h, at::kBFloat16));
+  k.ints = at::empty({(int64_t)(3 * T + 1)}, on(h, at::kInt));
+  k.lse2 = at::empty({(int64_t)T}, on(h, at::kFloat));
+  const Tensor work = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns + 1))}, on(h, at::kFloat));
+  int* ints = static_cast<int*>(k.ints.mutable_data_ptr());
+  LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), ints, ints + T, ints + 2 * T,
+                 ints + 3 * T, k.lse2.mutable_data_ptr(), work.mutable_data_ptr(), k.y.mutable_data_ptr(), (int)T, (int)V, (int)D,
+                 h.dim() == 2 ? h.stride(0) : D, w.stride(0), c.ignore, c.tau, stream_of(h));
+  return k;
+}
+struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const LogProbsCall* call) {
+    const LogProbsKept k = log_probs(h, w, *call);
+    ctx->save_for_backward({k.dense, w, k.ints, k.lse2});
+    ctx->saved_data["shape"] = h.sizes().vec();
+    ctx->saved_data["tau"] = (double)call->tau;
+    ctx->saved_data["slab_bytes"] = (int64_t)call->slab_bytes;
+    return k.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &dense = saved[0], &w = saved[1], &ints = saved[2], &lse2 = saved[3];
+    const long long T = lse2.numel(), V = w.size(0), D = w.size(1), padded = dense.size(0);
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const Tensor dy = grads[0].contiguous();
+    const long long slab = std::min((V + 7) / 8 * 8, std::max(256ll, ctx->saved_data["slab_bytes"].toInt() / (2 * padded) / 256 * 256));
+    const Tensor dx = at::empty({(int64_t)padded, (int64_t)slab}, on(w, at::kBFloat16));
+    Tensor dh, dh32, dw;
+    if (need_h) {
+      dh = at::empty(ctx->saved_data["shape"].toIntVector(), on(w, at::kBFloat16));
+      dh32 = at::empty({(int64_t)padded, (int64_t)D}, on(w, at::kFloat));
+    }
+    if (need_w) dw = at::empty({(int64_t)V, (int64_t)D}, on(w, at::kBFloat16));
+    const int* p = static_cast<const int*>(ints.const_data_ptr());
+    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, lse2.const_data_ptr(), dy.const_data_ptr(),
+                   dx.mutable_data_ptr(), need_h ? dh32.mutable_data_ptr() : nullptr, need_h ? dh.mutable_data_ptr() : nullptr,
+                   need_w ? dw.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D, w.stride(0), D, 0, 0, (int)slab, (float)ctx->saved_data["tau"].toDouble(),
+                   stream_of(w));
+    return {differentiated_once(dh), differentiated_once(dw), Tensor()};
+  }
+};
+
+// linear_log_probs(h [..., D], w, labels [...], ignore_index, temperature, row pad, columns of a sum, slab bytes) -> y [...]
+PyObject* py_linear_log_probs(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a(v, n);
+  const Tensor* h = a.tensor();
+  PyObject* weight = a.next();
+  if (!THPVariable_CheckExact(weight)) return none();
+  const Tensor& w = THPVariable_Unpack(weight);
+  LogProbsCall c;
+  c.labels = a.tensor(at::kLong);
+  c.ignore = a.integer();
+  c.tau = a.real();
+  c.pad = a.integer();
+  c.columns = a.integer();
+  PyObject* bytes = a.next();
+  c.slab_bytes = PyLong_Check(bytes) ? PyLong_AsLongLong(bytes) : -1;
+  if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  if (!a.ok() || !a.dense(w) || w.scalar_type() != at::kBFloat16 || !rows2d(&w) || !aligned(&w) || w.size(1) % 8 != 0 || w.stride(0) % 8 != 0 ||
+      w.stride(0) < w.size(1) || h->dim() < 1 || h->size(-1) != w.size(1) || c.labels->sizes() != h->sizes().slice(0, h->dim() - 1) ||
+      !(h->is_contiguous() || rows2d(h)) || !c.labels->is_contiguous() || !fits(w.size(0)) || c.labels->numel() > INT_MAX / 4 || !(c.tau > 0 && std::isfinite(c.tau)) ||
+      c.pad <= 0 || c.columns <= 0 || c.slab_bytes < 0)
+    return none();
+  const bool grad = wants_gradient(*h) || wants_gradient(w);
+  if (grad && PyObject_HasAttrString(weight, "main_grad")) return none();                  // its gradient goes to a buffer that Python knows
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    y = grad ? LogProbsNode::apply(*h, w, &c) : log_probs(*h, w, c).y;
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(g_launches.load()); }
 
 #define FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FN(gemm), FN(linear), FN(linear_dw), FN(dual_linear), FN(rms_norm), FN(rms_norm_bwd), FN(qk_norm_rope),
                            FN(qk_norm_rope_bwd), FN(swiglu), FN(swiglu_bwd), FN(linear_swiglu), FN(gemm_swiglu), FN(norm_linear), FN(attention),
                            FN(attention_bwd), FN(int4_cache_write), FN(int4_cache_read),
-                           FN(int4_decode_attention), FN(int4_linear), FN(launches), {nullptr, nullptr, 0, nullptr}};
+                           FN(int4_decode_attention), FN(int4_linear), FN(grad_norm), FN(policy_loss), FN(preference_loss),
+                           FN(linear_log_probs), FN(launches), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "ksa_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -19,7 +19,6 @@ returned to autograd in the weight's dtype.
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 from typing import Optional, Tuple
@@ -29,6 +28,7 @@ import torch
 from . import reference as ref
 from . import _lib
 from ._lib import native as _native
+from .calls import observed as _observed
 from .layout import SummaryLayout, get_layout
 
 UNBOUNDED_WINDOW = 1 << 30
@@ -47,19 +47,6 @@ class _NoGrad:
 
     def save_for_backward(self, *tensors):
         pass
-
-
-# private to PyTorch: without them every call counts as observed
-_transforms_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: True)
-_forward_level = functools.partial(getattr, torch.autograd.forward_ad, "_current_level", 0)
-_is_tracing, _is_compiling = torch.jit.is_tracing, torch.compiler.is_compiling
-
-
-def _observed() -> bool:
-    """Whether someone follows the calls themselves: a ``torch.func`` transform, forward-mode differentiation, a trace, a compiler.
-    They must meet the autograd function (its error, or its node in their graph) and not the bare kernel call, which would take
-    the wrappers' memory for that of their tensors."""
-    return _transforms_active() or _forward_level() >= 0 or _is_tracing() or _is_compiling()
 
 
 def _run(fn, *args):

@@ -17,6 +17,8 @@ import torch
 
 from . import _lib
 from . import reference as ref
+from ._lib import native as _native
+from .calls import observed as _observed
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -84,6 +86,11 @@ def grad_norm(grads: Iterable[torch.Tensor], scale: float = 1.0,
               max_norm: Optional[float] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """The global 2-norm of ``grads`` times ``scale``, an fp32 scalar on their device; with ``max_norm`` also the factor that
     clips: ``scale * min(1, max_norm / (norm + 1e-6))``."""
+    grads = grads if isinstance(grads, (list, tuple)) else list(grads)
+    if not _observed():
+        made = _native.grad_norm(grads, None, False, scale, math.inf if max_norm is None else max_norm)
+        if made is not None:
+            return made[0] if max_norm is None else made
     grads = _check(grads, scale)
     most = math.inf if max_norm is None else _check_most(max_norm)
     with torch.no_grad():
@@ -99,6 +106,11 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float, scale: float
     """Multiply every gradient by ``scale * min(1, max_norm / (norm + 1e-6))`` and return ``norm``, the global 2-norm times
     ``scale``.  In place, or into the tensors ``out`` (of the gradients' shapes and types); gradients that share memory with
     one another are refused.  A norm that is no number makes all of them so, an infinite one makes them zero where they are finite."""
+    grads = grads if isinstance(grads, (list, tuple)) else list(grads)
+    if not _observed():
+        made = _native.grad_norm(grads, out, True, scale, max_norm)
+        if made is not None:
+            return made[0]
     grads = _check(grads, scale)
     most = _check_most(max_norm)
     to = grads if out is None else list(out)
@@ -121,5 +133,5 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float, scale: float
         for o, d in zip(to, dst):
             if d is not o:
                 o.copy_(d)
-        torch.autograd.graph.increment_version(to)
+        torch.autograd.graph.increment_version([t for t in to if not t.is_inference()])
     return norm

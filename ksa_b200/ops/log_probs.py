@@ -8,7 +8,9 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import reference as ref
-from .token_losses import _Forward, _observed
+from ._lib import native as _native
+from .calls import observed as _observed
+from .token_losses import _Forward
 
 _ROW_PAD = 256              # rows of the gathered arrays: a multiple of this (kLpRowPad in csrc/log_probs.cu)
 _STAT_COLS = 128            # columns that share a log-sum (kLpStatCols)
@@ -90,6 +92,10 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  The logits are never in
     memory: the forward pass keeps what its tiles' sums need, the backward pass computes them again, at most 4 GB of their gradient at a time.
     With ``main_grad`` on the weight its gradient goes there."""
+    if not _observed():
+        y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES)
+        if y is not None:
+            return y
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"rows {tuple(hidden.shape)} and an output head {tuple(weight.shape)}")
     if labels.shape != hidden.shape[:-1] or labels.dtype not in (torch.int64, torch.int32):

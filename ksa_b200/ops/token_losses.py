@@ -18,6 +18,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import reference as ref
+from ._lib import native as _native
+from .calls import observed as _observed
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -132,6 +134,11 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
     have one of each sequence's mean; without any valid token the loss is 0.  ``stats`` (fp32 ``[3]``, no gradient): the same means of the clipped
     part, of ``K`` and of being cut off, that is ``A > 0`` with ``r > 1 + clip_high`` or ``A < 0`` with ``r < 1 - clip_low``; such a token has no
     gradient but that of ``K``.  With a ``kl_coef`` of 0 the reference counts in the statistics alone."""
+    if not _observed() and reduction in ("token", "sequence"):
+        made = _native.policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, cu_seqlens, clip_low, clip_high, kl_coef,
+                                   reduction == "sequence")
+        if made is not None:
+            return made
     _check(log_probs, mask, cu_seqlens, (("old_log_probs", old_log_probs), ("advantages", advantages), ("ref_log_probs", ref_log_probs)))
     seq = _sequences(log_probs, cu_seqlens)
     by_token = advantages.shape == log_probs.shape
@@ -186,6 +193,10 @@ def preference_loss(log_probs: torch.Tensor, ref_log_probs: Optional[torch.Tenso
     (``log_probs`` alone without a reference) over the valid tokens of sequence ``s``, ``z_i = beta (D_2i - D_2i+1)``; the loss is the mean over
     the pairs of ``(1 - label_smoothing) log(1 + exp(-z)) + label_smoothing log(1 + exp(z))``, 0 without any pair.  ``rewards`` (fp32
     ``[pairs, 2]``, no gradient): ``beta D``.  An answer without valid tokens has ``D = 0``."""
+    if not _observed():
+        made = _native.preference_loss(log_probs, ref_log_probs, mask, cu_seqlens, beta, label_smoothing)
+        if made is not None:
+            return made
     _check(log_probs, mask, cu_seqlens, (("ref_log_probs", ref_log_probs),))
     seq = _sequences(log_probs, cu_seqlens)
     if seq.count % 2 != 0:
@@ -198,7 +209,3 @@ def preference_loss(log_probs: torch.Tensor, ref_log_probs: Optional[torch.Tenso
         return ref.preference_loss(flat(log_probs), flat(ref_log_probs), flat(mask), of, seq.count, beta, label_smoothing)
     return _run(_PreferenceLossFn, log_probs, ref_log_probs, mask, seq, beta, label_smoothing)
 
-
-def _observed() -> bool:
-    from . import _observed as observed          # (defined beside the other operators)
-    return observed()
