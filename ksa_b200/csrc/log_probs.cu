@@ -2,9 +2,12 @@
 //   x_tv = h_t . w_v / tau,   y_t = x_t,label - log sum_v exp(x_tv);
 //   dx_tv = dy_t ([v = label] - exp(x_tv - lse_t)) / tau,   dh = dx w,   dw = dx^T h.
 //
-// Bound: the products, 2 n V D operations forward and three times that backward (the logits are computed again, from which dx
-// comes in the accumulators' precision; kept in bf16 they would save one product of four and cost their rounding, 2^-9 of a logit).  At 16 rows
-// and fewer the weights' bytes.
+// Bound: the products, 2 n V D operations forward and twice that backward; at 16 rows and fewer the weights' bytes.
+//
+// The backward pass needs the logits again.  Where 16 bits of each fit the caller's limit the forward pass keeps them, as the distance below the
+// maximum of their 128 columns in steps of 2^-10 of a power of two: probabilities from them are off by 2^-12 of themselves, next to
+// nothing beside the rounding of dx to bf16 (kept as bf16 a logit of 10 would be off by 2^-6), and what is more than 64 powers below the maximum counts as
+// that far.  Above the limit the product is computed again, a quarter more of all products.
 //
 // Rows without a label are left out first: the others are gathered into a dense array, and the kernels take their number from device
 // memory, so that prompts and masked turns cost nothing but their labels, and what their rows hold reaches no sum.
@@ -12,7 +15,7 @@
 // One kernel on CTA pairs (gemm2.cu describes its roles and barriers) serves four products, which differ in their epilogue:
 //   kStats  h w^T: every thread has one row of the tile; it takes the maximum and the sum of exponentials of 128 columns, and writes their
 //           log-sum (base 2) as one number.  A second kernel adds those of a row.
-//   kGrad   the same product again: dx in bf16.
+//   kStatsKeep  the same, and the logits in 16 bits;  kGrad  the product again, dx in bf16 from the accumulators.
 //   kDh     dx w, fp32, over the columns of one slab;  kDw  dx^T h.
 // dx exists for a slab of the vocabulary at a time (the caller says how wide): the slabs' dw are disjoint, and dh is added up in fp32.
 #include "common.cuh"
@@ -39,9 +42,10 @@ constexpr int kLpSmem = kLpStages * kLpStageBytes + kLpStoreBytes + 256 + 1024;
 static_assert(kLpSmem <= 232448, "227 KB");
 static_assert(kLpSmem >= kTmemClusterAlone, "a pair holds all tensor memory: no block of another cluster beside it (host.h)");
 constexpr int kLpStatCols = 128;                                        // columns that share a log-sum
+constexpr float kLpCodes = 1024.f;                                      // codes of a kept logit to a power of two
 constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
 
-enum LpMode : int { kStats = 0, kGrad = 1, kDh = 2, kDw = 3 };
+enum LpMode : int { kStats = 0, kGrad = 1, kDh = 2, kDw = 3, kStatsKeep = 4 };
 
 struct LpArgs {
   int M, N, K;                 // at most; *count stands for M, or for K in kDw
@@ -52,20 +56,37 @@ struct LpArgs {
   float inv_tau;
   float* stats;                // kStats: [ceil(N / 128)][ld_stats] log-sums, base 2
   float* picked;               // kStats: [rows] x of the label times log2(e)
+  float* tops;                 // kStatsKeep: [ceil(N / 128)][ld_stats] maxima, base 2
   long long ld_stats;
   const float* lse2;           // kGrad: [rows]
   const float* dy;             // kGrad: gradient of y, by the rows' places
   int col0;                    // kGrad: first column of the slab
   int add;                     // kDh, kDw: into fp32, added to what is there
+  int planes;                  // kDh: K is cut into at most so many parts, each with an output of its own
+  int plane_rows;
   int bf16_out;                // kDw
   int* status;
 };
+
+// Parts that kDh cuts K (the vocabulary) into: its tiles are few and long, 160 for 4915 rows of 2048 on 74 pairs, and the last wave of whole ones would be
+// a third of the time (2594 us; in parts 2200).  Every part has an output of its own, which the scattering kernel adds up in order.  The rule takes the fewest
+// steps of kLpBK on the busiest pair, a part costing some 10 more for its output.
+__device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int most) {
+  int best = 1;
+  const int last = tiles % n_pairs;
+  long long least = (long long)(tiles / n_pairs) * (num_kb + 10) + (last == 0 ? 0 : 2 * last <= n_pairs ? (num_kb * 5 + 7) / 8 + 10 : num_kb + 10);
+  for (int s = 2; s <= most && num_kb / s >= 8; ++s) {
+    const long long steps = ((long long)tiles * s + n_pairs - 1) / n_pairs * ((num_kb + s - 1) / s + 10);
+    if (steps < least) { least = steps; best = s; }
+  }
+  return best;
+}
 
 template <int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
 log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                       const __grid_constant__ LpArgs a) {
-  constexpr bool kAMn = kMode == kDw, kBMn = kMode == kDh || kMode == kDw;
+  constexpr bool kAMn = kMode == kDw, kBMn = kMode == kDh || kMode == kDw, kSums = kMode == kStats || kMode == kStatsKeep;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + kLpStages * kLpStageBytes;
@@ -102,10 +123,11 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const int tiles_m = (M + 2 * kLpBM - 1) / (2 * kLpBM), tiles_n = (N + kLpBN - 1) / kLpBN;
   const int num_tiles = tiles_m * tiles_n;
   const int num_kb = (K + kLpBK - 1) / kLpBK;
+  const int parts_k = kMode == kDh ? lp_parts(num_tiles, num_kb, n_pairs, a.planes) : 1, part_kb = (num_kb + parts_k - 1) / parts_k;
   // A last wave of at most half as many tiles as pairs is worked on as halves of 128 columns (gemm2.cu)
   const int last = num_tiles % n_pairs;
-  const int halves_from = 2 * last <= n_pairs ? num_tiles - last : num_tiles;
-  const int units = 2 * num_tiles - halves_from;
+  const int halves_from = parts_k > 1 ? num_tiles * parts_k : 2 * last <= n_pairs ? num_tiles - last : num_tiles;
+  const int units = parts_k > 1 ? num_tiles * parts_k : 2 * num_tiles - halves_from;
 
   auto tile_coords = [&](int tile, int& mb, int& nb) {
     const int per_group = kLpGroupM * tiles_n;
@@ -116,9 +138,11 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     mb = first_m + in_group % group_rows;
     nb = in_group / group_rows;
   };
-  // A unit is a tile, or one half of its columns: `side` is that half, -1 for the whole
+  // A unit is a tile, one half of its columns (`side` is that half, -1 for the whole), or one part of its K: all tiles of a part follow one
+  // another, so that pairs at work together read the same rows of both operands
   auto unit_tile = [&](int unit, int& side) {
     side = -1;
+    if (kMode == kDh && parts_k > 1) return unit % num_tiles;
     if (unit < halves_from) return unit;
     side = (unit - halves_from) & 1;
     return halves_from + ((unit - halves_from) >> 1);
@@ -136,7 +160,8 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         const int row0 = mb * 2 * kLpBM + (int)rank * kLpBM;
         const int col0 = side < 0 ? nb * kLpBN + (int)rank * kLpBNh : nb * kLpBN + side * kLpBNh + (int)rank * 64;
         const int boxes = side >= 0 ? 1 : 2;                             // of 64 rows
-        for (int kb = 0; kb < num_kb; ++kb) {
+        const int kb0 = kMode == kDh && parts_k > 1 ? unit / num_tiles * part_kb : 0, kb1 = min(kb0 + part_kb, num_kb);
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty)) { ok = false; break; }
           uint8_t* sa = smem + stage * kLpStageBytes;
           uint8_t* sb = sa + kLpABytes;
@@ -174,7 +199,8 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (!mbar_wait(&acc_empty[buf], acc_phase ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * kLpBN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        const int kb0 = kMode == kDh && parts_k > 1 ? unit / num_tiles * part_kb : 0, kb1 = min(kb0 + part_kb, num_kb);
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * kLpStageBytes);
@@ -183,7 +209,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           for (int k = 0; k < kLpBK / 16; ++k) {
             const uint64_t da = kAMn ? smem_desc_mnmajor_sw128(sa + k * 2048, 8192) : smem_desc_kmajor_sw128(sa + k * 32);
             const uint64_t db = kBMn ? smem_desc_mnmajor_sw128(sb + k * 2048, 8192) : smem_desc_kmajor_sw128(sb + k * 32);
-            umma2_ss(d_tmem, da, db, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma2_ss(d_tmem, da, db, idesc, kb != kb0 || k != 0 ? 1u : 0u);
           }
           umma2_commit_both(&empty[stage]);
           if (++stage == kLpStages) { stage = 0; phase ^= 1; }
@@ -225,7 +251,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       const bool live = kMode == kDw || row < M;
       int label = -1;
       float lse2 = 0.f, g = 0.f;
-      if ((kMode == kStats || kMode == kGrad) && live) label = a.row_label[row];
+      if ((kSums || kMode == kGrad) && live) label = a.row_label[row];
       if (kMode == kGrad && live) {
         lse2 = a.lse2[row];
         g = a.dy[a.rows[row]] * a.inv_tau;
@@ -238,7 +264,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       for (int part = 0; part < parts; ++part) {
         const int col = col_base + part * kLpStatCols;
         if (col >= N) break;
-        if (kMode == kStats) {
+        if (kSums) {
           uint32_t r[kLpStatCols];
 #pragma unroll
           for (int i = 0; i < kLpStatCols / 32; ++i) tmem_ld32(t_row + part * kLpStatCols + i * 32, *reinterpret_cast<uint32_t(*)[32]>(r + i * 32));
@@ -266,7 +292,24 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < kLpStatCols; ++j) s[j & 3] += fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -top));
-          if (live) a.stats[(long long)(col / kLpStatCols) * a.ld_stats + row] = top + __log2f((s[0] + s[1]) + (s[2] + s[3]));
+          const long long slot = (long long)(col / kLpStatCols) * a.ld_stats + row;
+          if (live) a.stats[slot] = top + __log2f((s[0] + s[1]) + (s[2] + s[3]));
+          if (kMode == kStatsKeep) {
+            if (live) a.tops[slot] = mx == -INFINITY ? mx : top;
+#pragma unroll
+            for (int piece = 0; piece < 2; ++piece) {
+              if (col + piece * 64 >= N) break;
+              uint32_t out[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                // a whole number next to 2^23 has it in its low bits
+                const float x0 = __uint_as_float(r[piece * 64 + 2 * j]), x1 = __uint_as_float(r[piece * 64 + 2 * j + 1]), by = -kLpCodes * a.scale2;
+                const float u0 = fminf(fmaf(x0, by, top * kLpCodes), 65535.f) + 8388608.f, u1 = fminf(fmaf(x1, by, top * kLpCodes), 65535.f) + 8388608.f;
+                out[j] = __byte_perm(__float_as_uint(u0), __float_as_uint(u1), 0x5410);
+              }
+              store_box(out, col + piece * 64, row_w, false);
+            }
+          }
         } else if (kMode == kGrad) {
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece) {
@@ -310,10 +353,10 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
               tmem_ld32(t_row + part * kLpStatCols + piece * 32, out);
               tmem_wait_ld();
             }
-            if (num_kb == 0)                                             // no rows at all: nothing was multiplied
+            if (kMode == kDw && num_kb == 0)                             // no rows at all: nothing was multiplied
 #pragma unroll
               for (int j = 0; j < 32; ++j) out[j] = 0u;
-            if (row_w < a.M) store_box(out, c, row_w, a.add != 0);
+            if (row_w < a.M) store_box(out, c, kMode == kDh && parts_k > 1 ? unit / num_tiles * a.plane_rows + row_w : row_w, a.add != 0);
           }
         }
       }
@@ -335,108 +378,238 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
-// Which rows have a label, in order: rows[i], row_label[i] and count; place[t] of every row (-1: none), and y[t] = 0 for those.
+// Which rows have a label, in order: rows[i], row_label[i] and count; place[t] of every row (-1: none), and y[t] = 0 for those.  One block; a
+// warp takes kLpSelectEach times 32 rows in a round, so that 8192 rows are one round of loads and one scan.
 constexpr int kLpSelect = 1024;
+constexpr int kLpSelectEach = 8;
+__device__ __forceinline__ bool lp_has_label(long long label, int V, long long ignore) { return label != ignore && label >= 0 && label < V; }
 __global__ void __launch_bounds__(kLpSelect)
 log_probs_select_kernel(const long long* labels, int T, int V, long long ignore, int* rows, int* row_label, int* place, int* count, float* y) {
   __shared__ int sums[kLpSelect / 32];
   grid_dependency_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int before = 0;
-  for (int t0 = 0; t0 < T; t0 += kLpSelect) {
-    const int t = t0 + threadIdx.x;
-    const long long label = t < T ? labels[t] : -1;
-    const bool has = t < T && label != ignore && label >= 0 && label < V;
-    const unsigned votes = __ballot_sync(0xffffffffu, has);
-    if (lane == 0) sums[warp] = __popc(votes);
+  for (long long t0 = 0; t0 < T; t0 += kLpSelect * kLpSelectEach) {
+    const long long t = t0 + warp * 32 * kLpSelectEach + lane;
+    long long label[kLpSelectEach];
+    unsigned votes[kLpSelectEach];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < kLpSelectEach; ++j) label[j] = t + j * 32 < T ? labels[t + j * 32] : -1;
+#pragma unroll
+    for (int j = 0; j < kLpSelectEach; ++j) {
+      votes[j] = __ballot_sync(0xffffffffu, t + j * 32 < T && lp_has_label(label[j], V, ignore));
+      mine += __popc(votes[j]);
+    }
+    if (lane == 0) sums[warp] = mine;
     __syncthreads();
-    int mine = sums[lane], up = mine;                                    // 32 warps: an inclusive sum over them in every warp
+    int all = sums[lane];                                                // 32 warps: an inclusive sum over them in every warp
+    const int own = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += v;
+      const int v = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += v;
     }
-    const int at = before + __shfl_sync(0xffffffffu, up - mine, warp) + __popc(votes & ((1u << lane) - 1));
-    if (t < T) {
-      place[t] = has ? at : -1;
-      if (has) { rows[at] = t; row_label[at] = (int)label; }
-      else y[t] = 0.f;
+    int at = before + __shfl_sync(0xffffffffu, all - own, warp);
+#pragma unroll
+    for (int j = 0; j < kLpSelectEach; ++j) {
+      if (t + j * 32 < T) {
+        const bool one = votes[j] >> lane & 1;
+        const int i = at + __popc(votes[j] & ((1u << lane) - 1));
+        place[t + j * 32] = one ? i : -1;
+        if (one) { rows[i] = (int)(t + j * 32); row_label[i] = (int)label[j]; }
+        else y[t + j * 32] = 0.f;
+      }
+      at += __popc(votes[j]);
     }
-    before += __shfl_sync(0xffffffffu, up, 31);
+    before += __shfl_sync(0xffffffffu, all, 31);
     __syncthreads();
   }
   if (threadIdx.x == 0) *count = before;
 }
 
-// dense[i] = h[rows[i]], and zeros up to the next multiple of kLpRowPad.  A warp has a row.
+// The same and the gathering of the rows in one launch, for at most kLpFewRows rows: a block has a row, and counts the labels before it itself.
+// The blocks behind the last row fill up with zeros.
+constexpr int kLpFewRows = 1024;
 __global__ void __launch_bounds__(256)
-log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int* count, bf16* dense, int D, int padded, int vec) {
+log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignore, int* rows, int* row_label, int* place, int* count, float* y,
+                          const bf16* h, long long ldh, bf16* dense, int D, int vec) {
+  __shared__ int sums[2][8];
   grid_dependency_enter();
-  const int n = *count, lane = threadIdx.x & 31, end = min((n + kLpRowPad - 1) / kLpRowPad * kLpRowPad, padded);
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < end; i += gridDim.x * 8) {
-    bf16* to = dense + (long long)i * D;
-    const bf16* from = i < n ? h + (long long)rows[i] * ldh : nullptr;
-    if (from == nullptr) {
-      for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(to + c) = make_uint4(0, 0, 0, 0);
-    } else if (vec) {
-      for (int c = lane * 8; c < D; c += 256) *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
-    } else {
-      for (int c = lane; c < D; c += 32) to[c] = from[c];
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int n = 0, before = 0;
+#pragma unroll
+  for (int j = 0; j < kLpFewRows / 256; ++j) {
+    const int i = j * 256 + threadIdx.x;
+    const bool one = i < T && lp_has_label(labels[i], V, ignore);
+    n += __popc(__ballot_sync(0xffffffffu, one));
+    before += __popc(__ballot_sync(0xffffffffu, one && i < t));
+  }
+  if (lane == 0) { sums[0][warp] = n; sums[1][warp] = before; }
+  __syncthreads();
+  n = before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) { n += sums[0][w]; before += sums[1][w]; }
+  const long long label = t < T ? labels[t] : -1;
+  const bool one = t < T && lp_has_label(label, V, ignore);
+  // a block without a labelled row of its own: row n + (which of those it is) of the dense array, if that is still in the last kLpBK
+  const int at = one ? before : n + (t - before);
+  if (threadIdx.x == 0) {
+    if (t == 0) *count = n;
+    if (t < T) {
+      place[t] = one ? at : -1;
+      if (one) { rows[at] = t; row_label[at] = (int)label; }
+      else y[t] = 0.f;
     }
+  }
+  if (!one && at >= (n + kLpBK - 1) / kLpBK * kLpBK) return;
+  const bf16* from = h + (long long)t * ldh;
+  for (int c = threadIdx.x * 8; c < D; c += 256 * 8) {
+    BF8 v{{0, 0, 0, 0}};
+    if (one) {
+      if (vec) v = *reinterpret_cast<const BF8*>(from + c);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[c + j];
+    }
+    *reinterpret_cast<BF8*>(dense + (long long)at * D + c) = v;
   }
 }
 
-// y and lse2 of a row from the log-sums of its columns: 8 rows to a block, 128 threads for each.
-constexpr int kLpSumRows = 8;
-__global__ void __launch_bounds__(1024)
-log_probs_sum_kernel(const float* stats, long long ld, int slots, const float* picked, const int* rows, const int* count, float* y, float* lse2) {
-  __shared__ float2 part[32][kLpSumRows];
+// dense[i] = h[rows[i]], and zeros up to the next multiple of kLpBK: those rows are part of dw's last products.
+__global__ void __launch_bounds__(256)
+log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int* count, bf16* dense, int D, int vec) {
   grid_dependency_enter();
-  const int n = *count, r = threadIdx.x % kLpSumRows, s0 = threadIdx.x / kLpSumRows, row = blockIdx.x * kLpSumRows + r;
-  if ((int)blockIdx.x * kLpSumRows >= n) return;
+  const int n = *count, end = (n + kLpBK - 1) / kLpBK * kLpBK, per_row = D / 8;
+  const long long all = (long long)end * per_row;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+    const int row = (int)(i / per_row), c = (int)(i - (long long)row * per_row) * 8;
+    BF8 v{{0, 0, 0, 0}};
+    if (row < n) {
+      const bf16* from = h + (long long)rows[row] * ldh + c;
+      if (vec) v = *reinterpret_cast<const BF8*>(from);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[j];
+    }
+    *reinterpret_cast<BF8*>(dense + i * 8) = v;
+  }
+}
+
+// y and lse2 of a row from the log-sums of its columns.  A block has kRows rows: 32 where that leaves enough blocks (a warp reads whole lines
+// then), else 8.  A thread takes kLpSumEach log-sums at a time: their maximum, then one exponential for each.
+constexpr int kLpSumEach = 8;
+template <int kRows>
+__global__ void __launch_bounds__(512)
+log_probs_sum_kernel(const float* stats, long long ld, int slots, const float* picked, const int* rows, const int* count, float* y, float* lse2,
+                     float* picked2) {
+  constexpr int kThreadsOfRow = 512 / kRows, kWarps = 16;
+  __shared__ float2 part[kWarps][kRows];
+  grid_dependency_enter();
+  const int n = *count, r = threadIdx.x % kRows, s0 = threadIdx.x / kRows, row = blockIdx.x * kRows + r;
+  if ((int)blockIdx.x * kRows >= n) return;
   float m = -INFINITY, s = 0.f;                                          // of 2^x
   if (row < n) {
-#pragma unroll 4
-    for (int i = s0; i < slots; i += 1024 / kLpSumRows) {
-      const float x = stats[(long long)i * ld + row];
-      const float top = fmaxf(m, x);
-      if (top > -INFINITY || x != x) {
-        s = s * exp2f(m == -INFINITY ? -INFINITY : m - top) + exp2f(x - top);
-        m = top;
-      }
+    for (int i = s0; i < slots; i += kThreadsOfRow * kLpSumEach) {
+      float x[kLpSumEach], top = m;
+#pragma unroll
+      for (int j = 0; j < kLpSumEach; ++j) x[j] = i + j * kThreadsOfRow < slots ? stats[(long long)(i + j * kThreadsOfRow) * ld + row] : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kLpSumEach; ++j) top = fmaxf(top, x[j]);
+      const float use = top == -INFINITY ? 0.f : top;
+      float t[2] = {s * fast_exp2(m - use), 0.f};                         // (0, before there is a maximum)
+#pragma unroll
+      for (int j = 0; j < kLpSumEach; ++j) t[j & 1] += fast_exp2(x[j] - use);
+      s = t[0] + t[1];
+      m = top;
     }
   }
   auto add = [](float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2);
-    const float a = m == -INFINITY ? s : s * exp2f(m - top), b = m2 == -INFINITY ? s2 : s2 * exp2f(m2 - top);      // (0, or what is no number)
+    const float a = m == -INFINITY ? s : s * fast_exp2(m - top), b = m2 == -INFINITY ? s2 : s2 * fast_exp2(m2 - top);      // (0, or what is no number)
     s = a + b;
     m = top;
   };
 #pragma unroll
-  for (int o = 16; o >= kLpSumRows; o >>= 1) add(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
-  if ((threadIdx.x & 31) < kLpSumRows) part[threadIdx.x >> 5][r] = make_float2(m, s);
+  for (int o = 16; o >= kRows; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    add(m, s, m2, s2);
+  }
+  if ((threadIdx.x & 31) < kRows) part[threadIdx.x >> 5][r] = make_float2(m, s);
   __syncthreads();
-  if (threadIdx.x < kLpSumRows && row < n) {
+  if (threadIdx.x < kRows && row < n) {
     m = part[0][r].x;
     s = part[0][r].y;
-    for (int w = 1; w < 32; ++w) add(m, s, part[w][r].x, part[w][r].y);
-    const float l = m + log2f(s);
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) add(m, s, part[w][r].x, part[w][r].y);
+    const float l = m + __log2f(s);
     lse2[row] = l;
+    picked2[row] = picked[row] - l;
     y[rows[row]] = (picked[row] - l) * 0.69314718056f;
   }
 }
 
-// dh[t] = the gathered gradient of row t in bf16, 0 without a label.  A warp has a row.
-__global__ void __launch_bounds__(256) log_probs_scatter_kernel(const float* dense, const int* place, bf16* dh, int T, int D) {
+// dx of the rows with a label from the kept logits, and zeros up to the next multiple of kLpBK.  A block has 8 rows and 1024 columns, a
+// warp one of the rows.
+constexpr int kLpDecodeCols = 1024;
+__global__ void __launch_bounds__(256)
+log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* tops, long long ld, const float* lse2, const float* picked2, const float* dy,
+                        const int* rows, const int* row_label, const int* count, bf16* dx, int V, float inv_tau, int col_blocks) {
   grid_dependency_enter();
-  const int lane = threadIdx.x & 31;
+  const int n = *count, lane = threadIdx.x & 31;
+  const long long row = blockIdx.x / col_blocks * 8LL + (threadIdx.x >> 5);
+  const int col0 = (int)(blockIdx.x % col_blocks) * kLpDecodeCols + lane * 8;
+  if (row >= (n + kLpBK - 1) / kLpBK * kLpBK) return;
+  const bool live = row < n;
+  const float g = live ? dy[rows[row]] * inv_tau : 0.f, lse = live ? lse2[row] : 0.f;
+  const int label = live ? row_label[row] : -1;
+  uint4 v[4];
+  float top[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = col0 + k * 256;
+    v[k] = make_uint4(0, 0, 0, 0);
+    top[k] = -INFINITY;
+    if (live && c < V) {                                                 // (the pitch is a multiple of 8)
+      v[k] = *reinterpret_cast<const uint4*>(codes + row * pitch + c);
+      top[k] = tops[(long long)(c / kLpStatCols) * ld + row];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int c = col0 + k * 256;
+    if (c >= V) break;
+    const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+    const float off = top[k] - lse;
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float code = __uint_as_float(0x4b000000u | (j & 1 ? u[j >> 1] >> 16 : u[j >> 1] & 0xffffu)) - 8388608.f;
+      d[j] = -g * fast_exp2(fmaf(code, -1.f / kLpCodes, off));
+      if (c + j == label) d[j] = g * (1.f - fast_exp2(picked2[row]));    // (of the exact logit: next to a probability of one its rounding would be all of it)
+      if (!live) d[j] = 0.f;
+    }
+    store8(dx + row * pitch + c, d);
+  }
+}
+
+// dh[t] = the gathered gradient of row t in bf16, its parts added up, and 0 without a label.  A warp has a row.
+__global__ void __launch_bounds__(256)
+log_probs_scatter_kernel(const float* dense, const int* place, const int* count, bf16* dh, int T, int D, int num_kb, int n_pairs, int planes, long long plane) {
+  grid_dependency_enter();
+  const int lane = threadIdx.x & 31, tiles = (min(*count, T) + 2 * kLpBM - 1) / (2 * kLpBM) * ((D + kLpBN - 1) / kLpBN);
+  const int parts = tiles > 0 ? lp_parts(tiles, num_kb, n_pairs, planes) : 0;
   for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += gridDim.x * 8) {
     const int i = place[t];
     for (int c = lane * 8; c < D; c += 256) {
       float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (i >= 0) {
-        const float4 u = *reinterpret_cast<const float4*>(dense + (long long)i * D + c), v = *reinterpret_cast<const float4*>(dense + (long long)i * D + c + 4);
-        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w; f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+        const float* from = dense + (long long)i * D + c;
+#pragma unroll 4
+        for (int p = 0; p < parts; ++p, from += plane) {
+          const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
+          f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w; f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+        }
       }
       store8(dh + (long long)t * D + c, f);
     }
@@ -449,6 +622,13 @@ static int lp_map(CUtensorMap* m, const void* base, int elem, long long cols, lo
   return make_tmap(m, base, elem, 2, dims, str, box, true);
 }
 
+// CTA pairs of a launch (where fewer rows have a label than there are, the last ones may stay idle)
+static int lp_pairs(long long tiles, int planes, int sms) {
+  const long long units = tiles * (planes > 2 ? planes : 2);
+  return (int)(units < sms / 2 ? units : sms / 2);
+}
+static long long lp_tiles(int M, int N) { return (long long)((M + 2 * kLpBM - 1) / (2 * kLpBM)) * ((N + kLpBN - 1) / kLpBN); }
+
 template <int kMode>
 static int launch_log_probs(const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, LpArgs a, cudaStream_t st) {
   const int sms = sm_count();
@@ -458,9 +638,9 @@ static int launch_log_probs(const CUtensorMap& A, const CUtensorMap& B, const CU
   auto kern = log_probs_pair_kernel<kMode>;
   static PerDevice raised;
   KSA_CHECK_CUDA(raise_smem_limit(raised, kern, kLpSmem));
-  const long long tiles = (long long)((a.M + 2 * kLpBM - 1) / (2 * kLpBM)) * ((a.N + kLpBN - 1) / kLpBN);
-  KSA_REQUIRE(tiles < (1 << 30), "log_probs: %lld tiles", tiles);
-  const int pairs = (int)(2 * tiles < sms / 2 ? 2 * tiles : sms / 2);     // (fewer rows than all may leave the last ones idle)
+  const long long tiles = lp_tiles(a.M, a.N);
+  KSA_REQUIRE(tiles < (1 << 27), "log_probs: %lld tiles", tiles);
+  const int pairs = lp_pairs(tiles, a.planes, sms);
   KSA_CHECK_CUDA(launch_kernel(kern, dim3(2 * pairs), dim3(kLpThreads), (size_t)kLpSmem, st, A, B, C, a));
   return 0;
 }
@@ -471,10 +651,12 @@ using namespace ksa;
 #define ST(s) reinterpret_cast<cudaStream_t>(s)
 
 // Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
-// Leaves what the backward pass needs: dense [T rounded up to 256, D] bf16, rows, row_label, place [T], count [1] int32, lse2 [T].
+// Leaves what the backward pass needs: dense [T rounded up to 256, D] bf16, rows, row_label, place [T], count [1] int32, lse2 [2 T] (the log-sums
+// and the labels' logits less those, base 2), and where codes is not null the logits in 16 bits, codes [T rounded up to 256, V rounded up to 8]
+// with tops, fp32 [ceil(V / 128) times T rounded up to 4].
 // work: fp32 [T rounded up to 4 times (ceil(V / 128) + 1)].  y [T] fp32.
 KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
-                          void* lse2, void* work, void* y, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
+                          void* lse2, void* work, void* y, void* codes, void* tops, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
                           void* stream) {
   KSA_ENTER(w);
   KSA_REQUIRE(T > 0 && V > 0 && D > 0, "log_probs: empty problem %d x %d x %d", T, V, D);
@@ -486,37 +668,50 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   const long long ld = (T + 3LL) / 4 * 4;
   float* stats = static_cast<float*>(work);
   float* picked = stats + ld * slots;
-  KSA_CHECK_CUDA(launch_kernel(log_probs_select_kernel, dim3(1), dim3(kLpSelect), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
-                               (int*)row_label, (int*)place, (int*)count, (float*)y));
   const int vec = ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
-  const int gather_blocks = padded / 8 < 148 * 8 ? padded / 8 : 148 * 8;
-  KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh, (const int*)rows,
-                                      (const int*)count, (bf16*)dense, D, padded, vec));
+  if (T <= kLpFewRows) {
+    KSA_CHECK_CUDA(launch_kernel(log_probs_few_rows_kernel, dim3(T + kLpBK - 1), dim3(256), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
+                                 (int*)row_label, (int*)place, (int*)count, (float*)y, (const bf16*)h, ldh, (bf16*)dense, D, vec));
+  } else {
+    KSA_CHECK_CUDA(launch_kernel(log_probs_select_kernel, dim3(1), dim3(kLpSelect), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
+                                 (int*)row_label, (int*)place, (int*)count, (float*)y));
+    const long long vectors = (T + 63LL) / 64 * 64 * (D / 8);
+    const int gather_blocks = (int)(vectors < 256 * 148 * 8 ? (vectors + 255) / 256 : 148 * 8);
+    KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh,
+                                        (const int*)rows, (const int*)count, (bf16*)dense, D, vec));
+  }
   CUtensorMap A, B;
   int rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
   if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
+  CUtensorMap C = A;
+  if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, (V + 7LL) / 8 * 8, 32);
   if (rc) return rc;
   LpArgs a{};
   a.M = T; a.N = V; a.K = D;
   a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
   a.scale2 = (float)(1.4426950408889634 / (double)tau);
-  a.stats = stats; a.picked = picked; a.ld_stats = ld;
-  rc = launch_log_probs<kStats>(A, B, A, a, st);
+  a.stats = stats; a.picked = picked; a.ld_stats = ld; a.tops = static_cast<float*>(tops);
+  rc = codes ? launch_log_probs<kStatsKeep>(A, B, C, a, st) : launch_log_probs<kStats>(A, B, C, a, st);
   if (rc) return rc;
-  KSA_CHECK_CUDA(launch_kernel(log_probs_sum_kernel, dim3((T + kLpSumRows - 1) / kLpSumRows), dim3(1024), 0, st, (const float*)stats, ld, slots,
-                               (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2));
+  const bool wide = T >= 32 * 148;
+  KSA_CHECK_CUDA(launch_kernel(wide ? log_probs_sum_kernel<32> : log_probs_sum_kernel<8>, dim3(wide ? (T + 31) / 32 : (T + 7) / 8), dim3(512), 0, st,
+                               (const float*)stats, ld, slots, (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2,
+                               (float*)lse2 + T));
   return 0;
 }
 
 // Backward.  dy [T] fp32; dh [T, D] bf16 or null; dw [V, D] (row pitch lddw) or null, bf16 or (dw_fp32) fp32, there with add_dw added to.
-// dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8); dh32: fp32 [T rounded up to 256, D] where dh is wanted.
+// dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8; with codes: V rounded up to 8).
+// dh32: fp32 [planes, T rounded up to 256, D] where dh is wanted, 1 to 8 planes, only one where not all columns are taken at a time.
 KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
-                              const void* lse2, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
-                              long long lddw, int dw_fp32, int add_dw, int slab, float tau, void* stream) {
+                              const void* lse2, const void* codes, const void* tops, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
+                              long long lddw, int dw_fp32, int add_dw, int slab, int planes, float tau, void* stream) {
   KSA_ENTER(w);
   KSA_REQUIRE(T > 0 && V > 0 && D > 0 && D % 8 == 0 && ldw % 8 == 0, "log_probs: backward of %d x %d x %d", T, V, D);
   KSA_REQUIRE(!dw || lddw % (dw_fp32 ? 4 : 8) == 0, "log_probs: the pitch %lld of the weights' gradient keeps no alignment of 16 bytes", lddw);
   KSA_REQUIRE(slab > 0 && slab % 8 == 0, "log_probs: %d columns at a time (a multiple of 8)", slab);
+  KSA_REQUIRE(planes >= 1 && planes <= 8 && (planes == 1 || slab >= V), "log_probs: %d planes", planes);
+  KSA_REQUIRE(!codes || (tops && slab == (V + 7) / 8 * 8), "log_probs: kept logits are taken all at a time");
   KSA_REQUIRE(!(add_dw && !dw_fp32), "log_probs: only an fp32 gradient is added to");
   KSA_REQUIRE(!dh || (reinterpret_cast<uintptr_t>(dh) & 15) == 0, "log_probs: the gradient of the rows must be 16-byte aligned");
   cudaStream_t st = ST(stream);
@@ -533,18 +728,27 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     a.scale2 = (float)(1.4426950408889634 / (double)tau); a.inv_tau = 1.f / tau;
     a.lse2 = static_cast<const float*>(lse2); a.dy = static_cast<const float*>(dy); a.col0 = (int)v0;
     a.M = T; a.N = n; a.K = D;
-    rc = lp_map(&wK, wv, 2, D, n, ldw, 64);
-    if (rc == 0) rc = lp_map(&dxOut, dx, 2, n, padded, slab, 32);
-    if (rc == 0) rc = launch_log_probs<kGrad>(denseK, wK, dxOut, a, st);
+    if (codes) {
+      const int col_blocks = (V + kLpDecodeCols - 1) / kLpDecodeCols;
+      const long long blocks = (T + 63LL) / 64 * 8 * col_blocks;
+      KSA_REQUIRE(blocks < (1LL << 31), "log_probs: %d x %d kept logits", T, V);
+      KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * V, log_probs_decode_kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const uint16_t*)codes,
+                                          (long long)slab, (const float*)tops, (T + 3LL) / 4 * 4, a.lse2, a.lse2 + T, a.dy, a.rows, a.row_label, a.count,
+                                          (bf16*)dx, V, a.inv_tau, col_blocks));
+    } else {
+      rc = lp_map(&wK, wv, 2, D, n, ldw, 64);
+      if (rc == 0) rc = lp_map(&dxOut, dx, 2, n, padded, slab, 32);
+      if (rc == 0) rc = launch_log_probs<kGrad>(denseK, wK, dxOut, a, st);
+    }
     if (rc == 0 && dh) {
-      a.M = T; a.N = D; a.K = n; a.add = v0 > 0;
+      a.M = T; a.N = D; a.K = n; a.add = v0 > 0; a.planes = planes; a.plane_rows = padded;
       rc = lp_map(&dxK, dx, 2, n, padded, slab, kLpBM);
       if (rc == 0) rc = lp_map(&wM, wv, 2, D, n, ldw, 64);
-      if (rc == 0) rc = lp_map(&out, dh32, 4, D, padded, D, 32);
+      if (rc == 0) rc = lp_map(&out, dh32, 4, D, (long long)planes * padded, D, 32);
       if (rc == 0) rc = launch_log_probs<kDh>(dxK, wM, out, a, st);
     }
     if (rc == 0 && dw) {
-      a.M = n; a.N = D; a.K = T; a.add = add_dw; a.bf16_out = !dw_fp32;
+      a.M = n; a.N = D; a.K = T; a.planes = 1; a.add = add_dw; a.bf16_out = !dw_fp32;
       rc = lp_map(&dxM, dx, 2, n, padded, slab, 64);
       if (rc == 0) rc = dw_fp32 ? lp_map(&out, static_cast<float*>(dw) + v0 * lddw, 4, D, n, lddw, 32) : lp_map(&out, static_cast<bf16*>(dw) + v0 * lddw, 2, D, n, lddw, 32);
       if (rc == 0) rc = launch_log_probs<kDw>(dxM, denseM, out, a, st);
@@ -554,7 +758,8 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
   if (dh) {
     const int blocks = (T + 7) / 8 < 148 * 8 ? (T + 7) / 8 : 148 * 8;
     KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, log_probs_scatter_kernel, dim3(blocks), dim3(256), 0, st, (const float*)dh32, (const int*)place,
-                                        (bf16*)dh, T, D));
+                                        (const int*)count, (bf16*)dh, T, D, (int)(((V < slab ? V : slab) + kLpBK - 1) / kLpBK), lp_pairs(lp_tiles(T, D), planes, sm_count()), planes,
+                                        (long long)padded * D));
   }
   return 0;
 }

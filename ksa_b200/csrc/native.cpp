@@ -114,11 +114,11 @@ int ksa_preference_loss(const void* y, const void* ref, const void* mask, const 
 int ksa_preference_loss_bwd(const void* mask, const void* coef, const void* dloss, void* dy, int type, const void* cu, int wide, long long n,
                             int sequences, long long length, void* stream);
 int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
-                  void* lse2, void* work, void* y, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
+                  void* lse2, void* work, void* y, void* codes, void* tops, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
                   void* stream);
 int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
-                      const void* lse2, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
-                      long long lddw, int dw_fp32, int add_dw, int slab, float tau, void* stream);
+                      const void* lse2, const void* codes, const void* tops, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
+                      long long lddw, int dw_fp32, int add_dw, int slab, int planes, float tau, void* stream);
 }
 
 namespace {
@@ -1121,59 +1121,73 @@ PyObject* py_preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
 
 struct LogProbsCall {
   const Tensor* labels = nullptr;
-  long long ignore = 0, pad = 0, columns = 0, slab_bytes = 0;
+  long long ignore = 0, pad = 0, columns = 0, slab_bytes = 0, plane_bytes = 0;
   float tau = 1;
 };
 struct LogProbsKept {
-  Tensor y, dense, ints, lse2;             // ints: rows, row_label, place, count
+  Tensor y, dense, ints, lse2, codes, tops;         // ints: rows, row_label, place, count
 };
-LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c) {
+// Columns of the vocabulary that the backward pass takes at a time (_slab in ops/log_probs.py).
+long long slab_of(long long padded, long long V, long long bytes) {
+  return std::min((V + 7) / 8 * 8, std::max(256ll, bytes / (2 * padded) / 256 * 256));
+}
+LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, bool grad) {
   const long long T = c.labels->numel(), V = w.size(0), D = w.size(1), padded = (T + c.pad - 1) / c.pad * c.pad;
   LogProbsKept k;
   k.y = at::empty(c.labels->sizes(), on(h, at::kFloat));
   k.dense = at::empty({(int64_t)padded, (int64_t)D}, on(h, at::kBFloat16));
   k.ints = at::empty({(int64_t)(3 * T + 1)}, on(h, at::kInt));
-  k.lse2 = at::empty({(int64_t)T}, on(h, at::kFloat));
+  k.lse2 = at::empty({(int64_t)(2 * T)}, on(h, at::kFloat));
+  const long long slab = slab_of(padded, V, c.slab_bytes);
+  const bool keep = grad && slab >= V;
+  if (keep) {
+    k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
+    k.tops = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns))}, on(h, at::kFloat));
+  }
   const Tensor work = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns + 1))}, on(h, at::kFloat));
   int* ints = static_cast<int*>(k.ints.mutable_data_ptr());
   LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), ints, ints + T, ints + 2 * T,
-                 ints + 3 * T, k.lse2.mutable_data_ptr(), work.mutable_data_ptr(), k.y.mutable_data_ptr(), (int)T, (int)V, (int)D,
+                 ints + 3 * T, k.lse2.mutable_data_ptr(), work.mutable_data_ptr(), k.y.mutable_data_ptr(), keep ? k.codes.mutable_data_ptr() : nullptr,
+                 keep ? k.tops.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D,
                  h.dim() == 2 ? h.stride(0) : D, w.stride(0), c.ignore, c.tau, stream_of(h));
   return k;
 }
 struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const LogProbsCall* call) {
-    const LogProbsKept k = log_probs(h, w, *call);
-    ctx->save_for_backward({k.dense, w, k.ints, k.lse2});
+    const LogProbsKept k = log_probs(h, w, *call, true);
+    ctx->save_for_backward({k.dense, w, k.ints, k.lse2, k.codes, k.tops});
     ctx->saved_data["shape"] = h.sizes().vec();
     ctx->saved_data["tau"] = (double)call->tau;
     ctx->saved_data["slab_bytes"] = (int64_t)call->slab_bytes;
+    ctx->saved_data["plane_bytes"] = (int64_t)call->plane_bytes;
     return k.y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &dense = saved[0], &w = saved[1], &ints = saved[2], &lse2 = saved[3];
-    const long long T = lse2.numel(), V = w.size(0), D = w.size(1), padded = dense.size(0);
+    const Tensor &dense = saved[0], &w = saved[1], &ints = saved[2], &lse2 = saved[3], &codes = saved[4], &tops = saved[5];
+    const long long T = lse2.numel() / 2, V = w.size(0), D = w.size(1), padded = dense.size(0);
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     const Tensor dy = grads[0].contiguous();
-    const long long slab = std::min((V + 7) / 8 * 8, std::max(256ll, ctx->saved_data["slab_bytes"].toInt() / (2 * padded) / 256 * 256));
+    const long long slab = codes.defined() ? codes.size(1) : slab_of(padded, V, ctx->saved_data["slab_bytes"].toInt());
     const Tensor dx = at::empty({(int64_t)padded, (int64_t)slab}, on(w, at::kBFloat16));
     Tensor dh, dh32, dw;
+    const long long planes = slab < V ? 1 : std::max(1ll, std::min(8ll, (long long)ctx->saved_data["plane_bytes"].toInt() / (4 * padded * D)));
     if (need_h) {
       dh = at::empty(ctx->saved_data["shape"].toIntVector(), on(w, at::kBFloat16));
-      dh32 = at::empty({(int64_t)padded, (int64_t)D}, on(w, at::kFloat));
+      dh32 = at::empty({(int64_t)planes, (int64_t)padded, (int64_t)D}, on(w, at::kFloat));
     }
     if (need_w) dw = at::empty({(int64_t)V, (int64_t)D}, on(w, at::kBFloat16));
     const int* p = static_cast<const int*>(ints.const_data_ptr());
-    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, lse2.const_data_ptr(), dy.const_data_ptr(),
+    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, lse2.const_data_ptr(), codes.defined() ? codes.const_data_ptr() : nullptr,
+                   codes.defined() ? tops.const_data_ptr() : nullptr, dy.const_data_ptr(),
                    dx.mutable_data_ptr(), need_h ? dh32.mutable_data_ptr() : nullptr, need_h ? dh.mutable_data_ptr() : nullptr,
-                   need_w ? dw.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D, w.stride(0), D, 0, 0, (int)slab, (float)ctx->saved_data["tau"].toDouble(),
+                   need_w ? dw.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D, w.stride(0), D, 0, 0, (int)slab, need_h ? (int)planes : 1, (float)ctx->saved_data["tau"].toDouble(),
                    stream_of(w));
     return {differentiated_once(dh), differentiated_once(dw), Tensor()};
   }
 };
 
-// linear_log_probs(h [..., D], w, labels [...], ignore_index, temperature, row pad, columns of a sum, slab bytes) -> y [...]
+// linear_log_probs(h [..., D], w, labels [...], ignore_index, temperature, row pad, columns of a sum, slab bytes, plane bytes) -> y [...]
 PyObject* py_linear_log_probs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(v, n);
@@ -1187,20 +1201,21 @@ PyObject* py_linear_log_probs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   c.tau = a.real();
   c.pad = a.integer();
   c.columns = a.integer();
-  PyObject* bytes = a.next();
-  c.slab_bytes = PyLong_Check(bytes) ? PyLong_AsLongLong(bytes) : -1;
+  PyObject *slab = a.next(), *planes = a.next();
+  c.slab_bytes = PyLong_Check(slab) ? PyLong_AsLongLong(slab) : -1;
+  c.plane_bytes = PyLong_Check(planes) ? PyLong_AsLongLong(planes) : -1;
   if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
   if (!a.ok() || !a.dense(w) || w.scalar_type() != at::kBFloat16 || !rows2d(&w) || !aligned(&w) || w.size(1) % 8 != 0 || w.stride(0) % 8 != 0 ||
       w.stride(0) < w.size(1) || h->dim() < 1 || h->size(-1) != w.size(1) || c.labels->sizes() != h->sizes().slice(0, h->dim() - 1) ||
       !(h->is_contiguous() || rows2d(h)) || !c.labels->is_contiguous() || !fits(w.size(0)) || c.labels->numel() > INT_MAX / 4 || !(c.tau > 0 && std::isfinite(c.tau)) ||
-      c.pad <= 0 || c.columns <= 0 || c.slab_bytes < 0)
+      c.pad <= 0 || c.columns <= 0 || c.slab_bytes < 0 || c.plane_bytes < 0)
     return none();
   const bool grad = wants_gradient(*h) || wants_gradient(w);
   if (grad && PyObject_HasAttrString(weight, "main_grad")) return none();                  // its gradient goes to a buffer that Python knows
   Tensor y;
   {
     pybind11::gil_scoped_release no_gil;
-    y = grad ? LogProbsNode::apply(*h, w, &c) : log_probs(*h, w, c).y;
+    y = grad ? LogProbsNode::apply(*h, w, &c) : log_probs(*h, w, c, false).y;
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS

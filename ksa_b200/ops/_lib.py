@@ -73,8 +73,8 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_int4_weight_values": [P, P, P, I, I, I, I, P],
     "ksa_int4_norm_linear": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P],
     "ksa_int4_linear": [P, P, P, P, I, I, I, I, I, L, L, I, P],
-    "ksa_log_probs": [P] * 11 + [I] * 3 + [L] * 3 + [F, P],
-    "ksa_log_probs_bwd": [P] * 12 + [I] * 3 + [L] * 2 + [I] * 3 + [F, P],
+    "ksa_log_probs": [P] * 13 + [I] * 3 + [L] * 3 + [F, P],
+    "ksa_log_probs_bwd": [P] * 14 + [I] * 3 + [L] * 2 + [I] * 4 + [F, P],
     "ksa_policy_loss": [P, P, P, P, P, P, I, P, P, P, P, P, I, L, I, L, I, I, P, F, P],
     "ksa_policy_loss_bwd": [P, P, P, P, I, P, I, L, I, L, I, P],
     "ksa_preference_loss": [P, P, P, P, I, P, P, P, P, I, L, I, L, F, F, P],

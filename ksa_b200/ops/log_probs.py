@@ -14,7 +14,15 @@ from .token_losses import _Forward
 
 _ROW_PAD = 256              # rows of the gathered arrays: a multiple of this (kLpRowPad in csrc/log_probs.cu)
 _STAT_COLS = 128            # columns that share a log-sum (kLpStatCols)
-SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16) of so many bytes at a time, or of 256 columns
+SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16) of so many bytes at a time, or of 256 columns;
+                            # where that is all of it, the forward pass keeps the logits in as many bytes
+
+
+PLANE_BYTES = 512 << 20     # and cuts the vocabulary of the rows' gradient into as many parts (at most 8) as have fp32 results of so many bytes
+
+
+def _planes(padded: int, D: int) -> int:
+    return max(1, min(8, PLANE_BYTES // (4 * padded * D)))
 
 
 def _slab(padded: int, V: int) -> int:
@@ -34,34 +42,39 @@ class _LinearLogProbsFn(torch.autograd.Function):
             dense = torch.empty((padded, D), dtype=h.dtype, device=dev)
             rows, row_label, place = torch.empty((3, T), dtype=torch.int32, device=dev).unbind()
             count = torch.empty(1, dtype=torch.int32, device=dev)
-            lse2 = torch.empty(T, dtype=torch.float32, device=dev)
+            lse2 = torch.empty(2 * T, dtype=torch.float32, device=dev)
+            codes = tops = None
+            if any(ctx.needs_input_grad[:2]) and _slab(padded, V) >= V:
+                codes = torch.empty((padded, _slab(padded, V)), dtype=torch.int16, device=dev)
+                tops = torch.empty(-(-T // 4) * 4 * -(-V // _STAT_COLS), dtype=torch.float32, device=dev)
             work = torch.empty(-(-T // 4) * 4 * (-(-V // _STAT_COLS) + 1), dtype=torch.float32, device=dev)
             weight = _pitched(w)
-            _lib.call("ksa_log_probs", h, weight, labels, dense, rows, row_label, place, count, lse2, work, y, T, V, D, h.stride(0),
+            _lib.call("ksa_log_probs", h, weight, labels, dense, rows, row_label, place, count, lse2, work, y, codes, tops, T, V, D, h.stride(0),
                       weight.stride(0), ignore_index, float(temperature))
-        ctx.save_for_backward(dense, w, rows, row_label, place, count, lse2)
+        ctx.save_for_backward(dense, w, rows, row_label, place, count, lse2, codes, tops)
         ctx.temperature = temperature
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        dense, w, rows, row_label, place, count, lse2 = ctx.saved_tensors
+        dense, w, rows, row_label, place, count, lse2, codes, tops = ctx.saved_tensors
         T, (V, D), dev = rows.shape[0], w.shape, w.device
         need_h, need_w = ctx.needs_input_grad[:2]
         dh = dw = dh32 = None
         with torch.cuda.device(dev):
             dy = dy.to(torch.float32).contiguous()
             weight = _pitched(w)
-            dx = torch.empty((dense.shape[0], _slab(dense.shape[0], V)), dtype=w.dtype, device=dev)
+            dx = torch.empty((dense.shape[0], codes.shape[1] if codes is not None else _slab(dense.shape[0], V)), dtype=w.dtype, device=dev)
             if need_h:
                 dh = torch.empty((T, D), dtype=w.dtype, device=dev)
-                dh32 = torch.empty(dense.shape, dtype=torch.float32, device=dev)
+                planes = _planes(*dense.shape) if dx.shape[1] >= V else 1
+                dh32 = torch.empty((planes, *dense.shape), dtype=torch.float32, device=dev)
 
             def run(out, add):
-                _lib.call("ksa_log_probs_bwd", dense, weight, rows, row_label, place, count, lse2, dy, dx, dh32, dh, out, T, V, D,
+                _lib.call("ksa_log_probs_bwd", dense, weight, rows, row_label, place, count, lse2, codes, tops, dy, dx, dh32, dh, out, T, V, D,
                           weight.stride(0), out.stride(0) if out is not None else D, int(out is not None and out.dtype == torch.float32),
-                          int(add), dx.shape[1], float(ctx.temperature))
+                          int(add), dx.shape[1], 1 if dh32 is None else dh32.shape[0], float(ctx.temperature))
 
             if not need_w:
                 run(None, False)
@@ -89,11 +102,12 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     row of ``weight``.
 
     ``hidden`` is ``[..., D]``, ``weight`` the output head ``[V, D]`` (both bf16 on a GPU, ``D`` a multiple of 8), ``labels`` ``[...]``.  Rows
-    without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  The logits are never in
-    memory: the forward pass keeps what its tiles' sums need, the backward pass computes them again, at most 4 GB of their gradient at a time.
+    without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  Without a
+    gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where that takes at most ``SLAB_BYTES`` (4 GB: 13824 rows of
+    151936 tokens); of more the backward pass computes them again, at most 4 GB of their gradient at a time.
     With ``main_grad`` on the weight its gradient goes there."""
     if not _observed():
-        y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES)
+        y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES, PLANE_BYTES)
         if y is not None:
             return y
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

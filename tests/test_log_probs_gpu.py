@@ -3,8 +3,8 @@
 Tolerances, by arithmetic.  A logit is a sum of ``D`` products in the tensor cores' 32-bit accumulators: 16 products at a time, each
 step off by at most 2^-22 of the sum of magnitudes ``S`` (a bit less than fp32 for what is aligned and cut off), so ``ex = (D / 16 + 2)
 2^-22 S / tau``.  ``y`` is the difference of a logit and a log-sum that is off by no more than the logits are, both rounded a few times in base 2:
-``2 ex + 8 2^-22 (1 + |x| + |lse|)``.  The logits' gradient is off by ``2 ex + 2^-18`` of itself by the exponential's argument and function, and
-is rounded to bf16 (2^-8); the products with it add ``(n / 16 + 2) 2^-22`` of the sum of magnitudes, and the results are rounded to bf16 unless
+``2 ex + 8 2^-22 (1 + |x| + |lse|)``.  Probabilities are off by ``2 ex + 2^-18`` of themselves by the exponential's argument and function, and
+by ln 2 times half a step of 2^-10, 2^-11.5, where they come from kept logits; the logits' gradient is rounded to bf16 (2^-8); the products with it add ``(n / 16 + 2) 2^-22`` of the sum of magnitudes, and the results are rounded to bf16 unless
 they go into an fp32 buffer.
 """
 import math
@@ -43,7 +43,7 @@ def _oracle(h, w, labels, dy, tau):
     dx = -p
     dx[i, at] += 1
     dx *= dy[:, None] / tau
-    off = (p * (2 * ex + 2.0 ** -18)[:, None] * dy.abs()[:, None] / tau) * (1 + 2.0 ** -8) + 2.0 ** -8 * dx.abs() + 2.0 ** -130
+    off = (p * (2 * ex + 2.0 ** -18 + 2.0 ** -11.5)[:, None] * dy.abs()[:, None] / tau) * (1 + 2.0 ** -8) + 2.0 ** -8 * dx.abs() + 2.0 ** -130
     out = {}
     full = lambda v: torch.zeros(T, *v.shape[1:], dtype=torch.float64, device=h.device).index_copy_(0, rows, v)  # noqa: E731
     out["y"] = full(yr), full(2 * ex + 8 * 2.0 ** -22 * (1 + x[i, at].abs() + lse.abs()))
@@ -119,6 +119,29 @@ def test_a_bad_row_spoils_itself_and_the_weights_gradient_alone():
     rest = torch.arange(40, device="cuda") != 7
     assert torch.isnan(y[7]) and torch.isnan(dh[7]).all() and torch.isnan(dw).any()
     assert torch.equal(y[rest], good[0][rest]) and torch.equal(dh[rest], good[1][rest])
+
+
+def test_tokens_of_probability_one():
+    """1 - p of a label that has nearly all of it comes from the exact logit: kept in 16 bits it would be lost."""
+    h, w, labels, dy = _inputs(96, 128, 500, 1.0, seed=15)
+    h = (h.float() * 0.05 + w[labels].float() * torch.linspace(20, 60, 96, device="cuda")[:, None]).bfloat16()
+    x = h.double() @ w.double().T
+    gap = 1 - (x - x.logsumexp(1, keepdim=True)).exp().gather(1, labels[:, None])[:, 0]
+    assert gap.min() < 1e-4 and (gap > 1e-6).any()
+    got = _run(h, w, labels, dy, 1.0)
+    for name, g in zip(("y", "dh", "dw"), got):
+        _close(g, _oracle(h, w, labels, dy, 1.0)[name], name)
+
+
+def test_logits_far_below_the_maximum():
+    """Columns more than 64 powers of two below the largest of their 128 count as nothing, and those of other columns keep their own scale."""
+    h, w, labels, dy = _inputs(40, 64, 600, 1.0, seed=16)
+    h = (h.float() * 6).bfloat16()
+    want = _oracle(h, w, labels, dy, 1.0)
+    x = h.double() @ w.double().T
+    assert (x.amax(1) - x.amin(1)).min() > 64 * math.log(2)
+    for name, g in zip(("y", "dh", "dw"), _run(h, w, labels, dy, 1.0)):
+        _close(g, want[name], name)
 
 
 def test_large_logits():
@@ -206,16 +229,33 @@ def test_slabs_of_the_vocabulary(V, monkeypatch):
     h, w, labels, dy = _inputs(300, 136, V, 0.8, seed=10)
     want = _oracle(h, w, labels, dy, 1.0)
     whole = _run(h, w, labels, dy, 1.0)
+    for name, got in zip(("y", "dh", "dw"), whole):
+        _close(got, want[name], name)
     monkeypatch.setattr(impl, "SLAB_BYTES", 2 * 512 * 256)
     assert impl._slab(512, V) == 256
     y, dh, dw = _run(h, w, labels, dy, 1.0)
-    assert torch.equal(y, whole[0]) and torch.equal(dw, whole[2])
+    assert torch.equal(y, whole[0])
     _close(dh, want["dh"], "dh")
+    _close(dw, want["dw"], "dw")
+    bad = torch.where(labels[:, None] == IGNORE, torch.full_like(h, float("nan")), h)
+    assert all(torch.equal(a, b) for a, b in zip(_run(bad, w, labels, dy, 1.0), (y, dh, dw)))
     p = torch.nn.Parameter(w)
     p.main_grad = torch.ones(w.shape, device="cuda")
     p._grad_written = True
     ops.linear_log_probs(h, p, labels).backward(dy)
     _close(p.main_grad - 1, (want["dw"][0], want["dw"][1] + 2.0 ** -23 * (1 + want["dw"][0].abs())), "added to")
+
+
+@pytest.mark.parametrize("T,D,V", [(300, 136, 1000), (256, 64, 33000), (77, 256, 4096), (700, 512, 20000)])
+def test_parts_of_the_vocabulary(T, D, V, monkeypatch):
+    """dh in several parts, added up in order, against the same in one."""
+    h, w, labels, dy = _inputs(T, D, V, 0.8, seed=17)
+    want = _oracle(h, w, labels, dy, 1.0)
+    one = _run(h, w, labels, dy, 1.0)
+    monkeypatch.setattr(impl, "PLANE_BYTES", 0)
+    for got in (one, _run(h, w, labels, dy, 1.0)):
+        for name, g in zip(("y", "dh", "dw"), got):
+            _close(g, want[name], name)
 
 
 def test_gradients_against_differences():
