@@ -378,6 +378,172 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   }
 }
 
+// The log-sums of a few rows without a backward pass.  Bound: the weights' bytes.  The kernel above would multiply 256 rows, most of them padding, and the
+// tensor cores' share of the power then slows the memory down (one row of 2560 against 151936 tokens 134 us by itself, 167 to 183 in a row of calls).
+// Here the weights are the 128 rows of the tensor cores' product and the activations, N of them, its columns.  Every CTA has as many weight rows
+// as the others, in steps of 8: tiles of 256 and a shorter last one, the end of which is loaded 8 rows at a time.
+// Epilogue: a thread has one weight row and N values; a warp adds up its 32 rows for every activation by exchanging halves, after which a
+// lane has one activation's maximum (or sum), and keeps it over its tiles.  A warp writes one log-sum for each activation.
+constexpr int kLfThreads = 192;      // warp 0 loads, warp 1 issues products, warps 2..5 epilogue
+constexpr int kLfTile = 256;         // weight rows that share a load of the activations: two products of 128 rows
+constexpr int kLfMostRows = 128;
+template <int N>
+struct LfShape {
+  static constexpr int stage_bytes = kLfTile * kLpBK * 2 + N * kLpBK * 2;
+  static constexpr int stages = 200 * 1024 / stage_bytes;
+  static constexpr int smem = stages * stage_bytes + 512 + N * 4 + 1024;
+};
+
+template <int N>
+__global__ void __launch_bounds__(kLfThreads, 1)
+log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW8, const __grid_constant__ CUtensorMap tmH, int V,
+                     int D, int rows_of_cta, const int* count, const int* row_label, float scale2, float* stats, long long ld, float* picked, int* status) {
+  using S = LfShape<N>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::stages * S::stage_bytes);
+  uint64_t* empty = full + S::stages;
+  uint64_t* acc_full = empty + S::stages;      // 2 buffers
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* label = reinterpret_cast<int*>(smem + S::stages * S::stage_bytes + 512);
+  static_assert((2 * S::stages + 4) * 8 + 8 <= 512, "barriers");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WaitGuard guard{abort_flag, status};
+  constexpr int kCols = 4 * N <= 128 ? 128 : 4 * N <= 256 ? 256 : 512;   // two buffers of two accumulators
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmH);
+  }
+  if (warp == 2) { tmem_alloc(tmem_slot, kCols); tmem_relinquish(); }
+  grid_dependency_enter();
+  const int n = min(*count, N);
+  for (int i = threadIdx.x; i < N; i += kLfThreads) label[i] = i < n ? row_label[i] : -1;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int v_lo = blockIdx.x * rows_of_cta, v_hi = min(V, v_lo + rows_of_cta);        // rows_of_cta a multiple of 8
+  const int tiles = n > 0 ? (v_hi - v_lo + kLfTile - 1) / kLfTile : 0, num_kb = (D + kLpBK - 1) / kLpBK;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = 0; tile < tiles && ok; ++tile) {
+        const int v0 = v_lo + tile * kLfTile, eights = (min(v_hi - v0, kLfTile) + 7) / 8;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty)) { ok = false; break; }
+          uint8_t* sw = smem + stage * S::stage_bytes;
+          mbar_expect_tx(&full[stage], eights * 1024 + N * 128);
+          int i = 0;
+          for (; i + 16 <= eights; i += 16) tma_load_2d(sw + i * 1024, &tmW, kb * kLpBK, v0 + i * 8, &full[stage]);
+          for (; i < eights; ++i) tma_load_2d(sw + i * 1024, &tmW8, kb * kLpBK, v0 + i * 8, &full[stage]);
+          tma_load_2d(sw + kLfTile * kLpBK * 2, &tmH, kb * kLpBK, 0, &full[stage]);
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_bf16(128, N, 0, 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = 0; tile < tiles && ok; ++tile) {
+        const int buf = tile & 1;
+        const bool both = v_hi - v_lo - tile * kLfTile > 128;
+        if (!mbar_wait(&acc_empty[buf], ((tile >> 1) & 1) ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
+        tc_fence_after();
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sw = smem_u32(smem + stage * S::stage_bytes), sh = sw + kLfTile * kLpBK * 2;
+#pragma unroll
+          for (int k = 0; k < kLpBK / 16; ++k) {
+            const uint64_t dh = smem_desc_kmajor_sw128(sh + k * 32);
+            const uint32_t add = kb != 0 || k != 0 ? 1u : 0u;
+            umma_ss(tmem_base + buf * 2 * N, smem_desc_kmajor_sw128(sw + k * 32), dh, idesc, add);
+            if (both) umma_ss(tmem_base + buf * 2 * N + N, smem_desc_kmajor_sw128(sw + 16384 + k * 32), dh, idesc, add);
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+        }
+        if (ok) umma_commit(&acc_full[buf]);
+      }
+    }
+  } else {
+    const int quad = warp & 3;
+    bool ok = true;
+    float run_m[N / 32], run_s[N / 32];          // of activation 32 c + lane, over this warp's rows so far
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) { run_m[c] = -INFINITY; run_s[c] = 0.f; }
+    for (int tile = 0; tile < tiles && ok; ++tile) {
+      const int buf = tile & 1;
+      if (!mbar_wait(&acc_full[buf], (tile >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int v0 = v_lo + tile * kLfTile + half * 128 + quad * 32, v = v0 + lane;
+        if (v0 >= v_hi) break;
+#pragma unroll
+        for (int c = 0; c < N / 32; ++c) {
+          if (c * 32 >= n) break;
+          uint32_t r[32];
+          tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (buf * 2 + half) * N + c * 32, r);
+          tmem_wait_ld();
+          float x[32], m[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            x[j] = v < v_hi ? __uint_as_float(r[j]) * scale2 : -INFINITY;
+            if (label[c * 32 + j] == v && v < v_hi) picked[c * 32 + j] = x[j];
+            m[j] = x[j];
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)             // lanes with bit o keep the upper half of what is left
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+              const bool up = lane & o;
+              const float other = __shfl_xor_sync(0xffffffffu, up ? m[j] : m[j + o], o);
+              m[j] = fmaxf(up ? m[j + o] : m[j], other);
+            }
+          const float top = fmaxf(run_m[c], m[0]), use = top == -INFINITY ? 0.f : top;         // of activation 32 c + lane
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = fast_exp2(x[j] - __shfl_sync(0xffffffffu, use, j));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < o; ++j) {
+              const bool up = lane & o;
+              const float other = __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + o], o);
+              x[j] = (up ? x[j + o] : x[j]) + other;
+            }
+          run_s[c] = run_s[c] * fast_exp2(run_m[c] - use) + x[0];                              // (0 before there is a maximum)
+          run_m[c] = top;
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c)
+      if (c * 32 + lane < n) stats[((long long)blockIdx.x * 4 + quad) * ld + c * 32 + lane] = (run_m[c] == -INFINITY ? 0.f : run_m[c]) + __log2f(run_s[c]);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kCols);
+  }
+}
+
 // Which rows have a label, in order: rows[i], row_label[i] and count; place[t] of every row (-1: none), and y[t] = 0 for those.  One block; a
 // warp takes kLpSelectEach times 32 rows in a round, so that 8192 rows are one round of loads and one scan.
 constexpr int kLpSelect = 1024;
@@ -429,11 +595,11 @@ log_probs_select_kernel(const long long* labels, int T, int V, long long ignore,
 }
 
 // The same and the gathering of the rows in one launch, for at most kLpFewRows rows: a block has a row, and counts the labels before it itself.
-// The blocks behind the last row fill up with zeros.
+// The blocks behind the last row fill up with zeros, to `fill` rows at least.
 constexpr int kLpFewRows = 1024;
 __global__ void __launch_bounds__(256)
 log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignore, int* rows, int* row_label, int* place, int* count, float* y,
-                          const bf16* h, long long ldh, bf16* dense, int D, int vec) {
+                          const bf16* h, long long ldh, bf16* dense, int D, int vec, int fill) {
   __shared__ int sums[2][8];
   grid_dependency_enter();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -462,7 +628,7 @@ log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignor
       else y[t] = 0.f;
     }
   }
-  if (!one && at >= (n + kLpBK - 1) / kLpBK * kLpBK) return;
+  if (!one && at >= max((n + kLpBK - 1) / kLpBK * kLpBK, fill)) return;
   const bf16* from = h + (long long)t * ldh;
   for (int c = threadIdx.x * 8; c < D; c += 256 * 8) {
     BF8 v{{0, 0, 0, 0}};
@@ -650,11 +816,25 @@ static int launch_log_probs(const CUtensorMap& A, const CUtensorMap& B, const CU
 using namespace ksa;
 #define ST(s) reinterpret_cast<cudaStream_t>(s)
 
+// Weight rows of a CTA of the kernel for few rows
+static int lf_rows(int V, int sms) {
+  const int each = (V + sms - 1) / sms;
+  return (each + 7) / 8 * 8;
+}
+
+// fp32 values of workspace for the forward pass
+KSA_API long long ksa_log_probs_work(int T, int V) {
+  const int sms = sm_count() > 0 ? sm_count() : 1, rows = lf_rows(V, sms);
+  const long long few = T <= kLfMostRows ? (V + rows - 1) / rows * 4 : 0;
+  const long long slots = (V + kLpStatCols - 1) / kLpStatCols;
+  return (T + 3LL) / 4 * 4 * ((few > slots ? few : slots) + 1);
+}
+
 // Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
 // Leaves what the backward pass needs: dense [T rounded up to 256, D] bf16, rows, row_label, place [T], count [1] int32, lse2 [2 T] (the log-sums
 // and the labels' logits less those, base 2), and where codes is not null the logits in 16 bits, codes [T rounded up to 256, V rounded up to 8]
 // with tops, fp32 [ceil(V / 128) times T rounded up to 4].
-// work: fp32 [T rounded up to 4 times (ceil(V / 128) + 1)].  y [T] fp32.
+// work: fp32 [ksa_log_probs_work(T, V)].  y [T] fp32.
 KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
                           void* lse2, void* work, void* y, void* codes, void* tops, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
                           void* stream) {
@@ -669,9 +849,12 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   float* stats = static_cast<float*>(work);
   float* picked = stats + ld * slots;
   const int vec = ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
+  const bool few = T <= kLfMostRows && codes == nullptr;
+  const int columns = (T + 31) / 32 * 32;                 // of the product with few rows
   if (T <= kLpFewRows) {
-    KSA_CHECK_CUDA(launch_kernel(log_probs_few_rows_kernel, dim3(T + kLpBK - 1), dim3(256), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
-                                 (int*)row_label, (int*)place, (int*)count, (float*)y, (const bf16*)h, ldh, (bf16*)dense, D, vec));
+    const int fill = few ? columns : 0, blocks = T + kLpBK - 1 > fill ? T + kLpBK - 1 : fill;
+    KSA_CHECK_CUDA(launch_kernel(log_probs_few_rows_kernel, dim3(blocks), dim3(256), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
+                                 (int*)row_label, (int*)place, (int*)count, (float*)y, (const bf16*)h, ldh, (bf16*)dense, D, vec, fill));
   } else {
     KSA_CHECK_CUDA(launch_kernel(log_probs_select_kernel, dim3(1), dim3(kLpSelect), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
                                  (int*)row_label, (int*)place, (int*)count, (float*)y));
@@ -680,22 +863,40 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh,
                                         (const int*)rows, (const int*)count, (bf16*)dense, D, vec));
   }
-  CUtensorMap A, B;
-  int rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
-  if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
-  CUtensorMap C = A;
-  if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, (V + 7LL) / 8 * 8, 32);
-  if (rc) return rc;
-  LpArgs a{};
-  a.M = T; a.N = V; a.K = D;
-  a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
-  a.scale2 = (float)(1.4426950408889634 / (double)tau);
-  a.stats = stats; a.picked = picked; a.ld_stats = ld; a.tops = static_cast<float*>(tops);
-  rc = codes ? launch_log_probs<kStatsKeep>(A, B, C, a, st) : launch_log_probs<kStats>(A, B, C, a, st);
-  if (rc) return rc;
+  CUtensorMap A, B, C;
+  int rc, sums = slots;
+  if (few) {
+    const int sms = sm_count(), rows_of_cta = lf_rows(V, sms), ctas = (V + rows_of_cta - 1) / rows_of_cta;
+    sums = ctas * 4;
+    picked = stats + ld * sums;
+    rc = lp_map(&A, w, 2, D, V, ldw, 128);
+    if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 8);
+    if (rc == 0) rc = lp_map(&C, dense, 2, D, padded, D, columns);
+    if (rc) return rc;
+    int* status = status_word();
+    KSA_REQUIRE(status != nullptr, "could not allocate the status word");
+    auto kern = columns == 32 ? log_probs_few_kernel<32> : columns == 64 ? log_probs_few_kernel<64> : columns == 96 ? log_probs_few_kernel<96> : log_probs_few_kernel<128>;
+    const int smem = columns == 32 ? LfShape<32>::smem : columns == 64 ? LfShape<64>::smem : columns == 96 ? LfShape<96>::smem : LfShape<128>::smem;
+    static PerDevice raised[4];
+    KSA_CHECK_CUDA(raise_smem_limit(raised[columns / 32 - 1], kern, smem));
+    KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, A, B, C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
+                                 (float)(1.4426950408889634 / (double)tau), stats, ld, picked, status));
+  } else {
+    rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
+    if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
+    if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, (V + 7LL) / 8 * 8, 32);
+    if (rc) return rc;
+    LpArgs a{};
+    a.M = T; a.N = V; a.K = D;
+    a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
+    a.scale2 = (float)(1.4426950408889634 / (double)tau);
+    a.stats = stats; a.picked = picked; a.ld_stats = ld; a.tops = static_cast<float*>(tops);
+    rc = codes ? launch_log_probs<kStatsKeep>(A, B, C, a, st) : launch_log_probs<kStats>(A, B, A, a, st);
+    if (rc) return rc;
+  }
   const bool wide = T >= 32 * 148;
   KSA_CHECK_CUDA(launch_kernel(wide ? log_probs_sum_kernel<32> : log_probs_sum_kernel<8>, dim3(wide ? (T + 31) / 32 : (T + 7) / 8), dim3(512), 0, st,
-                               (const float*)stats, ld, slots, (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2,
+                               (const float*)stats, ld, sums, (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2,
                                (float*)lse2 + T));
   return 0;
 }

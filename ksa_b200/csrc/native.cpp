@@ -113,6 +113,7 @@ int ksa_preference_loss(const void* y, const void* ref, const void* mask, const 
                         void* loss, int types, long long n, int sequences, long long length, float beta, float smoothing, void* stream);
 int ksa_preference_loss_bwd(const void* mask, const void* coef, const void* dloss, void* dy, int type, const void* cu, int wide, long long n,
                             int sequences, long long length, void* stream);
+long long ksa_log_probs_work(int T, int V);
 int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
                   void* lse2, void* work, void* y, void* codes, void* tops, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
                   void* stream);
@@ -1144,7 +1145,7 @@ LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, 
     k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
     k.tops = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns))}, on(h, at::kFloat));
   }
-  const Tensor work = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns + 1))}, on(h, at::kFloat));
+  const Tensor work = at::empty({(int64_t)ksa_log_probs_work((int)T, (int)V)}, on(h, at::kFloat));
   int* ints = static_cast<int*>(k.ints.mutable_data_ptr());
   LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), ints, ints + T, ints + 2 * T,
                  ints + 3 * T, k.lse2.mutable_data_ptr(), work.mutable_data_ptr(), k.y.mutable_data_ptr(), keep ? k.codes.mutable_data_ptr() : nullptr,

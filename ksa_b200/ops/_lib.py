@@ -131,6 +131,8 @@ def load() -> ctypes.CDLL:
     lib.ksa_int4_attn_workspace.restype = L
     lib.ksa_int4_cache_write_table.argtypes = [I] * 5
     lib.ksa_int4_cache_write_table.restype = L
+    lib.ksa_log_probs_work.argtypes = [I] * 2
+    lib.ksa_log_probs_work.restype = L
     lib.ksa_grad_norm_parts.argtypes = [I]
     lib.ksa_grad_norm_parts.restype = I
     lib.ksa_token_loss_units.argtypes = [L, I]
@@ -359,3 +361,6 @@ def grad_norm_parts(tensors: int) -> int:
 def token_loss_units(tokens: int, sequences: int) -> int:
     return load().ksa_token_loss_units(tokens, sequences)
 
+
+def log_probs_work(rows: int, vocabulary: int) -> int:
+    return load().ksa_log_probs_work(rows, vocabulary)

@@ -47,7 +47,7 @@ class _LinearLogProbsFn(torch.autograd.Function):
             if any(ctx.needs_input_grad[:2]) and _slab(padded, V) >= V:
                 codes = torch.empty((padded, _slab(padded, V)), dtype=torch.int16, device=dev)
                 tops = torch.empty(-(-T // 4) * 4 * -(-V // _STAT_COLS), dtype=torch.float32, device=dev)
-            work = torch.empty(-(-T // 4) * 4 * (-(-V // _STAT_COLS) + 1), dtype=torch.float32, device=dev)
+            work = torch.empty(_lib.log_probs_work(T, V), dtype=torch.float32, device=dev)
             weight = _pitched(w)
             _lib.call("ksa_log_probs", h, weight, labels, dense, rows, row_label, place, count, lse2, work, y, codes, tops, T, V, D, h.stride(0),
                       weight.stride(0), ignore_index, float(temperature))

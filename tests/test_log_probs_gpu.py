@@ -81,10 +81,40 @@ def test_values_and_gradients(T, D, V, answer, tau):
     assert y.dtype == torch.float32 and dh.dtype == dw.dtype == torch.bfloat16
     for name, got in (("y", y), ("dh", dh), ("dw", dw)):
         _close(got, want[name], name)
-    with torch.no_grad():
-        assert torch.equal(ops.linear_log_probs(h, w, labels, temperature=tau), y)
+    with torch.no_grad():           # (few rows have a kernel of their own without a gradient: another order of the log-sums)
+        alone = ops.linear_log_probs(h, w, labels, temperature=tau)
+    _close(alone, want["y"], "y alone")
     again = _run(h, w, labels, dy, tau)
     assert all(torch.equal(a, b) for a, b in zip(again, (y, dh, dw)))          # no order of summation varies
+
+
+@pytest.mark.parametrize("T", [1, 2, 31, 32, 33, 63, 64, 65, 100, 128, 129])
+@pytest.mark.parametrize("V", [1, 8, 31, 1000, 1185, 18944, 19001, 40000])
+def test_few_rows_without_a_gradient(T, V):
+    for answer, tau, D in ((1.0, 1.0, 72), (0.6, 0.7, 200)):
+        h, w, labels, dy = _inputs(T, D, V, answer, seed=T + V, tau=tau)
+        want = _oracle(h, w, labels, dy, tau)["y"]
+        with torch.no_grad():
+            y = ops.linear_log_probs(h, w, labels, temperature=tau)
+            assert torch.equal(ops.linear_log_probs(h, w, labels, temperature=tau), y)
+            _close(y, want, (T, V))
+            h[labels == IGNORE] = float("nan")
+            assert torch.equal(ops.linear_log_probs(h, w, labels, temperature=tau), y)
+
+
+def test_bad_rows_without_a_gradient():
+    h, w, labels, _ = _inputs(40, 64, 3000, 1.0, seed=18)
+    with torch.no_grad():
+        good = ops.linear_log_probs(h, w, labels)
+        h[3, 5], h[9, 0] = float("nan"), float("inf")
+        y = ops.linear_log_probs(h, w, labels)
+        h[:] = (h * 0 + 1).nan_to_num(1, 1, 1) * 300
+        far = ops.linear_log_probs(h, w, labels)
+    rest = torch.tensor([i not in (3, 9) for i in range(40)], device="cuda")
+    assert torch.isnan(y[3]) and torch.isnan(y[9]) and torch.equal(y[rest], good[rest])
+    x = h.double() @ w.double().T
+    want = (x - x.logsumexp(1, keepdim=True)).gather(1, labels[:, None])[:, 0]
+    assert (far.double() - want).abs().max() <= 6 * 2.0 ** -22 * 64 * 300 * 0.3 + 8 * 2.0 ** -22 * x.abs().max() * 2
 
 
 def test_every_row_without_a_label():
