@@ -107,6 +107,7 @@ class TrainingConfig(BaseConfig):
     model_dtype: Literal["bfloat16", "float16", "float32"] = "bfloat16"
     gradient_accumulation_steps: int = Field(default=1, ge=1)
     clip_range: float = Field(default=1.0, gt=0.0)
+    clip_norm: float = Field(default=0.0, ge=0.0)
     enable_gradient_checkpointing: bool = False
     chunked_loss_minibatch_size: int = Field(default=2048, ge=1)
     disable_chunked_loss: bool = False
@@ -156,7 +157,7 @@ _ARG_MAP: Dict[str, Tuple[str, str]] = {
     "cpu_offload": ("parallel", "cpu_offload"), "comm": ("parallel", "comm"), "overlap": ("parallel", "overlap"),
 }
 _TOP_ARGS = {"model_config": "model_config_path", "model_dtype": "model_dtype",
-             "gradient_accumulation_steps": "gradient_accumulation_steps", "clip_range": "clip_range",
+             "gradient_accumulation_steps": "gradient_accumulation_steps", "clip_range": "clip_range", "clip_norm": "clip_norm",
              "enable_gradient_checkpointing": "enable_gradient_checkpointing",
              "chunked_loss_minibatch_size": "chunked_loss_minibatch_size", "disable_chunked_loss": "disable_chunked_loss",
              "seed": "seed"}

@@ -397,8 +397,11 @@ class Qwen3Model(Model):
     def forward(self, tokens: torch.Tensor, labels: Optional[torch.Tensor] = None,
                 position_ids: Optional[torch.Tensor] = None, return_hidden: bool = False,
                 collect_attn: bool = False, ignore_index: int = -100, kv_sink=None, last_token_only: bool = False,
-                use_summary: bool = True, cu_seqlens: Optional[torch.Tensor] = None):
+                use_summary: bool = True, cu_seqlens: Optional[torch.Tensor] = None, log_probs: bool = False, temperature: float = 1.0):
         """``tokens`` ``[B, L]`` -> loss (with ``labels``), hidden ``[B, L, D]`` or logits ``[B, L, V]``.
+
+        ``log_probs``: with ``labels``, their log probabilities ``[B, L]`` instead of the loss (fp32, at a sampling ``temperature``, 0 where a
+        label is ignored): what the losses of :mod:`ksa_b200.losses.post_training` take.
 
         ``cu_seqlens`` (token offsets of documents packed into the sequence, the same for every sequence of the batch):
         full-attention layers keep every query inside its own document (the reference's varlen FlashAttention-2 path,
@@ -437,6 +440,12 @@ class Qwen3Model(Model):
         _, h = _add_norm(tp, x[:n_text], delta[:n_text] if delta is not None else None, self.norm.scale,
                          self.config.norm_eps)
         self.last_attn_outputs = collect
+        if log_probs:
+            if labels is None or self.skip_output_layer:
+                raise ValueError("log_probs needs labels and the output head")
+            if self.lm_head_weight.shape[0] != self.config.vocab_size:
+                raise ValueError("log_probs needs the whole output head on this rank")
+            return ops.linear_log_probs(h, self.lm_head_weight, labels.reshape(-1), ignore_index, temperature).view(B, L)
         if labels is not None and not self.skip_output_layer:
             return ops.linear_cross_entropy(h, self.lm_head_weight, labels.reshape(-1), ignore_index,
                                             self.loss_chunk_tokens)

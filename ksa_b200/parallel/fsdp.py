@@ -95,6 +95,9 @@ class FsdpEngine(TrainEngine):
                              else "collective")
         if self.comm == "fused" and not one_node:
             raise ValueError("comm='fused' needs all ranks on one node (peer memory); use comm='collective' across nodes")
+        if kw.get("clip_norm") and self.comm == "fused" and world_size > 1:
+            raise ValueError("clip_norm needs the reduced gradients of all units before the first update, and the fused back end reduces and "
+                             "updates a unit in one kernel: use comm='collective'")
         if self.reshard and (self.comm != "fused" or overlap != "stream" or world_size < 2):
             raise ValueError("reshard_after_forward needs the fused back end with overlap='stream' on 2 or more ranks")
         self._slot_holds = {}          # pool slot -> unit index whose weights it holds
@@ -420,27 +423,43 @@ class FsdpEngine(TrainEngine):
             return
         self._collect_autograd_grads()
         self.grad_sq.zero_()
+        shards = [None] * len(self.units)
+        if self.clip_norm:      # every rank's shards, then the norm of all of them, then the updates
+            shards = [self._reduced_shard(u) for u in self.units]
+            self._clip_by_norm(shards)
         for unit in reversed(self.units):
-            self._reduce_and_update(unit)
+            self._reduce_and_update(unit, shards[unit.index])
 
-    def _reduce_and_update(self, unit: Unit) -> None:
-        """Collective path: reduce-scatter -> AdamW on the shard -> all-gather of the refreshed weights."""
-        w = self.world_size
+    def _clip_by_norm(self, grads) -> None:
+        scale = 1.0 / (self.grad_accum_steps * max(self.world_size, 1))
+        total = ops.grad_norm(grads, scale).double().square().reshape(1)
+        if self.world_size > 1:
+            dist.all_reduce(total, group=self.group)
+        self.grad_sq.copy_(total)
+        self._grad_sq_reduced = self.grad_sq
+        self.hyper[3:4].copy_(scale * (self.clip_norm / (total.sqrt() + 1e-6)).clamp(max=1.0))
+
+    def _reduced_shard(self, unit: Unit) -> torch.Tensor:
+        """This rank's part of the unit's gradient, summed over the ranks."""
         lo, hi = unit.shard_lo, unit.shard_hi
-        if w > 1:
-            backend = dist.get_backend(self.group)
-            if backend == "nccl":
+        if self.world_size > 1:
+            if dist.get_backend(self.group) == "nccl":
                 shard = torch.empty(hi - lo, dtype=torch.float32, device=self.device)
                 dist.reduce_scatter_tensor(shard, unit.grad, group=self.group)
-            else:
-                dist.all_reduce(unit.grad, group=self.group)
-                shard = unit.grad[lo:hi]
-        else:
-            shard = unit.grad[lo:hi]
+                return shard
+            dist.all_reduce(unit.grad, group=self.group)
+        return unit.grad[lo:hi]
+
+    def _reduce_and_update(self, unit: Unit, shard: Optional[torch.Tensor] = None) -> None:
+        """Collective path: reduce-scatter (unless it has been done) -> AdamW on the shard -> all-gather of the refreshed weights."""
+        w = self.world_size
+        lo, hi = unit.shard_lo, unit.shard_hi
+        if shard is None:
+            shard = self._reduced_shard(unit)
         out = unit.compute[lo:hi] if self.param_dtype != torch.float32 else None
         with self._optimizer_state(unit) as (master, exp_avg, exp_avg_sq):
             ops.adamw_step(master, shard, exp_avg, exp_avg_sq, out, self.hyper, self.beta1, self.beta2,
-                           self.eps, self.weight_decay, self.clip_value, self.grad_sq)
+                           self.eps, self.weight_decay, self.clip_value, None if self.clip_norm else self.grad_sq)
             if self.param_dtype == torch.float32:
                 unit.compute[lo:hi].copy_(master)
         if w > 1:

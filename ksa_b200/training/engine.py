@@ -92,7 +92,16 @@ class TrainEngine:
                  param_dtype: Optional[torch.dtype] = None, device: Optional[torch.device] = None,
                  lr_lambda: Optional[Callable[[int], float]] = None, grad_accum_steps: int = 1,
                  world_size: int = 1, rank: int = 0, cpu_offload: bool = False,
-                 overlap_optimizer: Optional[bool] = None):
+                 overlap_optimizer: Optional[bool] = None, clip_norm: float = 0.0):
+        """``clip_value``: every element of the averaged gradient is cut to ``[-clip_value, clip_value]`` (0: not).
+        ``clip_norm``: the averaged gradients of a step are scaled down to this global 2-norm where theirs is larger (0: not), ahead of
+        ``clip_value``; :meth:`grad_norm` then is the norm before that.  It takes all gradients before the first update, so the
+        optimizer does not run under the backward pass."""
+        if not clip_norm >= 0:
+            raise ValueError(f"clip_norm must not be negative, got {clip_norm}")
+        if clip_norm and overlap_optimizer:
+            raise ValueError("clip_norm needs all gradients before the first update: overlap_optimizer cannot be had with it")
+        self.clip_norm = float(clip_norm)
         self.model = model
         self.cpu_offload = bool(cpu_offload)   # master weights and moments in pinned host memory (training/offload.py)
         self._offload = None
@@ -126,7 +135,7 @@ class TrainEngine:
         if overlap_optimizer is None:
             env = os.environ.get("KSA_OVERLAP_OPTIMIZER")
             overlap_optimizer = (env == "1") if env is not None else (self.cpu_offload and self.device.type == "cuda")
-        self.overlap_optimizer = bool(overlap_optimizer) and self._overlap_capable
+        self.overlap_optimizer = bool(overlap_optimizer) and self._overlap_capable and not self.clip_norm
         self._hooks_active = False
         self._overlap_step = False
         self._async_done: set = set()
@@ -360,15 +369,24 @@ class TrainEngine:
             ops.adamw_step(master, unit.grad, exp_avg, exp_avg_sq,
                            unit.compute if self.param_dtype != torch.float32 else None,
                            self.hyper, self.beta1, self.beta2, self.eps, self.weight_decay, self.clip_value,
-                           self.grad_sq)
+                           None if self.clip_norm else self.grad_sq)
             if self.param_dtype == torch.float32:
                 unit.compute.copy_(master)
+
+    def _clip_by_norm(self, grads: Sequence[torch.Tensor]) -> None:
+        """Make the gradient scale that AdamW reads what brings the global norm of ``grads`` down to ``clip_norm``: the gradients are read
+        once more, and scaled where they are read anyway."""
+        norm, factor = ops.grad_norm(grads, 1.0 / (self.grad_accum_steps * max(self.world_size, 1)), self.clip_norm)
+        self.grad_sq.copy_(norm.square())
+        self.hyper[3:4].copy_(factor)
 
     def optimizer_step(self) -> None:
         self._collect_autograd_grads()
         if not self._overlap_step:
             self.grad_sq.zero_()
             self._async_done = set()
+        if self.clip_norm:
+            self._clip_by_norm([u.grad for u in self.units])
         for unit in reversed(self.units):
             if unit.index not in self._async_done:     # updated under the backward pass already
                 self._reduce_and_update(unit)
@@ -382,7 +400,8 @@ class TrainEngine:
         pass
 
     def grad_norm(self) -> torch.Tensor:
-        """Global L2 norm of the (averaged) gradients of the last optimizer step, as a device scalar."""
+        """Global L2 norm of the (averaged) gradients of the last optimizer step, as a device scalar: before clipping by the norm, after
+        clipping by value."""
         return self.grad_sq.sqrt()
 
     # ------------------------------------------------------------------ steps

@@ -74,6 +74,7 @@ def get_argument_parser() -> argparse.ArgumentParser:
     a("--beta1", type=float, default=0.9)
     a("--beta2", type=float, default=0.95)
     a("--clip-range", type=float, default=1.0)
+    a("--clip-norm", type=float, default=0.0, help="scale the gradients of a step down to this global 2-norm, ahead of --clip-range (0: not)")
     a("--use-flash-attention-2", action="store_true")
     a("--enable-gradient-checkpointing", action="store_true")
     a("--gradient-checkpointing-mode", default="full", choices=["full", "mlp"],
@@ -220,7 +221,7 @@ def train(args) -> dict:
                               num_training_steps=args.num_training_steps, num_decay_steps=args.num_decay_steps,
                               base_lr=args.learning_rate, min_lr=args.min_lr)
     common = dict(lr=args.learning_rate, betas=(args.beta1, args.beta2), eps=1e-8, weight_decay=args.weight_decay,
-                  clip_value=args.clip_range, lr_lambda=lr_lambda, grad_accum_steps=args.gradient_accumulation_steps,
+                  clip_value=args.clip_range, clip_norm=args.clip_norm, lr_lambda=lr_lambda, grad_accum_steps=args.gradient_accumulation_steps,
                   cpu_offload=args.cpu_offload)
     if world > 1:
         from ksa_b200.parallel.fsdp import FsdpEngine, default_overlap
