@@ -973,25 +973,27 @@ struct PolicyCall {
   double bounds[4] = {0, 0, 0, 0};
   float beta = 0;
 
-  // {loss, statistics, gradients up to the normaliser (only where wanted), normalisers}
-  std::tuple<Tensor, Tensor, Tensor, Tensor> run(bool keep) const {
+  // fp32 values of the buffer in front of the partial sums: gradients up to the normaliser (only where wanted), then normalisers
+  static long long inv_at(long long n, bool keep) { return keep ? (n + 3) / 4 * 4 : 0; }
+  static long long partial_at(long long n, int sequences, bool keep) { return inv_at(n, keep) + (std::max(sequences, 1) + 3) / 4 * 4; }
+
+  std::tuple<Tensor, Tensor, Tensor> run(bool keep) const {                 // {loss, statistics, buffer}
     const Tensor& y = *t.y;
-    const Tensor loss = at::empty({}, on(y, at::kFloat)), stats = at::empty({3}, on(y, at::kFloat)), inv = at::empty({std::max(t.sequences, 1)}, on(y, at::kFloat));
-    const Tensor partial = at::empty({(int64_t)(4 * ksa_token_loss_units(t.n, t.sequences))}, on(y, at::kDouble));
-    Tensor grad;
-    if (keep) grad = at::empty({(int64_t)t.n}, on(y, at::kFloat));
+    const Tensor loss = at::empty({}, on(y, at::kFloat)), stats = at::empty({3}, on(y, at::kFloat));
+    const long long sums = partial_at(t.n, t.sequences, keep);
+    const Tensor work = at::empty({(int64_t)(sums + 8 * ksa_token_loss_units(t.n, t.sequences))}, on(y, at::kFloat));
+    float* at = static_cast<float*>(work.mutable_data_ptr());
     const int types = token_type(y) | token_type(*old) << 4 | (ref ? token_type(*ref) : 0) << 8 | token_type(*adv) << 12;
     LAUNCH_SEVERAL(2, ksa_policy_loss, y.const_data_ptr(), old->const_data_ptr(), ref ? ref->const_data_ptr() : nullptr, adv->const_data_ptr(),
-                   t.mask ? t.mask->const_data_ptr() : nullptr, t.offsets(), t.wide(), keep ? grad.mutable_data_ptr() : nullptr,
-                   partial.mutable_data_ptr(), inv.mutable_data_ptr(), loss.mutable_data_ptr(), stats.mutable_data_ptr(), types, t.n, t.sequences, t.length,
+                   t.mask ? t.mask->const_data_ptr() : nullptr, t.offsets(), t.wide(), keep ? at : nullptr, at + sums, at + inv_at(t.n, keep), loss.mutable_data_ptr(), stats.mutable_data_ptr(), types, t.n, t.sequences, t.length,
                    adv_by_sequence, by_sequence, bounds, beta, stream_of(y));
-    return {loss, stats, grad, inv};
+    return {loss, stats, work};
   }
 };
 struct PolicyNode : public torch::autograd::Function<PolicyNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& y, const PolicyCall* call) {
-    auto [loss, stats, grad, inv] = call->run(true);
-    ctx->save_for_backward({grad, inv, call->t.cu ? *call->t.cu : Tensor()});
+    auto [loss, stats, work] = call->run(true);
+    ctx->save_for_backward({work, call->t.cu ? *call->t.cu : Tensor()});
     ctx->saved_data["sequences"] = (int64_t)call->t.sequences;
     ctx->saved_data["length"] = (int64_t)call->t.length;
     ctx->saved_data["by_sequence"] = (int64_t)call->by_sequence;
@@ -1004,12 +1006,14 @@ struct PolicyNode : public torch::autograd::Function<PolicyNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const Tensor &grad = saved[0], &inv = saved[1], &cu = saved[2], &dloss = grads[0];
+    const Tensor &work = saved[0], &cu = saved[1], &dloss = grads[0];
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
-    Tensor dy = at::empty(ctx->saved_data["shape"].toIntVector(), on(grad, type));
-    LAUNCH(ksa_policy_loss_bwd, grad.const_data_ptr(), inv.const_data_ptr(), dloss.const_data_ptr(), dy.mutable_data_ptr(), token_type(dy),
-           cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, grad.numel(), (int)ctx->saved_data["sequences"].toInt(),
-           ctx->saved_data["length"].toInt(), (int)ctx->saved_data["by_sequence"].toInt(), stream_of(grad));
+    Tensor dy = at::empty(ctx->saved_data["shape"].toIntVector(), on(work, type));
+    const float* at = static_cast<const float*>(work.const_data_ptr());
+    const long long n = dy.numel();
+    LAUNCH(ksa_policy_loss_bwd, at, at + PolicyCall::inv_at(n, true), dloss.const_data_ptr(), dy.mutable_data_ptr(), token_type(dy),
+           cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, n, (int)ctx->saved_data["sequences"].toInt(),
+           ctx->saved_data["length"].toInt(), (int)ctx->saved_data["by_sequence"].toInt(), stream_of(work));
     return {differentiated_once(dy), Tensor()};
   }
 };
@@ -1045,7 +1049,7 @@ PyObject* py_policy_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
       loss = made[0];
       stats = made[1];
     } else {
-      std::tie(loss, stats, std::ignore, std::ignore) = c.run(false);
+      std::tie(loss, stats, std::ignore) = c.run(false);
     }
   }
   return wrap(loss, stats);
@@ -1057,20 +1061,23 @@ struct PreferenceCall {
   const Tensor* ref = nullptr;
   float beta = 0, smoothing = 0;
 
-  std::tuple<Tensor, Tensor, Tensor> run() const {          // {loss, rewards, coefficients}
+  std::tuple<Tensor, Tensor, Tensor> run() const {          // {loss, rewards, coefficients with the partial sums behind them}
     const Tensor& y = *t.y;
-    const Tensor loss = at::empty({}, on(y, at::kFloat)), rewards = at::empty({t.sequences / 2, 2}, on(y, at::kFloat)), coef = at::empty({t.sequences}, on(y, at::kFloat));
-    const Tensor partial = at::empty({(int64_t)ksa_token_loss_units(t.n, t.sequences)}, on(y, at::kDouble));
+    const Tensor loss = at::empty({}, on(y, at::kFloat)), rewards = at::empty({t.sequences / 2, 2}, on(y, at::kFloat));
+    const long long sums = (t.sequences + 3) / 4 * 4;
+    const Tensor work = at::empty({(int64_t)(sums + 2 * ksa_token_loss_units(t.n, t.sequences))}, on(y, at::kFloat));
+    float* at = static_cast<float*>(work.mutable_data_ptr());
     LAUNCH_SEVERAL(2, ksa_preference_loss, y.const_data_ptr(), ref ? ref->const_data_ptr() : nullptr, t.mask ? t.mask->const_data_ptr() : nullptr, t.offsets(), t.wide(),
-                   partial.mutable_data_ptr(), coef.mutable_data_ptr(), rewards.mutable_data_ptr(), loss.mutable_data_ptr(),
+                   at + sums, at, rewards.mutable_data_ptr(), loss.mutable_data_ptr(),
                    token_type(y) | (ref ? token_type(*ref) : 0) << 4, t.n, t.sequences, t.length, beta, smoothing, stream_of(y));
-    return {loss, rewards, coef};
+    return {loss, rewards, work};
   }
 };
 struct PreferenceNode : public torch::autograd::Function<PreferenceNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& y, const PreferenceCall* call) {
-    auto [loss, rewards, coef] = call->run();
-    ctx->save_for_backward({coef, call->t.mask ? *call->t.mask : Tensor(), call->t.cu ? *call->t.cu : Tensor()});
+    auto [loss, rewards, work] = call->run();
+    ctx->save_for_backward({work, call->t.mask ? *call->t.mask : Tensor(), call->t.cu ? *call->t.cu : Tensor()});
+    ctx->saved_data["sequences"] = (int64_t)call->t.sequences;
     ctx->saved_data["length"] = (int64_t)call->t.length;
     ctx->saved_data["shape"] = y.sizes().vec();
     ctx->saved_data["type"] = (int64_t)y.scalar_type();
@@ -1085,7 +1092,7 @@ struct PreferenceNode : public torch::autograd::Function<PreferenceNode> {
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
     Tensor dy = at::empty(ctx->saved_data["shape"].toIntVector(), on(coef, type));
     LAUNCH(ksa_preference_loss_bwd, mask.defined() ? mask.const_data_ptr() : nullptr, coef.const_data_ptr(), dloss.const_data_ptr(), dy.mutable_data_ptr(),
-           token_type(dy), cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, dy.numel(), (int)coef.numel(),
+           token_type(dy), cu.defined() ? cu.const_data_ptr() : nullptr, cu.defined() && cu.scalar_type() == at::kLong, dy.numel(), (int)ctx->saved_data["sequences"].toInt(),
            ctx->saved_data["length"].toInt(), stream_of(coef));
     return {differentiated_once(dy), Tensor()};
   }
@@ -1126,7 +1133,7 @@ struct LogProbsCall {
   float tau = 1;
 };
 struct LogProbsKept {
-  Tensor y, dense, ints, lse2, codes, tops;         // ints: rows, row_label, place, count
+  Tensor y, dense, kept, codes;            // kept, in words: rows, row_label, place (T each), count (4), log-sums (2 T), maxima of the kept logits
 };
 // Columns of the vocabulary that the backward pass takes at a time (_slab in ops/log_probs.py).
 long long slab_of(long long padded, long long V, long long bytes) {
@@ -1137,26 +1144,23 @@ LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, 
   LogProbsKept k;
   k.y = at::empty(c.labels->sizes(), on(h, at::kFloat));
   k.dense = at::empty({(int64_t)padded, (int64_t)D}, on(h, at::kBFloat16));
-  k.ints = at::empty({(int64_t)(3 * T + 1)}, on(h, at::kInt));
-  k.lse2 = at::empty({(int64_t)(2 * T)}, on(h, at::kFloat));
   const long long slab = slab_of(padded, V, c.slab_bytes);
   const bool keep = grad && slab >= V;
-  if (keep) {
-    k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
-    k.tops = at::empty({(int64_t)((T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns))}, on(h, at::kFloat));
-  }
+  if (keep) k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
+  k.kept = at::empty({(int64_t)(5 * T + 4 + (keep ? (T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns) : 0))}, on(h, at::kInt));
   const Tensor work = at::empty({(int64_t)ksa_log_probs_work((int)T, (int)V)}, on(h, at::kFloat));
-  int* ints = static_cast<int*>(k.ints.mutable_data_ptr());
-  LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), ints, ints + T, ints + 2 * T,
-                 ints + 3 * T, k.lse2.mutable_data_ptr(), work.mutable_data_ptr(), k.y.mutable_data_ptr(), keep ? k.codes.mutable_data_ptr() : nullptr,
-                 keep ? k.tops.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D,
+  int* kept = static_cast<int*>(k.kept.mutable_data_ptr());
+  LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), kept, kept + T, kept + 2 * T,
+                 kept + 3 * T, kept + 3 * T + 4, work.mutable_data_ptr(), k.y.mutable_data_ptr(), keep ? k.codes.mutable_data_ptr() : nullptr,
+                 keep ? kept + 5 * T + 4 : nullptr, (int)T, (int)V, (int)D,
                  h.dim() == 2 ? h.stride(0) : D, w.stride(0), c.ignore, c.tau, stream_of(h));
   return k;
 }
 struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const LogProbsCall* call) {
     const LogProbsKept k = log_probs(h, w, *call, true);
-    ctx->save_for_backward({k.dense, w, k.ints, k.lse2, k.codes, k.tops});
+    ctx->save_for_backward({k.dense, w, k.kept, k.codes});
+    ctx->saved_data["rows"] = (int64_t)call->labels->numel();
     ctx->saved_data["shape"] = h.sizes().vec();
     ctx->saved_data["tau"] = (double)call->tau;
     ctx->saved_data["slab_bytes"] = (int64_t)call->slab_bytes;
@@ -1165,8 +1169,8 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &dense = saved[0], &w = saved[1], &ints = saved[2], &lse2 = saved[3], &codes = saved[4], &tops = saved[5];
-    const long long T = lse2.numel() / 2, V = w.size(0), D = w.size(1), padded = dense.size(0);
+    const Tensor &dense = saved[0], &w = saved[1], &kept = saved[2], &codes = saved[3];
+    const long long T = ctx->saved_data["rows"].toInt(), V = w.size(0), D = w.size(1), padded = dense.size(0);
     const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     const Tensor dy = grads[0].contiguous();
     const long long slab = codes.defined() ? codes.size(1) : slab_of(padded, V, ctx->saved_data["slab_bytes"].toInt());
@@ -1178,9 +1182,9 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
       dh32 = at::empty({(int64_t)planes, (int64_t)padded, (int64_t)D}, on(w, at::kFloat));
     }
     if (need_w) dw = at::empty({(int64_t)V, (int64_t)D}, on(w, at::kBFloat16));
-    const int* p = static_cast<const int*>(ints.const_data_ptr());
-    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, lse2.const_data_ptr(), codes.defined() ? codes.const_data_ptr() : nullptr,
-                   codes.defined() ? tops.const_data_ptr() : nullptr, dy.const_data_ptr(),
+    const int* p = static_cast<const int*>(kept.const_data_ptr());
+    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, p + 3 * T + 4, codes.defined() ? codes.const_data_ptr() : nullptr,
+                   codes.defined() ? p + 5 * T + 4 : nullptr, dy.const_data_ptr(),
                    dx.mutable_data_ptr(), need_h ? dh32.mutable_data_ptr() : nullptr, need_h ? dh.mutable_data_ptr() : nullptr,
                    need_w ? dw.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D, w.stride(0), D, 0, 0, (int)slab, need_h ? (int)planes : 1, (float)ctx->saved_data["tau"].toDouble(),
                    stream_of(w));

@@ -16,8 +16,9 @@
 // and a block finds its sequence by bisection: no list is built first, and lengths of zero cost an empty unit.  The tokens behind the
 // last sequence are one more sequence, without valid tokens.
 //
-// Differences of log probabilities are taken in 64 bits, so that a token on the border of the clipped range falls on one side of it
-// wherever the sum is rounded; sums are kept in 64 bits in a fixed order.
+// A difference of two fp32 numbers is rounded once, which exponentials bear; next to the border of the clipped range it is taken again in 64
+// bits, so that a token falls on the side where it belongs.  A thread's few terms are summed in 32 bits, everything above that, and the log
+// ratios of whole answers from their first token on, in 64 and in a fixed order.
 #include "common.cuh"
 #include "host.h"
 
@@ -51,11 +52,16 @@ struct Piece {
   int s;
   long long lo, hi;            // its tokens; none where lo >= hi
 };
+// The last sequence whose first unit is not behind `unit`, by every warp: its lanes try 32 places at a time (two rounds of loads for 1000
+// sequences, where bisection takes ten).
 __device__ __forceinline__ Piece find_piece(const Sequences& q, long long unit) {
-  int lo = 0, hi = q.S + 1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (q.unit(mid) <= unit) lo = mid; else hi = mid;
+  int lo = 0, n = q.S + 1;
+  while (n > 1) {
+    const int step = (n + 31) / 32, at = (int)(threadIdx.x & 31) * step;
+    const unsigned yes = __ballot_sync(0xffffffffu, at < n && (at == 0 || q.unit(lo + at) <= unit));
+    const int found = (31 - __clz(yes)) * step;
+    lo += found;
+    n = min(step, n - found);
   }
   Piece p;
   p.s = lo;
@@ -148,6 +154,7 @@ struct PolicyArgs {
   const uint8_t* mask;
   int ty, told, tref, tadv, adv_by_sequence, by_sequence, vec;
   double above, below;         // log(1 + high), log(1 - low)
+  float above32, below32;
   float most, least;           // 1 + high, 1 - low
   float beta;
   float* grad;                 // [n] up to the normaliser, or null
@@ -163,25 +170,30 @@ struct TokenTerms {
 };
 __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float y, float old, float ref, float A) {
   TokenTerms t;
-  const double d = (double)y - (double)old;
-  t.cut = (A > 0.f && d > a.above) || (A < 0.f && d < a.below);
-  const float r = expf((float)d);
+  const float d = y - old;
+  t.cut = (A > 0.f && d > a.above32) || (A < 0.f && d < a.below32);
+  if (fabsf(d - (A > 0.f ? a.above32 : a.below32)) < 1e-6f * fabsf(d)) {         // next to the border the difference's rounding would decide
+    const double exact = (double)y - (double)old;
+    t.cut = (A > 0.f && exact > a.above) || (A < 0.f && exact < a.below);
+  }
+  const float r = expf(d);
   t.L = t.cut ? -(A > 0.f ? a.most : a.least) * A : -r * A;
   t.g = t.cut ? 0.f : -r * A;
   t.K = 0.f;
   if (a.ref) {
-    const float x = (float)((double)ref - (double)y);
+    const float x = ref - y;
     t.K = exp_minus_line(x);
     if (a.beta != 0.f) t.g -= a.beta * expm1f(x);
   }
   return t;
 }
 
-__global__ void __launch_bounds__(kTlThreads) policy_loss_kernel(const PolicyArgs a, const Sequences q) {
+__global__ void __launch_bounds__(kTlThreads, 5) policy_loss_kernel(const PolicyArgs a, const Sequences q) {
   __shared__ double red[4 * kTlThreads / 32];
   grid_dependency_enter();
   const Piece p = find_piece(q, blockIdx.x);
-  double sums[4] = {0, 0, 0, 0};
+  float sum_L = 0.f, sum_K = 0.f;
+  int cut = 0, count = 0;
   const bool none = p.s >= q.S;                                                   // behind the last sequence
   const float seq_adv = a.adv_by_sequence && !none ? load_token(a.adv, a.tadv, p.s) : 0.f;
   for (long long i = (p.lo & ~3LL) + 4 * threadIdx.x; i < p.hi; i += 4 * kTlThreads) {
@@ -208,23 +220,17 @@ __global__ void __launch_bounds__(kTlThreads) policy_loss_kernel(const PolicyArg
         if (!a.adv_by_sequence) A[j] = load_token(a.adv, a.tadv, i + j);
       }
     }
-    float L = 0.f, K = 0.f;
-    int cut = 0, count = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       g[j] = 0.f;
       if (!valid[j]) continue;
       const TokenTerms t = policy_token(a, y[j], old[j], ref[j], a.adv_by_sequence ? seq_adv : A[j]);
-      L += t.L;
-      K += t.K;
+      sum_L += t.L;
+      sum_K += t.K;
       cut += t.cut;
       ++count;
       g[j] = t.g;
     }
-    sums[0] += L;
-    sums[1] += K;
-    sums[2] += cut;
-    sums[3] += count;
     if (a.grad) {
       if (whole) store_tokens(a.grad, kTokF32, i, g);
       else
@@ -233,10 +239,24 @@ __global__ void __launch_bounds__(kTlThreads) policy_loss_kernel(const PolicyArg
           if (i + j >= p.lo && i + j < p.hi) a.grad[i + j] = g[j];
     }
   }
-  block_sums(sums, red);
-  if (threadIdx.x == 0)
+  double sums[2] = {sum_L, sum_K};
+  warp_sums(sums);
+  cut = __reduce_add_sync(0xffffffffu, cut);
+  count = __reduce_add_sync(0xffffffffu, count);
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    red[4 * warp] = sums[0];
+    red[4 * warp + 1] = sums[1];
+    red[4 * warp + 2] = cut;
+    red[4 * warp + 3] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    double v = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) a.partial[4 * (long long)blockIdx.x + k] = sums[k];
+    for (int w = 0; w < kTlThreads / 32; ++w) v += red[4 * w + threadIdx.x];
+    a.partial[4 * (long long)blockIdx.x + threadIdx.x] = v;
+  }
 }
 
 // The sums of a sequence's pieces, by a warp.
@@ -424,6 +444,7 @@ KSA_API int ksa_policy_loss(const void* y, const void* old, const void* ref, con
           (reinterpret_cast<uintptr_t>(mask) & 3) == 0 && aligned_for(grad, kTokF32);
   const double* b = static_cast<const double*>(bounds);
   a.above = b[0]; a.below = b[1]; a.most = (float)b[2]; a.least = (float)b[3];
+  a.above32 = (float)a.above; a.below32 = (float)a.below;
   a.beta = beta; a.grad = static_cast<float*>(grad); a.partial = static_cast<double*>(partial);
   a.inv = static_cast<float*>(inv); a.loss = static_cast<float*>(loss); a.stats = static_cast<float*>(stats);
   KSA_CHECK_CUDA(launch_stream_kernel(21LL * n, policy_loss_kernel, dim3(units), dim3(kTlThreads), 0, ST(stream), a, q));
@@ -438,8 +459,9 @@ KSA_API int ksa_policy_loss_bwd(const void* grad, const void* inv, const void* d
   KSA_SEQUENCES("policy_loss");
   KSA_REQUIRE(type_ok(type), "policy_loss: type %d", type);
   const int vec = aligned_for(grad, kTokF32) && aligned_for(dy, type);
-  KSA_CHECK_CUDA(launch_stream_kernel(8LL * n, policy_grad_kernel, dim3(units), dim3(kTlThreads), 0, ST(stream), (const float*)grad, (const float*)inv,
-                                      (const float*)dloss, dy, type, by_sequence, vec, q));
+  const Sequences all{nullptr, 0, 1, n, n};                                       // (one normaliser: nothing to look up)
+  KSA_CHECK_CUDA(launch_stream_kernel(8LL * n, policy_grad_kernel, dim3(by_sequence ? units : (unsigned)unit_count(n, 1)), dim3(kTlThreads), 0, ST(stream),
+                                      (const float*)grad, (const float*)inv, (const float*)dloss, dy, type, by_sequence, vec, by_sequence ? q : all));
   return 0;
 }
 
