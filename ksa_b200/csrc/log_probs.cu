@@ -31,13 +31,13 @@ constexpr int kLpBM = 128;          // rows of the tile in a CTA; a pair has 256
 constexpr int kLpBN = 256;          // columns of the tile
 constexpr int kLpBNh = 128;         // rows of B staged per CTA
 constexpr int kLpBK = 64;
-constexpr int kLpThreads = 192;     // warp 0 loads, warp 1 issues products, warps 2..5 epilogue
+constexpr int kLpThreads = 320;     // warp 0 loads, warp 1 issues products, warps 2..5 and 6..9 epilogue, each group of one accumulator buffer
 constexpr int kLpStages = 6;
 constexpr int kLpGroupM = 8;
 constexpr int kLpABytes = kLpBM * kLpBK * 2;
 constexpr int kLpBBytes = kLpBNh * kLpBK * 2;
 constexpr int kLpStageBytes = kLpABytes + kLpBBytes;
-constexpr int kLpStoreBytes = 4 * 2 * 4096;                              // two staging boxes of 128 bytes x 32 rows for each epilogue warp
+constexpr int kLpStoreBytes = 8 * 4096;                                  // a staging box of 128 bytes x 32 rows for each epilogue warp
 constexpr int kLpSmem = kLpStages * kLpStageBytes + kLpStoreBytes + 256 + 1024;
 static_assert(kLpSmem <= 232448, "227 KB");
 static_assert(kLpSmem >= kTmemClusterAlone, "a pair holds all tensor memory: no block of another cluster beside it (host.h)");
@@ -218,15 +218,14 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       }
     }
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int quad = warp & 3;
-    int local = 0;
+    // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    const int quad = warp & 3, buf = warp < 6 ? 0 : 1;
+    int local = buf;
     bool ok = true;
-    int out_buf = 0;           // staging box of this warp's next store
     // one box of 128 bytes x 32 rows: `v` is this lane's row of it
     auto store_box = [&](const uint32_t (&v)[32], int col, int row, bool add) {
-      uint8_t* box = ring + ((warp - 2) * 2 + out_buf) * 4096;
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the store before the last one has read its box
+      uint8_t* box = ring + (warp - 2) * 4096;
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the store before has read it
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -238,13 +237,11 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         else tma_store_2d(&tmC, box, col, row);
         tma_store_commit();
       }
-      out_buf ^= 1;
     };
-    for (int unit = pair; unit < units && ok; unit += n_pairs, ++local) {
+    for (int unit = pair + buf * n_pairs; unit < units && ok; unit += 2 * n_pairs, local += 2) {
       int mb, nb, side;
       tile_coords(unit_tile(unit, side), mb, nb);
       const int col_base = nb * kLpBN + (side > 0 ? kLpBNh : 0), parts = side < 0 ? 2 : 1;      // of 128 columns
-      const int buf = local & 1;
       const uint32_t acc_phase = (local >> 1) & 1;
       const int row_w = mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
       const int row = row_w + lane;
