@@ -1129,7 +1129,7 @@ PyObject* py_preference_loss(PyObject*, PyObject* const* v, Py_ssize_t n) {
 
 struct LogProbsCall {
   const Tensor* labels = nullptr;
-  long long ignore = 0, pad = 0, columns = 0, slab_bytes = 0, plane_bytes = 0;
+  long long ignore = 0, pad = 0, columns = 0, slab_bytes = 0, plane_bytes = 0, keep_width = 0;
   float tau = 1;
 };
 struct LogProbsKept {
@@ -1145,7 +1145,7 @@ LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, 
   k.y = at::empty(c.labels->sizes(), on(h, at::kFloat));
   k.dense = at::empty({(int64_t)padded, (int64_t)D}, on(h, at::kBFloat16));
   const long long slab = slab_of(padded, V, c.slab_bytes);
-  const bool keep = grad && slab >= V;
+  const bool keep = grad && slab >= V && D >= c.keep_width;
   if (keep) k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
   k.kept = at::empty({(int64_t)(5 * T + 4 + (keep ? (T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns) : 0))}, on(h, at::kInt));
   const Tensor work = at::empty({(int64_t)ksa_log_probs_work((int)T, (int)V)}, on(h, at::kFloat));
@@ -1192,7 +1192,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
   }
 };
 
-// linear_log_probs(h [..., D], w, labels [...], ignore_index, temperature, row pad, columns of a sum, slab bytes, plane bytes) -> y [...]
+// linear_log_probs(h [..., D], w, labels [...], ignore_index, temperature, row pad, columns of a sum, slab bytes, plane bytes, least width of kept logits) -> y [...]
 PyObject* py_linear_log_probs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(v, n);
@@ -1210,6 +1210,7 @@ PyObject* py_linear_log_probs(PyObject*, PyObject* const* v, Py_ssize_t n) {
   c.slab_bytes = PyLong_Check(slab) ? PyLong_AsLongLong(slab) : -1;
   c.plane_bytes = PyLong_Check(planes) ? PyLong_AsLongLong(planes) : -1;
   if (PyErr_Occurred()) { PyErr_Clear(); return none(); }
+  c.keep_width = a.integer();
   if (!a.ok() || !a.dense(w) || w.scalar_type() != at::kBFloat16 || !rows2d(&w) || !aligned(&w) || w.size(1) % 8 != 0 || w.stride(0) % 8 != 0 ||
       w.stride(0) < w.size(1) || h->dim() < 1 || h->size(-1) != w.size(1) || c.labels->sizes() != h->sizes().slice(0, h->dim() - 1) ||
       !(h->is_contiguous() || rows2d(h)) || !c.labels->is_contiguous() || !fits(w.size(0)) || c.labels->numel() > INT_MAX / 4 || !(c.tau > 0 && std::isfinite(c.tau)) ||

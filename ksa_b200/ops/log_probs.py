@@ -18,6 +18,8 @@ SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16
                             # where that is all of it, the forward pass keeps the logits in as many bytes
 
 
+KEEP_WIDTH = 1024           # least width at which it does: the product of narrower rows costs no more than keeping it (1000 rows of 256 against 151936
+                            # tokens 391 us, kept 432; of 1024 1024 to 1041 and 994 to 1030; 4915 of 2048 9.4 and 8.7 ms)
 PLANE_BYTES = 512 << 20     # and cuts the vocabulary of the rows' gradient into as many parts (at most 8) as have fp32 results of so many bytes
 
 
@@ -44,7 +46,7 @@ class _LinearLogProbsFn(torch.autograd.Function):
             count = torch.empty(1, dtype=torch.int32, device=dev)
             lse2 = torch.empty(2 * T, dtype=torch.float32, device=dev)
             codes = tops = None
-            if any(ctx.needs_input_grad[:2]) and _slab(padded, V) >= V:
+            if any(ctx.needs_input_grad[:2]) and D >= KEEP_WIDTH and _slab(padded, V) >= V:
                 codes = torch.empty((padded, _slab(padded, V)), dtype=torch.int16, device=dev)
                 tops = torch.empty(-(-T // 4) * 4 * -(-V // _STAT_COLS), dtype=torch.float32, device=dev)
             work = torch.empty(_lib.log_probs_work(T, V), dtype=torch.float32, device=dev)
@@ -103,11 +105,11 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
 
     ``hidden`` is ``[..., D]``, ``weight`` the output head ``[V, D]`` (both bf16 on a GPU, ``D`` a multiple of 8), ``labels`` ``[...]``.  Rows
     without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  Without a
-    gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where that takes at most ``SLAB_BYTES`` (4 GB: 13824 rows of
-    151936 tokens); of more the backward pass computes them again, at most 4 GB of their gradient at a time.
+    gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where the width is at least 1024 and that takes at most
+    ``SLAB_BYTES`` (4 GB: 13824 rows of 151936 tokens); else the backward pass computes them again, at most 4 GB of their gradient at a time.
     With ``main_grad`` on the weight its gradient goes there."""
     if not _observed():
-        y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES, PLANE_BYTES)
+        y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES, PLANE_BYTES, KEEP_WIDTH)
         if y is not None:
             return y
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

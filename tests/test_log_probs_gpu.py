@@ -19,6 +19,12 @@ pytestmark = pytest.mark.gpu
 IGNORE = -100
 
 
+@pytest.fixture(params=["kept", "again"], autouse=True)
+def _logits(request, monkeypatch):
+    """Every test with the logits kept for the backward pass and with them computed again, whatever the width."""
+    monkeypatch.setattr(impl, "KEEP_WIDTH", 0 if request.param == "kept" else 1 << 20)
+
+
 def _inputs(T, D, V, answer, seed=0, tau=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     w = (torch.randn(V, D, generator=g, device="cuda") * 0.05).bfloat16()
