@@ -13,8 +13,9 @@
 // memory, so that prompts and masked turns cost nothing but their labels, and what their rows hold reaches no sum.
 //
 // One kernel on CTA pairs (gemm2.cu describes its roles and barriers) serves four products, which differ in their epilogue:
-//   kStats  h w^T: every thread has one row of the tile; it takes the maximum and the sum of exponentials of 128 columns, and writes their
-//           log-sum (base 2) as one number.  A second kernel adds those of a row.
+//   kStats  h w^T: every thread has one row of the tile; it takes the maximum and the sum of exponentials of 128 columns.  A second kernel adds
+//           those of a row.  Maxima and the label's logit stay as they are, not times log2(e): y is then a difference of two numbers that
+//           were not rounded, where products of 20 would leave 1e-6.
 //   kStatsKeep  the same, and the logits in 16 bits;  kGrad  the product again, dx in bf16 from the accumulators.
 //   kDh     dx w, fp32, over the columns of one slab;  kDw  dx^T h.
 // dx exists for a slab of the vocabulary at a time (the caller says how wide): the slabs' dw are disjoint, and dh is added up in fp32.
@@ -54,8 +55,8 @@ struct LpArgs {
   const int* row_label;        // their labels
   float scale2;                // log2(e) / tau
   float inv_tau;
-  float* stats;                // kStats: [ceil(N / 128)][ld_stats] log-sums, base 2
-  float* picked;               // kStats: [rows] x of the label times log2(e)
+  float2* stats;               // kStats: [ceil(N / 128)][ld_stats] maximum m (times tau) and sum of exp(x - m / tau)
+  float* picked;               // kStats: [rows] the label's logit, times tau
   float* tops;                 // kStatsKeep: [ceil(N / 128)][ld_stats] maxima, base 2
   long long ld_stats;
   const float* lse2;           // kGrad: [rows]
@@ -80,6 +81,11 @@ __device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int 
     if (steps < least) { least = steps; best = s; }
   }
   return best;
+}
+
+// A maximum with its sum of exponentials.  The sum is of 2^(x scale2 - top), top being max scale2 rounded: what the rounding took goes into it.
+__device__ __forceinline__ float2 lp_sum(float mx, float top, float scale2, float sum) {
+  return make_float2(mx, mx == -INFINITY ? sum : sum * fast_exp2(-fmaf(mx, scale2, -top)));
 }
 
 template <int kMode>
@@ -275,7 +281,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             float x = 0.f;
 #pragma unroll
             for (int j = 0; j < kLpStatCols; ++j) x = j == at ? __uint_as_float(r[j]) : x;
-            if (at >= 0 && at < kLpStatCols) a.picked[row] = x * a.scale2;
+            if (at >= 0 && at < kLpStatCols) a.picked[row] = x;
           }
           float m[4];
 #pragma unroll
@@ -290,7 +296,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
           for (int j = 0; j < kLpStatCols; ++j) s[j & 3] += fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -top));
           const long long slot = (long long)(col / kLpStatCols) * a.ld_stats + row;
-          if (live) a.stats[slot] = top + __log2f((s[0] + s[1]) + (s[2] + s[3]));
+          if (live) a.stats[slot] = lp_sum(mx, top, a.scale2, (s[0] + s[1]) + (s[2] + s[3]));
           if (kMode == kStatsKeep) {
             if (live) a.tops[slot] = mx == -INFINITY ? mx : top;
 #pragma unroll
@@ -380,7 +386,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 // Here the weights are the 128 rows of the tensor cores' product and the activations, N of them, its columns.  Every CTA has as many weight rows
 // as the others, in steps of 8: tiles of 256 and a shorter last one, the end of which is loaded 8 rows at a time.
 // Epilogue: a thread has one weight row and N values; a warp adds up its 32 rows for every activation by exchanging halves, after which a
-// lane has one activation's maximum (or sum), and keeps it over its tiles.  A warp writes one log-sum for each activation.
+// lane has one activation's maximum (or sum), and keeps it over its tiles.  A warp writes one maximum and sum for each activation.
 constexpr int kLfThreads = 192;      // warp 0 loads, warp 1 issues products, warps 2..5 epilogue
 constexpr int kLfTile = 256;         // weight rows that share a load of the activations: two products of 128 rows
 constexpr int kLfMostRows = 128;
@@ -394,7 +400,7 @@ struct LfShape {
 template <int N>
 __global__ void __launch_bounds__(kLfThreads, 1)
 log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW8, const __grid_constant__ CUtensorMap tmH, int V,
-                     int D, int rows_of_cta, const int* count, const int* row_label, float scale2, float* stats, long long ld, float* picked, int* status) {
+                     int D, int rows_of_cta, const int* count, const int* row_label, float scale2, float2* stats, long long ld, float* picked, int* status) {
   using S = LfShape<N>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -498,7 +504,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
           float x[32], m[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            x[j] = v < v_hi ? __uint_as_float(r[j]) * scale2 : -INFINITY;
+            x[j] = v < v_hi ? __uint_as_float(r[j]) : -INFINITY;
             if (label[c * 32 + j] == v && v < v_hi) picked[c * 32 + j] = x[j];
             m[j] = x[j];
           }
@@ -510,9 +516,9 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
               const float other = __shfl_xor_sync(0xffffffffu, up ? m[j] : m[j + o], o);
               m[j] = fmaxf(up ? m[j + o] : m[j], other);
             }
-          const float top = fmaxf(run_m[c], m[0]), use = top == -INFINITY ? 0.f : top;         // of activation 32 c + lane
+          const float now = fmaxf(run_m[c], m[0]), top = now == -INFINITY ? 0.f : now * scale2;       // of activation 32 c + lane
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = fast_exp2(x[j] - __shfl_sync(0xffffffffu, use, j));
+          for (int j = 0; j < 32; ++j) x[j] = fast_exp2(fmaf(x[j], scale2, -__shfl_sync(0xffffffffu, top, j)));
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -521,8 +527,9 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
               const float other = __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + o], o);
               x[j] = (up ? x[j + o] : x[j]) + other;
             }
-          run_s[c] = run_s[c] * fast_exp2(run_m[c] - use) + x[0];                              // (0 before there is a maximum)
-          run_m[c] = top;
+          const float2 add = lp_sum(now, top, scale2, x[0]);
+          run_s[c] = run_m[c] == -INFINITY ? run_s[c] + add.y : run_s[c] * fast_exp2((run_m[c] - now) * scale2) + add.y;
+          run_m[c] = now;
         }
       }
       tc_fence_before();
@@ -531,7 +538,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     }
 #pragma unroll
     for (int c = 0; c < N / 32; ++c)
-      if (c * 32 + lane < n) stats[((long long)blockIdx.x * 4 + quad) * ld + c * 32 + lane] = (run_m[c] == -INFINITY ? 0.f : run_m[c]) + __log2f(run_s[c]);
+      if (c * 32 + lane < n) stats[((long long)blockIdx.x * 4 + quad) * ld + c * 32 + lane] = make_float2(run_m[c], run_s[c]);
   }
   tc_fence_before();
   __syncthreads();
@@ -659,38 +666,39 @@ log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int
   }
 }
 
-// y and lse2 of a row from the log-sums of its columns.  A block has kRows rows: 32 where that leaves enough blocks (a warp reads whole lines
-// then), else 8.  A thread takes kLpSumEach log-sums at a time: their maximum, then one exponential for each.
+// y and lse2 of a row from its columns' maxima and sums.  A block has kRows rows: 32 where that leaves enough blocks (a warp reads whole lines
+// then), else 8.  A thread takes kLpSumEach at a time: their maximum, then one exponential for each.
 constexpr int kLpSumEach = 8;
 template <int kRows>
 __global__ void __launch_bounds__(512)
-log_probs_sum_kernel(const float* stats, long long ld, int slots, const float* picked, const int* rows, const int* count, float* y, float* lse2,
-                     float* picked2) {
+log_probs_sum_kernel(const float2* stats, long long ld, int slots, const float* picked, const int* rows, const int* count, float scale2, float inv_tau, float* y,
+                     float* lse2, float* picked2) {
   constexpr int kThreadsOfRow = 512 / kRows, kWarps = 16;
   __shared__ float2 part[kWarps][kRows];
   grid_dependency_enter();
   const int n = *count, r = threadIdx.x % kRows, s0 = threadIdx.x / kRows, row = blockIdx.x * kRows + r;
   if ((int)blockIdx.x * kRows >= n) return;
-  float m = -INFINITY, s = 0.f;                                          // of 2^x
+  float m = -INFINITY, s = 0.f;
+  // (a sum without a maximum is 0, or what is no number)
+  auto scaled = [&](float s, float m, float top) { return m == -INFINITY ? s : s * fast_exp2((m - top) * scale2); };
   if (row < n) {
     for (int i = s0; i < slots; i += kThreadsOfRow * kLpSumEach) {
-      float x[kLpSumEach], top = m;
+      float2 x[kLpSumEach];
+      float top = m;
 #pragma unroll
-      for (int j = 0; j < kLpSumEach; ++j) x[j] = i + j * kThreadsOfRow < slots ? stats[(long long)(i + j * kThreadsOfRow) * ld + row] : -INFINITY;
+      for (int j = 0; j < kLpSumEach; ++j)
+        x[j] = i + j * kThreadsOfRow < slots ? stats[(long long)(i + j * kThreadsOfRow) * ld + row] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int j = 0; j < kLpSumEach; ++j) top = fmaxf(top, x[j]);
-      const float use = top == -INFINITY ? 0.f : top;
-      float t[2] = {s * fast_exp2(m - use), 0.f};                         // (0, before there is a maximum)
+      for (int j = 0; j < kLpSumEach; ++j) top = fmaxf(top, x[j].x);
+      s = scaled(s, m, top);
 #pragma unroll
-      for (int j = 0; j < kLpSumEach; ++j) t[j & 1] += fast_exp2(x[j] - use);
-      s = t[0] + t[1];
+      for (int j = 0; j < kLpSumEach; ++j) s += scaled(x[j].y, x[j].x, top);
       m = top;
     }
   }
-  auto add = [](float& m, float& s, float m2, float s2) {
+  auto add = [&](float& m, float& s, float m2, float s2) {
     const float top = fmaxf(m, m2);
-    const float a = m == -INFINITY ? s : s * fast_exp2(m - top), b = m2 == -INFINITY ? s2 : s2 * fast_exp2(m2 - top);      // (0, or what is no number)
-    s = a + b;
+    s = scaled(s, m, top) + scaled(s2, m2, top);
     m = top;
   };
 #pragma unroll
@@ -705,10 +713,12 @@ log_probs_sum_kernel(const float* stats, long long ld, int slots, const float* p
     s = part[0][r].y;
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) add(m, s, part[w][r].x, part[w][r].y);
-    const float l = m + __log2f(s);
-    lse2[row] = l;
-    picked2[row] = picked[row] - l;
-    y[rows[row]] = (picked[row] - l) * 0.69314718056f;
+    const float gap = picked[row] - m;                                   // (the fast logarithm is off by 2^-22 of itself)
+    const double l = log((double)s);
+    y[rows[row]] = (float)((double)gap * (double)inv_tau - l);
+    const float l2 = (float)(l * 1.4426950408889634);
+    lse2[row] = fmaf(m, scale2, l2);
+    picked2[row] = fmaf(gap, scale2, -l2);
   }
 }
 
@@ -824,7 +834,7 @@ KSA_API long long ksa_log_probs_work(int T, int V) {
   const int sms = sm_count() > 0 ? sm_count() : 1, rows = lf_rows(V, sms);
   const long long few = T <= kLfMostRows ? (V + rows - 1) / rows * 4 : 0;
   const long long slots = (V + kLpStatCols - 1) / kLpStatCols;
-  return (T + 3LL) / 4 * 4 * ((few > slots ? few : slots) + 1);
+  return (T + 3LL) / 4 * 4 * (2 * (few > slots ? few : slots) + 1);
 }
 
 // Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
@@ -843,8 +853,9 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   cudaStream_t st = ST(stream);
   const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad, slots = (V + kLpStatCols - 1) / kLpStatCols;
   const long long ld = (T + 3LL) / 4 * 4;
-  float* stats = static_cast<float*>(work);
-  float* picked = stats + ld * slots;
+  float2* stats = static_cast<float2*>(work);
+  const float scale2 = (float)(1.4426950408889634 / (double)tau);
+  float* picked = reinterpret_cast<float*>(stats + ld * slots);
   const int vec = ldh % 8 == 0 && (reinterpret_cast<uintptr_t>(h) & 15) == 0;
   const bool few = T <= kLfMostRows && codes == nullptr;
   const int columns = (T + 31) / 32 * 32;                 // of the product with few rows
@@ -865,7 +876,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   if (few) {
     const int sms = sm_count(), rows_of_cta = lf_rows(V, sms), ctas = (V + rows_of_cta - 1) / rows_of_cta;
     sums = ctas * 4;
-    picked = stats + ld * sums;
+    picked = reinterpret_cast<float*>(stats + ld * sums);
     rc = lp_map(&A, w, 2, D, V, ldw, 128);
     if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 8);
     if (rc == 0) rc = lp_map(&C, dense, 2, D, padded, D, columns);
@@ -877,7 +888,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     static PerDevice raised[4];
     KSA_CHECK_CUDA(raise_smem_limit(raised[columns / 32 - 1], kern, smem));
     KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, A, B, C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
-                                 (float)(1.4426950408889634 / (double)tau), stats, ld, picked, status));
+                                 scale2, stats, ld, picked, status));
   } else {
     rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
     if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
@@ -886,15 +897,15 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     LpArgs a{};
     a.M = T; a.N = V; a.K = D;
     a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
-    a.scale2 = (float)(1.4426950408889634 / (double)tau);
+    a.scale2 = scale2;
     a.stats = stats; a.picked = picked; a.ld_stats = ld; a.tops = static_cast<float*>(tops);
     rc = codes ? launch_log_probs<kStatsKeep>(A, B, C, a, st) : launch_log_probs<kStats>(A, B, A, a, st);
     if (rc) return rc;
   }
   const bool wide = T >= 32 * 148;
   KSA_CHECK_CUDA(launch_kernel(wide ? log_probs_sum_kernel<32> : log_probs_sum_kernel<8>, dim3(wide ? (T + 31) / 32 : (T + 7) / 8), dim3(512), 0, st,
-                               (const float*)stats, ld, sums, (const float*)picked, (const int*)rows, (const int*)count, (float*)y, (float*)lse2,
-                               (float*)lse2 + T));
+                               (const float2*)stats, ld, sums, (const float*)picked, (const int*)rows, (const int*)count, scale2, 1.f / tau, (float*)y,
+                               (float*)lse2, (float*)lse2 + T));
   return 0;
 }
 

@@ -18,8 +18,8 @@ SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16
                             # where that is all of it, the forward pass keeps the logits in as many bytes
 
 
-KEEP_WIDTH = 1024           # least width at which it does: the product of narrower rows costs no more than keeping it (1000 rows of 256 against 151936
-                            # tokens 391 us, kept 432; of 1024 1024 to 1041 and 994 to 1030; 4915 of 2048 9.4 and 8.7 ms)
+KEEP_WIDTH = 768            # least width at which it does: the product of narrower rows costs no more than keeping it (3000 rows of 256 against 151936
+                            # tokens 1017 us, kept 1141; of 512 the same; of 1024 3297 and 2839, 300 rows of 1024 478 and 406)
 PLANE_BYTES = 512 << 20     # and cuts the vocabulary of the rows' gradient into as many parts (at most 8) as have fp32 results of so many bytes
 
 
@@ -105,7 +105,7 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
 
     ``hidden`` is ``[..., D]``, ``weight`` the output head ``[V, D]`` (both bf16 on a GPU, ``D`` a multiple of 8), ``labels`` ``[...]``.  Rows
     without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  Without a
-    gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where the width is at least 1024 and that takes at most
+    gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where the width is at least 768 and that takes at most
     ``SLAB_BYTES`` (4 GB: 13824 rows of 151936 tokens); else the backward pass computes them again, at most 4 GB of their gradient at a time.
     With ``main_grad`` on the weight its gradient goes there."""
     if not _observed():
