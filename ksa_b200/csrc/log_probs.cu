@@ -32,7 +32,7 @@ constexpr int kLpBM = 128;          // rows of the tile in a CTA; a pair has 256
 constexpr int kLpBN = 256;          // columns of the tile
 constexpr int kLpBNh = 128;         // rows of B staged per CTA
 constexpr int kLpBK = 64;
-constexpr int kLpThreads = 320;     // warp 0 loads, warp 1 issues products, warps 2..5 and 6..9 epilogue, each group of one accumulator buffer
+constexpr int kLpThreads = 320;     // warp 0 loads, warp 1 issues products, warps 2..5 and 6..9 epilogue: every other tile is a group's, or half of every tile
 constexpr int kLpStages = 6;
 constexpr int kLpGroupM = 8;
 constexpr int kLpABytes = kLpBM * kLpBK * 2;
@@ -42,7 +42,12 @@ constexpr int kLpStoreBytes = 8 * 4096;                                  // a st
 constexpr int kLpSmem = kLpStages * kLpStageBytes + kLpStoreBytes + 256 + 1024;
 static_assert(kLpSmem <= 232448, "227 KB");
 static_assert(kLpSmem >= kTmemClusterAlone, "a pair holds all tensor memory: no block of another cluster beside it (host.h)");
-constexpr int kLpStatCols = 128;                                        // columns that share a log-sum
+constexpr int kLpStatCols = 128;                                        // columns that share a maximum and a sum
+// Steps of kLpBK after which a logit's partial sum leaves the tensor cores.  Their accumulators cut off what does not fit, towards zero: a logit over 2560
+// products came out 9e-7 of itself too small, and at a temperature of 0.6 y was off by 1.6e-6.  The epilogue adds the parts of 1024 products up:
+// 5e-7, for 1 % of the time (8192 x 151936 x 2048 3830 -> 3862 us; parts of 512 2.9e-7 and 3960).  An epilogue thread then keeps 128 sums in registers, so
+// that both groups of its warps share every tile; of narrower heads each takes every other tile, which costs less per tile (width 128 207 us, 235 shared).
+constexpr int kLpChunk = 16;
 constexpr float kLpCodes = 1024.f;                                      // codes of a kept logit to a power of two
 constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
 
@@ -108,9 +113,11 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   const WaitGuard guard{abort_flag, a.status};
   const int pair = (int)blockIdx.x >> 1, n_pairs = (int)gridDim.x >> 1;
 
+  const bool split = kSums && a.K > kLpChunk * kLpBK;                     // tiles in several parts of K, shared by the epilogue's two groups
+
   if (threadIdx.x == 0) {
     for (int i = 0; i < kLpStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], split ? 16 : 8); }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -198,44 +205,49 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int unit = pair; unit < units && ok; unit += n_pairs, ++local) {
+      for (int unit = pair; unit < units && ok; unit += n_pairs) {
         const uint32_t idesc = unit < halves_from ? idesc_full : idesc_half;
-        const int buf = local & 1;
-        const uint32_t acc_phase = (local >> 1) & 1;
-        if (!mbar_wait(&acc_empty[buf], acc_phase ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + buf * kLpBN;
         const int kb0 = kMode == kDh && parts_k > 1 ? unit / num_tiles * part_kb : 0, kb1 = min(kb0 + part_kb, num_kb);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+        int from = kb0;
+        do {                                                             // (once, of no steps at all, where nothing is multiplied)
+          const int to = kSums ? min(from + kLpChunk, kb1) : kb1;
+          const int buf = local & 1;
+          const uint32_t acc_phase = (local >> 1) & 1;
+          ++local;
+          if (!mbar_wait(&acc_empty[buf], acc_phase ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * kLpStageBytes);
-          const uint32_t sb = sa + kLpABytes;
+          const uint32_t d_tmem = tmem_base + buf * kLpBN;
+          for (int kb = from; kb < to; ++kb) {
+            if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + stage * kLpStageBytes);
+            const uint32_t sb = sa + kLpABytes;
 #pragma unroll
-          for (int k = 0; k < kLpBK / 16; ++k) {
-            const uint64_t da = kAMn ? smem_desc_mnmajor_sw128(sa + k * 2048, 8192) : smem_desc_kmajor_sw128(sa + k * 32);
-            const uint64_t db = kBMn ? smem_desc_mnmajor_sw128(sb + k * 2048, 8192) : smem_desc_kmajor_sw128(sb + k * 32);
-            umma2_ss(d_tmem, da, db, idesc, kb != kb0 || k != 0 ? 1u : 0u);
+            for (int k = 0; k < kLpBK / 16; ++k) {
+              const uint64_t da = kAMn ? smem_desc_mnmajor_sw128(sa + k * 2048, 8192) : smem_desc_kmajor_sw128(sa + k * 32);
+              const uint64_t db = kBMn ? smem_desc_mnmajor_sw128(sb + k * 2048, 8192) : smem_desc_kmajor_sw128(sb + k * 32);
+              umma2_ss(d_tmem, da, db, idesc, kb != from || k != 0 ? 1u : 0u);
+            }
+            umma2_commit_both(&empty[stage]);
+            if (++stage == kLpStages) { stage = 0; phase ^= 1; }
           }
-          umma2_commit_both(&empty[stage]);
-          if (++stage == kLpStages) { stage = 0; phase ^= 1; }
-        }
-        if (ok) umma2_commit_both(&acc_full[buf]);
+          if (ok) umma2_commit_both(&acc_full[buf]);
+          from = to;
+        } while (from < kb1 && ok);
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
-    const int quad = warp & 3, buf = warp < 6 ? 0 : 1;
-    int local = buf;
+    const int quad = warp & 3, group = warp < 6 ? 0 : 1;
+    int local = split ? 0 : group;
     bool ok = true;
-    // one box of 128 bytes x 32 rows: `v` is this lane's row of it
-    auto store_box = [&](const uint32_t (&v)[32], int col, int row, bool add) {
+    // One box of 128 bytes x 32 rows; `words(j)` are this lane's 16 bytes j of its row.
+    auto store_box = [&](auto&& words, int col, int row, bool add) {
       uint8_t* box = ring + (warp - 2) * 4096;
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the store before has read it
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) = words(j);
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
@@ -244,11 +256,16 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         tma_store_commit();
       }
     };
-    for (int unit = pair + buf * n_pairs; unit < units && ok; unit += 2 * n_pairs, local += 2) {
+    // one arrival per epilogue warp of either CTA on the leader's barrier: the accumulator buffer may be rewritten
+    auto arrive = [&]() {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[local & 1]), 0));
+      local += split ? 1 : 2;
+    };
+    for (int unit = split ? pair : pair + group * n_pairs; unit < units && ok; unit += split ? n_pairs : 2 * n_pairs) {
       int mb, nb, side;
       tile_coords(unit_tile(unit, side), mb, nb);
-      const int col_base = nb * kLpBN + (side > 0 ? kLpBNh : 0), parts = side < 0 ? 2 : 1;      // of 128 columns
-      const uint32_t acc_phase = (local >> 1) & 1;
       const int row_w = mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
       const int row = row_w + lane;
       const bool live = kMode == kDw || row < M;
@@ -260,18 +277,39 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         g = a.dy[a.rows[row]] * a.inv_tau;
         label -= a.col0;
       }
-      if (!mbar_wait(&acc_full[buf], acc_phase, guard, kTimeoutAccFull)) { ok = false; break; }
+      if (!mbar_wait(&acc_full[local & 1], (local >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + buf * kLpBN;
+      const int part_end = split ? group + 1 : 2;
 #pragma unroll 1
-      for (int part = 0; part < parts; ++part) {
-        const int col = col_base + part * kLpStatCols;
-        if (col >= N) break;
+      for (int part = split ? group : 0; part < part_end; ++part) {           // of 128 columns
+        const int col = nb * kLpBN + (side > 0 || part > 0 ? kLpStatCols : 0);
+        const bool work = (side < 0 || part == 0) && col < N;
+        const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (local & 1) * kLpBN + part * kLpStatCols;
         if (kSums) {
           uint32_t r[kLpStatCols];
+          if (work) {
 #pragma unroll
-          for (int i = 0; i < kLpStatCols / 32; ++i) tmem_ld32(t_row + part * kLpStatCols + i * 32, *reinterpret_cast<uint32_t(*)[32]>(r + i * 32));
-          tmem_wait_ld();
+            for (int i = 0; i < kLpStatCols / 32; ++i) tmem_ld32(t_row + i * 32, *reinterpret_cast<uint32_t(*)[32]>(r + i * 32));
+            tmem_wait_ld();
+          }
+          if (part + 1 == part_end) arrive();
+          if (split)
+            for (int from = kLpChunk; from < num_kb; from += kLpChunk) {
+              if (!mbar_wait(&acc_full[local & 1], (local >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
+              tc_fence_after();
+              if (work)
+#pragma unroll
+                for (int i = 0; i < kLpStatCols / 32; ++i) {
+                  uint32_t t[32];
+                  tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (local & 1) * kLpBN + part * kLpStatCols + i * 32, t);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) r[i * 32 + j] = __float_as_uint(__uint_as_float(r[i * 32 + j]) + __uint_as_float(t[j]));
+                }
+              arrive();
+            }
+          if (!ok) break;
+          if (!work) continue;
           if (col + kLpStatCols > N)
 #pragma unroll
             for (int j = 0; j < kLpStatCols; ++j)
@@ -299,21 +337,23 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           if (live) a.stats[slot] = lp_sum(mx, top, a.scale2, (s[0] + s[1]) + (s[2] + s[3]));
           if (kMode == kStatsKeep) {
             if (live) a.tops[slot] = mx == -INFINITY ? mx : top;
+            const float by = -kLpCodes * a.scale2, off = top * kLpCodes;
+            auto code = [&](uint32_t x) {                                // a whole number next to 2^23 has it in its low bits
+              return __float_as_uint(fminf(fmaf(__uint_as_float(x), by, off), 65535.f) + 8388608.f);
+            };
 #pragma unroll
             for (int piece = 0; piece < 2; ++piece) {
               if (col + piece * 64 >= N) break;
-              uint32_t out[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                // a whole number next to 2^23 has it in its low bits
-                const float x0 = __uint_as_float(r[piece * 64 + 2 * j]), x1 = __uint_as_float(r[piece * 64 + 2 * j + 1]), by = -kLpCodes * a.scale2;
-                const float u0 = fminf(fmaf(x0, by, top * kLpCodes), 65535.f) + 8388608.f, u1 = fminf(fmaf(x1, by, top * kLpCodes), 65535.f) + 8388608.f;
-                out[j] = __byte_perm(__float_as_uint(u0), __float_as_uint(u1), 0x5410);
-              }
-              store_box(out, col + piece * 64, row_w, false);
+              store_box([&](int j) {
+                const uint32_t* x = r + piece * 64 + 8 * j;
+                return make_uint4(__byte_perm(code(x[0]), code(x[1]), 0x5410), __byte_perm(code(x[2]), code(x[3]), 0x5410),
+                                  __byte_perm(code(x[4]), code(x[5]), 0x5410), __byte_perm(code(x[6]), code(x[7]), 0x5410));
+              }, col + piece * 64, row_w, false);
             }
           }
-        } else if (kMode == kGrad) {
+          continue;
+        }
+        if (work && kMode == kGrad) {
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece) {
             const int c = col + piece * 64;
@@ -322,7 +362,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               uint32_t r[32];
-              tmem_ld32(t_row + part * kLpStatCols + piece * 64 + half * 32, r);
+              tmem_ld32(t_row + piece * 64 + half * 32, r);
               tmem_wait_ld();
               const int at = label - c - half * 32;
               float d[32];
@@ -334,9 +374,9 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
               for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
             }
-            store_box(out, c, row_w, false);
+            store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
           }
-        } else {
+        } else if (work) {
           const bool bf = kMode == kDw && a.bf16_out;
 #pragma unroll 1
           for (int piece = 0; piece < (bf ? 2 : 4); ++piece) {
@@ -347,26 +387,25 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 uint32_t r[32];
-                tmem_ld32(t_row + part * kLpStatCols + piece * 64 + half * 32, r);
+                tmem_ld32(t_row + piece * 64 + half * 32, r);
                 tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) out[half * 16 + j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
               }
             } else {
-              tmem_ld32(t_row + part * kLpStatCols + piece * 32, out);
+              tmem_ld32(t_row + piece * 32, out);
               tmem_wait_ld();
             }
             if (kMode == kDw && num_kb == 0)                             // no rows at all: nothing was multiplied
 #pragma unroll
               for (int j = 0; j < 32; ++j) out[j] = 0u;
-            if (row_w < a.M) store_box(out, c, kMode == kDh && parts_k > 1 ? unit / num_tiles * a.plane_rows + row_w : row_w, a.add != 0);
+            if (row_w < a.M)
+              store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c,
+                        kMode == kDh && parts_k > 1 ? unit / num_tiles * a.plane_rows + row_w : row_w, a.add != 0);
           }
         }
+        if (part + 1 == part_end) arrive();
       }
-      // one arrival per epilogue warp of either CTA on the leader's barrier: this accumulator buffer may be rewritten
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
     }
     if (kMode != kStats && lane == 0) tma_store_wait0();                 // its stores have written their destination
   }
@@ -386,8 +425,8 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 // Here the weights are the 128 rows of the tensor cores' product and the activations, N of them, its columns.  Every CTA has as many weight rows
 // as the others, in steps of 8: tiles of 256 and a shorter last one, the end of which is loaded 8 rows at a time.
 // Epilogue: a thread has one weight row and N values; a warp adds up its 32 rows for every activation by exchanging halves, after which a
-// lane has one activation's maximum (or sum), and keeps it over its tiles.  A warp writes one maximum and sum for each activation.
-constexpr int kLfThreads = 192;      // warp 0 loads, warp 1 issues products, warps 2..5 epilogue
+// lane has one activation's maximum (or sum), and keeps it over its tiles.  A CTA writes one maximum and sum for each activation.
+constexpr int kLfThreads = 320;      // warp 0 loads, warp 1 issues products, warps 2..5 and 6..9 epilogue, each group of 128 weight rows
 constexpr int kLfTile = 256;         // weight rows that share a load of the activations: two products of 128 rows
 constexpr int kLfMostRows = 128;
 template <int N>
@@ -417,7 +456,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   constexpr int kCols = 4 * N <= 128 ? 128 : 4 * N <= 256 ? 256 : 512;   // two buffers of two accumulators
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 8); }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmW);
@@ -456,92 +495,111 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   } else if (warp == 1) {
     if (elect_one()) {
       constexpr uint32_t idesc = umma_idesc_bf16(128, N, 0, 0);
-      int stage = 0;
+      int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = 0; tile < tiles && ok; ++tile) {
-        const int buf = tile & 1;
         const bool both = v_hi - v_lo - tile * kLfTile > 128;
-        if (!mbar_wait(&acc_empty[buf], ((tile >> 1) & 1) ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
-        tc_fence_after();
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+        for (int from = 0; from < num_kb && ok; from += kLpChunk, ++local) {
+          const int buf = local & 1, to = min(from + kLpChunk, num_kb);
+          if (!mbar_wait(&acc_empty[buf], ((local >> 1) & 1) ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t sw = smem_u32(smem + stage * S::stage_bytes), sh = sw + kLfTile * kLpBK * 2;
+          for (int kb = from; kb < to; ++kb) {
+            if (!mbar_wait(&full[stage], phase, guard, kTimeoutTmaFull)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t sw = smem_u32(smem + stage * S::stage_bytes), sh = sw + kLfTile * kLpBK * 2;
 #pragma unroll
-          for (int k = 0; k < kLpBK / 16; ++k) {
-            const uint64_t dh = smem_desc_kmajor_sw128(sh + k * 32);
-            const uint32_t add = kb != 0 || k != 0 ? 1u : 0u;
-            umma_ss(tmem_base + buf * 2 * N, smem_desc_kmajor_sw128(sw + k * 32), dh, idesc, add);
-            if (both) umma_ss(tmem_base + buf * 2 * N + N, smem_desc_kmajor_sw128(sw + 16384 + k * 32), dh, idesc, add);
+            for (int k = 0; k < kLpBK / 16; ++k) {
+              const uint64_t dh = smem_desc_kmajor_sw128(sh + k * 32);
+              const uint32_t add = kb != from || k != 0 ? 1u : 0u;
+              umma_ss(tmem_base + buf * 2 * N, smem_desc_kmajor_sw128(sw + k * 32), dh, idesc, add);
+              if (both) umma_ss(tmem_base + buf * 2 * N + N, smem_desc_kmajor_sw128(sw + 16384 + k * 32), dh, idesc, add);
+            }
+            umma_commit(&empty[stage]);
+            if (++stage == S::stages) { stage = 0; phase ^= 1; }
           }
-          umma_commit(&empty[stage]);
-          if (++stage == S::stages) { stage = 0; phase ^= 1; }
+          if (ok) umma_commit(&acc_full[buf]);
         }
-        if (ok) umma_commit(&acc_full[buf]);
       }
     }
   } else {
-    const int quad = warp & 3;
+    const int quad = warp & 3, half = warp < 6 ? 0 : 1;
+    int local = 0;
     bool ok = true;
     float run_m[N / 32], run_s[N / 32];          // of activation 32 c + lane, over this warp's rows so far
 #pragma unroll
     for (int c = 0; c < N / 32; ++c) { run_m[c] = -INFINITY; run_s[c] = 0.f; }
     for (int tile = 0; tile < tiles && ok; ++tile) {
-      const int buf = tile & 1;
-      if (!mbar_wait(&acc_full[buf], (tile >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
-      tc_fence_after();
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const int v0 = v_lo + tile * kLfTile + half * 128 + quad * 32, v = v0 + lane;
-        if (v0 >= v_hi) break;
+      const int v0 = v_lo + tile * kLfTile + half * 128 + quad * 32, v = v0 + lane;
+      float acc[N];
 #pragma unroll
-        for (int c = 0; c < N / 32; ++c) {
-          if (c * 32 >= n) break;
-          uint32_t r[32];
-          tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + (buf * 2 + half) * N + c * 32, r);
-          tmem_wait_ld();
-          float x[32], m[32];
+      for (int j = 0; j < N; ++j) acc[j] = 0.f;
+      for (int from = 0; from < num_kb; from += kLpChunk, ++local) {
+        if (!mbar_wait(&acc_full[local & 1], (local >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
+        tc_fence_after();
+        if (v0 < v_hi)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            x[j] = v < v_hi ? __uint_as_float(r[j]) : -INFINITY;
-            if (label[c * 32 + j] == v && v < v_hi) picked[c * 32 + j] = x[j];
-            m[j] = x[j];
+          for (int c = 0; c < N / 32; ++c) {
+            uint32_t r[32];
+            tmem_ld32(tmem_base + ((uint32_t)(quad * 32) << 16) + ((local & 1) * 2 + half) * N + c * 32, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[c * 32 + j] += __uint_as_float(r[j]);
           }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)             // lanes with bit o keep the upper half of what is left
-#pragma unroll
-            for (int j = 0; j < o; ++j) {
-              const bool up = lane & o;
-              const float other = __shfl_xor_sync(0xffffffffu, up ? m[j] : m[j + o], o);
-              m[j] = fmaxf(up ? m[j + o] : m[j], other);
-            }
-          const float now = fmaxf(run_m[c], m[0]), top = now == -INFINITY ? 0.f : now * scale2;       // of activation 32 c + lane
-#pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = fast_exp2(fmaf(x[j], scale2, -__shfl_sync(0xffffffffu, top, j)));
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-            for (int j = 0; j < o; ++j) {
-              const bool up = lane & o;
-              const float other = __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + o], o);
-              x[j] = (up ? x[j + o] : x[j]) + other;
-            }
-          const float2 add = lp_sum(now, top, scale2, x[0]);
-          run_s[c] = run_m[c] == -INFINITY ? run_s[c] + add.y : run_s[c] * fast_exp2((run_m[c] - now) * scale2) + add.y;
-          run_m[c] = now;
-        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[local & 1]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
-    }
+      if (!ok || v0 >= v_hi) continue;
 #pragma unroll
-    for (int c = 0; c < N / 32; ++c)
-      if (c * 32 + lane < n) stats[((long long)blockIdx.x * 4 + quad) * ld + c * 32 + lane] = make_float2(run_m[c], run_s[c]);
+      for (int c = 0; c < N / 32; ++c) {
+        if (c * 32 >= n) break;
+        float x[32], m[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          x[j] = v < v_hi ? acc[c * 32 + j] : -INFINITY;
+          if (label[c * 32 + j] == v && v < v_hi) picked[c * 32 + j] = x[j];
+          m[j] = x[j];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)             // lanes with bit o keep the upper half of what is left
+#pragma unroll
+          for (int j = 0; j < o; ++j) {
+            const bool up = lane & o;
+            const float other = __shfl_xor_sync(0xffffffffu, up ? m[j] : m[j + o], o);
+            m[j] = fmaxf(up ? m[j + o] : m[j], other);
+          }
+        const float now = fmaxf(run_m[c], m[0]), top = now == -INFINITY ? 0.f : now * scale2;       // of activation 32 c + lane
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = fast_exp2(fmaf(x[j], scale2, -__shfl_sync(0xffffffffu, top, j)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int j = 0; j < o; ++j) {
+            const bool up = lane & o;
+            const float other = __shfl_xor_sync(0xffffffffu, up ? x[j] : x[j + o], o);
+            x[j] = (up ? x[j + o] : x[j]) + other;
+          }
+        const float2 add = lp_sum(now, top, scale2, x[0]);
+        run_s[c] = run_m[c] == -INFINITY ? run_s[c] + add.y : run_s[c] * fast_exp2((run_m[c] - now) * scale2) + add.y;
+        run_m[c] = now;
+      }
+    }
+    // (the stages are free: every product has been waited for)
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) reinterpret_cast<float2*>(smem)[(half * 4 + quad) * N + c * 32 + lane] = make_float2(run_m[c], run_s[c]);
   }
   tc_fence_before();
   __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kLfThreads) {
+    float m = -INFINITY, s = 0.f;
+    for (int w = 0; w < 8; ++w) m = fmaxf(m, reinterpret_cast<const float2*>(smem)[w * N + i].x);
+    for (int w = 0; w < 8; ++w) {
+      const float2 x = reinterpret_cast<const float2*>(smem)[w * N + i];
+      s += x.x == -INFINITY ? x.y : x.y * fast_exp2((x.x - m) * scale2);
+    }
+    stats[blockIdx.x * ld + i] = make_float2(m, s);
+  }
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kCols);
@@ -832,7 +890,7 @@ static int lf_rows(int V, int sms) {
 // fp32 values of workspace for the forward pass
 KSA_API long long ksa_log_probs_work(int T, int V) {
   const int sms = sm_count() > 0 ? sm_count() : 1, rows = lf_rows(V, sms);
-  const long long few = T <= kLfMostRows ? (V + rows - 1) / rows * 4 : 0;
+  const long long few = T <= kLfMostRows ? (V + rows - 1) / rows : 0;
   const long long slots = (V + kLpStatCols - 1) / kLpStatCols;
   return (T + 3LL) / 4 * 4 * (2 * (few > slots ? few : slots) + 1);
 }
@@ -875,7 +933,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   int rc, sums = slots;
   if (few) {
     const int sms = sm_count(), rows_of_cta = lf_rows(V, sms), ctas = (V + rows_of_cta - 1) / rows_of_cta;
-    sums = ctas * 4;
+    sums = ctas;
     picked = reinterpret_cast<float*>(stats + ld * sums);
     rc = lp_map(&A, w, 2, D, V, ldw, 128);
     if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 8);
