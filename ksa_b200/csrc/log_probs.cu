@@ -49,6 +49,9 @@ constexpr int kLpStatCols = 128;                                        // colum
 // that both groups of its warps share every tile; of narrower heads each takes every other tile, which costs less per tile (width 128 207 us, 235 shared).
 constexpr int kLpChunk = 16;
 constexpr float kLpCodes = 1024.f;                                      // codes of a kept logit to a power of two
+// Pitches of the arrays that are made here, in elements: rows that begin on 128 bytes are loaded in whole lines.  A width of 1352 as pitch took a third
+// of the loads' rate (1146 rows against 49042 tokens 150 us).
+__host__ __device__ constexpr long long lp_pitch(long long n) { return (n + 63) / 64 * 64; }
 constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
 
 enum LpMode : int { kStats = 0, kGrad = 1, kDh = 2, kDw = 3, kStatsKeep = 4 };
@@ -76,16 +79,31 @@ struct LpArgs {
 
 // Parts that kDh cuts K (the vocabulary) into: its tiles are few and long, 160 for 4915 rows of 2048 on 74 pairs, and the last wave of whole ones would be
 // a third of the time (2594 us; in parts 2200).  Every part has an output of its own, which the scattering kernel adds up in order.  The rule takes the fewest
-// steps of kLpBK on the busiest pair, a part costing some 10 more for its output.
+// steps of kLpBK on the busiest pair, a part costing some 10 more for its output and each of its tiles 0.13 to be read again.  By every warp, whose lanes try two numbers each (one after the other by
+// every thread they took 14 us).
 __device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int most) {
+  if (most <= 1 || num_kb <= 0 || tiles >= 64 * n_pairs) return 1;
+  const int lane = threadIdx.x & 31;
+  float least = INFINITY;
   int best = 1;
-  const int last = tiles % n_pairs;
-  long long least = (long long)(tiles / n_pairs) * (num_kb + 10) + (last == 0 ? 0 : 2 * last <= n_pairs ? (num_kb * 5 + 7) / 8 + 10 : num_kb + 10);
-  for (int s = 2; s <= most && num_kb / s >= 8; ++s) {
-    const long long steps = ((long long)tiles * s + n_pairs - 1) / n_pairs * ((num_kb + s - 1) / s + 10);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 1 + 32 * i;
+    if (s > most || (s > 1 && num_kb / s < 8)) continue;
+    const int last = tiles % n_pairs;
+    const float whole = (float)(num_kb + 10);
+    const float steps = s > 1 ? (float)((tiles * s + n_pairs - 1) / n_pairs) * (float)((num_kb + s - 1) / s + 10) + 0.13f * (float)(tiles * s)
+                              : (float)(tiles / n_pairs) * whole + (last == 0 ? 0.f : 2 * last <= n_pairs ? 0.6f * whole : whole);
     if (steps < least) { least = steps; best = s; }
   }
-  return best;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float steps = __shfl_xor_sync(0xffffffffu, least, o);
+    const int s = __shfl_xor_sync(0xffffffffu, best, o);
+    if (steps < least || (steps == least && s < best)) { least = steps; best = s; }
+  }
+  const int part = (num_kb + best - 1) / best;
+  return (num_kb + part - 1) / part;                                     // (rounding up may leave fewer parts than asked for; none is empty)
 }
 
 // A maximum with its sum of exponentials.  The sum is of 2^(x scale2 - top), top being max scale2 rounded: what the rounding took goes into it.
@@ -239,6 +257,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
     const int quad = warp & 3, group = warp < 6 ? 0 : 1;
+    const int dx_rows = (M + kLpBK - 1) / kLpBK * kLpBK;                 // that kDw reads
     int local = split ? 0 : group;
     bool ok = true;
     // One box of 128 bytes x 32 rows; `words(j)` are this lane's 16 bytes j of its row.
@@ -344,7 +363,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
             for (int piece = 0; piece < 2; ++piece) {
               if (col + piece * 64 >= N) break;
-              store_box([&](int j) {
+              if (row_w < M) store_box([&](int j) {
                 const uint32_t* x = r + piece * 64 + 8 * j;
                 return make_uint4(__byte_perm(code(x[0]), code(x[1]), 0x5410), __byte_perm(code(x[2]), code(x[3]), 0x5410),
                                   __byte_perm(code(x[4]), code(x[5]), 0x5410), __byte_perm(code(x[6]), code(x[7]), 0x5410));
@@ -374,7 +393,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
               for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
             }
-            store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
+            if (row_w < dx_rows) store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
           }
         } else if (work) {
           const bool bf = kMode == kDw && a.bf16_out;
@@ -700,7 +719,7 @@ log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignor
 #pragma unroll
         for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[c + j];
     }
-    *reinterpret_cast<BF8*>(dense + (long long)at * D + c) = v;
+    *reinterpret_cast<BF8*>(dense + at * lp_pitch(D) + c) = v;
   }
 }
 
@@ -720,7 +739,7 @@ log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int
 #pragma unroll
         for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[j];
     }
-    *reinterpret_cast<BF8*>(dense + i * 8) = v;
+    *reinterpret_cast<BF8*>(dense + row * lp_pitch(D) + c) = v;
   }
 }
 
@@ -824,26 +843,41 @@ log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* top
   }
 }
 
-// dh[t] = the gathered gradient of row t in bf16, its parts added up, and 0 without a label.  A warp has a row.
+// dh[t] = the gathered gradient of row t in bf16, its parts added up in order, and 0 without a label.  A thread has 4 columns of a row; kSplit threads
+// share them where there are few values and may be many parts (one row in 64 parts 39 us by one thread each, 6 by 8; 4915 rows in 6 parts 54 and 124).
+template <int kSplit>
 __global__ void __launch_bounds__(256)
 log_probs_scatter_kernel(const float* dense, const int* place, const int* count, bf16* dh, int T, int D, int num_kb, int n_pairs, int planes, long long plane) {
+  __shared__ float4 sums[kSplit][256 / kSplit];
   grid_dependency_enter();
-  const int lane = threadIdx.x & 31, tiles = (min(*count, T) + 2 * kLpBM - 1) / (2 * kLpBM) * ((D + kLpBN - 1) / kLpBN);
-  const int parts = tiles > 0 ? lp_parts(tiles, num_kb, n_pairs, planes) : 0;
-  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < T; t += gridDim.x * 8) {
-    const int i = place[t];
-    for (int c = lane * 8; c < D; c += 256) {
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (i >= 0) {
-        const float* from = dense + (long long)i * D + c;
-#pragma unroll 4
-        for (int p = 0; p < parts; ++p, from += plane) {
-          const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
-          f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w; f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
-        }
+  const int tiles = (min(*count, T) + 2 * kLpBM - 1) / (2 * kLpBM) * ((D + kLpBN - 1) / kLpBN);
+  const int parts = tiles > 0 ? lp_parts(tiles, num_kb, n_pairs, planes) : 0, per_row = D / 4;
+  const int lane = threadIdx.x % (256 / kSplit), first = threadIdx.x / (256 / kSplit);
+  const long long all = (long long)T * per_row;
+  for (long long i0 = blockIdx.x * (256LL / kSplit); i0 < all; i0 += gridDim.x * (256LL / kSplit)) {
+    const long long i = i0 + lane;
+    const int t = (int)(i / per_row), c = (int)(i - (long long)t * per_row) * 4, at = i < all ? place[t] : -1;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0) {
+      const float* from = dense + (long long)at * D + c;
+#pragma unroll 8
+      for (int p = first; p < parts; p += kSplit) {
+        const float4 u = *reinterpret_cast<const float4*>(from + p * plane);
+        f.x += u.x; f.y += u.y; f.z += u.z; f.w += u.w;
       }
-      store8(dh + (long long)t * D + c, f);
     }
+    if (kSplit > 1) {
+      __syncthreads();
+      sums[first][lane] = f;
+      __syncthreads();
+      if (first != 0) continue;
+#pragma unroll
+      for (int p = 1; p < kSplit; ++p) {
+        const float4 u = sums[p][lane];
+        f.x += u.x; f.y += u.y; f.z += u.z; f.w += u.w;
+      }
+    }
+    if (i < all) *reinterpret_cast<uint2*>(dh + i * 4) = make_uint2(pack_bf16x2(f.x, f.y), pack_bf16x2(f.z, f.w));
   }
 }
 
@@ -896,8 +930,8 @@ KSA_API long long ksa_log_probs_work(int T, int V) {
 }
 
 // Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
-// Leaves what the backward pass needs: dense [T rounded up to 256, D] bf16, rows, row_label, place [T], count [1] int32, lse2 [2 T] (the log-sums
-// and the labels' logits less those, base 2), and where codes is not null the logits in 16 bits, codes [T rounded up to 256, V rounded up to 8]
+// Leaves what the backward pass needs: dense [T rounded up to 256, D rounded up to 64] bf16, rows, row_label, place [T], count [1] int32, lse2 [2 T] (the log-sums
+// and the labels' logits less those, base 2), and where codes is not null the logits in 16 bits, codes [T rounded up to 256, V rounded up to 64]
 // with tops, fp32 [ceil(V / 128) times T rounded up to 4].
 // work: fp32 [ksa_log_probs_work(T, V)].  y [T] fp32.
 KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
@@ -937,7 +971,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     picked = reinterpret_cast<float*>(stats + ld * sums);
     rc = lp_map(&A, w, 2, D, V, ldw, 128);
     if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 8);
-    if (rc == 0) rc = lp_map(&C, dense, 2, D, padded, D, columns);
+    if (rc == 0) rc = lp_map(&C, dense, 2, D, padded, lp_pitch(D), columns);
     if (rc) return rc;
     int* status = status_word();
     KSA_REQUIRE(status != nullptr, "could not allocate the status word");
@@ -948,9 +982,9 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, A, B, C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
                                  scale2, stats, ld, picked, status));
   } else {
-    rc = lp_map(&A, dense, 2, D, padded, D, kLpBM);
+    rc = lp_map(&A, dense, 2, D, padded, lp_pitch(D), kLpBM);
     if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
-    if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, (V + 7LL) / 8 * 8, 32);
+    if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, lp_pitch(V), 32);
     if (rc) return rc;
     LpArgs a{};
     a.M = T; a.N = V; a.K = D;
@@ -968,8 +1002,8 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
 }
 
 // Backward.  dy [T] fp32; dh [T, D] bf16 or null; dw [V, D] (row pitch lddw) or null, bf16 or (dw_fp32) fp32, there with add_dw added to.
-// dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8; with codes: V rounded up to 8).
-// dh32: fp32 [planes, T rounded up to 256, D] where dh is wanted, 1 to 8 planes, only one where not all columns are taken at a time.
+// dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8; with codes: V rounded up to 64).
+// dh32: fp32 [planes, T rounded up to 256, D] where dh is wanted, 1 to 64 planes, only one where not all columns are taken at a time.
 KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
                               const void* lse2, const void* codes, const void* tops, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
                               long long lddw, int dw_fp32, int add_dw, int slab, int planes, float tau, void* stream) {
@@ -977,15 +1011,15 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
   KSA_REQUIRE(T > 0 && V > 0 && D > 0 && D % 8 == 0 && ldw % 8 == 0, "log_probs: backward of %d x %d x %d", T, V, D);
   KSA_REQUIRE(!dw || lddw % (dw_fp32 ? 4 : 8) == 0, "log_probs: the pitch %lld of the weights' gradient keeps no alignment of 16 bytes", lddw);
   KSA_REQUIRE(slab > 0 && slab % 8 == 0, "log_probs: %d columns at a time (a multiple of 8)", slab);
-  KSA_REQUIRE(planes >= 1 && planes <= 8 && (planes == 1 || slab >= V), "log_probs: %d planes", planes);
-  KSA_REQUIRE(!codes || (tops && slab == (V + 7) / 8 * 8), "log_probs: kept logits are taken all at a time");
+  KSA_REQUIRE(planes >= 1 && planes <= 64 && (planes == 1 || slab >= V), "log_probs: %d planes", planes);
+  KSA_REQUIRE(!codes || (tops && slab == lp_pitch(V)), "log_probs: kept logits are taken all at a time");
   KSA_REQUIRE(!(add_dw && !dw_fp32), "log_probs: only an fp32 gradient is added to");
   KSA_REQUIRE(!dh || (reinterpret_cast<uintptr_t>(dh) & 15) == 0, "log_probs: the gradient of the rows must be 16-byte aligned");
   cudaStream_t st = ST(stream);
   const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad;
   CUtensorMap denseK, denseM;
-  int rc = lp_map(&denseK, dense, 2, D, padded, D, kLpBM);
-  if (rc == 0) rc = lp_map(&denseM, dense, 2, D, padded, D, 64);
+  int rc = lp_map(&denseK, dense, 2, D, padded, lp_pitch(D), kLpBM);
+  if (rc == 0) rc = lp_map(&denseM, dense, 2, D, padded, lp_pitch(D), 64);
   for (long long v0 = 0; v0 < V && rc == 0; v0 += slab) {
     const int n = V - v0 < slab ? (int)(V - v0) : slab;
     const bf16* wv = static_cast<const bf16*>(w) + v0 * ldw;
@@ -1023,9 +1057,12 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
   }
   if (rc) return rc;
   if (dh) {
-    const int blocks = (T + 7) / 8 < 148 * 8 ? (T + 7) / 8 : 148 * 8;
-    KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, log_probs_scatter_kernel, dim3(blocks), dim3(256), 0, st, (const float*)dh32, (const int*)place,
-                                        (const int*)count, (bf16*)dh, T, D, (int)(((V < slab ? V : slab) + kLpBK - 1) / kLpBK), lp_pairs(lp_tiles(T, D), planes, sm_count()), planes,
+    const int split = planes > 8 && (long long)T * (D / 4) < 148 * 1024 ? 8 : 1;
+    const long long blocks = ((long long)T * (D / 4) * split + 255) / 256;
+    KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, split > 1 ? log_probs_scatter_kernel<8> : log_probs_scatter_kernel<1>,
+                                        dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const float*)dh32, (const int*)place,
+                                        (const int*)count, (bf16*)dh, T, D, (int)(((V < slab ? V : slab) + kLpBK - 1) / kLpBK),
+                                        lp_pairs(lp_tiles(T, D), planes, sm_count()), planes,
                                         (long long)padded * D));
   }
   return 0;

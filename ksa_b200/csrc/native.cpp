@@ -1137,13 +1137,13 @@ struct LogProbsKept {
 };
 // Columns of the vocabulary that the backward pass takes at a time (_slab in ops/log_probs.py).
 long long slab_of(long long padded, long long V, long long bytes) {
-  return std::min((V + 7) / 8 * 8, std::max(256ll, bytes / (2 * padded) / 256 * 256));
+  return std::min((V + 63) / 64 * 64, std::max(256ll, bytes / (2 * padded) / 256 * 256));
 }
 LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, bool grad) {
   const long long T = c.labels->numel(), V = w.size(0), D = w.size(1), padded = (T + c.pad - 1) / c.pad * c.pad;
   LogProbsKept k;
   k.y = at::empty(c.labels->sizes(), on(h, at::kFloat));
-  k.dense = at::empty({(int64_t)padded, (int64_t)D}, on(h, at::kBFloat16));
+  k.dense = at::empty({(int64_t)padded, (int64_t)((D + 63) / 64 * 64)}, on(h, at::kBFloat16));
   const long long slab = slab_of(padded, V, c.slab_bytes);
   const bool keep = grad && slab >= V && D >= c.keep_width;
   if (keep) k.codes = at::empty({(int64_t)padded, (int64_t)slab}, on(h, at::kShort));
@@ -1176,7 +1176,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
     const long long slab = codes.defined() ? codes.size(1) : slab_of(padded, V, ctx->saved_data["slab_bytes"].toInt());
     const Tensor dx = at::empty({(int64_t)padded, (int64_t)slab}, on(w, at::kBFloat16));
     Tensor dh, dh32, dw;
-    const long long planes = slab < V ? 1 : std::max(1ll, std::min(8ll, (long long)ctx->saved_data["plane_bytes"].toInt() / (4 * padded * D)));
+    const long long planes = slab < V ? 1 : std::max(1ll, std::min(64ll, (long long)ctx->saved_data["plane_bytes"].toInt() / (4 * padded * D)));
     if (need_h) {
       dh = at::empty(ctx->saved_data["shape"].toIntVector(), on(w, at::kBFloat16));
       dh32 = at::empty({(int64_t)planes, (int64_t)padded, (int64_t)D}, on(w, at::kFloat));

@@ -20,16 +20,21 @@ SLAB_BYTES = 4 << 30        # the backward pass holds the logits' gradient (bf16
 
 KEEP_WIDTH = 768            # least width at which it does: the product of narrower rows costs no more than keeping it (3000 rows of 256 against 151936
                             # tokens 1017 us, kept 1141; of 512 the same; of 1024 3297 and 2839, 300 rows of 1024 478 and 406)
-PLANE_BYTES = 512 << 20     # and cuts the vocabulary of the rows' gradient into as many parts (at most 8) as have fp32 results of so many bytes
+PLANE_BYTES = 512 << 20     # and cuts the vocabulary of the rows' gradient into as many parts (at most 64) as have fp32 results of so many bytes
+
+
+def _pitch(n: int) -> int:
+    """Elements from row to row of what the kernels make for themselves (``lp_pitch``)."""
+    return -(-n // 64) * 64
 
 
 def _planes(padded: int, D: int) -> int:
-    return max(1, min(8, PLANE_BYTES // (4 * padded * D)))
+    return max(1, min(64, PLANE_BYTES // (4 * padded * D)))
 
 
 def _slab(padded: int, V: int) -> int:
     """Columns of the vocabulary that the backward pass takes at a time."""
-    return min(-(-V // 8) * 8, max(256, SLAB_BYTES // (2 * padded) // 256 * 256))
+    return min(_pitch(V), max(256, SLAB_BYTES // (2 * padded) // 256 * 256))
 
 
 class _LinearLogProbsFn(torch.autograd.Function):
@@ -41,7 +46,7 @@ class _LinearLogProbsFn(torch.autograd.Function):
         with torch.cuda.device(dev):
             y = torch.empty(T, dtype=torch.float32, device=dev)
             padded = -(-T // _ROW_PAD) * _ROW_PAD
-            dense = torch.empty((padded, D), dtype=h.dtype, device=dev)
+            dense = torch.empty((padded, _pitch(D)), dtype=h.dtype, device=dev)
             rows, row_label, place = torch.empty((3, T), dtype=torch.int32, device=dev).unbind()
             count = torch.empty(1, dtype=torch.int32, device=dev)
             lse2 = torch.empty(2 * T, dtype=torch.float32, device=dev)
@@ -70,8 +75,8 @@ class _LinearLogProbsFn(torch.autograd.Function):
             dx = torch.empty((dense.shape[0], codes.shape[1] if codes is not None else _slab(dense.shape[0], V)), dtype=w.dtype, device=dev)
             if need_h:
                 dh = torch.empty((T, D), dtype=w.dtype, device=dev)
-                planes = _planes(*dense.shape) if dx.shape[1] >= V else 1
-                dh32 = torch.empty((planes, *dense.shape), dtype=torch.float32, device=dev)
+                planes = _planes(dense.shape[0], D) if dx.shape[1] >= V else 1
+                dh32 = torch.empty((planes, dense.shape[0], D), dtype=torch.float32, device=dev)
 
             def run(out, add):
                 _lib.call("ksa_log_probs_bwd", dense, weight, rows, row_label, place, count, lse2, codes, tops, dy, dx, dh32, dh, out, T, V, D,

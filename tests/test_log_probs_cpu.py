@@ -59,5 +59,5 @@ def test_slabs_cover_the_vocabulary_in_multiples():
     for rows in (256, 512, 8192, 32768, 1 << 20, 1 << 24):
         for V in (1, 7, 255, 256, 4096, 151936):
             slab = impl._slab(rows, V)
-            assert slab % 8 == 0 and (slab >= V or slab % 256 == 0) and slab <= -(-V // 8) * 8
+            assert slab % 64 == 0 and (slab >= V or slab % 256 == 0) and slab <= -(-V // 64) * 64
             assert 2 * rows * slab <= max(impl.SLAB_BYTES, 2 * rows * 256)
