@@ -167,11 +167,11 @@ __device__ __forceinline__ NormAndFactor grad_factor(const double* partial, int 
   return r;
 }
 
-__global__ void __launch_bounds__(1024) grad_factor_kernel(const double* partial, int parts, float scale, float most, float* result) {
+__global__ void __launch_bounds__(1024) grad_factor_kernel(const double* partial, int parts, float scale, float most, float* norm, float* factor) {
   __shared__ double red[32];
   grid_dependency_enter();
   const NormAndFactor r = grad_factor(partial, parts, scale, most, red);
-  if (threadIdx.x == 0) { result[0] = r.norm; result[1] = r.factor; }
+  if (threadIdx.x == 0) { *norm = r.norm; *factor = r.factor; }
 }
 
 template <int TYPE>
@@ -213,11 +213,11 @@ __device__ __forceinline__ void grad_clip_chunk(const GradChunk& g, float factor
 // The chunks from the last one on: what the norm has read last is still in the L2.
 template <int N>
 __global__ void __launch_bounds__(kGnThreads)
-grad_clip_kernel(const __grid_constant__ GradTable<N> table, const double* partial, int parts, float scale, float most, float* result) {
+grad_clip_kernel(const __grid_constant__ GradTable<N> table, const double* partial, int parts, float scale, float most, float* norm, float* factor) {
   __shared__ double red[32];
   grid_dependency_enter();
   const NormAndFactor r = grad_factor(partial, parts, scale, most, red);
-  if (blockIdx.x == 0 && threadIdx.x == 0) { result[0] = r.norm; result[1] = r.factor; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) { *norm = r.norm; *factor = r.factor; }
   const int chunks = table.begin[table.tensors];
   for (int c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
     const GradChunk g = grad_chunk(table, c);
@@ -248,7 +248,7 @@ static long long fill_table(GradTable<N>& t, const void* const* src, void* const
 
 template <int N>
 static int grad_norm_group(const void* const* src, void* const* dst, const long long* meta, int count, double* partial, int parts, int blocks_most,
-                           float scale, float most, float* result, int* blocks, cudaStream_t st) {
+                           float scale, float most, float* norm, float* factor, int* blocks, cudaStream_t st) {
   GradTable<N> t;
   const long long chunks = fill_table(t, src, dst, meta, count);
   KSA_REQUIRE(chunks >= 0, "grad_norm: too many values for one call");
@@ -258,7 +258,7 @@ static int grad_norm_group(const void* const* src, void* const* dst, const long 
     KSA_CHECK_CUDA(launch_stream_kernel(chunks * kGnChunk, grad_norm_kernel<N>, dim3(grid), dim3(kGnThreads), 0, st, t, partial));
   } else {
     KSA_CHECK_CUDA(launch_stream_kernel(chunks * kGnChunk, grad_clip_kernel<N>, dim3(grid), dim3(kGnThreads), 0, st, t, (const double*)partial, parts,
-                                        scale, most, result));
+                                        scale, most, norm, factor));
   }
   return 0;
 }
@@ -274,10 +274,10 @@ KSA_API int ksa_grad_norm_parts(int tensors) {
 }
 
 // src[i]: values of tensor i (meta[i] = number * 4 + type: 0 fp32, 1 bf16, 2 fp16), each aligned to its type.  dst: null for the norm alone, else
-// where the clipped values of each tensor go (src itself: in place).  result: norm, factor (fp32).  The arrays are host memory.
-KSA_API int ksa_grad_norm(const void* src, const void* dst, const void* meta, int tensors, float scale, float most, void* partial, void* result,
-                          void* stream) {
-  KSA_ENTER(result);
+// where the clipped values of each tensor go (src itself: in place).  norm, factor: fp32.  The arrays are host memory.
+KSA_API int ksa_grad_norm(const void* src, const void* dst, const void* meta, int tensors, float scale, float most, void* partial, void* norm,
+                          void* factor, void* stream) {
+  KSA_ENTER(norm);
   KSA_REQUIRE(tensors >= 0, "grad_norm: %d tensors", tensors);
   KSA_REQUIRE(scale > 0.f && isfinite(scale), "grad_norm: the scale must be a positive number");
   KSA_REQUIRE(most >= 0.f, "grad_norm: the largest norm must not be negative");
@@ -303,13 +303,14 @@ KSA_API int ksa_grad_norm(const void* src, const void* dst, const void* meta, in
       int blocks = 0;
       auto group = count <= kGnSmall ? grad_norm_group<kGnSmall> : grad_norm_group<kGnMost>;
       const int rc = group(from + i, to ? to + i : nullptr, m + i, count, pass == 0 ? parts + used : parts, used, most_blocks, scale, most,
-                           static_cast<float*>(result), pass == 0 ? &blocks : nullptr, st);
+                           static_cast<float*>(norm), static_cast<float*>(factor), pass == 0 ? &blocks : nullptr, st);
       if (rc) return rc;
       used += blocks;
       i += count;
     } while (i < tensors);
   }
   if (!to)
-    KSA_CHECK_CUDA(launch_kernel(grad_factor_kernel, dim3(1), dim3(1024), 0, st, (const double*)parts, used, scale, most, static_cast<float*>(result)));
+    KSA_CHECK_CUDA(launch_kernel(grad_factor_kernel, dim3(1), dim3(1024), 0, st, (const double*)parts, used, scale, most, static_cast<float*>(norm),
+                                 static_cast<float*>(factor)));
   return 0;
 }

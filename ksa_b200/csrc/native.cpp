@@ -101,8 +101,8 @@ int ksa_summary_attn_bwd(const void* q, const void* k, const void* v, const void
                          int chunk, int n_sum, int chunk0, int k_off, int s_off, float scale, const void* part_k,
                          const void* part_v, int n_keys, void* stream);
 int ksa_grad_norm_parts(int tensors);
-int ksa_grad_norm(const void* src, const void* dst, const void* meta, int tensors, float scale, float most, void* partial, void* result,
-                  void* stream);
+int ksa_grad_norm(const void* src, const void* dst, const void* meta, int tensors, float scale, float most, void* partial, void* norm,
+                  void* factor, void* stream);
 long long ksa_token_loss_units(long long n, int sequences);
 int ksa_policy_loss(const void* y, const void* old, const void* ref, const void* adv, const void* mask, const void* cu, int wide, void* grad,
                     void* partial, void* inv, void* loss, void* stats, int types, long long n, int sequences, long long length,
@@ -850,12 +850,13 @@ Tensor differentiated_once(const Tensor& t) {
   return (*error)({leaf})[0];
 }
 
-// grad_norm(gradients, targets | None, clip, scale, largest norm) -> (norm, factor)
+// grad_norm(gradients, targets | None, 0: norm | 1: and factor | 2: clip, scale, largest norm) -> norm, or (norm, factor)
 PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a(v, n);
   PyObject *grads = a.next(), *out = a.next();
-  const bool clip = a.integer() != 0;
+  const long long what = a.integer();
+  const bool clip = what == 2;
   const float scale = a.real(), most = a.real();
   if (!a.ok() || !(PyList_CheckExact(grads) || PyTuple_CheckExact(grads)) || (out != Py_None && !(PyList_CheckExact(out) || PyTuple_CheckExact(out))))
     return none();
@@ -881,25 +882,29 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
     meta[i] = 4 * (long long)t->numel() + token_type(*t);
     if (!clip) continue;
     const Tensor* o = out == Py_None ? t : plain(PySequence_Fast_GET_ITEM(out, i));
-    if (!o || o->device() != t->device() || o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() || o->strides() != t->strides() ||
-        o->is_inference())
+    if (!o || o->is_inference() || (o != t && (o->device() != t->device() || o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() ||
+                                               o->strides() != t->strides())))
       return none();
     to[i] = o;
     dst[i] = o->mutable_data_ptr();
   }
   if (first->device().index() != c10::cuda::current_device()) return none();
-  if (clip) {                              // memory that is written must not be another tensor's too (in the order of most lists there is nothing to sort)
+  if (clip) {                              // memory that is written must not be another tensor's too
     struct Span { uintptr_t lo, hi; bool written; };
     std::vector<Span> spans;
-    spans.reserve(2 * count);
+    spans.reserve(out == Py_None ? count : 2 * count);
+    bool sorted = true;                    // (as the views of one buffer are)
+    const auto add = [&](uintptr_t lo, uintptr_t bytes, bool written) {
+      sorted = sorted && (spans.empty() || spans.back().lo <= lo);
+      spans.push_back({lo, lo + bytes, written});
+    };
     for (Py_ssize_t i = 0; i < count; ++i) {
-      const uintptr_t bytes = (uintptr_t)(meta[i] >> 2) * to[i]->element_size(), s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
+      const uintptr_t bytes = (uintptr_t)(meta[i] >> 2) * ((meta[i] & 3) == 0 ? 4 : 2), s = reinterpret_cast<uintptr_t>(src[i]), d = reinterpret_cast<uintptr_t>(dst[i]);
       if (bytes == 0) continue;
-      spans.push_back({d, d + bytes, true});
-      if (s != d) spans.push_back({s, s + bytes, false});
+      add(d, bytes, true);
+      if (s != d) add(s, bytes, false);
     }
-    const auto before = [](const Span& x, const Span& y) { return x.lo < y.lo; };
-    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+    if (!sorted) std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.lo < y.lo; });
     uintptr_t any = 0, written = 0;
     for (const Span& s : spans) {
       if (s.lo < (s.written ? any : written)) return none();
@@ -907,16 +912,19 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
       if (s.written) written = std::max(written, s.hi);
     }
   }
-  Tensor result;
+  Tensor norm, factor;
   {
     pybind11::gil_scoped_release no_gil;
-    const Tensor partial = at::empty({ksa_grad_norm_parts((int)count)}, on(*first, at::kDouble));
-    result = at::empty({2}, on(*first, at::kFloat));
-    LAUNCH_SEVERAL(2, ksa_grad_norm, src.data(), clip ? dst.data() : nullptr, meta.data(), (int)count, scale, most, partial.mutable_data_ptr(),
-                   result.mutable_data_ptr(), stream_of(*first));
+    const int parts = ksa_grad_norm_parts((int)count);
+    const Tensor partial = at::empty({parts + 1}, on(*first, at::kDouble));
+    norm = at::empty({}, on(*first, at::kFloat));
+    if (what == 1) factor = at::empty({}, on(*first, at::kFloat));
+    double* sums = static_cast<double*>(partial.mutable_data_ptr());
+    LAUNCH_SEVERAL(2, ksa_grad_norm, src.data(), clip ? dst.data() : nullptr, meta.data(), (int)count, scale, most, sums, norm.mutable_data_ptr(),
+                   what == 1 ? factor.mutable_data_ptr() : sums + parts, stream_of(*first));
     for (const Tensor* o : to) o->unsafeGetTensorImpl()->bump_version();
   }
-  return wrap(result.select(0, 0), result.select(0, 1));
+  return what == 1 ? wrap(norm, factor) : wrap(norm);
   END_HANDLE_TH_ERRORS
 }
 

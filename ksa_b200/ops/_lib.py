@@ -79,7 +79,7 @@ _SIGNATURES: Dict[str, Sequence] = {
     "ksa_policy_loss_bwd": [P, P, P, P, I, P, I, L, I, L, I, P],
     "ksa_preference_loss": [P, P, P, P, I, P, P, P, P, I, L, I, L, F, F, P],
     "ksa_preference_loss_bwd": [P, P, P, P, I, P, I, L, I, L, P],
-    "ksa_grad_norm": [P, P, P, I, F, F, P, P, P],
+    "ksa_grad_norm": [P, P, P, I, F, F, P, P, P, P],
     "ksa_peer_gather": [P, I, I, L, I, P, P, ctypes.c_uint, I, P],
     "ksa_peer_reduce_adamw": [P, I, I, L, L, P, P, P, P, P, F, F, F, F, F, P, P, P, ctypes.c_uint, I, P],
     "ksa_signal_set": [P, I, P, ctypes.c_uint, P],

@@ -69,17 +69,17 @@ def _collide(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor]) -> bool:
     return False
 
 
-def _launch(src: Sequence[torch.Tensor], dst: Optional[Sequence[torch.Tensor]], scale: float, most: float) -> torch.Tensor:
+def _launch(src: Sequence[torch.Tensor], dst: Optional[Sequence[torch.Tensor]], scale: float, most: float) -> Tuple[torch.Tensor, torch.Tensor]:
     device = src[0].device
     n = len(src)
     with torch.cuda.device(device):
         parts = torch.empty(_lib.grad_norm_parts(n), dtype=torch.float64, device=device)
-        result = torch.empty(2, dtype=torch.float32, device=device)
+        norm, factor = torch.empty((), dtype=torch.float32, device=device), torch.empty((), dtype=torch.float32, device=device)
         at = (ctypes.c_void_p * n)(*[t.data_ptr() for t in src])
         to = None if dst is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in dst])
         meta = (ctypes.c_longlong * n)(*[4 * t.numel() + _TYPES[t.dtype] for t in src])
-        _lib.call("ksa_grad_norm", at, to, meta, n, float(scale), float(most), parts, result)
-    return result
+        _lib.call("ksa_grad_norm", at, to, meta, n, float(scale), float(most), parts, norm, factor)
+    return norm, factor
 
 
 def grad_norm(grads: Iterable[torch.Tensor], scale: float = 1.0,
@@ -88,16 +88,16 @@ def grad_norm(grads: Iterable[torch.Tensor], scale: float = 1.0,
     clips: ``scale * min(1, max_norm / (norm + 1e-6))``."""
     grads = grads if isinstance(grads, (list, tuple)) else list(grads)
     if not _observed():
-        made = _native.grad_norm(grads, None, False, scale, math.inf if max_norm is None else max_norm)
+        made = _native.grad_norm(grads, None, 0 if max_norm is None else 1, scale, math.inf if max_norm is None else max_norm)
         if made is not None:
-            return made[0] if max_norm is None else made
+            return made
     grads = _check(grads, scale)
     most = math.inf if max_norm is None else _check_most(max_norm)
     with torch.no_grad():
         if not grads or not grads[0].is_cuda:
             norm, factor = ref.grad_norm(grads, scale, most)
         else:
-            norm, factor = _launch([g if _dense(g) else g.contiguous() for g in grads], None, scale, most).unbind()
+            norm, factor = _launch([g if _dense(g) else g.contiguous() for g in grads], None, scale, most)
     return norm if max_norm is None else (norm, factor)
 
 
@@ -108,9 +108,9 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float, scale: float
     one another are refused.  A norm that is no number makes all of them so, an infinite one makes them zero where they are finite."""
     grads = grads if isinstance(grads, (list, tuple)) else list(grads)
     if not _observed():
-        made = _native.grad_norm(grads, out, True, scale, max_norm)
+        made = _native.grad_norm(grads, out, 2, scale, max_norm)
         if made is not None:
-            return made[0]
+            return made
     grads = _check(grads, scale)
     most = _check_most(max_norm)
     to = grads if out is None else list(out)
