@@ -401,4 +401,4 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     rows = hidden[keep].float()                # (rows without a label take part in nothing, whatever they hold)
     logp = F.log_softmax(F.linear(rows, weight.float()) / temperature, dim=-1)
     out = torch.zeros(labels.shape, dtype=torch.float32, device=hidden.device)
-    return out.masked_scatter(keep, logp.gather(-1, labels[keep][:, None])[:, 0])
+    return out.masked_scatter(keep, logp.gather(-1, labels[keep].to(torch.int64)[:, None])[:, 0])

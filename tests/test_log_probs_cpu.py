@@ -27,6 +27,11 @@ def test_plain_form(rows, tau):
     assert not torch.autograd.grad(ops.linear_log_probs(h, w, labels).sum(), h)[0].reshape(-1, 16)[0].any()
 
 
+def test_labels_of_32_bits():
+    h, w, labels = _inputs(9)
+    assert torch.equal(ops.linear_log_probs(h, w, labels.int()), ops.linear_log_probs(h, w, labels))
+
+
 def test_mean_of_the_labels_is_cross_entropy():
     h, w, labels = _inputs(30)
     labels[::3] = -100

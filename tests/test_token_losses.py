@@ -291,6 +291,33 @@ def test_other_layouts(device):
     assert torch.equal(one, ops.policy_loss(y, old, rows[:, None].expand(6, 12).contiguous(), ref, mask)[0])
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_offsets_behind_the_last_token_count_as_it(device):
+    y, old, ref, a, mask, cu = (t.to(device) for t in _tokens([50, 2060, 7, 0], True, seed=12))
+    y.requires_grad_(True)
+    far = cu.clone().long()
+    far[3:] = 1 << 40
+    for f in (lambda c: ops.policy_loss(y, old, a, ref, mask, c, kl_coef=0.1, reduction="sequence"), lambda c: ops.preference_loss(y, ref, mask, c)):
+        one, two = f(cu), f(far)
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+        assert torch.equal(torch.autograd.grad(one[0], y)[0], torch.autograd.grad(two[0], y)[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_no_sequences(device):
+    """Tokens that belong to none, and no rows: no loss, and gradients of zero."""
+    y = torch.randn(10, device=device, requires_grad=True)
+    cu = torch.zeros(1, dtype=torch.int32, device=device)
+    empty = torch.randn(0, 5, device=device, requires_grad=True)
+    for reduction in ("token", "sequence"):
+        for t, c, adv in ((y, cu, torch.randn(10, device=device)), (empty, None, torch.randn(0, 5, device=device))):
+            loss, stats = ops.policy_loss(t, t.detach(), adv, cu_seqlens=c, reduction=reduction)
+            assert float(loss.detach()) == 0 and not stats.any() and not torch.autograd.grad(loss, t)[0].any()
+    for t, c in ((y, cu), (empty, None)):
+        loss, rewards = ops.preference_loss(t, None, None, c)
+        assert float(loss.detach()) == 0 and rewards.shape == (0, 2) and not torch.autograd.grad(loss, t)[0].any()
+
+
 @pytest.mark.gpu
 def test_replayed_twice_at_once_and_on_another_stream():
     y, old, ref, a, mask, cu = (t.cuda() for t in _tokens([700, 0, 5000, 33], True, 4, seed=9))
@@ -366,3 +393,22 @@ def test_refusals(device):
             ops.policy_loss(y, old.cpu(), a)
         with pytest.raises(ValueError):
             ops.preference_loss(y, ref, mask.cpu(), cu)
+
+
+@pytest.mark.gpu
+def test_transforms_meet_an_error_and_not_the_kernels():
+    """Whoever follows the calls themselves gets the autograd functions' own refusal, not numbers from a wrapper's memory."""
+    y, old, ref, a, mask, cu = (t.cuda() for t in _tokens([50, 60], True, seed=13))
+    h, w = torch.randn(110, 64, device="cuda").bfloat16(), torch.randn(30, 64, device="cuda").bfloat16()
+    labels = torch.randint(0, 30, (110,), device="cuda")
+    calls = [lambda t: ops.policy_loss(t, old, a, ref, mask, cu)[0], lambda t: ops.preference_loss(t, ref, mask, cu)[0],
+             lambda t: ops.linear_log_probs(h * t[:, None].bfloat16(), w, labels).sum()]
+    for f in calls:
+        for transformed in (torch.func.grad(f), lambda t: torch.func.vmap(f)(torch.stack([t, t])), lambda t: torch.func.jvp(f, (t,), (t,))):
+            with pytest.raises(RuntimeError):
+                transformed(y)
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+            f(torch.autograd.forward_ad.make_dual(y, torch.ones_like(y)))
+        assert torch.isfinite(f(y))                            # and the next ordinary call is one
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: ops.grad_norm([t]))(torch.randn(3, 50, device="cuda"))
