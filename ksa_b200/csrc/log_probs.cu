@@ -17,7 +17,8 @@
 //           those of a row.  Maxima and the label's logit stay as they are, not times log2(e): y is then a difference of two numbers that
 //           were not rounded, where products of 20 would leave 1e-6.
 //   kStatsKeep  the same, and the logits in 16 bits;  kGrad  the product again, dx in bf16 from the accumulators.
-//   kDh     dx w, fp32, over the columns of one slab;  kDw  dx^T h.
+//   kProducts  dx w in fp32 over the columns of one slab, and dx^T h: up to some size one launch of both, so that the many short tiles of the second fill the
+//           waves of the few long ones of the first.
 // dx exists for a slab of the vocabulary at a time (the caller says how wide): the slabs' dw are disjoint, and dh is added up in fp32.
 #include "common.cuh"
 #include "host.h"
@@ -54,10 +55,10 @@ constexpr float kLpCodes = 1024.f;                                      // codes
 __host__ __device__ constexpr long long lp_pitch(long long n) { return (n + 63) / 64 * 64; }
 constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
 
-enum LpMode : int { kStats = 0, kGrad = 1, kDh = 2, kDw = 3, kStatsKeep = 4 };
+enum LpMode : int { kStats = 0, kStatsKeep = 1, kGrad = 2, kProducts = 3 };
 
 struct LpArgs {
-  int M, N, K;                 // at most; *count stands for M, or for K in kDw
+  int M, N, K;                 // kStats, kGrad: rows (at most; *count says how many), columns, width.  kProducts: rows, width, columns of the slab
   const int* count;            // rows with a label
   const int* rows;             // their places among all rows
   const int* row_label;        // their labels
@@ -70,18 +71,25 @@ struct LpArgs {
   const float* lse2;           // kGrad: [rows]
   const float* dy;             // kGrad: gradient of y, by the rows' places
   int col0;                    // kGrad: first column of the slab
-  int add;                     // kDh, kDw: into fp32, added to what is there
-  int planes;                  // kDh: K is cut into at most so many parts, each with an output of its own
+  int dh, dw;                  // kProducts: which are wanted
+  int add_dh, add_dw;          // into fp32, added to what is there
+  int planes;                  // dh: K is cut into at most so many parts, each with an output of its own
   int plane_rows;
-  int bf16_out;                // kDw
+  int bf16_out;                // dw
   int* status;
 };
 
-// Parts that kDh cuts K (the vocabulary) into: its tiles are few and long, 160 for 4915 rows of 2048 on 74 pairs, and the last wave of whole ones would be
-// a third of the time (2594 us; in parts 2200).  Every part has an output of its own, which the scattering kernel adds up in order.  The rule takes the fewest
-// steps of kLpBK on the busiest pair, a part costing some 10 more for its output and each of its tiles 0.13 to be read again.  By every warp, whose lanes try two numbers each (one after the other by
-// every thread they took 14 us).
-__device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int most) {
+// Steps of kLpBK that a tile's output costs besides its products: of dh, fp32 with nothing to hide behind, and of dw.
+constexpr int kLpDhOutput = 10, kLpDwOutput = 4;
+// All of dw, in those steps: `n` rows of the vocabulary, of `D`, over `count` rows.
+__device__ __forceinline__ float lp_dw_steps(int n, int D, int count) {
+  return (float)((n + 2 * kLpBM - 1) / (2 * kLpBM)) * (float)((D + kLpBN - 1) / kLpBN) * (float)((count + kLpBK - 1) / kLpBK + kLpDwOutput);
+}
+// Parts that K (the vocabulary) is cut into for dh.  Its tiles are few and long, 160 for 4915 rows of 2048 on 74 pairs, and the last wave of whole ones would be
+// a third of the time (2594 us by itself, in parts 2300) where dw's tiles do not fill it.  Every part has an output of its own, which the
+// scattering kernel adds up in order.  The rule takes the fewest steps of kLpBK on the busiest pair or, if that is more, of all pairs on average with dw's
+// (`other`); a tile of a part costs 0.13 more to be read again.  By every warp, whose lanes try two numbers each.
+__device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int most, float other) {
   if (most <= 1 || num_kb <= 0 || tiles >= 64 * n_pairs) return 1;
   const int lane = threadIdx.x & 31;
   float least = INFINITY;
@@ -90,10 +98,8 @@ __device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int 
   for (int i = 0; i < 2; ++i) {
     const int s = lane + 1 + 32 * i;
     if (s > most || (s > 1 && num_kb / s < 8)) continue;
-    const int last = tiles % n_pairs;
-    const float whole = (float)(num_kb + 10);
-    const float steps = s > 1 ? (float)((tiles * s + n_pairs - 1) / n_pairs) * (float)((num_kb + s - 1) / s + 10) + 0.13f * (float)(tiles * s)
-                              : (float)(tiles / n_pairs) * whole + (last == 0 ? 0.f : 2 * last <= n_pairs ? 0.6f * whole : whole);
+    const float each = (float)((num_kb + s - 1) / s + kLpDhOutput);
+    const float steps = fmaxf((float)((tiles * s + n_pairs - 1) / n_pairs) * each, ((float)(tiles * s) * each + other) / (float)n_pairs) + 0.13f * (float)(tiles * s);
     if (steps < least) { least = steps; best = s; }
   }
 #pragma unroll
@@ -106,6 +112,82 @@ __device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int 
   return (num_kb + part - 1) / part;                                     // (rounding up may leave fewer parts than asked for; none is empty)
 }
 
+// A product's tiles, and one unit of a pair's work: a tile, one half of its columns (`side` is that half, -1 for the whole) or one part of its K.
+struct LpTiles {
+  int m, n, all, num_kb;
+  __device__ __forceinline__ LpTiles(int M, int N, int K)
+      : m((M + 2 * kLpBM - 1) / (2 * kLpBM)), n((N + kLpBN - 1) / kLpBN), all(m * n), num_kb((K + kLpBK - 1) / kLpBK) {}
+  __device__ __forceinline__ void coords(int tile, int& mb, int& nb) const {
+    const int per_group = kLpGroupM * n, group = tile / per_group, first_m = group * kLpGroupM;
+    const int group_rows = min(m - first_m, kLpGroupM), in_group = tile - group * per_group;
+    mb = first_m + in_group % group_rows;
+    nb = in_group / group_rows;
+  }
+};
+struct LpUnit {
+  bool dh;
+  int mb, nb, side, part, kb0, kb1;
+};
+
+// What every pair works on, in order.  dh's parts come first, all tiles of a part before the next part, so that pairs at work together read the same rows
+// of both operands.  Where that leaves some pairs with one unit less, those begin with as many of the other product's tiles as make up for it.
+// Of those, a last wave of at most half as many tiles as pairs is worked on as halves of 128 columns (gemm2.cu).
+struct LpSchedule {
+  LpTiles dh, main;
+  int pair, n_pairs, parts, part_kb, dh_mine, heavy, first, first_mine, halves_from, units;
+
+  __device__ __forceinline__ LpSchedule(const LpTiles& dh, const LpTiles& main, int pair, int n_pairs, int parts)
+      : dh(dh), main(main), pair(pair), n_pairs(n_pairs), parts(parts) {
+    part_kb = (dh.num_kb + parts - 1) / parts;
+    const int dh_units = dh.all * parts;
+    dh_mine = dh_units > pair ? (dh_units - pair + n_pairs - 1) / n_pairs : 0;
+    heavy = dh_units % n_pairs;
+    first = first_mine = 0;
+    if (heavy > 0 && main.all > 0) {
+      const int lighter = n_pairs - heavy, each = main.num_kb + kLpDwOutput;
+      const int ahead = (part_kb + kLpDhOutput + each / 2) / each;       // tiles that take as long as one unit of dh
+      first = ahead >= (main.all + lighter - 1) / lighter ? main.all : ahead * lighter;
+      if (pair >= heavy && first > pair - heavy) first_mine = (first - (pair - heavy) + lighter - 1) / lighter;
+    }
+    const int left = main.all - first, last = left % n_pairs;
+    halves_from = 2 * last <= n_pairs ? left - last : left;
+    units = 2 * left - halves_from;
+  }
+  __device__ __forceinline__ bool get(int i, LpUnit& u) const {          // the i-th unit of this pair
+    u.dh = i < dh_mine;
+    u.side = -1;
+    u.part = 0;
+    if (u.dh) {
+      const int unit = pair + i * n_pairs;
+      u.part = unit / dh.all;
+      u.kb0 = u.part * part_kb;
+      u.kb1 = min(u.kb0 + part_kb, dh.num_kb);
+      dh.coords(unit - u.part * dh.all, u.mb, u.nb);
+      return true;
+    }
+    i -= dh_mine;
+    int tile = pair - heavy + i * (n_pairs - heavy);
+    if (i >= first_mine) {
+      const int unit = pair + (i - first_mine) * n_pairs;
+      if (unit >= units) return false;
+      tile = unit;
+      if (unit >= halves_from) {
+        u.side = (unit - halves_from) & 1;
+        tile = halves_from + ((unit - halves_from) >> 1);
+      }
+      tile += first;
+    }
+    u.kb0 = 0;
+    u.kb1 = main.num_kb;
+    main.coords(tile, u.mb, u.nb);
+    return true;
+  }
+};
+
+struct LpMaps {
+  CUtensorMap A, B, C;
+};
+
 // A maximum with its sum of exponentials.  The sum is of 2^(x scale2 - top), top being max scale2 rounded: what the rounding took goes into it.
 __device__ __forceinline__ float2 lp_sum(float mx, float top, float scale2, float sum) {
   return make_float2(mx, mx == -INFINITY ? sum : sum * fast_exp2(-fmaf(mx, scale2, -top)));
@@ -113,9 +195,8 @@ __device__ __forceinline__ float2 lp_sum(float mx, float top, float scale2, floa
 
 template <int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kLpThreads, 1)
-log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-                      const __grid_constant__ LpArgs a) {
-  constexpr bool kAMn = kMode == kDw, kBMn = kMode == kDh || kMode == kDw, kSums = kMode == kStats || kMode == kStatsKeep;
+log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant__ LpMaps maps_dh, const __grid_constant__ LpArgs a) {
+  constexpr bool kBMn = kMode == kProducts, kSums = kMode == kStats || kMode == kStatsKeep;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem + kLpStages * kLpStageBytes;
@@ -138,8 +219,8 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], split ? 16 : 8); }
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&maps.A);
+    tma_prefetch_desc(&maps.B);
   }
   if (warp == 2) { tmem_alloc2(tmem_slot, 512); tmem_relinquish2(); }
   tc_fence_before();
@@ -150,34 +231,12 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   grid_dependency_enter();
 
   const int count = *a.count;
-  const int M = kMode == kDw ? a.M : min(count, a.M), N = a.N, K = kMode == kDw ? min(count, a.K) : a.K;
-  const int tiles_m = (M + 2 * kLpBM - 1) / (2 * kLpBM), tiles_n = (N + kLpBN - 1) / kLpBN;
-  const int num_tiles = tiles_m * tiles_n;
-  const int num_kb = (K + kLpBK - 1) / kLpBK;
-  const int parts_k = kMode == kDh ? lp_parts(num_tiles, num_kb, n_pairs, a.planes) : 1, part_kb = (num_kb + parts_k - 1) / parts_k;
-  // A last wave of at most half as many tiles as pairs is worked on as halves of 128 columns (gemm2.cu)
-  const int last = num_tiles % n_pairs;
-  const int halves_from = parts_k > 1 ? num_tiles * parts_k : 2 * last <= n_pairs ? num_tiles - last : num_tiles;
-  const int units = parts_k > 1 ? num_tiles * parts_k : 2 * num_tiles - halves_from;
-
-  auto tile_coords = [&](int tile, int& mb, int& nb) {
-    const int per_group = kLpGroupM * tiles_n;
-    const int group = tile / per_group;
-    const int first_m = group * kLpGroupM;
-    const int group_rows = min(tiles_m - first_m, kLpGroupM);
-    const int in_group = tile - group * per_group;
-    mb = first_m + in_group % group_rows;
-    nb = in_group / group_rows;
-  };
-  // A unit is a tile, one half of its columns (`side` is that half, -1 for the whole), or one part of its K: all tiles of a part follow one
-  // another, so that pairs at work together read the same rows of both operands
-  auto unit_tile = [&](int unit, int& side) {
-    side = -1;
-    if (kMode == kDh && parts_k > 1) return unit % num_tiles;
-    if (unit < halves_from) return unit;
-    side = (unit - halves_from) & 1;
-    return halves_from + ((unit - halves_from) >> 1);
-  };
+  const int M = min(count, a.M), N = a.N;
+  const LpTiles dh(kMode == kProducts && a.dh ? M : 0, a.N, a.K);
+  const LpTiles main_tiles(kMode != kProducts ? M : a.dw ? a.K : 0, a.N, kMode != kProducts ? a.K : M);
+  const LpSchedule work_of(dh, main_tiles, pair, n_pairs,
+                           kMode == kProducts && dh.all > 0 ? lp_parts(dh.all, dh.num_kb, n_pairs, a.planes, a.dw ? lp_dw_steps(a.K, a.N, M) : 0.f) : 1);
+  const int num_kb = main_tiles.num_kb;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
@@ -185,30 +244,31 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int unit = pair; unit < units && ok; unit += n_pairs) {
-        int mb, nb, side;
-        tile_coords(unit_tile(unit, side), mb, nb);
-        const int row0 = mb * 2 * kLpBM + (int)rank * kLpBM;
-        const int col0 = side < 0 ? nb * kLpBN + (int)rank * kLpBNh : nb * kLpBN + side * kLpBNh + (int)rank * 64;
-        const int boxes = side >= 0 ? 1 : 2;                             // of 64 rows
-        const int kb0 = kMode == kDh && parts_k > 1 ? unit / num_tiles * part_kb : 0, kb1 = min(kb0 + part_kb, num_kb);
-        for (int kb = kb0; kb < kb1; ++kb) {
+      LpUnit u;
+      for (int i = 0; ok && work_of.get(i, u); ++i) {
+        const int row0 = u.mb * 2 * kLpBM + (int)rank * kLpBM;
+        const int col0 = u.side < 0 ? u.nb * kLpBN + (int)rank * kLpBNh : u.nb * kLpBN + u.side * kLpBNh + (int)rank * 64;
+        const int boxes = u.side >= 0 ? 1 : 2;                           // of 64 rows
+        const bool a_mn = kMode == kProducts && !u.dh;
+        const CUtensorMap* mA = kMode == kProducts && u.dh ? &maps_dh.A : &maps.A;
+        const CUtensorMap* mB = kMode == kProducts && u.dh ? &maps_dh.B : &maps.B;
+        for (int kb = u.kb0; kb < u.kb1; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty)) { ok = false; break; }
           uint8_t* sa = smem + stage * kLpStageBytes;
           uint8_t* sb = sa + kLpABytes;
           const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kLpABytes + boxes * 8192));
-          if (!kAMn) {
-            tma_load_2d_pair(sa, &tmA, kb * kLpBK, row0, bar);
+          if (!a_mn) {
+            tma_load_2d_pair(sa, mA, kb * kLpBK, row0, bar);
           } else {
 #pragma unroll
-            for (int i = 0; i < kLpBM / 64; ++i) tma_load_2d_pair(sa + i * 8192, &tmA, row0 + i * 64, kb * kLpBK, bar);
+            for (int j = 0; j < kLpBM / 64; ++j) tma_load_2d_pair(sa + j * 8192, mA, row0 + j * 64, kb * kLpBK, bar);
           }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i >= boxes) break;
-            if (!kBMn) tma_load_2d_pair(sb + i * 8192, &tmB, kb * kLpBK, col0 + i * 64, bar);
-            else tma_load_2d_pair(sb + i * 8192, &tmB, col0 + i * 64, kb * kLpBK, bar);
+          for (int j = 0; j < 2; ++j) {
+            if (j >= boxes) break;
+            if (!kBMn) tma_load_2d_pair(sb + j * 8192, mB, kb * kLpBK, col0 + j * 64, bar);
+            else tma_load_2d_pair(sb + j * 8192, mB, col0 + j * 64, kb * kLpBK, bar);
           }
           if (++stage == kLpStages) { stage = 0; phase ^= 1; }
         }
@@ -217,18 +277,17 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc_full = umma_idesc_bf16(2 * kLpBM, kLpBN, kAMn ? 1 : 0, kBMn ? 1 : 0);
-      constexpr uint32_t idesc_half = umma_idesc_bf16(2 * kLpBM, kLpBNh, kAMn ? 1 : 0, kBMn ? 1 : 0);
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int unit = pair; unit < units && ok; unit += n_pairs) {
-        const uint32_t idesc = unit < halves_from ? idesc_full : idesc_half;
-        const int kb0 = kMode == kDh && parts_k > 1 ? unit / num_tiles * part_kb : 0, kb1 = min(kb0 + part_kb, num_kb);
-        int from = kb0;
+      LpUnit u;
+      for (int i = 0; ok && work_of.get(i, u); ++i) {
+        const bool a_mn = kMode == kProducts && !u.dh;
+        const uint32_t idesc = umma_idesc_bf16(2 * kLpBM, u.side < 0 ? kLpBN : kLpBNh, a_mn ? 1 : 0, kBMn ? 1 : 0);
+        int from = u.kb0;
         do {                                                             // (once, of no steps at all, where nothing is multiplied)
-          const int to = kSums ? min(from + kLpChunk, kb1) : kb1;
+          const int to = kSums ? min(from + kLpChunk, u.kb1) : u.kb1;
           const int buf = local & 1;
           const uint32_t acc_phase = (local >> 1) & 1;
           ++local;
@@ -240,28 +299,29 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             tc_fence_after();
             const uint32_t sa = smem_u32(smem + stage * kLpStageBytes);
             const uint32_t sb = sa + kLpABytes;
+            // (advancing K by 16: 32 bytes where K is contiguous, 16 rows of 128 where it is not)
+            const uint64_t da = a_mn ? smem_desc_mnmajor_sw128(sa, 8192) : smem_desc_kmajor_sw128(sa), step = a_mn ? 2048 >> 4 : 32 >> 4;
 #pragma unroll
             for (int k = 0; k < kLpBK / 16; ++k) {
-              const uint64_t da = kAMn ? smem_desc_mnmajor_sw128(sa + k * 2048, 8192) : smem_desc_kmajor_sw128(sa + k * 32);
               const uint64_t db = kBMn ? smem_desc_mnmajor_sw128(sb + k * 2048, 8192) : smem_desc_kmajor_sw128(sb + k * 32);
-              umma2_ss(d_tmem, da, db, idesc, kb != from || k != 0 ? 1u : 0u);
+              umma2_ss(d_tmem, da + k * step, db, idesc, kb != from || k != 0 ? 1u : 0u);
             }
             umma2_commit_both(&empty[stage]);
             if (++stage == kLpStages) { stage = 0; phase ^= 1; }
           }
           if (ok) umma2_commit_both(&acc_full[buf]);
           from = to;
-        } while (from < kb1 && ok);
+        } while (from < u.kb1 && ok);
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
     const int quad = warp & 3, group = warp < 6 ? 0 : 1;
-    const int dx_rows = (M + kLpBK - 1) / kLpBK * kLpBK;                 // that kDw reads
+    const int dx_rows = (M + kLpBK - 1) / kLpBK * kLpBK;                 // that dx^T h reads
     int local = split ? 0 : group;
     bool ok = true;
     // One box of 128 bytes x 32 rows; `words(j)` are this lane's 16 bytes j of its row.
-    auto store_box = [&](auto&& words, int col, int row, bool add) {
+    auto store_box = [&](const CUtensorMap* map, auto&& words, int col, int row, bool add) {
       uint8_t* box = ring + (warp - 2) * 4096;
       if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the store before has read it
       __syncwarp();
@@ -270,8 +330,8 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        if (add) tma_reduce_add_2d(&tmC, box, col, row);
-        else tma_store_2d(&tmC, box, col, row);
+        if (add) tma_reduce_add_2d(map, box, col, row);
+        else tma_store_2d(map, box, col, row);
         tma_store_commit();
       }
     };
@@ -282,12 +342,12 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[local & 1]), 0));
       local += split ? 1 : 2;
     };
-    for (int unit = split ? pair : pair + group * n_pairs; unit < units && ok; unit += split ? n_pairs : 2 * n_pairs) {
-      int mb, nb, side;
-      tile_coords(unit_tile(unit, side), mb, nb);
-      const int row_w = mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
+    LpUnit u;
+    for (int i = split ? 0 : group; ok && work_of.get(i, u); i += split ? 1 : 2) {
+      const int nb = u.nb, side = u.side;
+      const int row_w = u.mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
       const int row = row_w + lane;
-      const bool live = kMode == kDw || row < M;
+      const bool live = row < M;
       int label = -1;
       float lse2 = 0.f, g = 0.f;
       if ((kSums || kMode == kGrad) && live) label = a.row_label[row];
@@ -363,7 +423,7 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
             for (int piece = 0; piece < 2; ++piece) {
               if (col + piece * 64 >= N) break;
-              if (row_w < M) store_box([&](int j) {
+              if (row_w < M) store_box(&maps.C, [&](int j) {
                 const uint32_t* x = r + piece * 64 + 8 * j;
                 return make_uint4(__byte_perm(code(x[0]), code(x[1]), 0x5410), __byte_perm(code(x[2]), code(x[3]), 0x5410),
                                   __byte_perm(code(x[4]), code(x[5]), 0x5410), __byte_perm(code(x[6]), code(x[7]), 0x5410));
@@ -393,10 +453,10 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 #pragma unroll
               for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
             }
-            if (row_w < dx_rows) store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
+            if (row_w < dx_rows) store_box(&maps.C, [&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
           }
         } else if (work) {
-          const bool bf = kMode == kDw && a.bf16_out;
+          const bool bf = !u.dh && a.bf16_out;
 #pragma unroll 1
           for (int piece = 0; piece < (bf ? 2 : 4); ++piece) {
             const int c = col + piece * (bf ? 64 : 32);
@@ -415,12 +475,12 @@ log_probs_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
               tmem_ld32(t_row + piece * 32, out);
               tmem_wait_ld();
             }
-            if (kMode == kDw && num_kb == 0)                             // no rows at all: nothing was multiplied
+            if (!u.dh && num_kb == 0)                                    // no rows at all: nothing was multiplied
 #pragma unroll
               for (int j = 0; j < 32; ++j) out[j] = 0u;
-            if (row_w < a.M)
-              store_box([&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c,
-                        kMode == kDh && parts_k > 1 ? unit / num_tiles * a.plane_rows + row_w : row_w, a.add != 0);
+            if (row_w < (u.dh ? a.M : a.K))
+              store_box(u.dh ? &maps_dh.C : &maps.C, [&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c,
+                        u.part * a.plane_rows + row_w, u.dh ? a.add_dh != 0 : a.add_dw != 0);
           }
         }
         if (part + 1 == part_end) arrive();
@@ -847,11 +907,12 @@ log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* top
 // share them where there are few values and may be many parts (one row in 64 parts 39 us by one thread each, 6 by 8; 4915 rows in 6 parts 54 and 124).
 template <int kSplit>
 __global__ void __launch_bounds__(256)
-log_probs_scatter_kernel(const float* dense, const int* place, const int* count, bf16* dh, int T, int D, int num_kb, int n_pairs, int planes, long long plane) {
+log_probs_scatter_kernel(const float* dense, const int* place, const int* count, bf16* dh, int T, int D, int n, int n_pairs, int planes, int dw, long long plane) {
   __shared__ float4 sums[kSplit][256 / kSplit];
   grid_dependency_enter();
-  const int tiles = (min(*count, T) + 2 * kLpBM - 1) / (2 * kLpBM) * ((D + kLpBN - 1) / kLpBN);
-  const int parts = tiles > 0 ? lp_parts(tiles, num_kb, n_pairs, planes) : 0, per_row = D / 4;
+  const int rows = min(*count, T), per_row = D / 4;
+  const LpTiles tiles(rows, D, n);
+  const int parts = tiles.all > 0 ? lp_parts(tiles.all, tiles.num_kb, n_pairs, planes, dw ? lp_dw_steps(n, D, rows) : 0.f) : 0;
   const int lane = threadIdx.x % (256 / kSplit), first = threadIdx.x / (256 / kSplit);
   const long long all = (long long)T * per_row;
   for (long long i0 = blockIdx.x * (256LL / kSplit); i0 < all; i0 += gridDim.x * (256LL / kSplit)) {
@@ -887,26 +948,31 @@ static int lp_map(CUtensorMap* m, const void* base, int elem, long long cols, lo
   return make_tmap(m, base, elem, 2, dims, str, box, true);
 }
 
-// CTA pairs of a launch (where fewer rows have a label than there are, the last ones may stay idle)
-static int lp_pairs(long long tiles, int planes, int sms) {
-  const long long units = tiles * (planes > 2 ? planes : 2);
-  return (int)(units < sms / 2 ? units : sms / 2);
-}
 static long long lp_tiles(int M, int N) { return (long long)((M + 2 * kLpBM - 1) / (2 * kLpBM)) * ((N + kLpBN - 1) / kLpBN); }
+// CTA pairs of a launch of so many units at most (where fewer rows have a label than there are, the last ones may stay idle)
+static int lp_pairs(long long units, int sms) { return (int)(units < sms / 2 ? units : sms / 2); }
+static long long lp_product_units(int T, int D, int n, bool dh, bool dw, int planes) { return (dh ? lp_tiles(T, D) * planes : 0) + (dw ? 2 * lp_tiles(n, D) : 0); }
+
+// Whether both products go into one launch: up to this many steps of kLpBK on a pair (half a millisecond).  600 rows of 2048 against 20000 tokens 198 -> 160 us,
+// 1000 of 512 against 50000 (half of them with a label) 145 -> 122, 3000 of 1024 against 50000 800 -> 788; 4915 of 2048 against 151936 take 8.43 ms in two
+// launches and 8.63 in one, at 1.5 % fewer cycles: the clock is lower by more than that under the power limit.
+constexpr long long kLpTogether = 1500;
+static bool lp_together(int T, int D, int n, bool dh, bool dw, int sms) {
+  const long long steps = lp_tiles(T, D) * ((n + kLpBK - 1) / kLpBK) + lp_tiles(n, D) * ((T + kLpBK - 1) / kLpBK);
+  return dh && dw && steps <= kLpTogether * (sms / 2);
+}
 
 template <int kMode>
-static int launch_log_probs(const CUtensorMap& A, const CUtensorMap& B, const CUtensorMap& C, LpArgs a, cudaStream_t st) {
+static int launch_log_probs(const LpMaps& maps, const LpMaps& maps_dh, LpArgs a, long long units, cudaStream_t st) {
   const int sms = sm_count();
   KSA_REQUIRE(sms > 1, "no device");
+  KSA_REQUIRE(units > 0 && units < (1 << 28), "log_probs: %lld tiles", units);
   a.status = status_word();
   KSA_REQUIRE(a.status != nullptr, "could not allocate the status word");
   auto kern = log_probs_pair_kernel<kMode>;
   static PerDevice raised;
   KSA_CHECK_CUDA(raise_smem_limit(raised, kern, kLpSmem));
-  const long long tiles = lp_tiles(a.M, a.N);
-  KSA_REQUIRE(tiles < (1 << 27), "log_probs: %lld tiles", tiles);
-  const int pairs = lp_pairs(tiles, a.planes, sms);
-  KSA_CHECK_CUDA(launch_kernel(kern, dim3(2 * pairs), dim3(kLpThreads), (size_t)kLpSmem, st, A, B, C, a));
+  KSA_CHECK_CUDA(launch_kernel(kern, dim3(2 * lp_pairs(units, sms)), dim3(kLpThreads), (size_t)kLpSmem, st, maps, maps_dh, a));
   return 0;
 }
 
@@ -963,15 +1029,15 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh,
                                         (const int*)rows, (const int*)count, (bf16*)dense, D, vec));
   }
-  CUtensorMap A, B, C;
+  LpMaps m;
   int rc, sums = slots;
   if (few) {
     const int sms = sm_count(), rows_of_cta = lf_rows(V, sms), ctas = (V + rows_of_cta - 1) / rows_of_cta;
     sums = ctas;
     picked = reinterpret_cast<float*>(stats + ld * sums);
-    rc = lp_map(&A, w, 2, D, V, ldw, 128);
-    if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 8);
-    if (rc == 0) rc = lp_map(&C, dense, 2, D, padded, lp_pitch(D), columns);
+    rc = lp_map(&m.A, w, 2, D, V, ldw, 128);
+    if (rc == 0) rc = lp_map(&m.B, w, 2, D, V, ldw, 8);
+    if (rc == 0) rc = lp_map(&m.C, dense, 2, D, padded, lp_pitch(D), columns);
     if (rc) return rc;
     int* status = status_word();
     KSA_REQUIRE(status != nullptr, "could not allocate the status word");
@@ -979,19 +1045,20 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     const int smem = columns == 32 ? LfShape<32>::smem : columns == 64 ? LfShape<64>::smem : columns == 96 ? LfShape<96>::smem : LfShape<128>::smem;
     static PerDevice raised[4];
     KSA_CHECK_CUDA(raise_smem_limit(raised[columns / 32 - 1], kern, smem));
-    KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, A, B, C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
+    KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, m.A, m.B, m.C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
                                  scale2, stats, ld, picked, status));
   } else {
-    rc = lp_map(&A, dense, 2, D, padded, lp_pitch(D), kLpBM);
-    if (rc == 0) rc = lp_map(&B, w, 2, D, V, ldw, 64);
-    if (rc == 0 && codes) rc = lp_map(&C, codes, 2, V, padded, lp_pitch(V), 32);
+    rc = lp_map(&m.A, dense, 2, D, padded, lp_pitch(D), kLpBM);
+    if (rc == 0) rc = lp_map(&m.B, w, 2, D, V, ldw, 64);
+    if (rc == 0 && codes) rc = lp_map(&m.C, codes, 2, V, padded, lp_pitch(V), 32);
     if (rc) return rc;
     LpArgs a{};
     a.M = T; a.N = V; a.K = D;
     a.count = static_cast<const int*>(count); a.row_label = static_cast<const int*>(row_label);
     a.scale2 = scale2;
     a.stats = stats; a.picked = picked; a.ld_stats = ld; a.tops = static_cast<float*>(tops);
-    rc = codes ? launch_log_probs<kStatsKeep>(A, B, C, a, st) : launch_log_probs<kStats>(A, B, A, a, st);
+    const long long units = 2 * lp_tiles(T, V);
+    rc = codes ? launch_log_probs<kStatsKeep>(m, m, a, units, st) : launch_log_probs<kStats>(m, m, a, units, st);
     if (rc) return rc;
   }
   const bool wide = T >= 32 * 148;
@@ -1017,18 +1084,18 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
   KSA_REQUIRE(!dh || (reinterpret_cast<uintptr_t>(dh) & 15) == 0, "log_probs: the gradient of the rows must be 16-byte aligned");
   cudaStream_t st = ST(stream);
   const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad;
-  CUtensorMap denseK, denseM;
-  int rc = lp_map(&denseK, dense, 2, D, padded, lp_pitch(D), kLpBM);
-  if (rc == 0) rc = lp_map(&denseM, dense, 2, D, padded, lp_pitch(D), 64);
+  const bool together = lp_together(T, D, V < slab ? V : slab, dh != nullptr, dw != nullptr, sm_count());
+  LpMaps grad, by_w, by_h;                                               // dx again; dx w; dx^T h
+  int rc = lp_map(&grad.A, dense, 2, D, padded, lp_pitch(D), kLpBM);
+  if (rc == 0) rc = lp_map(&by_h.B, dense, 2, D, padded, lp_pitch(D), 64);
+  if (rc == 0 && dh) rc = lp_map(&by_w.C, dh32, 4, D, (long long)planes * padded, D, 32);
   for (long long v0 = 0; v0 < V && rc == 0; v0 += slab) {
     const int n = V - v0 < slab ? (int)(V - v0) : slab;
     const bf16* wv = static_cast<const bf16*>(w) + v0 * ldw;
-    CUtensorMap wK, wM, dxOut, dxK, dxM, out;
     LpArgs a{};
     a.count = static_cast<const int*>(count); a.rows = static_cast<const int*>(rows); a.row_label = static_cast<const int*>(row_label);
     a.scale2 = (float)(1.4426950408889634 / (double)tau); a.inv_tau = 1.f / tau;
     a.lse2 = static_cast<const float*>(lse2); a.dy = static_cast<const float*>(dy); a.col0 = (int)v0;
-    a.M = T; a.N = n; a.K = D;
     if (codes) {
       const int col_blocks = (V + kLpDecodeCols - 1) / kLpDecodeCols;
       const long long blocks = (T + 63LL) / 64 * 8 * col_blocks;
@@ -1037,22 +1104,30 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
                                           (long long)slab, (const float*)tops, (T + 3LL) / 4 * 4, a.lse2, a.lse2 + T, a.dy, a.rows, a.row_label, a.count,
                                           (bf16*)dx, V, a.inv_tau, col_blocks));
     } else {
-      rc = lp_map(&wK, wv, 2, D, n, ldw, 64);
-      if (rc == 0) rc = lp_map(&dxOut, dx, 2, n, padded, slab, 32);
-      if (rc == 0) rc = launch_log_probs<kGrad>(denseK, wK, dxOut, a, st);
+      a.M = T; a.N = n; a.K = D;
+      rc = lp_map(&grad.B, wv, 2, D, n, ldw, 64);
+      if (rc == 0) rc = lp_map(&grad.C, dx, 2, n, padded, slab, 32);
+      if (rc == 0) rc = launch_log_probs<kGrad>(grad, grad, a, 2 * lp_tiles(T, n), st);
     }
-    if (rc == 0 && dh) {
-      a.M = T; a.N = D; a.K = n; a.add = v0 > 0; a.planes = planes; a.plane_rows = padded;
-      rc = lp_map(&dxK, dx, 2, n, padded, slab, kLpBM);
-      if (rc == 0) rc = lp_map(&wM, wv, 2, D, n, ldw, 64);
-      if (rc == 0) rc = lp_map(&out, dh32, 4, D, (long long)planes * padded, D, 32);
-      if (rc == 0) rc = launch_log_probs<kDh>(dxK, wM, out, a, st);
-    }
-    if (rc == 0 && dw) {
-      a.M = n; a.N = D; a.K = T; a.planes = 1; a.add = add_dw; a.bf16_out = !dw_fp32;
-      rc = lp_map(&dxM, dx, 2, n, padded, slab, 64);
-      if (rc == 0) rc = dw_fp32 ? lp_map(&out, static_cast<float*>(dw) + v0 * lddw, 4, D, n, lddw, 32) : lp_map(&out, static_cast<bf16*>(dw) + v0 * lddw, 2, D, n, lddw, 32);
-      if (rc == 0) rc = launch_log_probs<kDw>(dxM, denseM, out, a, st);
+    if (rc == 0 && (dh || dw)) {
+      a.M = T; a.N = D; a.K = n; a.dh = a.dw = 1; a.add_dh = v0 > 0; a.add_dw = add_dw;
+      a.planes = planes; a.plane_rows = padded; a.bf16_out = !dw_fp32;
+      if (dh) {
+        rc = lp_map(&by_w.A, dx, 2, n, padded, slab, kLpBM);
+        if (rc == 0) rc = lp_map(&by_w.B, wv, 2, D, n, ldw, 64);
+      }
+      if (rc == 0 && dw) {
+        rc = lp_map(&by_h.A, dx, 2, n, padded, slab, 64);
+        if (rc == 0) rc = dw_fp32 ? lp_map(&by_h.C, static_cast<float*>(dw) + v0 * lddw, 4, D, n, lddw, 32) : lp_map(&by_h.C, static_cast<bf16*>(dw) + v0 * lddw, 2, D, n, lddw, 32);
+      }
+      if (together) {
+        if (rc == 0) rc = launch_log_probs<kProducts>(by_h, by_w, a, lp_product_units(T, D, n, true, true, planes), st);
+      } else {
+        a.dw = 0;
+        if (rc == 0 && dh) rc = launch_log_probs<kProducts>(by_w, by_w, a, lp_product_units(T, D, n, true, false, planes), st);
+        a.dh = 0; a.dw = 1;
+        if (rc == 0 && dw) rc = launch_log_probs<kProducts>(by_h, by_h, a, lp_product_units(T, D, n, false, true, planes), st);
+      }
     }
   }
   if (rc) return rc;
@@ -1061,8 +1136,8 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     const long long blocks = ((long long)T * (D / 4) * split + 255) / 256;
     KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, split > 1 ? log_probs_scatter_kernel<8> : log_probs_scatter_kernel<1>,
                                         dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const float*)dh32, (const int*)place,
-                                        (const int*)count, (bf16*)dh, T, D, (int)(((V < slab ? V : slab) + kLpBK - 1) / kLpBK),
-                                        lp_pairs(lp_tiles(T, D), planes, sm_count()), planes,
+                                        (const int*)count, (bf16*)dh, T, D, V < slab ? V : slab,
+                                        lp_pairs(lp_product_units(T, D, V < slab ? V : slab, true, together, planes), sm_count()), planes, (int)together,
                                         (long long)padded * D));
   }
   return 0;

@@ -1158,7 +1158,7 @@ LogProbsKept log_probs(const Tensor& h, const Tensor& w, const LogProbsCall& c, 
   k.kept = at::empty({(int64_t)(5 * T + 4 + (keep ? (T + 3) / 4 * 4 * ((V + c.columns - 1) / c.columns) : 0))}, on(h, at::kInt));
   const Tensor work = at::empty({(int64_t)ksa_log_probs_work((int)T, (int)V)}, on(h, at::kFloat));
   int* kept = static_cast<int*>(k.kept.mutable_data_ptr());
-  LAUNCH_SEVERAL(4, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), kept, kept + T, kept + 2 * T,
+  LAUNCH_SEVERAL(3, ksa_log_probs, h.const_data_ptr(), w.const_data_ptr(), c.labels->const_data_ptr(), k.dense.mutable_data_ptr(), kept, kept + T, kept + 2 * T,
                  kept + 3 * T, kept + 3 * T + 4, work.mutable_data_ptr(), k.y.mutable_data_ptr(), keep ? k.codes.mutable_data_ptr() : nullptr,
                  keep ? kept + 5 * T + 4 : nullptr, (int)T, (int)V, (int)D,
                  h.dim() == 2 ? h.stride(0) : D, w.stride(0), c.ignore, c.tau, stream_of(h));
@@ -1191,7 +1191,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
     }
     if (need_w) dw = at::empty({(int64_t)V, (int64_t)D}, on(w, at::kBFloat16));
     const int* p = static_cast<const int*>(kept.const_data_ptr());
-    LAUNCH_SEVERAL(4, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, p + 3 * T + 4, codes.defined() ? codes.const_data_ptr() : nullptr,
+    LAUNCH_SEVERAL(3, ksa_log_probs_bwd, dense.const_data_ptr(), w.const_data_ptr(), p, p + T, p + 2 * T, p + 3 * T, p + 3 * T + 4, codes.defined() ? codes.const_data_ptr() : nullptr,
                    codes.defined() ? p + 5 * T + 4 : nullptr, dy.const_data_ptr(),
                    dx.mutable_data_ptr(), need_h ? dh32.mutable_data_ptr() : nullptr, need_h ? dh.mutable_data_ptr() : nullptr,
                    need_w ? dw.mutable_data_ptr() : nullptr, (int)T, (int)V, (int)D, w.stride(0), D, 0, 0, (int)slab, need_h ? (int)planes : 1, (float)ctx->saved_data["tau"].toDouble(),

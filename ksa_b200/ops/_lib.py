@@ -211,8 +211,8 @@ def _address(x: torch.Tensor) -> int:
 
 # kernels launched by one call of an entry point (default 1)
 _KERNELS_PER_CALL = {"ksa_attn_bwd": 2, "ksa_attn_bwd_fused": 3, "ksa_attn_bwd_fused_cp": 3, "ksa_rmsnorm_bwd": 2,
-                     "ksa_grad_norm": 2, "ksa_policy_loss": 2, "ksa_preference_loss": 2, "ksa_log_probs": 4,
-                     "ksa_log_probs_bwd": 4}
+                     "ksa_grad_norm": 2, "ksa_policy_loss": 2, "ksa_preference_loss": 2, "ksa_log_probs": 3,
+                     "ksa_log_probs_bwd": 3}
 _launch_count = 0
 
 

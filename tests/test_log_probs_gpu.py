@@ -282,7 +282,7 @@ def test_slabs_of_the_vocabulary(V, monkeypatch):
     _close(p.main_grad - 1, (want["dw"][0], want["dw"][1] + 2.0 ** -23 * (1 + want["dw"][0].abs())), "added to")
 
 
-@pytest.mark.parametrize("T,D,V", [(300, 136, 1000), (256, 64, 33000), (77, 256, 4096), (700, 512, 20000)])
+@pytest.mark.parametrize("T,D,V", [(300, 136, 1000), (256, 64, 33000), (77, 256, 4096), (700, 512, 20000), (8000, 1024, 30000)])
 def test_parts_of_the_vocabulary(T, D, V, monkeypatch):
     """dh in several parts, added up in order, against the same in one."""
     h, w, labels, dy = _inputs(T, D, V, 0.8, seed=17)
