@@ -502,11 +502,12 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
 // The log-sums of a few rows without a backward pass.  Bound: the weights' bytes.  The kernel above would multiply 256 rows, most of them padding, and the
 // tensor cores' share of the power then slows the memory down (one row of 2560 against 151936 tokens 134 us by itself, 167 to 183 in a row of calls).
 // Here the weights are the 128 rows of the tensor cores' product and the activations, N of them, its columns.  Every CTA has as many weight rows
-// as the others, in steps of 8: tiles of 256 and a shorter last one, the end of which is loaded 8 rows at a time.
+// as the others, in steps of 8, in tiles of one size of at most 256, whose last rows are loaded 8 at a time: a short last tile would load
+// all activations for little (1032 rows as 4 x 256 and 8: 77 rows against 151936 tokens of 2048 119.9 us).
 // Epilogue: a thread has one weight row and N values; a warp adds up its 32 rows for every activation by exchanging halves, after which a
 // lane has one activation's maximum (or sum), and keeps it over its tiles.  A CTA writes one maximum and sum for each activation.
 constexpr int kLfThreads = 320;      // warp 0 loads, warp 1 issues products, warps 2..5 and 6..9 epilogue, each group of 128 weight rows
-constexpr int kLfTile = 256;         // weight rows that share a load of the activations: two products of 128 rows
+constexpr int kLfTile = 256;         // weight rows that share a load of the activations, at most: two products of 128 rows
 constexpr int kLfMostRows = 128;
 template <int N>
 struct LfShape {
@@ -518,7 +519,7 @@ struct LfShape {
 template <int N>
 __global__ void __launch_bounds__(kLfThreads, 1)
 log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW8, const __grid_constant__ CUtensorMap tmH, int V,
-                     int D, int rows_of_cta, const int* count, const int* row_label, float scale2, float2* stats, long long ld, float* picked, int* status) {
+                     int D, int rows_of_cta, int tile_rows, const int* count, const int* row_label, float scale2, float2* stats, long long ld, float* picked, int* status) {
   using S = LfShape<N>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -550,7 +551,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int v_lo = blockIdx.x * rows_of_cta, v_hi = min(V, v_lo + rows_of_cta);        // rows_of_cta a multiple of 8
-  const int tiles = n > 0 ? (v_hi - v_lo + kLfTile - 1) / kLfTile : 0, num_kb = (D + kLpBK - 1) / kLpBK;
+  const int tiles = n > 0 ? (v_hi - v_lo + tile_rows - 1) / tile_rows : 0, num_kb = (D + kLpBK - 1) / kLpBK;
 
   if (warp == 0) {
     if (elect_one()) {
@@ -558,7 +559,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = 0; tile < tiles && ok; ++tile) {
-        const int v0 = v_lo + tile * kLfTile, eights = (min(v_hi - v0, kLfTile) + 7) / 8;
+        const int v0 = v_lo + tile * tile_rows, eights = (min(v_hi - v0, tile_rows) + 7) / 8;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1, guard, kTimeoutStageEmpty)) { ok = false; break; }
           uint8_t* sw = smem + stage * S::stage_bytes;
@@ -578,7 +579,7 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = 0; tile < tiles && ok; ++tile) {
-        const bool both = v_hi - v_lo - tile * kLfTile > 128;
+        const bool both = min(v_hi - v_lo - tile * tile_rows, tile_rows) > 128;
         for (int from = 0; from < num_kb && ok; from += kLpChunk, ++local) {
           const int buf = local & 1, to = min(from + kLpChunk, num_kb);
           if (!mbar_wait(&acc_empty[buf], ((local >> 1) & 1) ^ 1, guard, kTimeoutAccEmpty)) { ok = false; break; }
@@ -609,14 +610,14 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
 #pragma unroll
     for (int c = 0; c < N / 32; ++c) { run_m[c] = -INFINITY; run_s[c] = 0.f; }
     for (int tile = 0; tile < tiles && ok; ++tile) {
-      const int v0 = v_lo + tile * kLfTile + half * 128 + quad * 32, v = v0 + lane;
+      const int v0 = v_lo + tile * tile_rows + half * 128 + quad * 32, v = v0 + lane, v_end = min(v_hi, v_lo + (tile + 1) * tile_rows);
       float acc[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = 0.f;
       for (int from = 0; from < num_kb; from += kLpChunk, ++local) {
         if (!mbar_wait(&acc_full[local & 1], (local >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
         tc_fence_after();
-        if (v0 < v_hi)
+        if (v0 < v_end)
 #pragma unroll
           for (int c = 0; c < N / 32; ++c) {
             uint32_t r[32];
@@ -629,15 +630,15 @@ log_probs_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc_empty[local & 1]);
       }
-      if (!ok || v0 >= v_hi) continue;
+      if (!ok || v0 >= v_end) continue;
 #pragma unroll
       for (int c = 0; c < N / 32; ++c) {
         if (c * 32 >= n) break;
         float x[32], m[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          x[j] = v < v_hi ? acc[c * 32 + j] : -INFINITY;
-          if (label[c * 32 + j] == v && v < v_hi) picked[c * 32 + j] = x[j];
+          x[j] = v < v_end ? acc[c * 32 + j] : -INFINITY;
+          if (label[c * 32 + j] == v && v < v_end) picked[c * 32 + j] = x[j];
           m[j] = x[j];
         }
 #pragma unroll
@@ -1033,6 +1034,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   int rc, sums = slots;
   if (few) {
     const int sms = sm_count(), rows_of_cta = lf_rows(V, sms), ctas = (V + rows_of_cta - 1) / rows_of_cta;
+    const int tiles = (rows_of_cta + kLfTile - 1) / kLfTile, tile_rows = (rows_of_cta + 8 * tiles - 1) / (8 * tiles) * 8;
     sums = ctas;
     picked = reinterpret_cast<float*>(stats + ld * sums);
     rc = lp_map(&m.A, w, 2, D, V, ldw, 128);
@@ -1045,7 +1047,7 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
     const int smem = columns == 32 ? LfShape<32>::smem : columns == 64 ? LfShape<64>::smem : columns == 96 ? LfShape<96>::smem : LfShape<128>::smem;
     static PerDevice raised[4];
     KSA_CHECK_CUDA(raise_smem_limit(raised[columns / 32 - 1], kern, smem));
-    KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, m.A, m.B, m.C, V, D, rows_of_cta, (const int*)count, (const int*)row_label,
+    KSA_CHECK_CUDA(launch_kernel(kern, dim3(ctas), dim3(kLfThreads), (size_t)smem, st, m.A, m.B, m.C, V, D, rows_of_cta, tile_rows, (const int*)count, (const int*)row_label,
                                  scale2, stats, ld, picked, status));
   } else {
     rc = lp_map(&m.A, dense, 2, D, padded, lp_pitch(D), kLpBM);

@@ -219,6 +219,38 @@ def test_layouts_of_rows_and_labels(layout):
         assert torch.equal(a, b)
 
 
+def test_a_single_row_without_a_dimension_of_its_own():
+    h, w, labels, _ = _inputs(3, 72, 400, 1.0, seed=19)
+    want = _run(h[1:2], w, labels[1:2], torch.ones(1, device="cuda"), 1.0)
+    y, dh, dw = _run(h[1], w, labels[1], torch.ones((), device="cuda"), 1.0)
+    assert y.shape == () and torch.equal(y, want[0][0]) and torch.equal(dh, want[1][0]) and torch.equal(dw, want[2])
+    with torch.no_grad():
+        assert torch.equal(ops.linear_log_probs(h[1], w, labels[1]), ops.linear_log_probs(h[1:2], w, labels[1:2])[0])
+
+
+def test_two_threads_at_once():
+    """Calls of two threads on streams of their own, on the same tensors: nothing of one call is another's."""
+    import threading
+    h, w, labels, dy = _inputs(200, 136, 3000, 0.7, seed=20)
+    want = _run(h, w, labels, dy, 1.0)
+    got = {}
+    torch.cuda.synchronize()
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [_run(h, w, labels, dy, 1.0) for _ in range(5)]
+        stream.synchronize()
+        got[k] = outs
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for outs in got.values():
+        assert len(outs) == 5 and all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+
+
 @pytest.mark.parametrize("layout", ["pitch", "odd", "columns"])
 def test_layouts_of_the_head(layout):
     T, D, V = 66, 72, 400
