@@ -89,7 +89,8 @@ def _name(lengths):
     return f"{len(lengths)} of {sum(lengths)}"
 
 
-LENGTHS = [[1], [7], [2048], [2049], [4096], [3, 5], [257] * 4, [0, 0, 3], [5, 0, 0, 4100, 1, 2047, 2048, 0], [1] * 300, [6000, 1, 9000], []]
+LENGTHS = [[1], [7], [2048], [2049], [4096], [3, 5], [257] * 4, [0, 0, 3], [5, 0, 0, 4100, 1, 2047, 2048, 0], [1] * 300, [6000, 1, 9000],
+           [4095, 4097, 8193], [33001, 2], [2] * 1100, []]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -238,7 +239,7 @@ def _preference(y, ref, mask, cu, beta, eps):
     return loss, r, dy.view(y.shape)
 
 
-PAIRS = [[1, 1], [2048, 2049], [0, 5], [0, 0], [257] * 4, [1] * 300, [4097, 3, 0, 6000, 2048, 1], []]
+PAIRS = [[1, 1], [2048, 2049], [0, 5], [0, 0], [257] * 4, [1] * 300, [4097, 3, 0, 6000, 2048, 1], [33001, 4096], [2] * 1026, [1] * 2500, []]
 
 
 @pytest.mark.parametrize("device", DEVICES)
