@@ -188,7 +188,7 @@ struct LpMaps {
   CUtensorMap A, B, C;
 };
 
-// A maximum with its sum of exponentials.  The sum is of 2^(x scale2 - top), top being max scale2 rounded: what the rounding took goes into it.
+// A maximum with its sum of exponentials.  The sum is of 2^(x scale2 - top), top being max scale2 rounded: what the rounding took or added goes into it.
 __device__ __forceinline__ float2 lp_sum(float mx, float top, float scale2, float sum) {
   return make_float2(mx, mx == -INFINITY ? sum : sum * fast_exp2(-fmaf(mx, scale2, -top)));
 }
@@ -408,7 +408,8 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
 #pragma unroll
             for (int i = 0; i < 4; ++i) m[i] = max3(m[i], __uint_as_float(r[j + 2 * i]), __uint_as_float(r[j + 2 * i + 1]));
           const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-          const float top = mx == -INFINITY ? 0.f : mx * a.scale2;       // (scale2 > 0)
+          // (scale2 > 0.  Rounded up: no code of a kept logit may be below zero, where from 2^12 on half a step of the maximum is a quarter of a code and more)
+          const float top = mx == -INFINITY ? 0.f : __fmul_ru(mx, a.scale2);
           float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < kLpStatCols; ++j) s[j & 3] += fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -top));

@@ -1,0 +1,87 @@
+"""``ops.linear_log_probs`` where its arithmetic is at its limits, against the definition in 64 bits, on logits that are exact.
+
+Rows and weights are small whole numbers and multiples of 2^-7, so that every partial sum of a logit is exact in 32 bits and in the tensor cores: what is
+left are the errors of the softmax.  Row ``t`` has a column of its own with a one in it, and no weight has anything there: the logits' gradient of
+that row can then be read from the weights' gradient, where it is a single product, as ``dx`` rounded to bf16.
+
+Tolerances.  The distance below the maximum is taken in base 2 with one factor, ``log2(e) / tau`` in 32 bits: off by 2^-24 of the distance with its product.  The
+log-sum is one 32-bit number: half a step, 2^-24 of it.  Exponentials (2^-22), the correction of a tile's sum for its rounded maximum (2^-22) and the
+sum's roundings: 2^-20.  Kept logits: half a step of 2^-10 of a power of two, 2^-11.5 of the probability; not so the label's, which comes
+from the exact logit by way of a distance that is rounded by itself.  dx is rounded to bf16, 2^-8.
+"""
+import pytest
+import torch
+
+from ksa_b200 import ops
+from ksa_b200.ops import log_probs as impl
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["kept", "again"], autouse=True)
+def logits(request, monkeypatch):
+    """Every test with the logits kept for the backward pass and with them computed again, whatever the width."""
+    monkeypatch.setattr(impl, "KEEP_WIDTH", 0 if request.param == "kept" else 1 << 20)
+    return request.param
+
+
+def _exact(T, V, D, factor, steps, unit, label_on_top, seed=0):
+    """h, w, labels, dy and each row's own column.  Row t has its two largest logits in the columns 2 g and 2 g + 1, the first ``steps`` to
+    its number times ``unit`` above the second; all others are far below."""
+    assert V % 2 == 0 and D >= T + 48
+    g = torch.Generator().manual_seed(seed)
+    place = torch.randperm(D, generator=g)
+    main, fine, own = place[:40], place[40], place[48:48 + T]
+    w = torch.zeros(V, D)
+    trits = torch.randint(-1, 2, (V // 2, 40), generator=g).float()
+    w[:, main] = trits.repeat_interleave(2, 0)
+    w[1::2, fine] = -1
+    group = torch.randint(0, V // 2, (T,), generator=g)
+    h = torch.zeros(T, D)
+    h[:, main] = trits[group] * (factor * torch.randint(8, 16, (T, 1), generator=g))
+    h[:, fine] = torch.randint(*steps, (T,), generator=g) * unit
+    h[torch.arange(T), own] = 1
+    labels = 2 * group if label_on_top else torch.randint(0, V, (T,), generator=g)
+    dy = torch.randn(T, generator=g)
+    assert torch.equal(h.bfloat16().float(), h)
+    return h.bfloat16().cuda(), w.bfloat16().cuda(), labels.cuda(), dy.cuda(), own.cuda()
+
+
+def _check(h, w, labels, dy, own, tau, kept):
+    t32 = float(torch.tensor(tau, dtype=torch.float32))
+    T = h.shape[0]
+    i = torch.arange(T, device="cuda")
+    x = h.double() @ w.double().T / t32
+    lse = x.logsumexp(1, keepdim=True)
+    p = (x - lse).exp()
+    g = dy.double()[:, None] / t32
+    dx = -p * g
+    # (of the label next to a probability of one: by the sum of the others)
+    rest = p.clone()
+    rest[i, labels] = 0
+    dx[i, labels] = rest.sum(1) * g[:, 0]
+    gap = x.amax(1, keepdim=True) - x
+    far = 2.0 ** -24 * gap + 2.0 ** -20                                     # of what is taken as a distance below the maximum
+    off = p * (far + 2.0 ** -24 * (lse.abs() + 1) + (2.0 ** -11.5 if kept else 0)) + (2.0 ** -63 if kept else 2.0 ** -126)
+    off[i, labels] = (p * far)[i, labels] + 2.0 ** -126
+    tol = off * g.abs() * (1 + 2.0 ** -8) + 2.0 ** -8 * dx.abs()
+    h, w = h.requires_grad_(), w.requires_grad_()
+    y = ops.linear_log_probs(h, w, labels, temperature=tau)
+    dh, dw = torch.autograd.grad(y, (h, w), dy)
+    want = x[i, labels] - lse[:, 0]
+    assert ((y.detach().double() - want).abs() <= 2.0 ** -23 * (want.abs() + 1) + 2.0 ** -20).all()
+    got = dw[:, own].T.double()
+    bad = (got - dx).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((got - dx).abs() / tol).max()))
+    # dh adds up to two or three terms of any size in 32 bits, and is rounded once
+    wd = w.detach().double()
+    assert ((dh.double() - dx @ wd).abs() <= (tol @ wd.abs()) * (1 + 2.0 ** -8) + (dx.abs() @ wd.abs()) * 2.0 ** -18 + 2.0 ** -8 * (dx @ wd).abs()).all()
+
+
+@pytest.mark.parametrize("T,V", [(90, 600), (200, 1002), (300, 5000)])
+@pytest.mark.parametrize("factor,steps,unit,tau", [(16, (0, 12), 0.25, 1.0), (256, (0, 12), 0.25, 1.0), (1, (0, 4), 2.0 ** -7, 0.01)])
+def test_probabilities_at_logits_of_thousands(T, V, factor, steps, unit, tau, logits):
+    """The two largest logits share the row's probability however far from zero they are: by the hundreds, by the hundred thousand, at a
+    sampling temperature of a hundredth."""
+    h, w, labels, dy, own = _exact(T, V, -(-(T + 48) // 8) * 8, factor, steps, unit, False, seed=T)
+    _check(h, w, labels, dy, own, tau, logits == "kept")
