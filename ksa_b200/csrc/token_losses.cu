@@ -188,8 +188,9 @@ __device__ __forceinline__ TokenTerms policy_token(const PolicyArgs& a, float y,
     t.cut = (A > 0.f && exact > a.above) || (A < 0.f && exact < a.below);
   }
   const float r = expf(d);
-  t.L = t.cut ? -(A > 0.f ? a.most : a.least) * A : -r * A;
-  t.g = t.cut ? 0.f : -r * A;
+  const float part = A == 0.f && !isnan(d) ? 0.f : -r * A;                        // (no advantage, no loss: not even where the ratio is infinite)
+  t.L = t.cut ? -(A > 0.f ? a.most : a.least) * A : part;
+  t.g = t.cut ? 0.f : part;
   t.K = 0.f;
   if (a.ref) {
     const float x = ref - y;

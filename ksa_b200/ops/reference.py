@@ -363,8 +363,9 @@ def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, of, s
     d = y - pick(old_log_probs)
     cut = ((a > 0) & (d > math.log1p(clip_high))) | ((a < 0) & (d < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)))
     bound = torch.where(a > 0, torch.full_like(a, 1 + clip_high), torch.full_like(a, 1 - clip_low))
-    # (a token that is cut off takes part with a ratio of one and no advantage, so that nothing flows through it)
-    part = torch.where(cut, -bound * a, -torch.exp(torch.where(cut, torch.zeros_like(d), d)) * torch.where(cut, torch.zeros_like(a), a))
+    # (a token that is cut off, or has no advantage, takes part with a ratio of one and no advantage, so that nothing flows through it)
+    still = cut | ((a == 0) & ~d.isnan())
+    part = torch.where(cut, -bound * a, -torch.exp(torch.where(still, torch.zeros_like(d), d)) * torch.where(still, torch.zeros_like(a), a))
     part = torch.where(valid, part, torch.zeros_like(part))
     x = pick(ref_log_probs) - y if ref_log_probs is not None else torch.zeros_like(y)
     kl = torch.expm1(x) - x

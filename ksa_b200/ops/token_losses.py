@@ -129,7 +129,7 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
     """The clipped policy loss with a KL term: ``(loss, stats)``.
 
     With ``r = exp(log_probs - old_log_probs)`` a token's loss is ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef K``,
-    ``K = exp(x) - 1 - x`` for ``x = ref_log_probs - log_probs`` (0 without a reference).  ``advantages``: a value for every token, or for every
+    ``K = exp(x) - 1 - x`` for ``x = ref_log_probs - log_probs`` (0 without a reference); where ``A`` is 0 so is the first part, however large ``r``.  ``advantages``: a value for every token, or for every
     sequence (``[sequences]``, which also is what ``[sequences]`` means where the length is the same number).  ``reduction``: "token", the mean over the valid tokens, or "sequence", the mean over the sequences that
     have one of each sequence's mean; without any valid token the loss is 0.  ``stats`` (fp32 ``[3]``, no gradient): the same means of the clipped
     part, of ``K`` and of being cut off, that is ``A > 0`` with ``r > 1 + clip_high`` or ``A < 0`` with ``r < 1 - clip_low``; such a token has no

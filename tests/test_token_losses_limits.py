@@ -1,0 +1,45 @@
+"""The policy and preference losses where a term is infinite or nothing, on the CPU and (marked) on the GPU."""
+import math
+
+import pytest
+import torch
+
+from ksa_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+INF = math.inf
+
+
+def _on(device, *values):
+    return [torch.tensor(v, device=device) for v in values]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+@pytest.mark.parametrize("by_sequence", [False, True])
+def test_no_advantage_is_no_policy_loss_whatever_the_ratio(device, reduction, by_sequence):
+    """-min(r 0, clip(r) 0) is 0 for a ratio that overflows, is infinite or is zero; the other tokens keep loss and gradient."""
+    y, old = _on(device, [[0.0, 0.0, 0.0, -INF], [-1.0, -1.0, -1.0, -1.0]], [[-100.0, -INF, 200.0, -1.0], [-1.0, -1.0, -1.0, -1.0]])
+    y.requires_grad_(True)
+    adv = torch.tensor([0.0, 1.0], device=device)
+    if not by_sequence:
+        adv = adv[:, None].expand(2, 4).contiguous()
+    loss, stats = ops.policy_loss(y, old, adv, reduction=reduction)
+    dy, = torch.autograd.grad(loss, y)
+    assert float(loss.detach()) == -0.5 and stats.tolist() == [-0.5, 0.0, 0.0]
+    assert torch.equal(dy.cpu(), torch.tensor([[0.0] * 4, [-0.125] * 4]))
+    # a difference that is no number stays one
+    with torch.no_grad():
+        y[0, 0] = old[0, 0] = -INF
+    assert math.isnan(float(ops.policy_loss(y, old, adv, reduction=reduction)[0].detach()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_gradient_of_the_kl_term_stays_without_an_advantage(device):
+    y, old, ref, adv = _on(device, [0.0, 0.0], [-100.0, 0.0], [0.5, -0.5], [0.0, 0.0])
+    y.requires_grad_(True)
+    loss, _ = ops.policy_loss(y, old, adv, ref, kl_coef=0.5)
+    want = 0.5 * sum(math.expm1(x) - x for x in (0.5, -0.5)) / 2
+    assert abs(float(loss.detach()) - want) <= 1e-6
+    dy, = torch.autograd.grad(loss, y)
+    assert all(abs(float(g) + 0.25 * math.expm1(x)) <= 1e-6 for g, x in zip(dy, (0.5, -0.5)))
