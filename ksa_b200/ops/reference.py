@@ -351,15 +351,15 @@ def sequence_of(n: int, sequences: int, cu_seqlens: Optional[torch.Tensor], devi
 
 
 def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, of, sequences: int, clip_low: float, clip_high: float, kl_coef: float,
-                by_sequence: bool):
-    """Flat arguments: a value for every token (``advantages``: or sequence), ``of`` its sequence.  Returns the loss and the means of
-    its clipped part, of the KL term and of being cut off."""
+                by_sequence: bool, adv_by_sequence: bool):
+    """Flat arguments: a value for every token (``advantages``, with ``adv_by_sequence``: for every sequence), ``of`` its sequence.  Returns the
+    loss and the means of its clipped part, of the KL term and of being cut off."""
     valid = of < sequences
     if mask is not None:
         valid = valid & (mask != 0)
     y = torch.where(valid, log_probs, log_probs.new_zeros(())).double()
     pick = lambda t: torch.where(valid, t, t.new_zeros(())).double()  # noqa: E731
-    a = pick(advantages if advantages.shape == of.shape else torch.cat([advantages, advantages.new_zeros(1)])[of])
+    a = pick(torch.cat([advantages, advantages.new_zeros(1)])[of] if adv_by_sequence else advantages)
     d = y - pick(old_log_probs)
     cut = ((a > 0) & (d > math.log1p(clip_high))) | ((a < 0) & (d < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)))
     bound = torch.where(a > 0, torch.full_like(a, 1 + clip_high), torch.full_like(a, 1 - clip_low))

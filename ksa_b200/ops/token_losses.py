@@ -129,9 +129,11 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
     """The clipped policy loss with a KL term: ``(loss, stats)``.
 
     With ``r = exp(log_probs - old_log_probs)`` a token's loss is ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef K``,
-    ``K = exp(x) - 1 - x`` for ``x = ref_log_probs - log_probs`` (0 without a reference); where ``A`` is 0 so is the first part, however large ``r``.  ``advantages``: a value for every token, or for every
-    sequence (``[sequences]``, which also is what ``[sequences]`` means where the length is the same number).  ``reduction``: "token", the mean over the valid tokens, or "sequence", the mean over the sequences that
-    have one of each sequence's mean; without any valid token the loss is 0.  ``stats`` (fp32 ``[3]``, no gradient): the same means of the clipped
+    ``K = exp(x) - 1 - x`` for ``x = ref_log_probs - log_probs`` (0 without a reference); where ``A`` is 0 so is the first part, however large ``r``.
+    ``advantages``: of the shape of ``log_probs``, a value for every token; else ``[sequences]`` or ``[sequences, 1]``, one for every sequence.  (Packed in
+    one dimension, as many values as tokens are one for every token, also where there are as many sequences; ``[sequences, 1]`` says otherwise.)
+    ``reduction``: "token", the mean over the valid tokens, or "sequence", the mean over the sequences that have one of each sequence's mean;
+    without any valid token the loss is 0.  ``stats`` (fp32 ``[3]``, no gradient): the same means of the clipped
     part, of ``K`` and of being cut off, that is ``A > 0`` with ``r > 1 + clip_high`` or ``A < 0`` with ``r < 1 - clip_low``; such a token has no
     gradient but that of ``K``.  With a ``kl_coef`` of 0 the reference counts in the statistics alone."""
     if not _observed() and reduction in ("token", "sequence"):
@@ -152,7 +154,7 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
         flat = lambda t: None if t is None else t.reshape(-1)  # noqa: E731
         of = ref.sequence_of(seq.n, seq.count, seq.cu, log_probs.device)
         return ref.policy_loss(flat(log_probs), flat(old_log_probs), flat(advantages), flat(ref_log_probs), flat(mask), of, seq.count, clip_low,
-                               clip_high, kl_coef, reduction == "sequence")
+                               clip_high, kl_coef, reduction == "sequence", not by_token)
     return _run(_PolicyLossFn, log_probs, old_log_probs, advantages, ref_log_probs, mask, seq, not by_token, clip_low, clip_high, kl_coef,
                 reduction == "sequence")
 

@@ -1,4 +1,4 @@
-"""The policy and preference losses where a term is infinite or nothing, on the CPU and (marked) on the GPU."""
+"""The policy and preference losses where a term is infinite or nothing, and with as many sequences as tokens, on the CPU and (marked) on the GPU."""
 import math
 
 import pytest
@@ -43,3 +43,25 @@ def test_the_gradient_of_the_kl_term_stays_without_an_advantage(device):
     assert abs(float(loss.detach()) - want) <= 1e-6
     dy, = torch.autograd.grad(loss, y)
     assert all(abs(float(g) + 0.25 * math.expm1(x)) <= 1e-6 for g, x in zip(dy, (0.5, -0.5)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("wide", [False, True])
+def test_as_many_sequences_as_tokens(device, wide):
+    """Two of the four sequences are empty.  A shape that is the log probabilities' own is a value for every token, any other one for every
+    sequence: tokens 0 and 1 are sequence 1, tokens 2 and 3 are sequence 3."""
+    cu = torch.tensor([0, 0, 2, 2, 4], device=device, dtype=torch.int64 if wide else torch.int32)
+    y = torch.zeros(4, device=device)
+    adv = torch.tensor([1.0, 2.0, 3.0, 4.0], device=device)
+    by_token, by_sequence = -2.5, -3.0
+    for rows, a, want in ((y, adv, by_token), (y, adv[:, None], by_sequence), (y[None], adv[None], by_token), (y[None], adv, by_sequence),
+                          (y[None], adv[:, None], by_sequence)):
+        for leaf in (rows, rows.clone().requires_grad_(True)):
+            loss, stats = ops.policy_loss(leaf, torch.zeros_like(rows), a, cu_seqlens=cu)
+            assert float(loss.detach()) == want and float(stats[0]) == want
+            if leaf.requires_grad:
+                dy, = torch.autograd.grad(loss, leaf)
+                assert dy.reshape(-1).tolist() == ([-0.25, -0.5, -0.75, -1.0] if want == by_token else [-0.5, -0.5, -1.0, -1.0])
+    # the tokens behind the last offset belong to no sequence
+    loss, _ = ops.policy_loss(y, torch.zeros_like(y), adv[:, None], cu_seqlens=torch.tensor([0, 0, 1, 1, 3], device=device))
+    assert abs(float(loss) + (2.0 + 4.0 + 4.0) / 3) <= 1e-6
