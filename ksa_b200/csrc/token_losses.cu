@@ -5,7 +5,7 @@
 // sequence's mean.  L is cut off, and has no gradient, where A > 0 and d > log(1 + high) or A < 0 and d < log(1 - low); elsewhere
 // dL / dy = -A r, and dK / dy = 1 - exp(x).
 // Preference loss.  D_s = sum over the valid tokens of sequence s of y - y_ref, z_i = beta (D_2i - D_2i+1); the loss is the mean over the
-// pairs of log(1 + exp(-z)) + smoothing z, and dz = smoothing - 1 / (1 + exp(z)).
+// pairs of (1 - smoothing) log(1 + exp(-z)) + smoothing log(1 + exp(z)), and dz = smoothing - 1 / (1 + exp(z)).
 //
 // Bound: memory from some hundred thousand tokens on (17 bytes of a token read by the policy loss, 9 by the preference loss), launches
 // below.  The policy loss writes each token's gradient up to the normaliser in the same pass, in 32 bits, and the backward pass reads
@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(1024) preference_finish_kernel(const Preferenc
     const int s = s0 + 2 * threadIdx.x;
     if (threadIdx.x < 512 && s < q.S) {
       const double better = sum_of[2 * threadIdx.x], worse = sum_of[2 * threadIdx.x + 1], z = (double)a.beta * (better - worse);
-      loss[0] += log1p(exp(-fabs(z))) + fmax(-z, 0.0) + (isnan(z) ? z : a.smoothing != 0.f ? (double)a.smoothing * z : 0);
+      const double even = 1 - (double)a.smoothing, one = fmax(-z, 0.0), other = fmax(z, 0.0);       // (a weight of zero takes no infinity)
+      loss[0] += isnan(z) ? z : log1p(exp(-fabs(z))) + (even > 0 ? even * one : 0) + (a.smoothing > 0.f ? (double)a.smoothing * other : 0);
       const double dz = ((double)a.smoothing - 1 / (1 + exp(z))) * (double)a.beta / (q.S / 2);
       a.coef[s] = (float)dz;
       a.coef[s + 1] = (float)-dz;

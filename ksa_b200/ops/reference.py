@@ -391,7 +391,11 @@ def preference_loss(log_probs, ref_log_probs, mask, of, sequences: int, beta: fl
         v = v - torch.where(valid, ref_log_probs, ref_log_probs.new_zeros(())).double()
     rewards = beta * torch.zeros(sequences + 1, dtype=torch.float64, device=v.device).index_add(0, of, v)[:sequences].view(-1, 2)
     z = rewards[:, 0] - rewards[:, 1]
-    per = F.softplus(-z) + label_smoothing * z if label_smoothing else F.softplus(-z)
+    per = torch.zeros_like(z)                  # (a weight of zero takes no infinity)
+    if label_smoothing < 1:
+        per = per + (1 - label_smoothing) * F.softplus(-z)
+    if label_smoothing > 0:
+        per = per + label_smoothing * F.softplus(z)
     return (per.sum() / max(z.numel(), 1)).float(), rewards.detach().float()
 
 

@@ -65,3 +65,21 @@ def test_as_many_sequences_as_tokens(device, wide):
     # the tokens behind the last offset belong to no sequence
     loss, _ = ops.policy_loss(y, torch.zeros_like(y), adv[:, None], cu_seqlens=torch.tensor([0, 0, 1, 1, 3], device=device))
     assert abs(float(loss) + (2.0 + 4.0 + 4.0) / 3) <= 1e-6
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 1.0])
+def test_preference_at_infinities(device, smoothing):
+    """(1 - s) log(1 + exp(-z)) + s log(1 + exp(z)): infinite on the side that counts, and never infinity less infinity."""
+    for better, worse, z in ((-INF, 0.0, -INF), (0.0, -INF, INF), (-1e30, 0.0, -1e30), (0.0, -1e30, 1e30)):
+        y = torch.tensor([[better, 0.0], [worse, 0.0]], device=device, requires_grad=True)
+        loss, rewards = ops.preference_loss(y, beta=1.0, label_smoothing=smoothing)
+        weight = 1 - smoothing if z < 0 else smoothing
+        want = weight * abs(z) if weight else 0.0
+        assert float(loss.detach()) == want or abs(float(loss.detach()) - want) <= 2.0 ** -22 * want
+        assert rewards.flatten().tolist() == [float(torch.tensor(better)), float(torch.tensor(worse))]
+        g = smoothing - (1.0 if z < 0 else 0.0)
+        dy, = torch.autograd.grad(loss, y)
+        assert all(abs(float(a) - b) <= 2.0 ** -23 for a, b in zip(dy.flatten(), (g, g, -g, -g)))
+    both = torch.full((2, 1), -INF, device=device)
+    assert math.isnan(float(ops.preference_loss(both, label_smoothing=smoothing)[0]))
