@@ -141,7 +141,7 @@ __device__ __forceinline__ ExpLess exp_less(float x) {
   ExpLess e;
   if (!(fabsf(x) < 1.f)) {
     e.one = expf(x) - 1.f;
-    e.line = e.one - x;
+    e.line = e.one == INFINITY ? INFINITY : e.one - x;                            // (x itself may be infinite)
     return e;
   }
   float p = 1.f / 479001600.f;                                                    // 1 / 12!

@@ -368,7 +368,9 @@ def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, of, s
     part = torch.where(cut, -bound * a, -torch.exp(torch.where(still, torch.zeros_like(d), d)) * torch.where(still, torch.zeros_like(a), a))
     part = torch.where(valid, part, torch.zeros_like(part))
     x = pick(ref_log_probs) - y if ref_log_probs is not None else torch.zeros_like(y)
-    kl = torch.expm1(x) - x
+    far = x == math.inf                        # (by the exponential alone: neither infinity less infinity nor the gradient of that)
+    near = torch.where(far, torch.zeros_like(x), x)
+    kl = torch.where(far, torch.exp(torch.where(far, x, torch.zeros_like(x))), torch.expm1(near) - near)
     weight = valid.double()
     if by_sequence:
         count = torch.zeros(sequences + 1, dtype=torch.float64, device=y.device).index_add_(0, of, weight)[:sequences]

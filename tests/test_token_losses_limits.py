@@ -83,3 +83,27 @@ def test_preference_at_infinities(device, smoothing):
         assert all(abs(float(a) - b) <= 2.0 ** -23 for a, b in zip(dy.flatten(), (g, g, -g, -g)))
     both = torch.full((2, 1), -INF, device=device)
     assert math.isnan(float(ops.preference_loss(both, label_smoothing=smoothing)[0]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_infinite_kl_term(device):
+    """exp(x) - 1 - x grows beyond all numbers on both sides."""
+    for x in (INF, -INF, 200.0, -1e30):
+        ref = torch.tensor([x], device=device)
+        loss, stats = ops.policy_loss(torch.zeros(1, device=device), torch.zeros(1, device=device), torch.zeros(1, device=device), ref, kl_coef=1.0)
+        assert float(loss) == float(stats[1]) and (float(loss) == INF if x != -1e30 else abs(float(loss) - 1e30) <= 1e24)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradient_of_an_infinite_kl_term(device):
+    """-(exp(x) - 1): beyond all numbers where the reference has a token that the model has not, 1 where it is the other way round."""
+    y = torch.zeros(3, device=device, requires_grad=True)
+    ref, adv = _on(device, [INF, -INF, 0.0], [0.0, 0.0, 1.0])
+    loss, stats = ops.policy_loss(y, torch.zeros_like(y), adv, ref, kl_coef=0.5)
+    dy, = torch.autograd.grad(loss, y)
+    assert float(loss.detach()) == INF and stats.tolist()[1] == INF
+    assert float(dy[0]) == -INF and abs(float(dy[1]) - 0.5 / 3) <= 2.0 ** -24 and abs(float(dy[2]) + 1 / 3) <= 2.0 ** -24
+    # without a coefficient the reference counts in the statistics alone
+    loss, stats = ops.policy_loss(y, torch.zeros_like(y), adv, ref)
+    assert abs(float(loss.detach()) + 1 / 3) <= 2.0 ** -24 and float(stats[1]) == INF
+    assert torch.equal(torch.autograd.grad(loss, y)[0].cpu(), torch.tensor([0.0, 0.0, -1 / 3]))
