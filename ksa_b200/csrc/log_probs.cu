@@ -48,6 +48,8 @@ constexpr int kLpStatCols = 128;                                        // colum
 // products came out 9e-7 of itself too small, and at a temperature of 0.6 y was off by 1.6e-6.  The epilogue adds the parts of 1024 products up:
 // 5e-7, for 1 % of the time (8192 x 151936 x 2048 3830 -> 3862 us; parts of 512 2.9e-7 and 3960).  An epilogue thread then keeps 128 sums in registers, so
 // that both groups of its warps share every tile; of narrower heads each takes every other tile, which costs less per tile (width 128 207 us, 235 shared).
+// kGrad takes its logits whole: 9e-7 of a logit of 30 is 3e-5 of a probability, next to nothing beside dx's rounding (2^-9), and the label's 1 - p, where it
+// would not be, comes from the forward pass.
 constexpr int kLpChunk = 16;
 constexpr float kLpCodes = 1024.f;                                      // codes of a kept logit to a power of two
 // Pitches of the arrays that are made here, in elements: rows that begin on 128 bytes are loaded in whole lines.  A width of 1352 as pitch took a third
@@ -69,6 +71,7 @@ struct LpArgs {
   float* tops;                 // kStatsKeep: [ceil(N / 128)][ld_stats] maxima, base 2
   long long ld_stats;
   const float* lse2;           // kGrad: [rows]
+  const float* picked2;        // kGrad: [rows] the label's logit less the log-sum, base 2
   const float* dy;             // kGrad: gradient of y, by the rows' places
   int col0;                    // kGrad: first column of the slab
   int dh, dw;                  // kProducts: which are wanted
@@ -448,9 +451,11 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
               float d[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) d[j] = -g * fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -lse2));
-              if (__any_sync(0xffffffffu, at >= 0 && at < 32))
+              if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {         // 1 - p of the label: from the forward pass, as in log_probs_decode_kernel
+                const float mine = at >= 0 && at < 32 ? g * (1.f - fast_exp2(a.picked2[row])) : 0.f;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) d[j] = j == at ? d[j] + g : d[j];
+                for (int j = 0; j < 32; ++j) d[j] = j == at ? mine : d[j];
+              }
 #pragma unroll
               for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
             }
@@ -1098,13 +1103,13 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     LpArgs a{};
     a.count = static_cast<const int*>(count); a.rows = static_cast<const int*>(rows); a.row_label = static_cast<const int*>(row_label);
     a.scale2 = (float)(1.4426950408889634 / (double)tau); a.inv_tau = 1.f / tau;
-    a.lse2 = static_cast<const float*>(lse2); a.dy = static_cast<const float*>(dy); a.col0 = (int)v0;
+    a.lse2 = static_cast<const float*>(lse2); a.picked2 = a.lse2 + T; a.dy = static_cast<const float*>(dy); a.col0 = (int)v0;
     if (codes) {
       const int col_blocks = (V + kLpDecodeCols - 1) / kLpDecodeCols;
       const long long blocks = (T + 63LL) / 64 * 8 * col_blocks;
       KSA_REQUIRE(blocks < (1LL << 31), "log_probs: %d x %d kept logits", T, V);
       KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * V, log_probs_decode_kernel, dim3((unsigned)blocks), dim3(256), 0, st, (const uint16_t*)codes,
-                                          (long long)slab, (const float*)tops, (T + 3LL) / 4 * 4, a.lse2, a.lse2 + T, a.dy, a.rows, a.row_label, a.count,
+                                          (long long)slab, (const float*)tops, (T + 3LL) / 4 * 4, a.lse2, a.picked2, a.dy, a.rows, a.row_label, a.count,
                                           (bf16*)dx, V, a.inv_tau, col_blocks));
     } else {
       a.M = T; a.N = n; a.K = D;

@@ -85,3 +85,10 @@ def test_probabilities_at_logits_of_thousands(T, V, factor, steps, unit, tau, lo
     sampling temperature of a hundredth."""
     h, w, labels, dy, own = _exact(T, V, -(-(T + 48) // 8) * 8, factor, steps, unit, False, seed=T)
     _check(h, w, labels, dy, own, tau, logits == "kept")
+
+
+@pytest.mark.parametrize("T,V,D", [(64, 500, 136), (64, 500, 2056), (300, 1002, 1096)])
+def test_gradient_of_a_label_next_to_probability_one(T, V, D, logits):
+    """1 - p from 2e-2 down to 3e-6, with logits of a few hundred."""
+    h, w, labels, dy, own = _exact(T, V, D, 1, (16, 52), 0.25, True, seed=T + D)
+    _check(h, w, labels, dy, own, 1.0, logits == "kept")
