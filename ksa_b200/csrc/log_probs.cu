@@ -78,6 +78,7 @@ struct LpArgs {
   int add_dh, add_dw;          // into fp32, added to what is there
   int planes;                  // dh: K is cut into at most so many parts, each with an output of its own
   int plane_rows;
+  int* parts;                  // dh: how many parts it is
   int bf16_out;                // dw
   int* status;
 };
@@ -90,7 +91,7 @@ __device__ __forceinline__ float lp_dw_steps(int n, int D, int count) {
 }
 // Parts that K (the vocabulary) is cut into for dh.  Its tiles are few and long, 160 for 4915 rows of 2048 on 74 pairs, and the last wave of whole ones would be
 // a third of the time (2594 us by itself, in parts 2300) where dw's tiles do not fill it.  Every part has an output of its own, which the
-// scattering kernel adds up in order.  The rule takes the fewest steps of kLpBK on the busiest pair or, if that is more, of all pairs on average with dw's
+// scattering kernel adds up in order: it is told how many there are, as a rule in fp32 may come out differently in another kernel.  The rule takes the fewest steps of kLpBK on the busiest pair or, if that is more, of all pairs on average with dw's
 // (`other`); a tile of a part costs 0.13 more to be read again.  By every warp, whose lanes try two numbers each.
 __device__ __forceinline__ int lp_parts(int tiles, int num_kb, int n_pairs, int most, float other) {
   if (most <= 1 || num_kb <= 0 || tiles >= 64 * n_pairs) return 1;
@@ -237,8 +238,9 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
   const int M = min(count, a.M), N = a.N;
   const LpTiles dh(kMode == kProducts && a.dh ? M : 0, a.N, a.K);
   const LpTiles main_tiles(kMode != kProducts ? M : a.dw ? a.K : 0, a.N, kMode != kProducts ? a.K : M);
-  const LpSchedule work_of(dh, main_tiles, pair, n_pairs,
-                           kMode == kProducts && dh.all > 0 ? lp_parts(dh.all, dh.num_kb, n_pairs, a.planes, a.dw ? lp_dw_steps(a.K, a.N, M) : 0.f) : 1);
+  const int parts = kMode == kProducts && dh.all > 0 ? lp_parts(dh.all, dh.num_kb, n_pairs, a.planes, a.dw ? lp_dw_steps(a.K, a.N, M) : 0.f) : 1;
+  if (kMode == kProducts && a.dh && blockIdx.x == 0 && threadIdx.x == 0) *a.parts = dh.all > 0 ? parts : 0;
+  const LpSchedule work_of(dh, main_tiles, pair, n_pairs, parts);
   const int num_kb = main_tiles.num_kb;
 
   if (warp == 0) {
@@ -914,12 +916,10 @@ log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* top
 // share them where there are few values and may be many parts (one row in 64 parts 39 us by one thread each, 6 by 8; 4915 rows in 6 parts 54 and 124).
 template <int kSplit>
 __global__ void __launch_bounds__(256)
-log_probs_scatter_kernel(const float* dense, const int* place, const int* count, bf16* dh, int T, int D, int n, int n_pairs, int planes, int dw, long long plane) {
+log_probs_scatter_kernel(const float* dense, const int* place, const int* parts_made, bf16* dh, int T, int D, long long plane) {
   __shared__ float4 sums[kSplit][256 / kSplit];
   grid_dependency_enter();
-  const int rows = min(*count, T), per_row = D / 4;
-  const LpTiles tiles(rows, D, n);
-  const int parts = tiles.all > 0 ? lp_parts(tiles.all, tiles.num_kb, n_pairs, planes, dw ? lp_dw_steps(n, D, rows) : 0.f) : 0;
+  const int parts = *parts_made, per_row = D / 4;
   const int lane = threadIdx.x % (256 / kSplit), first = threadIdx.x / (256 / kSplit);
   const long long all = (long long)T * per_row;
   for (long long i0 = blockIdx.x * (256LL / kSplit); i0 < all; i0 += gridDim.x * (256LL / kSplit)) {
@@ -1078,7 +1078,8 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
 
 // Backward.  dy [T] fp32; dh [T, D] bf16 or null; dw [V, D] (row pitch lddw) or null, bf16 or (dw_fp32) fp32, there with add_dw added to.
 // dx: bf16 [T rounded up to 256, slab], the vocabulary's columns being taken `slab` at a time (a multiple of 8; with codes: V rounded up to 64).
-// dh32: fp32 [planes, T rounded up to 256, D] where dh is wanted, 1 to 64 planes, only one where not all columns are taken at a time.
+// dh32: fp32 [planes, T rounded up to 256, D] where dh is wanted, 1 to 64 planes, only one where not all columns are taken at a time; and one word
+// (int32) behind the planes, how many of them were used.
 KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows, const void* row_label, const void* place, const void* count,
                               const void* lse2, const void* codes, const void* tops, const void* dy, void* dx, void* dh32, void* dh, void* dw, int T, int V, int D, long long ldw,
                               long long lddw, int dw_fp32, int add_dw, int slab, int planes, float tau, void* stream) {
@@ -1093,6 +1094,7 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
   cudaStream_t st = ST(stream);
   const int padded = (T + kLpRowPad - 1) / kLpRowPad * kLpRowPad;
   const bool together = lp_together(T, D, V < slab ? V : slab, dh != nullptr, dw != nullptr, sm_count());
+  float* planes_end = dh ? static_cast<float*>(dh32) + (long long)planes * padded * D : nullptr;
   LpMaps grad, by_w, by_h;                                               // dx again; dx w; dx^T h
   int rc = lp_map(&grad.A, dense, 2, D, padded, lp_pitch(D), kLpBM);
   if (rc == 0) rc = lp_map(&by_h.B, dense, 2, D, padded, lp_pitch(D), 64);
@@ -1119,7 +1121,7 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     }
     if (rc == 0 && (dh || dw)) {
       a.M = T; a.N = D; a.K = n; a.dh = a.dw = 1; a.add_dh = v0 > 0; a.add_dw = add_dw;
-      a.planes = planes; a.plane_rows = padded; a.bf16_out = !dw_fp32;
+      a.planes = planes; a.plane_rows = padded; a.parts = reinterpret_cast<int*>(planes_end); a.bf16_out = !dw_fp32;
       if (dh) {
         rc = lp_map(&by_w.A, dx, 2, n, padded, slab, kLpBM);
         if (rc == 0) rc = lp_map(&by_w.B, wv, 2, D, n, ldw, 64);
@@ -1144,9 +1146,7 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     const long long blocks = ((long long)T * (D / 4) * split + 255) / 256;
     KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, split > 1 ? log_probs_scatter_kernel<8> : log_probs_scatter_kernel<1>,
                                         dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const float*)dh32, (const int*)place,
-                                        (const int*)count, (bf16*)dh, T, D, V < slab ? V : slab,
-                                        lp_pairs(lp_product_units(T, D, V < slab ? V : slab, true, together, planes), sm_count()), planes, (int)together,
-                                        (long long)padded * D));
+                                        (const int*)planes_end, (bf16*)dh, T, D, (long long)padded * D));
   }
   return 0;
 }

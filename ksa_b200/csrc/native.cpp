@@ -1187,7 +1187,7 @@ struct LogProbsNode : public torch::autograd::Function<LogProbsNode> {
     const long long planes = slab < V ? 1 : std::max(1ll, std::min(64ll, (long long)ctx->saved_data["plane_bytes"].toInt() / (4 * padded * D)));
     if (need_h) {
       dh = at::empty(ctx->saved_data["shape"].toIntVector(), on(w, at::kBFloat16));
-      dh32 = at::empty({(int64_t)planes, (int64_t)padded, (int64_t)D}, on(w, at::kFloat));
+      dh32 = at::empty({(int64_t)(planes * padded * D + 1)}, on(w, at::kFloat));               // (the word behind them: how many were used)
     }
     if (need_w) dw = at::empty({(int64_t)V, (int64_t)D}, on(w, at::kBFloat16));
     const int* p = static_cast<const int*>(kept.const_data_ptr());

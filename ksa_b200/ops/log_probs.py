@@ -69,6 +69,7 @@ class _LinearLogProbsFn(torch.autograd.Function):
         T, (V, D), dev = rows.shape[0], w.shape, w.device
         need_h, need_w = ctx.needs_input_grad[:2]
         dh = dw = dh32 = None
+        planes = 1
         with torch.cuda.device(dev):
             dy = dy.to(torch.float32).contiguous()
             weight = _pitched(w)
@@ -76,12 +77,12 @@ class _LinearLogProbsFn(torch.autograd.Function):
             if need_h:
                 dh = torch.empty((T, D), dtype=w.dtype, device=dev)
                 planes = _planes(dense.shape[0], D) if dx.shape[1] >= V else 1
-                dh32 = torch.empty((planes, dense.shape[0], D), dtype=torch.float32, device=dev)
+                dh32 = torch.empty(planes * dense.shape[0] * D + 1, dtype=torch.float32, device=dev)      # (the word behind them: how many were used)
 
             def run(out, add):
                 _lib.call("ksa_log_probs_bwd", dense, weight, rows, row_label, place, count, lse2, codes, tops, dy, dx, dh32, dh, out, T, V, D,
                           weight.stride(0), out.stride(0) if out is not None else D, int(out is not None and out.dtype == torch.float32),
-                          int(add), dx.shape[1], 1 if dh32 is None else dh32.shape[0], float(ctx.temperature))
+                          int(add), dx.shape[1], planes, float(ctx.temperature))
 
             if not need_w:
                 run(None, False)

@@ -9,11 +9,14 @@ log-sum is one 32-bit number: half a step, 2^-24 of it.  Exponentials (2^-22), t
 sum's roundings: 2^-20.  Kept logits: half a step of 2^-10 of a power of two, 2^-11.5 of the probability; not so the label's, which comes
 from the exact logit by way of a distance that is rounded by itself.  dx is rounded to bf16, 2^-8.
 """
+from types import SimpleNamespace
+
 import pytest
 import torch
 
 from ksa_b200 import ops
 from ksa_b200.ops import log_probs as impl
+from test_log_probs_gpu import _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +95,39 @@ def test_gradient_of_a_label_next_to_probability_one(T, V, D, logits):
     """1 - p from 2e-2 down to 3e-6, with logits of a few hundred."""
     h, w, labels, dy, own = _exact(T, V, D, 1, (16, 52), 0.25, True, seed=T + D)
     _check(h, w, labels, dy, own, 1.0, logits == "kept")
+
+
+@pytest.mark.parametrize("T,D,V", [(1, 152, 99667), (70, 64, 4096), (300, 136, 1000), (333, 256, 4096), (600, 512, 20000), (1300, 1024, 30000), (4100, 128, 2000)])
+@pytest.mark.parametrize("answer", [1.0, 0.4, 0.0])
+@pytest.mark.parametrize("head", [True, False])
+def test_parts_of_the_rows_gradient_are_those_that_were_written(T, D, V, answer, head, monkeypatch):
+    """The products say how many parts they made, and so many are added up; the memory of the others holds anything."""
+    h, w, labels, dy = _inputs(T, D, V, answer, seed=T)
+    seen = []
+    call = impl._lib.call
+
+    def watched(name, *args):
+        if name != "ksa_log_probs_bwd":
+            return call(name, *args)
+        parts, dh, planes, rows = args[11], args[12], args[22], args[0].shape[0]
+        parts.fill_(float("nan"))
+        call(name, *args)
+        made = int(parts.view(torch.int32)[planes * rows * D])
+        seen.append((made, planes))
+        planes_of = parts[:planes * rows * D].view(planes, rows, D)
+        count = int(args[5][0])
+        assert (made == 0) if count == 0 else 1 <= made <= planes
+        assert planes_of[made:].isnan().all() and planes_of[:made, :count].isfinite().all()
+        total = torch.zeros(T, D, device="cuda", dtype=torch.float64)
+        at = args[2][:count].long()
+        total[at] = planes_of[:made, :count].double().sum(0)
+        # added up in 32 bits, in order or by eight at a time: 64 roundings of partial sums at most
+        bound = torch.zeros_like(total)
+        bound[at] = planes_of[:made, :count].double().abs().sum(0)
+        assert ((dh.double() - total).abs() <= 2.0 ** -8 * total.abs() + 2.0 ** -17 * bound + 2.0 ** -130).all()
+    monkeypatch.setattr(impl._lib, "call", watched)
+    monkeypatch.setattr(impl, "_native", SimpleNamespace(linear_log_probs=lambda *args: None))
+    h.requires_grad_()
+    w.requires_grad_(head)
+    torch.autograd.grad(ops.linear_log_probs(h, w, labels), (h, w) if head else h, dy)
+    assert len(seen) == 1
