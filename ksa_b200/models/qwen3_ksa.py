@@ -401,7 +401,8 @@ class Qwen3Model(Model):
         """``tokens`` ``[B, L]`` -> loss (with ``labels``), hidden ``[B, L, D]`` or logits ``[B, L, V]``.
 
         ``log_probs``: with ``labels``, their log probabilities ``[B, L]`` instead of the loss (fp32, at a sampling ``temperature``, 0 where a
-        label is ignored): what the losses of :mod:`ksa_b200.losses.post_training` take.
+        label is ignored): what the losses of :mod:`ksa_b200.losses.post_training` take.  An output head that is sharded by tensor
+        parallelism and sequences that are sharded by context parallelism are refused: those losses need whole answers.
 
         ``cu_seqlens`` (token offsets of documents packed into the sequence, the same for every sequence of the batch):
         full-attention layers keep every query inside its own document (the reference's varlen FlashAttention-2 path,
@@ -411,6 +412,14 @@ class Qwen3Model(Model):
         ``labels`` are already shifted (label of position t is token t+1) with ``ignore_index`` where masked,
         as the reference trainer builds them (``recipes/pretrain_kai_summary_unified.py:867-873``).
         """
+        if log_probs:
+            if labels is None or self.skip_output_layer:
+                raise ValueError("log_probs needs labels and the output head")
+            if self.lm_head_weight.shape[0] != self.config.vocab_size:
+                raise ValueError("log_probs needs the whole output head on this rank")
+            if self.cp is not None:
+                raise ValueError("log_probs of a shard of the sequence are parts of answers, and their losses need whole ones: under context parallelism take "
+                                 "ops.linear_log_probs of the rows that return_hidden=True gives, and gather them")
         B, L = tokens.shape
         # use_summary=False runs every layer as plain causal attention on the base projections (the distillation
         # teacher: same weights, no summary tokens, recipes/pretrain_kai_summary_unified.py:967-997)
@@ -441,10 +450,6 @@ class Qwen3Model(Model):
                          self.config.norm_eps)
         self.last_attn_outputs = collect
         if log_probs:
-            if labels is None or self.skip_output_layer:
-                raise ValueError("log_probs needs labels and the output head")
-            if self.lm_head_weight.shape[0] != self.config.vocab_size:
-                raise ValueError("log_probs needs the whole output head on this rank")
             return ops.linear_log_probs(h, self.lm_head_weight, labels.reshape(-1), ignore_index, temperature).view(B, L)
         if labels is not None and not self.skip_output_layer:
             return ops.linear_cross_entropy(h, self.lm_head_weight, labels.reshape(-1), ignore_index,
