@@ -415,6 +415,8 @@ class Qwen3Model(Model):
         if log_probs:
             if labels is None or self.skip_output_layer:
                 raise ValueError("log_probs needs labels and the output head")
+            if last_token_only:
+                raise ValueError("log_probs are of every position: last_token_only returns logits")
             if self.lm_head_weight.shape[0] != self.config.vocab_size:
                 raise ValueError("log_probs needs the whole output head on this rank")
             if self.cp is not None:
