@@ -91,7 +91,8 @@ class FsdpEngine(TrainEngine):
         from .groups import spans_nodes
         # the fused back end reaches the other ranks through CUDA IPC peer memory, which ends at the node
         one_node = not spans_nodes(world_size)
-        self.comm = comm or ("fused" if torch.device(dev).type == "cuda" and world_size > 1 and one_node
+        # ... and reduces and updates a unit in one kernel, before the norm of all units' gradients is known
+        self.comm = comm or ("fused" if torch.device(dev).type == "cuda" and world_size > 1 and one_node and not kw.get("clip_norm")
                              else "collective")
         if self.comm == "fused" and not one_node:
             raise ValueError("comm='fused' needs all ranks on one node (peer memory); use comm='collective' across nodes")

@@ -57,7 +57,7 @@ def get_argument_parser() -> argparse.ArgumentParser:
     a("--fp32-reduce", action="store_true", help="fp32 gradient reduction (always on in this engine)")
     a("--reshard-after-forward", action="store_true")
     a("--prefetch-params-in-forward", action="store_true")
-    a("--comm", default=None, choices=["fused", "collective"], help="FSDP back end (default: fused on GPUs)")
+    a("--comm", default=None, choices=["fused", "collective"], help="FSDP back end (default: fused on GPUs, collective with --clip-norm)")
     a("--overlap", default="auto", choices=["auto", "stream", "gemm2"],
       help="fused back end: parameter gathers on a side stream, or inside the gate/up GEMM launches (auto: gemm2 for "
            "plain FSDP on 4 or more GPUs, else stream)")
@@ -74,7 +74,8 @@ def get_argument_parser() -> argparse.ArgumentParser:
     a("--beta1", type=float, default=0.9)
     a("--beta2", type=float, default=0.95)
     a("--clip-range", type=float, default=1.0)
-    a("--clip-norm", type=float, default=0.0, help="scale the gradients of a step down to this global 2-norm, ahead of --clip-range (0: not)")
+    a("--clip-norm", type=float, default=0.0, help="scale the gradients of a step down to this global 2-norm, ahead of --clip-range (0: not); "
+      "on several GPUs with the collective back end")
     a("--use-flash-attention-2", action="store_true")
     a("--enable-gradient-checkpointing", action="store_true")
     a("--gradient-checkpointing-mode", default="full", choices=["full", "mlp"],
