@@ -69,6 +69,75 @@ def _collide(src: Sequence[torch.Tensor], dst: Sequence[torch.Tensor]) -> bool:
     return False
 
 
+def _layout(t: torch.Tensor) -> List[Tuple[int, int]]:
+    """(stride in bytes, size) of the dimensions that have more than one element, the widest first."""
+    return sorted(((st * t.element_size(), n) for n, st in zip(t.shape, t.stride()) if n > 1), reverse=True)
+
+
+def _end(t: torch.Tensor) -> int:
+    return t.data_ptr() + sum((n - 1) * st for st, n in _layout(t)) + t.element_size()
+
+
+def _folded(t: torch.Tensor) -> bool:
+    """Whether elements of ``t`` may share memory with one another: a dimension steps over less than those below it take."""
+    reach = t.element_size()
+    for st, n in reversed(_layout(t)):
+        if st < reach:
+            return True
+        reach += (n - 1) * st
+    return False
+
+
+_MOST_STEPS = 10000         # of the search below; layouts that take more count as meeting
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of ``a`` has memory in common with one of ``b``, by the difference of their places: a sum of strides, each as often as
+    the indices of the two may differ, which has to come within an element of the distance between the tensors."""
+    often = {}
+    for t, sign in ((a, 1), (b, -1)):
+        for st, n in _layout(t):
+            lo, hi = often.get(st, (0, 0))
+            often[st] = (lo, hi + n - 1) if sign > 0 else (lo - n + 1, hi)
+    dims = sorted(often.items(), reverse=True)
+    low, high = [0], [0]                                # what the strides from here on can add up to
+    for st, (lo, hi) in reversed(dims):
+        low.insert(0, low[0] + lo * st)
+        high.insert(0, high[0] + hi * st)
+    apart = b.data_ptr() - a.data_ptr()
+    first, last = apart - a.element_size() + 1, apart + b.element_size() - 1
+    steps = 0
+
+    def search(i: int, at: int) -> bool:
+        nonlocal steps
+        steps += 1
+        if steps > _MOST_STEPS:
+            return True
+        if i == len(dims):
+            return first <= at <= last
+        st, (lo, hi) = dims[i]
+        lo, hi = max(lo, -((at + high[i + 1] - first) // st)), min(hi, (last - at - low[i + 1]) // st)
+        return any(search(i + 1, at + k * st) for k in range(lo, hi + 1))
+    return search(0, 0)
+
+
+def _share(targets: Sequence[torch.Tensor]) -> bool:
+    """Whether two of the targets, or two elements of one, have memory in common; those that fill theirs are compared by :func:`_collide`."""
+    targets = [(t, _dense(t)) for t in targets if t.numel() > 0]
+    if all(dense for _, dense in targets):
+        return False
+    if any(not dense and _folded(t) for t, dense in targets):
+        return True
+    targets = sorted(((t.data_ptr(), _end(t), dense, t) for t, dense in targets), key=lambda x: x[:2])
+    for i, (_, end, dense, t) in enumerate(targets):
+        for lo, _, other_dense, other in targets[i + 1:]:
+            if lo >= end:
+                break
+            if not (dense and other_dense) and _meet(t, other):
+                return True
+    return False
+
+
 def _launch(src: Sequence[torch.Tensor], dst: Optional[Sequence[torch.Tensor]], scale: float, most: float) -> Tuple[torch.Tensor, torch.Tensor]:
     device = src[0].device
     n = len(src)
@@ -105,7 +174,7 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float, scale: float
                     out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Multiply every gradient by ``scale * min(1, max_norm / (norm + 1e-6))`` and return ``norm``, the global 2-norm times
     ``scale``.  In place, or into the tensors ``out`` (of the gradients' shapes and types); gradients that share memory with
-    one another are refused.  A norm that is no number makes all of them so, an infinite one makes them zero where they are finite."""
+    one another are refused (those that only interleave, as the columns of one matrix do, are fine).  A norm that is no number makes all of them so, an infinite one makes them zero where they are finite."""
     grads = grads if isinstance(grads, (list, tuple)) else list(grads)
     if not _observed():
         made = _native.grad_norm(grads, out, 2, scale, max_norm)
@@ -117,8 +186,8 @@ def clip_grad_norm_(grads: Iterable[torch.Tensor], max_norm: float, scale: float
     if len(to) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device for o, g in zip(to, grads)):
         raise ValueError("the clipped gradients go into tensors of the same number, shapes, types and device")
     with torch.no_grad():
-        if any(t.numel() > 1 and any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())) for t in to):
-            raise ValueError("clipped gradients cannot go into one value expanded")
+        if _share(to):
+            raise ValueError("gradients that are clipped must not share memory")
         # values that do not fill their memory, or in another order than their target's: through a copy
         src = [g if _dense(g) and g.stride() == o.stride() else g.contiguous() for g, o in zip(grads, to)]
         dst = [o if s.stride() == o.stride() and _dense(o) else torch.empty_like(s) for s, o in zip(src, to)]

@@ -1,0 +1,101 @@
+"""Clipping of gradients that share memory, in layouts that do not fill theirs: refused where they meet, clipped where they only interleave."""
+import random
+
+import pytest
+import torch
+
+from ksa_b200 import ops
+from ksa_b200.ops import clipping
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _base(device):
+    return torch.arange(1.0, 241.0, device=device).view(12, 20)
+
+
+MEET = {
+    "the same columns twice": lambda b: [b[:, ::2], b[:, ::2]],
+    "columns that overlap": lambda b: [b[:, :7], b[:, 6:13]],
+    "a row and columns": lambda b: [b[3], b[:, 4:9]],
+    "one value of a row": lambda b: [b[5, 7:8], b[:, ::7]],
+    "steps of two and of three": lambda b: [b.view(-1)[::2], b.view(-1)[3::3]],
+    "transposed": lambda b: [b[2:5, 2:5], b.t()[4:9, 4:9]],
+    "another type": lambda b: [b[:, :5], b.view(torch.bfloat16)[:, 9:12]],
+}
+APART = {
+    "even and odd columns": lambda b: [b[:, ::2], b[:, 1::2]],
+    "left and right": lambda b: [b[:, :7], b[:, 7:]],
+    "a column and the others": lambda b: [b[:, 0], b[:, 1:]],
+    "rows, and columns of the others": lambda b: [b[:4], b[4:, :3], b[4:, 3:]],
+    "steps of six": lambda b: [b.view(-1)[::6], b.view(-1)[3::6], b.view(-1)[4::6]],
+    "a block and one around it": lambda b: [b[2:5, 2:5], b[:2], b[5:], b[2:5, 5:], b[2:5, :2].t()],
+    "another type": lambda b: [b[:, :5], b.view(torch.bfloat16)[:, 10:12]],
+}
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("case", MEET)
+def test_shared_memory_is_refused(device, case):
+    base = _base(device)
+    views = MEET[case](base)
+    for grads in (views, views[::-1]):
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_(grads, 1.0)
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_([torch.ones_like(v, memory_format=torch.contiguous_format) for v in grads], 1.0, out=grads)
+    assert torch.equal(base, _base(device))
+    # what is only read may be shared
+    out = [torch.empty_like(v, memory_format=torch.contiguous_format) for v in views]
+    norm = ops.clip_grad_norm_(views, 1.0, out=out)
+    want = sum(float(v.double().square().sum()) for v in views) ** 0.5
+    assert abs(float(norm) - want) <= 1e-5 * want
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("case", APART)
+def test_interleaved_memory_is_clipped(device, case):
+    base = _base(device)
+    views = APART[case](base)
+    before = [v.clone() for v in views]
+    want = sum(float(v.double().square().sum()) for v in before) ** 0.5
+    norm = ops.clip_grad_norm_(views, 10.0)
+    assert abs(float(norm) - want) <= 1e-5 * want
+    factor = 10.0 / (want + 1e-6)
+    for v, b in zip(views, before):
+        half = 2.0 ** -24 if v.dtype == torch.float32 else 2.0 ** -8
+        assert ((v.double() - b.double() * factor).abs() <= b.double().abs() * factor * (40 * 2.0 ** -24 + half) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_targets_that_overlap_themselves_are_refused(device):
+    memory = torch.ones(40, device=device)
+    for out in (memory.as_strided((10, 4), (2, 1)), memory.as_strided((5, 3), (3, 3)), memory.as_strided((3, 5), (0, 1))):
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_([torch.ones(out.shape, device=device)], 1.0, out=[out])
+        with pytest.raises(ValueError):
+            ops.clip_grad_norm_([out], 1.0)
+    assert torch.equal(memory, torch.ones_like(memory))
+
+
+def test_the_search_agrees_with_the_sets_of_addresses():
+    draw = random.Random(0)
+    memory, met = torch.zeros(400), 0
+
+    def view():
+        dtype = draw.choice([torch.float32, torch.bfloat16])
+        shape = [draw.randint(1, 5) for _ in range(draw.randint(0, 3))]
+        return memory.view(dtype).as_strided(shape, [draw.choice([1, 2, 3, 4, 5, 6, 7, 10, 12, 20]) for _ in shape], draw.randint(0, 60))
+
+    def places(t):
+        out = [t.data_ptr()]
+        for n, st in zip(t.shape, t.stride()):
+            out = [p + k * st * t.element_size() for p in out for k in range(n)]
+        return out
+    for _ in range(4000):
+        a, b = view(), view()
+        at, bt = ({p + i for p in places(t) for i in range(t.element_size())} for t in (a, b))
+        assert clipping._meet(a, b) == clipping._meet(b, a) == bool(at & bt)
+        assert clipping._folded(a) or len(set(places(a))) == len(places(a))
+        met += bool(at & bt)
+    assert 500 < met < 3500
