@@ -16,7 +16,7 @@ import torch
 
 from ksa_b200 import ops
 from ksa_b200.ops import log_probs as impl
-from test_log_probs_gpu import _inputs
+from test_log_probs_gpu import IGNORE, _close, _inputs, _oracle, _run
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,49 @@ def test_parts_of_the_rows_gradient_are_those_that_were_written(T, D, V, answer,
     w.requires_grad_(head)
     torch.autograd.grad(ops.linear_log_probs(h, w, labels), (h, w) if head else h, dy)
     assert len(seen) == 1
+
+
+@pytest.mark.parametrize("T,D,V", [(1, 1032, 300), (33, 2048, 1003), (128, 2560, 300), (129, 1160, 1003), (300, 2048, 2600), (520, 2568, 700)])
+@pytest.mark.parametrize("answer,tau", [(1.0, 1.0), (0.5, 0.7)])
+def test_wide_rows(T, D, V, answer, tau):
+    """Widths above 1024, where a logit is added up from several parts: the last one whole and ragged, tiles in halves, few rows and many."""
+    h, w, labels, dy = _inputs(T, D, V, answer, seed=T, tau=tau)
+    want = _oracle(h, w, labels, dy, tau)
+    got = _run(h, w, labels, dy, tau)
+    for name, g in zip(("y", "dh", "dw"), got):
+        _close(g, want[name], name)
+    with torch.no_grad():
+        _close(ops.linear_log_probs(h, w, labels, temperature=tau), want["y"], "y alone")
+    assert all(torch.equal(a, b) for a, b in zip(_run(h, w, labels, dy, tau), got))
+
+
+@pytest.mark.parametrize("T", [8192, 8193, 8200, 16390, 20000])
+def test_more_rows_than_one_round_of_the_selection(T):
+    """Rows are chosen 8192 at a time; the places of a round begin where the one before it ended."""
+    h, w, labels, dy = _inputs(T, 16, 40, 0.6, seed=T)
+    labels[8190:8195] = torch.tensor([3, -100, 5, 39, -100], device="cuda")[:max(0, T - 8190)][:5]
+    want = _oracle(h, w, labels, dy, 1.0)
+    for name, g in zip(("y", "dh", "dw"), _run(h, w, labels, dy, 1.0)):
+        _close(g, want[name], name)
+    only = torch.full_like(labels, IGNORE)
+    only[-1] = 7                                                            # a single label, in the last round
+    want = _oracle(h, w, only, dy, 1.0)
+    for name, g in zip(("y", "dh", "dw"), _run(h, w, only, dy, 1.0)):
+        _close(g, want[name], name)
+
+
+@pytest.mark.parametrize("T,D,V", [(1, 64, 1000), (128, 136, 1003), (129, 136, 1003), (300, 264, 1000), (1030, 64, 5000)])
+@pytest.mark.parametrize("slab,planes", [(4 << 30, 512 << 20), (2 * 512 * 512, 512 << 20), (2 * 512 * 1024, 0), (1, 1 << 20)])
+def test_both_ways_to_the_kernels_decide_alike(T, D, V, slab, planes, monkeypatch):
+    """Calls by way of Python (which a head with a gradient buffer takes) and of native code give the same bits, wherever the
+    rules for kept logits, slabs and parts put them."""
+    monkeypatch.setattr(impl, "SLAB_BYTES", slab)
+    monkeypatch.setattr(impl, "PLANE_BYTES", planes)
+    h, w, labels, dy = _inputs(T, D, V, 0.7, seed=T)
+    native = _run(h, w, labels, dy, 0.7)
+    with torch.no_grad():
+        alone = ops.linear_log_probs(h, w, labels, temperature=0.7)
+    monkeypatch.setattr(impl, "_native", SimpleNamespace(linear_log_probs=lambda *args: None))
+    assert all(torch.equal(a, b) for a, b in zip(_run(h, w, labels, dy, 0.7), native))
+    with torch.no_grad():
+        assert torch.equal(ops.linear_log_probs(h, w, labels, temperature=0.7), alone)
