@@ -56,6 +56,12 @@ constexpr float kLpCodes = 1024.f;                                      // codes
 // of the loads' rate (1146 rows against 49042 tokens 150 us).
 __host__ __device__ constexpr long long lp_pitch(long long n) { return (n + 63) / 64 * 64; }
 constexpr int kLpRowPad = 256;                                          // rows of the gathered arrays: a multiple of this
+// dx enters its products in bf16, 2^-9 of itself off.  Over many rows that is 1.4 times the error that rounding the results leaves anyway; of few rows each
+// gradient is nearly one row's, whose largest elements' rounding all its values share, and was off by 2.5 times as much.  Up to so many rows
+// with a label (a pair's tile has twice as many) dx is two bf16 numbers, the second of them what the rounding of the first left, in the rows
+// from kLpLow on: dh is the sum of both rows' products, dw runs over both.  64 rows of 2048 against 151936 tokens 456 -> 476 us.
+constexpr int kLpLow = 128;
+static_assert(kLpLow == kLpBM && 2 * kLpLow <= kLpRowPad, "the second halves have rows of their own, those of the pair's other CTA");
 
 enum LpMode : int { kStats = 0, kStatsKeep = 1, kGrad = 2, kProducts = 3 };
 
@@ -236,9 +242,11 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
 
   const int count = *a.count;
   const int M = min(count, a.M), N = a.N;
-  const LpTiles dh(kMode == kProducts && a.dh ? M : 0, a.N, a.K);
-  const LpTiles main_tiles(kMode != kProducts ? M : a.dw ? a.K : 0, a.N, kMode != kProducts ? a.K : M);
-  const int parts = kMode == kProducts && dh.all > 0 ? lp_parts(dh.all, dh.num_kb, n_pairs, a.planes, a.dw ? lp_dw_steps(a.K, a.N, M) : 0.f) : 1;
+  const bool low = (kMode == kGrad || kMode == kProducts) && M <= kLpLow;
+  const int dh_rows = low && M > 0 ? kLpLow + M : M, dw_rows = low ? 2 * ((M + kLpBK - 1) / kLpBK * kLpBK) : M;
+  const LpTiles dh(kMode == kProducts && a.dh ? dh_rows : 0, a.N, a.K);
+  const LpTiles main_tiles(kMode != kProducts ? M : a.dw ? a.K : 0, a.N, kMode != kProducts ? a.K : dw_rows);
+  const int parts = kMode == kProducts && dh.all > 0 ? lp_parts(dh.all, dh.num_kb, n_pairs, a.planes, a.dw ? lp_dw_steps(a.K, a.N, dw_rows) : 0.f) : 1;
   if (kMode == kProducts && a.dh && blockIdx.x == 0 && threadIdx.x == 0) *a.parts = dh.all > 0 ? parts : 0;
   const LpSchedule work_of(dh, main_tiles, pair, n_pairs, parts);
   const int num_kb = main_tiles.num_kb;
@@ -263,17 +271,19 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
           uint8_t* sb = sa + kLpABytes;
           const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
           if (rank == 0) mbar_expect_tx(&full[stage], 2 * (kLpABytes + boxes * 8192));
+          const bool second = low && a_mn && 2 * kb >= num_kb;           // dw: the same rows of h again, with the second halves of dx
+          const int k = (second ? kb - num_kb / 2 : kb) * kLpBK;
           if (!a_mn) {
-            tma_load_2d_pair(sa, mA, kb * kLpBK, row0, bar);
+            tma_load_2d_pair(sa, mA, k, row0, bar);
           } else {
 #pragma unroll
-            for (int j = 0; j < kLpBM / 64; ++j) tma_load_2d_pair(sa + j * 8192, mA, row0 + j * 64, kb * kLpBK, bar);
+            for (int j = 0; j < kLpBM / 64; ++j) tma_load_2d_pair(sa + j * 8192, mA, row0 + j * 64, second ? kLpLow + k : k, bar);
           }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             if (j >= boxes) break;
-            if (!kBMn) tma_load_2d_pair(sb + j * 8192, mB, kb * kLpBK, col0 + j * 64, bar);
-            else tma_load_2d_pair(sb + j * 8192, mB, col0 + j * 64, kb * kLpBK, bar);
+            if (!kBMn) tma_load_2d_pair(sb + j * 8192, mB, k, col0 + j * 64, bar);
+            else tma_load_2d_pair(sb + j * 8192, mB, col0 + j * 64, k, bar);
           }
           if (++stage == kLpStages) { stage = 0; phase ^= 1; }
         }
@@ -351,14 +361,16 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
     for (int i = split ? 0 : group; ok && work_of.get(i, u); i += split ? 1 : 2) {
       const int nb = u.nb, side = u.side;
       const int row_w = u.mb * 2 * kLpBM + (int)rank * kLpBM + quad * 32;      // first of this warp's 32 rows
-      const int row = row_w + lane;
+      const int second = kMode == kGrad && low && rank == 1 ? kLpLow : 0;      // the other CTA has the same rows, for the second halves of dx
+      const int row = row_w - second + lane;
       const bool live = row < M;
       int label = -1;
-      float lse2 = 0.f, g = 0.f;
+      float lse2 = 0.f, g = 0.f, own = 0.f;
       if ((kSums || kMode == kGrad) && live) label = a.row_label[row];
       if (kMode == kGrad && live) {
         lse2 = a.lse2[row];
         g = a.dy[a.rows[row]] * a.inv_tau;
+        own = g * (1.f - fast_exp2(a.picked2[row]));                     // 1 - p of the label: from the forward pass, as in log_probs_decode_kernel
         label -= a.col0;
       }
       if (!mbar_wait(&acc_full[local & 1], (local >> 1) & 1, guard, kTimeoutAccFull)) { ok = false; break; }
@@ -453,15 +465,16 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
               float d[32];
 #pragma unroll
               for (int j = 0; j < 32; ++j) d[j] = -g * fast_exp2(fmaf(__uint_as_float(r[j]), a.scale2, -lse2));
-              if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {         // 1 - p of the label: from the forward pass, as in log_probs_decode_kernel
-                const float mine = at >= 0 && at < 32 ? g * (1.f - fast_exp2(a.picked2[row])) : 0.f;
+              if (__any_sync(0xffffffffu, at >= 0 && at < 32))
 #pragma unroll
-                for (int j = 0; j < 32; ++j) d[j] = j == at ? mine : d[j];
-              }
+                for (int j = 0; j < 32; ++j) d[j] = j == at ? own : d[j];
+              if (second)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) d[j] -= __bfloat162float(__float2bfloat16_rn(d[j]));
 #pragma unroll
               for (int j = 0; j < 16; ++j) out[half * 16 + j] = live ? pack_bf16x2(d[2 * j], d[2 * j + 1]) : 0u;
             }
-            if (row_w < dx_rows) store_box(&maps.C, [&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
+            if (row_w - second < dx_rows) store_box(&maps.C, [&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c, row_w, false);
           }
         } else if (work) {
           const bool bf = !u.dh && a.bf16_out;
@@ -486,7 +499,7 @@ log_probs_pair_kernel(const __grid_constant__ LpMaps maps, const __grid_constant
             if (!u.dh && num_kb == 0)                                    // no rows at all: nothing was multiplied
 #pragma unroll
               for (int j = 0; j < 32; ++j) out[j] = 0u;
-            if (row_w < (u.dh ? a.M : a.K))
+            if (row_w < (u.dh ? dh_rows : a.K))
               store_box(u.dh ? &maps_dh.C : &maps.C, [&](int j) { return make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]); }, c,
                         u.part * a.plane_rows + row_w, u.dh ? a.add_dh != 0 : a.add_dw != 0);
           }
@@ -745,11 +758,11 @@ log_probs_select_kernel(const long long* labels, int T, int V, long long ignore,
 }
 
 // The same and the gathering of the rows in one launch, for at most kLpFewRows rows: a block has a row, and counts the labels before it itself.
-// The blocks behind the last row fill up with zeros, to `fill` rows at least.
+// The blocks behind the last row fill up with zeros, to `fill` rows at least.  `twice`: up to kLpLow labelled rows are there twice, which kGrad wants.
 constexpr int kLpFewRows = 1024;
 __global__ void __launch_bounds__(256)
 log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignore, int* rows, int* row_label, int* place, int* count, float* y,
-                          const bf16* h, long long ldh, bf16* dense, int D, int vec, int fill) {
+                          const bf16* h, long long ldh, bf16* dense, int D, int vec, int fill, int twice) {
   __shared__ int sums[2][8];
   grid_dependency_enter();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -789,12 +802,13 @@ log_probs_few_rows_kernel(const long long* labels, int T, int V, long long ignor
         for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[c + j];
     }
     *reinterpret_cast<BF8*>(dense + at * lp_pitch(D) + c) = v;
+    if (twice && n <= kLpLow && one) *reinterpret_cast<BF8*>(dense + (at + kLpLow) * lp_pitch(D) + c) = v;
   }
 }
 
 // dense[i] = h[rows[i]], and zeros up to the next multiple of kLpBK: those rows are part of dw's last products.
 __global__ void __launch_bounds__(256)
-log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int* count, bf16* dense, int D, int vec) {
+log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int* count, bf16* dense, int D, int vec, int twice) {
   grid_dependency_enter();
   const int n = *count, end = (n + kLpBK - 1) / kLpBK * kLpBK, per_row = D / 8;
   const long long all = (long long)end * per_row;
@@ -809,6 +823,7 @@ log_probs_gather_kernel(const bf16* h, long long ldh, const int* rows, const int
         for (int j = 0; j < 8; ++j) reinterpret_cast<bf16*>(&v)[j] = from[j];
     }
     *reinterpret_cast<BF8*>(dense + row * lp_pitch(D) + c) = v;
+    if (twice && n <= kLpLow && row < n) *reinterpret_cast<BF8*>(dense + (row + kLpLow) * lp_pitch(D) + c) = v;
   }
 }
 
@@ -868,7 +883,7 @@ log_probs_sum_kernel(const float2* stats, long long ld, int slots, const float* 
   }
 }
 
-// dx of the rows with a label from the kept logits, and zeros up to the next multiple of kLpBK.  A block has 8 rows and 1024 columns, a
+// dx of the rows with a label from the kept logits (both halves of it of few rows), and zeros up to the next multiple of kLpBK.  A block has 8 rows and 1024 columns, a
 // warp one of the rows.
 constexpr int kLpDecodeCols = 1024;
 __global__ void __launch_bounds__(256)
@@ -909,6 +924,11 @@ log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* top
       if (!live) d[j] = 0.f;
     }
     store8(dx + row * pitch + c, d);
+    if (n <= kLpLow) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] -= __bfloat162float(__float2bfloat16_rn(d[j]));
+      store8(dx + (row + kLpLow) * pitch + c, d);
+    }
   }
 }
 
@@ -916,10 +936,11 @@ log_probs_decode_kernel(const uint16_t* codes, long long pitch, const float* top
 // share them where there are few values and may be many parts (one row in 64 parts 39 us by one thread each, 6 by 8; 4915 rows in 6 parts 54 and 124).
 template <int kSplit>
 __global__ void __launch_bounds__(256)
-log_probs_scatter_kernel(const float* dense, const int* place, const int* parts_made, bf16* dh, int T, int D, long long plane) {
+log_probs_scatter_kernel(const float* dense, const int* place, const int* count, const int* parts_made, bf16* dh, int T, int D, long long plane) {
   __shared__ float4 sums[kSplit][256 / kSplit];
   grid_dependency_enter();
   const int parts = *parts_made, per_row = D / 4;
+  const bool low = *count <= kLpLow;
   const int lane = threadIdx.x % (256 / kSplit), first = threadIdx.x / (256 / kSplit);
   const long long all = (long long)T * per_row;
   for (long long i0 = blockIdx.x * (256LL / kSplit); i0 < all; i0 += gridDim.x * (256LL / kSplit)) {
@@ -932,6 +953,10 @@ log_probs_scatter_kernel(const float* dense, const int* place, const int* parts_
       for (int p = first; p < parts; p += kSplit) {
         const float4 u = *reinterpret_cast<const float4*>(from + p * plane);
         f.x += u.x; f.y += u.y; f.z += u.z; f.w += u.w;
+        if (low) {
+          const float4 v = *reinterpret_cast<const float4*>(from + p * plane + (long long)kLpLow * D);
+          f.x += v.x; f.y += v.y; f.z += v.z; f.w += v.w;
+        }
       }
     }
     if (kSplit > 1) {
@@ -1027,14 +1052,14 @@ KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void
   if (T <= kLpFewRows) {
     const int fill = few ? columns : 0, blocks = T + kLpBK - 1 > fill ? T + kLpBK - 1 : fill;
     KSA_CHECK_CUDA(launch_kernel(log_probs_few_rows_kernel, dim3(blocks), dim3(256), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
-                                 (int*)row_label, (int*)place, (int*)count, (float*)y, (const bf16*)h, ldh, (bf16*)dense, D, vec, fill));
+                                 (int*)row_label, (int*)place, (int*)count, (float*)y, (const bf16*)h, ldh, (bf16*)dense, D, vec, fill, (int)(codes == nullptr)));
   } else {
     KSA_CHECK_CUDA(launch_kernel(log_probs_select_kernel, dim3(1), dim3(kLpSelect), 0, st, (const long long*)labels, T, V, ignore_index, (int*)rows,
                                  (int*)row_label, (int*)place, (int*)count, (float*)y));
     const long long vectors = (T + 63LL) / 64 * 64 * (D / 8);
     const int gather_blocks = (int)(vectors < 256 * 148 * 8 ? (vectors + 255) / 256 : 148 * 8);
     KSA_CHECK_CUDA(launch_stream_kernel(4LL * T * D, log_probs_gather_kernel, dim3(gather_blocks), dim3(256), 0, st, (const bf16*)h, ldh,
-                                        (const int*)rows, (const int*)count, (bf16*)dense, D, vec));
+                                        (const int*)rows, (const int*)count, (bf16*)dense, D, vec, (int)(codes == nullptr)));
   }
   LpMaps m;
   int rc, sums = slots;
@@ -1146,7 +1171,7 @@ KSA_API int ksa_log_probs_bwd(const void* dense, const void* w, const void* rows
     const long long blocks = ((long long)T * (D / 4) * split + 255) / 256;
     KSA_CHECK_CUDA(launch_stream_kernel(6LL * T * D, split > 1 ? log_probs_scatter_kernel<8> : log_probs_scatter_kernel<1>,
                                         dim3((unsigned)(blocks < 148 * 16 ? blocks : 148 * 16)), dim3(256), 0, st, (const float*)dh32, (const int*)place,
-                                        (const int*)planes_end, (bf16*)dh, T, D, (long long)padded * D));
+                                        (const int*)count, (const int*)planes_end, (bf16*)dh, T, D, (long long)padded * D));
   }
   return 0;
 }

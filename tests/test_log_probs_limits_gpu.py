@@ -97,6 +97,42 @@ def test_gradient_of_a_label_next_to_probability_one(T, V, D, logits):
     _check(h, w, labels, dy, own, 1.0, logits == "kept")
 
 
+@pytest.mark.parametrize("T,D,V,answer", [(1, 64, 1000, 1), (1, 2048, 3003, 1), (2, 136, 5000, 2), (9, 1032, 700, 9), (64, 128, 4096, 64),
+                                              (65, 256, 300, 65), (128, 64, 2000, 128), (300, 136, 1000, 64), (1500, 64, 500, 128), (9000, 16, 300, 3)])
+@pytest.mark.parametrize("which", ["both", "rows", "head", "slabs"])
+def test_gradients_of_few_rows_are_rounded_once(T, D, V, answer, which, logits, monkeypatch):
+    """Up to 128 rows with a label, wherever they are: the logits' gradient takes part with 16 bits, so that what the results are off by is
+    their own rounding to bf16, 2^-8, and what the probabilities are (see test_log_probs_gpu)."""
+    h, w, labels, dy = _inputs(T, D, V, 1.0, seed=T + D)
+    labels[torch.randperm(T, device="cuda")[:T - answer]] = IGNORE
+    if which == "slabs":
+        monkeypatch.setattr(impl, "SLAB_BYTES", 1)
+    x = h.double() @ w.double().T
+    lse = x.logsumexp(1, keepdim=True)
+    p = (x - lse).exp()
+    live = labels != IGNORE
+    one = torch.zeros_like(p)
+    one[live, labels[live]] = 1
+    g = torch.where(live, dy, torch.zeros_like(dy)).double()[:, None]
+    dx = (one - p) * g
+    ex = (D / 16 + 2) * 2.0 ** -22 * (h.double().abs() @ w.double().abs().T).amax(1, keepdim=True)
+    kept = 2.0 ** -11.5 if logits == "kept" and which != "slabs" else 0.0
+    off = p * (2 * ex + 2.0 ** -18 + kept) * g.abs() + 2.0 ** -16 * dx.abs() + 2.0 ** -120
+    need = {"both": (True, True), "slabs": (True, True), "rows": (True, False), "head": (False, True)}[which]
+    h.requires_grad_(need[0])
+    w.requires_grad_(need[1])
+    y = ops.linear_log_probs(h, w, labels)
+    grads = iter(torch.autograd.grad(y, [t for t, n in zip((h, w), need) if n], dy))
+    hd, wd = h.detach().double(), w.detach().double()
+    for wanted, value, spread, sums in ((need[0], dx @ wd, off @ wd.abs(), (V / 16 + 80) * 2.0 ** -22 * (dx.abs() @ wd.abs())),
+                                        (need[1], dx.T @ hd, off.T @ hd.abs(), (2 * T / 16 + 8) * 2.0 ** -22 * (dx.abs().T @ hd.abs()))):
+        if wanted:
+            got = next(grads).double()
+            tol = 2.0 ** -8 * value.abs() + (spread + sums) * 1.01 + 1e-30
+            bad = (got - value).abs() > tol
+            assert not bad.any(), (int(bad.sum()), float(((got - value).abs() / tol).max()))
+
+
 @pytest.mark.parametrize("T,D,V", [(1, 152, 99667), (70, 64, 4096), (300, 136, 1000), (333, 256, 4096), (600, 512, 20000), (1300, 1024, 30000), (4100, 128, 2000)])
 @pytest.mark.parametrize("answer", [1.0, 0.4, 0.0])
 @pytest.mark.parametrize("head", [True, False])
@@ -120,10 +156,13 @@ def test_parts_of_the_rows_gradient_are_those_that_were_written(T, D, V, answer,
         assert planes_of[made:].isnan().all() and planes_of[:made, :count].isfinite().all()
         total = torch.zeros(T, D, device="cuda", dtype=torch.float64)
         at = args[2][:count].long()
-        total[at] = planes_of[:made, :count].double().sum(0)
-        # added up in 32 bits, in order or by eight at a time: 64 roundings of partial sums at most
+        used = planes_of[:made, :count]
+        if count <= 128:                                                    # few rows: the products of both halves of the logits' gradient
+            used = torch.cat([used, planes_of[:made, 128:128 + count]])
+        total[at] = used.double().sum(0)
+        # added up in 32 bits, in order or by eight at a time: 128 roundings of partial sums at most
         bound = torch.zeros_like(total)
-        bound[at] = planes_of[:made, :count].double().abs().sum(0)
+        bound[at] = used.double().abs().sum(0)
         assert ((dh.double() - total).abs() <= 2.0 ** -8 * total.abs() + 2.0 ** -17 * bound + 2.0 ** -130).all()
     monkeypatch.setattr(impl._lib, "call", watched)
     monkeypatch.setattr(impl, "_native", SimpleNamespace(linear_log_probs=lambda *args: None))
