@@ -2,12 +2,12 @@
 //   x_tv = h_t . w_v / tau,   y_t = x_t,label - log sum_v exp(x_tv);
 //   dx_tv = dy_t ([v = label] - exp(x_tv - lse_t)) / tau,   dh = dx w,   dw = dx^T h.
 //
-// Bound: the products, 2 n V D operations forward and twice that backward; at 16 rows and fewer the weights' bytes.
+// Bound: the products, 2 n V D operations forward and twice that backward; below some 210 rows (1376 TFLOP/s to 6550 GB/s) the weights' bytes.
 //
-// The backward pass needs the logits again.  Where 16 bits of each fit the caller's limit the forward pass keeps them, as the distance below the
-// maximum of their 128 columns in steps of 2^-10 of a power of two: probabilities from them are off by 2^-12 of themselves, next to
-// nothing beside the rounding of dx to bf16 (kept as bf16 a logit of 10 would be off by 2^-6), and what is more than 64 powers below the maximum counts as
-// that far.  Above the limit the product is computed again, a quarter more of all products.
+// The backward pass needs the logits again.  Where the caller wants them kept (16 bits of each fit its limit, and the heads are wide enough that the
+// product costs more than keeping it) the forward pass keeps them, as the distance below the maximum of their 128 columns in steps of 2^-10 of a power
+// of two: probabilities from them are off by 2^-11.5 of themselves at most, less than the rounding of dx to bf16 (kept as bf16 a logit of 10 would be off by
+// 2^-6), and what is more than 64 powers below the maximum counts as that far.  Else the product is computed again: four products in place of three.
 //
 // Rows without a label are left out first: the others are gathered into a dense array, and the kernels take their number from device
 // memory, so that prompts and masked turns cost nothing but their labels, and what their rows hold reaches no sum.
@@ -16,7 +16,7 @@
 //   kStats  h w^T: every thread has one row of the tile; it takes the maximum and the sum of exponentials of 128 columns.  A second kernel adds
 //           those of a row.  Maxima and the label's logit stay as they are, not times log2(e): y is then a difference of two numbers that
 //           were not rounded, where products of 20 would leave 1e-6.
-//   kStatsKeep  the same, and the logits in 16 bits;  kGrad  the product again, dx in bf16 from the accumulators.
+//   kStatsKeep  the same, and the logits in 16 bits;  kGrad  the product again, dx in bf16 (kLpLow) from the accumulators.
 //   kProducts  dx w in fp32 over the columns of one slab, and dx^T h: up to some size one launch of both, so that the many short tiles of the second fill the
 //           waves of the few long ones of the first.
 // dx exists for a slab of the vocabulary at a time (the caller says how wide): the slabs' dw are disjoint, and dh is added up in fp32.

@@ -112,7 +112,8 @@ def linear_log_probs(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.T
     ``hidden`` is ``[..., D]``, ``weight`` the output head ``[V, D]`` (both bf16 on a GPU, ``D`` a multiple of 8), ``labels`` ``[...]``.  Rows
     without a label cost next to nothing and take part in nothing, whatever they hold; their gradient is 0.  Without a
     gradient the logits are never in memory.  With one the forward pass keeps them in 16 bits where the width is at least 768 and that takes at most
-    ``SLAB_BYTES`` (4 GB: 13824 rows of 151936 tokens); else the backward pass computes them again, at most 4 GB of their gradient at a time.
+    ``SLAB_BYTES`` (4 GB: 14080 rows of 151936 tokens); else the backward pass computes them again, at most 4 GB of their gradient at a time.
+    The logits' gradient enters its products in bf16, of up to 128 labelled rows in two parts of bf16 each.
     With ``main_grad`` on the weight its gradient goes there."""
     if not _observed():
         y = _native.linear_log_probs(hidden, weight, labels, ignore_index, temperature, _ROW_PAD, _STAT_COLS, SLAB_BYTES, PLANE_BYTES, KEEP_WIDTH)
