@@ -860,8 +860,14 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const float scale = a.real(), most = a.real();
   if (!a.ok() || !(PyList_CheckExact(grads) || PyTuple_CheckExact(grads)) || (out != Py_None && !(PyList_CheckExact(out) || PyTuple_CheckExact(out))))
     return none();
-  const Py_ssize_t count = PySequence_Fast_GET_SIZE(grads);
-  if (count == 0 || count > INT_MAX || (out != Py_None && PySequence_Fast_GET_SIZE(out) != count) || !(scale > 0.f && std::isfinite(scale)) || !(most >= 0.f))
+  // (another thread may empty the lists while this one works without the interpreter's lock)
+  const auto held_grads = pybind11::reinterpret_steal<pybind11::object>(PySequence_Tuple(grads));
+  const auto held_out = out == Py_None ? pybind11::object() : pybind11::reinterpret_steal<pybind11::object>(PySequence_Tuple(out));
+  if (!held_grads || (out != Py_None && !held_out)) throw python_error();
+  grads = held_grads.ptr();
+  if (out != Py_None) out = held_out.ptr();
+  const Py_ssize_t count = PyTuple_GET_SIZE(grads);
+  if (count == 0 || count > INT_MAX || (out != Py_None && PyTuple_GET_SIZE(out) != count) || !(scale > 0.f && std::isfinite(scale)) || !(most >= 0.f))
     return none();
   std::vector<const void*> src(count);
   std::vector<void*> dst(clip ? count : 0);
@@ -875,13 +881,13 @@ PyObject* py_grad_norm(PyObject*, PyObject* const* v, Py_ssize_t n) {
   };
   const Tensor* first = nullptr;
   for (Py_ssize_t i = 0; i < count; ++i) {
-    const Tensor* t = plain(PySequence_Fast_GET_ITEM(grads, i));
+    const Tensor* t = plain(PyTuple_GET_ITEM(grads, i));
     if (!t || (first && t->device() != first->device())) return none();
     if (!first) first = t;
     src[i] = t->const_data_ptr();
     meta[i] = 4 * (long long)t->numel() + token_type(*t);
     if (!clip) continue;
-    const Tensor* o = out == Py_None ? t : plain(PySequence_Fast_GET_ITEM(out, i));
+    const Tensor* o = out == Py_None ? t : plain(PyTuple_GET_ITEM(out, i));
     if (!o || o->is_inference() || (o != t && (o->device() != t->device() || o->scalar_type() != t->scalar_type() || o->sizes() != t->sizes() ||
                                                o->strides() != t->strides())))
       return none();

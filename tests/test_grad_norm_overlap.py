@@ -1,5 +1,6 @@
 """Clipping of gradients that share memory, in layouts that do not fill theirs: refused where they meet, clipped where they only interleave."""
 import random
+import threading
 
 import pytest
 import torch
@@ -99,3 +100,23 @@ def test_the_search_agrees_with_the_sets_of_addresses():
         assert clipping._folded(a) or len(set(places(a))) == len(places(a))
         met += bool(at & bt)
     assert 500 < met < 3500
+
+
+@pytest.mark.gpu
+def test_a_list_that_another_thread_empties():
+    """The call keeps the tensors that it was given until it has launched."""
+    given, done = [], threading.Event()
+
+    def empty():
+        while not done.is_set():
+            given.clear()
+    thread = threading.Thread(target=empty)
+    thread.start()
+    try:
+        for _ in range(20):
+            given[:] = [torch.full((1000,), 0.01, device="cuda") for _ in range(10)]
+            norm = float(ops.clip_grad_norm_(given, 1e9))
+            assert norm == 0 or abs(norm - 0.01 * 10000 ** 0.5) <= 1e-6          # (0: emptied before the call had looked at it)
+    finally:
+        done.set()
+        thread.join()
