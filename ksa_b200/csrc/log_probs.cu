@@ -1030,7 +1030,7 @@ KSA_API long long ksa_log_probs_work(int T, int V) {
 // Forward.  h [T, D] (row pitch ldh, any alignment of its type), w [V, D] (row pitch ldw, a multiple of 8, 16-byte aligned), labels [T] int64.
 // Leaves what the backward pass needs: dense [T rounded up to 256, D rounded up to 64] bf16, rows, row_label, place [T], count [1] int32, lse2 [2 T] (the log-sums
 // and the labels' logits less those, base 2), and where codes is not null the logits in 16 bits, codes [T rounded up to 256, V rounded up to 64]
-// with tops, fp32 [ceil(V / 128) times T rounded up to 4].
+// with tops, fp32 [ceil(V / 128) times T rounded up to 4].  (Without codes up to 128 labelled rows are in dense twice: a backward pass without them needs that.)
 // work: fp32 [ksa_log_probs_work(T, V)].  y [T] fp32.
 KSA_API int ksa_log_probs(const void* h, const void* w, const void* labels, void* dense, void* rows, void* row_label, void* place, void* count,
                           void* lse2, void* work, void* y, void* codes, void* tops, int T, int V, int D, long long ldh, long long ldw, long long ignore_index, float tau,
